@@ -369,7 +369,7 @@ def run(st):
         return vs.rotary(st["x"], st["pos"], st["freq"], layout=c["layout"], lengthen=st["lengthen"])
     if st["op"] == "append":
         after = vs.paged_append(st["k"], st["v"], st["k_pages"], st["v_pages"], st["table"], st["before"], st["starts"],
-                                max_new=st["max_new"], positions=st["pos"], frequencies=st["freq"], layout=c["layout"],
+                                positions=st["pos"], frequencies=st["freq"], layout=c["layout"],
                                 lengthen=st["lengthen"], ids=st["ids"], new_ids=st["pos"], weights=st["weights"],
                                 new_weights=st["init"])
         return st["k_pages"], st["v_pages"], st["ids"], st["weights"], after
