@@ -914,6 +914,25 @@ bool encode_tmap_3d_sw128(CUtensorMap* map, const void* ptr, int dtype, int64_t 
             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+bool encode_tmap_sw128(CUtensorMap* map, const void* ptr, int dtype, int rank,
+                       const uint64_t* dims, const uint64_t* strides, const uint32_t* box) {
+  tcattn::EncodeTiledFn fn = tcattn::encode_fn();
+  if (!fn || rank < 1 || rank > 5) return false;
+  cuuint64_t d[5], s[5];
+  cuuint32_t b[5], estr[5];
+  for (int i = 0; i < rank; ++i) {
+    d[i] = dims[i];
+    s[i] = i + 1 < rank ? strides[i] : 0;
+    b[i] = box[i];
+    estr[i] = 1;
+  }
+  const CUtensorMapDataType dt =
+      dtype == VGGT_DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  return fn(map, dt, (cuuint32_t)rank, const_cast<void*>(ptr), d, s, b, estr,
+            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 bool attn_tc05_supported(const AttnArgs& a) {
   return a.dim == 64 && a.block_q == 64 && a.block_k == 64 && a.n_patch >= 1 &&
          a.scale > 0.f && a.nb <= 65536 && a.max_blocks <= 65536 && a.n_tokens <= 0x7fffffffLL &&

@@ -80,6 +80,34 @@ int64_t pair_min_blocks() {
 
 }  // namespace
 
+namespace vggt {
+
+int api_fail(const char* fmt, ...) {
+  if (fmt == nullptr) {
+    g_err[0] = '\0';
+    return 0;
+  }
+  va_list ap;
+  va_start(ap, fmt);
+  vsnprintf(g_err, sizeof(g_err), fmt, ap);
+  va_end(ap);
+  return -1;
+}
+
+int api_cuda(cudaError_t e) {
+  if (e == cudaSuccess) return api_fail(nullptr);
+  return cuda_rc(e);
+}
+
+int api_device_sms() { return current_device_sms(); }
+
+uint64_t api_wait_ns() {
+  const uint64_t ns = g_wait_ns.load();
+  return ns > 0 ? ns : 1000000000ull;
+}
+
+}  // namespace vggt
+
 extern "C" {
 
 int vggt_sparse_version(void) { return (1 << 16) | 0; }

@@ -6,6 +6,14 @@
 
 namespace vggt {
 
+// capi.cu: an argument error (sets the message, returns -1); with a null
+// format no error (clears it, returns 0).  A CUDA error as a return code.
+int api_fail(const char* fmt, ...);
+int api_cuda(cudaError_t e);
+int api_device_sms();
+// limit of every bounded wait, vggt_sparse_set_wait_limit_ns
+uint64_t api_wait_ns();
+
 inline bool units_zero(int64_t a, int64_t b) { return a == 0 || b == 0; }
 
 // estimator.cu

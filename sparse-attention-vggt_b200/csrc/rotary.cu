@@ -1,0 +1,430 @@
+// Rotary positions, and the append of rotated keys and of values to a paged
+// cache.
+//
+// A pair (x, y) of a head turns by the angle a = position * freq:
+//   (x cos a - y sin a, x sin a + y cos a) * lengthen.
+// No table of cosines is read.  The angle is kept as a fraction of a turn in
+// 64-bit fixed point: step = round(freq / 2 pi * 2^64) modulo 2^64, and
+// position * step wraps to exactly the fraction that the product has, so the
+// reduction is exact for every 32-bit position (a 32-bit float product
+// position * freq is off by 4e-3 radians at position 65,536).  Its upper 32
+// bits go to sincospif: the angle is then within 2^-24 of a radian or two.
+//
+// Both kernels are bound by memory: every element is read and written once.
+// A thread owns up to 8 pairs (two 16-byte vectors of a 2-byte type) of a
+// token, takes their sines once and walks over heads with them, four heads'
+// loads in flight at a time.  With few tokens the heads are dealt to more
+// threads, until the grid fills the card.
+#include "kernels.h"
+#include "paged.cuh"
+
+namespace vggt {
+namespace {
+
+constexpr int kThreads = 256;
+
+// `N` bytes, moved by one instruction where N is 2, 4, 8 or 16.
+template <int N>
+struct Bytes;
+template <>
+struct Bytes<2> { using T = uint16_t; };
+template <>
+struct Bytes<4> { using T = uint32_t; };
+template <>
+struct Bytes<8> { using T = uint2; };
+template <>
+struct Bytes<16> { using T = uint4; };
+
+template <typename T>
+__device__ __forceinline__ float to_f(T v);
+template <>
+__device__ __forceinline__ float to_f<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ float to_f<__half>(__half v) { return __half2float(v); }
+template <>
+__device__ __forceinline__ float to_f<__nv_bfloat16>(__nv_bfloat16 v) {
+  return __bfloat162float(v);
+}
+template <typename T>
+__device__ __forceinline__ T from_f(float v);
+template <>
+__device__ __forceinline__ float from_f<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ __half from_f<__half>(float v) { return __float2half_rn(v); }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float v) {
+  return __float2bfloat16_rn(v);
+}
+
+// N elements in vectors of at most 16 bytes.
+template <typename T, int N>
+struct Vec {
+  static constexpr int kBytes = N * (int)sizeof(T) > 16 ? 16 : N * (int)sizeof(T);
+  static constexpr int kCount = N * (int)sizeof(T) / kBytes;
+  using V = typename Bytes<kBytes>::T;
+  V v[kCount];
+  __device__ __forceinline__ void load(const T* p) {
+#pragma unroll
+    for (int i = 0; i < kCount; ++i) v[i] = reinterpret_cast<const V*>(p)[i];
+  }
+  __device__ __forceinline__ void store(T* p) const {
+#pragma unroll
+    for (int i = 0; i < kCount; ++i) reinterpret_cast<V*>(p)[i] = v[i];
+  }
+  __device__ __forceinline__ T* e() { return reinterpret_cast<T*>(v); }
+};
+
+struct Angles {
+  const int32_t* positions;  // [tokens][axes]
+  const double* freq;        // [pairs]
+  int axes, pairs, interleaved;
+  float lengthen, sign;
+};
+
+// One unit of a head: 2 * N elements, as two runs of N at offsets a and b.
+// Units below axes * pairs / N rotate N pairs; the rest copy.
+template <int N>
+struct Unit {
+  int a, b;
+  bool turns;
+  float c[N], s[N];
+
+  __device__ __forceinline__ Unit(const Angles& g, int64_t token, int unit) {
+    const int first = unit * N;  // pair number over all axes
+    turns = first < g.axes * g.pairs;
+    if (!turns) {
+      a = 2 * first;
+      b = a + N;
+      return;
+    }
+    const int axis = first / g.pairs, i0 = first % g.pairs;
+    if (g.interleaved) {
+      a = 2 * first;
+      b = a + N;
+    } else {
+      a = 2 * axis * g.pairs + i0;
+      b = a + g.pairs;
+    }
+    const uint64_t pos = (uint64_t)(int64_t)__ldg(g.positions + token * g.axes + axis);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      double t = __ldg(g.freq + i0 + i) * 0.15915494309189535;  // turns per position
+      t -= rint(t);
+      const uint64_t step = (uint64_t)__double2ll_rn(t * 9223372036854775808.0) << 1;
+      const int32_t turn = (int32_t)((pos * step) >> 32);
+      sincospif((float)turn * 4.656612873077393e-10f, &s[i], &c[i]);  // 2^-31: half turns
+      c[i] *= g.lengthen;
+      s[i] *= g.lengthen * g.sign;
+    }
+  }
+
+  template <typename T>
+  __device__ __forceinline__ void turn(T* x, T* y, bool interleaved) const {
+    if (!turns) return;
+    if (interleaved) {  // pairs lie side by side over both runs
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        T* p = 2 * i < N ? x + 2 * i : y + (2 * i - N);
+        T* q = 2 * i + 1 < N ? x + 2 * i + 1 : y + (2 * i + 1 - N);
+        const float u = to_f(*p), w = to_f(*q);
+        *p = from_f<T>(u * c[i] - w * s[i]);
+        *q = from_f<T>(u * s[i] + w * c[i]);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const float u = to_f(x[i]), w = to_f(y[i]);
+        x[i] = from_f<T>(u * c[i] - w * s[i]);
+        y[i] = from_f<T>(u * s[i] + w * c[i]);
+      }
+    }
+  }
+};
+
+struct RotaryArgs {
+  const void* x;
+  void* out;
+  int64_t tokens, xt, xh, ot, oh;
+  int heads, units, deal;  // units per head; threads that share a token's heads
+  Angles g;
+};
+
+template <typename T, int N>
+__global__ void __launch_bounds__(kThreads) rotary_kernel(RotaryArgs p) {
+  const int64_t at = (int64_t)blockIdx.x * kThreads + threadIdx.x;
+  const int unit = (int)(at % p.units);
+  const int64_t rest = at / p.units;
+  const int part = (int)(rest % p.deal);
+  const int64_t token = rest / p.deal;
+  if (token >= p.tokens) return;
+  const Unit<N> u(p.g, token, unit);
+  const T* x = static_cast<const T*>(p.x) + token * p.xt;
+  T* o = static_cast<T*>(p.out) + token * p.ot;
+  constexpr int kBatch = 4;
+  for (int h0 = part; h0 < p.heads; h0 += kBatch * p.deal) {
+    Vec<T, N> a[kBatch], b[kBatch];
+#pragma unroll
+    for (int j = 0; j < kBatch; ++j) {
+      const int64_t h = h0 + j * p.deal;
+      if (h < p.heads) {
+        a[j].load(x + h * p.xh + u.a);
+        b[j].load(x + h * p.xh + u.b);
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < kBatch; ++j) {
+      const int64_t h = h0 + j * p.deal;
+      if (h < p.heads) {
+        u.turn(a[j].e(), b[j].e(), p.g.interleaved);
+        a[j].store(o + h * p.oh + u.a);
+        b[j].store(o + h * p.oh + u.b);
+      }
+    }
+  }
+}
+
+struct AppendArgs {
+  const void *k, *v;
+  void *kp, *vp;
+  int64_t kt, kh, vt, vh;
+  Pool pool;
+  PageTable t;  // lengths: before the call
+  int units, deal;
+  int64_t main_blocks;
+  Angles g;
+  int32_t *ids, *after;
+  const int32_t* new_ids;
+  float* weights;
+  const float* new_weights;
+};
+
+// Slot of packed row `row`, or -1 (no sequence, or past the last slot).
+__device__ __forceinline__ int64_t append_slot(const AppendArgs& p, int64_t row, int64_t& seq) {
+  seq = sequence_of_row(p.t.starts, p.t.seqs, row);
+  if (seq < 0) {
+    raise_status(p.t.status, VGGT_STATUS_BAD_LENGTH);
+    return -1;
+  }
+  const int64_t slot = checked_length(p.t, p.pool, seq) + row - __ldg(p.t.starts + seq);
+  if (slot < (p.t.width << p.pool.page_shift)) return slot;
+  raise_status(p.t.status, VGGT_STATUS_BAD_LENGTH);
+  return -1;
+}
+
+template <typename T, int N>
+__global__ void __launch_bounds__(kThreads) append_kernel(AppendArgs p) {
+  if (blockIdx.x >= p.main_blocks) {
+    // ids, weights (tokens along the lanes, so that a warp writes neighbours)
+    // and the new lengths
+    const int64_t at = ((int64_t)blockIdx.x - p.main_blocks) * kThreads + threadIdx.x;
+    if (at < p.t.seqs) {
+      int64_t first;
+      const int64_t n = checked_length(p.t, p.pool, at) + checked_rows(p.t, at, first);
+      const int64_t slots = p.t.width << p.pool.page_shift;
+      p.after[at] = (int32_t)(n < slots ? n : slots);
+    }
+    if (at >= p.t.total || (p.ids == nullptr && p.weights == nullptr)) return;
+    int64_t seq;
+    const int64_t slot = append_slot(p, at, seq);
+    if (slot < 0) return;
+    const int64_t slots = p.t.width << p.pool.page_shift;
+    const int64_t dst = seq * p.pool.kv_heads * slots + slot;
+    const int32_t id = p.ids != nullptr ? __ldg(p.new_ids + at) : 0;
+    const float w = p.new_weights != nullptr ? __ldg(p.new_weights + at) : 0.f;
+    for (int h = 0; h < p.pool.kv_heads; ++h) {
+      if (p.ids != nullptr) p.ids[dst + h * slots] = id;
+      if (p.weights != nullptr) p.weights[dst + h * slots] = w;
+    }
+    return;
+  }
+  const int64_t at = (int64_t)blockIdx.x * kThreads + threadIdx.x;
+  const int unit = (int)(at % p.units);
+  const int64_t rest = at / p.units;
+  const int part = (int)(rest % p.deal);
+  const int64_t row = rest / p.deal;
+  if (row >= p.t.total) return;
+  int64_t seq;
+  const int64_t slot = append_slot(p, row, seq);
+  if (slot < 0) return;
+  const int page = checked_page(p.t, p.pool, seq, slot >> p.pool.page_shift);
+  if (page < 0) return;
+  const Unit<N> u(p.g, row, unit);
+  const int64_t dst = page * p.pool.page_stride + (slot & (p.pool.page - 1)) * p.pool.row_stride;
+  const T* k = static_cast<const T*>(p.k) + row * p.kt;
+  const T* v = static_cast<const T*>(p.v) + row * p.vt;
+  T* kp = static_cast<T*>(p.kp) + dst;
+  T* vp = static_cast<T*>(p.vp) + dst;
+  constexpr int kBatch = 2;
+  for (int h0 = part; h0 < p.pool.kv_heads; h0 += kBatch * p.deal) {
+    Vec<T, N> a[kBatch], b[kBatch], c[kBatch], d[kBatch];
+#pragma unroll
+    for (int j = 0; j < kBatch; ++j) {
+      const int64_t h = h0 + j * p.deal;
+      if (h < p.pool.kv_heads) {
+        a[j].load(k + h * p.kh + u.a);
+        b[j].load(k + h * p.kh + u.b);
+        c[j].load(v + h * p.vh + u.a);
+        d[j].load(v + h * p.vh + u.b);
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < kBatch; ++j) {
+      const int64_t h = h0 + j * p.deal;
+      if (h < p.pool.kv_heads) {
+        u.turn(a[j].e(), b[j].e(), p.g.interleaved);
+        a[j].store(kp + h * p.pool.head_stride + u.a);
+        b[j].store(kp + h * p.pool.head_stride + u.b);
+        c[j].store(vp + h * p.pool.head_stride + u.a);
+        d[j].store(vp + h * p.pool.head_stride + u.b);
+      }
+    }
+  }
+}
+
+// Pairs per thread: the widest vector that divides the pairs of an axis and
+// the rest of the head, and that every address is aligned to.
+int pairs_per_thread(int size, int dim, int axes, int pairs, std::initializer_list<int64_t> strides,
+                     std::initializer_list<const void*> bases) {
+  for (int n = 8; n > 1; n >>= 1) {
+    const int64_t bytes = (int64_t)n * size > 16 ? 16 : (int64_t)n * size;
+    bool ok = (axes == 0 || pairs % n == 0) && (dim - 2 * axes * pairs) % (2 * n) == 0;
+    for (int64_t s : strides) ok = ok && (s * size) % bytes == 0;
+    for (const void* b : bases) ok = ok && reinterpret_cast<uintptr_t>(b) % bytes == 0;
+    if (ok) return n;
+  }
+  return 1;
+}
+
+// Threads that share a token's heads: one, or as many as it takes to give
+// every SM a thousand threads.
+int deal_heads(int64_t threads, int heads) {
+  const int64_t want = 148 * 1024;
+  int64_t d = threads > 0 ? (want + threads - 1) / threads : 1;
+  return (int)(d < 1 ? 1 : (d > heads ? heads : d));
+}
+
+template <typename T>
+cudaError_t rotary_n(int n, const RotaryArgs& a, unsigned grid, cudaStream_t st) {
+  switch (n) {
+    case 8: rotary_kernel<T, 8><<<grid, kThreads, 0, st>>>(a); break;
+    case 4: rotary_kernel<T, 4><<<grid, kThreads, 0, st>>>(a); break;
+    case 2: rotary_kernel<T, 2><<<grid, kThreads, 0, st>>>(a); break;
+    default: rotary_kernel<T, 1><<<grid, kThreads, 0, st>>>(a); break;
+  }
+  return cudaGetLastError();
+}
+
+template <typename T>
+cudaError_t append_n(int n, const AppendArgs& a, unsigned grid, cudaStream_t st) {
+  switch (n) {
+    case 8: append_kernel<T, 8><<<grid, kThreads, 0, st>>>(a); break;
+    case 4: append_kernel<T, 4><<<grid, kThreads, 0, st>>>(a); break;
+    case 2: append_kernel<T, 2><<<grid, kThreads, 0, st>>>(a); break;
+    default: append_kernel<T, 1><<<grid, kThreads, 0, st>>>(a); break;
+  }
+  return cudaGetLastError();
+}
+
+}  // namespace
+}  // namespace vggt
+
+using namespace vggt;
+
+namespace {
+
+int check_rotation(int dim, const int32_t* positions, int axes, const double* freq, int pairs,
+                   int layout, float lengthen) {
+  if (layout != VGGT_ROTARY_HALF && layout != VGGT_ROTARY_INTERLEAVED)
+    return api_fail("unknown rotary layout %d", layout);
+  if (axes < 1 || axes > 4) return api_fail("axes %d outside [1, 4]", axes);
+  if (pairs < 1 || (int64_t)2 * axes * pairs > dim)
+    return api_fail("2 * axes * pairs = %lld elements rotate in heads of %d",
+                    (long long)2 * axes * pairs, dim);
+  if (!(lengthen - lengthen == 0.f)) return api_fail("lengthen must be finite");
+  if (!positions || !freq) return api_fail("positions and freq must be non-NULL");
+  return 0;
+}
+
+}  // namespace
+
+extern "C" int vggt_rotary(const void* x, int dtype, int64_t tokens, int heads, int dim,
+                           int64_t x_token_stride, int64_t x_head_stride,
+                           const int32_t* positions, int axes, const double* freq, int pairs,
+                           int layout, float lengthen, int inverse, void* out,
+                           int64_t out_token_stride, int64_t out_head_stride, void* stream) {
+  if (dtype != VGGT_DTYPE_BF16 && dtype != VGGT_DTYPE_FP16 && dtype != VGGT_DTYPE_FP32)
+    return api_fail("rotary requires BF16, FP16 or FP32 (dtype code %d)", dtype);
+  if (tokens < 0 || heads < 0) return api_fail("negative size argument");
+  if (dim < 2 || dim % 2 || dim > 65536) return api_fail("head dim %d must be even and positive", dim);
+  if (tokens == 0 || heads == 0) return api_fail(nullptr);
+  if (int rc = check_rotation(dim, positions, axes, freq, pairs, layout, lengthen)) return rc;
+  if (!x || !out) return api_fail("x and out must be non-NULL");
+  const int size = dtype == VGGT_DTYPE_FP32 ? 4 : 2;
+  const int n = pairs_per_thread(size, dim, axes, pairs,
+                                 {x_token_stride, x_head_stride, out_token_stride, out_head_stride},
+                                 {x, out});
+  RotaryArgs a{x, out, tokens, x_token_stride, x_head_stride, out_token_stride, out_head_stride,
+               heads, dim / (2 * n), 1,
+               {positions, freq, axes, pairs, layout == VGGT_ROTARY_INTERLEAVED, lengthen,
+                inverse ? -1.f : 1.f}};
+  a.deal = deal_heads(tokens * a.units, heads);
+  const int64_t grid = (tokens * a.units * a.deal + kThreads - 1) / kThreads;
+  if (grid > 0x7fffffffLL) return api_fail("too many tokens (%lld)", (long long)tokens);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  return api_cuda(dtype == VGGT_DTYPE_FP32   ? rotary_n<float>(n, a, (unsigned)grid, st)
+                  : dtype == VGGT_DTYPE_FP16 ? rotary_n<__half>(n, a, (unsigned)grid, st)
+                                             : rotary_n<__nv_bfloat16>(n, a, (unsigned)grid, st));
+}
+
+extern "C" int vggt_paged_append(
+    const void* k, const void* v, int dtype, int64_t total, int64_t k_token_stride,
+    int64_t k_head_stride, int64_t v_token_stride, int64_t v_head_stride, void* k_pages,
+    void* v_pages, int64_t n_pages, int kv_heads, int page, int dim, int64_t page_stride,
+    int64_t head_stride, int64_t row_stride, const int32_t* table, int64_t table_width,
+    int64_t seqs, const int32_t* before, const int32_t* starts, const int32_t* positions, int axes,
+    const double* freq, int pairs, int layout, float lengthen, int32_t* ids,
+    const int32_t* new_ids, float* weights, const float* new_weights, int32_t* after,
+    int32_t* status, void* stream) {
+  AppendArgs a{};
+  if (int rc = check_pool(dtype, n_pages, kv_heads, page, dim, page_stride, head_stride,
+                          row_stride, table_width, seqs, total, &a.pool))
+    return rc;
+  if (seqs == 0) return api_fail(nullptr);
+  if (positions != nullptr) {
+    if (int rc = check_rotation(dim, positions, axes, freq, pairs, layout, lengthen)) return rc;
+  } else {
+    axes = 0;
+    pairs = 1;
+  }
+  if (!before || !starts || !after) return api_fail("before, starts and after must be non-NULL");
+  if (total > 0 && (!k || !v || !k_pages || !v_pages || !table))
+    return api_fail("k, v, the pools and the table must be non-NULL");
+  if (ids != nullptr && new_ids == nullptr) return api_fail("ids needs new_ids");
+  const int n = pairs_per_thread(2, dim, axes, pairs,
+                                 {k_token_stride, k_head_stride, v_token_stride, v_head_stride,
+                                  page_stride, head_stride, row_stride},
+                                 {k, v, k_pages, v_pages});
+  a.k = k;
+  a.v = v;
+  a.kp = k_pages;
+  a.vp = v_pages;
+  a.kt = k_token_stride;
+  a.kh = k_head_stride;
+  a.vt = v_token_stride;
+  a.vh = v_head_stride;
+  a.t = {table, before, starts, table_width, seqs, total, status};
+  a.units = dim / (2 * n);
+  a.deal = deal_heads(total * a.units, kv_heads);
+  a.main_blocks = (total * a.units * a.deal + kThreads - 1) / kThreads;
+  a.g = {positions, freq, axes, pairs, layout == VGGT_ROTARY_INTERLEAVED, lengthen, 1.f};
+  a.ids = ids;
+  a.after = after;
+  a.new_ids = new_ids;
+  a.weights = weights;
+  a.new_weights = new_weights;
+  const int64_t grid = a.main_blocks + ((total > seqs ? total : seqs) + kThreads - 1) / kThreads;
+  if (grid > 0x7fffffffLL) return api_fail("too many new tokens (%lld)", (long long)total);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  return api_cuda(dtype == VGGT_DTYPE_FP16 ? append_n<__half>(n, a, (unsigned)grid, st)
+                                           : append_n<__nv_bfloat16>(n, a, (unsigned)grid, st));
+}

@@ -103,6 +103,15 @@ __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map
       : "memory");
 }
 
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, uint32_t bar,
+                                            int c0, int c1, int c2, int c3) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
+      : "memory");
+}
+
 __device__ __forceinline__ void prefetch_tmap(const CUtensorMap* map) {
   asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(map)) : "memory");
 }
@@ -236,6 +245,10 @@ __device__ __forceinline__ void tmem_wait_st() {
 // Host: 3-D tensor map [d2][d1][d0] of 2-byte elements (VGGT_DTYPE_*), box
 // (box0, box1, 1), 128-byte swizzle, zero fill out of bounds.  False when the
 // driver entry point is unavailable or the driver rejects the arguments.
+// Tiled map of 2-byte elements of any rank (strides in bytes, of dimensions 1
+// and up), 128-byte swizzle, zero fill out of bounds.
+bool encode_tmap_sw128(CUtensorMap* map, const void* ptr, int dtype, int rank,
+                       const uint64_t* dims, const uint64_t* strides, const uint32_t* box);
 bool encode_tmap_3d_sw128(CUtensorMap* map, const void* ptr, int dtype, int64_t d0, int64_t d1,
                           int64_t d2, uint32_t box0, uint32_t box1);
 

@@ -1,4 +1,5 @@
-"""ctypes binding of the C ABI declared in include/vggt_sparse.h.
+"""ctypes binding of the C ABI declared in include/vggt_sparse.h and
+include/vggt_cache.h.
 
 The shared library is built in-tree (``vggt_sparse.build``).  There is no
 CPU or Python fallback: if the library is missing every operator raises
@@ -12,12 +13,18 @@ from .build import LIB_PATH
 DTYPE_BF16, DTYPE_FP16 = 0, 1
 SELECT_TOPK, SELECT_MASS = 0, 1
 ATTN_AUTO, ATTN_MMA_SYNC, ATTN_TCGEN05 = 0, 1, 2
+DTYPE_FP32 = 2  # vggt_rotary only
+ROTARY_HALF, ROTARY_INTERLEAVED = 0, 1
 STATUS_BAD_INDEX, STATUS_BAD_COUNT, STATUS_TIMEOUT, STATUS_BAD_HEAD = 1, 2, 4, 8
+STATUS_BAD_PAGE, STATUS_BAD_LENGTH = 16, 32
 
-# Every symbol the header declares, with its ctypes signature.
+# Every symbol the headers declare, with its ctypes signature.
 _P = ctypes.c_void_p
 _I64 = ctypes.c_int64
 _I = ctypes.c_int
+_F = ctypes.c_float
+# pools: n_pages, kv_heads, page, dim, three strides; table, its width, seqs
+_POOL = [_I64, _I, _I, _I, _I64, _I64, _I64, _P, _I64, _I64]
 SIGNATURES = {
     "vggt_sparse_version": (_I, []),
     "vggt_sparse_last_error": (ctypes.c_char_p, []),
@@ -52,6 +59,19 @@ SIGNATURES = {
     "vggt_block_mask_estimate_noalloc": (_I, [_P, _P, _I, _I64, _I64, _I64, _I, _P, _I64, _I, _I,
                                               _I, _I64, ctypes.c_double, ctypes.c_float, _P, _I64,
                                               _P, _P, _P, _P]),
+    "vggt_rotary": (_I, [_P, _I, _I64, _I, _I, _I64, _I64, _P, _I, _P, _I, _I, _F, _I, _P, _I64,
+                         _I64, _P]),
+    "vggt_paged_append": (_I, [_P, _P, _I, _I64, _I64, _I64, _I64, _I64, _P, _P, *_POOL, _P, _P,
+                               _P, _I, _P, _I, _I, _F, _P, _P, _P, _P, _P, _P, _P]),
+    "vggt_paged_attention_workspace_size": (ctypes.c_size_t, [_I64, _I64, _I, _I, _I, _I64,
+                                                              _I64]),
+    "vggt_paged_attention": (_I, [_P, _I, _I64, _I64, _I64, _P, _P, *_POOL, _P, _P, _I, _I, _F,
+                                  _I64, _I64, _P, _I64, _I64, _P, _P, _P, ctypes.c_size_t, _P]),
+    "vggt_paged_weights": (_I, [_P, _I, _I64, _I64, _I64, _P, _P, *_POOL, _P, _P, _I, _I, _F, _F,
+                                _I64, _I64, _P, _P, _P]),
+    "vggt_paged_evict_workspace_size": (ctypes.c_size_t, [_I64, _I, _I64, _I64]),
+    "vggt_paged_evict": (_I, [_P, _P, _I, _P, _P, *_POOL, _P, _I64, _P, _I64, _P, _P, _P, _P, _P,
+                              ctypes.c_size_t, _P]),
 }
 
 
