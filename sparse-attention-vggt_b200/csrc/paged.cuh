@@ -183,6 +183,9 @@ struct PagedPlan {
 PagedPlan paged_rows_plan(int64_t total, int64_t seqs, int kv_heads, int group, int dim,
                           int64_t max_new, int64_t max_len);
 cudaError_t launch_paged_rows(const PagedAttnArgs& a, const PagedPlan& plan, cudaStream_t st);
+PagedPlan paged_tc05_plan(int64_t total, int64_t seqs, int kv_heads, int group, int dim,
+                          int64_t max_len);
+cudaError_t launch_paged_tc05(const PagedAttnArgs& a, const PagedPlan& plan, cudaStream_t st);
 
 // Host: checks the sizes that every paged entry point takes and fills `pool`.
 int check_pool(int dtype, int64_t n_pages, int kv_heads, int page, int dim, int64_t page_stride,

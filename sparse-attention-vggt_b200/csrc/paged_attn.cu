@@ -8,9 +8,15 @@ using namespace vggt;
 
 namespace {
 
+// Up to 64 rows per sequence and key head go to the warp-level kernel, more to
+// the tcgen05 one.
+bool few_rows(int64_t max_new, int group) { return max_new * group <= 64; }
+
 PagedPlan plan_of(int64_t total, int64_t seqs, int kv_heads, int group, int dim, int64_t max_new,
                   int64_t max_len) {
-  return paged_rows_plan(total, seqs, kv_heads, group, dim, max_new, max_len);
+  return few_rows(max_new, group)
+             ? paged_rows_plan(total, seqs, kv_heads, group, dim, max_new, max_len)
+             : paged_tc05_plan(total, seqs, kv_heads, group, dim, max_len);
 }
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
@@ -77,5 +83,7 @@ extern "C" int vggt_paged_attention(
   a.max_len = max_len;
   a.workspace = workspace;
   a.wait_ns = api_wait_ns();
-  return api_cuda(launch_paged_rows(a, plan, static_cast<cudaStream_t>(stream)));
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  return api_cuda(few_rows(max_new, group) ? launch_paged_rows(a, plan, st)
+                                           : launch_paged_tc05(a, plan, st));
 }

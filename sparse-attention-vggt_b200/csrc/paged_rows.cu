@@ -62,7 +62,7 @@ struct Shared {
 template <typename T, int D, int MT>
 __global__ void __launch_bounds__(kThreads, 2)
     paged_rows_kernel(const __grid_constant__ CUtensorMap tm_k,
-                      const __grid_constant__ CUtensorMap tm_v, const RowsParams p) {
+                      const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ RowsParams p) {
   using R = Ring<D>;
   constexpr int kRows = 16 * MT;
   constexpr int kGroups = 4 / MT;             // warps that share a row tile's keys
