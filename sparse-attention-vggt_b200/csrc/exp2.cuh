@@ -5,27 +5,33 @@
 
 namespace vggt {
 
-// (d0, d1) = (a0, a1) * b + c with one packed instruction
-__device__ __forceinline__ void fma_pair(float& d0, float& d1, float a0, float a1, float b,
-                                         float c) {
-  asm("{\n\t.reg .b64 ra, rb, rc, rd;\n\t"
-      "mov.b64 ra, {%2, %3};\n\t"
-      "mov.b64 rb, {%4, %4};\n\t"
-      "mov.b64 rc, {%5, %5};\n\t"
-      "fma.rn.f32x2 rd, ra, rb, rc;\n\t"
-      "mov.b64 {%0, %1}, rd;\n\t}"
-      : "=f"(d0), "=f"(d1)
-      : "f"(a0), "f"(a1), "f"(b), "f"(c));
-}
+// Two floats in a 64-bit register, as the packed instructions take them.
+// Operands that do not change are packed once: a packing inside the loop costs
+// up to four moves per packed instruction, more than the instruction saves.
+typedef uint64_t float_pair;
 
-__device__ __forceinline__ void add_pair(float& d0, float& d1, float a0, float a1) {
-  asm("{\n\t.reg .b64 ra, rd;\n\t"
-      "mov.b64 ra, {%2, %3};\n\t"
-      "mov.b64 rd, {%0, %1};\n\t"
-      "add.rn.f32x2 rd, rd, ra;\n\t"
-      "mov.b64 {%0, %1}, rd;\n\t}"
-      : "+f"(d0), "+f"(d1)
-      : "f"(a0), "f"(a1));
+__device__ __forceinline__ float_pair pack_pair(float a, float b) {
+  float_pair r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void unpack_pair(float& a, float& b, float_pair v) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
+}
+__device__ __forceinline__ float_pair fma_pair(float_pair a, float_pair b, float_pair c) {
+  float_pair r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ float_pair add_pair(float_pair a, float_pair b) {
+  float_pair r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ float_pair sub_pair(float_pair a, float_pair b) {
+  float_pair r;
+  asm("sub.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
 }
 
 // 2^a, 2^b for arguments up to 126 without the multi-function unit: x = n + f
@@ -33,32 +39,36 @@ __device__ __forceinline__ void add_pair(float& d0, float& d1, float a0, float a
 // polynomial of degree 4 for 2^f on [-1/2, 1/2] (fitted to the least largest
 // relative error, 2.7e-6 in fp32), n added to its exponent.  Arguments below
 // -126 give 2^-126 at most.
-__device__ __forceinline__ void exp2_poly_pair(float& ea, float& eb, float a, float b) {
-  a = fmaxf(a, -126.f);
-  b = fmaxf(b, -126.f);
-  float qa, qb, ta, tb;
-  asm("{\n\t.reg .b64 x, m, t, n, f, q, c4, c3, c2, c1, c0;\n\t"
-      "mov.b64 x, {%4, %5};\n\t"
-      "mov.b64 m, {%6, %6};\n\t"
-      "mov.b64 c4, {%7, %7};\n\t"
-      "mov.b64 c3, {%8, %8};\n\t"
-      "mov.b64 c2, {%9, %9};\n\t"
-      "mov.b64 c1, {%10, %10};\n\t"
-      "mov.b64 c0, {%11, %11};\n\t"
-      "add.rn.f32x2 t, x, m;\n\t"
-      "sub.rn.f32x2 n, t, m;\n\t"
-      "sub.rn.f32x2 f, x, n;\n\t"
-      "fma.rn.f32x2 q, f, c4, c3;\n\t"
-      "fma.rn.f32x2 q, q, f, c2;\n\t"
-      "fma.rn.f32x2 q, q, f, c1;\n\t"
-      "fma.rn.f32x2 q, q, f, c0;\n\t"
-      "mov.b64 {%0, %1}, q;\n\t"
-      "mov.b64 {%2, %3}, t;\n\t}"
-      : "=f"(qa), "=f"(qb), "=f"(ta), "=f"(tb)
-      : "f"(a), "f"(b), "f"(12582912.f), "f"(0.0095701022f), "f"(0.0559178591f),
-        "f"(0.2402474433f), "f"(0.6931217909f), "f"(0.9999992847f));
-  ea = __int_as_float(__float_as_int(qa) + (__float_as_int(ta) << 23));
-  eb = __int_as_float(__float_as_int(qb) + (__float_as_int(tb) << 23));
+struct Exp2Poly {
+  float_pair magic, c4, c3, c2, c1, c0;
+  __device__ __forceinline__ Exp2Poly()
+      : magic(pack_pair(12582912.f, 12582912.f)),
+        c4(pack_pair(0.0095701022f, 0.0095701022f)),
+        c3(pack_pair(0.0559178591f, 0.0559178591f)),
+        c2(pack_pair(0.2402474433f, 0.2402474433f)),
+        c1(pack_pair(0.6931217909f, 0.6931217909f)),
+        c0(pack_pair(0.9999992847f, 0.9999992847f)) {}
+  __device__ __forceinline__ void operator()(float& ea, float& eb, float_pair x) const {
+    float a, b, ta, tb, qa, qb;
+    unpack_pair(a, b, x);
+    x = pack_pair(fmaxf(a, -126.f), fmaxf(b, -126.f));
+    const float_pair t = add_pair(x, magic);
+    const float_pair f = sub_pair(x, sub_pair(t, magic));
+    float_pair q = fma_pair(f, c4, c3);
+    q = fma_pair(q, f, c2);
+    q = fma_pair(q, f, c1);
+    q = fma_pair(q, f, c0);
+    unpack_pair(qa, qb, q);
+    unpack_pair(ta, tb, t);
+    ea = __int_as_float(__float_as_int(qa) + (__float_as_int(ta) << 23));
+    eb = __int_as_float(__float_as_int(qb) + (__float_as_int(tb) << 23));
+  }
+};
+
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
 }
 
 // Maximum of three that keeps a NaN.

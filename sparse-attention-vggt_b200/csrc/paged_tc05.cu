@@ -5,23 +5,34 @@
 // group, so grouped heads fill the tile) and one run of 64-key tiles:
 //   warp 0     streams K and V tiles by TMA, a box per page (or per 64 slots
 //              of a larger page), into two rings; page numbers are read 32
-//              boxes ahead, one lane issues one box
-//   warp 1     one lane issues S_t = Q K_t^T (Q, K in shared memory, S double-
-//              buffered in TMEM) and O += P_t V_t (P read from TMEM, where it
-//              overwrote S_t; O stays in TMEM for the whole run)
-//   warps 2-5  softmax, one query row per thread
-// Two CTAs share an SM, so that one's softmax runs under the other's MMAs.
+//              boxes ahead
+//   warp 1     issues S_t = Q K_t^T (Q, K in shared memory, S double-buffered
+//              in TMEM)
+//   warp 2     issues O += P_t V_t (P read from TMEM, where it overwrote S_t;
+//              O stays in TMEM for the whole run)
+//   warps 4-7  softmax, one query row per thread
+// Two CTAs share an SM.  The issue is split over two warps, whole warps that
+// wait and elect a lane to issue: on this chip a wait on a barrier costs a
+// warp some 150 clocks even where it is satisfied, and the issue of four MMAs
+// 200 to 300, so that one warp's four steps per tile took longer than the
+// tile's softmax (510 us for a frame over 31 cached ones against 375).
 //
 // The row's reference maximum moves only when a tile's maximum exceeds it by
-// more than 2^8 in the exp2 domain; O is rescaled then.  P is published in
-// two halves, so that the first half's product runs under the second half's
-// exponentials.  Sums are fp32, of the exponentials before P is rounded: the
-// log-sum-exp is good to fp32 and only the product with V sees the rounding.
+// more than 2^8 in the exp2 domain; O is rescaled then.  Sums are fp32, of the
+// exponentials before P is rounded: the log-sum-exp is good to fp32 and only
+// the product with V sees the rounding.
 //
 // What bounds it: the multi-function unit gives 16 exponentials per clock and
-// SM, so a 128 x 64 tile costs 512 clocks there, against 256 (dim 64) or 512
-// (dim 128) of MMA at full rate.  Therefore some column pairs take a
-// polynomial on the FMA pipe instead.
+// SM, so a 128 x 64 tile costs 512 clocks there, against 320 (dim 64) or 640
+// (dim 128) of MMA (A from shared memory takes 48 clocks per MMA at N = 64, 32
+// from TMEM).  One column pair of eight therefore takes a polynomial on the
+// FMA pipe; at two of eight the instructions cost what the unit saves (374
+// against 381 us).  A tile takes 650 clocks: the softmax warps' own chain
+// (wait, load, maximum, exponentials, store) is not fully covered by the other
+// CTA's.  Tried and slower: 32 keys per thread and 8 softmax warps (404 us),
+// 128-key tiles with one S buffer (449 us), the next tile's maximum between
+// the exponentials (634 us: its small TMEM loads wait for the stores), no
+// maximum but a check of the tile's sum (388 us).
 //
 // Slots past the last key that any row sees are cleared in shared memory
 // before their product (their content is not defined).  A key that only later
@@ -40,7 +51,14 @@
 namespace vggt {
 namespace {
 
-constexpr int kRows = 128, kTile = 64, kThreads = 192;
+constexpr int kRows = 128, kTile = 64;
+// Warps 0-3: TMA producer, S issuer, O issuer, one idle; warps 4-7: softmax.
+constexpr int kThreads = 256;
+// setmaxnreg: the launch gives every thread kLaunchRegs (two CTAs fill the
+// register file); warps 0-3 give back down to kControlRegs, the softmax takes
+// what that frees.
+constexpr int kLaunchRegs = 128, kControlRegs = 64, kSoftRegs = 192;
+static_assert(kControlRegs + kSoftRegs == 2 * kLaunchRegs, "register split");
 constexpr uint32_t kTmemCols = 256;  // S0 | S1 | O
 constexpr uint64_t kDrainNs = 1000000000ull;
 
@@ -56,8 +74,8 @@ struct Smem {
 };
 
 struct Bars {
-  uint64_t q_full, k_full[4], k_empty[4], v_full[4], v_empty[4];
-  uint64_t s_full[2], p_full[2][2], pv_done, o_full, drain;
+  uint64_t q_full, full[2][4], empty[2][4];  // of K, of V
+  uint64_t s_full[2], s_free[2], p_full[2], o_full, drain[2];
 };
 
 struct TcParams {
@@ -69,7 +87,7 @@ struct TcParams {
 };
 
 // column pairs of every 8 whose exponentials take the polynomial
-constexpr unsigned kPolyPairs = 0x11u;
+constexpr unsigned kPolyPairs = 0x01u;
 
 template <typename T, int D>
 __global__ void __launch_bounds__(kThreads, 2)
@@ -113,26 +131,25 @@ __global__ void __launch_bounds__(kThreads, 2)
 
   volatile int* abort_flag = &s_abort;
   if (tid == 0) {
-    tc::mbar_init(smem_u32(&bars.q_full), 128);
+    tc::mbar_init(smem_u32(&bars.q_full), kRows);
     for (int s = 0; s < kStages; ++s) {
-      tc::mbar_init(smem_u32(&bars.k_full[s]), 1);
-      tc::mbar_init(smem_u32(&bars.k_empty[s]), 1);
-      tc::mbar_init(smem_u32(&bars.v_full[s]), 1);
-      tc::mbar_init(smem_u32(&bars.v_empty[s]), 1);
+      for (int kv = 0; kv < 2; ++kv) {
+        tc::mbar_init(smem_u32(&bars.full[kv][s]), 1);
+        tc::mbar_init(smem_u32(&bars.empty[kv][s]), 1);
+      }
     }
     for (int b = 0; b < 2; ++b) {
       tc::mbar_init(smem_u32(&bars.s_full[b]), 1);
-      tc::mbar_init(smem_u32(&bars.p_full[b][0]), 128);
-      tc::mbar_init(smem_u32(&bars.p_full[b][1]), 128);
+      tc::mbar_init(smem_u32(&bars.s_free[b]), 1);
+      tc::mbar_init(smem_u32(&bars.p_full[b]), kRows);
     }
-    tc::mbar_init(smem_u32(&bars.pv_done), 1);
     tc::mbar_init(smem_u32(&bars.o_full), 1);
-    tc::mbar_init(smem_u32(&bars.drain), 1);
+    for (int i = 0; i < 2; ++i) tc::mbar_init(smem_u32(&bars.drain[i]), 1);
     s_abort = 0;
     s_odd = 0;
     tc::mbar_fence_init();
   }
-  if (warp == 1) {
+  if (warp == 4) {
     tc::tmem_alloc(smem_u32(&s_tmem), kTmemCols);
     tc::tmem_relinquish();
   }
@@ -142,113 +159,169 @@ __global__ void __launch_bounds__(kThreads, 2)
   const uint32_t tmem = s_tmem;
   const uint32_t t_o = tmem + 128u;
 
-  if (warp == 0) {
+  if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kControlRegs));
+    if (warp == 0) {
     // ================= TMA producer =================
-    const int box = a.pool.page < kTile ? a.pool.page : kTile;
-    const int boxes = kTile / box, ahead = 32 / boxes;
-    // a lane issues box `b` of half `half` of K (matrix 0) or V (matrix 1)
-    const int b = lane & (boxes - 1), half = (lane / boxes) % kHalves;
-    const int matrix = lane / (boxes * kHalves);
-    int page = -1;
-    int issued_k = 0, issued_v = 0;
-    for (int t = 0; t < tiles; ++t) {
-      const int64_t key0 = (tile0 + t) * kTile;
-      if (t % ahead == 0) {
-        const int64_t slot = key0 + (int64_t)lane * box;
-        page = (int)a.pool.n_pages;  // past the pool: reads as zeros
-        if (slot < most && slot < (tile0 + tiles) * kTile) {
-          const int got = checked_page(a.t, a.pool, rt.seq, slot >> a.pool.page_shift);
-          if (got >= 0) page = got;
+    const int keys = (int)(most - tile0 * kTile);  // to the end of the last row's keys
+    auto produce = [&](auto boxes_) {
+      constexpr int kBoxes = decltype(boxes_)::value;  // boxes per tile
+      constexpr int kBox = kTile / kBoxes;             // slots per box
+      constexpr int kAhead = 32 / kBoxes;              // tiles per read of the table
+      const uint32_t full0 = smem_u32(&bars.full[0][0]), empty0 = smem_u32(&bars.empty[0][0]);
+      constexpr uint32_t kToV = sizeof(bars.full[0]);  // from K's barriers to V's
+      const int32_t* table = a.t.table + rt.seq * a.t.width;
+      const int64_t first_slot = tile0 * kTile;
+      const int in_page = (int)first_slot & (a.pool.page - 1), page_mask = a.pool.page - 1;
+      int page = 0, stage = 0;
+      int issued_at[2] = {0, 0};  // of the elected lane
+      uint32_t phase = 1;
+      for (int t = 0; t < tiles; ++t) {
+        const int key0 = t * kTile;
+        const int turn = t & (kAhead - 1);
+        if (turn == 0) {
+          const int key = key0 + lane * kBox;
+          page = (int)a.pool.n_pages;  // past the pool: reads as zeros
+          if (key < keys && key < tiles * kTile) {
+            const int got = __ldg(table + ((first_slot + key) >> a.pool.page_shift));
+            if (got >= 0 && got < a.pool.n_pages)
+              page = got;
+            else
+              raise_status(a.t.status, VGGT_STATUS_BAD_PAGE);
+          }
+        }
+        int pages[kBoxes];
+#pragma unroll
+        for (int b = 0; b < kBoxes; ++b)
+          pages[b] = __shfl_sync(0xffffffffu, page, turn * kBoxes + b);
+        int live = (keys - key0 + kBox - 1) / kBox;
+        live = live < kBoxes ? live : kBoxes;
+        const int row = (in_page + key0) & page_mask;
+        bool ok = true;
+#pragma unroll
+        for (int kv = 0; kv < 2; ++kv) {
+          if (t >= kStages)
+            ok = ok && __all_sync(0xffffffffu, tc::mbar_wait(empty0 + kv * kToV + 8u * stage, phase,
+                                                             abort_flag, a.wait_ns));
+          if (ok && tc::elect_one()) {
+            const uint32_t bar = full0 + kv * kToV + 8u * stage;
+            tc::mbar_expect_tx(bar, (uint32_t)(live * kBox) * D * 2u);
+            const uint32_t dst = base + (kv ? L::kV : L::kK) + stage * L::kMatrix;
+#pragma unroll
+            for (int b = 0; b < kBoxes; ++b)
+              if (b < live)
+#pragma unroll
+                for (int h = 0; h < kHalves; ++h)
+                  tc::tma_load_4d(dst + h * (kTile * 128) + b * kBox * 128, kv ? &tm_v : &tm_k,
+                                  bar, h * 64, (row + b * kBox) & page_mask, head, pages[b]);
+            issued_at[kv] = t + 1;
+          }
+          __syncwarp();
+        }
+        if (!ok) break;
+        if (++stage == kStages) {
+          stage = 0;
+          phase ^= 1u;
         }
       }
-      const int mine = __shfl_sync(0xffffffffu, page, (t % ahead) * boxes + b);
-      const int need = (int)((most - key0 + box - 1) / box);
-      const int live = need < boxes ? need : boxes;
-      const int row = (int)((key0 + b * box) & (a.pool.page - 1));
-      const int stage = t % kStages;
-      const uint32_t phase = (uint32_t)((t / kStages - 1) & 1);
-      const uint32_t off = stage * L::kMatrix + half * (kTile * 128) + b * box * 128;
-      bool ok = t < kStages || tc::mbar_wait(smem_u32(&bars.k_empty[stage]), phase, abort_flag,
-                                             a.wait_ns);
-      if (!__all_sync(0xffffffffu, ok)) break;
-      if (lane == 0)
-        tc::mbar_expect_tx(smem_u32(&bars.k_full[stage]), (uint32_t)(live * box) * D * 2u);
-      __syncwarp();
-      if (matrix == 0 && b < live)
-        tc::tma_load_4d(base + L::kK + off, &tm_k, smem_u32(&bars.k_full[stage]), half * 64, row,
-                        head, mine);
-      ++issued_k;
-      ok = t < kStages || tc::mbar_wait(smem_u32(&bars.v_empty[stage]), phase, abort_flag,
-                                        a.wait_ns);
-      if (!__all_sync(0xffffffffu, ok)) break;
-      if (lane == 0)
-        tc::mbar_expect_tx(smem_u32(&bars.v_full[stage]), (uint32_t)(live * box) * D * 2u);
-      __syncwarp();
-      if (matrix == 1 && b < live)
-        tc::tma_load_4d(base + L::kV + off, &tm_v, smem_u32(&bars.v_full[stage]), half * 64, row,
-                        head, mine);
-      ++issued_v;
-    }
-    // no copy may be in flight when the CTA leaves
-    for (int t = issued_k > kStages ? issued_k - kStages : 0; t < issued_k; ++t)
-      tc::mbar_wait_drain(smem_u32(&bars.k_full[t % kStages]), (uint32_t)((t / kStages) & 1),
-                          kDrainNs);
-    for (int t = issued_v > kStages ? issued_v - kStages : 0; t < issued_v; ++t)
-      tc::mbar_wait_drain(smem_u32(&bars.v_full[t % kStages]), (uint32_t)((t / kStages) & 1),
-                          kDrainNs);
-  } else if (warp == 1) {
-    // ================= MMA issuer =================
-    if (lane == 0) {
-      const uint32_t fmt = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
+      // no copy may be in flight when the CTA leaves
+      for (int kv = 0; kv < 2; ++kv)
+        for (int t = issued_at[kv] > kStages ? issued_at[kv] - kStages : 0; t < issued_at[kv]; ++t)
+          tc::mbar_wait_drain(full0 + kv * kToV + 8u * (t % kStages),
+                              (uint32_t)((t / kStages) & 1), kDrainNs);
+    };
+    if (a.pool.page >= 64)
+      produce(std::integral_constant<int, 1>{});
+    else if (a.pool.page == 32)
+      produce(std::integral_constant<int, 2>{});
+    else
+      produce(std::integral_constant<int, 4>{});
+    } else if (warp < 3) {
+    // ================= MMA issuers: warp 1 S = Q K^T, warp 2 O += P V ========
+    // Two warps, because a wait on a barrier costs a warp some 200 clocks and
+    // the issue of four MMAs 300: in one warp the four steps of a tile took
+    // longer than its softmax.  A whole warp walks through the tiles and waits;
+    // one elected lane issues, which keeps the MMA operands in uniform
+    // registers.
+    const uint32_t fmt = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
+    auto wait = [&](uint32_t bar, uint32_t parity) {
+      return __all_sync(0xffffffffu, tc::mbar_wait(bar, parity, abort_flag, a.wait_ns));
+    };
+    const uint32_t kfull0 = smem_u32(&bars.full[0][0]), kempty0 = smem_u32(&bars.empty[0][0]);
+    const uint32_t vfull0 = smem_u32(&bars.full[1][0]), vempty0 = smem_u32(&bars.empty[1][0]);
+    const uint32_t sfull0 = smem_u32(&bars.s_full[0]), pfull0 = smem_u32(&bars.p_full[0]);
+    const uint32_t sfree0 = smem_u32(&bars.s_free[0]);
+    int stage = 0;
+    uint32_t phase = 0;
+    bool ok = true;
+    if (warp == 1) {
       const uint32_t id_qk = tc::idesc_f16(fmt, 0u, kRows, kTile);
-      const uint32_t id_pv = tc::idesc_f16(fmt, 1u, kRows, D);
-      bool ok = tc::mbar_wait(smem_u32(&bars.q_full), 0, abort_flag, a.wait_ns);
       const uint64_t qdesc = tc::sw128_desc(base + L::kQ, 16);
-      auto issue_pv = [&](int u) -> bool {
-        const int stage = u % kStages, buf = u & 1;
-        if (!tc::mbar_wait(smem_u32(&bars.v_full[stage]), (uint32_t)((u / kStages) & 1),
-                           abort_flag, a.wait_ns))
-          return false;
-        // 64-element groups of V's rows lie kTile * 128 bytes apart
-        const uint64_t vdesc = tc::sw128_desc(base + L::kV + stage * L::kMatrix, kTile * 128);
-#pragma unroll
-        for (int part = 0; part < 2; ++part) {
-          if (!tc::mbar_wait(smem_u32(&bars.p_full[buf][part]), (uint32_t)((u >> 1) & 1),
-                             abort_flag, a.wait_ns))
-            return false;
-          tc::tc_fence_after();
-#pragma unroll
-          for (int kk = 2 * part; kk < 2 * part + 2; ++kk)
-            tc::mma_ts(t_o, tmem + 64u * buf + 8u * kk, vdesc + (uint64_t)(kk * 128), id_pv,
-                       (u > 0 || kk > 0) ? 1u : 0u);
-        }
-        tc::mma_commit(smem_u32(&bars.pv_done));
-        tc::mma_commit(smem_u32(&bars.v_empty[stage]));
-        return true;
-      };
+      const uint64_t kdesc0 = tc::sw128_desc(base + L::kK, 16);
+      ok = wait(smem_u32(&bars.q_full), 0);
       for (int t = 0; ok && t < tiles; ++t) {
-        const int stage = t % kStages, buf = t & 1;
-        ok = tc::mbar_wait(smem_u32(&bars.k_full[stage]), (uint32_t)((t / kStages) & 1),
-                           abort_flag, a.wait_ns);
+        const uint32_t buf = t & 1;
+        // P of tile t - 2 lay where S_t goes: its product must be done
+        ok = (t < 2 || wait(sfree0 + 8u * buf, (uint32_t)((t >> 1) + 1) & 1u)) &&
+             wait(kfull0 + 8u * stage, phase);
         if (!ok) break;
         tc::tc_fence_after();
-        const uint64_t kdesc = tc::sw128_desc(base + L::kK + stage * L::kMatrix, 16);
+        if (tc::elect_one()) {
+          const uint64_t kdesc = kdesc0 + (uint64_t)(stage * (L::kMatrix / 16));
 #pragma unroll
-        for (int kk = 0; kk < D / 16; ++kk)
-          tc::mma_ss(tmem + 64u * buf,
-                     qdesc + (uint64_t)((kk >> 2) * (kRows * 128 / 16) + (kk & 3) * 2),
-                     kdesc + (uint64_t)((kk >> 2) * (kTile * 128 / 16) + (kk & 3) * 2), id_qk,
-                     kk > 0 ? 1u : 0u);
-        tc::mma_commit(smem_u32(&bars.s_full[buf]));
-        tc::mma_commit(smem_u32(&bars.k_empty[stage]));
-        if (t >= 1) ok = issue_pv(t - 1);
+          for (int kk = 0; kk < D / 16; ++kk)
+            tc::mma_ss(tmem + 64u * buf,
+                       qdesc + (uint64_t)((kk >> 2) * (kRows * 128 / 16) + (kk & 3) * 2),
+                       kdesc + (uint64_t)((kk >> 2) * (kTile * 128 / 16) + (kk & 3) * 2), id_qk,
+                       kk > 0 ? 1u : 0u);
+          tc::mma_commit(sfull0 + 8u * buf);
+          tc::mma_commit(kempty0 + 8u * stage);
+        }
+        __syncwarp();
+        if (++stage == kStages) {
+          stage = 0;
+          phase ^= 1u;
+        }
       }
-      if (ok && tiles > 0 && issue_pv(tiles - 1)) tc::mma_commit(smem_u32(&bars.o_full));
-      // every issued MMA must finish before the TMEM columns are released
-      tc::mma_commit(smem_u32(&bars.drain));
-      tc::mbar_wait_drain(smem_u32(&bars.drain), 0, kDrainNs);
+    } else {
+      const uint32_t id_pv = tc::idesc_f16(fmt, 1u, kRows, D);
+      // 64-element groups of V's rows lie kTile * 128 bytes apart
+      const uint64_t vdesc0 = tc::sw128_desc(base + L::kV, kTile * 128);
+      for (int t = 0; ok && t < tiles; ++t) {
+        const uint32_t buf = t & 1;
+        ok = wait(vfull0 + 8u * stage, phase) && wait(pfull0 + 8u * buf, (uint32_t)(t >> 1) & 1u);
+        if (!ok) break;
+        tc::tc_fence_after();
+        if (tc::elect_one()) {
+          const uint64_t vdesc = vdesc0 + (uint64_t)(stage * (L::kMatrix / 16));
+#pragma unroll
+          for (int kk = 0; kk < kTile / 16; ++kk)
+            tc::mma_ts(t_o, tmem + 64u * buf + 8u * kk, vdesc + (uint64_t)(kk * 128), id_pv,
+                       (t > 0 || kk > 0) ? 1u : 0u);
+          tc::mma_commit(sfree0 + 8u * buf);
+          tc::mma_commit(vempty0 + 8u * stage);
+        }
+        __syncwarp();
+        if (++stage == kStages) {
+          stage = 0;
+          phase ^= 1u;
+        }
+      }
     }
-  } else {
+    if (tc::elect_one()) {
+      if (warp == 2 && ok && tiles > 0) tc::mma_commit(smem_u32(&bars.o_full));
+      // every issued MMA must finish before the TMEM columns are released
+      tc::mma_commit(smem_u32(&bars.drain[warp - 1]));
+    }
+    __syncwarp();
+    tc::mbar_wait_drain(smem_u32(&bars.drain[warp - 1]), 0, kDrainNs);
+    }
+    return;  // what follows runs on the softmax warps alone
+  }
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftRegs));
+  const int stid = tid - 128;
+  auto sync_softmax = [] { asm volatile("bar.sync 1, 128;" ::: "memory"); };
+  {
     // ================= softmax: one query row per thread =================
     const int sub = warp & 3;  // TMEM lane quarter of this warp
     const int row = sub * 32 + lane;
@@ -272,126 +345,142 @@ __global__ void __launch_bounds__(kThreads, 2)
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       tc::mbar_arrive(smem_u32(&bars.q_full));
     }
-    float m_ref = -INFINITY, l0 = 0.f, l1 = 0.f;
-    bool ok = true;
+    // counted from the run's first key, within one tile of its ends
+    const int span = tiles * kTile;
+    auto within = [&](int64_t key) {
+      const int64_t n = key - tile0 * kTile;
+      return (int)(n < 0 ? 0 : (n < span ? n : span));
+    };
+    const int lim_at = within(lim), least_at = within(least), most_at = within(most);
+    const uint32_t sfull0 = smem_u32(&bars.s_full[0]), pfull0 = smem_u32(&bars.p_full[0]);
+    auto wait = [&](uint32_t bar, uint32_t parity) {
+      return __all_sync(0xffffffffu, tc::mbar_wait(bar, parity, abort_flag, a.wait_ns));
+    };
+    // whether some row of the CTA does not see all of tile t (for all warps alike)
+    auto is_edge = [&](int t) { return (t + 1) * kTile > least_at; };
+    float m_ref = -INFINITY;  // in score units; exponents are relative to it
+    float_pair sum = pack_pair(0.f, 0.f);
+    const float_pair c2 = pack_pair(c, c);
+    const Exp2Poly poly;
+    bool ok = true, ready = false;
     for (int t = 0; t < tiles; ++t) {
-      const int buf = t & 1;
-      const int64_t key0 = (tile0 + t) * kTile;
-      if (!__all_sync(0xffffffffu, tc::mbar_wait(smem_u32(&bars.s_full[buf]),
-                                                 (uint32_t)((t >> 1) & 1), abort_flag,
-                                                 a.wait_ns))) {
+      const uint32_t buf = t & 1;
+      const uint32_t t_s = tmem + lane_off + 64u * buf;
+      if (!__all_sync(0xffffffffu, ready) &&
+          !wait(sfull0 + 8u * buf, (uint32_t)(t >> 1) & 1u)) {
         ok = false;
         break;
       }
       tc::tc_fence_after();
       uint32_t s[64];
-      tc::tmem_ld32(tmem + 64u * buf + lane_off, s);
-      tc::tmem_ld32(tmem + 64u * buf + lane_off + 32u, s + 32);
-      if (key0 + kTile > least) {  // the same for all four warps
+      tc::tmem_ld32(t_s, s);
+      tc::tmem_ld32(t_s + 32u, s + 32);
+      // the next tile's S is mostly there already: asked for here, used above
+      ready = t + 1 < tiles &&
+              tc::mbar_try_wait(sfull0 + 8u * (buf ^ 1u), (uint32_t)((t + 1) >> 1) & 1u);
+      tc::tmem_wait_ld();
+      if (is_edge(t)) {
         // V: clear the rows that nobody sees, look at those that only some see
         const int stage = t % kStages;
-        if (!__all_sync(0xffffffffu, tc::mbar_wait(smem_u32(&bars.v_full[stage]),
-                                                   (uint32_t)((t / kStages) & 1), abort_flag,
-                                                   a.wait_ns))) {
+        if (!wait(smem_u32(&bars.full[1][stage]), (uint32_t)((t / kStages) & 1))) {
           ok = false;
           break;
         }
-        const int vrow = row & 63;
-        unsigned char* v = sbase + L::kV + stage * L::kMatrix + vrow * 128;
-        if (key0 + vrow >= most) {
-#pragma unroll
-          for (int h = row >> 6; h < 2 * kHalves; h += 2)  // 64 bytes at a time
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              *reinterpret_cast<uint4*>(v + (h >> 1) * (kTile * 128) + (h & 1) * 64 + i * 16) =
-                  make_uint4(0u, 0u, 0u, 0u);
-          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        } else if (key0 + vrow >= least) {
+        const int vkey = t * kTile + (row & 63);
+        if (vkey >= least_at) {
+          unsigned char* v = sbase + L::kV + stage * L::kMatrix + (row & 63) * 128;
           bool odd = false;
-          for (int h = row >> 6; h < 2 * kHalves; h += 2)
+          for (int h = row >> 6; h < 2 * kHalves; h += 2) {  // 64 bytes each
+            uint4* at = reinterpret_cast<uint4*>(v + (h >> 1) * (kTile * 128) + (h & 1) * 64);
             for (int i = 0; i < 4; ++i) {
-              const uint4 x = *reinterpret_cast<const uint4*>(v + (h >> 1) * (kTile * 128) +
-                                                              (h & 1) * 64 + i * 16);
-              odd = odd || has_nonfinite<T>(x.x) || has_nonfinite<T>(x.y) ||
-                    has_nonfinite<T>(x.z) || has_nonfinite<T>(x.w);
+              if (vkey >= most_at) {
+                at[i] = make_uint4(0u, 0u, 0u, 0u);
+              } else {
+                const uint4 x = at[i];
+                odd = odd || has_nonfinite<T>(x.x) || has_nonfinite<T>(x.y) ||
+                      has_nonfinite<T>(x.z) || has_nonfinite<T>(x.w);
+              }
             }
+          }
           if (odd) s_odd = 1;
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         }
         __syncwarp();
-      }
-      tc::tmem_wait_ld();
-      const bool masked = __any_sync(0xffffffffu, key0 + kTile > lim);
-      if (masked) {
-        const int n = (int)(lim - key0 < 0 ? 0 : (lim - key0 < kTile ? lim - key0 : kTile));
+        const int seen = lim_at - t * kTile;
 #pragma unroll
         for (int i = 0; i < kTile; ++i)
-          if (i >= n) s[i] = __float_as_uint(-INFINITY);
+          if (i >= seen) s[i] = __float_as_uint(-INFINITY);
       }
       float mx[8];
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         const float* f = reinterpret_cast<const float*>(s) + 8 * j;
         mx[j] = max3_nan(max3_nan(f[0], f[1], f[2]), max3_nan(f[3], f[4], f[5]),
-                         max3_nan(f[6], f[7], f[7]));
+                         max_nan(f[6], f[7]));
       }
-      const float mloc = max3_nan(max3_nan(mx[0], mx[1], mx[2]), max3_nan(mx[3], mx[4], mx[5]),
-                                  max3_nan(mx[6], mx[7], mx[7]));
-      // also true where either is NaN or both are -inf (nothing to rescale then)
-      const bool grow = !((mloc - m_ref) * c <= 8.f);
-      const bool rescale = grow && m_ref != -INFINITY;
-      if (__any_sync(0xffffffffu, rescale)) {
-        // O must hold the products of all tiles before this one
-        if (!__all_sync(0xffffffffu, tc::mbar_wait(smem_u32(&bars.pv_done),
-                                                   (uint32_t)((t - 1) & 1), abort_flag,
-                                                   a.wait_ns))) {
-          ok = false;
-          break;
-        }
-        tc::tc_fence_after();
-        const float f = rescale ? fast_exp2((m_ref - mloc) * c) : 1.f;
-        l0 *= f;
-        l1 *= f;
+      const float m = max3_nan(max3_nan(mx[0], mx[1], mx[2]), max3_nan(mx[3], mx[4], mx[5]),
+                               max_nan(mx[6], mx[7]));
+      // also true where m or m_ref is NaN; a tile of which the row sees nothing
+      // changes nothing (a NaN in the sum stays)
+      const bool grow = !((m - m_ref) * c <= 8.f) && m != -INFINITY;
+      if (__any_sync(0xffffffffu, grow)) {
+        const bool rescale = grow && m_ref != -INFINITY;
+        if (__any_sync(0xffffffffu, rescale)) {
+          // O must hold the products of all tiles before this one
+          if (!wait(smem_u32(&bars.s_free[(t - 1) & 1]), (uint32_t)(((t - 1) >> 1) & 1))) {
+            ok = false;
+            break;
+          }
+          tc::tc_fence_after();
+          const float f = rescale ? fast_exp2((m_ref - m) * c) : 1.f;
+          sum = fma_pair(sum, pack_pair(f, f), pack_pair(0.f, 0.f));
+#pragma unroll 1
+          for (int h = 0; h < D / 16; ++h) {
+            uint32_t r[16];
+            tc::tmem_ld16(t_o + lane_off + 16u * h, r);
+            tc::tmem_wait_ld();
 #pragma unroll
-        for (int h = 0; h < D / 32; ++h) {
-          uint32_t r[32];
-          tc::tmem_ld32(t_o + lane_off + 32u * h, r);
-          tc::tmem_wait_ld();
-#pragma unroll
-          for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(__uint_as_float(r[i]) * f);
-          tc::tmem_st32(t_o + lane_off + 32u * h, r);
+            for (int i = 0; i < 16; ++i) r[i] = __float_as_uint(__uint_as_float(r[i]) * f);
+            tc::tmem_st16(t_o + lane_off + 16u * h, r);
+          }
         }
+        if (grow) m_ref = m;
       }
-      if (grow) m_ref = mloc;
-      // a row that has seen nothing keeps a finite base: its masked scores give 0
+      // a row that has seen nothing keeps a finite base: its masked scores give
+      // 0, or 2^-126 where the polynomial is taken
       const float mc = m_ref == -INFINITY ? 0.f : m_ref * c;
+      const float_pair minus = pack_pair(-mc, -mc);
+      float_pair part[2] = {sum, pack_pair(0.f, 0.f)};
       uint32_t pk[32];
 #pragma unroll
       for (int i = 0; i < 32; ++i) {
-        float xa, xb, ea, eb;
-        fma_pair(xa, xb, __uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1]), c, -mc);
-        if (((kPolyPairs >> (i & 7)) & 1u) && !masked) {
-          exp2_poly_pair(ea, eb, xa, xb);
+        const float_pair x = fma_pair(
+            pack_pair(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])), c2, minus);
+        float ea, eb;
+        if ((kPolyPairs >> (i & 7)) & 1u) {
+          poly(ea, eb, x);
         } else {
-          ea = fast_exp2(xa);
-          eb = fast_exp2(xb);
+          unpack_pair(ea, eb, x);
+          ea = fast_exp2(ea);
+          eb = fast_exp2(eb);
         }
-        add_pair(l0, l1, ea, eb);
+        part[i & 1] = add_pair(part[i & 1], pack_pair(ea, eb));
         pk[i] = ElemOps<T>::pack2(ea, eb);
-        if (i == 15 || i == 31) {
-          const int part = i >> 4;
-          tc::tmem_st16(tmem + 64u * buf + lane_off + 16u * part, pk + 16 * part);
-          tc::tmem_wait_st();
-          tc::tc_fence_before();
-          tc::mbar_arrive(smem_u32(&bars.p_full[buf][part]));
-        }
       }
+      sum = add_pair(part[0], part[1]);
+      tc::tmem_st32(t_s, pk);
+      tc::tmem_wait_st();
+      tc::tc_fence_before();
+      tc::mbar_arrive(pfull0 + 8u * buf);
     }
     if (ok && tiles > 0)
       ok = __all_sync(0xffffffffu,
                       tc::mbar_wait(smem_u32(&bars.o_full), 0, abort_flag, a.wait_ns));
     tc::tc_fence_after();
     const bool have = ok && tiles > 0;
-    const float l = have ? l0 + l1 : 0.f;
+    float l0, l1;
+    unpack_pair(l0, l1, sum);
+    const float l = have && m_ref != -INFINITY ? l0 + l1 : 0.f;
     s_m[row] = m_ref * c;
     s_l[row] = l;
     const float inv = runs > 1 ? 1.f : (l == 0.f ? 0.f : 1.f / l);
@@ -434,17 +523,19 @@ __global__ void __launch_bounds__(kThreads, 2)
   }
 
   tc::tc_fence_before();
-  __syncthreads();
-  if (warp == 1) {
+  sync_softmax();
+  if (warp == 4) {
+    // every MMA must have ended before the columns go back
+    for (int i = 0; i < 2; ++i) tc::mbar_wait_drain(smem_u32(&bars.drain[i]), 0, kDrainNs);
     tc::tc_fence_after();
     tc::tmem_dealloc(tmem, kTmemCols);
   }
-  if (tid == 0 && s_abort) raise_status(a.t.status, VGGT_STATUS_TIMEOUT);
+  if (stid == 0 && s_abort) raise_status(a.t.status, VGGT_STATUS_TIMEOUT);
   float* mine = p.partial + (item * p.splits + split) * (int64_t)(kRows * (D + 2));
   if (s_odd) {
     // a value that only some rows see is not finite: zero times it is not zero
-    float* rowbuf = reinterpret_cast<float*>(sbase) + warp * D;  // the rings are free
-    for (int r = warp; r < rows; r += kThreads / 32) {
+    float* rowbuf = reinterpret_cast<float*>(sbase) + (warp - 4) * D;  // the rings are free
+    for (int r = warp - 4; r < rows; r += 4) {
       slow_row<T, D>(a, rt, r, head, p.scale_log2, tile0 * kTile, (tile0 + tiles) * kTile,
                      limit_of(r), rowbuf, &s_m[r], &s_l[r]);
       __syncwarp();
@@ -460,64 +551,84 @@ __global__ void __launch_bounds__(kThreads, 2)
       }
       __syncwarp();
     }
-    __syncthreads();
+    sync_softmax();
   }
   if (runs > 1) {
-    if (tid < rows) {
-      mine[kRows * D + tid] = s_m[tid];
-      mine[kRows * (D + 1) + tid] = s_l[tid];
+    if (stid < rows) {
+      mine[kRows * D + stid] = s_m[stid];
+      mine[kRows * (D + 1) + stid] = s_l[stid];
     }
     __threadfence();
-    __syncthreads();
-    if (tid == 0) {
+    sync_softmax();
+    if (stid == 0) {
       s_last = atomicAdd(p.counters + item, 1) == (int)runs - 1;
       if (s_last) p.counters[item] = 0;
     }
-    __syncthreads();
+    sync_softmax();
     if (!s_last) return;
     __threadfence();
     // the CTA that finishes last joins the runs, in their order
     const float* from = p.partial + item * p.splits * (int64_t)(kRows * (D + 2));
     float* wgt = reinterpret_cast<float*>(sbase);  // [runs][128], at most 64 runs
-    if (tid < rows) {
+    if (stid < rows) {
       float mx = -INFINITY, l = 0.f;
+#pragma unroll 8
       for (int64_t s = 0; s < runs; ++s)
-        mx = fmaxf(mx, __ldcg(from + s * kRows * (D + 2) + kRows * D + tid));
+        mx = fmaxf(mx, __ldcg(from + s * kRows * (D + 2) + kRows * D + stid));
       const float b = mx == -INFINITY ? 0.f : mx;
+#pragma unroll 8
       for (int64_t s = 0; s < runs; ++s) {
-        const float* ml = from + s * kRows * (D + 2) + kRows * D + tid;
+        const float* ml = from + s * kRows * (D + 2) + kRows * D + stid;
         const float f = fast_exp2(__ldcg(ml) - b);
-        wgt[s * kRows + tid] = f;
+        wgt[s * kRows + stid] = f;
         l += __ldcg(ml + kRows) * f;
       }
-      s_m[tid] = mx;
-      s_l[tid] = l;
+      s_m[stid] = mx;
+      s_l[stid] = l;
     }
-    __syncthreads();
-    for (int i = tid; i < rows * (D / 4); i += kThreads) {
-      const int r = i / (D / 4), d = (i % (D / 4)) * 4;
-      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
+    sync_softmax();
+    // 8 vectors per thread and run in flight: one at a time took 18 us
+    constexpr int kBatch = 8;
+    for (int i0 = stid; i0 < rows * (D / 4); i0 += kBatch * kRows) {
+      float4 acc[kBatch];
+#pragma unroll
+      for (int j = 0; j < kBatch; ++j) acc[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 2
       for (int s = 0; s < (int)runs; ++s) {
-        const float f = wgt[s * kRows + r];
-        const float4 v = __ldcg(reinterpret_cast<const float4*>(from + (int64_t)s * kRows * (D + 2)) + i);
-        acc.x = fmaf(f, v.x, acc.x);
-        acc.y = fmaf(f, v.y, acc.y);
-        acc.z = fmaf(f, v.z, acc.z);
-        acc.w = fmaf(f, v.w, acc.w);
+        const float4* src = reinterpret_cast<const float4*>(from + (int64_t)s * kRows * (D + 2));
+        float4 v[kBatch];
+#pragma unroll
+        for (int j = 0; j < kBatch; ++j) {
+          const int i = i0 + j * kRows;
+          v[j] = i < rows * (D / 4) ? __ldcg(src + i) : make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+#pragma unroll
+        for (int j = 0; j < kBatch; ++j) {
+          const float f = wgt[s * kRows + (i0 + j * kRows) / (D / 4) % kRows];
+          acc[j].x = fmaf(f, v[j].x, acc[j].x);
+          acc[j].y = fmaf(f, v[j].y, acc[j].y);
+          acc[j].z = fmaf(f, v[j].z, acc[j].z);
+          acc[j].w = fmaf(f, v[j].w, acc[j].w);
+        }
       }
-      const float l = s_l[r], inv = l == 0.f ? 0.f : 1.f / l;
-      const int q = rt.row0 + r;
-      T* dst = static_cast<T*>(a.out) + (rt.first + q / a.group) * a.o_token +
-               ((int64_t)head * a.group + q % a.group) * a.o_head + d;
-      *reinterpret_cast<uint2*>(dst) = make_uint2(ElemOps<T>::pack2(acc.x * inv, acc.y * inv),
-                                                  ElemOps<T>::pack2(acc.z * inv, acc.w * inv));
+#pragma unroll
+      for (int j = 0; j < kBatch; ++j) {
+        const int i = i0 + j * kRows, r = i / (D / 4), d = (i % (D / 4)) * 4;
+        if (r >= rows) break;
+        const float l = s_l[r], inv = l == 0.f ? 0.f : 1.f / l;
+        const int q = rt.row0 + r;
+        T* dst = static_cast<T*>(a.out) + (rt.first + q / a.group) * a.o_token +
+                 ((int64_t)head * a.group + q % a.group) * a.o_head + d;
+        *reinterpret_cast<uint2*>(dst) =
+            make_uint2(ElemOps<T>::pack2(acc[j].x * inv, acc[j].y * inv),
+                       ElemOps<T>::pack2(acc[j].z * inv, acc[j].w * inv));
+      }
     }
   }
-  if (a.lse != nullptr && tid < rows) {
-    const int q = rt.row0 + tid;
+  if (a.lse != nullptr && stid < rows) {
+    const int q = rt.row0 + stid;
     a.lse[(rt.first + q / a.group) * (p.heads * a.group) + (int64_t)head * a.group + q % a.group] =
-        s_l[tid] == 0.f ? -INFINITY : (s_m[tid] + log2f(s_l[tid])) * 0.6931471805599453f;
+        s_l[stid] == 0.f ? -INFINITY : (s_m[stid] + log2f(s_l[stid])) * 0.6931471805599453f;
   }
 }
 
@@ -526,6 +637,10 @@ cudaError_t launch_tc05(const TcParams& p, const CUtensorMap& mk, const CUtensor
                         cudaStream_t st) {
   auto kernel = paged_tc05_kernel<T, D>;
   const size_t smem = Smem<D>::kEnd + 1024;
+  // with another register count at launch the softmax's setmaxnreg would wait for ever
+  cudaFuncAttributes fa;
+  if (const cudaError_t r = cudaFuncGetAttributes(&fa, kernel); r != cudaSuccess) return r;
+  if (fa.numRegs != kLaunchRegs) return cudaErrorInvalidConfiguration;
   const cudaError_t e =
       cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
   if (e != cudaSuccess) return e;
@@ -542,13 +657,16 @@ PagedPlan paged_tc05_plan(int64_t total, int64_t seqs, int kv_heads, int group, 
   plan.tiles = most_tiles(total, seqs, group, kRows);
   const int64_t items = plan.tiles * kv_heads, key_tiles = (max_len + kTile - 1) / kTile;
   // Runs per row tile: the number that ends the last wave of 2 CTAs per SM
-  // soonest, a CTA's start and end counted as six key tiles.
+  // soonest.  In units of a key tile (0.7 us): a CTA's start and end cost ten,
+  // joining the runs of a tile fourteen.  1 frame over 31 cached ones (176
+  // items): 1 run 536 us, 3 runs 387, 5 runs 375, 10 runs 422; 4 prompts
+  // (2,024 items): 1 run 1,292 us, 2 runs 1,546.
   plan.splits = 1;
   int64_t best = -1;
   const int64_t slots = 2 * 148;
-  for (int64_t s = 1; s <= 64 && (s == 1 || items <= kMaxCounters) && s * 4 <= key_tiles + 4; ++s) {
+  for (int64_t s = 1; s <= 64 && (s == 1 || (items <= kMaxCounters && s <= key_tiles)); ++s) {
     const int64_t waves = (items * s + slots - 1) / slots;
-    const int64_t cost = waves * ((key_tiles + s - 1) / s + 6);
+    const int64_t cost = waves * ((key_tiles + s - 1) / s + 10) + (s > 1 ? 14 : 0);
     if (best < 0 || cost < best) {
       best = cost;
       plan.splits = s;
@@ -584,3 +702,4 @@ cudaError_t launch_paged_tc05(const PagedAttnArgs& a, const PagedPlan& plan, cud
 }
 
 }  // namespace vggt
+
