@@ -168,6 +168,9 @@ struct EvictArgs {
   int32_t *new_ids, *new_lengths;
 };
 
+cudaError_t launch_paged_weigh_rows(const WeighArgs& a, cudaStream_t st);
+cudaError_t launch_paged_weigh_tc05(const WeighArgs& a, cudaStream_t st);
+
 // Counters of unfinished items at the front of a workspace: zero before the
 // first call and after every call, in a place that no call uses otherwise.
 constexpr int64_t kMaxCounters = 4096;

@@ -201,8 +201,7 @@ __global__ void __launch_bounds__(kThreads, 2)
 #pragma unroll
         for (int kv = 0; kv < 2; ++kv) {
           if (t >= kStages)
-            ok = ok && __all_sync(0xffffffffu, tc::mbar_wait(empty0 + kv * kToV + 8u * stage, phase,
-                                                             abort_flag, a.wait_ns));
+            ok = ok && tc::warp_wait(empty0 + kv * kToV + 8u * stage, phase, abort_flag, a.wait_ns);
           if (ok && tc::elect_one()) {
             const uint32_t bar = full0 + kv * kToV + 8u * stage;
             tc::mbar_expect_tx(bar, (uint32_t)(live * kBox) * D * 2u);
@@ -245,7 +244,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     // registers.
     const uint32_t fmt = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
     auto wait = [&](uint32_t bar, uint32_t parity) {
-      return __all_sync(0xffffffffu, tc::mbar_wait(bar, parity, abort_flag, a.wait_ns));
+      return tc::warp_wait(bar, parity, abort_flag, a.wait_ns);
     };
     const uint32_t kfull0 = smem_u32(&bars.full[0][0]), kempty0 = smem_u32(&bars.empty[0][0]);
     const uint32_t vfull0 = smem_u32(&bars.full[1][0]), vempty0 = smem_u32(&bars.empty[1][0]);
@@ -354,7 +353,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     const int lim_at = within(lim), least_at = within(least), most_at = within(most);
     const uint32_t sfull0 = smem_u32(&bars.s_full[0]), pfull0 = smem_u32(&bars.p_full[0]);
     auto wait = [&](uint32_t bar, uint32_t parity) {
-      return __all_sync(0xffffffffu, tc::mbar_wait(bar, parity, abort_flag, a.wait_ns));
+      return tc::warp_wait(bar, parity, abort_flag, a.wait_ns);
     };
     // whether some row of the CTA does not see all of tile t (for all warps alike)
     auto is_edge = [&](int t) { return (t + 1) * kTile > least_at; };
@@ -362,12 +361,11 @@ __global__ void __launch_bounds__(kThreads, 2)
     float_pair sum = pack_pair(0.f, 0.f);
     const float_pair c2 = pack_pair(c, c);
     const Exp2Poly poly;
-    bool ok = true, ready = false;
+    bool ok = true;
     for (int t = 0; t < tiles; ++t) {
       const uint32_t buf = t & 1;
       const uint32_t t_s = tmem + lane_off + 64u * buf;
-      if (!__all_sync(0xffffffffu, ready) &&
-          !wait(sfull0 + 8u * buf, (uint32_t)(t >> 1) & 1u)) {
+      if (!wait(sfull0 + 8u * buf, (uint32_t)(t >> 1) & 1u)) {
         ok = false;
         break;
       }
@@ -375,9 +373,6 @@ __global__ void __launch_bounds__(kThreads, 2)
       uint32_t s[64];
       tc::tmem_ld32(t_s, s);
       tc::tmem_ld32(t_s + 32u, s + 32);
-      // the next tile's S is mostly there already: asked for here, used above
-      ready = t + 1 < tiles &&
-              tc::mbar_try_wait(sfull0 + 8u * (buf ^ 1u), (uint32_t)((t + 1) >> 1) & 1u);
       tc::tmem_wait_ld();
       if (is_edge(t)) {
         // V: clear the rows that nobody sees, look at those that only some see
@@ -474,8 +469,7 @@ __global__ void __launch_bounds__(kThreads, 2)
       tc::mbar_arrive(pfull0 + 8u * buf);
     }
     if (ok && tiles > 0)
-      ok = __all_sync(0xffffffffu,
-                      tc::mbar_wait(smem_u32(&bars.o_full), 0, abort_flag, a.wait_ns));
+      ok = tc::warp_wait(smem_u32(&bars.o_full), 0, abort_flag, a.wait_ns);
     tc::tc_fence_after();
     const bool have = ok && tiles > 0;
     float l0, l1;

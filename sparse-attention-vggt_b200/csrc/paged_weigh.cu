@@ -163,6 +163,7 @@ __global__ void __launch_bounds__(kThreads, 2)
               l = a.lse[(first + row / a.group) * ((int64_t)a.pool.kv_heads * a.group) +
                         (int64_t)head * a.group + row % a.group] *
                   1.4426950408889634f;
+              if (l == -INFINITY) l = INFINITY;  // a row without keys gives nothing
               n = a.causal ? len - n_new + row / a.group + 1 : len;
             }
             lse2[tid] = l;
@@ -303,5 +304,9 @@ extern "C" int vggt_paged_weights(const void* q, int dtype, int64_t total, int64
   a.max_new = max_new;
   a.max_len = max_len;
   a.wait_ns = api_wait_ns();
-  return api_cuda(launch_paged_weigh_rows(a, static_cast<cudaStream_t>(stream)));
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  // up to 64 rows per sequence and key head (and groups wider than a tile) go
+  // to the warp-level kernel
+  const bool rows = max_new * group <= 64 || group > 128 || total == 0;
+  return api_cuda(rows ? launch_paged_weigh_rows(a, st) : launch_paged_weigh_tc05(a, st));
 }

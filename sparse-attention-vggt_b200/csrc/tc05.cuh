@@ -71,6 +71,23 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatil
 #endif
 }
 
+// The bounded wait of a full warp: true on all lanes or on none.  The probe
+// that mostly succeeds is straight-line code with one uniform branch.
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag,
+                                          uint64_t limit_ns) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "vote.sync.all.pred q, p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  if (ok) return true;
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, limit_ns));
+}
+
 // true on exactly one lane of a fully active warp
 __device__ __forceinline__ bool elect_one() {
   uint32_t pred = 0;
