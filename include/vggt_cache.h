@@ -44,6 +44,9 @@ extern "C" {
 #define VGGT_STATUS_BAD_PAGE 16   /* a needed page number is outside [0, n_pages) */
 #define VGGT_STATUS_BAD_LENGTH 32 /* a length or a start was out of range and clamped */
 
+/* front of the workspace of vggt_paged_attention that has to be zero */
+#define VGGT_PAGED_WORKSPACE_ZERO_BYTES 16384
+
 /* which elements of a head form the pairs that are rotated */
 #define VGGT_ROTARY_HALF 0        /* element i with element i + pairs */
 #define VGGT_ROTARY_INTERLEAVED 1 /* element 2i with element 2i + 1 */
@@ -95,9 +98,10 @@ int vggt_paged_append(const void* k, const void* v, int dtype, int64_t total,
  * max_new and max_len are the most new tokens of a sequence and the greatest
  * length as the caller expects them; they choose the kernel and how the work
  * is cut, the result is right for any lengths.  The workspace holds at least
- * vggt_paged_attention_workspace_size bytes (same arguments), is zeroed before
- * its first use (a call leaves it ready for the next one, of any sizes) and
- * serves one stream at a time.
+ * vggt_paged_attention_workspace_size bytes (same arguments), its first
+ * VGGT_PAGED_WORKSPACE_ZERO_BYTES are zeroed before its first use (a call
+ * leaves it ready for the next one, of any sizes), and it serves one stream at
+ * a time.
  */
 size_t vggt_paged_attention_workspace_size(int64_t total, int64_t seqs, int kv_heads, int group,
                                            int dim, int64_t max_new, int64_t max_len);

@@ -173,7 +173,7 @@ cudaError_t launch_paged_weigh_tc05(const WeighArgs& a, cudaStream_t st);
 
 // Counters of unfinished items at the front of a workspace: zero before the
 // first call and after every call, in a place that no call uses otherwise.
-constexpr int64_t kMaxCounters = 4096;
+constexpr int64_t kMaxCounters = VGGT_PAGED_WORKSPACE_ZERO_BYTES / 4;
 
 // How a launch cuts its work.
 struct PagedPlan {

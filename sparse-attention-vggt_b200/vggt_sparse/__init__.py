@@ -13,13 +13,14 @@ from .block_attention import block_attention, check_status  # noqa: F401
 from .configs import CONFIGS, LayerConfig  # noqa: F401
 from .estimator import BlockMasks, block_mask_estimate, block_select  # noqa: F401
 from .frame_topk import compute_qk_topk_indices_fused  # noqa: F401
-from .kv_cache import (check_cache_status, paged_append, paged_attention,  # noqa: F401
+from .kv_cache import (PagedKVCache, check_cache_status, paged_append, paged_attention,  # noqa: F401
                        paged_attention_workspace_size, paged_evict, paged_weights, rotary,
                        rotary_frequencies)
 from .layer import SparseGlobalLayer, topk_budget  # noqa: F401
 from .layout import LayerShape, split_keys, token_layout  # noqa: F401
 from .pipeline import HostPipeline  # noqa: F401
 from .qkv import QkvOut, project_qkv, rope_tables  # noqa: F401
+from .streaming import StreamingGlobalLayer  # noqa: F401
 from .token_attention import token_sparse_attention  # noqa: F401
 from .profile import (dense_heads_from_decisions, dense_heads_from_profile,  # noqa: F401
                       head_modes_from_profile, split_heads)

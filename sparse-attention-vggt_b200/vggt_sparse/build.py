@@ -18,6 +18,7 @@ CSRC = os.path.join(ROOT, "csrc")
 INCLUDE = os.path.join(REPO, "include")
 BUILD_DIR = os.path.join(ROOT, "_build")
 LIB_PATH = os.path.join(PKG_DIR, "libvggt_sparse.so")
+BINDING_PATH = os.path.join(PKG_DIR, "_cache_binding.so")  # Python module over the library
 
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = ["-std=c++17", "-O3", "-lineinfo", "-Xcompiler", "-fPIC", "--expt-relaxed-constexpr",
@@ -56,6 +57,29 @@ def _compile(nvcc, src, obj, extra):
     return res.stderr
 
 
+def _build_binding(force):
+    """The Python module of csrc/cache_binding.cpp, linked against the library next to it."""
+    src = os.path.join(CSRC, "cache_binding.cpp")
+    if not force and not _stale(BINDING_PATH, [src, *_headers()]):
+        return
+    import sysconfig
+
+    import torch
+    root = os.path.dirname(torch.__file__)
+    cuda = os.path.dirname(os.path.dirname(os.path.realpath(_nvcc())))
+    include = [INCLUDE, os.path.join(root, "include"),
+               os.path.join(root, "include", "torch", "csrc", "api", "include"),
+               sysconfig.get_paths()["include"], os.path.join(cuda, "include")]
+    cmd = [os.environ.get("CXX") or "g++", "-std=c++17", "-O2", "-fPIC", "-shared", "-w",
+           "-D_GLIBCXX_USE_CXX11_ABI=%d" % torch._C._GLIBCXX_USE_CXX11_ABI,
+           *["-I" + d for d in include], src, "-o", BINDING_PATH, "-L" + PKG_DIR,
+           "-l:libvggt_sparse.so", "-Wl,-rpath,$ORIGIN", "-L" + os.path.join(root, "lib"), "-lc10",
+           "-lc10_cuda", "-ltorch_cpu", "-ltorch_python"]
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        raise RuntimeError("building the Python module failed:\n%s\n%s" % (res.stdout, res.stderr))
+
+
 def build(force=False, verbose=False, ptxas_info=False):
     """Compile every CUDA source for sm_100a and link the shared library."""
     nvcc = _nvcc()
@@ -80,6 +104,7 @@ def build(force=False, verbose=False, ptxas_info=False):
         res = subprocess.run(cmd, capture_output=True, text=True)
         if res.returncode != 0:
             raise RuntimeError("link failed:\n%s\n%s" % (res.stdout, res.stderr))
+    _build_binding(force)
     if verbose:
         for log in logs:
             sys.stderr.write(log)

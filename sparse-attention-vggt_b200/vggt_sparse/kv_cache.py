@@ -28,15 +28,28 @@ Page numbers, lengths and starts are checked on the device; ``status`` (an
 int32 tensor) collects VGGT_STATUS_* bits, see ``check_cache_status``.
 """
 import math
+import os
 
 import torch
 
 from . import _lib
-from .ops import _ptr, _require_cuda, _stream, dtype_code
+from .build import BINDING_PATH
 
-_LAYOUTS = {"half": _lib.ROTARY_HALF, "interleaved": _lib.ROTARY_INTERLEAVED}
-_ROTARY_DTYPES = {torch.bfloat16: _lib.DTYPE_BF16, torch.float16: _lib.DTYPE_FP16,
-                  torch.float32: _lib.DTYPE_FP32}
+_module = None
+
+
+def _binding():
+    """The compiled module of csrc/cache_binding.cpp, which checks arguments
+    and calls the C ABI; there is no fallback."""
+    global _module
+    if _module is None:
+        if not os.path.exists(BINDING_PATH):
+            raise _lib.ExtensionMissing(
+                "%s not found: build it with `python -m vggt_sparse.build`" % BINDING_PATH)
+        _lib.load()
+        from . import _cache_binding
+        _module = _cache_binding
+    return _module
 
 
 def rotary_frequencies(rotary_dim, *, base=10000.0, axes=1, scaling=None, factor=1.0,
@@ -79,34 +92,6 @@ def rotary_frequencies(rotary_dim, *, base=10000.0, axes=1, scaling=None, factor
     return torch.tensor(f, dtype=torch.float64, device=device), lengthen
 
 
-def _ints(name, t, shape):
-    if t.dtype != torch.int32 or t.shape != shape or not t.is_contiguous():
-        raise ValueError("%s must be a contiguous int32 tensor of shape %s" % (name, tuple(shape)))
-    return t.data_ptr()
-
-
-def _status(status):
-    if status is None:
-        return None
-    if status.dtype != torch.int32 or status.numel() < 1:
-        raise ValueError("status must be an int32 tensor with at least one element")
-    return status.data_ptr()
-
-
-def _positions(positions, tokens, frequencies, layout):
-    """(pointer, axes) of positions [tokens] or [tokens, axes]."""
-    axes = 1 if positions.dim() == 1 else positions.shape[-1]
-    if positions.dim() > 2 or positions.shape[0] != tokens or positions.dtype != torch.int32 \
-            or not positions.is_contiguous():
-        raise ValueError("positions must be contiguous int32 [tokens] or [tokens, axes]")
-    if frequencies is None or frequencies.dtype != torch.float64 or frequencies.dim() != 1 \
-            or not frequencies.is_contiguous():
-        raise ValueError("frequencies must be a contiguous float64 vector (rotary_frequencies)")
-    if layout not in _LAYOUTS:
-        raise ValueError("layout must be 'half' or 'interleaved'")
-    return positions.data_ptr(), axes
-
-
 def rotary(x, positions, frequencies, *, layout="half", lengthen=1.0, inverse=False, out=None):
     """x [tokens, heads, dim] (bf16, fp16 or fp32; last dimension contiguous)
     with the first 2 * axes * len(frequencies) elements of each head turned by
@@ -116,47 +101,7 @@ def rotary(x, positions, frequencies, *, layout="half", lengthen=1.0, inverse=Fa
     "interleaved" 2i with 2i + 1.  ``inverse`` turns the other way, which is
     the gradient of ``rotary`` with respect to x.  ``out`` may be x itself.
     """
-    if x.dim() != 3 or x.dtype not in _ROTARY_DTYPES or x.stride(2) != 1:
-        raise ValueError("x must be [tokens, heads, dim], BF16, FP16 or FP32, last dimension "
-                         "contiguous")
-    t, h, d = x.shape
-    pos, axes = _positions(positions, t, frequencies, layout)
-    if out is None:
-        out = torch.empty((t, h, d), dtype=x.dtype, device=x.device)
-    elif out.shape != x.shape or out.dtype != x.dtype or out.stride(2) != 1:
-        raise ValueError("out must have x's shape and dtype, last dimension contiguous")
-    _require_cuda(x, positions, frequencies, out)
-    _lib.check(_lib.load().vggt_rotary(
-        x.data_ptr(), _ROTARY_DTYPES[x.dtype], t, h, d, x.stride(0), x.stride(1), pos, axes,
-        frequencies.data_ptr(), frequencies.shape[0], _LAYOUTS[layout], lengthen, int(inverse),
-        out.data_ptr(), out.stride(0), out.stride(1), _stream(x.device)))
-    return out
-
-
-def _pool_args(k_pages, v_pages, table, seqs):
-    """The pool arguments of the C ABI (sizes, strides, table)."""
-    if k_pages.dim() != 4 or k_pages.stride(3) != 1:
-        raise ValueError("pools must be [pages, kv_heads, page, dim], last dimension contiguous")
-    if v_pages is not None and (v_pages.shape != k_pages.shape or v_pages.dtype != k_pages.dtype
-                                or v_pages.stride() != k_pages.stride()):
-        raise ValueError("k_pages and v_pages must have the same shape, strides and dtype")
-    if table.dim() != 2 or table.dtype != torch.int32 or not table.is_contiguous() \
-            or (seqs is not None and table.shape[0] != seqs):
-        raise ValueError("table must be contiguous int32 [seqs, width]")
-    n, h, p, d = k_pages.shape
-    s = k_pages.stride()
-    return (n, h, p, d, s[0], s[1], s[2], table.data_ptr(), table.shape[1], table.shape[0])
-
-
-def _rows_of(name, t, heads, k_pages):
-    """t [tokens, heads, dim] with strides that the kernels take (else a copy)."""
-    if t.dim() != 3 or t.shape[2] != k_pages.shape[3] or t.dtype != k_pages.dtype \
-            or (heads is not None and t.shape[1] != heads):
-        raise ValueError("%s must be [tokens, %s, %d] %s" % (
-            name, "heads" if heads is None else heads, k_pages.shape[3], k_pages.dtype))
-    if t.stride(2) != 1 or t.stride(0) % 8 or t.stride(1) % 8 or t.data_ptr() % 16:
-        t = t.contiguous()
-    return t
+    return _binding().rotary(x, positions, frequencies, layout, lengthen, inverse, out)
 
 
 def paged_append(k, v, k_pages, v_pages, table, before, starts, *, positions=None,
@@ -171,66 +116,13 @@ def paged_append(k, v, k_pages, v_pages, table, before, starts, *, positions=Non
     head; a weight of +inf keeps a token from eviction.  Tokens past a
     sequence's last slot are dropped (STATUS_BAD_LENGTH).
     """
-    code = dtype_code(k_pages.dtype)
-    pool = _pool_args(k_pages, v_pages, table, None)
-    seqs, slots = pool[9], pool[8] * pool[2]
-    k, v = _rows_of("k", k, pool[1], k_pages), _rows_of("v", v, pool[1], k_pages)
-    total = k.shape[0]
-    if v.shape != k.shape:
-        raise ValueError("k and v must have the same shape")
-    pos, axes, freq, pairs = None, 0, None, 0
-    if positions is not None:
-        pos, axes = _positions(positions, total, frequencies, layout)
-        freq, pairs = frequencies.data_ptr(), frequencies.shape[0]
-    if ids is not None:
-        _ints("ids", ids, (seqs, pool[1], slots))
-        if new_ids is None:
-            raise ValueError("ids needs new_ids")
-        _ints("new_ids", new_ids, (total,))
-    if weights is not None:
-        _weights("weights", weights, (seqs, pool[1], slots))
-        if new_weights is not None:
-            _weights("new_weights", new_weights, (total,))
-    if after is None:
-        after = torch.empty_like(before)
-    elif after.data_ptr() == before.data_ptr():
-        raise ValueError("after must not be before")
-    _require_cuda(k, v, k_pages, v_pages, table, before, starts, positions, frequencies, ids,
-                  new_ids, weights, new_weights, after, status)
-    _lib.check(_lib.load().vggt_paged_append(
-        k.data_ptr(), v.data_ptr(), code, total, k.stride(0), k.stride(1), v.stride(0),
-        v.stride(1), k_pages.data_ptr(), v_pages.data_ptr(), *pool,
-        _ints("before", before, (seqs,)), _ints("starts", starts, (seqs + 1,)), pos, axes, freq,
-        pairs, _LAYOUTS.get(layout, 0), lengthen, _ptr(ids), _ptr(new_ids), _ptr(weights),
-        _ptr(new_weights), _ints("after", after, (seqs,)), _status(status), _stream(k.device)))
-    return after
-
-
-def _weights(name, t, shape):
-    if t.dtype != torch.float32 or t.shape != shape or not t.is_contiguous():
-        raise ValueError("%s must be a contiguous float32 tensor of shape %s"
-                         % (name, tuple(shape)))
-
-
-# One zeroed workspace per stream: its calls run one after another, and every
-# call leaves the part that has to be zero at zero.
-_WORKSPACES = {}
-
-
-def _workspace(need, device, stream):
-    if torch.cuda.is_current_stream_capturing():
-        # a graph may be replayed on any stream: it gets a workspace of its own
-        return torch.zeros(need, dtype=torch.uint8, device=device)
-    key = (device.index, stream)
-    ws = _WORKSPACES.get(key)
-    if ws is None or ws.numel() < need:
-        ws = _WORKSPACES[key] = torch.zeros(max(need, 1 << 20), dtype=torch.uint8, device=device)
-    return ws
+    return _binding().append(k, v, k_pages, v_pages, table, before, starts, positions, frequencies,
+                             layout, lengthen, ids, new_ids, weights, new_weights, after, status)
 
 
 def paged_attention_workspace_size(total, seqs, kv_heads, group, dim, max_new, max_len):
-    """Bytes of the workspace of ``paged_attention`` (zero-filled before its
-    first use; one stream at a time)."""
+    """Bytes of the workspace of ``paged_attention``: a uint8 tensor zeroed
+    before its first use, used by one stream at a time."""
     return int(_lib.load().vggt_paged_attention_workspace_size(total, seqs, kv_heads, group, dim,
                                                                max_new, max_len))
 
@@ -251,38 +143,8 @@ def paged_attention(q, k_pages, v_pages, table, lengths, starts, *, max_new, max
     kernel and the split, the result holds for any.  Without ``workspace`` the
     current stream's own is used.
     """
-    code = dtype_code(k_pages.dtype)
-    pool = _pool_args(k_pages, v_pages, table, None)
-    kv_heads, dim, seqs = pool[1], pool[3], pool[9]
-    q = _rows_of("q", q, None, k_pages)
-    total, heads = q.shape[0], q.shape[1]
-    if heads < 1 or heads % kv_heads:
-        raise ValueError("q's heads (%d) must be a multiple of the pools' (%d)" % (heads, kv_heads))
-    if out is None:
-        out = torch.empty((total, heads, dim), dtype=q.dtype, device=q.device)
-    elif out.shape != q.shape or out.dtype != q.dtype or out.stride(2) != 1 \
-            or out.stride(0) % 8 or out.stride(1) % 8 or out.data_ptr() % 16:
-        raise ValueError("out must have q's shape and dtype and 16-byte aligned rows")
-    if lse is None:
-        lse = torch.empty((total, heads), dtype=torch.float32, device=q.device)
-    else:
-        _weights("lse", lse, (total, heads))
-    _require_cuda(q, k_pages, v_pages, table, lengths, starts, out, lse, workspace, status)
-    max_len = pool[8] * pool[2] if max_len is None else max_len
-    lib = _lib.load()
-    need = lib.vggt_paged_attention_workspace_size(total, seqs, kv_heads, heads // kv_heads, dim,
-                                                   max_new, max_len)
-    stream = _stream(q.device)
-    if workspace is None:
-        workspace = _workspace(max(need, 1), q.device, stream)
-    _lib.check(lib.vggt_paged_attention(
-        q.data_ptr(), code, total, q.stride(0), q.stride(1), k_pages.data_ptr(),
-        v_pages.data_ptr(), *pool, _ints("lengths", lengths, (seqs,)),
-        _ints("starts", starts, (seqs + 1,)), heads // kv_heads, int(causal),
-        dim ** -0.5 if scale is None else scale, max_new, max_len, out.data_ptr(), out.stride(0),
-        out.stride(1), lse.data_ptr(), _status(status), workspace.data_ptr(),
-        workspace.numel() * workspace.element_size(), stream))
-    return out, lse
+    return _binding().attention(q, k_pages, v_pages, table, lengths, starts, max_new, max_len,
+                                causal, scale, out, lse, workspace, status)
 
 
 def paged_weights(q, lse, k_pages, table, lengths, starts, weights, *, max_new, max_len=None,
@@ -291,23 +153,8 @@ def paged_weights(q, lse, k_pages, table, lengths, starts, weights, *, max_new, 
     tokens' rows gave each cached key: decay * weights + sum exp(s - lse) over
     the rows and the query heads of the key's head.  q, lse, lengths, starts,
     causal and scale as in ``paged_attention``, whose lse it takes."""
-    code = dtype_code(k_pages.dtype)
-    pool = _pool_args(k_pages, None, table, None)
-    kv_heads, dim, seqs, slots = pool[1], pool[3], pool[9], pool[8] * pool[2]
-    q = _rows_of("q", q, None, k_pages)
-    total, heads = q.shape[0], q.shape[1]
-    if heads < 1 or heads % kv_heads:
-        raise ValueError("q's heads (%d) must be a multiple of the pools' (%d)" % (heads, kv_heads))
-    _weights("lse", lse, (total, heads))
-    _weights("weights", weights, (seqs, kv_heads, slots))
-    _require_cuda(q, lse, k_pages, table, lengths, starts, weights, status)
-    _lib.check(_lib.load().vggt_paged_weights(
-        q.data_ptr(), code, total, q.stride(0), q.stride(1), lse.data_ptr(), k_pages.data_ptr(),
-        *pool, _ints("lengths", lengths, (seqs,)), _ints("starts", starts, (seqs + 1,)),
-        heads // kv_heads, int(causal), dim ** -0.5 if scale is None else scale, decay, max_new,
-        slots if max_len is None else max_len, weights.data_ptr(), _status(status),
-        _stream(q.device)))
-    return weights
+    return _binding().weigh(q, lse, k_pages, table, lengths, starts, weights, max_new, max_len,
+                            causal, scale, decay, status)
 
 
 def paged_evict(weights, ids, k_pages, v_pages, table, lengths, budget, *, max_len=None,
@@ -322,30 +169,9 @@ def paged_evict(weights, ids, k_pages, v_pages, table, lengths, budget, *, max_l
     others fill the holes there in order.  The sequences' pages must not be
     shared with other sequences.
     """
-    code = dtype_code(k_pages.dtype)
-    pool = _pool_args(k_pages, v_pages, table, None)
-    seqs, slots = pool[9], pool[8] * pool[2]
-    shape = (seqs, pool[1], slots)
-    _weights("weights", weights, shape)
-    _ints("ids", ids, shape)
-    if out is None:
-        out = torch.empty_like(weights), torch.empty_like(ids), torch.empty_like(lengths)
-    new_weights, new_ids, new_lengths = out
-    _weights("out[0]", new_weights, shape)
-    _ints("out[1]", new_ids, shape)
-    if recent_from is not None:
-        _ints("recent_from", recent_from, (seqs,))
-    _require_cuda(weights, ids, k_pages, v_pages, table, lengths, recent_from, *out, status)
-    lib = _lib.load()
-    ws = torch.empty(max(1, lib.vggt_paged_evict_workspace_size(seqs, pool[1], slots, budget)),
-                     dtype=torch.uint8, device=weights.device)
-    _lib.check(lib.vggt_paged_evict(
-        weights.data_ptr(), ids.data_ptr(), code, k_pages.data_ptr(), v_pages.data_ptr(), *pool,
-        _ints("lengths", lengths, (seqs,)), budget, _ptr(recent_from),
-        slots if max_len is None else max_len, new_weights.data_ptr(), new_ids.data_ptr(),
-        _ints("out[2]", new_lengths, (seqs,)), _status(status), ws.data_ptr(), ws.numel(),
-        _stream(weights.device)))
-    return new_weights, new_ids, new_lengths
+    new = (None, None, None) if out is None else out
+    return _binding().evict(weights, ids, k_pages, v_pages, table, lengths, budget, max_len,
+                            recent_from, *new, status)
 
 
 _MESSAGES = ((_lib.STATUS_TIMEOUT, "a device pipeline wait timed out"),
@@ -358,3 +184,140 @@ def check_cache_status(status):
     bits = int(status[0].item())
     if bits:
         raise ValueError("paged cache: " + "; ".join(m for b, m in _MESSAGES if bits & b))
+
+
+class PagedKVCache:
+    """Pools, page tables and books of a streaming cache.
+
+    seqs sequences share ``pages`` pages of ``page`` slots; each may hold up to
+    ``max_length`` tokens.  A step appends new tokens, attends from them and,
+    where the cache is bounded, evicts:
+
+        starts = cache.append(k, v, counts, positions=..., frequencies=...)
+        out, lse = cache.attend(q, causal=False)     # also adds to the weights
+        cache.evict(budget, recent=...)
+
+    Lengths are known on the host (eviction leaves min(length, budget)), so
+    pages are given out and taken back without waiting for the device.  All
+    calls belong on one stream; ``check()`` waits and raises what the device
+    found wrong.
+    """
+
+    def __init__(self, seqs, kv_heads, dim, *, pages, max_length, page=64,
+                 dtype=torch.bfloat16, device="cuda"):
+        if seqs < 1 or pages < 1 or max_length < 1:
+            raise ValueError("seqs, pages and max_length must be positive")
+        self.seqs, self.page, self.max_length = seqs, page, max_length
+        self.width = -(-max_length // page)
+        shape = (pages, kv_heads, page, dim)
+        self.k_pages = torch.empty(shape, dtype=dtype, device=device)
+        self.v_pages = torch.empty(shape, dtype=dtype, device=device)
+        self.table = torch.zeros(seqs, self.width, dtype=torch.int32, device=device)
+        slots = (seqs, kv_heads, self.width * page)
+        self.ids = torch.full(slots, -1, dtype=torch.int32, device=device)
+        self.weights = torch.zeros(slots, device=device)
+        self._spare = torch.empty_like(self.weights), torch.empty_like(self.ids)
+        self.length = torch.zeros(seqs, dtype=torch.int32, device=device)
+        self.status = torch.zeros(1, dtype=torch.int32, device=device)
+        self.lengths = [0] * seqs        # the same on the host
+        self.seen = [0] * seqs           # tokens ever appended: the next token's id
+        self._pages = [[] for _ in range(seqs)]
+        self._free = list(range(pages - 1, -1, -1))
+        self._step = None                # (starts, counts) of the last append
+
+    def _ints(self, values):
+        return torch.tensor(values, dtype=torch.int32).to(self.table.device, non_blocking=True)
+
+    def append(self, k, v, counts, *, positions=None, frequencies=None, layout="half",
+               lengthen=1.0, new_weights=None):
+        """Append counts[b] tokens to sequence b (k, v packed in that order).
+        Tokens are numbered as they come (``ids``); ``positions`` default to
+        those numbers where ``frequencies`` are given.  ``new_weights`` of +inf
+        keep tokens from eviction.  Returns starts."""
+        if len(counts) != self.seqs or min(counts) < 0:
+            raise ValueError("counts needs one number, not negative, per sequence")
+        if sum(counts) != k.shape[0]:
+            raise ValueError("counts add up to %d, k has %d tokens" % (sum(counts), k.shape[0]))
+        need = []
+        for b, n in enumerate(counts):
+            if self.lengths[b] + n > self.max_length:
+                raise ValueError("sequence %d would pass max_length %d" % (b, self.max_length))
+            need.append(-(-(self.lengths[b] + n) // self.page) - len(self._pages[b]))
+        if sum(max(0, n) for n in need) > len(self._free):
+            raise ValueError("the pool is out of pages (%d free)" % len(self._free))
+        for b, n in enumerate(need):
+            if n > 0:
+                first = len(self._pages[b])
+                self._pages[b] += [self._free.pop() for _ in range(n)]
+                self.table[b, first:first + n] = self._ints(self._pages[b][first:])
+        starts, ids = [0], []
+        for b, n in enumerate(counts):
+            starts.append(starts[-1] + n)
+            ids += range(self.seen[b], self.seen[b] + n)
+        starts, ids = self._ints(starts), self._ints(ids)
+        if frequencies is not None and positions is None:
+            positions = ids
+        self.length = paged_append(k, v, self.k_pages, self.v_pages, self.table, self.length,
+                                   starts, positions=positions, frequencies=frequencies,
+                                   layout=layout, lengthen=lengthen, ids=self.ids, new_ids=ids,
+                                   weights=self.weights, new_weights=new_weights,
+                                   status=self.status)
+        for b, n in enumerate(counts):
+            self.lengths[b] += n
+            self.seen[b] += n
+        self._step = (starts, max(1, max(counts)))
+        return starts
+
+    def attend(self, q, *, causal=True, scale=None, weigh=True, decay=1.0, out=None):
+        """Attention of the last appended tokens over the cache: (out, lse).
+        With ``weigh`` their probabilities are added to the keys' weights."""
+        if self._step is None:
+            raise ValueError("append comes before attend")
+        starts, most = self._step
+        longest = max(self.lengths)
+        out, lse = paged_attention(q, self.k_pages, self.v_pages, self.table, self.length, starts,
+                                   max_new=most, max_len=longest, causal=causal, scale=scale,
+                                   out=out, status=self.status)
+        if weigh:
+            paged_weights(q, lse, self.k_pages, self.table, self.length, starts, self.weights,
+                          max_new=most, max_len=longest, causal=causal, scale=scale, decay=decay,
+                          status=self.status)
+        return out, lse
+
+    def evict(self, budget, *, recent=0):
+        """Keep at most ``budget`` tokens of every sequence and key head; the
+        ``recent`` last appended ones of a sequence go last.  A sequence that
+        is evicted from can not be attended from again before an append."""
+        if budget < 0:
+            raise ValueError("budget must not be negative")
+        longest = max(self.lengths)
+        if longest <= budget:
+            return
+        newest = self._ints([n - recent for n in self.seen]) if recent > 0 else None
+        new = (*self._spare, torch.empty_like(self.length))
+        paged_evict(self.weights, self.ids, self.k_pages, self.v_pages, self.table, self.length,
+                    budget, max_len=longest, recent_from=newest, out=new, status=self.status)
+        self._spare = self.weights, self.ids
+        self.weights, self.ids, self.length = new
+        self._step = None
+        for b in range(self.seqs):
+            self.lengths[b] = min(self.lengths[b], budget)
+            keep = -(-self.lengths[b] // self.page)
+            self._free += reversed(self._pages[b][keep:])
+            del self._pages[b][keep:]
+
+    def release(self, seq):
+        """Empty a sequence and take its pages back."""
+        self._free += reversed(self._pages[seq])
+        self._pages[seq] = []
+        self.lengths[seq] = self.seen[seq] = 0
+        self.length = self.length.clone()
+        self.length[seq] = 0
+        self.ids[seq] = -1
+        self.weights[seq] = 0
+        self._step = None
+
+    def check(self):
+        """Wait for the device and raise ValueError if an operator found bad
+        pages, lengths or starts, or timed out."""
+        check_cache_status(self.status)
