@@ -106,6 +106,8 @@ uint64_t api_wait_ns() {
   return ns > 0 ? ns : 1000000000ull;
 }
 
+int api_wait_selftest() { return g_wait_selftest.load(); }
+
 }  // namespace vggt
 
 extern "C" {

@@ -13,6 +13,8 @@ int api_cuda(cudaError_t e);
 int api_device_sms();
 // limit of every bounded wait, vggt_sparse_set_wait_limit_ns
 uint64_t api_wait_ns();
+// vggt_sparse_set_wait_selftest
+int api_wait_selftest();
 
 inline bool units_zero(int64_t a, int64_t b) { return a == 0 || b == 0; }
 

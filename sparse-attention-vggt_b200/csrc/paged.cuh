@@ -140,6 +140,9 @@ struct PagedAttnArgs {
   int64_t max_new, max_len;  // what the caller expects; only the choice of variant depends on them
   void* workspace;  // counters (zero before and after), then partial results
   uint64_t wait_ns;
+  // self-test of the failure detection: one warp waits on a barrier that
+  // nothing completes and takes the CTA through the abort path
+  int wait_selftest;
 };
 
 struct WeighArgs {
@@ -154,6 +157,7 @@ struct WeighArgs {
   float* weights;  // [seqs][kv_heads][slots]
   int64_t max_new, max_len;
   uint64_t wait_ns;
+  int wait_selftest;
 };
 
 struct EvictArgs {

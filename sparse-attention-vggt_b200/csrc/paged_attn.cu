@@ -83,6 +83,7 @@ extern "C" int vggt_paged_attention(
   a.max_len = max_len;
   a.workspace = workspace;
   a.wait_ns = api_wait_ns();
+  a.wait_selftest = api_wait_selftest();
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   return api_cuda(few_rows(max_new, group) ? launch_paged_rows(a, plan, st)
                                            : launch_paged_tc05(a, plan, st));

@@ -54,7 +54,7 @@ struct RowsParams {
 
 template <int MT>
 struct Shared {
-  uint64_t full[8], empty[8];
+  uint64_t full[8], empty[8], never;  // never: nothing arrives (wait self-test)
   int abort, last, odd;
   float m[4][16 * MT], l[4][16 * MT];  // per warp, then per row
 };
@@ -106,6 +106,7 @@ __global__ void __launch_bounds__(kThreads, 2)
       tc::mbar_init(full(s), 1);
       tc::mbar_init(empty(s), 4);
     }
+    tc::mbar_init(smem_u32(&sh.never), 1);
     sh.abort = 0;
     sh.odd = 0;
     tc::mbar_fence_init();
@@ -126,7 +127,9 @@ __global__ void __launch_bounds__(kThreads, 2)
     const int ahead = 32 / boxes;                               // tiles per read of the table
     int page = -1;
     int64_t issued = 0;
-    for (int64_t t = 0; t < tiles; ++t) {
+    const bool go = !a.wait_selftest ||
+                    __all_sync(0xffffffffu, tc::mbar_wait(smem_u32(&sh.never), 0, abort_flag, a.wait_ns));
+    for (int64_t t = 0; go && t < tiles; ++t) {
       const int64_t key0 = (tile0 + t) * kTile;
       if (t % ahead == 0) {
         const int64_t slot = key0 + (int64_t)lane * box;

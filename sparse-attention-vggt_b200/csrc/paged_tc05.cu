@@ -76,6 +76,7 @@ struct Smem {
 struct Bars {
   uint64_t q_full, full[2][4], empty[2][4];  // of K, of V
   uint64_t s_full[2], s_free[2], p_full[2], o_full, drain[2];
+  uint64_t never;  // nothing arrives (wait self-test)
 };
 
 struct TcParams {
@@ -145,6 +146,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     }
     tc::mbar_init(smem_u32(&bars.o_full), 1);
     for (int i = 0; i < 2; ++i) tc::mbar_init(smem_u32(&bars.drain[i]), 1);
+    tc::mbar_init(smem_u32(&bars.never), 1);
     s_abort = 0;
     s_odd = 0;
     tc::mbar_fence_init();
@@ -258,6 +260,7 @@ __global__ void __launch_bounds__(kThreads, 2)
       const uint64_t qdesc = tc::sw128_desc(base + L::kQ, 16);
       const uint64_t kdesc0 = tc::sw128_desc(base + L::kK, 16);
       ok = wait(smem_u32(&bars.q_full), 0);
+      if (a.wait_selftest) ok = ok && wait(smem_u32(&bars.never), 0);
       for (int t = 0; ok && t < tiles; ++t) {
         const uint32_t buf = t & 1;
         // P of tile t - 2 lay where S_t goes: its product must be done

@@ -53,7 +53,7 @@ __global__ void __launch_bounds__(kThreads, 2)
   unsigned char* ring = raw + ((1024u - (smem_u32(raw) & 1023u)) & 1023u);
   const uint32_t ring_addr = smem_u32(ring);
   const uint32_t q_addr = ring_addr + kStages * kStage;  // [half][64 rows][128 B], swizzled
-  __shared__ uint64_t bars[2 * kStages];
+  __shared__ uint64_t bars[2 * kStages + 1];  // the last: nothing arrives (wait self-test)
   __shared__ float lse2[kRowsMax];
   __shared__ int64_t limit[kRowsMax];
   __shared__ int s_abort;
@@ -82,6 +82,7 @@ __global__ void __launch_bounds__(kThreads, 2)
       tc::mbar_init(full(s), 1);
       tc::mbar_init(empty(s), 4);
     }
+    tc::mbar_init(smem_u32(&bars[2 * kStages]), 1);
     s_abort = 0;
     tc::mbar_fence_init();
   }
@@ -93,7 +94,9 @@ __global__ void __launch_bounds__(kThreads, 2)
     const int boxes = kTile / box, ahead = 32 / boxes;
     int page = -1;
     int64_t issued = 0;
-    for (int64_t t = 0; t < tiles; ++t) {
+    const bool go = !a.wait_selftest || __all_sync(0xffffffffu, tc::mbar_wait(smem_u32(&bars[2 * kStages]), 0,
+                                                             abort_flag, a.wait_ns));
+    for (int64_t t = 0; go && t < tiles; ++t) {
       const int64_t key0 = (tile0 + t) * kTile;
       if (t % ahead == 0) {
         const int64_t slot = key0 + (int64_t)lane * box;
@@ -304,6 +307,7 @@ extern "C" int vggt_paged_weights(const void* q, int dtype, int64_t total, int64
   a.max_new = max_new;
   a.max_len = max_len;
   a.wait_ns = api_wait_ns();
+  a.wait_selftest = api_wait_selftest();
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   // up to 64 rows per sequence and key head (and groups wider than a tile) go
   // to the warp-level kernel

@@ -55,7 +55,7 @@ struct Smem {
 
 struct Bars {
   uint64_t k_full[2], k_empty[2], q_full[4], q_empty[4], lse_empty[kLseStages];
-  uint64_t s_full[2], s_empty[2], drain;
+  uint64_t s_full[2], s_empty[2], drain, never;  // never: nothing arrives (wait self-test)
 };
 
 struct WeighTcParams {
@@ -119,6 +119,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     }
     for (int s = 0; s < kLseStages; ++s) tc::mbar_init(smem_u32(&bars.lse_empty[s]), 4);
     tc::mbar_init(smem_u32(&bars.drain), 1);
+    tc::mbar_init(smem_u32(&bars.never), 1);
     s_abort = 0;
     tc::mbar_fence_init();
   }
@@ -246,7 +247,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     const uint64_t kdesc0 = tc::sw128_desc(base + L::kK, 16);
     const uint64_t qdesc0 = tc::sw128_desc(base + L::kQ, 16);
     int n_k = 0, n = 0;
-    bool ok = true;
+    bool ok = !a.wait_selftest || wait(smem_u32(&bars.never), 0);
     for (int kt = 0; ok && kt < tiles && row_tiles > 0; ++kt) {
       const int rt0 = first_row_tile(kt);
       const int kstage = n_k % L::kKStages;

@@ -545,3 +545,126 @@ def test_evict_bad_pages(cuda):
     third, second = int(c.table[0, 2]), int(c.table[0, 0])
     kp0[second] = kp0[third]
     assert torch.equal(torch.nan_to_num(kp0, nan=7.0), torch.nan_to_num(c.kp, nan=7.0))
+
+
+# ------------------------------------------------------------------ the parts together
+def test_cache_serves_ragged_sequences(cuda):
+    """Prompts, decode steps, an eviction and more steps over two sequences,
+    grouped heads, causal: each step against plain attention over the tokens
+    that the cache says it holds (its ids), with the turned keys in 64 bits."""
+    g = torch.Generator().manual_seed(9)
+    heads, group, dim = 2, 2, 64
+    cache = vggt_sparse.PagedKVCache(2, heads, dim, pages=24, max_length=160, page=16, device=cuda)
+    freq, _ = vggt_sparse.rotary_frequencies(dim)
+    kept_k, kept_v = [[], []], [[], []]
+    free = len(cache._free)
+    for step, counts in enumerate(([70, 9], [1, 1], [1, 1], [5, 40], [1, 1], [1, 0], [30, 1])):
+        total = sum(counts)
+        q, k, v = (torch.randn(total, h, dim, generator=g).to(BF).to(cuda)
+                   for h in (heads * group, heads, heads))
+        ids = torch.cat([torch.arange(cache.seen[b], cache.seen[b] + n) for b, n in enumerate(counts)])
+        ids = ids.to(torch.int32).to(cuda)
+        kept = [cache.lengths[b] for b in range(2)]
+        cache.append(k, v, counts, frequencies=freq)
+        q = vggt_sparse.rotary(q, ids, freq)
+        out, _ = cache.attend(q, causal=True)
+        turned_k = turned(k, ids, freq, 1.0, "half").to(BF)
+        row = 0
+        for b, n in enumerate(counts):
+            kept_k[b].append(turned_k[row:row + n])
+            kept_v[b].append(v[row:row + n])
+            all_k, all_v = torch.cat(kept_k[b]), torch.cat(kept_v[b])
+            m = cache.lengths[b]
+            for h in range(heads * group):
+                at = cache.ids[b, h // group, :m].long()
+                s = q[row:row + n, h].double() @ all_k[at, h // group].double().T * dim ** -0.5
+                limit = kept[b] + torch.arange(n, device=cuda)[:, None]
+                s = s.masked_fill(torch.arange(m, device=cuda)[None] > limit, -math.inf)
+                p, val = torch.softmax(s, -1), all_v[at, h // group].double()
+                # the keys differ by a rounding step from the kernel's own: u per score unit
+                bound = U[BF] * (p @ val).abs() + 3 * U[BF] * (p @ val.abs()) + 1e-6
+                assert bool(((out[row:row + n, h].double() - p @ val).abs() <= bound).all()), (step, b, h)
+            row += n
+        if step == 3:
+            want = [cache.weights[b, :, :cache.lengths[b]].sum(-1) for b in range(2)]
+            cache.evict(50, recent=4)
+            assert cache.lengths == [50, 50] and int(cache.length.sum()) == 100
+            assert len(cache._free) == free - 2 * 4
+            for b in range(2):
+                held = cache.ids[b, :, :50]
+                for h in range(heads):  # the newest stay, nothing twice, weights move along
+                    assert set(range(cache.seen[b] - 4, cache.seen[b])) <= set(held[h].tolist())
+                    assert len(set(held[h].tolist())) == 50
+                assert bool((cache.weights[b].sum(-1) <= want[b] + 1e-3).all())
+            with pytest.raises(ValueError, match="append comes before"):
+                cache.attend(q)
+    cache.check()
+    cache.release(0)
+    cache.release(1)
+    assert sorted(cache._free) == list(range(24))
+
+
+def test_streaming_layer_keeps_specials_and_equals_full_attention(cuda):
+    """Frames of 5 special and 36 patch tokens.  While nothing is evicted the
+    layer is attention over all frames so far; afterwards the specials of every
+    frame and the whole last frame are still there."""
+    g = torch.Generator().manual_seed(4)
+    heads, dim, per, frames = 3, 64, 41, 6
+    layer = vggt_sparse.StreamingGlobalLayer(heads, dim, per, 4 * per, page=32, device=cuda)
+    yy, xx = torch.meshgrid(torch.arange(6), torch.arange(6), indexing="ij")
+    pos = torch.cat((torch.zeros(5, 2), torch.stack((yy.flatten() + 1, xx.flatten() + 1), -1)))
+    pos = pos.to(torch.int32).to(cuda)
+    keys, vals = [], []
+    for f in range(frames):
+        q, k, v = (torch.randn(per, heads, dim, generator=g).to(BF).to(cuda) for _ in range(3))
+        out = layer(q, k, v, pos)
+        keys.append(turned(k, pos, layer.frequencies, 1.0, "half").to(BF).double())
+        vals.append(v.double())
+        if f < 4:
+            tq = turned(q, pos, layer.frequencies, 1.0, "half").to(BF).double()
+            s = torch.einsum("nhd,mhd->hnm", tq, torch.cat(keys)) * dim ** -0.5
+            p, val = torch.softmax(s, -1), torch.cat(vals)
+            want = torch.einsum("hnm,mhd->nhd", p, val)
+            mag = torch.einsum("hnm,mhd->nhd", p, val.abs())
+            assert bool(((out.double() - want).abs() <= U[BF] * want.abs() + 3 * U[BF] * mag).all())
+    layer.cache.check()
+    assert layer.cache.lengths == [4 * per]
+    for h in range(heads):
+        held = set(layer.cache.ids[0, h, :4 * per].tolist())
+        assert len(held) == 4 * per
+        assert {f * per + i for f in range(frames) for i in range(5)} <= held
+        assert set(range((frames - 1) * per, frames * per)) <= held
+
+
+@pytest.mark.parametrize("new,lengths", [(300, 3000), (1, 3000), (70, 64)])
+def test_wait_limit_is_reported(cuda, new, lengths):
+    """The self-test switch lets one warp of every CTA wait on a barrier that
+    nothing completes; with a limit of 2 ms each CTA gives up through its
+    ordinary path, the status says so, and the next calls are right."""
+    c = Case(cuda, [lengths], [new], 2, 1, 64, 64)
+    w = torch.zeros(1, 2, c.table.shape[1] * 64, device=cuda)
+
+    def weigh(lse):
+        vggt_sparse.paged_weights(c.q, lse, c.kp, c.table, c.len, c.starts, w, max_new=new,
+                                  status=c.status)
+    prev_limit = _lib.set_wait_limit_ns(2_000_000)
+    prev_test = _lib.set_wait_selftest(True)
+    try:
+        for call in (lambda: c.attend(True),
+                     lambda: weigh(torch.zeros(new, 2, device=cuda))):
+            c.status.zero_()
+            call()
+            torch.cuda.synchronize()
+            assert int(c.status) == _lib.STATUS_TIMEOUT
+            with pytest.raises(ValueError, match="timed out"):
+                vggt_sparse.check_cache_status(c.status)
+    finally:
+        _lib.set_wait_selftest(prev_test)
+        _lib.set_wait_limit_ns(prev_limit)
+    c.status.zero_()
+    w.zero_()
+    out, lse = c.attend(True)
+    c.check(out, lse, True)
+    weigh(lse)
+    seen = int((lse > -math.inf).sum())
+    assert abs(float(w.sum()) - seen) <= 1e-4 * seen
