@@ -79,20 +79,23 @@ __device__ __forceinline__ int64_t sequence_of_row(const int32_t* starts, int64_
 // g the query head within the head's group, cut into tiles of `tile` rows.
 // (The entry points keep total * group below 2^31, so row numbers fit an int.)
 struct RowTile {
-  int64_t seq, first;
+  int64_t seq, first, len;  // len: cached tokens
   int n_new, row0, rows;  // rows: of the sequence, over all its tiles
 };
 
 // Finds the `index`-th row tile over all sequences; false past the last one.
 // Called by full warps, every lane gets the answer.
-__device__ __forceinline__ bool locate_tile(const PageTable& t, int group, int tile, int64_t index,
-                                            RowTile& out) {
+__device__ __forceinline__ bool locate_tile(const PageTable& t, const Pool& pool, int group,
+                                            int tile, int64_t index, RowTile& out) {
   const int lane = threadIdx.x & 31;
   int64_t base = 0;
   for (int64_t s0 = 0; s0 < t.seqs; s0 += 32) {
     const int64_t b = s0 + lane;
-    int64_t first = 0, n = 0;
-    if (b < t.seqs) n = checked_rows(t, b, first);
+    int64_t first = 0, n = 0, len = 0;
+    if (b < t.seqs) {
+      len = checked_length(t, pool, b);  // beside the starts: one latency for both
+      n = checked_rows(t, b, first);
+    }
     const int64_t tiles = (n * group + tile - 1) / tile;
     int64_t sum = tiles;
 #pragma unroll
@@ -105,6 +108,7 @@ __device__ __forceinline__ bool locate_tile(const PageTable& t, int group, int t
       const int src = __ffs(hit) - 1;
       out.seq = s0 + src;
       out.first = __shfl_sync(0xffffffffu, first, src);
+      out.len = __shfl_sync(0xffffffffu, len, src);
       out.n_new = (int)__shfl_sync(0xffffffffu, n, src);
       out.row0 = (int)(index - base - __shfl_sync(0xffffffffu, sum - tiles, src)) * tile;
       out.rows = out.n_new * group;
@@ -188,7 +192,7 @@ struct PagedPlan {
 };
 
 PagedPlan paged_rows_plan(int64_t total, int64_t seqs, int kv_heads, int group, int dim,
-                          int64_t max_new, int64_t max_len);
+                          int64_t max_len);
 cudaError_t launch_paged_rows(const PagedAttnArgs& a, const PagedPlan& plan, cudaStream_t st);
 PagedPlan paged_tc05_plan(int64_t total, int64_t seqs, int kv_heads, int group, int dim,
                           int64_t max_len);

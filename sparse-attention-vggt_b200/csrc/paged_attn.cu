@@ -8,14 +8,16 @@ using namespace vggt;
 
 namespace {
 
-// Up to 64 rows per sequence and key head go to the warp-level kernel, more to
-// the tcgen05 one.
-bool few_rows(int64_t max_new, int group) { return max_new * group <= 64; }
+// Up to 16 rows per sequence and key head go to the warp-level kernel, more to
+// the tcgen05 one.  32 sequences over 32,768 keys of 128, in us, warp-level
+// against tcgen05: 4 rows 473 / 578, 20 rows 559 / 563, 32 rows 548 / 514, 64
+// rows 974 / 530 (the warp-level kernel with tiles of 32 and 64 rows).
+bool few_rows(int64_t max_new, int group) { return max_new * group <= 16; }
 
 PagedPlan plan_of(int64_t total, int64_t seqs, int kv_heads, int group, int dim, int64_t max_new,
                   int64_t max_len) {
   return few_rows(max_new, group)
-             ? paged_rows_plan(total, seqs, kv_heads, group, dim, max_new, max_len)
+             ? paged_rows_plan(total, seqs, kv_heads, group, dim, max_len)
              : paged_tc05_plan(total, seqs, kv_heads, group, dim, max_len);
 }
 

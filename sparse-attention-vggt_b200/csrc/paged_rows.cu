@@ -2,14 +2,14 @@
 //
 // For a sequence and a key head the query rows (tokens x the head's group)
 // are few, and every key and value is used by all of them: the pass is bound
-// by reading K and V once.  So a CTA takes one tile of 16 * MT rows and one
+// by reading K and V once.  So a CTA takes one tile of 16 rows and one
 // run of key tiles, and what matters is that loads never pause:
 //  * warp 4 streams 64-key K and V tiles by TMA (boxes of one page, 128-byte
 //    swizzle) into a ring; page numbers are read 32 boxes ahead.
-//  * warps 0-3 share a tile's keys when there are 16 rows (16 keys each), and
-//    its rows when there are 64; each keeps its own running maximum, sum and
-//    output rows in registers (mma.sync m16n8k16, fp32), so no warp waits for
-//    another before the end.  tcgen05 would spend M = 128 rows on 16.
+//  * warps 0-3 share a tile's keys, 16 each; each keeps its own running
+//    maximum, sum and output rows in registers (mma.sync m16n8k16, fp32), so no
+//    warp waits for another before the end.  tcgen05 would spend M = 128 rows
+//    on 16; it is as fast from 20 rows on (see paged_attn.cu).
 //  * a long cache is cut into runs of `chunk` tiles, one CTA each; the CTA
 //    that finishes last (a counter per item) joins the runs' results in their
 //    order and leaves the counter at zero, so there is one launch and the
@@ -33,6 +33,10 @@ namespace {
 
 constexpr int kTile = 64;  // keys per ring stage
 constexpr int kThreads = 160;
+constexpr int kRows = 16;
+constexpr int kGroups = 4;              // warps that share a tile's keys
+constexpr int kKeys = kTile / kGroups;  // keys of a warp in a tile
+constexpr int kN = kKeys / 8;           // n-tiles of S
 
 template <int D>
 struct Ring {
@@ -52,27 +56,22 @@ struct RowsParams {
   float* partial;                // [tiles * heads][splits][rows * (D + 2)]
 };
 
-template <int MT>
 struct Shared {
   uint64_t full[8], empty[8], never;  // never: nothing arrives (wait self-test)
   int abort, last, odd;
-  float m[4][16 * MT], l[4][16 * MT];  // per warp, then per row
+  float m[4][kRows], l[4][kRows];  // per warp, then per row
 };
 
-template <typename T, int D, int MT>
+template <typename T, int D>
 __global__ void __launch_bounds__(kThreads, 2)
     paged_rows_kernel(const __grid_constant__ CUtensorMap tm_k,
                       const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ RowsParams p) {
   using R = Ring<D>;
-  constexpr int kRows = 16 * MT;
-  constexpr int kGroups = 4 / MT;             // warps that share a row tile's keys
-  constexpr int kKeys = kTile / kGroups;      // keys of a warp in a tile
-  constexpr int kN = kKeys / 8;               // n-tiles of S
   constexpr int kSteps = D / 16;
   extern __shared__ unsigned char raw[];
   unsigned char* ring = raw + ((1024u - (smem_u32(raw) & 1023u)) & 1023u);
   const uint32_t ring_addr = smem_u32(ring);
-  __shared__ Shared<MT> sh;
+  __shared__ Shared sh;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
   // ---- which rows and which keys ----
@@ -80,8 +79,8 @@ __global__ void __launch_bounds__(kThreads, 2)
   const int head = (int)(item % p.heads);
   const PagedAttnArgs& a = p.a;
   RowTile rt;
-  if (!locate_tile(a.t, a.group, kRows, item / p.heads, rt)) return;
-  const int64_t len = checked_length(a.t, a.pool, rt.seq);
+  if (!locate_tile(a.t, a.pool, a.group, kRows, item / p.heads, rt)) return;
+  const int64_t len = rt.len;
   const int rows = rt.rows - rt.row0 < kRows ? rt.rows - rt.row0 : kRows;
   // keys that row r of the tile sees
   auto limit_of = [&](int r) -> int64_t {
@@ -169,8 +168,8 @@ __global__ void __launch_bounds__(kThreads, 2)
                           1000000000ull);
   } else {
     // ================= S, softmax, O =================
-    const int mi = warp / kGroups, kg = warp % kGroups;
-    const int r0 = mi * 16 + (lane >> 2);  // this thread's rows: r0, r0 + 8
+    const int kg = warp;
+    const int r0 = lane >> 2;  // this thread's rows: r0, r0 + 8
     int64_t lim[2];
     uint32_t qf[kSteps][4];
     {
@@ -309,8 +308,8 @@ __global__ void __launch_bounds__(kThreads, 2)
   __syncthreads();  // the ring is free now: its space takes the output rows
   float* obuf = reinterpret_cast<float*>(ring);  // [kGroups][kRows][D]
   if (warp < 4) {
-    const int mi = warp / kGroups, kg = warp % kGroups;
-    const int r0 = mi * 16 + (lane >> 2);
+    const int kg = warp;
+    const int r0 = lane >> 2;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const int r = r0 + 8 * i;
@@ -339,13 +338,11 @@ __global__ void __launch_bounds__(kThreads, 2)
     sh.m[0][tid] = rm;
     sh.l[0][tid] = rl;
   }
-  if constexpr (kGroups > 1) {
-    for (int i = tid; i < kRows * D; i += kThreads) {
-      float v = obuf[i];
+  for (int i = tid; i < kRows * D; i += kThreads) {
+    float v = obuf[i];
 #pragma unroll
-      for (int g = 1; g < kGroups; ++g) v += obuf[g * kRows * D + i];
-      obuf[i] = v;
-    }
+    for (int g = 1; g < kGroups; ++g) v += obuf[g * kRows * D + i];
+    obuf[i] = v;
   }
   __syncthreads();
   if (sh.odd) {
@@ -376,36 +373,54 @@ __global__ void __launch_bounds__(kThreads, 2)
     __syncthreads();
     if (!sh.last) return;
     __threadfence();
-    const float* from = p.partial + item * p.splits * (int64_t)(kRows * (D + 2));
+    // the runs' maxima and sums, then the rows, 4 vectors of 4 runs in flight
+    constexpr int64_t kRun = kRows * (D + 2);
+    const float* from = p.partial + item * p.splits * kRun;
+    float* wgt = obuf + kRows * D;        // [runs][kRows], 64 runs at most
+    float* sums = wgt + 64 * kRows;
+    for (int i = tid; i < (int)runs * kRows; i += kThreads) {
+      const float* ml = from + (i / kRows) * kRun + kRows * D + i % kRows;
+      wgt[i] = __ldcg(ml);
+      sums[i] = __ldcg(ml + kRows);
+    }
+    __syncthreads();
     if (tid < kRows) {
       float mx = -INFINITY, l = 0.f;
-      for (int64_t s = 0; s < runs; ++s)
-        mx = fmaxf(mx, __ldcg(from + s * kRows * (D + 2) + kRows * D + tid));
-      const float b = mx == -INFINITY ? 0.f : mx;
-      for (int64_t s = 0; s < runs; ++s) {
-        const float* ml = from + s * kRows * (D + 2) + kRows * D + tid;
-        l += __ldcg(ml + kRows) * fast_exp2(__ldcg(ml) - b);
+      for (int s = 0; s < (int)runs; ++s) mx = fmaxf(mx, wgt[s * kRows + tid]);
+      for (int s = 0; s < (int)runs; ++s) {
+        const float f = fast_exp2(wgt[s * kRows + tid] - (mx == -INFINITY ? 0.f : mx));
+        wgt[s * kRows + tid] = f;
+        l = fmaf(f, sums[s * kRows + tid], l);
       }
       sh.m[0][tid] = mx;
       sh.l[0][tid] = l;
     }
     __syncthreads();
-    for (int i = tid; i < kRows * D / 4; i += kThreads) {
-      const int r = i / (D / 4);
-      const float b = sh.m[0][r] == -INFINITY ? 0.f : sh.m[0][r];
-      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    constexpr int kBatch = 4;
+    for (int i0 = tid; i0 < kRows * D / 4; i0 += kBatch * kThreads) {
+      float4 acc[kBatch];
+#pragma unroll
+      for (int j = 0; j < kBatch; ++j) acc[j] = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
-      for (int64_t s = 0; s < runs; ++s) {
-        const float* ps = from + s * kRows * (D + 2);
-        const float f = fast_exp2(__ldcg(ps + kRows * D + r) - b);
-        const float4 v = __ldcg(reinterpret_cast<const float4*>(ps) + i);
-        // a run that saw nothing of this row holds zeros, and f is zero
-        acc.x = fmaf(f, v.x, acc.x);
-        acc.y = fmaf(f, v.y, acc.y);
-        acc.z = fmaf(f, v.z, acc.z);
-        acc.w = fmaf(f, v.w, acc.w);
+      for (int s = 0; s < (int)runs; ++s) {
+        const float4* src = reinterpret_cast<const float4*>(from + s * kRun);
+#pragma unroll
+        for (int j = 0; j < kBatch; ++j) {
+          const int i = i0 + j * kThreads;
+          if (i < kRows * D / 4) {
+            const float4 v = __ldcg(src + i);
+            const float f = wgt[s * kRows + i / (D / 4)];
+            acc[j].x = fmaf(f, v.x, acc[j].x);
+            acc[j].y = fmaf(f, v.y, acc[j].y);
+            acc[j].z = fmaf(f, v.z, acc[j].z);
+            acc[j].w = fmaf(f, v.w, acc[j].w);
+          }
+        }
       }
-      reinterpret_cast<float4*>(obuf)[i] = acc;
+#pragma unroll
+      for (int j = 0; j < kBatch; ++j)
+        if (i0 + j * kThreads < kRows * D / 4)
+          reinterpret_cast<float4*>(obuf)[i0 + j * kThreads] = acc[j];
     }
     __syncthreads();
   }
@@ -430,10 +445,10 @@ __global__ void __launch_bounds__(kThreads, 2)
   }
 }
 
-template <typename T, int D, int MT>
+template <typename T, int D>
 cudaError_t launch_rows(const RowsParams& p, const CUtensorMap& mk, const CUtensorMap& mv,
                         cudaStream_t st) {
-  auto kernel = paged_rows_kernel<T, D, MT>;
+  auto kernel = paged_rows_kernel<T, D>;
   const size_t smem = Ring<D>::kBytes + 1024;
   const cudaError_t e =
       cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
@@ -442,26 +457,38 @@ cudaError_t launch_rows(const RowsParams& p, const CUtensorMap& mk, const CUtens
   return cudaGetLastError();
 }
 
-// 16-row tiles per CTA: the fewest that hold the rows of a sequence, at most 4.
-int row_tiles(int64_t rows) { return rows <= 16 ? 1 : (rows <= 32 ? 2 : 4); }
-
 }  // namespace
 
 PagedPlan paged_rows_plan(int64_t total, int64_t seqs, int kv_heads, int group, int dim,
-                          int64_t max_new, int64_t max_len) {
+                          int64_t max_len) {
   PagedPlan plan{};
-  plan.rows = 16 * row_tiles(max_new * group);
+  plan.rows = kRows;
   plan.tiles = most_tiles(total, seqs, group, plan.rows);
   const int64_t items = plan.tiles * kv_heads;
   const int64_t key_tiles = (max_len + kTile - 1) / kTile;
-  // runs short enough for four waves of two CTAs on every SM, two tiles at
-  // least, so that ragged sequences share the card evenly
-  plan.chunk = items * key_tiles / (4 * 2 * 148);
-  if (plan.chunk < 2) plan.chunk = 2;
-  plan.splits =
-      key_tiles > 0 && items <= kMaxCounters ? (key_tiles + plan.chunk - 1) / plan.chunk : 1;
+  // Runs per row tile, in microseconds as measured: a CTA takes 0.63 a key tile
+  // (dim 64), twice that where K and V rows are twice as wide; 5 to start, 3
+  // more where two share an SM; joining 3 and 0.1 a run.  Beyond one wave of
+  // 296, sequences of different lengths leave half a run idle at the end.  One
+  // token over 1,375 keys in 16 heads: 8 runs 11.6 us, 1 run 19.9, 11 runs
+  // 15.6; over 43,001 keys: 16 runs 43.5, 8 runs 64.4, 22 runs 69.1.
+  const double tile_us = dim == 64 ? 0.63 : 1.26;
+  double best = -1;
+  plan.splits = 1;
+  for (int64_t s = 1; s <= 64 && (s == 1 || (s <= key_tiles && items <= kMaxCounters)); ++s) {
+    const int64_t ctas = items * s;
+    const double run = (double)((key_tiles + s - 1) / s) * tile_us;
+    const double waves = ctas > 296 ? (double)ctas / 296 : 1.0;
+    const double cost = waves * (run + (ctas > 148 ? 8 : 5)) + (ctas > 296 ? 0.5 * run : 0) +
+                        (s > 1 ? 3 + 0.1 * s : 0);
+    if (best < 0 || cost < best) {
+      best = cost;
+      plan.splits = s;
+    }
+  }
+  plan.chunk = key_tiles > 0 ? (key_tiles + plan.splits - 1) / plan.splits : 1;
   plan.partial_bytes =
-      plan.splits > 1 ? (size_t)items * plan.splits * plan.rows * (dim + 2) * 4 : 0;
+      plan.splits > 1 ? (size_t)items * plan.splits * kRows * (dim + 2) * 4 : 0;
   return plan;
 }
 
@@ -482,14 +509,11 @@ cudaError_t launch_paged_rows(const PagedAttnArgs& a, const PagedPlan& plan, cud
   if (!encode_pool_tmap(&mk, a.k_pages, a.dtype, a.pool, box) ||
       !encode_pool_tmap(&mv, a.v_pages, a.dtype, a.pool, box))
     return cudaErrorInvalidValue;
-#define VGGT_ROWS(T, D)                                                     \
-  (plan.rows == 16   ? launch_rows<T, D, 1>(p, mk, mv, st)                  \
-   : plan.rows == 32 ? launch_rows<T, D, 2>(p, mk, mv, st)                  \
-                     : launch_rows<T, D, 4>(p, mk, mv, st))
   if (a.dtype == VGGT_DTYPE_BF16)
-    return a.pool.dim == 64 ? VGGT_ROWS(__nv_bfloat16, 64) : VGGT_ROWS(__nv_bfloat16, 128);
-  return a.pool.dim == 64 ? VGGT_ROWS(__half, 64) : VGGT_ROWS(__half, 128);
-#undef VGGT_ROWS
+    return a.pool.dim == 64 ? launch_rows<__nv_bfloat16, 64>(p, mk, mv, st)
+                            : launch_rows<__nv_bfloat16, 128>(p, mk, mv, st);
+  return a.pool.dim == 64 ? launch_rows<__half, 64>(p, mk, mv, st)
+                          : launch_rows<__half, 128>(p, mk, mv, st);
 }
 
 }  // namespace vggt

@@ -113,8 +113,8 @@ __global__ void __launch_bounds__(kThreads, 2)
   const int64_t tile = p.tiles - 1 - w % p.tiles;
   const int64_t item = head * p.tiles + tile;
   RowTile rt;
-  if (!locate_tile(a.t, a.group, kRows, tile, rt)) return;
-  const int64_t len = checked_length(a.t, a.pool, rt.seq);
+  if (!locate_tile(a.t, a.pool, a.group, kRows, tile, rt)) return;
+  const int64_t len = rt.len;
   const int rows = rt.rows - rt.row0 < kRows ? rt.rows - rt.row0 : kRows;
   auto limit_of = [&](int r) -> int64_t {
     if (!a.causal) return len;

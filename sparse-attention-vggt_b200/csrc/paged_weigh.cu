@@ -16,12 +16,20 @@
 #include "kernels.h"
 #include "mma.cuh"
 #include "paged.cuh"
+#include "paged_producer.cuh"
 #include "tc05.cuh"
 
 namespace vggt {
 namespace {
 
 constexpr int kTile = 64, kRowsMax = 64, kThreads = 160;
+
+// short rings, and so three or four CTAs to an SM: a tile's chain of wait,
+// products, exponentials and sums takes longer than its copy
+template <int D>
+constexpr int kStagesOf = D == 64 ? 5 : 3;
+template <int D>
+constexpr int kCtas = D == 64 ? 4 : 3;
 
 struct WeighParams {
   WeighArgs a;
@@ -44,18 +52,18 @@ __device__ __forceinline__ bool all_of_128(bool ok) {
 }
 
 template <typename T, int D>
-__global__ void __launch_bounds__(kThreads, 2)
+__global__ void __launch_bounds__(kThreads, kCtas<D>)
     weigh_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const WeighParams p) {
   constexpr int kHalves = D / 64, kSteps = D / 16;
   constexpr uint32_t kStage = kTile * D * 2;
-  constexpr int kStages = D == 64 ? 10 : 5;
+  constexpr int kStages = kStagesOf<D>;
   extern __shared__ unsigned char raw[];
   unsigned char* ring = raw + ((1024u - (smem_u32(raw) & 1023u)) & 1023u);
   const uint32_t ring_addr = smem_u32(ring);
   const uint32_t q_addr = ring_addr + kStages * kStage;  // [half][64 rows][128 B], swizzled
   __shared__ uint64_t bars[2 * kStages + 1];  // the last: nothing arrives (wait self-test)
   __shared__ float lse2[kRowsMax];
-  __shared__ int64_t limit[kRowsMax];
+  __shared__ int limit[kRowsMax];
   __shared__ int s_abort;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const WeighArgs& a = p.a;
@@ -90,92 +98,90 @@ __global__ void __launch_bounds__(kThreads, 2)
 
   if (warp == 4) {
     // ================= TMA producer =================
-    const int box = a.pool.page < kTile ? a.pool.page : kTile;
-    const int boxes = kTile / box, ahead = 32 / boxes;
-    int page = -1;
-    int64_t issued = 0;
-    const bool go = !a.wait_selftest || __all_sync(0xffffffffu, tc::mbar_wait(smem_u32(&bars[2 * kStages]), 0,
-                                                             abort_flag, a.wait_ns));
-    for (int64_t t = 0; go && t < tiles; ++t) {
-      const int64_t key0 = (tile0 + t) * kTile;
-      if (t % ahead == 0) {
-        const int64_t slot = key0 + (int64_t)lane * box;
-        page = (int)a.pool.n_pages;
-        if (slot < len && slot < (tile0 + tiles) * kTile) {
-          const int got = checked_page(a.t, a.pool, seq, slot >> a.pool.page_shift);
-          if (got >= 0) page = got;
-        }
-      }
-      const int stage = (int)(t % kStages);
-      bool ok = true;
-      if (t >= kStages)
-        ok = tc::mbar_wait(empty(stage), (uint32_t)((t / kStages - 1) & 1), abort_flag, a.wait_ns);
-      if (!__all_sync(0xffffffffu, ok)) break;
-      const int need = (int)((len - key0 + box - 1) / box);
-      const int live = need < boxes ? need : boxes;
-      if (lane == 0) tc::mbar_expect_tx(full(stage), (uint32_t)(live * box) * D * 2u);
-      __syncwarp();
-      const int b = lane & (boxes - 1), half = lane / boxes;
-      const int mine = __shfl_sync(0xffffffffu, page, (int)(t % ahead) * boxes + b);
-      if (half < kHalves && b < live)
-        tc::tma_load_4d(ring_addr + (uint32_t)stage * kStage + half * (kTile * 128) + b * box * 128,
-                        &tm_k, full(stage), half * 64, (int)((key0 + b * box) & (a.pool.page - 1)),
-                        head, mine);
-      ++issued;
-    }
-    const int64_t from = issued > kStages ? issued - kStages : 0;
-    for (int64_t t = from; t < issued; ++t)
-      tc::mbar_wait_drain(full((int)(t % kStages)), (uint32_t)((t / kStages) & 1), 1000000000ull);
+    if (!a.wait_selftest || tc::warp_wait(smem_u32(&bars[2 * kStages]), 0, abort_flag, a.wait_ns))
+      produce_tiles<kHalves, 1, kStages>(a.t, a.pool, seq, head, tile0 * kTile,
+                                         (int)(len - tile0 * kTile), (int)tiles, &tm_k, &tm_k,
+                                         ring_addr, full(0), empty(0), abort_flag, a.wait_ns);
   } else {
     const int krow = ((lane >> 4) & 1) * 8 + (lane & 7), kchunk = (lane >> 3) & 1;
     const int qrow = ((lane >> 3) & 1) * 8 + (lane & 7), qchunk = (lane >> 4) & 1;
-    int loaded = -1;  // first row of the rows in shared memory
+    // rows c0 .. c0 + 63 into shared memory; rows that are not there are zeros
+    // with lse +inf, which gives nothing
+    auto load_rows = [&](int c0) {
+      const int here = rows - c0 < kRowsMax ? rows - c0 : kRowsMax;
+      for (int i = tid; i < kRowsMax * (D / 8); i += 128) {
+        const int r = i / (D / 8), c = i % (D / 8);
+        uint4 v = make_uint4(0u, 0u, 0u, 0u);
+        if (r < here) {
+          const int row = c0 + r;
+          v = __ldg(reinterpret_cast<const uint4*>(
+              static_cast<const T*>(a.q) + (first + row / a.group) * a.q_token +
+              ((int64_t)head * a.group + row % a.group) * a.q_head + c * 8));
+        }
+        const uint32_t dst =
+            q_addr + (c >> 3) * (kRowsMax * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4);
+        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "r"(v.x), "r"(v.y),
+                     "r"(v.z), "r"(v.w)
+                     : "memory");
+      }
+      if (tid < kRowsMax) {
+        const int row = c0 + tid;
+        float l = -INFINITY;
+        if (tid < here)
+          l = a.lse[(first + row / a.group) * ((int64_t)a.pool.kv_heads * a.group) +
+                    (int64_t)head * a.group + row % a.group];
+        // a row without keys gives nothing either
+        lse2[tid] = l == -INFINITY ? INFINITY : l * 1.4426950408889634f;
+        // keys of this CTA's run that the row sees
+        const int64_t n = (a.causal ? len - n_new + row / a.group + 1 : len) - tile0 * kTile;
+        limit[tid] = (int)(n < 0 ? 0 : (n < tiles * kTile ? n : tiles * kTile));
+      }
+    };
+    auto sync_rows = [] { asm volatile("bar.sync 1, 128;" ::: "memory"); };
+    // With 64 rows at most they are loaded once and the warps go their own
+    // ways; more rows (the caller expected fewer) are loaded again per tile.
+    const bool once = rows <= kRowsMax;
+    if (once) {
+      load_rows(0);
+      sync_rows();
+    }
+    float* weights =
+        a.weights + (seq * a.pool.kv_heads + head) * (a.t.width << a.pool.page_shift);
+    // the old weights of this lane's keys in tile t, loaded a tile ahead: their
+    // latency is a tile's whole time
+    auto load_old = [&](int64_t t, float* v) {
+      if (lane >= 4) return;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int64_t key =
+            (tile0 + t) * kTile + warp * 16 + (j >> 1) * 8 + lane * 2 + (j & 1);
+        v[j] = t < tiles && key < len ? weights[key] : 0.f;
+      }
+    };
+    float next_old[4];
+    load_old(0, next_old);
     for (int64_t t = 0; t < tiles; ++t) {
       const int stage = (int)(t % kStages);
-      // the four warps go on or leave together: they share barriers below
-      if (!all_of_128(tc::mbar_wait(full(stage), (uint32_t)((t / kStages) & 1), abort_flag,
-                                    a.wait_ns)))
-        break;
-      const int64_t key0 = (tile0 + t) * kTile + warp * 16;
+      const bool got =
+          tc::warp_wait(full(stage), (uint32_t)((t / kStages) & 1), abort_flag, a.wait_ns);
+      // sharing barriers below, the warps go on or leave together
+      if (once ? !got : !all_of_128(got)) break;
+      const int at = (int)t * kTile + warp * 16;  // this warp's first key, in the run
+      const int64_t key0 = tile0 * kTile + at;
       const uint32_t kbase = ring_addr + (uint32_t)stage * kStage + warp * 16 * 128;
+      float old[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) old[j] = next_old[j];
+      load_old(t + 1, next_old);
       float sum[4] = {0.f, 0.f, 0.f, 0.f};
       for (int c0 = 0; c0 < rows; c0 += kRowsMax) {
-        const int here = rows - c0 < kRowsMax ? rows - c0 : kRowsMax;
-        if (loaded != c0) {
-          asm volatile("bar.sync 1, 128;" ::: "memory");
-          for (int i = tid; i < kRowsMax * (D / 8); i += 128) {
-            const int r = i / (D / 8), c = i % (D / 8);
-            uint4 v = make_uint4(0u, 0u, 0u, 0u);
-            if (r < here) {
-              const int row = c0 + r;
-              v = __ldg(reinterpret_cast<const uint4*>(
-                  static_cast<const T*>(a.q) + (first + row / a.group) * a.q_token +
-                  ((int64_t)head * a.group + row % a.group) * a.q_head + c * 8));
-            }
-            const uint32_t dst = q_addr + (c >> 3) * (kRowsMax * 128) + r * 128 +
-                                 (((c & 7) ^ (r & 7)) << 4);
-            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "r"(v.x), "r"(v.y),
-                         "r"(v.z), "r"(v.w)
-                         : "memory");
-          }
-          if (tid < kRowsMax) {
-            const int row = c0 + tid;
-            float l = 0.f;
-            int64_t n = 0;
-            if (tid < here) {
-              l = a.lse[(first + row / a.group) * ((int64_t)a.pool.kv_heads * a.group) +
-                        (int64_t)head * a.group + row % a.group] *
-                  1.4426950408889634f;
-              if (l == -INFINITY) l = INFINITY;  // a row without keys gives nothing
-              n = a.causal ? len - n_new + row / a.group + 1 : len;
-            }
-            lse2[tid] = l;
-            limit[tid] = n;
-          }
-          asm volatile("bar.sync 1, 128;" ::: "memory");
-          loaded = c0;
+        if (!once) {
+          sync_rows();
+          load_rows(c0);
+          sync_rows();
         }
-        const bool masked = here < kRowsMax || key0 + 16 > limit[0];
+        const int here = rows - c0 < kRowsMax ? rows - c0 : kRowsMax;
+        const bool masked = at + 16 > limit[0];
         for (int m0 = 0; m0 < here; m0 += 16) {
           float s[2][4];
 #pragma unroll
@@ -197,11 +203,10 @@ __global__ void __launch_bounds__(kThreads, 2)
           for (int i = 0; i < 2; ++i) {
             const int r = m0 + (lane >> 2) + 8 * i;
             const float l = lse2[r];
-            const int64_t n = limit[r];
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
               float e = fast_exp2(fmaf(s[j >> 1][2 * i + (j & 1)], p.scale_log2, -l));
-              if (masked && key0 + (j >> 1) * 8 + (lane & 3) * 2 + (j & 1) >= n) e = 0.f;
+              if (masked && at + (j >> 1) * 8 + (lane & 3) * 2 + (j & 1) >= limit[r]) e = 0.f;
               sum[j] += e;
             }
           }
@@ -216,11 +221,10 @@ __global__ void __launch_bounds__(kThreads, 2)
         sum[j] += __shfl_xor_sync(0xffffffffu, sum[j], 16);
       }
       if (lane < 4) {
-        float* w = a.weights + (seq * a.pool.kv_heads + head) * (a.t.width << a.pool.page_shift);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const int64_t key = key0 + (j >> 1) * 8 + lane * 2 + (j & 1);
-          if (key < len) w[key] = fmaf(w[key], a.decay, sum[j]);
+          if (key < len) weights[key] = fmaf(old[j], a.decay, sum[j]);
         }
       }
     }
@@ -232,7 +236,7 @@ __global__ void __launch_bounds__(kThreads, 2)
 template <typename T, int D>
 cudaError_t launch_weigh_rows(const WeighParams& p, const CUtensorMap& mk, cudaStream_t st) {
   auto kernel = weigh_rows_kernel<T, D>;
-  const size_t smem = (D == 64 ? 10 : 5) * kTile * D * 2 + kRowsMax * D * 2 + 1024;
+  const size_t smem = kStagesOf<D> * kTile * D * 2 + kRowsMax * D * 2 + 1024;
   const cudaError_t e =
       cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
   if (e != cudaSuccess) return e;
@@ -248,7 +252,7 @@ cudaError_t launch_paged_weigh_rows(const WeighArgs& a, cudaStream_t st) {
   p.scale_log2 = a.scale * 1.4426950408889634f;
   const int64_t items = a.t.seqs * a.pool.kv_heads;
   const int64_t key_tiles = (a.max_len + kTile - 1) / kTile;
-  p.chunk = items * key_tiles / (4 * 2 * 148);
+  p.chunk = items * key_tiles / (4 * 3 * 148);
   if (p.chunk < 2) p.chunk = 2;
   p.splits = key_tiles > 0 ? (key_tiles + p.chunk - 1) / p.chunk : 1;
   if (items * p.splits > 0x7fffffffLL) return cudaErrorInvalidValue;
@@ -309,8 +313,10 @@ extern "C" int vggt_paged_weights(const void* q, int dtype, int64_t total, int64
   a.wait_ns = api_wait_ns();
   a.wait_selftest = api_wait_selftest();
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  // up to 64 rows per sequence and key head (and groups wider than a tile) go
-  // to the warp-level kernel
-  const bool rows = max_new * group <= 64 || group > 128 || total == 0;
+  // Up to 40 rows per sequence and key head (and groups wider than a tile) go to
+  // the warp-level kernel: 32 sequences over 32,768 keys of 128, in us,
+  // warp-level against tcgen05: 20 rows 356 / 442, 32 rows 395 / 441, 64 rows
+  // 594 / 451.
+  const bool rows = max_new * group <= 40 || group > 128 || total == 0;
   return api_cuda(rows ? launch_paged_weigh_rows(a, st) : launch_paged_weigh_tc05(a, st));
 }
