@@ -10,11 +10,14 @@
 // position * freq is off by 4e-3 radians at position 65,536).  Its upper 32
 // bits go to sincospif: the angle is then within 2^-24 of a radian or two.
 //
-// Both kernels are bound by memory: every element is read and written once.
+// Both kernels are bound by memory: every element is read and written once (32
+// frames' queries, 180 MB, in 35.8 us: 5.0 TB/s, 0.79 of the measured copy
+// rate).
 // A thread owns up to 8 pairs (two 16-byte vectors of a 2-byte type) of a
 // token, takes their sines once and walks over heads with them, four heads'
 // loads in flight at a time.  With few tokens the heads are dealt to more
-// threads, until the grid fills the card.
+// threads, until the grid fills the card.  (Sines of a CTA's tokens in shared
+// memory and rows in the order of memory: 47.9 us.)
 #include "kernels.h"
 #include "paged.cuh"
 
@@ -211,8 +214,10 @@ __device__ __forceinline__ int64_t append_slot(const AppendArgs& p, int64_t row,
   return -1;
 }
 
+// (Three CTAs to an SM at least: 4 prompts of up to 2,048 tokens 17.1 us, at the
+// 106 registers of two CTAs 20.1.)
 template <typename T, int N>
-__global__ void __launch_bounds__(kThreads) append_kernel(AppendArgs p) {
+__global__ void __launch_bounds__(kThreads, 3) append_kernel(AppendArgs p) {
   if (blockIdx.x >= p.main_blocks) {
     // ids, weights (tokens along the lanes, so that a warp writes neighbours)
     // and the new lengths
