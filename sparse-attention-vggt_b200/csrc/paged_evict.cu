@@ -18,12 +18,12 @@
 //    so that every hole and mover knows its number, and writes the lists;
 //  * copies weights and numbers (out of place), then moves the rows, all CTAs
 //    of the cluster taking their share of the list, 16 bytes a lane.
-// What bounds it: one frame out of 32 in 16 heads (21.6 MB) takes 36 us, a chain
+// What bounds it: one frame out of 32 in 16 heads (21.6 MB) takes 34 us, a chain
 // of four passes of 2 us each, two scans and the moves' dependent loads.  16
 // prompts cut from 16,383 to 4,096 tokens (379 MB moved in rows of 256 bytes)
-// take 161 us, 2.4 TB/s: 512 threads a CTA, so that the passes of some CTAs run
-// beside the moves of others (1,024 threads: 190 us; 256: 151 us, but 47 us for
-// the frame).
+// take 101 us, 3.8 TB/s: 512 threads a CTA, so that the passes of some CTAs run
+// beside the moves of others, and the moves' addresses resolved a round ahead of
+// the rows (with every row's look-ups before its copy: 162 us).
 #include <cooperative_groups.h>
 
 #include "kernels.h"
@@ -86,7 +86,7 @@ __device__ __forceinline__ int64_t row_of(const EvictArgs& a, int64_t seq, int h
 template <int C, int D>
 __global__ void __launch_bounds__(kThreads, 4) evict_kernel(const EvictParams p) {
   extern __shared__ uint32_t keys[];
-  __shared__ int copies[256 * kCopies];
+  __shared__ __align__(16) int copies[256 * kCopies];
   __shared__ int hist[2][256], sums[256];
   __shared__ uint64_t warp_sums[32];
   __shared__ uint64_t share[2];  // this CTA's ties; its holes and movers
@@ -268,32 +268,41 @@ __global__ void __launch_bounds__(kThreads, 4) evict_kernel(const EvictParams p)
   });
   sync();  // the lists are complete
 
-  // ---- the rows: D / 8 lanes to a row of K, as many to its row of V ----
-  constexpr int kLanes = D / 4, kBatch = 4, kStep = C * kThreads / kLanes;
+  // ---- the moves: addresses first, a pair a thread, then the rows, D / 8 lanes
+  // to a row of K and as many to its row of V ----
+  static_assert(sizeof(copies) >= 2 * kThreads * sizeof(int64_t), "room for a round's pairs");
+  int64_t* src_at = reinterpret_cast<int64_t*>(copies);
+  int64_t* dst_at = src_at + kThreads;
+  constexpr int kLanes = D / 4, kBatch = 4, kStep = kThreads / kLanes;
   uint4* pages = reinterpret_cast<uint4*>(tid % kLanes < kLanes / 2 ? a.k_pages : a.v_pages);
   const int chunk = tid % (kLanes / 2);
-  for (int i0 = (rank * kThreads + tid) / kLanes; i0 < moves; i0 += kBatch * kStep) {
-    uint4 row[kBatch];
-    int64_t dst[kBatch];
+  // (a round is 512 neighbours, even where that leaves CTAs without: the same
+  // pairs dealt evenly over the cluster took 114 us for the 16 prompts, not 101)
+  for (int base = rank * kThreads; base < moves; base += C * kThreads) {
+    const int here = moves - base < kThreads ? moves - base : kThreads;
+    __syncthreads();
+    if (tid < here) {
+      const int src = movers[base + tid], dst = holes[base + tid];
+      const int64_t from_row = row_of(a, seq, head, src), to_row = row_of(a, seq, head, dst);
+      src_at[tid] = from_row / 8;
+      dst_at[tid] = from_row < 0 || to_row < 0 ? -1 : to_row / 8;
+      w2[dst] = w[src];
+      ids2[dst] = ids[src];
+    }
+    __syncthreads();
+    for (int i0 = tid / kLanes; i0 < here; i0 += kBatch * kStep) {
+      uint4 row[kBatch];
 #pragma unroll
-    for (int j = 0; j < kBatch; ++j) {
-      const int i = i0 + j * kStep;
-      dst[j] = -1;
-      if (i < moves) {
-        const int src_slot = movers[i], dst_slot = holes[i];
-        const int64_t src = row_of(a, seq, head, src_slot);
-        dst[j] = row_of(a, seq, head, dst_slot);
-        if (src < 0) dst[j] = -1;
-        if (dst[j] >= 0) row[j] = pages[src / 8 + chunk];
-        if (tid % kLanes == 0) {
-          w2[dst_slot] = w[src_slot];
-          ids2[dst_slot] = ids[src_slot];
-        }
+      for (int j = 0; j < kBatch; ++j) {
+        const int i = i0 + j * kStep;
+        if (i < here && dst_at[i] >= 0) row[j] = pages[src_at[i] + chunk];
+      }
+#pragma unroll
+      for (int j = 0; j < kBatch; ++j) {
+        const int i = i0 + j * kStep;
+        if (i < here && dst_at[i] >= 0) pages[dst_at[i] + chunk] = row[j];
       }
     }
-#pragma unroll
-    for (int j = 0; j < kBatch; ++j)
-      if (dst[j] >= 0) pages[dst[j] / 8 + chunk] = row[j];
   }
 }
 
