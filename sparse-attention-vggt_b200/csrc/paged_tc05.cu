@@ -61,6 +61,7 @@ constexpr int kLaunchRegs = 128, kControlRegs = 64, kSoftRegs = 192;
 static_assert(kControlRegs + kSoftRegs == 2 * kLaunchRegs, "register split");
 constexpr uint32_t kTmemCols = 256;  // S0 | S1 | O
 constexpr uint64_t kDrainNs = 1000000000ull;
+constexpr int kMaxRuns = 64;  // per row tile
 
 template <int D>
 struct Smem {
@@ -83,9 +84,27 @@ struct TcParams {
   PagedAttnArgs a;
   float scale_log2;
   int64_t tiles, heads, splits, chunk;
-  int* counters;
   float* partial;  // [tiles * heads][splits][128 rows x D, 128 maxima, 128 sums]
 };
+
+// The keys that the last of a tile's `rows` rows sees, cut into runs.
+struct Runs {
+  int64_t tiles, chunk;  // key tiles, and those of a run
+  int count;
+};
+__device__ __forceinline__ Runs runs_of(const TcParams& p, const RowTile& rt, int rows) {
+  int64_t keys = rt.len;
+  if (p.a.causal) {
+    const int64_t n = rt.len - rt.n_new + (rt.row0 + rows - 1) / p.a.group + 1;
+    keys = n < 0 ? 0 : (n < keys ? n : keys);
+  }
+  Runs r;
+  r.tiles = (keys + kTile - 1) / kTile;
+  r.chunk = (r.tiles + p.splits - 1) / p.splits;
+  if (r.chunk < p.chunk) r.chunk = p.chunk;
+  r.count = r.tiles > 0 ? (int)((r.tiles + r.chunk - 1) / r.chunk) : 1;
+  return r;
+}
 
 // column pairs of every 8 whose exponentials take the polynomial
 constexpr unsigned kPolyPairs = 0x01u;
@@ -101,7 +120,7 @@ __global__ void __launch_bounds__(kThreads, 2)
   const uint32_t base = smem_u32(sbase);
   __shared__ Bars bars;
   __shared__ uint32_t s_tmem;
-  __shared__ int s_abort, s_odd, s_last;
+  __shared__ int s_abort, s_odd;
   __shared__ float s_m[kRows], s_l[kRows];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const PagedAttnArgs& a = p.a;
@@ -122,13 +141,11 @@ __global__ void __launch_bounds__(kThreads, 2)
     return n < 0 ? 0 : (n < len ? n : len);
   };
   const int64_t most = limit_of(rows - 1), least = limit_of(0);
-  const int64_t all_tiles = (most + kTile - 1) / kTile;
-  int64_t chunk = (all_tiles + p.splits - 1) / p.splits;
-  if (chunk < p.chunk) chunk = p.chunk;
-  const int64_t runs = all_tiles > 0 ? (all_tiles + chunk - 1) / chunk : 1;
+  const Runs cut = runs_of(p, rt, rows);
+  const int64_t runs = cut.count;
   if (split >= runs) return;
-  const int64_t tile0 = split * chunk;
-  const int tiles = (int)(all_tiles - tile0 < chunk ? all_tiles - tile0 : chunk);
+  const int64_t tile0 = split * cut.chunk;
+  const int tiles = (int)(cut.tiles - tile0 < cut.chunk ? cut.tiles - tile0 : cut.chunk);
 
   volatile int* abort_flag = &s_abort;
   if (tid == 0) {
@@ -550,83 +567,93 @@ __global__ void __launch_bounds__(kThreads, 2)
     }
     sync_softmax();
   }
-  if (runs > 1) {
+  if (runs > 1) {  // the join kernel makes the output of these
     if (stid < rows) {
       mine[kRows * D + stid] = s_m[stid];
       mine[kRows * (D + 1) + stid] = s_l[stid];
     }
-    __threadfence();
-    sync_softmax();
-    if (stid == 0) {
-      s_last = atomicAdd(p.counters + item, 1) == (int)runs - 1;
-      if (s_last) p.counters[item] = 0;
-    }
-    sync_softmax();
-    if (!s_last) return;
-    __threadfence();
-    // the CTA that finishes last joins the runs, in their order
-    const float* from = p.partial + item * p.splits * (int64_t)(kRows * (D + 2));
-    float* wgt = reinterpret_cast<float*>(sbase);  // [runs][128], at most 64 runs
-    if (stid < rows) {
-      float mx = -INFINITY, l = 0.f;
-#pragma unroll 8
-      for (int64_t s = 0; s < runs; ++s)
-        mx = fmaxf(mx, __ldcg(from + s * kRows * (D + 2) + kRows * D + stid));
-      const float b = mx == -INFINITY ? 0.f : mx;
-#pragma unroll 8
-      for (int64_t s = 0; s < runs; ++s) {
-        const float* ml = from + s * kRows * (D + 2) + kRows * D + stid;
-        const float f = fast_exp2(__ldcg(ml) - b);
-        wgt[s * kRows + stid] = f;
-        l += __ldcg(ml + kRows) * f;
-      }
-      s_m[stid] = mx;
-      s_l[stid] = l;
-    }
-    sync_softmax();
-    // 8 vectors per thread and run in flight: one at a time took 18 us
-    constexpr int kBatch = 8;
-    for (int i0 = stid; i0 < rows * (D / 4); i0 += kBatch * kRows) {
-      float4 acc[kBatch];
-#pragma unroll
-      for (int j = 0; j < kBatch; ++j) acc[j] = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 2
-      for (int s = 0; s < (int)runs; ++s) {
-        const float4* src = reinterpret_cast<const float4*>(from + (int64_t)s * kRows * (D + 2));
-        float4 v[kBatch];
-#pragma unroll
-        for (int j = 0; j < kBatch; ++j) {
-          const int i = i0 + j * kRows;
-          v[j] = i < rows * (D / 4) ? __ldcg(src + i) : make_float4(0.f, 0.f, 0.f, 0.f);
-        }
-#pragma unroll
-        for (int j = 0; j < kBatch; ++j) {
-          const float f = wgt[s * kRows + (i0 + j * kRows) / (D / 4) % kRows];
-          acc[j].x = fmaf(f, v[j].x, acc[j].x);
-          acc[j].y = fmaf(f, v[j].y, acc[j].y);
-          acc[j].z = fmaf(f, v[j].z, acc[j].z);
-          acc[j].w = fmaf(f, v[j].w, acc[j].w);
-        }
-      }
-#pragma unroll
-      for (int j = 0; j < kBatch; ++j) {
-        const int i = i0 + j * kRows, r = i / (D / 4), d = (i % (D / 4)) * 4;
-        if (r >= rows) break;
-        const float l = s_l[r], inv = l == 0.f ? 0.f : 1.f / l;
-        const int q = rt.row0 + r;
-        T* dst = static_cast<T*>(a.out) + (rt.first + q / a.group) * a.o_token +
-                 ((int64_t)head * a.group + q % a.group) * a.o_head + d;
-        *reinterpret_cast<uint2*>(dst) =
-            make_uint2(ElemOps<T>::pack2(acc[j].x * inv, acc[j].y * inv),
-                       ElemOps<T>::pack2(acc[j].z * inv, acc[j].w * inv));
-      }
-    }
+    return;
   }
   if (a.lse != nullptr && stid < rows) {
     const int q = rt.row0 + stid;
     a.lse[(rt.first + q / a.group) * (p.heads * a.group) + (int64_t)head * a.group + q % a.group] =
         s_l[stid] == 0.f ? -INFINITY : (s_m[stid] + log2f(s_l[stid])) * 0.6931471805599453f;
   }
+}
+
+// Joins the runs of a row tile, in their order: a CTA takes 512 / D rows of an
+// item, a thread 4 of their elements, 8 runs' loads in flight.  A launch of its
+// own, since it spreads over the card: the CTA that finished last took 10 us
+// for 5 runs of dim 64 and 40 for 40 runs of dim 128.
+constexpr int kJoinThreads = 128;
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kJoinThreads)
+    join_runs_kernel(const __grid_constant__ TcParams p) {
+  constexpr int kHere = 4 * kJoinThreads / D;  // rows
+  constexpr int64_t kRun = kRows * (D + 2);
+  __shared__ float wgt[kMaxRuns][kHere], sums[kMaxRuns][kHere], inv_l[kHere];
+  const PagedAttnArgs& a = p.a;
+  const int64_t item = blockIdx.x / (kRows / kHere);
+  const int r0 = (int)(blockIdx.x % (kRows / kHere)) * kHere, tid = threadIdx.x;
+  const int head = (int)(item / p.tiles);
+  RowTile rt;
+  if (!locate_tile(a.t, a.pool, a.group, kRows, item % p.tiles, rt)) return;
+  const int in_tile = rt.rows - rt.row0 < kRows ? rt.rows - rt.row0 : kRows;
+  const int rows = in_tile - r0 < kHere ? in_tile - r0 : kHere;
+  const int count = runs_of(p, rt, in_tile).count;
+  if (rows <= 0 || count == 1) return;
+  const float* from = p.partial + item * p.splits * kRun;
+  for (int i = tid; i < count * kHere; i += kJoinThreads) {
+    const int s = i / kHere, r = i % kHere;
+    if (r < rows) {
+      wgt[s][r] = from[s * kRun + kRows * D + r0 + r];
+      sums[s][r] = from[s * kRun + kRows * (D + 1) + r0 + r];
+    }
+  }
+  __syncthreads();
+  if (tid < rows) {
+    float mx = -INFINITY, l = 0.f;
+    for (int s = 0; s < count; ++s) mx = fmaxf(mx, wgt[s][tid]);
+    const float b = mx == -INFINITY ? 0.f : mx;
+    for (int s = 0; s < count; ++s) {
+      const float f = fast_exp2(wgt[s][tid] - b);
+      wgt[s][tid] = f;
+      l = fmaf(f, sums[s][tid], l);
+    }
+    inv_l[tid] = l == 0.f ? 0.f : 1.f / l;
+    if (a.lse != nullptr) {
+      const int q = rt.row0 + r0 + tid;
+      a.lse[(rt.first + q / a.group) * (p.heads * a.group) + (int64_t)head * a.group +
+            q % a.group] = l == 0.f ? -INFINITY : (mx + log2f(l)) * 0.6931471805599453f;
+    }
+  }
+  __syncthreads();
+  const int r = tid / (D / 4), d = (tid % (D / 4)) * 4;
+  if (r >= rows) return;
+  const float* mine = from + (r0 + r) * D + d;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int s0 = 0; s0 < count; s0 += 8) {
+    float4 v[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (s0 + j < count) v[j] = *reinterpret_cast<const float4*>(mine + (s0 + j) * kRun);
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (s0 + j < count) {
+        const float f = wgt[s0 + j][r];
+        acc.x = fmaf(f, v[j].x, acc.x);
+        acc.y = fmaf(f, v[j].y, acc.y);
+        acc.z = fmaf(f, v[j].z, acc.z);
+        acc.w = fmaf(f, v[j].w, acc.w);
+      }
+  }
+  const float inv = inv_l[r];
+  const int q = rt.row0 + r0 + r;
+  T* dst = static_cast<T*>(a.out) + (rt.first + q / a.group) * a.o_token +
+           ((int64_t)head * a.group + q % a.group) * a.o_head + d;
+  *reinterpret_cast<uint2*>(dst) = make_uint2(ElemOps<T>::pack2(acc.x * inv, acc.y * inv),
+                                              ElemOps<T>::pack2(acc.z * inv, acc.w * inv));
 }
 
 template <typename T, int D>
@@ -642,6 +669,10 @@ cudaError_t launch_tc05(const TcParams& p, const CUtensorMap& mk, const CUtensor
       cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
   if (e != cudaSuccess) return e;
   kernel<<<(unsigned)(p.tiles * p.heads * p.splits), kThreads, smem, st>>>(mk, mv, p);
+  const cudaError_t launched = cudaGetLastError();
+  if (launched != cudaSuccess || p.splits == 1) return launched;
+  join_runs_kernel<T, D>
+      <<<(unsigned)(p.tiles * p.heads * (kRows * D / (4 * kJoinThreads))), kJoinThreads, 0, st>>>(p);
   return cudaGetLastError();
 }
 
@@ -655,15 +686,15 @@ PagedPlan paged_tc05_plan(int64_t total, int64_t seqs, int kv_heads, int group, 
   const int64_t items = plan.tiles * kv_heads, key_tiles = (max_len + kTile - 1) / kTile;
   // Runs per row tile: the number that ends the last wave of 2 CTAs per SM
   // soonest.  In units of a key tile (0.7 us): a CTA's start and end cost ten,
-  // joining the runs of a tile fourteen.  1 frame over 31 cached ones (176
-  // items): 1 run 536 us, 3 runs 387, 5 runs 375, 10 runs 422; 4 prompts
+  // joining the runs eight.  1 frame over 31 cached ones (176 items), the join
+  // in the kernel: 1 run 536 us, 3 runs 387, 5 runs 375, 10 runs 422; 4 prompts
   // (2,024 items): 1 run 1,292 us, 2 runs 1,546.
   plan.splits = 1;
   int64_t best = -1;
   const int64_t slots = 2 * 148;
-  for (int64_t s = 1; s <= 64 && (s == 1 || (items <= kMaxCounters && s <= key_tiles)); ++s) {
+  for (int64_t s = 1; s <= kMaxRuns && s <= (key_tiles > 0 ? key_tiles : 1); ++s) {
     const int64_t waves = (items * s + slots - 1) / slots;
-    const int64_t cost = waves * ((key_tiles + s - 1) / s + 10) + (s > 1 ? 14 : 0);
+    const int64_t cost = waves * ((key_tiles + s - 1) / s + 10) + (s > 1 ? 8 : 0);
     if (best < 0 || cost < best) {
       best = cost;
       plan.splits = s;
@@ -683,7 +714,6 @@ cudaError_t launch_paged_tc05(const PagedAttnArgs& a, const PagedPlan& plan, cud
   p.heads = a.pool.kv_heads;
   p.splits = plan.splits;
   p.chunk = plan.chunk;
-  p.counters = static_cast<int*>(a.workspace);
   p.partial = reinterpret_cast<float*>(static_cast<char*>(a.workspace) + kMaxCounters * 4);
   if (plan.tiles == 0) return cudaSuccess;
   CUtensorMap mk, mv;
