@@ -8,10 +8,11 @@
 // position * step wraps to exactly the fraction that the product has, so the
 // reduction is exact for every 32-bit position (a 32-bit float product
 // position * freq is off by 4e-3 radians at position 65,536).  Its upper 32
-// bits go to sincospif: the angle is then within 2^-24 of a radian or two.
+// bits name the quarter turn and what is left of it, which keeps 24 bits as a
+// float: the angle is within 2^-24 of a radian.
 //
-// Both kernels are bound by memory: every element is read and written once (32
-// frames' queries, 180 MB, in 35.8 us: 5.0 TB/s, 0.79 of the measured copy
+// The kernels are bound by memory: every element is read and written once (32
+// frames' queries, 180 MB, in 34.7 us: 5.2 TB/s, 0.81 of the measured copy
 // rate).
 // A thread owns up to 8 pairs (two 16-byte vectors of a 2-byte type) of a
 // token, takes their sines once and walks over heads with them, four heads'
@@ -77,6 +78,26 @@ struct Vec {
   __device__ __forceinline__ T* e() { return reinterpret_cast<T*>(v); }
 };
 
+// Sine and cosine of `turn` / 2^32 of a turn.  The nearest quarter comes off
+// as an integer, exactly; the rest, at most pi/4, goes through the Taylor
+// series, whose first terms left out are 1.8e-9 (x^11 / 11!) and 1.2e-10
+// (x^12 / 12!).  Odd quarters swap the two, the signs follow the quarter.
+__device__ __forceinline__ void sine(uint32_t turn, float& s, float& c) {
+  const uint32_t quarter = (turn + 0x20000000u) >> 30;
+  const float x = (float)(int32_t)(turn - (quarter << 30)) * 1.4629180792671596e-9f;  // 2 pi / 2^32
+  const float y = x * x;
+  float u = fmaf(y, 1.f / 362880.f, -1.f / 5040.f), w = fmaf(y, -1.f / 3628800.f, 1.f / 40320.f);
+  u = fmaf(y, u, 1.f / 120.f);
+  w = fmaf(y, w, -1.f / 720.f);
+  u = fmaf(y, u, -1.f / 6.f);
+  w = fmaf(y, w, 1.f / 24.f);
+  u = fmaf(x * y, u, x);
+  w = fmaf(y, fmaf(y, w, -0.5f), 1.f);
+  const uint32_t a = __float_as_uint(quarter & 1 ? w : u), b = __float_as_uint(quarter & 1 ? u : w);
+  s = __uint_as_float(a ^ ((quarter << 30) & 0x80000000u));
+  c = __uint_as_float(b ^ (((quarter + 1) << 30) & 0x80000000u));
+}
+
 struct Angles {
   const int32_t* positions;  // [tokens][axes]
   const double* freq;        // [pairs]
@@ -89,18 +110,20 @@ struct Angles {
 template <int N>
 struct Unit {
   int a, b;
-  bool turns;
+  int axis;  // -1: copies
+  uint64_t step[N];
   float c[N], s[N];
 
-  __device__ __forceinline__ Unit(const Angles& g, int64_t token, int unit) {
+  __device__ __forceinline__ Unit(const Angles& g, int unit) {
     const int first = unit * N;  // pair number over all axes
-    turns = first < g.axes * g.pairs;
-    if (!turns) {
+    if (first >= g.axes * g.pairs) {
+      axis = -1;
       a = 2 * first;
       b = a + N;
       return;
     }
-    const int axis = first / g.pairs, i0 = first % g.pairs;
+    axis = first / g.pairs;
+    const int i0 = first % g.pairs;
     if (g.interleaved) {
       a = 2 * first;
       b = a + N;
@@ -108,14 +131,21 @@ struct Unit {
       a = 2 * axis * g.pairs + i0;
       b = a + g.pairs;
     }
-    const uint64_t pos = (uint64_t)(int64_t)__ldg(g.positions + token * g.axes + axis);
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       double t = __ldg(g.freq + i0 + i) * 0.15915494309189535;  // turns per position
       t -= rint(t);
-      const uint64_t step = (uint64_t)__double2ll_rn(t * 9223372036854775808.0) << 1;
-      const int32_t turn = (int32_t)((pos * step) >> 32);
-      sincospif((float)turn * 4.656612873077393e-10f, &s[i], &c[i]);  // 2^-31: half turns
+      step[i] = (uint64_t)__double2ll_rn(t * 9223372036854775808.0) << 1;
+    }
+  }
+
+  // the sines of a token's position
+  __device__ __forceinline__ void at(const Angles& g, int64_t token) {
+    if (axis < 0) return;
+    const uint64_t pos = (uint64_t)(int64_t)__ldg(g.positions + token * g.axes + axis);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      sine((uint32_t)((pos * step[i]) >> 32), s[i], c[i]);
       c[i] *= g.lengthen;
       s[i] *= g.lengthen * g.sign;
     }
@@ -123,7 +153,7 @@ struct Unit {
 
   template <typename T>
   __device__ __forceinline__ void turn(T* x, T* y, bool interleaved) const {
-    if (!turns) return;
+    if (axis < 0) return;
     if (interleaved) {  // pairs lie side by side over both runs
 #pragma unroll
       for (int i = 0; i < N; ++i) {
@@ -144,26 +174,39 @@ struct Unit {
   }
 };
 
+// at / d and at % d, in 32 bits where `at` has no more.
+__device__ __forceinline__ int64_t divided(int64_t at, int d, int& rest) {
+  if ((at >> 32) == 0) {
+    const uint32_t q = (uint32_t)at / (uint32_t)d;
+    rest = (int)((uint32_t)at - q * (uint32_t)d);
+    return q;
+  }
+  const int64_t q = at / d;
+  rest = (int)(at - q * d);
+  return q;
+}
+
+constexpr int kBatch = 4;  // rows of a token or tokens whose loads are in flight together
+
 struct RotaryArgs {
   const void* x;
   void* out;
   int64_t tokens, xt, xh, ot, oh;
   int heads, units, deal;  // units per head; threads that share a token's heads
+  int64_t stride;          // few heads: a thread's tokens are this far apart
   Angles g;
 };
 
 template <typename T, int N>
 __global__ void __launch_bounds__(kThreads) rotary_kernel(RotaryArgs p) {
-  const int64_t at = (int64_t)blockIdx.x * kThreads + threadIdx.x;
-  const int unit = (int)(at % p.units);
-  const int64_t rest = at / p.units;
-  const int part = (int)(rest % p.deal);
-  const int64_t token = rest / p.deal;
+  int unit, part;
+  const int64_t token =
+      divided(divided((int64_t)blockIdx.x * kThreads + threadIdx.x, p.units, unit), p.deal, part);
   if (token >= p.tokens) return;
-  const Unit<N> u(p.g, token, unit);
+  Unit<N> u(p.g, unit);
   const T* x = static_cast<const T*>(p.x) + token * p.xt;
   T* o = static_cast<T*>(p.out) + token * p.ot;
-  constexpr int kBatch = 4;
+#pragma unroll 1
   for (int h0 = part; h0 < p.heads; h0 += kBatch * p.deal) {
     Vec<T, N> a[kBatch], b[kBatch];
 #pragma unroll
@@ -174,6 +217,7 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(RotaryArgs p) {
         b[j].load(x + h * p.xh + u.b);
       }
     }
+    if (h0 == part) u.at(p.g, token);
 #pragma unroll
     for (int j = 0; j < kBatch; ++j) {
       const int64_t h = h0 + j * p.deal;
@@ -182,6 +226,40 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(RotaryArgs p) {
         a[j].store(o + h * p.oh + u.a);
         b[j].store(o + h * p.oh + u.b);
       }
+    }
+  }
+}
+
+// Few heads: a thread takes kBatch tokens of one head, so that as many loads
+// are in flight as with many heads, and the steps are formed once for them.
+// (One head of 64, 703,488 tokens: 53 us, against 99; what is left are the
+// sines, 50 instructions each.)
+template <typename T, int N>
+__global__ void __launch_bounds__(kThreads, sizeof(T) == 4 ? 2 : 3) rotary_few_heads_kernel(RotaryArgs p) {
+  int unit, head;
+  const int64_t first =
+      divided(divided((int64_t)blockIdx.x * kThreads + threadIdx.x, p.units, unit), p.heads, head);
+  if (first >= p.stride) return;
+  Unit<N> u(p.g, unit);
+  const T* x = static_cast<const T*>(p.x) + head * p.xh;
+  T* o = static_cast<T*>(p.out) + head * p.oh;
+  Vec<T, N> a[kBatch], b[kBatch];
+#pragma unroll
+  for (int j = 0; j < kBatch; ++j) {
+    const int64_t token = first + j * p.stride;
+    if (token < p.tokens) {
+      a[j].load(x + token * p.xt + u.a);
+      b[j].load(x + token * p.xt + u.b);
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < kBatch; ++j) {
+    const int64_t token = first + j * p.stride;
+    if (token < p.tokens) {
+      u.at(p.g, token);
+      u.turn(a[j].e(), b[j].e(), p.g.interleaved);
+      a[j].store(o + token * p.ot + u.a);
+      b[j].store(o + token * p.ot + u.b);
     }
   }
 }
@@ -242,24 +320,23 @@ __global__ void __launch_bounds__(kThreads, 3) append_kernel(AppendArgs p) {
     }
     return;
   }
-  const int64_t at = (int64_t)blockIdx.x * kThreads + threadIdx.x;
-  const int unit = (int)(at % p.units);
-  const int64_t rest = at / p.units;
-  const int part = (int)(rest % p.deal);
-  const int64_t row = rest / p.deal;
+  int unit, part;
+  const int64_t row =
+      divided(divided((int64_t)blockIdx.x * kThreads + threadIdx.x, p.units, unit), p.deal, part);
   if (row >= p.t.total) return;
   int64_t seq;
   const int64_t slot = append_slot(p, row, seq);
   if (slot < 0) return;
   const int page = checked_page(p.t, p.pool, seq, slot >> p.pool.page_shift);
   if (page < 0) return;
-  const Unit<N> u(p.g, row, unit);
+  Unit<N> u(p.g, unit);
+  u.at(p.g, row);
   const int64_t dst = page * p.pool.page_stride + (slot & (p.pool.page - 1)) * p.pool.row_stride;
   const T* k = static_cast<const T*>(p.k) + row * p.kt;
   const T* v = static_cast<const T*>(p.v) + row * p.vt;
   T* kp = static_cast<T*>(p.kp) + dst;
   T* vp = static_cast<T*>(p.vp) + dst;
-  constexpr int kBatch = 2;
+  constexpr int kBatch = 2;  // of keys and of values
   for (int h0 = part; h0 < p.pool.kv_heads; h0 += kBatch * p.deal) {
     Vec<T, N> a[kBatch], b[kBatch], c[kBatch], d[kBatch];
 #pragma unroll
@@ -300,21 +377,30 @@ int pairs_per_thread(int size, int dim, int axes, int pairs, std::initializer_li
   return 1;
 }
 
-// Threads that share a token's heads: one, or as many as it takes to give
-// every SM a thousand threads.
+constexpr int64_t kFill = 148 * 1024;  // threads that fill the card
+
+// Threads that share a token's heads: one, or as many as it takes to fill the
+// card.
 int deal_heads(int64_t threads, int heads) {
-  const int64_t want = 148 * 1024;
-  int64_t d = threads > 0 ? (want + threads - 1) / threads : 1;
+  int64_t d = threads > 0 ? (kFill + threads - 1) / threads : 1;
   return (int)(d < 1 ? 1 : (d > heads ? heads : d));
+}
+
+template <typename T, int N>
+void launch_rotary(const RotaryArgs& a, unsigned grid, cudaStream_t st) {
+  if (a.stride < a.tokens)
+    rotary_few_heads_kernel<T, N><<<grid, kThreads, 0, st>>>(a);
+  else
+    rotary_kernel<T, N><<<grid, kThreads, 0, st>>>(a);
 }
 
 template <typename T>
 cudaError_t rotary_n(int n, const RotaryArgs& a, unsigned grid, cudaStream_t st) {
   switch (n) {
-    case 8: rotary_kernel<T, 8><<<grid, kThreads, 0, st>>>(a); break;
-    case 4: rotary_kernel<T, 4><<<grid, kThreads, 0, st>>>(a); break;
-    case 2: rotary_kernel<T, 2><<<grid, kThreads, 0, st>>>(a); break;
-    default: rotary_kernel<T, 1><<<grid, kThreads, 0, st>>>(a); break;
+    case 8: launch_rotary<T, 8>(a, grid, st); break;
+    case 4: launch_rotary<T, 4>(a, grid, st); break;
+    case 2: launch_rotary<T, 2>(a, grid, st); break;
+    default: launch_rotary<T, 1>(a, grid, st); break;
   }
   return cudaGetLastError();
 }
@@ -369,11 +455,17 @@ extern "C" int vggt_rotary(const void* x, int dtype, int64_t tokens, int heads, 
                                  {x_token_stride, x_head_stride, out_token_stride, out_head_stride},
                                  {x, out});
   RotaryArgs a{x, out, tokens, x_token_stride, x_head_stride, out_token_stride, out_head_stride,
-               heads, dim / (2 * n), 1,
+               heads, dim / (2 * n), 1, tokens,
                {positions, freq, axes, pairs, layout == VGGT_ROTARY_INTERLEAVED, lengthen,
                 inverse ? -1.f : 1.f}};
   a.deal = deal_heads(tokens * a.units, heads);
-  const int64_t grid = (tokens * a.units * a.deal + kThreads - 1) / kThreads;
+  // Half a batch of heads at most (two heads: 53 against 64 us; three: 52
+  // against 42), and tokens that fill the card with a thread for each
+  if (heads <= kBatch / 2 && tokens * a.units * heads >= kFill) {
+    a.stride = (tokens + kBatch - 1) / kBatch;
+    a.deal = heads;
+  }
+  const int64_t grid = (a.stride * a.units * a.deal + kThreads - 1) / kThreads;
   if (grid > 0x7fffffffLL) return api_fail("too many tokens (%lld)", (long long)tokens);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   return api_cuda(dtype == VGGT_DTYPE_FP32   ? rotary_n<float>(n, a, (unsigned)grid, st)

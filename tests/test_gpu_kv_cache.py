@@ -175,6 +175,34 @@ def test_rotary(cuda, t, h, d, rot, axes, layout, dtype, inverse):
     assert torch.equal(got[..., rot:], x[..., rot:].double())
 
 
+@pytest.mark.parametrize("t,h,d,rot,axes,layout,dtype", [
+    (40003, 1, 64, 64, 1, "half", BF), (40003, 1, 64, 32, 1, "interleaved", FP),
+    (20001, 2, 128, 128, 2, "half", torch.float32), (9999, 2, 72, 12, 2, "interleaved", BF),
+    (160000, 1, 6, 2, 1, "half", FP), (37886, 1, 64, 64, 1, "half", BF)])
+def test_rotary_many_tokens_of_few_heads(cuda, t, h, d, rot, axes, layout, dtype):
+    """Several tokens to a thread, and odd numbers of them; every eighth of a
+    turn and its neighbours are among the angles."""
+    g = torch.Generator().manual_seed(t)
+    wide = torch.randn(t, h + 1, d + 8, generator=g).to(dtype).to(cuda)
+    x = wide[:, 1:, :d]
+    pos = torch.randint(-70000, 70000, (t, axes), generator=g)
+    pos[:4096] = torch.arange(-2048, 2048)[:, None]
+    pos = pos.to(torch.int32).to(cuda)
+    freq, lengthen = vggt_sparse.rotary_frequencies(rot, axes=axes)
+    freq = freq.clone()
+    freq[0] = 2 * math.pi / 8
+    freq[-1] = 2 * math.pi / 4096
+    pos = pos if axes > 1 else pos[:, 0].contiguous()
+    want = turned(x, pos, freq, lengthen, layout)
+    got = vggt_sparse.rotary(x, pos, freq, layout=layout, lengthen=lengthen)
+    size = 1.5 * x.double().abs().amax(-1, keepdim=True)
+    err = (got.double() - want).abs()
+    assert bool((err <= U[dtype] * want.abs() + 2.0 ** -21 * size).all())
+    assert torch.equal(got[..., rot:], x[..., rot:])
+    assert torch.equal(vggt_sparse.rotary(x, pos, freq, layout=layout, lengthen=lengthen, out=x), got)
+    assert not torch.isnan(wide).any()
+
+
 def test_rotary_in_place_and_gradient(cuda):
     """In place gives the same bits; the inverse is the transposed map (the
     gradient), checked by a difference quotient: the map is linear."""
