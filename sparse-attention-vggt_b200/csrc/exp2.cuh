@@ -23,6 +23,11 @@ __device__ __forceinline__ float_pair fma_pair(float_pair a, float_pair b, float
   asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
   return r;
 }
+__device__ __forceinline__ float_pair mul_pair(float_pair a, float_pair b) {
+  float_pair r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
 __device__ __forceinline__ float_pair add_pair(float_pair a, float_pair b) {
   float_pair r;
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
@@ -34,11 +39,17 @@ __device__ __forceinline__ float_pair sub_pair(float_pair a, float_pair b) {
   return r;
 }
 
-// 2^a, 2^b for arguments up to 126 without the multi-function unit: x = n + f
-// with n = round(x) (adding 1.5 * 2^23 leaves it in the low mantissa bits), a
-// polynomial of degree 4 for 2^f on [-1/2, 1/2] (fitted to the least largest
-// relative error, 2.7e-6 in fp32), n added to its exponent.  Arguments below
-// -126 give 2^-126 at most.
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
+
+// 2^x of a pair for arguments up to 126 without the multi-function unit, as
+// q * scale: x = n + f with n = round(x) (adding 1.5 * 2^23 leaves it in the low
+// mantissa bits), q a polynomial of degree 4 for 2^f on [-1/2, 1/2] (fitted to
+// the least largest relative error, 2.7e-6 in fp32), scale = 2^n.  Arguments
+// below -126 give 2^-126 at most; a NaN stays one (in q).
 struct Exp2Poly {
   float_pair magic, c4, c3, c2, c1, c0;
   __device__ __forceinline__ Exp2Poly()
@@ -48,28 +59,22 @@ struct Exp2Poly {
         c2(pack_pair(0.2402474433f, 0.2402474433f)),
         c1(pack_pair(0.6931217909f, 0.6931217909f)),
         c0(pack_pair(0.9999992847f, 0.9999992847f)) {}
-  __device__ __forceinline__ void operator()(float& ea, float& eb, float_pair x) const {
-    float a, b, ta, tb, qa, qb;
+  __device__ __forceinline__ void operator()(float_pair& q, float_pair& scale, float_pair x) const {
+    float a, b, ta, tb;
     unpack_pair(a, b, x);
-    x = pack_pair(fmaxf(a, -126.f), fmaxf(b, -126.f));
+    x = pack_pair(max_nan(a, -126.f), max_nan(b, -126.f));
     const float_pair t = add_pair(x, magic);
     const float_pair f = sub_pair(x, sub_pair(t, magic));
-    float_pair q = fma_pair(f, c4, c3);
+    q = fma_pair(f, c4, c3);
     q = fma_pair(q, f, c2);
     q = fma_pair(q, f, c1);
     q = fma_pair(q, f, c0);
-    unpack_pair(qa, qb, q);
     unpack_pair(ta, tb, t);
-    ea = __int_as_float(__float_as_int(qa) + (__float_as_int(ta) << 23));
-    eb = __int_as_float(__float_as_int(qb) + (__float_as_int(tb) << 23));
+    // of a NaN the exponent is any
+    scale = pack_pair(__int_as_float((__float_as_int(ta) << 23) + 0x3f800000),
+                      __int_as_float((__float_as_int(tb) << 23) + 0x3f800000));
   }
 };
-
-__device__ __forceinline__ float max_nan(float a, float b) {
-  float d;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
-  return d;
-}
 
 // Maximum of three that keeps a NaN.
 __device__ __forceinline__ float max3_nan(float a, float b, float c) {

@@ -473,7 +473,9 @@ __global__ void __launch_bounds__(kThreads, 2)
             pack_pair(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])), c2, minus);
         float ea, eb;
         if ((kPolyPairs >> (i & 7)) & 1u) {
-          poly(ea, eb, x);
+          float_pair q, scale;
+          poly(q, scale, x);
+          unpack_pair(ea, eb, mul_pair(q, scale));
         } else {
           unpack_pair(ea, eb, x);
           ea = fast_exp2(ea);

@@ -361,15 +361,15 @@ __global__ void __launch_bounds__(kThreads, 2)
             const float_pair x = fma_pair(pack_pair(__uint_as_float(sc[2 * (i + j)]),
                                                     __uint_as_float(sc[2 * (i + j) + 1])),
                                           c2, j ? pack_pair(m.z, m.w) : pack_pair(m.x, m.y));
-            float ea, eb;
             if ((kPolyPairs >> ((i + j) & 7)) & 1u) {
-              poly(ea, eb, x);
+              float_pair q, scale;
+              poly(q, scale, x);
+              sum[j] = fma_pair(q, scale, sum[j]);
             } else {
+              float ea, eb;
               unpack_pair(ea, eb, x);
-              ea = fast_exp2(ea);
-              eb = fast_exp2(eb);
+              sum[j] = add_pair(sum[j], pack_pair(fast_exp2(ea), fast_exp2(eb)));
             }
-            sum[j] = add_pair(sum[j], pack_pair(ea, eb));
           }
         }
       }

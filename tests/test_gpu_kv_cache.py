@@ -359,6 +359,25 @@ def test_attention_later_tokens_do_not_reach_earlier_rows(cuda, new, dim):
     assert torch.equal(out[full:], out0[full:])
 
 
+@pytest.mark.parametrize("new", [4, 70])
+def test_attention_infinite_score_spoils_its_row(cuda, new):
+    """A score of +inf makes the row's probabilities inf - inf, in whichever
+    column of a tile it stands; rows that do not see the key stay as they are."""
+    c = Case(cuda, [100], [new], 1, 1, 64, 16, FP)
+    c.q[..., 0] = c.q[..., 0].abs() + 1
+    clean, _ = c.attend(True)
+    for j in [*range(20), 63, 64, 97, 99]:
+        at = int(c.table[0, j // 16]), 0, j % 16, 0
+        old = c.kp[at].clone()
+        c.kp[at] = math.inf
+        out, lse = c.attend(True)
+        c.kp[at] = old
+        first = max(0, j - (100 - new))
+        assert bool(torch.isnan(out[first:]).all()), j
+        assert not torch.isfinite(lse[first:]).any(), j
+        assert torch.equal(out[:first], clean[:first]), j
+
+
 def test_attention_infinite_value_is_seen(cuda):
     c = Case(cuda, [100], [1], 1, 1, 64, 16, FP)
     p = int(c.table[0, 2])
@@ -486,6 +505,30 @@ def test_weights_rows_without_keys_and_odd_keys(cuda, max_new):
     vggt_sparse.paged_weights(c.q, lse, c.kp, c.table, c.len, c.starts, w, max_new=max_new)
     assert bool(torch.isnan(w[0, 0, 2])) and int(torch.isnan(w).sum()) == 1
     assert abs(float(w[1].sum()) - 3 * 2) <= 1e-4
+
+
+@pytest.mark.parametrize("max_new", [1, 500])
+def test_weights_odd_rows_and_scores(cuda, max_new):
+    """A NaN row spoils the weights of all keys that it sees, a score of +inf
+    that of its key, in whichever column of a tile they stand."""
+    c = Case(cuda, [100], [60], 1, 1, 64, 16)
+    c.q[..., 0] = c.q[..., 0].abs() + 1
+    _, lse = c.attend(True)
+
+    def weights(q, lse):
+        w = torch.zeros(1, 1, c.table.shape[1] * 16, device=cuda)
+        vggt_sparse.paged_weights(q, lse, c.kp, c.table, c.len, c.starts, w, max_new=max_new)
+        return torch.isnan(w[0, 0, :100])
+
+    j = torch.arange(100, device=cuda)
+    for r in range(60):
+        q = c.q.clone()
+        q[r] = math.nan
+        assert torch.equal(weights(q, lse), j <= 40 + r), r
+    at = int(c.table[0, 99 // 16]), 0, 99 % 16, 0
+    c.kp[at] = math.inf  # only the last row sees it
+    lse[59] = math.inf
+    assert torch.equal(weights(c.q, lse), j == 99)
 
 
 # ------------------------------------------------------------------ eviction
