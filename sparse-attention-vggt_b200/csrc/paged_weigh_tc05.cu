@@ -16,11 +16,14 @@
 // tiles for each; two CTAs share an SM.
 //
 // What bounds it: 128 x 128 exponentials cost the multi-function unit 1,024
-// clocks, the MMAs 256 (dim 64) or 512; so two column pairs of eight take a
+// clocks, the MMAs 256 (dim 64) or 512; so three column pairs of eight take a
 // polynomial (error 2.7e-6) on the FMA pipe.  One frame of 1,374 tokens over
-// 43,968 keys in 16 heads: 341 us (354 at one pair of eight, 345 at three);
+// 43,968 keys in 16 heads: 333 us (338 at two pairs of eight, 355 at four);
 // without any exponential the same kernel takes 243 us, with loads of S alone
-// 169 us.  Eight exponential warps instead of four were slower (356 us).
+// 169 us.  Two exponential warps share an SM's quarter; 32 columns take the two
+// some 600 clocks, where the unit needs 320 and the packed instructions as
+// much: they wait for one another's results.  Eight exponential warps instead
+// of four were slower (356 us).
 #include <cuda.h>
 
 #include <type_traits>
@@ -38,7 +41,7 @@ constexpr int kLseStages = 4;
 constexpr uint32_t kTmemCols = 256;
 constexpr uint64_t kDrainNs = 1000000000ull;
 // column pairs of every 8 whose exponentials take the polynomial
-constexpr unsigned kPolyPairs = 0x11u;
+constexpr unsigned kPolyPairs = 0x49u;
 
 template <int D>
 struct Smem {
