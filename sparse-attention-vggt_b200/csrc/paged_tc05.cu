@@ -15,7 +15,8 @@
 // wait and elect a lane to issue: on this chip a wait on a barrier costs a
 // warp some 150 clocks even where it is satisfied, and the issue of four MMAs
 // 200 to 300, so that one warp's four steps per tile took longer than the
-// tile's softmax (510 us for a frame over 31 cached ones against 375).
+// tile's softmax (510 us for a frame over 31 cached ones against 375, both
+// before the steps below; 340 now).
 //
 // The row's reference maximum moves only when a tile's maximum exceeds it by
 // more than 2^8 in the exp2 domain; O is rescaled then.  Sums are fp32, of the
@@ -26,10 +27,16 @@
 // SM, so a 128 x 64 tile costs 512 clocks there, against 320 (dim 64) or 640
 // (dim 128) of MMA (A from shared memory takes 48 clocks per MMA at N = 64, 32
 // from TMEM).  One column pair of eight therefore takes a polynomial on the
-// FMA pipe; at two of eight the instructions cost what the unit saves (374
-// against 381 us).  A tile takes 650 clocks: the softmax warps' own chain
+// FMA pipe (at two of eight dim 64 gains nothing and dim 128 loses: 462 us for
+// its frame against 451).  A tile takes 650 clocks: the softmax warps' own chain
 // (wait, load, maximum, exponentials, store) is not fully covered by the other
-// CTA's.  Tried and slower: 32 keys per thread and 8 softmax warps (404 us),
+// CTA's.  A CTA's start and end are 12,000 clocks of latency (sequence look-up,
+// set-up, Q, the first product, the last one, the output), which short caches
+// feel most: Q is loaded and the output stored with a row's pieces in
+// neighbouring lanes, the row arithmetic is in 32 bits, and the output's loop
+// is not unrolled, since instructions that run once come from afar (729 tokens
+// of 3 sequences, 64 heads of 128: 82 us before, 73 after).
+// Tried and slower: 32 keys per thread and 8 softmax warps (404 us),
 // 128-key tiles with one S buffer (449 us), the next tile's maximum between
 // the exponentials (634 us: its small TMEM loads wait for the stores), no
 // maximum but a check of the tile's sum (388 us).
@@ -83,31 +90,32 @@ struct Bars {
 struct TcParams {
   PagedAttnArgs a;
   float scale_log2;
-  int64_t tiles, heads, splits, chunk;
-  float* partial;  // [tiles * heads][splits][128 rows x D, 128 maxima, 128 sums]
+  int tiles, heads, splits, chunk;
+  float* partial;  // [tiles * heads][splits] of [D / 4][128 rows][4], 128 maxima, 128 sums
 };
 
 // The keys that the last of a tile's `rows` rows sees, cut into runs.
 struct Runs {
-  int64_t tiles, chunk;  // key tiles, and those of a run
-  int count;
+  int tiles, chunk, count;  // key tiles, and those of a run
 };
+// Keys that row `r` of the tile sees.
+__device__ __forceinline__ int keys_of(const PagedAttnArgs& a, const RowTile& rt, int r) {
+  const int len = (int)rt.len;
+  if (!a.causal) return len;
+  const int n = len - rt.n_new + (rt.row0 + r) / a.group + 1;
+  return n < 0 ? 0 : (n < len ? n : len);
+}
 __device__ __forceinline__ Runs runs_of(const TcParams& p, const RowTile& rt, int rows) {
-  int64_t keys = rt.len;
-  if (p.a.causal) {
-    const int64_t n = rt.len - rt.n_new + (rt.row0 + rows - 1) / p.a.group + 1;
-    keys = n < 0 ? 0 : (n < keys ? n : keys);
-  }
   Runs r;
-  r.tiles = (keys + kTile - 1) / kTile;
+  r.tiles = (int)(((unsigned)keys_of(p.a, rt, rows - 1) + kTile - 1) / kTile);
   r.chunk = (r.tiles + p.splits - 1) / p.splits;
   if (r.chunk < p.chunk) r.chunk = p.chunk;
-  r.count = r.tiles > 0 ? (int)((r.tiles + r.chunk - 1) / r.chunk) : 1;
+  r.count = r.tiles > 0 ? (r.tiles + r.chunk - 1) / r.chunk : 1;
   return r;
 }
 
 // column pairs of every 8 whose exponentials take the polynomial
-constexpr unsigned kPolyPairs = 0x01u;
+constexpr unsigned kPolyPairs = 0x80u;
 
 template <typename T, int D>
 __global__ void __launch_bounds__(kThreads, 2)
@@ -126,26 +134,40 @@ __global__ void __launch_bounds__(kThreads, 2)
   const PagedAttnArgs& a = p.a;
 
   // ---- rows and keys of this CTA; the tiles with most keys come first ----
-  const int64_t split = blockIdx.x % p.splits;
-  const int64_t w = blockIdx.x / p.splits;
-  const int head = (int)(w / p.tiles);
-  const int64_t tile = p.tiles - 1 - w % p.tiles;
-  const int64_t item = head * p.tiles + tile;
+  const int split = (int)(blockIdx.x % (unsigned)p.splits);
+  const unsigned w = blockIdx.x / (unsigned)p.splits;
+  const int head = (int)(w / (unsigned)p.tiles);
+  const int tile = p.tiles - 1 - (int)(w % (unsigned)p.tiles);
+  const int64_t item = (int64_t)head * p.tiles + tile;
   RowTile rt;
   if (!locate_tile(a.t, a.pool, a.group, kRows, tile, rt)) return;
-  const int64_t len = rt.len;
   const int rows = rt.rows - rt.row0 < kRows ? rt.rows - rt.row0 : kRows;
-  auto limit_of = [&](int r) -> int64_t {
-    if (!a.causal) return len;
-    const int64_t n = len - rt.n_new + (rt.row0 + r) / a.group + 1;
-    return n < 0 ? 0 : (n < len ? n : len);
-  };
-  const int64_t most = limit_of(rows - 1), least = limit_of(0);
   const Runs cut = runs_of(p, rt, rows);
-  const int64_t runs = cut.count;
+  const int runs = cut.count;
   if (split >= runs) return;
-  const int64_t tile0 = split * cut.chunk;
-  const int tiles = (int)(cut.tiles - tile0 < cut.chunk ? cut.tiles - tile0 : cut.chunk);
+  const int first_key = split * cut.chunk * kTile;
+  const int tiles = min(cut.tiles - split * cut.chunk, cut.chunk);
+
+  // The softmax warps' rows of Q, a row's 16-byte pieces in neighbouring lanes:
+  // on their way while the CTA sets up
+  constexpr int kPieces = D / 8, kAtOnce = 32 / kPieces;  // of a row; rows per instruction
+  const int row = (warp & 3) * 32 + lane, piece = lane % kPieces;
+  uint4 q_in[kPieces];
+  if (warp >= 4) {
+    const int r = rt.row0 + (row < rows ? row : 0);
+    const int64_t mine = (rt.first + r / a.group) * a.q_token +
+                         ((int64_t)head * a.group + r % a.group) * a.q_head;
+#pragma unroll
+    for (int k = 0; k < kPieces; ++k) {
+      const int64_t at = __shfl_sync(0xffffffffu, mine, k * kAtOnce + lane / kPieces);
+      q_in[k] = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + at) + piece);
+    }
+  }
+  // Where piece c of row r lies: halves of 64 elements, 128-byte swizzle, as
+  // the MMA reads Q
+  auto piece_at = [&](int r, int c) -> uint32_t {
+    return base + L::kQ + (c >> 3) * (kRows * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4);
+  };
 
   volatile int* abort_flag = &s_abort;
   if (tid == 0) {
@@ -182,7 +204,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kControlRegs));
     if (warp == 0) {
     // ================= TMA producer =================
-    const int keys = (int)(most - tile0 * kTile);  // to the end of the last row's keys
+    const int keys = keys_of(a, rt, rows - 1) - first_key;  // to the end of the last row's keys
     auto produce = [&](auto boxes_) {
       constexpr int kBoxes = decltype(boxes_)::value;  // boxes per tile
       constexpr int kBox = kTile / kBoxes;             // slots per box
@@ -190,8 +212,7 @@ __global__ void __launch_bounds__(kThreads, 2)
       const uint32_t full0 = smem_u32(&bars.full[0][0]), empty0 = smem_u32(&bars.empty[0][0]);
       constexpr uint32_t kToV = sizeof(bars.full[0]);  // from K's barriers to V's
       const int32_t* table = a.t.table + rt.seq * a.t.width;
-      const int64_t first_slot = tile0 * kTile;
-      const int in_page = (int)first_slot & (a.pool.page - 1), page_mask = a.pool.page - 1;
+      const int in_page = first_key & (a.pool.page - 1), page_mask = a.pool.page - 1;
       int page = 0, stage = 0;
       int issued_at[2] = {0, 0};  // of the elected lane
       uint32_t phase = 1;
@@ -202,7 +223,7 @@ __global__ void __launch_bounds__(kThreads, 2)
           const int key = key0 + lane * kBox;
           page = (int)a.pool.n_pages;  // past the pool: reads as zeros
           if (key < keys && key < tiles * kTile) {
-            const int got = __ldg(table + ((first_slot + key) >> a.pool.page_shift));
+            const int got = __ldg(table + ((first_key + key) >> a.pool.page_shift));
             if (got >= 0 && got < a.pool.n_pages)
               page = got;
             else
@@ -343,34 +364,27 @@ __global__ void __launch_bounds__(kThreads, 2)
   {
     // ================= softmax: one query row per thread =================
     const int sub = warp & 3;  // TMEM lane quarter of this warp
-    const int row = sub * 32 + lane;
     const uint32_t lane_off = (uint32_t)(sub * 32) << 16;
     const float c = p.scale_log2;
-    const int64_t lim = limit_of(row < rows ? row : 0);  // a spare row masks nothing new
-    {
-      const int r = rt.row0 + (row < rows ? row : 0);
-      const uint4* src = reinterpret_cast<const uint4*>(
-          static_cast<const T*>(a.q) + (rt.first + r / a.group) * a.q_token +
-          ((int64_t)head * a.group + r % a.group) * a.q_head);
 #pragma unroll
-      for (int k = 0; k < D / 8; ++k) {
-        const uint4 v = __ldg(src + k);
-        const uint32_t dst = base + L::kQ + (k >> 3) * (kRows * 128) + row * 128 +
-                             (((k & 7) ^ (row & 7)) << 4);
-        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "r"(v.x), "r"(v.y),
-                     "r"(v.z), "r"(v.w)
-                     : "memory");
-      }
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      tc::mbar_arrive(smem_u32(&bars.q_full));
+    for (int k = 0; k < kPieces; ++k) {
+      const uint4 v = q_in[k];
+      asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(
+                       piece_at(sub * 32 + k * kAtOnce + lane / kPieces, piece)),
+                   "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w)
+                   : "memory");
     }
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    tc::mbar_arrive(smem_u32(&bars.q_full));
     // counted from the run's first key, within one tile of its ends
     const int span = tiles * kTile;
-    auto within = [&](int64_t key) {
-      const int64_t n = key - tile0 * kTile;
-      return (int)(n < 0 ? 0 : (n < span ? n : span));
+    auto within = [&](int key) {
+      const int n = key - first_key;
+      return n < 0 ? 0 : (n < span ? n : span);
     };
-    const int lim_at = within(lim), least_at = within(least), most_at = within(most);
+    // a spare row masks nothing new
+    const int lim_at = within(keys_of(a, rt, row < rows ? row : 0));
+    const int least_at = within(keys_of(a, rt, 0)), most_at = within(keys_of(a, rt, rows - 1));
     const uint32_t sfull0 = smem_u32(&bars.s_full[0]), pfull0 = smem_u32(&bars.p_full[0]);
     auto wait = [&](uint32_t bar, uint32_t parity) {
       return tc::warp_wait(bar, parity, abort_flag, a.wait_ns);
@@ -500,14 +514,10 @@ __global__ void __launch_bounds__(kThreads, 2)
     s_m[row] = m_ref * c;
     s_l[row] = l;
     const float inv = runs > 1 ? 1.f : (l == 0.f ? 0.f : 1.f / l);
-    float* part = p.partial + (item * p.splits + split) * (int64_t)(kRows * (D + 2)) + row * D;
-    T* dst = nullptr;
-    if (row < rows) {
-      const int r = rt.row0 + row;
-      dst = static_cast<T*>(a.out) + (rt.first + r / a.group) * a.o_token +
-            ((int64_t)head * a.group + r % a.group) * a.o_head;
-    }
-#pragma unroll
+    float4* part = reinterpret_cast<float4*>(
+                       p.partial + (item * p.splits + split) * (int64_t)(kRows * (D + 2))) +
+                   row;
+#pragma unroll 1  // run once: its instructions come from afar, few are faster
     for (int h = 0; h < D / 32; ++h) {
       uint32_t r[32];
       if (have) {
@@ -517,23 +527,43 @@ __global__ void __launch_bounds__(kThreads, 2)
 #pragma unroll
         for (int i = 0; i < 32; ++i) r[i] = 0u;
       }
-      if (row < rows) {
-        if (runs > 1) {
+      const float* f = reinterpret_cast<const float*>(r);
+      if (runs > 1) {
+        if (row < rows) {
 #pragma unroll
           for (int i = 0; i < 8; ++i)
-            reinterpret_cast<uint4*>(part + 32 * h)[i] =
-                make_uint4(r[4 * i], r[4 * i + 1], r[4 * i + 2], r[4 * i + 3]);
-        } else {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float* f = reinterpret_cast<const float*>(r) + 8 * i;
-            reinterpret_cast<uint4*>(dst + 32 * h)[i] =
-                make_uint4(ElemOps<T>::pack2(f[0] * inv, f[1] * inv),
-                           ElemOps<T>::pack2(f[2] * inv, f[3] * inv),
-                           ElemOps<T>::pack2(f[4] * inv, f[5] * inv),
-                           ElemOps<T>::pack2(f[6] * inv, f[7] * inv));
-          }
+            part[(8 * h + i) * kRows] =
+                make_float4(f[4 * i], f[4 * i + 1], f[4 * i + 2], f[4 * i + 3]);
         }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i, f += 8)
+          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(piece_at(row, 4 * h + i)),
+                       "r"(ElemOps<T>::pack2(f[0] * inv, f[1] * inv)),
+                       "r"(ElemOps<T>::pack2(f[2] * inv, f[3] * inv)),
+                       "r"(ElemOps<T>::pack2(f[4] * inv, f[5] * inv)),
+                       "r"(ElemOps<T>::pack2(f[6] * inv, f[7] * inv))
+                       : "memory");
+      }
+    }
+    if (runs == 1) {
+      // through Q's place, which no MMA reads any more, so that neighbouring
+      // lanes store neighbouring pieces
+      const int r = rt.row0 + (row < rows ? row : 0);
+      const int64_t mine = (rt.first + r / a.group) * a.o_token +
+                           ((int64_t)head * a.group + r % a.group) * a.o_head;
+      __syncwarp();
+#pragma unroll 4
+      for (int k = 0; k < kPieces; ++k) {
+        const int from = k * kAtOnce + lane / kPieces;
+        const int64_t at = __shfl_sync(0xffffffffu, mine, from);
+        uint4 v;
+        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                     : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                     : "r"(piece_at(sub * 32 + from, piece))
+                     : "memory");
+        if (sub * 32 + from < rows)
+          reinterpret_cast<uint4*>(static_cast<T*>(a.out) + at)[piece] = v;
       }
     }
   }
@@ -551,9 +581,10 @@ __global__ void __launch_bounds__(kThreads, 2)
   if (s_odd) {
     // a value that only some rows see is not finite: zero times it is not zero
     float* rowbuf = reinterpret_cast<float*>(sbase) + (warp - 4) * D;  // the rings are free
+    const RowTile here = rt;  // of which the call takes the address: not of rt
     for (int r = warp - 4; r < rows; r += 4) {
-      slow_row<T, D>(a, rt, r, head, p.scale_log2, tile0 * kTile, (tile0 + tiles) * kTile,
-                     limit_of(r), rowbuf, &s_m[r], &s_l[r]);
+      slow_row<T, D>(a, here, r, head, p.scale_log2, first_key, (int64_t)first_key + tiles * kTile,
+                     keys_of(a, rt, r), rowbuf, &s_m[r], &s_l[r]);
       __syncwarp();
       const float l = s_l[r], inv = l == 0.f ? 0.f : 1.f / l;
       const int q = rt.row0 + r;
@@ -561,7 +592,7 @@ __global__ void __launch_bounds__(kThreads, 2)
                ((int64_t)head * a.group + q % a.group) * a.o_head;
       for (int d = lane; d < D; d += 32) {
         if (runs > 1)
-          mine[r * D + d] = rowbuf[d];
+          mine[(d / 4 * kRows + r) * 4 + d % 4] = rowbuf[d];
         else
           dst[d] = ElemOps<T>::from_float(rowbuf[d] * inv);
       }
@@ -578,7 +609,7 @@ __global__ void __launch_bounds__(kThreads, 2)
   }
   if (a.lse != nullptr && stid < rows) {
     const int q = rt.row0 + stid;
-    a.lse[(rt.first + q / a.group) * (p.heads * a.group) + (int64_t)head * a.group + q % a.group] =
+    a.lse[((rt.first + q / a.group) * p.heads + head) * a.group + q % a.group] =
         s_l[stid] == 0.f ? -INFINITY : (s_m[stid] + log2f(s_l[stid])) * 0.6931471805599453f;
   }
 }
@@ -596,16 +627,16 @@ __global__ void __launch_bounds__(kJoinThreads)
   constexpr int64_t kRun = kRows * (D + 2);
   __shared__ float wgt[kMaxRuns][kHere], sums[kMaxRuns][kHere], inv_l[kHere];
   const PagedAttnArgs& a = p.a;
-  const int64_t item = blockIdx.x / (kRows / kHere);
+  const unsigned item = blockIdx.x / (kRows / kHere);
   const int r0 = (int)(blockIdx.x % (kRows / kHere)) * kHere, tid = threadIdx.x;
-  const int head = (int)(item / p.tiles);
+  const int head = (int)(item / (unsigned)p.tiles);
   RowTile rt;
-  if (!locate_tile(a.t, a.pool, a.group, kRows, item % p.tiles, rt)) return;
+  if (!locate_tile(a.t, a.pool, a.group, kRows, item % (unsigned)p.tiles, rt)) return;
   const int in_tile = rt.rows - rt.row0 < kRows ? rt.rows - rt.row0 : kRows;
   const int rows = in_tile - r0 < kHere ? in_tile - r0 : kHere;
   const int count = runs_of(p, rt, in_tile).count;
   if (rows <= 0 || count == 1) return;
-  const float* from = p.partial + item * p.splits * kRun;
+  const float* from = p.partial + (int64_t)item * p.splits * kRun;
   for (int i = tid; i < count * kHere; i += kJoinThreads) {
     const int s = i / kHere, r = i % kHere;
     if (r < rows) {
@@ -626,14 +657,14 @@ __global__ void __launch_bounds__(kJoinThreads)
     inv_l[tid] = l == 0.f ? 0.f : 1.f / l;
     if (a.lse != nullptr) {
       const int q = rt.row0 + r0 + tid;
-      a.lse[(rt.first + q / a.group) * (p.heads * a.group) + (int64_t)head * a.group +
-            q % a.group] = l == 0.f ? -INFINITY : (mx + log2f(l)) * 0.6931471805599453f;
+      a.lse[((rt.first + q / a.group) * p.heads + head) * a.group + q % a.group] =
+          l == 0.f ? -INFINITY : (mx + log2f(l)) * 0.6931471805599453f;
     }
   }
   __syncthreads();
-  const int r = tid / (D / 4), d = (tid % (D / 4)) * 4;
+  const int r = tid % kHere, d = tid / kHere * 4;
   if (r >= rows) return;
-  const float* mine = from + (r0 + r) * D + d;
+  const float* mine = from + d * kRows + (r0 + r) * 4;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
   for (int s0 = 0; s0 < count; s0 += 8) {
     float4 v[8];
@@ -670,11 +701,11 @@ cudaError_t launch_tc05(const TcParams& p, const CUtensorMap& mk, const CUtensor
   const cudaError_t e =
       cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
   if (e != cudaSuccess) return e;
-  kernel<<<(unsigned)(p.tiles * p.heads * p.splits), kThreads, smem, st>>>(mk, mv, p);
+  kernel<<<(unsigned)p.tiles * p.heads * p.splits, kThreads, smem, st>>>(mk, mv, p);
   const cudaError_t launched = cudaGetLastError();
   if (launched != cudaSuccess || p.splits == 1) return launched;
   join_runs_kernel<T, D>
-      <<<(unsigned)(p.tiles * p.heads * (kRows * D / (4 * kJoinThreads))), kJoinThreads, 0, st>>>(p);
+      <<<(unsigned)p.tiles * p.heads * (kRows * D / (4 * kJoinThreads)), kJoinThreads, 0, st>>>(p);
   return cudaGetLastError();
 }
 
@@ -688,9 +719,10 @@ PagedPlan paged_tc05_plan(int64_t total, int64_t seqs, int kv_heads, int group, 
   const int64_t items = plan.tiles * kv_heads, key_tiles = (max_len + kTile - 1) / kTile;
   // Runs per row tile: the number that ends the last wave of 2 CTAs per SM
   // soonest.  In units of a key tile (0.7 us): a CTA's start and end cost ten,
-  // joining the runs eight.  1 frame over 31 cached ones (176 items), the join
-  // in the kernel: 1 run 536 us, 3 runs 387, 5 runs 375, 10 runs 422; 4 prompts
-  // (2,024 items): 1 run 1,292 us, 2 runs 1,546.
+  // joining the runs eight.  (Measured when the last CTA of a row tile joined
+  // its runs: 1 frame over 31 cached ones, 176 items, 1 run 536 us, 3 runs 387,
+  // 5 runs 375, 10 runs 422; 4 prompts, 2,024 items, 1 run 1,292 us, 2 runs
+  // 1,546.)
   plan.splits = 1;
   int64_t best = -1;
   const int64_t slots = 2 * 148;
@@ -712,10 +744,10 @@ cudaError_t launch_paged_tc05(const PagedAttnArgs& a, const PagedPlan& plan, cud
   TcParams p;
   p.a = a;
   p.scale_log2 = a.scale * 1.4426950408889634f;
-  p.tiles = plan.tiles;
+  p.tiles = (int)plan.tiles;  // the entry point holds tiles * heads * splits below 2^31
   p.heads = a.pool.kv_heads;
-  p.splits = plan.splits;
-  p.chunk = plan.chunk;
+  p.splits = (int)plan.splits;
+  p.chunk = (int)plan.chunk;
   p.partial = reinterpret_cast<float*>(static_cast<char*>(a.workspace) + kMaxCounters * 4);
   if (plan.tiles == 0) return cudaSuccess;
   CUtensorMap mk, mv;
