@@ -16,14 +16,12 @@
 // tiles for each; two CTAs share an SM.
 //
 // What bounds it: 128 x 128 exponentials cost the multi-function unit 1,024
-// clocks, the MMAs 256 (dim 64) or 512; so three column pairs of eight take a
+// clocks, the MMAs 256 (dim 64) or 512; so two column pairs of eight take a
 // polynomial (error 2.7e-6) on the FMA pipe.  One frame of 1,374 tokens over
-// 43,968 keys in 16 heads: 333 us (338 at two pairs of eight, 355 at four);
-// without any exponential the same kernel takes 243 us, with loads of S alone
-// 169 us.  Two exponential warps share an SM's quarter; 32 columns take the two
-// some 600 clocks, where the unit needs 320 and the packed instructions as
-// much: they wait for one another's results.  Eight exponential warps instead
-// of four were slower (356 us).
+// 43,968 keys in 16 heads: 297 us (303 at three pairs of eight, 331 at four).
+// Two exponential warps share an SM's quarter; 32 columns take the two some 520
+// clocks, where the unit needs 384: they wait for one another's results.  Eight
+// exponential warps instead of four were slower (356 us against 341 then).
 #include <cuda.h>
 
 #include <type_traits>
@@ -41,7 +39,7 @@ constexpr int kLseStages = 4;
 constexpr uint32_t kTmemCols = 256;
 constexpr uint64_t kDrainNs = 1000000000ull;
 // column pairs of every 8 whose exponentials take the polynomial
-constexpr unsigned kPolyPairs = 0x49u;
+constexpr unsigned kPolyPairs = 0x11u;
 
 template <int D>
 struct Smem {
@@ -306,13 +304,18 @@ __global__ void __launch_bounds__(kThreads, 2)
     float old = 0.f;
     float_pair sum[2] = {};
     int64_t from = 0;  // rows from this one on see the key
+    int plain_rt = 0;  // row tiles from this one to the last but one need no mask
     while (ok && row_tiles > 0 && kt < tiles) {
       const int64_t key = key_at + kt * kKeys;
       if (kt != at) {
         at = kt;
         old = key < len ? w[key] : 0.f;
         sum[0] = sum[1] = pack_pair(0.f, 0.f);
-        from = a.causal ? (key - past) * group : 0;
+        if (a.causal) {
+          from = (key - past) * group;
+          const int64_t all = __shfl_sync(0xffffffffu, from, 31);  // see the warp's last key
+          plain_rt = all > 0 ? (int)((all + tile_rows - 1) / tile_rows) : 0;
+        }
       }
       const int slot = n % kLseStages, buf = n & 1;
       const uint32_t t_s = tmem + lane_off + 128u * buf;
@@ -322,60 +325,72 @@ __global__ void __launch_bounds__(kThreads, 2)
         ++next_kt;
         next_rt = next_kt < tiles ? first_row_tile(next_kt) : 0;
       }
-      const int64_t r0 = (int64_t)rt * tile_rows;
-      const int left = (n_new - rt * p.tokens) * group;
-      // This thread's key is seen by the columns [lo, left); the warp's keys by
-      // none below lo_warp and by all from hi_warp on.
-      const int lo = (int)(from - r0 < 0 ? 0 : (from - r0 < kCols ? from - r0 : kCols));
-      const int lo_warp = __shfl_sync(0xffffffffu, lo, 0);
-      const int hi_warp = __shfl_sync(0xffffffffu, lo, 31);
+      // Tiles that need no mask take a copy without its branches, so that the
+      // compiler orders a part's instructions among one another (a frame: 338
+      // us where every part asks, 297).
+      auto walk = [&](auto masked) {
+        // This thread's key is seen by the columns [lo, left); the warp's keys by
+        // none below lo_warp and by all from hi_warp on.
+        int lo = 0, lo_warp = 0, hi_warp = 0, left = kCols;
+        if (decltype(masked)::value) {
+          const int64_t r0 = (int64_t)rt * tile_rows;
+          left = (n_new - rt * p.tokens) * group;
+          lo = (int)(from - r0 < 0 ? 0 : (from - r0 < kCols ? from - r0 : kCols));
+          lo_warp = __shfl_sync(0xffffffffu, lo, 0);
+          hi_warp = __shfl_sync(0xffffffffu, lo, 31);
+        }
 #pragma unroll
-      for (int part = 0; part < 4; ++part) {
-        const int col0 = 32 * part;
-        tc::tmem_wait_ld();
-        if (part < 3) {
-          tc::tmem_ld32(t_s + 32u * (part + 1), s[(part + 1) & 1]);
-        } else {
-          // S_t is read
-          tc::tc_fence_before();
-          __syncwarp();
-          if (lane == 0) tc::mbar_arrive(sempty0 + 8u * buf);
-          if (next_kt < tiles) {
-            ok = wait(sfull0 + 8u * (buf ^ 1), (uint32_t)((n + 1) >> 1) & 1u);
-            if (!ok) break;
-            tc::tc_fence_after();
-            tc::tmem_ld32(t_next, s[0]);
+        for (int part = 0; part < 4; ++part) {
+          const int col0 = 32 * part;
+          tc::tmem_wait_ld();
+          if (part < 3) {
+            tc::tmem_ld32(t_s + 32u * (part + 1), s[(part + 1) & 1]);
+          } else {
+            // S_t is read
+            tc::tc_fence_before();
+            __syncwarp();
+            if (lane == 0) tc::mbar_arrive(sempty0 + 8u * buf);
+            if (next_kt < tiles) {
+              ok = wait(sfull0 + 8u * (buf ^ 1), (uint32_t)((n + 1) >> 1) & 1u);
+              if (!ok) return;
+              tc::tc_fence_after();
+              tc::tmem_ld32(t_next, s[0]);
+            }
           }
-        }
-        if (col0 >= left || col0 + 32 <= lo_warp) continue;
-        uint32_t* sc = s[part & 1];
-        if (col0 + 32 > left || col0 < hi_warp) {
-          // gives 0, or 2^-126 where the polynomial is taken
+          if (decltype(masked)::value && (col0 >= left || col0 + 32 <= lo_warp)) continue;
+          uint32_t* sc = s[part & 1];
+          if (decltype(masked)::value && (col0 + 32 > left || col0 < hi_warp)) {
+            // gives 0, or 2^-126 where the polynomial is taken
 #pragma unroll
-          for (int i = 0; i < 32; ++i)
-            if (col0 + i < lo || col0 + i >= left) sc[i] = __float_as_uint(-INFINITY);
-        }
-        const float4* minus = reinterpret_cast<const float4*>(&s_lse[slot][col0]);
+            for (int i = 0; i < 32; ++i)
+              if (col0 + i < lo || col0 + i >= left) sc[i] = __float_as_uint(-INFINITY);
+          }
+          const float4* minus = reinterpret_cast<const float4*>(&s_lse[slot][col0]);
 #pragma unroll
-        for (int i = 0; i < 16; i += 2) {
-          const float4 m = minus[i / 2];
+          for (int i = 0; i < 16; i += 2) {
+            const float4 m = minus[i / 2];
 #pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            const float_pair x = fma_pair(pack_pair(__uint_as_float(sc[2 * (i + j)]),
-                                                    __uint_as_float(sc[2 * (i + j) + 1])),
-                                          c2, j ? pack_pair(m.z, m.w) : pack_pair(m.x, m.y));
-            if ((kPolyPairs >> ((i + j) & 7)) & 1u) {
-              float_pair q, scale;
-              poly(q, scale, x);
-              sum[j] = fma_pair(q, scale, sum[j]);
-            } else {
-              float ea, eb;
-              unpack_pair(ea, eb, x);
-              sum[j] = add_pair(sum[j], pack_pair(fast_exp2(ea), fast_exp2(eb)));
+            for (int j = 0; j < 2; ++j) {
+              const float_pair x = fma_pair(pack_pair(__uint_as_float(sc[2 * (i + j)]),
+                                                      __uint_as_float(sc[2 * (i + j) + 1])),
+                                            c2, j ? pack_pair(m.z, m.w) : pack_pair(m.x, m.y));
+              if ((kPolyPairs >> ((i + j) & 7)) & 1u) {
+                float_pair q, scale;
+                poly(q, scale, x);
+                sum[j] = fma_pair(q, scale, sum[j]);
+              } else {
+                float ea, eb;
+                unpack_pair(ea, eb, x);
+                sum[j] = add_pair(sum[j], pack_pair(fast_exp2(ea), fast_exp2(eb)));
+              }
             }
           }
         }
-      }
+      };
+      if (rt < plain_rt || rt == row_tiles - 1)
+        walk(std::true_type{});
+      else
+        walk(std::false_type{});
       if (!ok) break;
       __syncwarp();
       if (lane == 0) tc::mbar_arrive(lempty0 + 8u * slot);
