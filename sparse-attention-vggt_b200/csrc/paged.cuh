@@ -141,7 +141,6 @@ struct PagedAttnArgs {
   void* out;
   int64_t o_token, o_head;
   float* lse;       // [total][q_heads] or null
-  int64_t max_new, max_len;  // what the caller expects; only the choice of variant depends on them
   void* workspace;  // counters (zero before and after), then partial results
   uint64_t wait_ns;
   // self-test of the failure detection: one warp waits on a barrier that

@@ -81,8 +81,6 @@ extern "C" int vggt_paged_attention(
   a.o_token = out_token_stride;
   a.o_head = out_head_stride;
   a.lse = lse;
-  a.max_new = max_new;
-  a.max_len = max_len;
   a.workspace = workspace;
   a.wait_ns = api_wait_ns();
   a.wait_selftest = api_wait_selftest();

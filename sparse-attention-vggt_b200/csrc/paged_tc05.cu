@@ -205,158 +205,156 @@ __global__ void __launch_bounds__(kThreads, 2)
   if (warp < 4) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kControlRegs));
     if (warp == 0) {
-    // ================= TMA producer =================
-    const int keys = keys_of(a, rt, rows - 1) - first_key;  // to the end of the last row's keys
-    auto produce = [&](auto boxes_) {
-      constexpr int kBoxes = decltype(boxes_)::value;  // boxes per tile
-      constexpr int kBox = kTile / kBoxes;             // slots per box
-      constexpr int kAhead = 32 / kBoxes;              // tiles per read of the table
-      const uint32_t full0 = smem_u32(&bars.full[0][0]), empty0 = smem_u32(&bars.empty[0][0]);
-      constexpr uint32_t kToV = sizeof(bars.full[0]);  // from K's barriers to V's
-      const int32_t* table = a.t.table + rt.seq * a.t.width;
-      const int in_page = first_key & (a.pool.page - 1), page_mask = a.pool.page - 1;
-      int page = 0, stage = 0;
-      int issued_at[2] = {0, 0};  // of the elected lane
-      uint32_t phase = 1;
-      for (int t = 0; t < tiles; ++t) {
-        const int key0 = t * kTile;
-        const int turn = t & (kAhead - 1);
-        if (turn == 0) {
-          const int key = key0 + lane * kBox;
-          page = (int)a.pool.n_pages;  // past the pool: reads as zeros
-          if (key < keys && key < tiles * kTile) {
-            const int got = __ldg(table + ((first_key + key) >> a.pool.page_shift));
-            if (got >= 0 && got < a.pool.n_pages)
-              page = got;
-            else
-              raise_status(a.t.status, VGGT_STATUS_BAD_PAGE);
+      // ================= TMA producer =================
+      const int keys = keys_of(a, rt, rows - 1) - first_key;  // to the end of the last row's keys
+      auto produce = [&](auto boxes_) {
+        constexpr int kBoxes = decltype(boxes_)::value;  // boxes per tile
+        constexpr int kBox = kTile / kBoxes;             // slots per box
+        constexpr int kAhead = 32 / kBoxes;              // tiles per read of the table
+        const uint32_t full0 = smem_u32(&bars.full[0][0]), empty0 = smem_u32(&bars.empty[0][0]);
+        constexpr uint32_t kToV = sizeof(bars.full[0]);  // from K's barriers to V's
+        const int32_t* table = a.t.table + rt.seq * a.t.width;
+        const int in_page = first_key & (a.pool.page - 1), page_mask = a.pool.page - 1;
+        int page = 0, stage = 0;
+        int issued_at[2] = {0, 0};  // of the elected lane
+        uint32_t phase = 1;
+        for (int t = 0; t < tiles; ++t) {
+          const int key0 = t * kTile;
+          const int turn = t & (kAhead - 1);
+          if (turn == 0) {
+            const int key = key0 + lane * kBox;
+            page = (int)a.pool.n_pages;  // past the pool: reads as zeros
+            if (key < keys && key < tiles * kTile) {
+              const int got = __ldg(table + ((first_key + key) >> a.pool.page_shift));
+              if (got >= 0 && got < a.pool.n_pages)
+                page = got;
+              else
+                raise_status(a.t.status, VGGT_STATUS_BAD_PAGE);
+            }
+          }
+          int pages[kBoxes];
+#pragma unroll
+          for (int b = 0; b < kBoxes; ++b)
+            pages[b] = __shfl_sync(0xffffffffu, page, turn * kBoxes + b);
+          int live = (keys - key0 + kBox - 1) / kBox;
+          live = live < kBoxes ? live : kBoxes;
+          const int row = (in_page + key0) & page_mask;
+          bool ok = true;
+#pragma unroll
+          for (int kv = 0; kv < 2; ++kv) {
+            if (t >= kStages)
+              ok = ok &&
+                   tc::warp_wait(empty0 + kv * kToV + 8u * stage, phase, abort_flag, a.wait_ns);
+            if (ok && tc::elect_one()) {
+              const uint32_t bar = full0 + kv * kToV + 8u * stage;
+              tc::mbar_expect_tx(bar, (uint32_t)(live * kBox) * D * 2u);
+              const uint32_t dst = base + (kv ? L::kV : L::kK) + stage * L::kMatrix;
+#pragma unroll
+              for (int b = 0; b < kBoxes; ++b)
+                if (b < live)
+#pragma unroll
+                  for (int h = 0; h < kHalves; ++h)
+                    tc::tma_load_4d(dst + h * (kTile * 128) + b * kBox * 128, kv ? &tm_v : &tm_k,
+                                    bar, h * 64, (row + b * kBox) & page_mask, head, pages[b]);
+              issued_at[kv] = t + 1;
+            }
+            __syncwarp();
+          }
+          if (!ok) break;
+          if (++stage == kStages) {
+            stage = 0;
+            phase ^= 1u;
           }
         }
-        int pages[kBoxes];
+        // no copy may be in flight when the CTA leaves
+        for (int kv = 0; kv < 2; ++kv)
+          for (int t = max(issued_at[kv] - kStages, 0); t < issued_at[kv]; ++t)
+            tc::mbar_wait_drain(full0 + kv * kToV + 8u * (t % kStages),
+                                (uint32_t)((t / kStages) & 1), kDrainNs);
+      };
+      if (a.pool.page >= 64)
+        produce(std::integral_constant<int, 1>{});
+      else if (a.pool.page == 32)
+        produce(std::integral_constant<int, 2>{});
+      else
+        produce(std::integral_constant<int, 4>{});
+    } else if (warp < 3) {
+      // ================= MMA issuers: warp 1 S = Q K^T, warp 2 O += P V ========
+      // The whole warp walks through the tiles and waits; one elected lane
+      // issues, which keeps the MMA operands in uniform registers.
+      const uint32_t fmt = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
+      auto wait = [&](uint32_t bar, uint32_t parity) {
+        return tc::warp_wait(bar, parity, abort_flag, a.wait_ns);
+      };
+      const uint32_t kfull0 = smem_u32(&bars.full[0][0]), kempty0 = smem_u32(&bars.empty[0][0]);
+      const uint32_t vfull0 = smem_u32(&bars.full[1][0]), vempty0 = smem_u32(&bars.empty[1][0]);
+      const uint32_t sfull0 = smem_u32(&bars.s_full[0]), pfull0 = smem_u32(&bars.p_full[0]);
+      const uint32_t sfree0 = smem_u32(&bars.s_free[0]);
+      int stage = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      if (warp == 1) {
+        const uint32_t id_qk = tc::idesc_f16(fmt, 0u, kRows, kTile);
+        const uint64_t qdesc = tc::sw128_desc(base + L::kQ, 16);
+        const uint64_t kdesc0 = tc::sw128_desc(base + L::kK, 16);
+        ok = wait(smem_u32(&bars.q_full), 0);
+        if (a.wait_selftest) ok = ok && wait(smem_u32(&bars.never), 0);
+        for (int t = 0; ok && t < tiles; ++t) {
+          const uint32_t buf = t & 1;
+          // P of tile t - 2 lay where S_t goes: its product must be done
+          ok = (t < 2 || wait(sfree0 + 8u * buf, (uint32_t)((t >> 1) + 1) & 1u)) &&
+               wait(kfull0 + 8u * stage, phase);
+          if (!ok) break;
+          tc::tc_fence_after();
+          if (tc::elect_one()) {
+            const uint64_t kdesc = kdesc0 + (uint64_t)(stage * (L::kMatrix / 16));
 #pragma unroll
-        for (int b = 0; b < kBoxes; ++b)
-          pages[b] = __shfl_sync(0xffffffffu, page, turn * kBoxes + b);
-        int live = (keys - key0 + kBox - 1) / kBox;
-        live = live < kBoxes ? live : kBoxes;
-        const int row = (in_page + key0) & page_mask;
-        bool ok = true;
-#pragma unroll
-        for (int kv = 0; kv < 2; ++kv) {
-          if (t >= kStages)
-            ok = ok && tc::warp_wait(empty0 + kv * kToV + 8u * stage, phase, abort_flag, a.wait_ns);
-          if (ok && tc::elect_one()) {
-            const uint32_t bar = full0 + kv * kToV + 8u * stage;
-            tc::mbar_expect_tx(bar, (uint32_t)(live * kBox) * D * 2u);
-            const uint32_t dst = base + (kv ? L::kV : L::kK) + stage * L::kMatrix;
-#pragma unroll
-            for (int b = 0; b < kBoxes; ++b)
-              if (b < live)
-#pragma unroll
-                for (int h = 0; h < kHalves; ++h)
-                  tc::tma_load_4d(dst + h * (kTile * 128) + b * kBox * 128, kv ? &tm_v : &tm_k,
-                                  bar, h * 64, (row + b * kBox) & page_mask, head, pages[b]);
-            issued_at[kv] = t + 1;
+            for (int kk = 0; kk < D / 16; ++kk)
+              tc::mma_ss(tmem + 64u * buf,
+                         qdesc + (uint64_t)((kk >> 2) * (kRows * 128 / 16) + (kk & 3) * 2),
+                         kdesc + (uint64_t)((kk >> 2) * (kTile * 128 / 16) + (kk & 3) * 2), id_qk,
+                         kk > 0 ? 1u : 0u);
+            tc::mma_commit(sfull0 + 8u * buf);
+            tc::mma_commit(kempty0 + 8u * stage);
           }
           __syncwarp();
+          if (++stage == kStages) {
+            stage = 0;
+            phase ^= 1u;
+          }
         }
-        if (!ok) break;
-        if (++stage == kStages) {
-          stage = 0;
-          phase ^= 1u;
-        }
-      }
-      // no copy may be in flight when the CTA leaves
-      for (int kv = 0; kv < 2; ++kv)
-        for (int t = issued_at[kv] > kStages ? issued_at[kv] - kStages : 0; t < issued_at[kv]; ++t)
-          tc::mbar_wait_drain(full0 + kv * kToV + 8u * (t % kStages),
-                              (uint32_t)((t / kStages) & 1), kDrainNs);
-    };
-    if (a.pool.page >= 64)
-      produce(std::integral_constant<int, 1>{});
-    else if (a.pool.page == 32)
-      produce(std::integral_constant<int, 2>{});
-    else
-      produce(std::integral_constant<int, 4>{});
-    } else if (warp < 3) {
-    // ================= MMA issuers: warp 1 S = Q K^T, warp 2 O += P V ========
-    // Two warps, because a wait on a barrier costs a warp some 200 clocks and
-    // the issue of four MMAs 300: in one warp the four steps of a tile took
-    // longer than its softmax.  A whole warp walks through the tiles and waits;
-    // one elected lane issues, which keeps the MMA operands in uniform
-    // registers.
-    const uint32_t fmt = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
-    auto wait = [&](uint32_t bar, uint32_t parity) {
-      return tc::warp_wait(bar, parity, abort_flag, a.wait_ns);
-    };
-    const uint32_t kfull0 = smem_u32(&bars.full[0][0]), kempty0 = smem_u32(&bars.empty[0][0]);
-    const uint32_t vfull0 = smem_u32(&bars.full[1][0]), vempty0 = smem_u32(&bars.empty[1][0]);
-    const uint32_t sfull0 = smem_u32(&bars.s_full[0]), pfull0 = smem_u32(&bars.p_full[0]);
-    const uint32_t sfree0 = smem_u32(&bars.s_free[0]);
-    int stage = 0;
-    uint32_t phase = 0;
-    bool ok = true;
-    if (warp == 1) {
-      const uint32_t id_qk = tc::idesc_f16(fmt, 0u, kRows, kTile);
-      const uint64_t qdesc = tc::sw128_desc(base + L::kQ, 16);
-      const uint64_t kdesc0 = tc::sw128_desc(base + L::kK, 16);
-      ok = wait(smem_u32(&bars.q_full), 0);
-      if (a.wait_selftest) ok = ok && wait(smem_u32(&bars.never), 0);
-      for (int t = 0; ok && t < tiles; ++t) {
-        const uint32_t buf = t & 1;
-        // P of tile t - 2 lay where S_t goes: its product must be done
-        ok = (t < 2 || wait(sfree0 + 8u * buf, (uint32_t)((t >> 1) + 1) & 1u)) &&
-             wait(kfull0 + 8u * stage, phase);
-        if (!ok) break;
-        tc::tc_fence_after();
-        if (tc::elect_one()) {
-          const uint64_t kdesc = kdesc0 + (uint64_t)(stage * (L::kMatrix / 16));
+      } else {
+        const uint32_t id_pv = tc::idesc_f16(fmt, 1u, kRows, D);
+        // 64-element groups of V's rows lie kTile * 128 bytes apart
+        const uint64_t vdesc0 = tc::sw128_desc(base + L::kV, kTile * 128);
+        for (int t = 0; ok && t < tiles; ++t) {
+          const uint32_t buf = t & 1;
+          ok = wait(vfull0 + 8u * stage, phase) && wait(pfull0 + 8u * buf, (uint32_t)(t >> 1) & 1u);
+          if (!ok) break;
+          tc::tc_fence_after();
+          if (tc::elect_one()) {
+            const uint64_t vdesc = vdesc0 + (uint64_t)(stage * (L::kMatrix / 16));
 #pragma unroll
-          for (int kk = 0; kk < D / 16; ++kk)
-            tc::mma_ss(tmem + 64u * buf,
-                       qdesc + (uint64_t)((kk >> 2) * (kRows * 128 / 16) + (kk & 3) * 2),
-                       kdesc + (uint64_t)((kk >> 2) * (kTile * 128 / 16) + (kk & 3) * 2), id_qk,
-                       kk > 0 ? 1u : 0u);
-          tc::mma_commit(sfull0 + 8u * buf);
-          tc::mma_commit(kempty0 + 8u * stage);
-        }
-        __syncwarp();
-        if (++stage == kStages) {
-          stage = 0;
-          phase ^= 1u;
-        }
-      }
-    } else {
-      const uint32_t id_pv = tc::idesc_f16(fmt, 1u, kRows, D);
-      // 64-element groups of V's rows lie kTile * 128 bytes apart
-      const uint64_t vdesc0 = tc::sw128_desc(base + L::kV, kTile * 128);
-      for (int t = 0; ok && t < tiles; ++t) {
-        const uint32_t buf = t & 1;
-        ok = wait(vfull0 + 8u * stage, phase) && wait(pfull0 + 8u * buf, (uint32_t)(t >> 1) & 1u);
-        if (!ok) break;
-        tc::tc_fence_after();
-        if (tc::elect_one()) {
-          const uint64_t vdesc = vdesc0 + (uint64_t)(stage * (L::kMatrix / 16));
-#pragma unroll
-          for (int kk = 0; kk < kTile / 16; ++kk)
-            tc::mma_ts(t_o, tmem + 64u * buf + 8u * kk, vdesc + (uint64_t)(kk * 128), id_pv,
-                       (t > 0 || kk > 0) ? 1u : 0u);
-          tc::mma_commit(sfree0 + 8u * buf);
-          tc::mma_commit(vempty0 + 8u * stage);
-        }
-        __syncwarp();
-        if (++stage == kStages) {
-          stage = 0;
-          phase ^= 1u;
+            for (int kk = 0; kk < kTile / 16; ++kk)
+              tc::mma_ts(t_o, tmem + 64u * buf + 8u * kk, vdesc + (uint64_t)(kk * 128), id_pv,
+                         (t > 0 || kk > 0) ? 1u : 0u);
+            tc::mma_commit(sfree0 + 8u * buf);
+            tc::mma_commit(vempty0 + 8u * stage);
+          }
+          __syncwarp();
+          if (++stage == kStages) {
+            stage = 0;
+            phase ^= 1u;
+          }
         }
       }
-    }
-    if (tc::elect_one()) {
-      if (warp == 2 && ok && tiles > 0) tc::mma_commit(smem_u32(&bars.o_full));
-      // every issued MMA must finish before the TMEM columns are released
-      tc::mma_commit(smem_u32(&bars.drain[warp - 1]));
-    }
-    __syncwarp();
-    tc::mbar_wait_drain(smem_u32(&bars.drain[warp - 1]), 0, kDrainNs);
+      if (tc::elect_one()) {
+        if (warp == 2 && ok && tiles > 0) tc::mma_commit(smem_u32(&bars.o_full));
+        // every issued MMA must finish before the TMEM columns are released
+        tc::mma_commit(smem_u32(&bars.drain[warp - 1]));
+      }
+      __syncwarp();
+      tc::mbar_wait_drain(smem_u32(&bars.drain[warp - 1]), 0, kDrainNs);
     }
     return;  // what follows runs on the softmax warps alone
   }

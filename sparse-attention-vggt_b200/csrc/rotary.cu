@@ -235,7 +235,8 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(RotaryArgs p) {
 // (One head of 64, 703,488 tokens: 53 us, against 99; what is left are the
 // sines, 50 instructions each.)
 template <typename T, int N>
-__global__ void __launch_bounds__(kThreads, sizeof(T) == 4 ? 2 : 3) rotary_few_heads_kernel(RotaryArgs p) {
+__global__ void __launch_bounds__(kThreads, sizeof(T) == 4 ? 2 : 3)
+    rotary_few_heads_kernel(RotaryArgs p) {
   int unit, head;
   const int64_t first =
       divided(divided((int64_t)blockIdx.x * kThreads + threadIdx.x, p.units, unit), p.heads, head);
