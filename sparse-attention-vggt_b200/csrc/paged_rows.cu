@@ -15,9 +15,12 @@
 //    order and leaves the counter at zero, so there is one launch and the
 //    result does not depend on the order in which CTAs finish.
 //
-// P is rounded to the tensors' type for the product with V (its error is that
-// of the output's own rounding); maxima, sums and outputs are fp32, and the
-// sums take P before it is rounded.
+// P is rounded to the tensors' type for the product with V; maxima, sums and
+// outputs are fp32, and the sums take P before it is rounded.  In fp16 the
+// exponents are shifted up by 15, so that P <= 2^15 and probabilities down to
+// 2^-29 of the row's largest keep all of the type's bits (with P <= 1 those of
+// 2^-25 and less were lost to the product, though not to the sum); bf16 has the
+// exponents of fp32.  So P's error is that of the output's own rounding.
 #include <cuda.h>
 
 #include <type_traits>
@@ -68,6 +71,7 @@ __global__ void __launch_bounds__(kThreads, 2)
                       const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ RowsParams p) {
   using R = Ring<D>;
   constexpr int kSteps = D / 16;
+  constexpr float kShift = std::is_same<T, __half>::value ? 15.f : 0.f;
   extern __shared__ unsigned char raw[];
   unsigned char* ring = raw + ((1024u - (smem_u32(raw) & 1023u)) & 1023u);
   const uint32_t ring_addr = smem_u32(ring);
@@ -234,7 +238,9 @@ __global__ void __launch_bounds__(kThreads, 2)
         for (int n = 0; n < kN; ++n) mx = fmaxf(mx, fmaxf(s[n][2 * i], s[n][2 * i + 1]));
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-        mx = fmaxf(m_run[i], mx * p.scale_log2);
+        // less the shift, rounded up: no exponent passes the shift, however
+        // large the scores are
+        mx = fmaxf(m_run[i], __fmaf_ru(mx, p.scale_log2, -kShift));
         // a row that has seen nothing yet keeps a finite base, so that its
         // masked scores give 2^(-inf - 0) = 0
         base[i] = mx == -INFINITY ? 0.f : mx;

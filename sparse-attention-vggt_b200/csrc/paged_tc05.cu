@@ -21,7 +21,9 @@
 // The row's reference maximum moves only when a tile's maximum exceeds it by
 // more than 2^8 in the exp2 domain; O is rescaled then.  Sums are fp32, of the
 // exponentials before P is rounded: the log-sum-exp is good to fp32 and only
-// the product with V sees the rounding.
+// the product with V sees the rounding.  In fp16 the exponents are shifted up
+// by 7 (PRange): P reaches 2^15 at most, and what lies 2^21 under the
+// reference still has all of the type's bits.
 //
 // What bounds it: the multi-function unit gives 16 exponentials per clock and
 // SM, so a 128 x 64 tile costs 512 clocks there, against 320 (dim 64) or 640
@@ -69,6 +71,19 @@ static_assert(kControlRegs + kSoftRegs == 2 * kLaunchRegs, "register split");
 constexpr uint32_t kTmemCols = 256;  // S0 | S1 | O
 constexpr uint64_t kDrainNs = 1000000000ull;
 constexpr int kMaxRuns = 64;  // per row tile
+
+// How far a row's scores may pass its reference before that moves, and what
+// exponents are shifted by, in units of log2.  With P <= 1 at the reference,
+// fp16 would drop probabilities of 2^-25 and less from the product with V,
+// which their sum still counts: 65,000 keys under one strong one lost 0.2 % of
+// the output.  Lag and shift share the 15 steps up to 2^15.  A smaller lag moves
+// the reference more often (4 prompts of dim 128: 1,430 to 1,480 us; 1,560 at 4
+// and 11, 1,640 at 2 and 13).  bf16 has the exponents of fp32.
+template <typename T>
+struct PRange {
+  static constexpr bool kHalf = std::is_same<T, __half>::value;
+  static constexpr float kLag = 8.f, kShift = kHalf ? 7.f : 0.f;
+};
 
 template <int D>
 struct Smem {
@@ -391,7 +406,11 @@ __global__ void __launch_bounds__(kThreads, 2)
     };
     // whether some row of the CTA does not see all of tile t (for all warps alike)
     auto is_edge = [&](int t) { return (t + 1) * kTile > least_at; };
-    float m_ref = -INFINITY;  // in score units; exponents are relative to it
+    // The reference in score units, and what is added to a score's exponent:
+    // PRange's shift less the reference, rounded down, so that the largest P is
+    // known however large the scores are.  A row that has seen nothing keeps 0:
+    // its masked scores give 0, or 2^-126 where the polynomial is taken.
+    float m_ref = -INFINITY, minus = 0.f;
     float_pair sum = pack_pair(0.f, 0.f);
     const float_pair c2 = pack_pair(c, c);
     const Exp2Poly poly;
@@ -451,9 +470,10 @@ __global__ void __launch_bounds__(kThreads, 2)
                                max_nan(mx[6], mx[7]));
       // also true where m or m_ref is NaN; a tile of which the row sees nothing
       // changes nothing (a NaN in the sum stays)
-      const bool grow = !((m - m_ref) * c <= 8.f) && m != -INFINITY;
+      const bool grow = !((m - m_ref) * c <= PRange<T>::kLag) && m != -INFINITY;
       if (__any_sync(0xffffffffu, grow)) {
         const bool rescale = grow && m_ref != -INFINITY;
+        const float moved = __fmaf_rd(-m, c, PRange<T>::kShift);
         if (__any_sync(0xffffffffu, rescale)) {
           // O must hold the products of all tiles before this one
           if (!wait(smem_u32(&bars.s_free[(t - 1) & 1]), (uint32_t)(((t - 1) >> 1) & 1))) {
@@ -461,7 +481,7 @@ __global__ void __launch_bounds__(kThreads, 2)
             break;
           }
           tc::tc_fence_after();
-          const float f = rescale ? fast_exp2((m_ref - m) * c) : 1.f;
+          const float f = rescale ? fast_exp2(moved - minus) : 1.f;
           sum = fma_pair(sum, pack_pair(f, f), pack_pair(0.f, 0.f));
 #pragma unroll 1
           for (int h = 0; h < D / 16; ++h) {
@@ -473,18 +493,18 @@ __global__ void __launch_bounds__(kThreads, 2)
             tc::tmem_st16(t_o + lane_off + 16u * h, r);
           }
         }
-        if (grow) m_ref = m;
+        if (grow) {
+          m_ref = m;
+          minus = moved;
+        }
       }
-      // a row that has seen nothing keeps a finite base: its masked scores give
-      // 0, or 2^-126 where the polynomial is taken
-      const float mc = m_ref == -INFINITY ? 0.f : m_ref * c;
-      const float_pair minus = pack_pair(-mc, -mc);
+      const float_pair minus2 = pack_pair(minus, minus);
       float_pair part[2] = {sum, pack_pair(0.f, 0.f)};
       uint32_t pk[32];
 #pragma unroll
       for (int i = 0; i < 32; ++i) {
         const float_pair x = fma_pair(
-            pack_pair(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])), c2, minus);
+            pack_pair(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])), c2, minus2);
         float ea, eb;
         if ((kPolyPairs >> (i & 7)) & 1u) {
           float_pair q, scale;
@@ -511,7 +531,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     float l0, l1;
     unpack_pair(l0, l1, sum);
     const float l = have && m_ref != -INFINITY ? l0 + l1 : 0.f;
-    s_m[row] = m_ref * c;
+    s_m[row] = m_ref == -INFINITY ? -INFINITY : -minus;
     s_l[row] = l;
     const float inv = runs > 1 ? 1.f : (l == 0.f ? 0.f : 1.f / l);
     float4* part = reinterpret_cast<float4*>(

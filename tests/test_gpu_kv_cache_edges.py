@@ -1,0 +1,66 @@
+"""The streaming cache's operators at the edges of their types, layouts and
+arguments, on the GPU against plain 64-bit code.  The bounds are those of
+test_gpu_kv_cache.py; what a test adds to them it derives where it stands.
+"""
+import math
+
+import pytest
+import torch
+
+from test_gpu_kv_cache import BF, FP, Case
+
+pytestmark = pytest.mark.gpu
+
+
+# ------------------------------------------------------------------ attention
+@pytest.mark.parametrize("where", [0, 11990])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("new", [1, 70])
+def test_attention_keeps_the_tail_in_fp16(cuda, new, dim, where):
+    """One key 17.6 nats (2^25.4) above 12,000 others, with values of zero: the
+    output is what the others add up to.  A probability goes to the product
+    with V in fp16, shifted by 2^15 (single tokens) or 2^7 against a reference
+    that may lie 2^8 low: within the type's rounding, or half its least step."""
+    c = Case(cuda, [12000], [new], 1, 1, dim, 64, FP)
+    weak, strong = 0.5, 18.125
+    page = c.table[0, torch.arange(12000, device=cuda) // 64].long()
+    row = torch.arange(12000, device=cuda) % 64
+    k = torch.zeros(12000, 1, dim, device=cuda, dtype=FP)
+    k[:, :, 0] = weak
+    k[where, :, 0] = strong
+    v = (torch.rand(12000, 1, dim, generator=torch.Generator().manual_seed(1)) + 0.5).to(FP).to(cuda)
+    v[where] = 0
+    c.kp[page, :, row], c.vp[page, :, row] = k, v
+    c.q.zero_()
+    c.q[:, :, 0] = 1
+    out, lse = c.attend(True, scale=1.0)
+    for i in range(new):
+        n = 12000 - new + i + 1
+        sees = where < n
+        s = k[:n, 0, 0].double()
+        want_l = torch.logsumexp(s, 0)
+        p = torch.exp(s - want_l)
+        want = p @ v[:n, 0].double()
+        step = 2.0 ** -(25 + (15 if new == 1 else 7)) * 1.5 * n if sees else 0.0
+        bound = (2 * 2.0 ** -11 + 2.0 ** -13) * want + step
+        err = (out[i, 0].double() - want).abs()
+        assert bool((err <= bound).all()), (i, float((err / want).max()))
+        assert abs(float(lse[i, 0]) - float(want_l)) <= 2.0 ** -16 + 2.0 ** -20 * strong
+
+
+def test_attention_of_scores_beyond_fp16(cuda):
+    """Scores of 10^8, whose exponents fp32 holds to several units: the shifted
+    probabilities stay within the type, and the largest scores (exact in fp32,
+    the next ones 960,000 below) share the row."""
+    for new in (1, 70):
+        c = Case(cuda, [300], [new], 1, 1, 64, 16, FP)
+        c.q.zero_()
+        c.q[..., 0] = 30000
+        at = torch.arange(300, device=cuda)
+        c.kp[c.table[0, at // 16].long(), :, at % 16] = 0
+        c.kp[c.table[0, at // 16].long(), 0, at % 16, 0] = (4 * (at % 97) + 10).to(FP)
+        out, lse = c.attend(False, scale=8.0)
+        top = [j for j in range(300) if j % 97 == 96]
+        want = c.v[0][top, 0].double().mean(0)
+        assert bool(((out[:, 0].double() - want).abs() <= 2.0 ** -10 * want.abs() + 2.0 ** -10 * 4).all())
+        assert torch.isfinite(lse).all()
