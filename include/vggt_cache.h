@@ -119,7 +119,9 @@ int vggt_paged_attention(const void* q, int dtype, int64_t total, int64_t q_toke
  * Adds to each cached key's weight what the new tokens gave it:
  *   weights[j] = decay * weights[j] + sum_i exp(s_ij - lse_i)
  * over the rows i of its key head's group that see it (causal as above), lse
- * as vggt_paged_attention wrote it.  Slots past the length are left alone.
+ * as vggt_paged_attention wrote it.  A weight of +inf (a token that is never
+ * evicted) stays as it is, whatever the decay.  Slots past the length are left
+ * alone.
  */
 int vggt_paged_weights(const void* q, int dtype, int64_t total, int64_t q_token_stride,
                        int64_t q_head_stride, const float* lse, const void* k_pages,

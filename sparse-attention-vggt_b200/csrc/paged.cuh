@@ -182,6 +182,12 @@ cudaError_t launch_paged_weigh_tc05(const WeighArgs& a, cudaStream_t st);
 // first call and after every call, in a place that no call uses otherwise.
 constexpr int64_t kMaxCounters = VGGT_PAGED_WORKSPACE_ZERO_BYTES / 4;
 
+// A key's weight after a call.  +inf, which keeps a token from eviction, stays
+// whatever the decay (0 times it would be NaN, the lowest rank) and the sum.
+__device__ __forceinline__ float new_weight(float old, float decay, float sum) {
+  return old == INFINITY ? old : fmaf(old, decay, sum);
+}
+
 // How a launch cuts its work.
 struct PagedPlan {
   int rows;               // query rows per CTA

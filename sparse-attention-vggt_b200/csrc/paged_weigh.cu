@@ -224,7 +224,7 @@ __global__ void __launch_bounds__(kThreads, kCtas<D>)
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const int64_t key = key0 + (j >> 1) * 8 + lane * 2 + (j & 1);
-          if (key < len) weights[key] = fmaf(old[j], a.decay, sum[j]);
+          if (key < len) weights[key] = new_weight(old[j], a.decay, sum[j]);
         }
       }
     }

@@ -289,7 +289,8 @@ __global__ void __launch_bounds__(kThreads, 2)
     const int64_t key_at = tile0 * kKeys + sub * 32 + lane;
     if (row_tiles == 0) {  // no new tokens
       for (int kt = 0; kt < tiles; ++kt)
-        if (key_at + kt * kKeys < len) w[key_at + kt * kKeys] *= a.decay;
+        if (key_at + kt * kKeys < len)
+          w[key_at + kt * kKeys] = new_weight(w[key_at + kt * kKeys], a.decay, 0.f);
     }
     // The tiles in a row, those of the next key tile behind the last row tile.
     // A part's 32 columns are loaded under the exponentials of the part before,
@@ -397,7 +398,7 @@ __global__ void __launch_bounds__(kThreads, 2)
       if (next_kt != kt && key < len) {
         float x, y;
         unpack_pair(x, y, add_pair(sum[0], sum[1]));
-        w[key] = fmaf(old, a.decay, x + y);
+        w[key] = new_weight(old, a.decay, x + y);
       }
       kt = next_kt;
       rt = next_rt;

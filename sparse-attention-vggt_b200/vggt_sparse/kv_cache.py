@@ -151,8 +151,9 @@ def paged_weights(q, lse, k_pages, table, lengths, starts, weights, *, max_new, 
                   causal=True, scale=None, decay=1.0, status=None):
     """Add to ``weights`` (in place, returned) the probabilities that the new
     tokens' rows gave each cached key: decay * weights + sum exp(s - lse) over
-    the rows and the query heads of the key's head.  q, lse, lengths, starts,
-    causal and scale as in ``paged_attention``, whose lse it takes."""
+    the rows and the query heads of the key's head; weights of +inf stay.  q,
+    lse, lengths, starts, causal and scale as in ``paged_attention``, whose lse
+    it takes."""
     return _binding().weigh(q, lse, k_pages, table, lengths, starts, weights, max_new, max_len,
                             causal, scale, decay, status)
 

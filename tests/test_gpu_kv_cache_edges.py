@@ -7,7 +7,8 @@ import math
 import pytest
 import torch
 
-from test_gpu_kv_cache import BF, FP, Case
+import vggt_sparse
+from test_gpu_kv_cache import BF, FP, Case, ints
 
 pytestmark = pytest.mark.gpu
 
@@ -64,3 +65,33 @@ def test_attention_of_scores_beyond_fp16(cuda):
         want = c.v[0][top, 0].double().mean(0)
         assert bool(((out[:, 0].double() - want).abs() <= 2.0 ** -10 * want.abs() + 2.0 ** -10 * 4).all())
         assert torch.isfinite(lse).all()
+
+
+# ------------------------------------------------------------------ weights
+@pytest.mark.parametrize("decay", [0.0, 0.5, -1.0])
+@pytest.mark.parametrize("max_new", [1, 500])
+def test_weights_of_infinity_stay(cuda, max_new, decay):
+    """+inf keeps a token from eviction whatever the decay, in a sequence
+    without new tokens too and where the token's key is NaN; the other weights
+    are decay * weight + sum as ever."""
+    c = Case(cuda, [300, 40], [60, 0], 2, 1, 64, 16)
+    out, lse = c.attend(True)
+    w0 = torch.rand(2, 2, c.table.shape[1] * 16, device=cuda)
+    w0[:, :, 1:300:7] = math.inf
+    c.kp[int(c.table[0, 0]), :, 8] = math.nan
+    w = w0.clone()
+    vggt_sparse.paged_weights(c.q, lse, c.kp, c.table, c.len, c.starts, w, max_new=max_new,
+                              decay=decay, status=c.status)
+    added = torch.zeros_like(w0)
+    vggt_sparse.paged_weights(c.q, lse, c.kp, c.table, c.len, c.starts, added, max_new=max_new)
+    pinned = w0 == math.inf
+    assert bool((w[pinned] == math.inf).all()) and int(c.status) == 0
+    for b, n in enumerate(c.lengths):
+        want = (w0[b, :, :n] * decay + added[b, :, :n])[~pinned[b, :, :n]]
+        got = w[b, :, :n][~pinned[b, :, :n]]
+        assert bool(((got - want).abs() <= 2.0 ** -22 * (1 + added.nan_to_num().max())).all())
+    ids = torch.arange(w.shape[2], device=cuda, dtype=torch.int32).expand(2, 2, -1).contiguous()
+    _, kept, n = vggt_sparse.paged_evict(w, ids, c.kp, c.vp, c.table, c.len, 50)
+    assert n.tolist() == [50, 40]
+    for h in range(2):
+        assert set(range(1, 300, 7)) <= set(kept[0, h, :50].tolist())
