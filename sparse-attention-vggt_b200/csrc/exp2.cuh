@@ -48,8 +48,10 @@ __device__ __forceinline__ float max_nan(float a, float b) {
 // 2^x of a pair for arguments up to 126 without the multi-function unit, as
 // q * scale: x = n + f with n = round(x) (adding 1.5 * 2^23 leaves it in the low
 // mantissa bits), q a polynomial of degree 4 for 2^f on [-1/2, 1/2] (fitted to
-// the least largest relative error, 2.7e-6 in fp32), scale = 2^n.  Arguments
-// below -126 give 2^-126 at most; a NaN stays one (in q).
+// the least largest relative error, 2.7e-6 in fp32), scale = 2^n.  Where n would
+// be below -126 the exponent's bits come to zero, and scale with them: -inf
+// gives exactly 0, as a masked score must (2^-126 is a number of bf16, and times
+// a value of 1e38 one that shows).  A NaN stays one (in q).
 struct Exp2Poly {
   float_pair magic, c4, c3, c2, c1, c0;
   __device__ __forceinline__ Exp2Poly()
@@ -62,7 +64,7 @@ struct Exp2Poly {
   __device__ __forceinline__ void operator()(float_pair& q, float_pair& scale, float_pair x) const {
     float a, b, ta, tb;
     unpack_pair(a, b, x);
-    x = pack_pair(max_nan(a, -126.f), max_nan(b, -126.f));
+    x = pack_pair(max_nan(a, -127.f), max_nan(b, -127.f));
     const float_pair t = add_pair(x, magic);
     const float_pair f = sub_pair(x, sub_pair(t, magic));
     q = fma_pair(f, c4, c3);

@@ -409,7 +409,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     // The reference in score units, and what is added to a score's exponent:
     // PRange's shift less the reference, rounded down, so that the largest P is
     // known however large the scores are.  A row that has seen nothing keeps 0:
-    // its masked scores give 0, or 2^-126 where the polynomial is taken.
+    // its masked scores give 0.
     float m_ref = -INFINITY, minus = 0.f;
     float_pair sum = pack_pair(0.f, 0.f);
     const float_pair c2 = pack_pair(c, c);

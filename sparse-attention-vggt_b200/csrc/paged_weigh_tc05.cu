@@ -361,7 +361,6 @@ __global__ void __launch_bounds__(kThreads, 2)
           if (decltype(masked)::value && (col0 >= left || col0 + 32 <= lo_warp)) continue;
           uint32_t* sc = s[part & 1];
           if (decltype(masked)::value && (col0 + 32 > left || col0 < hi_warp)) {
-            // gives 0, or 2^-126 where the polynomial is taken
 #pragma unroll
             for (int i = 0; i < 32; ++i)
               if (col0 + i < lo || col0 + i >= left) sc[i] = __float_as_uint(-INFINITY);

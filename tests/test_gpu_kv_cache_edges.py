@@ -67,6 +67,24 @@ def test_attention_of_scores_beyond_fp16(cuda):
         assert torch.isfinite(lse).all()
 
 
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("new", [5, 200])
+def test_attention_large_values_of_later_tokens(cuda, new, dim):
+    """Values of 1e38 (bf16) in the chunk's later tokens, in every column of a
+    tile: rows that do not see them are the same bits as with zeros there."""
+    c = Case(cuda, [450, 200], [new, new], 1, 2, dim, 16, BF)
+    first = new // 2
+    at = torch.arange(450 - new + first, 450, device=cuda)
+    page = c.table[0, at // 16].long()
+    c.vp[page, :, at % 16] = 0
+    want, want_lse = c.attend(True)
+    c.vp[page, :, at % 16] = 1e38
+    out, lse = c.attend(True)
+    assert torch.equal(out[:first], want[:first]) and torch.equal(lse[:first], want_lse[:first])
+    assert torch.equal(out[new:], want[new:])
+    assert bool((out[first:new].abs() > 1e30).all())
+
+
 # ------------------------------------------------------------------ weights
 @pytest.mark.parametrize("decay", [0.0, 0.5, -1.0])
 @pytest.mark.parametrize("max_new", [1, 500])
