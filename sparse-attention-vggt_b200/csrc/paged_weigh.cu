@@ -105,19 +105,20 @@ __global__ void __launch_bounds__(kThreads, kCtas<D>)
   } else {
     const int krow = ((lane >> 4) & 1) * 8 + (lane & 7), kchunk = (lane >> 3) & 1;
     const int qrow = ((lane >> 3) & 1) * 8 + (lane & 7), qchunk = (lane >> 4) & 1;
-    // rows c0 .. c0 + 63 into shared memory; rows that are not there are zeros
-    // with lse +inf, which gives nothing
+    // rows c0 .. c0 + 63 into shared memory, filled up to a multiple of 16 with
+    // the first one, its limit and lse +inf, which gives nothing (rows of zeros
+    // would give NaN against a key with an infinite element, whose scores may
+    // all be -inf)
     auto load_rows = [&](int c0) {
       const int here = rows - c0 < kRowsMax ? rows - c0 : kRowsMax;
+#pragma unroll
       for (int i = tid; i < kRowsMax * (D / 8); i += 128) {
         const int r = i / (D / 8), c = i % (D / 8);
-        uint4 v = make_uint4(0u, 0u, 0u, 0u);
-        if (r < here) {
-          const int row = c0 + r;
-          v = __ldg(reinterpret_cast<const uint4*>(
-              static_cast<const T*>(a.q) + (first + row / a.group) * a.q_token +
-              ((int64_t)head * a.group + row % a.group) * a.q_head + c * 8));
-        }
+        if (r >= (here + 15) / 16 * 16) break;
+        const int row = c0 + (r < here ? r : 0);
+        const uint4 v = __ldg(reinterpret_cast<const uint4*>(
+            static_cast<const T*>(a.q) + (first + row / a.group) * a.q_token +
+            ((int64_t)head * a.group + row % a.group) * a.q_head + c * 8));
         const uint32_t dst =
             q_addr + (c >> 3) * (kRowsMax * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4);
         asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "r"(v.x), "r"(v.y),
@@ -125,7 +126,7 @@ __global__ void __launch_bounds__(kThreads, kCtas<D>)
                      : "memory");
       }
       if (tid < kRowsMax) {
-        const int row = c0 + tid;
+        const int row = c0 + (tid < here ? tid : 0);
         float l = -INFINITY;
         if (tid < here)
           l = a.lse[(first + row / a.group) * ((int64_t)a.pool.kv_heads * a.group) +

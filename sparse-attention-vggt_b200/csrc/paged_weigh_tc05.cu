@@ -124,9 +124,23 @@ __global__ void __launch_bounds__(kThreads, 2)
     s_abort = 0;
     tc::mbar_fence_init();
   }
-  // rows of a Q tile past tile_rows are never loaded: zeros, with lse +inf
-  for (int i = tid; i < kStages * (int)L::kTile / 16; i += kThreads)
-    reinterpret_cast<uint4*>(sbase + L::kQ)[i] = make_uint4(0u, 0u, 0u, 0u);
+  // Rows of a Q tile past tile_rows are never loaded.  They hold the last token,
+  // which sees every key, with lse +inf: that gives nothing, or NaN where the
+  // token itself does.  (Zeros would give NaN against a key with an infinite
+  // element, whose scores may all be -inf; to mask the columns in every tile
+  // took a frame with groups of three and seven a third longer.)
+  if (n_new > 0) {
+    const T* last = static_cast<const T*>(a.q) + (first + n_new - 1) * a.q_token +
+                    (int64_t)head * group * a.q_head;
+    const int pad = kCols - tile_rows;
+    for (int i = tid; i < pad * (D / 8); i += kThreads) {
+      const int r = tile_rows + i / (D / 8), c = i % (D / 8);
+      const uint4 v = __ldg(reinterpret_cast<const uint4*>(last) + c);
+      for (int s = 0; s < kStages; ++s)
+        *reinterpret_cast<uint4*>(sbase + L::kQ + s * L::kTile + (c >> 3) * L::kHalf + r * 128 +
+                                  (((c & 7) ^ (r & 7)) << 4)) = v;
+    }
+  }
   for (int i = tid; i < kLseStages * kCols; i += kThreads) s_lse[i / kCols][i % kCols] = -INFINITY;
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   if (warp == 1) {

@@ -113,3 +113,27 @@ def test_weights_of_infinity_stay(cuda, max_new, decay):
     assert n.tolist() == [50, 40]
     for h in range(2):
         assert set(range(1, 300, 7)) <= set(kept[0, h, :50].tolist())
+
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("max_new", [1, 500])
+@pytest.mark.parametrize("new,group", [(1, 1), (2, 7), (40, 7), (90, 3), (70, 65), (17, 1)])
+def test_weights_of_keys_that_nobody_looks_at(cuda, new, group, max_new, causal):
+    """Keys with an infinite element whose scores are all -inf receive nothing,
+    whatever fills up the tiles of rows: their weights stay, and the others are
+    what they are without such keys."""
+    c = Case(cuda, [300], [new], 1, group, 64, 16)
+    c.q[..., 5] = -(c.q[..., 5].abs() + 0.5)
+    at = torch.arange(0, 300, 3, device=cuda)
+    where = c.table[0, at // 16].long(), 0, at % 16, 5
+    c.kp[where] = 1e4  # scores of -600 and less: exponentials of zero
+    out, lse = c.attend(causal)
+
+    def weights():
+        w = torch.full((1, 1, c.table.shape[1] * 16), 0.25, device=cuda)
+        return vggt_sparse.paged_weights(c.q, lse, c.kp, c.table, c.len, c.starts, w,
+                                         max_new=max_new, causal=causal, status=c.status)[0, 0]
+    want = weights()
+    assert bool((want[at] == 0.25).all())
+    c.kp[where] = math.inf
+    assert torch.equal(weights(), want) and int(c.status) == 0
