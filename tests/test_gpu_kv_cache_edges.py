@@ -137,3 +137,27 @@ def test_weights_of_keys_that_nobody_looks_at(cuda, new, group, max_new, causal)
     assert bool((want[at] == 0.25).all())
     c.kp[where] = math.inf
     assert torch.equal(weights(), want) and int(c.status) == 0
+
+
+# ------------------------------------------------------------------ the streaming layer
+@pytest.mark.parametrize("budget,special", [(41, 5), (50, 5), (60, 5), (82, 5), (70, 0), (45, 1)])
+def test_streaming_layer_keeps_what_it_promises(cuda, budget, special):
+    """Streams far past the point where the special tokens of all frames no
+    longer fit: after each frame the cache holds the whole frame and the special
+    tokens of the first frames, as many as there is room for."""
+    g = torch.Generator().manual_seed(budget)
+    per = 41
+    layer = vggt_sparse.StreamingGlobalLayer(2, 64, per, budget, special=special, page=16, device=cuda)
+    pos = torch.arange(2 * per).reshape(per, 2).to(torch.int32).to(cuda)
+    pinned = (budget - per) // special if special else 0
+    for f in range(pinned + 8):
+        layer(*(torch.randn(per, 2, 64, generator=g).to(BF).to(cuda) for _ in range(3)), pos)
+        n = layer.cache.lengths[0]
+        assert n == min(budget, (f + 1) * per)
+        for h in range(2):
+            held = set(layer.cache.ids[0, h, :n].tolist())
+            assert len(held) == n
+            assert set(range(f * per, (f + 1) * per)) <= held, f
+            assert {e * per + i for e in range(min(f + 1, pinned)) for i in range(special)} <= held, f
+    layer.cache.check()
+    assert layer.pinned_frames == pinned
