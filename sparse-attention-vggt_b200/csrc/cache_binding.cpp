@@ -153,16 +153,33 @@ void plain_strides(Pools& p) {
   if (p.pages == 1) p.page_stride = p.heads * p.head_stride;
 }
 
-// [tokens, heads, dim] with strides that the kernels take, else a copy.
-at::Tensor rows_of(const char* name, const at::Tensor& t, const at::Tensor& pages, int64_t heads) {
+// Packed rows [tokens, heads, dim] and their strides.
+struct Rows {
+  at::Tensor t;
+  int64_t token, head;
+  explicit Rows(const at::Tensor& x) : t(x) {
+    // those of a dimension of size one are never used, and may be anything
+    head = t.size(1) == 1 ? t.size(2) : t.stride(1);
+    token = t.size(0) == 1 ? t.size(1) * head : t.stride(0);
+  }
+  // whether the attention kernels take them as they are
+  bool fit() const {
+    return t.stride(2) == 1 && token % 8 == 0 && head % 8 == 0 &&
+           reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
+  }
+};
+
+// A tensor argument with strides and an address that the kernels take, else a
+// copy.  (A contiguous one at any address will do for append.)
+Rows rows_of(const char* name, const at::Tensor& t, const at::Tensor& pages, int64_t heads,
+             bool aligned) {
   if (t.dim() != 3 || t.size(2) != pages.size(3) || t.scalar_type() != pages.scalar_type() ||
       (heads > 0 && t.size(1) != heads))
     refuse("%s must be [tokens, heads, dim] with the pools' dim, dtype%s", name,
            heads > 0 ? " and heads" : "");
-  if (t.stride(2) != 1 || t.stride(0) % 8 || t.stride(1) % 8 ||
-      reinterpret_cast<uintptr_t>(t.data_ptr()) % 16)
-    return t.contiguous();
-  return t;
+  const Rows rows(t);
+  if (rows.fit()) return rows;
+  return Rows(aligned ? t.clone(at::MemoryFormat::Contiguous) : t.contiguous());
 }
 
 struct Turn {
@@ -281,8 +298,9 @@ PyObject* append(PyObject*, PyObject* const* a, Py_ssize_t n) {
                      *status = tensor_or_none(a[16], "status");
     Pools p = pools_of(kp, &vp, table);
     plain_strides(p);
-    const at::Tensor k = rows_of("k", tensor(a[0], "k"), kp, p.heads);
-    const at::Tensor v = rows_of("v", tensor(a[1], "v"), kp, p.heads);
+    const Rows kr = rows_of("k", tensor(a[0], "k"), kp, p.heads, false);
+    const Rows vr = rows_of("v", tensor(a[1], "v"), kp, p.heads, false);
+    const at::Tensor &k = kr.t, &v = vr.t;
     const int64_t total = k.size(0);
     if (v.size(0) != total) refuse("k and v must have the same shape");
     const Turn t = turn_of(pos, freq, a[9], total);
@@ -307,8 +325,8 @@ PyObject* append(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const c10::cuda::CUDAGuard guard(device);
     const at::Tensor after = given ? *given : at::empty({p.seqs}, before.options());
     check(vggt_paged_append(
-        k.data_ptr(), v.data_ptr(), p.dtype, total, k.stride(0), k.stride(1), v.stride(0),
-        v.stride(1), kp.data_ptr(), vp.data_ptr(), p.pages, (int)p.heads, (int)p.page, (int)p.dim,
+        k.data_ptr(), v.data_ptr(), p.dtype, total, kr.token, kr.head, vr.token,
+        vr.head, kp.data_ptr(), vp.data_ptr(), p.pages, (int)p.heads, (int)p.page, (int)p.dim,
         p.page_stride, p.head_stride, p.row_stride, p.table, p.width, p.seqs,
         static_cast<const int32_t*>(before.data_ptr()),
         static_cast<const int32_t*>(starts.data_ptr()), t.positions, t.axes, t.freq, t.pairs,
@@ -338,7 +356,8 @@ PyObject* attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
                      *status = tensor_or_none(a[13], "status");
     Pools p = pools_of(kp, &vp, table);
     plain_strides(p);
-    const at::Tensor q = rows_of("q", tensor(a[0], "q"), kp, 0);
+    const Rows qr = rows_of("q", tensor(a[0], "q"), kp, 0, true);
+    const at::Tensor& q = qr.t;
     const int64_t total = q.size(0), heads = q.size(1), group = group_of(q, p);
     if (group > 65535) refuse("too many heads");
     need("lengths", lengths, at::kInt, {p.seqs});
@@ -348,8 +367,7 @@ PyObject* attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const float scale =
         a[9] == Py_None ? 1.f / std::sqrt((float)p.dim) : (float)number(a[9], "scale");
     if (given && (given->sizes() != q.sizes() || given->scalar_type() != q.scalar_type() ||
-                  given->stride(2) != 1 || given->stride(0) % 8 || given->stride(1) % 8 ||
-                  reinterpret_cast<uintptr_t>(given->data_ptr()) % 16))
+                  !Rows(*given).fit()))
       refuse("out must have q's shape and dtype and 16-byte aligned rows");
     if (given_lse) need("lse", *given_lse, at::kFloat, {total, heads});
     int32_t* word = status_of(status);
@@ -357,6 +375,7 @@ PyObject* attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
                                           space, status);
     const c10::cuda::CUDAGuard guard(device);
     const at::Tensor out = given ? *given : at::empty(q.sizes(), q.options());
+    const Rows to(out);
     const at::Tensor lse =
         given_lse ? *given_lse : at::empty({total, heads}, q.options().dtype(at::kFloat));
     const size_t bytes = vggt_paged_attention_workspace_size(
@@ -364,11 +383,11 @@ PyObject* attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const cudaStream_t stream = c10::cuda::getCurrentCUDAStream().stream();
     const at::Tensor ws = space ? *space : workspace_of(bytes, device, stream);
     check(vggt_paged_attention(
-        q.data_ptr(), p.dtype, total, q.stride(0), q.stride(1), kp.data_ptr(), vp.data_ptr(),
+        q.data_ptr(), p.dtype, total, qr.token, qr.head, kp.data_ptr(), vp.data_ptr(),
         p.pages, (int)p.heads, (int)p.page, (int)p.dim, p.page_stride, p.head_stride, p.row_stride,
         p.table, p.width, p.seqs, static_cast<const int32_t*>(lengths.data_ptr()),
         static_cast<const int32_t*>(starts.data_ptr()), (int)group, truth(a[8]), scale, max_new,
-        max_len, out.data_ptr(), out.stride(0), out.stride(1), static_cast<float*>(lse.data_ptr()),
+        max_len, out.data_ptr(), to.token, to.head, static_cast<float*>(lse.data_ptr()),
         word, ws.data_ptr(), ws.numel() * ws.element_size(), stream));
     PyObject *o = returned(a[10], out), *l = returned(a[11], lse);
     PyObject* both = o && l ? PyTuple_Pack(2, o, l) : nullptr;
@@ -386,7 +405,8 @@ PyObject* weigh(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const at::Tensor* status = tensor_or_none(a[12], "status");
     Pools p = pools_of(kp, nullptr, table);
     plain_strides(p);
-    const at::Tensor q = rows_of("q", tensor(a[0], "q"), kp, 0);
+    const Rows qr = rows_of("q", tensor(a[0], "q"), kp, 0, true);
+    const at::Tensor& q = qr.t;
     const int64_t total = q.size(0), heads = q.size(1), group = group_of(q, p);
     if (group > 65535) refuse("too many heads");
     need("lse", lse, at::kFloat, {total, heads});
@@ -400,7 +420,7 @@ PyObject* weigh(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const c10::cuda::CUDAGuard guard(
         one_device(q, &lse, &kp, &table, &lengths, &starts, &weights, status));
     check(vggt_paged_weights(
-        q.data_ptr(), p.dtype, total, q.stride(0), q.stride(1),
+        q.data_ptr(), p.dtype, total, qr.token, qr.head,
         static_cast<const float*>(lse.data_ptr()), kp.data_ptr(), p.pages, (int)p.heads,
         (int)p.page, (int)p.dim, p.page_stride, p.head_stride, p.row_stride, p.table, p.width,
         p.seqs, static_cast<const int32_t*>(lengths.data_ptr()),

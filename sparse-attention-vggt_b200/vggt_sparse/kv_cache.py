@@ -15,12 +15,13 @@ cache is paged, bounded by eviction, and served by five operators:
 ``PagedKVCache`` holds pools, page tables, lengths, ids and weights, gives out
 pages and calls the operators in turn.
 
-Layouts.  Pools are [pages, kv_heads, page, dim] bf16 or fp16 (any strides
-whose last dimension is contiguous, K and V alike; dim 64 or 128, page a power
-of two from 16 to 1024).  ``table`` [seqs, width] int32 names the pages of
+Layouts.  Pools are [pages, kv_heads, page, dim] bf16 or fp16 (strides that are
+multiples of 8 elements, the last dimension contiguous, 16-byte aligned, K and V
+alike; dim 64 or 128, page a power of two from 16 to 1024).  ``table`` [seqs, width] int32 names the pages of
 each sequence; slot s lies in page table[b, s // page].  New tokens of all
 sequences are packed: rows starts[b] .. starts[b + 1] of q, k and v
-[tokens, heads, dim] belong to sequence b.  ids and weights are
+[tokens, heads, dim] belong to sequence b; where their strides or address do not
+suit the kernels they are copied.  ids and weights are
 [seqs, kv_heads, width * page].
 
 Like the other operators these only enqueue work on the current stream.

@@ -161,3 +161,43 @@ def test_streaming_layer_keeps_what_it_promises(cuda, budget, special):
             assert {e * per + i for e in range(min(f + 1, pinned)) for i in range(special)} <= held, f
     layer.cache.check()
     assert layer.pinned_frames == pinned
+
+
+# ------------------------------------------------------------------ arguments
+@pytest.mark.parametrize("new,heads,group", [(1, 2, 2), (1, 1, 1), (20, 1, 1), (60, 2, 2)])
+def test_rows_of_any_stride_and_address(cuda, new, heads, group):
+    """q as a contiguous tensor that is not 16-byte aligned, with an odd stride
+    of its one token or its one head, and with a strided last dimension: copied
+    where need be, the same bits.  So are outputs of one token or head."""
+    c = Case(cuda, [200], [new], heads, group, 64, 16)
+    n, h, d = c.q.shape
+    out, lse = c.attend(True)
+
+    def weights(q):
+        w = torch.zeros(1, heads, c.table.shape[1] * 16, device=cuda)
+        return vggt_sparse.paged_weights(q, lse, c.kp, c.table, c.len, c.starts, w, max_new=new)
+    want_w, q0 = weights(c.q), c.q
+    shifted = torch.empty(q0.numel() + 1, device=cuda, dtype=BF)[1:].view(n, h, d)
+    wide = torch.empty(n, h * d + 5, device=cuda, dtype=BF)[:, :h * d].unflatten(1, (h, d))
+    odd = torch.empty(n, h, d + 3, device=cuda, dtype=BF)[:, :, :d]
+    apart = torch.empty(n, h, d, 2, device=cuda, dtype=BF)[..., 0]
+    for q in (shifted, wide, odd, apart):
+        q.copy_(q0)
+        c.q = q
+        got, got_lse = c.attend(True)
+        assert torch.equal(got, out) and torch.equal(got_lse, lse)
+        assert torch.equal(weights(q), want_w)
+    c.q = q0
+    if n == 1:
+        o = torch.empty(1, h * d + 5, device=cuda, dtype=BF)[:, :h * d].unflatten(1, (h, d))
+        assert torch.equal(c.attend(True, out=o)[0], out) and torch.equal(o, out)
+    if h == 1:
+        o = torch.empty(n, d, 1, device=cuda, dtype=BF).transpose(1, 2)
+        o = o.as_strided((n, 1, d), (d, 3, 1))
+        assert torch.equal(c.attend(True, out=o)[0], out) and torch.equal(o, out)
+    for k in (shifted, wide) if group == 1 else ():
+        kp, vp = c.kp.clone(), c.vp.clone()
+        vggt_sparse.paged_append(q0, q0, c.kp, c.vp, c.table, c.len - new, c.starts)
+        vggt_sparse.paged_append(k, k, kp, vp, c.table, c.len - new, c.starts)
+        same = lambda x, y: torch.equal(x.nan_to_num(7.0), y.nan_to_num(7.0))  # noqa: E731
+        assert same(kp, c.kp) and same(vp, c.vp)
