@@ -90,10 +90,12 @@ int vggt_paged_append(const void* k, const void* v, int dtype, int64_t total,
  * sees slots j <= lengths[b] - n + i, else all of its sequence's slots:
  *   s_ij = scale q_i . k_j,  lse_i = log sum_j exp s_ij,
  *   out_i = sum_j exp(s_ij - lse_i) v_j
- * A row that sees no key gets zeros and lse -inf.  Slots past the length are
- * never used, whatever they hold; keys and values that only later tokens see
- * do not reach a row, finite or not.  lse [total][kv_heads * group] fp32, or
- * NULL.
+ * A row that sees no key gets zeros and lse -inf.  So does a row that belongs
+ * to no sequence (before starts[0], or at or past starts[seqs]), which also
+ * sets VGGT_STATUS_BAD_LENGTH; with seqs == 0 nothing is written.  Slots past
+ * the length are never used, whatever they hold; keys and values that only
+ * later tokens see do not reach a row, finite or not.  lse
+ * [total][kv_heads * group] fp32, or NULL.
  *
  * max_new and max_len are the most new tokens of a sequence and the greatest
  * length as the caller expects them; they choose the kernel and how the work

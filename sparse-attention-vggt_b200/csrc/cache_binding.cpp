@@ -378,6 +378,11 @@ PyObject* attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const Rows to(out);
     const at::Tensor lse =
         given_lse ? *given_lse : at::empty({total, heads}, q.options().dtype(at::kFloat));
+    if (p.seqs == 0) {  // the rows belong to no sequence; no kernel will run
+      out.zero_();
+      lse.fill_(-INFINITY);
+      if (status && total > 0) status->flatten().narrow(0, 0, 1).bitwise_or_(VGGT_STATUS_BAD_LENGTH);
+    }
     const size_t bytes = vggt_paged_attention_workspace_size(
         total, p.seqs, (int)p.heads, (int)group, (int)p.dim, max_new, max_len);
     const cudaStream_t stream = c10::cuda::getCurrentCUDAStream().stream();

@@ -148,6 +148,33 @@ struct PagedAttnArgs {
   int wait_selftest;
 };
 
+// Zeros and -inf for the packed rows that belong to no sequence, those before
+// the first start and behind the last.  Every CTA calls it once, by one of its
+// warps, and takes its share of them.
+template <typename T, int D>
+__device__ __forceinline__ void fill_rows_of_no_sequence(const PagedAttnArgs& a) {
+  const int64_t total = a.t.total;
+  int64_t lo = __ldg(a.t.starts), hi = __ldg(a.t.starts + a.t.seqs);
+  lo = lo < 0 ? 0 : (lo < total ? lo : total);
+  hi = hi < lo ? lo : (hi < total ? hi : total);
+  const int64_t rows = lo + total - hi;
+  if (rows == 0) return;
+  const int lane = threadIdx.x & 31;
+  if (blockIdx.x == 0 && lane == 0) raise_status(a.t.status, VGGT_STATUS_BAD_LENGTH);
+  const int heads = a.pool.kv_heads * a.group;
+#pragma unroll 1
+  for (int64_t i = blockIdx.x; i < rows; i += gridDim.x) {
+    const int64_t row = i < lo ? i : hi + i - lo;
+#pragma unroll 1
+    for (int j = lane; j < heads * (D / 8); j += 32)
+      reinterpret_cast<uint4*>(static_cast<T*>(a.out) + row * a.o_token +
+                               j / (D / 8) * a.o_head)[j % (D / 8)] = make_uint4(0u, 0u, 0u, 0u);
+    if (a.lse != nullptr)
+#pragma unroll 1
+      for (int j = lane; j < heads; j += 32) a.lse[row * heads + j] = -INFINITY;
+  }
+}
+
 struct WeighArgs {
   const void* q;
   int64_t q_token, q_head;

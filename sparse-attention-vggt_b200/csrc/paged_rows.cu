@@ -83,7 +83,10 @@ __global__ void __launch_bounds__(kThreads, 2)
   const int head = (int)(item % p.heads);
   const PagedAttnArgs& a = p.a;
   RowTile rt;
-  if (!locate_tile(a.t, a.pool, a.group, kRows, item / p.heads, rt)) return;
+  if (!locate_tile(a.t, a.pool, a.group, kRows, item / p.heads, rt)) {
+    if (warp == 0) fill_rows_of_no_sequence<T, D>(a);
+    return;
+  }
   const int64_t len = rt.len;
   const int rows = rt.rows - rt.row0 < kRows ? rt.rows - rt.row0 : kRows;
   // keys that row r of the tile sees
@@ -97,7 +100,10 @@ __global__ void __launch_bounds__(kThreads, 2)
   int64_t chunk = (all_tiles + p.splits - 1) / p.splits;
   if (chunk < p.chunk) chunk = p.chunk;
   const int64_t runs = all_tiles > 0 ? (all_tiles + chunk - 1) / chunk : 1;
-  if (split >= runs) return;
+  if (split >= runs) {
+    if (warp == 0) fill_rows_of_no_sequence<T, D>(a);
+    return;
+  }
   const int64_t tile0 = split * chunk;
   const int64_t tiles = all_tiles - tile0 < chunk ? all_tiles - tile0 : chunk;
 
@@ -170,6 +176,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     for (int64_t t = from; t < issued; ++t)
       tc::mbar_wait_drain(full((int)(t % R::kStages)), (uint32_t)((t / R::kStages) & 1),
                           1000000000ull);
+    fill_rows_of_no_sequence<T, D>(a);  // while the others finish
   } else {
     // ================= S, softmax, O =================
     const int kg = warp;

@@ -61,7 +61,8 @@ namespace vggt {
 namespace {
 
 constexpr int kRows = 128, kTile = 64;
-// Warps 0-3: TMA producer, S issuer, O issuer, one idle; warps 4-7: softmax.
+// Warps 0-3: TMA producer, S issuer, O issuer, and one that only fills rows of no
+// sequence; warps 4-7: softmax.
 constexpr int kThreads = 256;
 // setmaxnreg: the launch gives every thread kLaunchRegs (two CTAs fill the
 // register file); warps 0-3 give back down to kControlRegs, the softmax takes
@@ -157,11 +158,17 @@ __global__ void __launch_bounds__(kThreads, 2)
   const int tile = p.tiles - 1 - (int)(w % (unsigned)p.tiles);
   const int64_t item = (int64_t)head * p.tiles + tile;
   RowTile rt;
-  if (!locate_tile(a.t, a.pool, a.group, kRows, tile, rt)) return;
+  if (!locate_tile(a.t, a.pool, a.group, kRows, tile, rt)) {
+    if (warp == 0) fill_rows_of_no_sequence<T, D>(a);
+    return;
+  }
   const int rows = rt.rows - rt.row0 < kRows ? rt.rows - rt.row0 : kRows;
   const Runs cut = runs_of(p, rt, rows);
   const int runs = cut.count;
-  if (split >= runs) return;
+  if (split >= runs) {
+    if (warp == 0) fill_rows_of_no_sequence<T, D>(a);
+    return;
+  }
   const int first_key = split * cut.chunk * kTile;
   const int tiles = min(cut.tiles - split * cut.chunk, cut.chunk);
 
@@ -370,6 +377,8 @@ __global__ void __launch_bounds__(kThreads, 2)
       }
       __syncwarp();
       tc::mbar_wait_drain(smem_u32(&bars.drain[warp - 1]), 0, kDrainNs);
+    } else {
+      fill_rows_of_no_sequence<T, D>(a);
     }
     return;  // what follows runs on the softmax warps alone
   }

@@ -137,7 +137,8 @@ def paged_attention(q, k_pages, v_pages, table, lengths, starts, *, max_new, max
     heads); ``lengths`` count the new tokens.  With ``causal`` new token i of n
     sees the slots up to lengths[b] - n + i, otherwise every slot of its
     sequence.  lse [tokens, q_heads] fp32 is the row's log-sum-exp; a row
-    without keys gives zeros and -inf.
+    without keys gives zeros and -inf, and so does one that belongs to no
+    sequence (STATUS_BAD_LENGTH).
 
     ``max_new`` and ``max_len`` (default: all the table can hold) are the most
     new tokens of a sequence and the greatest length expected: they choose the

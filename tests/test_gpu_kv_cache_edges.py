@@ -8,6 +8,7 @@ import pytest
 import torch
 
 import vggt_sparse
+from vggt_sparse import _lib
 from test_gpu_kv_cache import BF, FP, Case, ints
 
 pytestmark = pytest.mark.gpu
@@ -201,3 +202,33 @@ def test_rows_of_any_stride_and_address(cuda, new, heads, group):
         vggt_sparse.paged_append(k, k, kp, vp, c.table, c.len - new, c.starts)
         same = lambda x, y: torch.equal(x.nan_to_num(7.0), y.nan_to_num(7.0))  # noqa: E731
         assert same(kp, c.kp) and same(vp, c.vp)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("new,length", [(1, 70), (3, 5000), (90, 300), (90, 5000)])
+def test_attention_rows_of_no_sequence(cuda, new, length, dim):
+    """Rows before the first start and behind the last one give zeros and -inf
+    and set a status bit; those of the sequences are what they are alone."""
+    c = Case(cuda, [length, length // 2], [new, new], 1, 2, dim, 16)
+    out, lse = c.attend(True)
+    c.check(out, lse, True)
+    q = torch.randn(2 * new + 5, 2, dim, device=cuda).to(BF)
+    q[3:-2] = c.q
+    o, l = torch.full_like(q, 7.0), torch.full(q.shape[:2], 7.0, device=cuda)
+    vggt_sparse.paged_attention(q, c.kp, c.vp, c.table, c.len, c.starts + 3, max_new=new, out=o,
+                                lse=l, status=c.status)
+    assert int(c.status) == _lib.STATUS_BAD_LENGTH
+    rest = torch.tensor([0, 1, 2, 2 * new + 3, 2 * new + 4], device=cuda)
+    assert bool((o[rest] == 0).all()) and bool((l[rest] == -math.inf).all())
+    # the split goes by the rows, so that sums may be cut elsewhere
+    c.status.zero_()
+    c.check(o[3:-2], l[3:-2], True)
+    o, l = vggt_sparse.paged_attention(q, c.kp, c.vp, c.table, c.len, torch.zeros_like(c.starts),
+                                       max_new=new, status=c.status)
+    assert bool((o == 0).all()) and bool((l == -math.inf).all())
+    assert int(c.status) == _lib.STATUS_BAD_LENGTH
+    c.status.zero_()
+    o, l = vggt_sparse.paged_attention(q, c.kp, c.vp, c.table[:0], c.len[:0], c.starts[:1],
+                                       max_new=new, out=torch.full_like(q, 7.0), status=c.status)
+    assert bool((o == 0).all()) and bool((l == -math.inf).all())
+    assert int(c.status) == _lib.STATUS_BAD_LENGTH
