@@ -24,6 +24,11 @@ sequences are packed: rows starts[b] .. starts[b + 1] of q, k and v
 suit the kernels they are copied.  ids and weights are
 [seqs, kv_heads, width * page].
 
+Gradients.  ``rotary`` is differentiable in x.  The cache holds values: what is
+appended to it takes no part in a graph, nor do weights.  ``paged_attention`` has
+no gradient; called with grad mode on and a q (or pools) that requires one, its
+results are part of the graph, and a backward pass through them raises.
+
 Like the other operators these only enqueue work on the current stream.
 Page numbers, lengths and starts are checked on the device; ``status`` (an
 int32 tensor) collects VGGT_STATUS_* bits, see ``check_cache_status``.
@@ -51,6 +56,41 @@ def _binding():
         from . import _cache_binding
         _module = _cache_binding
     return _module
+
+
+class _Rotary(torch.autograd.Function):
+    """The map is linear, its transpose the turn the other way."""
+
+    @staticmethod
+    def forward(ctx, x, positions, frequencies, layout, lengthen, inverse, out):
+        ctx.save_for_backward(positions, frequencies)
+        ctx.turn = layout, lengthen, not inverse
+        if out is not None:
+            ctx.mark_dirty(out)
+        return _binding().rotary(x, positions, frequencies, layout, lengthen, inverse, out)
+
+    @staticmethod
+    def backward(ctx, grad):
+        positions, frequencies = ctx.saved_tensors
+        layout, lengthen, inverse = ctx.turn
+        if grad.stride(2) != 1:
+            grad = grad.contiguous()
+        return (rotary(grad, positions, frequencies, layout=layout, lengthen=lengthen,
+                       inverse=inverse), None, None, None, None, None, None)
+
+
+class _NoGradient(torch.autograd.Function):
+    """Makes ``t``, computed from ``inputs``, part of their graph."""
+
+    @staticmethod
+    def forward(ctx, t, *inputs):
+        ctx.mark_dirty(t)
+        return t
+
+    @staticmethod
+    def backward(ctx, grad):
+        raise RuntimeError("paged_attention has no gradient: call it under torch.no_grad(), or "
+                           "train with an attention that has one")
 
 
 def rotary_frequencies(rotary_dim, *, base=10000.0, axes=1, scaling=None, factor=1.0,
@@ -100,8 +140,11 @@ def rotary(x, positions, frequencies, *, layout="half", lengthen=1.0, inverse=Fa
 
     layout "half" pairs element i with i + n of an axis's 2n elements,
     "interleaved" 2i with 2i + 1.  ``inverse`` turns the other way, which is
-    the gradient of ``rotary`` with respect to x.  ``out`` may be x itself.
+    the gradient of ``rotary`` with respect to x (autograd uses it).  ``out``
+    may be x itself.
     """
+    if getattr(x, "requires_grad", False) and torch.is_grad_enabled():
+        return _Rotary.apply(x, positions, frequencies, layout, lengthen, inverse, out)
     return _binding().rotary(x, positions, frequencies, layout, lengthen, inverse, out)
 
 
@@ -145,8 +188,12 @@ def paged_attention(q, k_pages, v_pages, table, lengths, starts, *, max_new, max
     kernel and the split, the result holds for any.  Without ``workspace`` the
     current stream's own is used.
     """
-    return _binding().attention(q, k_pages, v_pages, table, lengths, starts, max_new, max_len,
+    both = _binding().attention(q, k_pages, v_pages, table, lengths, starts, max_new, max_len,
                                 causal, scale, out, lse, workspace, status)
+    if ((q.requires_grad or k_pages.requires_grad or v_pages.requires_grad)
+            and torch.is_grad_enabled()):
+        both = tuple(_NoGradient.apply(t, q, k_pages, v_pages) for t in both)
+    return both
 
 
 def paged_weights(q, lse, k_pages, table, lengths, starts, weights, *, max_new, max_len=None,

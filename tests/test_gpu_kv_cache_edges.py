@@ -9,7 +9,7 @@ import torch
 
 import vggt_sparse
 from vggt_sparse import _lib
-from test_gpu_kv_cache import BF, FP, Case, ints
+from test_gpu_kv_cache import BF, FP, Case, ints, turned
 
 pytestmark = pytest.mark.gpu
 
@@ -232,3 +232,62 @@ def test_attention_rows_of_no_sequence(cuda, new, length, dim):
                                        max_new=new, out=torch.full_like(q, 7.0), status=c.status)
     assert bool((o == 0).all()) and bool((l == -math.inf).all())
     assert int(c.status) == _lib.STATUS_BAD_LENGTH
+
+
+# ------------------------------------------------------------------ gradients
+@pytest.mark.parametrize("layout", ["half", "interleaved"])
+@pytest.mark.parametrize("inverse", [False, True])
+@pytest.mark.parametrize("dtype", [torch.float32, BF])
+def test_rotary_in_a_graph(cuda, dtype, inverse, layout):
+    """The gradient of a weighted sum against the formula's, in place too."""
+    g = torch.Generator().manual_seed(2)
+    x, y = (torch.randn(9, 3, 64, generator=g).to(dtype).to(cuda) for _ in range(2))
+    pos = torch.randint(0, 4000, (9, 2), generator=g).to(torch.int32).to(cuda)
+    freq, lengthen = vggt_sparse.rotary_frequencies(48, axes=2, scaling="by_parts", factor=8.0,
+                                                    original_length=512)
+    kw = dict(layout=layout, lengthen=lengthen, inverse=inverse)
+    want = turned(y, pos, freq, lengthen, layout, not inverse)
+    u = {torch.float32: 2.0 ** -24, BF: 2.0 ** -8}[dtype]
+    bound = u * want.abs() + 2.0 ** -20 * 1.5 * lengthen * y.double().abs().amax(-1, keepdim=True)
+    for form in ("out", "in place", "other out", "strided gradient"):
+        leaf = x.clone().requires_grad_()
+        z = leaf * 1
+        if form == "out":
+            r = vggt_sparse.rotary(z, pos, freq, **kw)
+        else:
+            into = z if form == "in place" else torch.empty_like(x)
+            r = vggt_sparse.rotary(z, pos, freq, out=into, **kw)
+            assert r.data_ptr() == into.data_ptr()
+        assert r.requires_grad
+        assert torch.equal(r.detach(), vggt_sparse.rotary(x, pos, freq, **kw))
+        if form == "strided gradient":
+            r.backward(y.transpose(1, 2).contiguous().transpose(1, 2))
+        else:
+            (r * y).sum().backward()
+        assert bool(((leaf.grad.double() - want).abs() <= bound).all()), form
+    with torch.no_grad():
+        assert not vggt_sparse.rotary(leaf, pos, freq, **kw).requires_grad
+
+
+@pytest.mark.parametrize("new", [1, 40])
+def test_attention_says_that_it_has_no_gradient(cuda, new):
+    """Inputs that require gradients give the same numbers, with a graph whose
+    backward pass raises instead of none."""
+    c = Case(cuda, [200], [new], 1, 2, 64, 16)
+    out, lse = c.attend(True)
+    leaf = c.q.clone().requires_grad_()
+    c.q = leaf * 1
+    for kw in ({}, dict(out=torch.empty_like(out), lse=torch.empty_like(lse))):
+        got, got_lse = c.attend(True, **kw)
+        assert torch.equal(got, out) and torch.equal(got_lse, lse)
+        for t in (got, got_lse):
+            assert t.requires_grad
+            with pytest.raises(RuntimeError, match="no gradient"):
+                t.sum().backward()
+        if kw:
+            assert got.data_ptr() == kw["out"].data_ptr()
+    w = torch.zeros(1, 1, c.table.shape[1] * 16, device=cuda)
+    vggt_sparse.paged_weights(c.q, got_lse, c.kp, c.table, c.len, c.starts, w, max_new=new)
+    assert not w.requires_grad and abs(float(w.sum()) - 2 * new) <= 1e-4 * new
+    with torch.no_grad():
+        assert not c.attend(True)[0].requires_grad
