@@ -370,6 +370,8 @@ PyObject* attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
                   !Rows(*given).fit()))
       refuse("out must have q's shape and dtype and 16-byte aligned rows");
     if (given_lse) need("lse", *given_lse, at::kFloat, {total, heads});
+    // its elements are taken as bytes that lie one behind the other
+    if (space && !space->is_contiguous()) refuse("workspace must be contiguous");
     int32_t* word = status_of(status);
     const c10::Device device = one_device(q, &kp, &vp, &table, &lengths, &starts, given, given_lse,
                                           space, status);

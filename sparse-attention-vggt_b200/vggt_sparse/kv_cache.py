@@ -165,8 +165,8 @@ def paged_append(k, v, k_pages, v_pages, table, before, starts, *, positions=Non
 
 
 def paged_attention_workspace_size(total, seqs, kv_heads, group, dim, max_new, max_len):
-    """Bytes of the workspace of ``paged_attention``: a uint8 tensor zeroed
-    before its first use, used by one stream at a time."""
+    """Bytes of the workspace of ``paged_attention``: a contiguous uint8 tensor
+    zeroed before its first use, used by one stream at a time."""
     return int(_lib.load().vggt_paged_attention_workspace_size(total, seqs, kv_heads, group, dim,
                                                                max_new, max_len))
 
