@@ -215,6 +215,13 @@ __device__ __forceinline__ float new_weight(float old, float decay, float sum) {
   return old == INFINITY ? old : fmaf(old, decay, sum);
 }
 
+// The expected most new tokens and greatest length, cut down to what can be, so
+// that the plans' arithmetic holds for any.
+inline void clamp_expected(int64_t total, int64_t& max_new, int64_t& max_len) {
+  if (max_new > total) max_new = total > 0 ? total : 1;
+  if (max_len > 0x7fffffffLL) max_len = 0x7fffffffLL;
+}
+
 // How a launch cuts its work.
 struct PagedPlan {
   int rows;               // query rows per CTA

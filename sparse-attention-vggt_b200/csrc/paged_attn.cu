@@ -31,6 +31,7 @@ extern "C" size_t vggt_paged_attention_workspace_size(int64_t total, int64_t seq
   if (total <= 0 || seqs <= 0 || kv_heads < 1 || group < 1 || max_new < 1 || max_len < 0 ||
       (dim != 64 && dim != 128))
     return 0;
+  clamp_expected(total, max_new, max_len);
   return (size_t)kMaxCounters * 4 +
          plan_of(total, seqs, kv_heads, group, dim, max_new, max_len).partial_bytes;
 }
@@ -61,6 +62,7 @@ extern "C" int vggt_paged_attention(
     return api_fail("q, out, the pools and the workspace must be 16-byte aligned");
   if (q_token_stride % 8 || q_head_stride % 8 || out_token_stride % 8 || out_head_stride % 8)
     return api_fail("strides of q and out must be multiples of 8 elements");
+  clamp_expected(total, max_new, max_len);
   const PagedPlan plan = plan_of(total, seqs, kv_heads, group, dim, max_new, max_len);
   const size_t need = (size_t)kMaxCounters * 4 + plan.partial_bytes;
   if (workspace_bytes < need)

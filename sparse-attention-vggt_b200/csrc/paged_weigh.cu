@@ -309,6 +309,7 @@ extern "C" int vggt_paged_weights(const void* q, int dtype, int64_t total, int64
   a.scale = scale;
   a.decay = decay;
   a.weights = weights;
+  clamp_expected(total, max_new, max_len);
   a.max_new = max_new;
   a.max_len = max_len;
   a.wait_ns = api_wait_ns();

@@ -291,3 +291,27 @@ def test_attention_says_that_it_has_no_gradient(cuda, new):
     assert not w.requires_grad and abs(float(w.sum()) - 2 * new) <= 1e-4 * new
     with torch.no_grad():
         assert not c.attend(True)[0].requires_grad
+
+
+# ------------------------------------------------------------------ expectations
+HINTS = [(1, 1), (1, 2 ** 62), (2 ** 62, 1), (2 ** 62, 2 ** 62), (2 ** 63 - 1, 2 ** 63 - 1), (40, 300)]
+
+
+@pytest.mark.parametrize("max_new,max_len", HINTS)
+@pytest.mark.parametrize("new", [1, 40])
+def test_attention_and_weights_hold_for_any_expectation(cuda, new, max_new, max_len):
+    """Many sequences and heads (132 of them), and hints from far too low to
+    far too high: the same weights but for the order of sums."""
+    c = Case(cuda, [33 * b + 60 for b in range(11)], [new] * 11, 12, 1, 64, 16)
+    out, lse = c.attend(True, max_new=max_new, max_len=max_len)
+    c.check(out, lse, True)
+    w = torch.zeros(11, 12, c.table.shape[1] * 16, device=cuda)
+    vggt_sparse.paged_weights(c.q, lse, c.kp, c.table, c.len, c.starts, w, max_new=max_new,
+                              max_len=max_len, status=c.status)
+    assert int(c.status) == 0
+    for b, n in enumerate(c.lengths):
+        s, _ = c.scores(b, True)
+        p = torch.exp(s - lse[c.rows(b)].T[..., None].double())
+        bound = (2e-5 + new * 2.0 ** -24) * p.sum(1) + 2.0 ** -23 * p.sum(1)
+        assert bool(((w[b, :, :n].double() - p.sum(1)).abs() <= bound).all())
+        assert bool((w[b, :, n:] == 0).all())

@@ -27,3 +27,13 @@ def test_workspace_must_be_contiguous(workspace):
     with pytest.raises(ValueError, match="workspace must be contiguous"):
         vggt_sparse.paged_attention(q, pool, pool, ints(1, 3), ints(1), ints(2), max_new=1,
                                     workspace=workspace)
+
+
+def test_workspace_size_of_any_expectation():
+    """What is expected beyond what can be counts as the most that can be."""
+    size = vggt_sparse.paged_attention_workspace_size
+    for total, seqs, heads, group, dim in ((40, 2, 8, 4, 64), (1, 1, 16, 1, 128), (1374, 1, 16, 1, 64)):
+        most = size(total, seqs, heads, group, dim, total, 2 ** 31 - 1)
+        for max_new in (total, 2 ** 40, 2 ** 61, 2 ** 62, 2 ** 63 - 1):
+            for max_len in (2 ** 31, 2 ** 50, 2 ** 62, 2 ** 63 - 1):
+                assert size(total, seqs, heads, group, dim, max_new, max_len) == most
