@@ -315,3 +315,26 @@ def test_attention_and_weights_hold_for_any_expectation(cuda, new, max_new, max_
         bound = (2e-5 + new * 2.0 ** -24) * p.sum(1) + 2.0 ** -23 * p.sum(1)
         assert bool(((w[b, :, :n].double() - p.sum(1)).abs() <= bound).all())
         assert bool((w[b, :, n:] == 0).all())
+
+
+@pytest.mark.parametrize("max_len", [0, 40, 500, 3000, 2 ** 62])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_evict_holds_for_any_expectation(cuda, dim, max_len):
+    """max_len below the lengths (the shares do not fit what was set aside for
+    them, and are read again) and above: the same choice, the same bits."""
+    c = Case(cuda, [2900, 700], [0, 0], 2, 1, dim, 16)
+    g = torch.Generator().manual_seed(3)
+    w = (torch.rand(2, 2, c.table.shape[1] * 16, generator=g) * 50).floor().to(cuda)
+    ids = torch.arange(w.shape[2], dtype=torch.int32, device=cuda).expand(2, 2, -1).contiguous()
+    recent = ints([2800, 650], cuda)
+    kp, vp = c.kp.clone(), c.vp.clone()
+    want = vggt_sparse.paged_evict(w, ids, kp, vp, c.table, c.len, 600, recent_from=recent)
+    got = vggt_sparse.paged_evict(w, ids, c.kp, c.vp, c.table, c.len, 600, max_len=max_len,
+                                  recent_from=recent, status=c.status)
+    assert all(torch.equal(a, b) for a, b in zip(got, want)) and int(c.status) == 0
+    assert torch.equal(kp.nan_to_num(7.0), c.kp.nan_to_num(7.0))
+    assert torch.equal(vp.nan_to_num(7.0), c.vp.nan_to_num(7.0))
+    rank = torch.where(ids[0] >= 2800, math.inf, w[0])[:, :2900]
+    keep = torch.sort(rank, dim=-1, descending=True, stable=True).indices[:, :600]
+    for h in range(2):
+        assert set(got[1][0, h, :600].tolist()) == set(keep[h].tolist())
