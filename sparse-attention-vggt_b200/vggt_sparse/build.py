@@ -58,13 +58,20 @@ def _compile(nvcc, src, obj, extra):
 
 
 def _build_binding(force):
-    """The Python module of csrc/cache_binding.cpp, linked against the library next to it."""
-    src = os.path.join(CSRC, "cache_binding.cpp")
-    if not force and not _stale(BINDING_PATH, [src, *_headers()]):
-        return
+    """The Python module of csrc/cache_binding.cpp, linked against the library next to it.
+
+    It uses torch's C++ interface, which holds for one version: a stamp beside
+    the objects says which torch and which Python it was built for."""
     import sysconfig
 
     import torch
+    src = os.path.join(CSRC, "cache_binding.cpp")
+    stamp = os.path.join(BUILD_DIR, "_cache_binding.stamp")
+    made_for = "torch %s, %s\n" % (torch.__version__, sys.implementation.cache_tag)
+    if not force and not _stale(BINDING_PATH, [src, *_headers()]) and os.path.exists(stamp):
+        with open(stamp) as f:
+            if f.read() == made_for:
+                return
     root = os.path.dirname(torch.__file__)
     cuda = os.path.dirname(os.path.dirname(os.path.realpath(_nvcc())))
     include = [INCLUDE, os.path.join(root, "include"),
@@ -78,6 +85,8 @@ def _build_binding(force):
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:
         raise RuntimeError("building the Python module failed:\n%s\n%s" % (res.stdout, res.stderr))
+    with open(stamp, "w") as f:
+        f.write(made_for)
 
 
 def build(force=False, verbose=False, ptxas_info=False):

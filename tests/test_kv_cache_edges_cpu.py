@@ -37,3 +37,25 @@ def test_workspace_size_of_any_expectation():
         for max_new in (total, 2 ** 40, 2 ** 61, 2 ** 62, 2 ** 63 - 1):
             for max_len in (2 ** 31, 2 ** 50, 2 ** 62, 2 ** 63 - 1):
                 assert size(total, seqs, heads, group, dim, max_new, max_len) == most
+
+
+def test_binding_is_built_again_for_another_torch(monkeypatch, tmp_path):
+    """The compiled module holds for the torch and the Python it was built for."""
+    import subprocess
+    from vggt_sparse import build
+    made = []
+
+    def run(cmd, **kw):
+        made.append(cmd)
+        (tmp_path / "binding.so").write_text("")
+        return subprocess.CompletedProcess(cmd, 0, "", "")
+    monkeypatch.setattr(build, "BINDING_PATH", str(tmp_path / "binding.so"))
+    monkeypatch.setattr(build, "BUILD_DIR", str(tmp_path))
+    monkeypatch.setattr(build.subprocess, "run", run)
+    for version, builds in ((torch.__version__, 1), (torch.__version__, 1), ("0.1", 2), ("0.1", 2),
+                            (torch.__version__, 3)):
+        monkeypatch.setattr(torch, "__version__", version)
+        build._build_binding(False)
+        assert len(made) == builds
+    build._build_binding(True)
+    assert len(made) == 4
