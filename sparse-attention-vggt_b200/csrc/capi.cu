@@ -99,8 +99,6 @@ int api_cuda(cudaError_t e) {
   return cuda_rc(e);
 }
 
-int api_device_sms() { return current_device_sms(); }
-
 uint64_t api_wait_ns() {
   const uint64_t ns = g_wait_ns.load();
   return ns > 0 ? ns : 1000000000ull;

@@ -51,7 +51,9 @@ __device__ __forceinline__ float max_nan(float a, float b) {
 // the least largest relative error, 2.7e-6 in fp32), scale = 2^n.  Where n would
 // be below -126 the exponent's bits come to zero, and scale with them: -inf
 // gives exactly 0, as a masked score must (2^-126 is a number of bf16, and times
-// a value of 1e38 one that shows).  A NaN stays one (in q).
+// a value of 1e38 one that shows).  A NaN stays one (in q).  (The block-sparse
+// attention's cubic, attn_tc05.cu, goes under the rounding of its P; here the
+// exponentials are summed in fp32 for log-sum-exps and weights.)
 struct Exp2Poly {
   float_pair magic, c4, c3, c2, c1, c0;
   __device__ __forceinline__ Exp2Poly()

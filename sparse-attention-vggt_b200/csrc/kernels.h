@@ -10,7 +10,6 @@ namespace vggt {
 // format no error (clears it, returns 0).  A CUDA error as a return code.
 int api_fail(const char* fmt, ...);
 int api_cuda(cudaError_t e);
-int api_device_sms();
 // limit of every bounded wait, vggt_sparse_set_wait_limit_ns
 uint64_t api_wait_ns();
 // vggt_sparse_set_wait_selftest

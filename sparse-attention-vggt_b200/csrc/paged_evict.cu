@@ -23,7 +23,9 @@
 // prompts cut from 16,383 to 4,096 tokens (379 MB moved in rows of 256 bytes)
 // take 101 us, 3.8 TB/s: 512 threads a CTA, so that the passes of some CTAs run
 // beside the moves of others, and the moves' addresses resolved a round ahead of
-// the rows (with every row's look-ups before its copy: 162 us).
+// the rows (with every row's look-ups before its copy: 162 us).  Four CTAs to an
+// SM leave a thread 32 registers, and spill 44 bytes of them (60 with one CTA a
+// row).
 #include <cooperative_groups.h>
 
 #include "kernels.h"

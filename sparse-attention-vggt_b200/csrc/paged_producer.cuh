@@ -1,5 +1,5 @@
-// The TMA producer of the kernels that stream 64-key tiles of K (and V) through
-// one ring.
+// The TMA producer of the weights of few rows, which streams 64-key tiles of K
+// through a ring.
 #pragma once
 
 #include <type_traits>
@@ -10,9 +10,8 @@
 namespace vggt {
 
 // Run by one full warp.  Tile t of the run that starts at slot `first_slot`
-// (a multiple of 64) goes to stage t % kStages: the matrices one behind the
-// other, each as kHalves blocks of 64 rows x 128 bytes (swizzled), one box per
-// page or per 64 slots of a larger page.  Slots at or past `keys` (counted from
+// (a multiple of 64) goes to stage t % kStages as kHalves blocks of 64 rows x
+// 128 bytes (swizzled), one box per page or per 64 slots of a larger page.  Slots at or past `keys` (counted from
 // first_slot) are not loaded where a whole box of them can be left out; page
 // numbers that may not be used read as zeros.  full / empty: the first of
 // kStages barriers each.  Returns when no copy is in flight.
@@ -20,14 +19,13 @@ namespace vggt {
 // Page numbers are read 32 boxes ahead and the rest is 32-bit arithmetic on
 // constants of the box count: with 64-bit counters and divisions by the box
 // size a tile took this warp 1,400 clocks, longer than the copies.
-template <int kHalves, int kMatrices, int kStages>
+template <int kHalves, int kStages>
 __device__ __forceinline__ void produce_tiles(const PageTable& table, const Pool& pool,
                                               int64_t seq, int head, int64_t first_slot, int keys,
-                                              int tiles, const CUtensorMap* map0,
-                                              const CUtensorMap* map1, uint32_t ring,
+                                              int tiles, const CUtensorMap* map, uint32_t ring,
                                               uint32_t full, uint32_t empty,
                                               volatile int* abort_flag, uint64_t wait_ns) {
-  constexpr uint32_t kBlock = 64 * 128, kMatrix = kHalves * kBlock, kStage = kMatrices * kMatrix;
+  constexpr uint32_t kBlock = 64 * 128, kStage = kHalves * kBlock;
   const int lane = threadIdx.x & 31;
   const int32_t* row_of_table = table.table + seq * table.width;
   const int in_page = (int)first_slot & (pool.page - 1), page_mask = pool.page - 1;
@@ -59,16 +57,14 @@ __device__ __forceinline__ void produce_tiles(const PageTable& table, const Pool
       if (tc::elect_one()) {
         const uint32_t bar = full + 8u * stage, dst = ring + stage * kStage;
         const int row = (in_page + key0) & page_mask;
-        tc::mbar_expect_tx(bar, (uint32_t)(live * kBox) * kHalves * kMatrices * 128u);
+        tc::mbar_expect_tx(bar, (uint32_t)(live * kBox) * kHalves * 128u);
 #pragma unroll
-        for (int m = 0; m < kMatrices; ++m)
+        for (int b = 0; b < kBoxes; ++b)
+          if (b < live)
 #pragma unroll
-          for (int b = 0; b < kBoxes; ++b)
-            if (b < live)
-#pragma unroll
-              for (int h = 0; h < kHalves; ++h)
-                tc::tma_load_4d(dst + m * kMatrix + h * kBlock + b * kBox * 128, m ? map1 : map0,
-                                bar, h * 64, (row + b * kBox) & page_mask, head, pages[b]);
+            for (int h = 0; h < kHalves; ++h)
+              tc::tma_load_4d(dst + h * kBlock + b * kBox * 128, map, bar, h * 64,
+                              (row + b * kBox) & page_mask, head, pages[b]);
       }
       __syncwarp();
       ++issued;

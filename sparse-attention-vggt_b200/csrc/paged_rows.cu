@@ -5,7 +5,9 @@
 // by reading K and V once.  So a CTA takes one tile of 16 rows and one
 // run of key tiles, and what matters is that loads never pause:
 //  * warp 4 streams 64-key K and V tiles by TMA (boxes of one page, 128-byte
-//    swizzle) into a ring; page numbers are read 32 boxes ahead.
+//    swizzle) into a ring; page numbers are read 32 boxes ahead.  (Its 64-bit
+//    counters cost what paged_producer.cuh says; long caches are at the memory's
+//    rate all the same.)
 //  * warps 0-3 share a tile's keys, 16 each; each keeps its own running
 //    maximum, sum and output rows in registers (mma.sync m16n8k16, fp32), so no
 //    warp waits for another before the end.  tcgen05 would spend M = 128 rows

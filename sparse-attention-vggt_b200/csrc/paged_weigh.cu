@@ -99,9 +99,9 @@ __global__ void __launch_bounds__(kThreads, kCtas<D>)
   if (warp == 4) {
     // ================= TMA producer =================
     if (!a.wait_selftest || tc::warp_wait(smem_u32(&bars[2 * kStages]), 0, abort_flag, a.wait_ns))
-      produce_tiles<kHalves, 1, kStages>(a.t, a.pool, seq, head, tile0 * kTile,
-                                         (int)(len - tile0 * kTile), (int)tiles, &tm_k, &tm_k,
-                                         ring_addr, full(0), empty(0), abort_flag, a.wait_ns);
+      produce_tiles<kHalves, kStages>(a.t, a.pool, seq, head, tile0 * kTile,
+                                      (int)(len - tile0 * kTile), (int)tiles, &tm_k, ring_addr,
+                                      full(0), empty(0), abort_flag, a.wait_ns);
   } else {
     const int krow = ((lane >> 4) & 1) * 8 + (lane & 7), kchunk = (lane >> 3) & 1;
     const int qrow = ((lane >> 3) & 1) * 8 + (lane & 7), qchunk = (lane >> 4) & 1;

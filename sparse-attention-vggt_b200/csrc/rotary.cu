@@ -233,7 +233,8 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(RotaryArgs p) {
 // Few heads: a thread takes kBatch tokens of one head, so that as many loads
 // are in flight as with many heads, and the steps are formed once for them.
 // (One head of 64, 703,488 tokens: 53 us, against 99; what is left are the
-// sines, 50 instructions each.)
+// sines, 50 instructions each.  With 8 pairs to a thread three CTAs to an SM
+// spill 28 bytes and take 53 us, two without a spill 61.)
 template <typename T, int N>
 __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 ? 2 : 3)
     rotary_few_heads_kernel(RotaryArgs p) {
@@ -293,8 +294,8 @@ __device__ __forceinline__ int64_t append_slot(const AppendArgs& p, int64_t row,
   return -1;
 }
 
-// (Three CTAs to an SM at least: 4 prompts of up to 2,048 tokens 17.1 us, at the
-// 106 registers of two CTAs 20.1.)
+// (Three CTAs to an SM at least, which spills 4 bytes in one form: 4 prompts of
+// up to 2,048 tokens 17.1 us, at the 106 registers of two CTAs 20.1.)
 template <typename T, int N>
 __global__ void __launch_bounds__(kThreads, 3) append_kernel(AppendArgs p) {
   if (blockIdx.x >= p.main_blocks) {
