@@ -760,17 +760,23 @@ PagedPlan paged_tc05_plan(int64_t total, int64_t seqs, int kv_heads, int group, 
   plan.tiles = most_tiles(total, seqs, group, kRows);
   const int64_t items = plan.tiles * kv_heads, key_tiles = (max_len + kTile - 1) / kTile;
   // Runs per row tile: the number that ends the last wave of 2 CTAs per SM
-  // soonest.  In units of a key tile (0.7 us): a CTA's start and end cost ten,
-  // joining the runs eight.  (Measured when the last CTA of a row tile joined
-  // its runs: 1 frame over 31 cached ones, 176 items, 1 run 536 us, 3 runs 387,
-  // 5 runs 375, 10 runs 422; 4 prompts, 2,024 items, 1 run 1,292 us, 2 runs
-  // 1,546.)
+  // soonest.  In units of a key tile (0.7 us, 1.0 at dim 128): a CTA's start and
+  // end cost ten, the join's launch two, and a run's partial result, written and
+  // read at 4 TB/s, 1/40 (1/30).  Of 15 shapes the rule takes the fastest number
+  // for 13 and loses 4 % at two.  In us, taken ones in brackets: a frame over 31
+  // cached ones, 176 items, 1 run 535, 3 runs 377, 5 runs (343), 10 runs 351; the
+  // same of dim 128, 88 items, 1 run 517, 3 runs (235), 10 runs 248; 100 tokens
+  // over 43,000 keys, 16 items, 8 runs 61, 18 runs (49), 32 runs 57; 4 prompts,
+  // 1,840 items, 1 run (1,273), 2 runs 1,482; 8 chunks of 500 tokens, 976 items,
+  // 1 run (451), 2 runs 528.
   plan.splits = 1;
-  int64_t best = -1;
+  double best = -1;
   const int64_t slots = 2 * 148;
+  const double partial = dim == 64 ? 1.0 / 40 : 1.0 / 30;
   for (int64_t s = 1; s <= kMaxRuns && s <= (key_tiles > 0 ? key_tiles : 1); ++s) {
     const int64_t waves = (items * s + slots - 1) / slots;
-    const int64_t cost = waves * ((key_tiles + s - 1) / s + 10) + (s > 1 ? 8 : 0);
+    const double cost = (double)(waves * ((key_tiles + s - 1) / s + 10)) +
+                        (s > 1 ? 2 + (double)(items * s) * partial : 0);
     if (best < 0 || cost < best) {
       best = cost;
       plan.splits = s;

@@ -59,3 +59,13 @@ def test_binding_is_built_again_for_another_torch(monkeypatch, tmp_path):
         assert len(made) == builds
     build._build_binding(True)
     assert len(made) == 4
+
+
+def test_runs_are_not_split_where_partial_results_cost_more():
+    """The workspace shows the split: many row tiles stay whole (16 KB of
+    counters alone), few ones over a long cache are cut."""
+    size = vggt_sparse.paged_attention_workspace_size
+    assert size(7300, 4, 8, 4, 128, 1999, 14288) == 16384
+    assert size(3900, 8, 8, 4, 128, 500, 8500) == 16384
+    frame = 11 * 16 * 128 * (64 + 2) * 4  # a run of each item
+    assert size(1374, 1, 16, 1, 64, 1374, 43968) == 16384 + 5 * frame
