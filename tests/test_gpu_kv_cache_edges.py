@@ -86,6 +86,32 @@ def test_attention_large_values_of_later_tokens(cuda, new, dim):
     assert bool((out[first:new].abs() > 1e30).all())
 
 
+@pytest.mark.parametrize("bad", [math.inf, -math.inf, math.nan])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("new,length", [(5, 450), (200, 450), (200, 3000)])
+def test_attention_values_of_later_tokens_that_are_not_finite(cuda, new, length, dim, bad):
+    """bf16: one such value in the chunk, in one run of the keys or in the last of
+    several.  Rows that see it get it, the others are as if it were zero."""
+    c = Case(cuda, [length, 70], [new, new], 1, 2, dim, 16)
+    first = new // 2
+    j = length - new + first
+    at = int(c.table[0, j // 16]), 0, j % 16, 9
+    c.vp[at] = 0
+    want, want_lse = c.attend(True)
+    c.vp[at] = bad
+    out, lse = c.attend(True)
+    assert torch.equal(out[new:], want[new:]) and torch.equal(lse[new:], want_lse[new:])
+    seen = out[first:new, :, 9]
+    assert bool(torch.isnan(seen).all()) if bad != bad else bool((seen == bad).all())
+    others = torch.ones_like(out[:new], dtype=torch.bool)
+    others[first:, :, 9] = False
+    # both sides round the probabilities (or not) and the output: two bounds apart
+    size = 4 * c.v[0].abs().max().double()
+    diff = (out[:new].double() - want[:new].double()).abs()[others]
+    assert bool((diff <= 2 * (2 * 2.0 ** -8 + 2.0 ** -13) * size).all())
+    assert bool(((lse[:new] - want_lse[:new]).abs() <= 2.0 ** -14).all())
+
+
 # ------------------------------------------------------------------ weights
 @pytest.mark.parametrize("decay", [0.0, 0.5, -1.0])
 @pytest.mark.parametrize("max_new", [1, 500])
