@@ -16,7 +16,8 @@
 // warp some 150 clocks even where it is satisfied, and the issue of four MMAs
 // 200 to 300, so that one warp's four steps per tile took longer than the
 // tile's softmax (510 us for a frame over 31 cached ones against 375, both
-// before the steps below; 335 now).
+// before the steps below; 335 now).  These and the figures below are of launches
+// replayed from a graph; an ordinary call of the frame takes 374 us.
 //
 // The row's reference maximum moves only when a tile's maximum exceeds it by
 // more than 2^8 in the exp2 domain; O is rescaled then.  Sums are fp32, of the
@@ -78,8 +79,8 @@ constexpr int kMaxRuns = 64;  // per row tile
 // fp16 would drop probabilities of 2^-25 and less from the product with V,
 // which their sum still counts: 65,000 keys under one strong one lost 0.2 % of
 // the output.  Lag and shift share the 15 steps up to 2^15.  A smaller lag moves
-// the reference more often (4 prompts of dim 128: 1,430 to 1,480 us; 1,560 at 4
-// and 11, 1,640 at 2 and 13).  bf16 has the exponents of fp32.
+// the reference more often (4 prompts of dim 128 in two runs: 1,430 to 1,480 us;
+// 1,560 at 4 and 11, 1,640 at 2 and 13).  bf16 has the exponents of fp32.
 template <typename T>
 struct PRange {
   static constexpr bool kHalf = std::is_same<T, __half>::value;

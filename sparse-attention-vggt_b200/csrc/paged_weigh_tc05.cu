@@ -20,8 +20,12 @@
 // polynomial (error 2.7e-6) on the FMA pipe.  One frame of 1,374 tokens over
 // 43,968 keys in 16 heads: 297 us (303 at three pairs of eight, 331 at four).
 // Two exponential warps share an SM's quarter; 32 columns take the two some 520
-// clocks, where the unit needs 384: they wait for one another's results.  Eight
-// exponential warps instead of four were slower (356 us against 341 then).
+// clocks, where the unit needs 384: they wait for one another's results.  That
+// is a third of the time: without the exponentials the frame takes 202 us, and
+// without the arithmetic on S 181, which are the tile's own chain of loads from
+// TMEM and waits (a Q tile is loaded again for every 128 keys, 1.3 GB of tiles in
+// all, but L2 is at 16 % of its rate).  Eight exponential warps instead of four
+// were slower (356 us against 341 then).
 #include <cuda.h>
 
 #include <type_traits>
