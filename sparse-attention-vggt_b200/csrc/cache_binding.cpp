@@ -383,7 +383,7 @@ PyObject* attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (p.seqs == 0) {  // the rows belong to no sequence; no kernel will run
       out.zero_();
       lse.fill_(-INFINITY);
-      if (status && total > 0) status->flatten().narrow(0, 0, 1).bitwise_or_(VGGT_STATUS_BAD_LENGTH);
+      if (status && total > 0) status->as_strided({1}, {1}).bitwise_or_(VGGT_STATUS_BAD_LENGTH);
     }
     const size_t bytes = vggt_paged_attention_workspace_size(
         total, p.seqs, (int)p.heads, (int)group, (int)p.dim, max_new, max_len);

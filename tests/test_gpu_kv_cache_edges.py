@@ -254,10 +254,11 @@ def test_attention_rows_of_no_sequence(cuda, new, length, dim):
     assert bool((o == 0).all()) and bool((l == -math.inf).all())
     assert int(c.status) == _lib.STATUS_BAD_LENGTH
     c.status.zero_()
+    word = torch.zeros(4, dtype=torch.int32, device=cuda)[::2]
     o, l = vggt_sparse.paged_attention(q, c.kp, c.vp, c.table[:0], c.len[:0], c.starts[:1],
-                                       max_new=new, out=torch.full_like(q, 7.0), status=c.status)
+                                       max_new=new, out=torch.full_like(q, 7.0), status=word)
     assert bool((o == 0).all()) and bool((l == -math.inf).all())
-    assert int(c.status) == _lib.STATUS_BAD_LENGTH
+    assert word.tolist() == [_lib.STATUS_BAD_LENGTH, 0]
 
 
 # ------------------------------------------------------------------ gradients
