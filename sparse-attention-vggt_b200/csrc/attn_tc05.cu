@@ -926,8 +926,9 @@ bool encode_tmap_sw128(CUtensorMap* map, const void* ptr, int dtype, int rank,
     b[i] = box[i];
     estr[i] = 1;
   }
-  const CUtensorMapDataType dt =
-      dtype == VGGT_DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  const CUtensorMapDataType dt = dtype == VGGT_DTYPE_BF16   ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                 : dtype == VGGT_DTYPE_FP16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                                            : CU_TENSOR_MAP_DATA_TYPE_FLOAT32;
   return fn(map, dt, (cuuint32_t)rank, const_cast<void*>(ptr), d, s, b, estr,
             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;

@@ -14,6 +14,8 @@ int api_cuda(cudaError_t e);
 uint64_t api_wait_ns();
 // vggt_sparse_set_wait_selftest
 int api_wait_selftest();
+// residual_norm.cu: multiprocessors of the current device
+cudaError_t device_sms(int* sms);
 
 inline bool units_zero(int64_t a, int64_t b) { return a == 0 || b == 0; }
 

@@ -1,0 +1,911 @@
+// Matrix product on the tensor cores with bias, activation, gate and residual in its epilogue.
+//
+// A tile of C is 128 CTA x 128 CTA elements, CTA = 1 or 2 CTAs (a pair works on one tile: each
+// holds half of A's rows and half of B's, the MMA of the pair reads both halves of B).  Warp 0
+// streams the operands by TMA through a ring of 64-element reduction blocks, warp 1 issues the
+// MMAs into one of two accumulators in TMEM, and warps 4-11, two warpgroups that take alternate
+// 64-column pieces, run the epilogue of the tile before: TMEM -> registers -> bias, activation,
+// gate, residual -> a swizzled 16 KB buffer -> TMA store.  The residual comes by TMA into the same
+// buffer before.  What TMA cannot address (odd widths, other strides) is copied between buffer
+// and memory by the warps that own the rows.
+//
+// Bound by the tensor cores and by the operands' way from L2 (a pair's 256 x 256 tile needs
+// 64 B a cycle and SM at the full rate, a single CTA's 128 x 128 twice that).
+//
+// Every wait is bounded; on expiry the CTA raises its abort flag, VGGT_STATUS_TIMEOUT is set and
+// all roles leave.
+#include "linear.cuh"
+
+#include <algorithm>
+#include <climits>
+#include <type_traits>
+
+#include "activation.cuh"
+#include "tc05.cuh"
+
+namespace vggt {
+namespace lin {
+
+constexpr int BM = 128, BK = 64;
+constexpr int STAGES = 5;
+constexpr int THREADS = 384;
+constexpr uint32_t HALF_BYTES = BM * BK * 2;         // one operand's block: 16 KB
+constexpr uint32_t STAGE_BYTES = 2 * HALF_BYTES;
+constexpr uint32_t BUF_BYTES = BM * 128;             // epilogue buffer: 128 rows of 128 bytes
+constexpr uint32_t OFF_BUF = STAGES * STAGE_BYTES;   // [2 groups][2]
+constexpr uint32_t OFF_VEC = OFF_BUF + 4 * BUF_BYTES;  // float[2 groups][bias 64, gate 64]
+constexpr uint32_t OFF_BAR = OFF_VEC + 2 * 128 * 4;
+constexpr int B_FULL = 0, B_EMPTY = B_FULL + STAGES, B_ACCFULL = B_EMPTY + STAGES,
+              B_ACCEMPTY = B_ACCFULL + 2, B_RES = B_ACCEMPTY + 2 /* [2 groups][2] */,
+              B_DRAIN = B_RES + 4, NBAR = B_DRAIN + 1;
+constexpr uint32_t OFF_MISC = OFF_BAR + NBAR * 8;  // tmem base, abort flag, votes[2 groups][2][2][4]
+constexpr uint32_t SMEM_BYTES = OFF_MISC + 8 + 32 * 4 + 1024;  // and the way to a 1024-byte border
+static_assert(SMEM_BYTES <= 232448, "shared memory");
+
+struct Params {
+  int64_t m, n;
+  int64_t tiles, tiles_n;
+  int blocks;   // reduction blocks of a tile
+  int workers;
+  int split;
+  int a_heads64, b_heads64, y_heads64;  // 64-element pieces of a row in one head
+  const void* bias;
+  const void* gate;
+  int act;
+  int y_fp32, y_tma, res_tma, z_tma;
+  const void* residual;
+  int64_t residual_stride;
+  void* y;
+  int64_t y_stride, y_head_stride;
+  void* z;
+  int64_t z_stride;
+  float* slots;
+  int32_t* status;
+  uint64_t wait_ns;
+  int wait_selftest;
+};
+
+// A worker's next piece of work: reduction blocks [k0, k1) of a tile.
+struct Walk {
+  int64_t at, end, step;
+  int blocks;
+  bool split;
+  int64_t tile;
+  int k0, k1;
+  __device__ __forceinline__ Walk(const Params& p, int worker) : blocks(p.blocks), split(p.split) {
+    if (split) {
+      const int64_t units = p.tiles * p.blocks;
+      at = worker * units / p.workers;
+      end = (worker + 1) * units / p.workers;
+    } else {
+      at = worker;
+      end = p.tiles;
+      step = p.workers;
+    }
+  }
+  __device__ __forceinline__ bool next() {
+    if (at >= end) return false;
+    if (split) {
+      tile = at / blocks;
+      k0 = (int)(at - tile * blocks);
+      k1 = (int)min((int64_t)blocks, k0 + (end - at));
+      at += k1 - k0;
+    } else {
+      tile = at;
+      k0 = 0;
+      k1 = blocks;
+      at += step;
+    }
+    return true;
+  }
+};
+
+// ---- what pairs of CTAs need beside tc05.cuh -------------------------------------------------
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::
+                   : "memory");
+}
+__device__ __forceinline__ uint32_t map_rank(uint32_t addr, uint32_t rank) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ void arrive_cluster(uint32_t bar) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar)
+               : "memory");
+}
+
+template <int CTA>
+struct Pair;
+template <>
+struct Pair<1> {
+  static __device__ __forceinline__ void alloc(uint32_t dst) { tc::tmem_alloc(dst, 256); }
+  static __device__ __forceinline__ void relinquish() { tc::tmem_relinquish(); }
+  static __device__ __forceinline__ void dealloc(uint32_t t) { tc::tmem_dealloc(t, 256); }
+  static __device__ __forceinline__ void load(uint32_t dst, const CUtensorMap* map, uint32_t bar,
+                                              int c0, int c1, int c2) {
+    tc::tma_load_3d(dst, map, bar, c0, c1, c2);
+  }
+  static __device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
+                                             uint32_t acc) {
+    tc::mma_ss(d, a, b, idesc, acc);
+  }
+  static __device__ __forceinline__ void commit(uint32_t bar) { tc::mma_commit(bar); }
+};
+template <>
+struct Pair<2> {
+  static __device__ __forceinline__ void alloc(uint32_t dst) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(dst)
+                 : "memory");
+  }
+  static __device__ __forceinline__ void relinquish() {
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
+  static __device__ __forceinline__ void dealloc(uint32_t t) {
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(t) : "memory");
+  }
+  // into this CTA's memory, completion on a barrier of either CTA of the pair
+  static __device__ __forceinline__ void load(uint32_t dst, const CUtensorMap* map, uint32_t bar,
+                                              int c0, int c1, int c2) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(c0), "r"(c1), "r"(c2)
+        : "memory");
+  }
+  static __device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
+                                             uint32_t acc) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(acc)
+        : "memory");
+  }
+  // arrives on the barrier at this address in both CTAs
+  static __device__ __forceinline__ void commit(uint32_t bar) {
+    asm volatile(
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64"
+        " [%0], %1;" ::"r"(bar),
+        "h"((uint16_t)3)
+        : "memory");
+  }
+};
+
+__device__ __forceinline__ void store_3d(const CUtensorMap* map, uint32_t src, int c0, int c1,
+                                         int c2) {
+  asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%2, %3, %4}], [%1];" ::
+                   "l"(reinterpret_cast<uint64_t>(map)),
+               "r"(src), "r"(c0), "r"(c1), "r"(c2)
+               : "memory");
+}
+__device__ __forceinline__ void store_bulk(void* dst, uint32_t src, uint32_t bytes) {
+  asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(dst), "r"(src),
+               "r"(bytes)
+               : "memory");
+}
+__device__ __forceinline__ void store_commit() {
+  asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+}
+// all but the newest N stores have read their buffers
+template <int N>
+__device__ __forceinline__ void store_wait_read() {
+  asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void lds128(uint32_t a, uint32_t* r) {
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(a));
+}
+__device__ __forceinline__ void sts128(uint32_t a, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
+  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(x), "r"(y), "r"(z), "r"(w)
+               : "memory");
+}
+
+template <typename E>
+__device__ __forceinline__ float to_float(E v) {
+  return (float)v;
+}
+
+// Address of 16-byte piece j of row r in an epilogue buffer (the 128-byte swizzle of TMA).
+__device__ __forceinline__ uint32_t piece(uint32_t buf, int r, int j) {
+  return buf + (uint32_t)(r * 128 + ((j ^ (r & 7)) << 4));
+}
+
+// Copies this warp's 32 rows between an epilogue buffer and memory, element by element: 128 bytes
+// of a row, `left` elements of which exist, in the first `rows` rows.
+template <typename E>
+__device__ __forceinline__ void copy_rows(uint32_t buf, int row0, E* g, int64_t stride, int64_t rows,
+                                          int64_t left, bool in) {
+  constexpr int kPer = 128 / (int)sizeof(E) / 32, kPiece = 16 / (int)sizeof(E);
+  const int lane = threadIdx.x & 31;
+  for (int r = 0; r < 32 && r < rows; ++r) {
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      const int c = lane * kPer + i;
+      if (c >= left) continue;
+      const uint32_t a = piece(buf, row0 + r, c / kPiece) + (uint32_t)(c % kPiece) * sizeof(E);
+      E* p = g + (int64_t)r * stride + c;
+      if (sizeof(E) == 2) {
+        uint16_t v;
+        if (in) {
+          v = *reinterpret_cast<const uint16_t*>(p);
+          asm volatile("st.shared.u16 [%0], %1;" ::"r"(a), "h"(v) : "memory");
+        } else {
+          asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(a) : "memory");
+          *reinterpret_cast<uint16_t*>(p) = v;
+        }
+      } else {
+        uint32_t v;
+        if (in) {
+          v = *reinterpret_cast<const uint32_t*>(p);
+          asm volatile("st.shared.u32 [%0], %1;" ::"r"(a), "r"(v) : "memory");
+        } else {
+          asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
+          *reinterpret_cast<uint32_t*>(p) = v;
+        }
+      }
+    }
+  }
+}
+
+// What one use of an epilogue buffer holds.
+enum { kUseZ, kUseY, kUseSlot };
+
+template <typename T, int CTA, bool AMN, bool BMN, bool SPLIT>
+__global__ void __launch_bounds__(THREADS, 1)
+    product_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b,
+                   const __grid_constant__ CUtensorMap tm_y,
+                   const __grid_constant__ CUtensorMap tm_res,
+                   const __grid_constant__ CUtensorMap tm_z, const Params p) {
+  constexpr int BN = 128 * CTA;  // columns of a tile; 128 of B's rows lie in each CTA
+  extern __shared__ unsigned char smem_raw[];
+  const uint32_t raw = smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
+  unsigned char* sbase = smem_raw + (base - raw);
+  auto bar = [&](int i) { return base + OFF_BAR + 8u * (uint32_t)i; };
+  uint32_t* misc = reinterpret_cast<uint32_t*>(sbase + OFF_MISC);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(misc + 1);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int rank = CTA == 2 ? (int)cluster_rank() : 0;
+  const int worker = (int)blockIdx.x / CTA;
+
+  if (tid == 0) {
+    for (int s = 0; s < STAGES; ++s) {
+      tc::mbar_init(bar(B_FULL + s), 1);
+      tc::mbar_init(bar(B_EMPTY + s), 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      tc::mbar_init(bar(B_ACCFULL + b), 1);
+      tc::mbar_init(bar(B_ACCEMPTY + b), 8 * CTA);
+    }
+    for (int b = 0; b < 4; ++b) tc::mbar_init(bar(B_RES + b), 1);
+    tc::mbar_init(bar(B_DRAIN), 1);
+    misc[1] = 0u;
+    tc::mbar_fence_init();
+  }
+  if (warp == 2) {
+    Pair<CTA>::alloc(base + OFF_MISC);
+    Pair<CTA>::relinquish();
+  }
+  tc::tc_fence_before();
+  __syncthreads();
+  if (CTA == 2) cluster_sync();
+  tc::tc_fence_after();
+  const uint32_t tmem = misc[0];
+
+  if (warp == 0) {
+    // ================= TMA producer =================
+    if (lane == 0) {
+      tc::prefetch_tmap(&tm_a);
+      tc::prefetch_tmap(&tm_b);
+      Walk w(p, worker);
+      uint32_t it = 0;
+      bool ok = true;
+      while (ok && w.next()) {
+        const int m0 = (int)(w.tile / p.tiles_n) * BN + rank * BM;
+        const int n0 = (int)(w.tile % p.tiles_n) * BN + rank * BM;
+        for (int k = w.k0; k < w.k1; ++k, ++it) {
+          const uint32_t s = it % STAGES;
+          if (it >= STAGES && !tc::mbar_wait(bar(B_EMPTY + s), (it / STAGES - 1) & 1, abort_flag,
+                                             p.wait_ns)) {
+            ok = false;
+            break;
+          }
+          // the barrier is the first CTA's: it counts both CTAs' bytes
+          uint32_t full = bar(B_FULL + s);
+          if (CTA == 2) full = map_rank(full, 0);
+          if (rank == 0) tc::mbar_expect_tx(bar(B_FULL + s), CTA * STAGE_BYTES);
+          const uint32_t a = base + s * STAGE_BYTES, b = a + HALF_BYTES;
+          if (AMN) {
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              const int c = m0 / 64 + j, head = c / p.a_heads64;
+              Pair<CTA>::load(a + j * (HALF_BYTES / 2), &tm_a, full, (c - head * p.a_heads64) * 64,
+                              k * BK, head);
+            }
+          } else {
+            const int head = k / p.a_heads64;
+            Pair<CTA>::load(a, &tm_a, full, (k - head * p.a_heads64) * BK, m0, head);
+          }
+          if (BMN) {
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              const int c = n0 / 64 + j, head = c / p.b_heads64;
+              Pair<CTA>::load(b + j * (HALF_BYTES / 2), &tm_b, full, (c - head * p.b_heads64) * 64,
+                              k * BK, head);
+            }
+          } else {
+            const int head = k / p.b_heads64;
+            Pair<CTA>::load(b, &tm_b, full, (k - head * p.b_heads64) * BK, n0, head);
+          }
+        }
+      }
+      // the last copies have landed before the memory goes (the MMAs that read them are awaited
+      // by their issuer)
+      if (rank == 0)
+        for (uint32_t t = it > STAGES ? it - STAGES : 0; t < it; ++t)
+          tc::mbar_wait_drain(bar(B_FULL + t % STAGES), (t / STAGES) & 1, p.wait_ns);
+    }
+  } else if (warp == 1) {
+    // ================= MMA issuer (of the pair's first CTA) =================
+    if (lane == 0 && rank == 0) {
+      const uint32_t fmt = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
+      const uint32_t idesc = tc::idesc_f16(fmt, BMN ? 1u : 0u, BN, BN) | (AMN ? 1u << 15 : 0u);
+      // a step of 16 reduced elements: 32 bytes along a K-major row, 16 MN-major rows
+      constexpr uint64_t kStepA = AMN ? 16 * 128 / 16 : 2, kStepB = BMN ? 16 * 128 / 16 : 2;
+      bool ok = true;
+      if (p.wait_selftest) ok = tc::mbar_wait(bar(B_DRAIN), 0, abort_flag, p.wait_ns);
+      Walk w(p, worker);
+      uint32_t it = 0, i = 0;
+      while (ok && w.next()) {
+        const uint32_t b = i & 1;
+        if (i >= 2 &&
+            !tc::mbar_wait(bar(B_ACCEMPTY + b), ((i >> 1) + 1) & 1, abort_flag, p.wait_ns)) {
+          ok = false;
+          break;
+        }
+        tc::tc_fence_after();
+        const uint32_t acc = tmem + b * BN;
+        for (int k = w.k0; k < w.k1; ++k, ++it) {
+          const uint32_t s = it % STAGES;
+          if (!tc::mbar_wait(bar(B_FULL + s), (it / STAGES) & 1, abort_flag, p.wait_ns)) {
+            ok = false;
+            break;
+          }
+          tc::tc_fence_after();
+          const uint32_t a = base + s * STAGE_BYTES;
+          const uint64_t ad = tc::sw128_desc(a, HALF_BYTES / 2),
+                         bd = tc::sw128_desc(a + HALF_BYTES, HALF_BYTES / 2);
+#pragma unroll
+          for (int kk = 0; kk < BK / 16; ++kk)
+            Pair<CTA>::mma(acc, ad + kk * kStepA, bd + kk * kStepB, idesc,
+                           (k > w.k0 || kk > 0) ? 1u : 0u);
+          Pair<CTA>::commit(bar(B_EMPTY + s));
+        }
+        if (ok) Pair<CTA>::commit(bar(B_ACCFULL + b));
+        ++i;
+      }
+      if (!p.wait_selftest) {
+        Pair<CTA>::commit(bar(B_DRAIN));
+        tc::mbar_wait_drain(bar(B_DRAIN), 0, p.wait_ns);
+      }
+    }
+  } else if (warp >= 4) {
+    // ================= epilogue: groups of warps 4-7 and 8-11 =================
+    const int g = (warp - 4) >> 2, sub = warp & 3, row = sub * 32 + lane, t = tid & 127;
+    const uint32_t lanes = (uint32_t)(sub * 32) << 16;
+    float* vec = reinterpret_cast<float*>(sbase + OFF_VEC) + g * 128;  // bias | gate
+    volatile int* votes = reinterpret_cast<volatile int*>(misc + 2) + g * 16;
+    const T* bias = static_cast<const T*>(p.bias);
+    const T* gate = static_cast<const T*>(p.gate);
+    auto group_sync = [&] { asm volatile("bar.sync %0, 128;" ::"r"(1 + g) : "memory"); };
+    // true in all four warps or in none: the barriers of a group are not bounded, so that its
+    // warps have to leave together
+    auto agree = [&](int* slots4, bool ok) {
+      const bool all = __all_sync(0xffffffffu, ok);
+      volatile int* v = slots4;
+      if (lane == 0) v[sub] = all ? 1 : 0;
+      group_sync();
+      return v[0] && v[1] && v[2] && v[3];
+    };
+    const bool has_res = !SPLIT && p.residual != nullptr, has_z = !SPLIT && p.z != nullptr;
+    Walk w(p, worker);
+    uint32_t i = 0, uses = 0, res_uses[2] = {0, 0};
+    bool ok = true;
+    while (ok && w.next()) {
+      const uint32_t b = i & 1;
+      const int64_t m0 = w.tile / p.tiles_n * BN + rank * BM, n0 = w.tile % p.tiles_n * BN;
+      const bool got = tc::warp_wait(bar(B_ACCFULL + b), (i >> 1) & 1, abort_flag, p.wait_ns);
+      if (!agree(const_cast<int*>(votes) + 4 * b, got)) {
+        ok = false;
+        break;
+      }
+      tc::tc_fence_after();
+      const uint32_t acc = tmem + b * BN + lanes;
+      for (int sc = g; ok && sc < BN / 64; sc += 2) {
+        const int64_t col = n0 + sc * 64;
+        if (col >= p.n) continue;
+        if (!SPLIT) {
+          // seen by the group after the next barrier; the last readers are before the last one
+          const int64_t c = col + (t & 63);
+          float v = t < 64 ? 0.f : 1.f;
+          const T* src = t < 64 ? bias : gate;
+          if (src != nullptr && c < p.n) v = to_float(src[c]);
+          vec[t] = v;
+        }
+        const int first = has_z ? kUseZ : SPLIT ? kUseSlot : kUseY;
+        for (int kind = first; ok && kind <= (SPLIT ? kUseSlot : kUseY); ++kind) {
+          // a buffer row is 64 elements of T or 32 of fp32
+          const bool wide = SPLIT || (kind == kUseY && p.y_fp32);
+          for (int part = 0; ok && part < (wide ? 2 : 1); ++part, ++uses) {
+            const int64_t c0 = col + part * 32;  // first column of the use
+            if (!SPLIT && c0 >= p.n) break;
+            const uint32_t u = uses & 1, buf = base + OFF_BUF + (uint32_t)(2 * g + u) * BUF_BYTES;
+            const bool res = kind == kUseY && has_res;
+            const int head = (int)(c0 / 64) / p.y_heads64;
+            const int in_head = (int)(c0 - (int64_t)head * p.y_heads64 * 64);
+            bool fine = true;
+            if (t == 0) store_wait_read<1>();  // the store before last, from this buffer
+            if (res && p.res_tma) {
+              if (t == 0) {
+                tc::mbar_expect_tx(bar(B_RES + 2 * g + u), BUF_BYTES);
+                tc::tma_load_3d(buf, &tm_res, bar(B_RES + 2 * g + u), (int)c0, (int)m0, 0);
+              }
+              __syncwarp();
+              fine = tc::warp_wait(bar(B_RES + 2 * g + u), res_uses[u] & 1, abort_flag, p.wait_ns);
+              ++res_uses[u];
+            }
+            if (!agree(const_cast<int*>(votes) + 8 + 4 * u, fine)) {
+              ok = false;
+              break;
+            }
+            if (res && !p.res_tma) {
+              const int64_t r0 = m0 + sub * 32;
+              if (p.y_fp32)
+                copy_rows(buf, sub * 32,
+                          const_cast<float*>(static_cast<const float*>(p.residual)) +
+                              r0 * p.residual_stride + c0,
+                          p.residual_stride, p.m - r0, p.n - c0, true);
+              else
+                copy_rows(buf, sub * 32,
+                          const_cast<T*>(static_cast<const T*>(p.residual)) +
+                              r0 * p.residual_stride + c0,
+                          p.residual_stride, p.m - r0, p.n - c0, true);
+              __syncwarp();
+            }
+            // 32 columns at a time: TMEM -> registers -> buffer
+            for (int h = wide ? part : 0; h < (wide ? part + 1 : 2); ++h) {
+              uint32_t r[32];
+              tc::tmem_ld32(acc + sc * 64 + h * 32, r);
+              tc::tmem_wait_ld();
+              if (SPLIT) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                  sts128(piece(buf, row, j), r[4 * j], r[4 * j + 1], r[4 * j + 2], r[4 * j + 3]);
+                continue;
+              }
+              const float* bv = vec + h * 32;
+              float v[32];
+#pragma unroll
+              for (int j = 0; j < 8; ++j) {
+                const float4 q = reinterpret_cast<const float4*>(bv)[j];
+                v[4 * j] = __uint_as_float(r[4 * j]) + q.x;
+                v[4 * j + 1] = __uint_as_float(r[4 * j + 1]) + q.y;
+                v[4 * j + 2] = __uint_as_float(r[4 * j + 2]) + q.z;
+                v[4 * j + 3] = __uint_as_float(r[4 * j + 3]) + q.w;
+              }
+              if (kind == kUseY) {
+                act::dispatch(p.act, [&](auto k) {
+#pragma unroll
+                  for (int j = 0; j < 32; ++j) v[j] = act::value<decltype(k)::value>(v[j]);
+                });
+                if (gate != nullptr) {
+#pragma unroll
+                  for (int j = 0; j < 8; ++j) {
+                    const float4 q = reinterpret_cast<const float4*>(bv + 64)[j];
+                    v[4 * j] *= q.x;
+                    v[4 * j + 1] *= q.y;
+                    v[4 * j + 2] *= q.z;
+                    v[4 * j + 3] *= q.w;
+                  }
+                }
+              }
+              if (wide) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                  const uint32_t a = piece(buf, row, j);
+                  if (res) {
+                    uint32_t q[4];
+                    lds128(a, q);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) v[4 * j + e] += __uint_as_float(q[e]);
+                  }
+                  sts128(a, __float_as_uint(v[4 * j]), __float_as_uint(v[4 * j + 1]),
+                         __float_as_uint(v[4 * j + 2]), __float_as_uint(v[4 * j + 3]));
+                }
+              } else {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                  const uint32_t a = piece(buf, row, h * 4 + j);
+                  if (res) {
+                    uint32_t q[4];
+                    lds128(a, q);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                      const float2 f = ElemOps<T>::to_float2(q[e]);
+                      v[8 * j + 2 * e] += f.x;
+                      v[8 * j + 2 * e + 1] += f.y;
+                    }
+                  }
+                  sts128(a, ElemOps<T>::pack2(v[8 * j], v[8 * j + 1]),
+                         ElemOps<T>::pack2(v[8 * j + 2], v[8 * j + 3]),
+                         ElemOps<T>::pack2(v[8 * j + 4], v[8 * j + 5]),
+                         ElemOps<T>::pack2(v[8 * j + 6], v[8 * j + 7]));
+                }
+              }
+            }
+            const bool by_tma = SPLIT || (kind == kUseZ ? p.z_tma : p.y_tma);
+            if (by_tma) {
+              asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+              group_sync();
+              if (t == 0) {
+                if (SPLIT) {
+                  const int64_t slot = worker + w.tile;
+                  store_bulk(reinterpret_cast<unsigned char*>(p.slots) +
+                                 ((slot * CTA + rank) * (BN / 32) + sc * 2 + part) * BUF_BYTES,
+                             buf, BUF_BYTES);
+                } else if (m0 < p.m) {
+                  if (kind == kUseZ)
+                    store_3d(&tm_z, buf, (int)c0, (int)m0, 0);
+                  else
+                    store_3d(&tm_y, buf, in_head, (int)m0, head);
+                }
+                store_commit();
+              }
+            } else {
+              __syncwarp();
+              const int64_t r0 = m0 + sub * 32, rows = p.m - r0, left = p.n - c0;
+              if (kind == kUseZ)
+                copy_rows(buf, sub * 32, static_cast<T*>(p.z) + r0 * p.z_stride + c0, p.z_stride,
+                          rows, left, false);
+              else if (p.y_fp32)
+                copy_rows(buf, sub * 32, static_cast<float*>(p.y) + r0 * p.y_stride + c0,
+                          p.y_stride, rows, left, false);
+              else
+                copy_rows(buf, sub * 32,
+                          static_cast<T*>(p.y) + head * p.y_head_stride + r0 * p.y_stride + in_head,
+                          p.y_stride, rows, left, false);
+              // the buffer's next use may begin with a copy by TMA
+              asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+              group_sync();
+              if (t == 0) store_commit();  // a group per use, this one empty
+            }
+          }
+        }
+      }
+      if (!ok) break;
+      tc::tc_fence_before();
+      __syncwarp();
+      if (lane == 0) {
+        if (CTA == 2)
+          arrive_cluster(map_rank(bar(B_ACCEMPTY + b), 0));
+        else
+          tc::mbar_arrive(bar(B_ACCEMPTY + b));
+      }
+      ++i;
+    }
+    if (t == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+  }
+
+  tc::tc_fence_before();
+  __syncthreads();
+  __syncwarp();
+  if (CTA == 2) cluster_sync();
+  tc::tc_fence_after();
+  if (tid == 0 && *abort_flag && p.status != nullptr) atomicOr(p.status, VGGT_STATUS_TIMEOUT);
+  if (warp == 2) Pair<CTA>::dealloc(tmem);
+}
+
+// Adds up a split product's partial sums and runs the epilogue: a thread takes 8 columns of a row.
+template <typename T>
+__global__ void __launch_bounds__(256)
+    finish_kernel(const Slots s, int64_t m, int64_t n, const Epilogue e, bool wide) {
+  const int64_t groups = (n + 7) / 8, all = m * groups;
+  for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < all;
+       i += (int64_t)gridDim.x * blockDim.x) {
+    const int64_t r = i / groups, c = (i - r * groups) * 8;
+    const int k = (int)min((int64_t)8, n - c);
+    float v[8];
+    s.get8(r, c, v);
+    float t[8];
+    if (e.bias != nullptr) {
+      get8(static_cast<const T*>(e.bias) + c, k, wide, t);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] += t[j];
+    }
+    if (e.z != nullptr) put8(static_cast<T*>(e.z) + r * e.z_stride + c, k, wide, v);
+    act::dispatch(e.act, [&](auto kind) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = act::value<decltype(kind)::value>(v[j]);
+    });
+    if (e.gate != nullptr) {
+      get8(static_cast<const T*>(e.gate) + c, k, wide, t);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] *= t[j];
+    }
+    const bool fp32 = e.y_type == VGGT_DTYPE_FP32;
+    if (e.residual != nullptr) {
+      const int64_t at = r * e.residual_stride + c;
+      if (fp32)
+        get8(static_cast<const float*>(e.residual) + at, k, wide, t);
+      else
+        get8(static_cast<const T*>(e.residual) + at, k, wide, t);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] += t[j];
+    }
+    const int64_t head = c / e.y_dim;
+    const int64_t at = head * e.y_head_stride + r * e.y_stride + (c - head * e.y_dim);
+    if (fp32)
+      put8(static_cast<float*>(e.y) + at, k, wide, v);
+    else
+      put8(static_cast<T*>(e.y) + at, k, wide, v);
+  }
+}
+
+// ---- host -------------------------------------------------------------------------------------
+size_t Plan::slot_bytes() const {
+  return split ? (size_t)(workers + tiles_m * tiles_n) * cta * cta * BM * 128 * 4 : 0;
+}
+
+static int sm_count() {
+  int sms = 0;
+  return device_sms(&sms) == cudaSuccess && sms > 0 ? sms : 148;
+}
+
+Plan plan_product(int64_t m, int64_t n, int64_t red, bool must_split) {
+  const int sms = sm_count();
+  Plan p;
+  p.cta = 1;
+  p.split = must_split ? 1 : 0;
+  p.workers = sms / p.cta;
+  p.tiles_m = (m + 128 * p.cta - 1) / (128 * p.cta);
+  p.tiles_n = (n + 128 * p.cta - 1) / (128 * p.cta);
+  p.blocks = (red + BK - 1) / BK;
+  const int64_t work = p.tiles_m * p.tiles_n * (p.split ? p.blocks : 1);
+  if (p.workers > work) p.workers = (int)work;
+  return p;
+}
+
+static bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
+static bool operand_map(CUtensorMap* map, const Operand& o, int dtype, int64_t rows) {
+  const uint64_t dims[3] = {(uint64_t)o.dim, (uint64_t)rows, (uint64_t)o.heads};
+  // a stride that is never used may be anything: give a valid one
+  const int64_t row = rows > 1 ? o.stride : (o.dim + 7) / 8 * 8;
+  const uint64_t strides[2] = {(uint64_t)row * 2,
+                               (uint64_t)(o.heads > 1 ? o.head_stride : row * rows) * 2};
+  const uint32_t box[3] = {64, o.mn_major ? (uint32_t)BK : (uint32_t)BM, 1};
+  return encode_tmap_sw128(map, o.p, dtype, 3, dims, strides, box);
+}
+
+// Rows of an output or of the residual, for copies of 128 rows x 128 bytes; false where TMA
+// cannot address them.
+static bool rows_map(CUtensorMap* map, const void* p, int type, int64_t stride, int64_t head_stride,
+                     int64_t heads, int64_t dim, int64_t rows) {
+  const int per = type == VGGT_DTYPE_FP32 ? 4 : 8, size = 16 / per;
+  if (!aligned16(p) || dim % per || (rows > 1 && stride % per) || (heads > 1 && head_stride % per))
+    return false;
+  const int64_t row = rows > 1 ? stride : dim;
+  const uint64_t dims[3] = {(uint64_t)dim, (uint64_t)rows, (uint64_t)heads};
+  const uint64_t strides[2] = {(uint64_t)row * size,
+                               (uint64_t)(heads > 1 ? head_stride : row * rows) * size};
+  const uint32_t box[3] = {(uint32_t)(128 / size), (uint32_t)BM, 1};
+  return encode_tmap_sw128(map, p, type, 3, dims, strides, box);
+}
+
+template <typename T, int CTA, bool AMN, bool BMN, bool SPLIT>
+static cudaError_t launch_kernel(const CUtensorMap* maps, const Params& p, cudaStream_t stream) {
+  auto k = product_kernel<T, CTA, AMN, BMN, SPLIT>;
+  cudaError_t e =
+      cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SMEM_BYTES);
+  if (e != cudaSuccess) return e;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)(p.workers * CTA));
+  cfg.blockDim = dim3(THREADS);
+  cfg.dynamicSmemBytes = SMEM_BYTES;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = CTA;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  e = cudaLaunchKernelEx(&cfg, k, maps[0], maps[1], maps[2], maps[3], maps[4], p);
+  return e != cudaSuccess ? e : cudaGetLastError();
+}
+
+template <typename T, int CTA>
+static cudaError_t launch_majors(bool amn, bool bmn, bool split, const CUtensorMap* maps,
+                                 const Params& p, cudaStream_t stream) {
+  if (!amn && !bmn)
+    return split ? launch_kernel<T, CTA, false, false, true>(maps, p, stream)
+                 : launch_kernel<T, CTA, false, false, false>(maps, p, stream);
+  if (!amn)
+    return split ? launch_kernel<T, CTA, false, true, true>(maps, p, stream)
+                 : launch_kernel<T, CTA, false, true, false>(maps, p, stream);
+  // the weight's gradient is always split
+  return split && bmn ? launch_kernel<T, CTA, true, true, true>(maps, p, stream)
+                      : cudaErrorInvalidValue;
+}
+
+cudaError_t launch_product(const Plan& plan, int dtype, int64_t m, int64_t n, int64_t red,
+                           const Operand& a, const Operand& b, const Epilogue& e, float* slots,
+                           int32_t* status, cudaStream_t stream) {
+  CUtensorMap maps[5] = {};
+  if (!operand_map(&maps[0], a, dtype, a.mn_major ? red : m) ||
+      !operand_map(&maps[1], b, dtype, b.mn_major ? red : n))
+    return cudaErrorInvalidValue;
+  Params p{};
+  p.m = m;
+  p.n = n;
+  p.tiles = plan.tiles_m * plan.tiles_n;
+  p.tiles_n = plan.tiles_n;
+  p.blocks = (int)plan.blocks;
+  p.workers = plan.workers;
+  p.split = plan.split;
+  auto heads64 = [](int64_t heads, int64_t dim) { return heads > 1 ? (int)(dim / 64) : INT_MAX; };
+  p.a_heads64 = heads64(a.heads, a.dim);
+  p.b_heads64 = heads64(b.heads, b.dim);
+  p.y_heads64 = heads64(e.y_heads, e.y_dim);
+  p.bias = e.bias;
+  p.gate = e.gate;
+  p.act = e.act;
+  p.y_fp32 = e.y_type == VGGT_DTYPE_FP32;
+  p.residual = e.residual;
+  p.residual_stride = e.residual_stride;
+  p.y = e.y;
+  p.y_stride = e.y_stride;
+  p.y_head_stride = e.y_head_stride;
+  p.z = e.z;
+  p.z_stride = e.z_stride;
+  if (!plan.split) {
+    p.y_tma = rows_map(&maps[2], e.y, e.y_type, e.y_stride, e.y_head_stride, e.y_heads, e.y_dim, m);
+    p.res_tma = e.residual &&
+                rows_map(&maps[3], e.residual, e.y_type, e.residual_stride, 0, 1, n, m);
+    p.z_tma = e.z && rows_map(&maps[4], e.z, dtype, e.z_stride, 0, 1, n, m);
+  }
+  p.slots = slots;
+  p.status = status;
+  p.wait_ns = api_wait_ns();
+  p.wait_selftest = api_wait_selftest();
+  if (dtype == VGGT_DTYPE_BF16)
+    return launch_majors<__nv_bfloat16, 1>(a.mn_major, b.mn_major, plan.split, maps, p, stream);
+  return launch_majors<__half, 1>(a.mn_major, b.mn_major, plan.split, maps, p, stream);
+}
+
+Slots slots_of(const Plan& plan, const float* p) {
+  return {p, plan.tiles_m * plan.tiles_n * plan.blocks, plan.tiles_n, plan.cta, (int)plan.blocks,
+          plan.workers};
+}
+
+cudaError_t finish_product(const Plan& plan, int dtype, int64_t m, int64_t n, const Epilogue& e,
+                           const float* slots, cudaStream_t stream) {
+  const int64_t all = m * ((n + 7) / 8);
+  const unsigned grid = (unsigned)std::min<int64_t>((all + 255) / 256, 148 * 16);
+  const bool wide = wide_rows(e.y, e.y_stride, e.y_type) && e.y_dim % 8 == 0 &&
+                    (e.y_heads <= 1 || e.y_head_stride % 8 == 0) &&
+                    wide_rows(e.z, e.z_stride, dtype) && wide_rows(e.bias, 8, dtype) &&
+                    wide_rows(e.gate, 8, dtype) &&
+                    wide_rows(e.residual, e.residual_stride, e.y_type);
+  const Slots s = slots_of(plan, slots);
+  if (dtype == VGGT_DTYPE_BF16)
+    finish_kernel<__nv_bfloat16><<<grid, 256, 0, stream>>>(s, m, n, e, wide);
+  else
+    finish_kernel<__half><<<grid, 256, 0, stream>>>(s, m, n, e, wide);
+  return cudaGetLastError();
+}
+
+}  // namespace lin
+}  // namespace vggt
+
+// ---- C ABI ------------------------------------------------------------------------------------
+namespace vggt {
+namespace lin {
+
+int check(const vggt_linear_args* a) {
+  if (!a) return api_fail("args must be non-NULL");
+  if (a->dtype != VGGT_DTYPE_BF16 && a->dtype != VGGT_DTYPE_FP16)
+    return api_fail("linear requires BF16 or FP16");
+  if (a->stream_dtype != a->dtype && a->stream_dtype != VGGT_DTYPE_FP32)
+    return api_fail("the residual and y are of x's type or FP32");
+  if (a->rows < 0 || a->inner < 1 || a->outer < 1) return api_fail("bad size argument");
+  if (a->rows > INT_MAX - 512 || a->inner > INT_MAX - 512 || a->outer > INT_MAX - 512)
+    return api_fail("too many rows or too wide");
+  if (a->inner % 8) return api_fail("inner (%lld) must be a multiple of 8", (long long)a->inner);
+  if (a->heads > 1 && (a->inner % a->heads || a->inner / a->heads % 64))
+    return api_fail("a head-major x needs heads of a multiple of 64 elements");
+  if (a->activation < VGGT_ACT_NONE || a->activation > VGGT_ACT_RELU)
+    return api_fail("unknown activation %d", a->activation);
+  if (a->rows == 0) return 0;
+  if (!a->x || !a->weight) return api_fail("x and weight must be non-NULL");
+  const int64_t dim = a->heads > 1 ? a->inner / a->heads : a->inner;
+  if (!aligned16(a->x) || !aligned16(a->weight) || (a->rows > 1 && a->x_stride % 8) ||
+      (a->heads > 1 && a->x_head_stride % 8) || (a->outer > 1 && a->weight_stride % 8))
+    return api_fail("x and weight must start on 16 bytes, with strides that are multiples of 8");
+  if ((a->rows > 1 && a->x_stride < dim) || (a->heads > 1 && a->x_head_stride < dim) ||
+      (a->outer > 1 && a->weight_stride < a->inner))
+    return api_fail("a stride of x or weight is below the row's width");
+  if (a->residual && a->rows > 1 && a->residual_stride < 0) return api_fail("negative stride");
+  return 0;
+}
+
+Operand x_operand(const vggt_linear_args* a, bool mn_major) {
+  const int64_t heads = a->heads > 1 ? a->heads : 1;
+  Operand o;
+  o.p = a->x;
+  o.stride = a->x_stride;
+  o.head_stride = a->x_head_stride;
+  o.heads = heads;
+  o.dim = a->inner / heads;
+  o.mn_major = mn_major;
+  return o;
+}
+
+Operand matrix(const void* p, int64_t width, int64_t stride, bool mn_major) {
+  Operand o;
+  o.p = p;
+  o.stride = stride;
+  o.dim = width;
+  o.mn_major = mn_major;
+  return o;
+}
+
+}  // namespace lin
+}  // namespace vggt
+
+extern "C" size_t vggt_linear_workspace_size(const vggt_linear_args* a) {
+  using namespace vggt::lin;
+  if (!a || a->rows <= 0 || a->inner < 1 || a->outer < 1) return 0;
+  return plan_product(a->rows, a->outer, a->inner, false).slot_bytes();
+}
+
+extern "C" int vggt_linear(const vggt_linear_args* a, void* y, int64_t y_stride, void* z,
+                           int64_t z_stride, int32_t* status, void* workspace,
+                           size_t workspace_bytes, void* stream) {
+  using namespace vggt;
+  using namespace vggt::lin;
+  if (int rc = check(a)) return rc;
+  if (a->rows == 0) return api_fail(nullptr);
+  if (!y) return api_fail("y must be non-NULL");
+  if (a->rows > 1 && (y_stride < a->outer || (z && z_stride < a->outer)))
+    return api_fail("an output's rows overlap: its stride is below outer");
+  const Plan plan = plan_product(a->rows, a->outer, a->inner, false);
+  if (plan.slot_bytes() > 0 &&
+      (!workspace || !aligned16(workspace) || workspace_bytes < plan.slot_bytes()))
+    return api_fail("the workspace is too small or not 16-byte aligned");
+  Epilogue e;
+  e.bias = a->bias;
+  e.gate = a->gate;
+  e.act = a->activation;
+  e.residual = a->residual;
+  e.residual_stride = a->residual_stride;
+  e.y = y;
+  e.y_stride = y_stride;
+  e.y_dim = a->outer;
+  e.y_type = a->stream_dtype;
+  e.z = z;
+  e.z_stride = z_stride;
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  float* slots = static_cast<float*>(workspace);
+  cudaError_t rc = launch_product(plan, a->dtype, a->rows, a->outer, a->inner, x_operand(a, false),
+                                  matrix(a->weight, a->inner, a->weight_stride, false), e, slots,
+                                  status, st);
+  if (rc == cudaSuccess && plan.split)
+    rc = finish_product(plan, a->dtype, a->rows, a->outer, e, slots, st);
+  return api_cuda(rc);
+}

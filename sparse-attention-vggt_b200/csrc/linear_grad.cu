@@ -1,0 +1,371 @@
+// Gradients of y = residual + gate * act(x W^T + b).
+//
+// With an activation: dz = dy gate act'(z) and, from z, dgate = sum dy act(z); then
+//   dx = dz W,  dW = dz^T x,  db = sum dz.
+// Without one, z is not needed.  With G = dy^T x and s = sum dy (over the rows),
+//   dW = gate G,  db = gate s,  dgate_n = <W_n, G_n> + b_n s_n,  dx = dy (gate W):
+// the only pass over [rows][outer] beside the two products is the one that forms s.
+//
+// dW is a product over the rows, cut evenly over the SMs (its tiles are few); the partial sums
+// lie in fp32 in the workspace until finish_weight adds them, scales them by the gate and forms
+// the row products of dgate.  Nothing is added with atomics: equal calls give equal bits.
+#include <algorithm>
+
+#include "activation.cuh"
+#include "linear.cuh"
+
+namespace vggt {
+namespace lin {
+
+// The pass over dy: column sums of dz (and of dy act(z)) per block of rows, and dz rounded for the
+// products.  A thread takes 8 columns of every 8th row of its block.
+struct Sums {
+  const void* dy;
+  int64_t dy_stride;
+  const void* z;
+  int64_t z_stride;
+  const void* gate;
+  int act;
+  void* dz;      // [rows][dz_stride], or null
+  void* scaled;  // gate dy (no activation), or null
+  int64_t dz_stride;
+  float* bias_part;  // [row blocks][outer], or null
+  float* gate_part;
+  int64_t rows, outer, per_block;
+  bool wide;
+};
+
+template <typename S, typename T>
+__global__ void __launch_bounds__(256) sums_kernel(const Sums a) {
+  __shared__ float fold[8][256];
+  const int cx = threadIdx.x & 31, ry = threadIdx.x >> 5;
+  const int64_t c = ((int64_t)blockIdx.x * 32 + cx) * 8;
+  const int n = (int)max((int64_t)0, min((int64_t)8, a.outer - c));
+  const int64_t r0 = blockIdx.y * a.per_block, r1 = min(a.rows, r0 + a.per_block);
+  float sb[8], sg[8], gate[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) sb[i] = sg[i] = 0.f, gate[i] = 1.f;
+  if (n > 0) {
+    if (a.gate != nullptr) get8(static_cast<const T*>(a.gate) + c, n, a.wide, gate);
+    act::dispatch(a.act, [&](auto k) {
+      constexpr int kind = decltype(k)::value;
+#pragma unroll 4
+      for (int64_t r = r0 + ry; r < r1; r += 8) {
+        float d[8];
+        get8(static_cast<const S*>(a.dy) + r * a.dy_stride + c, n, a.wide, d);
+        if (kind != VGGT_ACT_NONE) {
+          float z[8];
+          get8(static_cast<const T*>(a.z) + r * a.z_stride + c, n, a.wide, z);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            float slope;
+            const float v = act::value_slope<kind>(z[i], slope);
+            sg[i] = fmaf(d[i], v, sg[i]);
+            d[i] *= gate[i] * slope;
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) sb[i] += d[i];
+        if (a.dz != nullptr) put8(static_cast<T*>(a.dz) + r * a.dz_stride + c, n, a.wide, d);
+        if (a.scaled != nullptr) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) d[i] *= gate[i];
+          put8(static_cast<T*>(a.scaled) + r * a.dz_stride + c, n, a.wide, d);
+        }
+      }
+    });
+  }
+  for (int which = 0; which < 2; ++which) {
+    float* out = which == 0 ? a.bias_part : a.gate_part;
+    if (out == nullptr) continue;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 8; ++i) fold[ry][cx * 8 + i] = which == 0 ? sb[i] : sg[i];
+    __syncthreads();
+    const int64_t col = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (col < a.outer) {
+      float s = 0.f;
+#pragma unroll
+      for (int q = 0; q < 8; ++q) s += fold[q][threadIdx.x];
+      out[blockIdx.y * a.outer + col] = s;
+    }
+  }
+}
+
+// gate W, rounded once more to W's type: one rounding of dx's factors, as dy gate would be.
+template <typename T>
+__global__ void __launch_bounds__(256)
+    scale_weight_kernel(const T* w, int64_t stride, const T* gate, T* to, int64_t outer,
+                        int64_t inner) {
+  const int64_t groups = inner / 8, all = outer * groups;
+  for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < all;
+       i += (int64_t)gridDim.x * blockDim.x) {
+    const int64_t r = i / groups, c = (i - r * groups) * 8;
+    float v[8];
+    Elem<T>::load8(w + r * stride + c, v);
+    const float g = (float)gate[r];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] *= g;
+    Elem<T>::store8(to + r * inner + c, v);
+  }
+}
+
+// A block per row of W: adds the partial sums of dW's row, and what the row's bias and gate get.
+struct Weights {
+  const void* weight;
+  int64_t weight_stride;
+  const void* bias;
+  const void* gate;
+  bool act;       // with an activation dz has the gate already, and gate_part the gate's sums
+  void* dweight;  // or null
+  int64_t dweight_stride;
+  void* dbias;
+  void* dgate;
+  const float* bias_part;
+  const float* gate_part;
+  int64_t row_blocks, outer, inner;
+  bool product;  // whether there are partial sums of a product
+  bool wide;
+};
+
+__device__ __forceinline__ float block_sum(float v, float* fold) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0) fold[threadIdx.x >> 5] = v;
+  __syncthreads();
+  return fold[0] + fold[1] + fold[2] + fold[3];
+}
+
+template <typename T>
+__global__ void __launch_bounds__(128) finish_weight_kernel(const Slots s, const Weights a) {
+  __shared__ float fold[4];
+  const int64_t r = blockIdx.x;
+  const float gate = a.gate != nullptr && !a.act ? (float)static_cast<const T*>(a.gate)[r] : 1.f;
+  const bool want_dot = a.dgate != nullptr && !a.act;
+  float dot = 0.f;
+  if (a.product)
+    for (int64_t c = threadIdx.x * 8; c < a.inner; c += 128 * 8) {
+      float v[8];
+      s.get8(r, c, v);
+      if (want_dot) {
+        float w[8];
+        Elem<T>::load8(static_cast<const T*>(a.weight) + r * a.weight_stride + c, w);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) dot = fmaf(v[i], w[i], dot);
+      }
+      if (a.dweight != nullptr) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] *= gate;
+        put8(static_cast<T*>(a.dweight) + r * a.dweight_stride + c, 8, a.wide, v);
+      }
+    }
+  float sum = 0.f;
+  if (a.bias_part != nullptr) {
+    for (int64_t i = threadIdx.x; i < a.row_blocks; i += 128) sum += a.bias_part[i * a.outer + r];
+    sum = block_sum(sum, fold);
+  }
+  if (a.dbias != nullptr && threadIdx.x == 0)
+    static_cast<T*>(a.dbias)[r] = ElemOps<T>::from_float(gate * sum);
+  if (a.dgate == nullptr) return;
+  float g = 0.f;
+  if (a.act) {
+    for (int64_t i = threadIdx.x; i < a.row_blocks; i += 128) g += a.gate_part[i * a.outer + r];
+  } else {
+    g = dot;
+  }
+  g = block_sum(g, fold);
+  if (threadIdx.x == 0) {
+    if (!a.act && a.bias != nullptr) g = fmaf((float)static_cast<const T*>(a.bias)[r], sum, g);
+    static_cast<T*>(a.dgate)[r] = ElemOps<T>::from_float(g);
+  }
+}
+
+// What a backward call does, and where its workspace lies (offsets in bytes).
+struct Back {
+  bool act, dx, product, sums, copy_dy, scale_dy, scale_w;
+  int64_t row_blocks, per_block, pad;  // pad: row stride of dz
+  Plan px, pw;
+  size_t dz, scaled, weight, bias_part, gate_part, slots, bytes;
+};
+
+static bool tma_rows(const void* p, int64_t stride, int64_t width, int64_t rows) {
+  return (reinterpret_cast<uintptr_t>(p) & 15u) == 0 &&
+         (rows <= 1 || (stride % 8 == 0 && stride >= width));
+}
+
+static Back plan_back(const vggt_linear_args* a, const vggt_linear_grads* g) {
+  Back b{};
+  b.act = a->activation != VGGT_ACT_NONE;
+  const bool dgate = g->dgate && a->gate;
+  b.dx = g->dx != nullptr;
+  b.product = g->dweight != nullptr || (dgate && !b.act);
+  // dy as it lies, where it is of the products' type and TMA can read it
+  b.copy_dy = (b.dx || b.product) &&
+              (b.act || a->stream_dtype == VGGT_DTYPE_FP32 ||
+               !tma_rows(g->dy, g->dy_stride, a->outer, a->rows));
+  if (b.dx && a->gate && !b.act) {
+    // the gate goes to the smaller factor of dx
+    b.scale_dy = a->rows < a->inner;
+    b.scale_w = !b.scale_dy;
+  }
+  b.sums = b.copy_dy || b.scale_dy || (g->dbias && a->bias) || dgate;
+  const int64_t cols = (a->outer + 255) / 256;
+  b.row_blocks = std::max<int64_t>(1, std::min<int64_t>((a->rows + 31) / 32, 148 * 8 / cols));
+  b.per_block = (a->rows + b.row_blocks - 1) / b.row_blocks;
+  b.row_blocks = (a->rows + b.per_block - 1) / b.per_block;
+  b.pad = (a->outer + 7) / 8 * 8;
+  auto take = [&](bool need, size_t bytes) {
+    const size_t at = b.bytes;
+    if (need) b.bytes += (bytes + 255) / 256 * 256;
+    return at;
+  };
+  b.dz = take(b.copy_dy, (size_t)a->rows * b.pad * 2);
+  b.scaled = take(b.scale_dy, (size_t)a->rows * b.pad * 2);
+  b.weight = take(b.scale_w, (size_t)a->outer * a->inner * 2);
+  b.bias_part = take(b.sums, (size_t)b.row_blocks * a->outer * 4);
+  b.gate_part = take(b.sums && b.act, (size_t)b.row_blocks * a->outer * 4);
+  if (b.dx) b.px = plan_product(a->rows, a->inner, a->outer, false);
+  if (b.product) b.pw = plan_product(a->outer, a->inner, a->rows, true);
+  // the products run one after the other
+  b.slots = take(true, std::max(b.dx ? b.px.slot_bytes() : 0, b.product ? b.pw.slot_bytes() : 0));
+  return b;
+}
+
+template <typename T>
+static cudaError_t run_back(const vggt_linear_args* a, const vggt_linear_grads* g, const Back& b,
+                            int32_t* status, unsigned char* ws, cudaStream_t stream) {
+  const int64_t rows = a->rows, inner = a->inner, outer = a->outer;
+  float* bias_part = reinterpret_cast<float*>(ws + b.bias_part);
+  float* gate_part = reinterpret_cast<float*>(ws + b.gate_part);
+  float* slots = reinterpret_cast<float*>(ws + b.slots);
+  T* scaled = reinterpret_cast<T*>(ws + b.scaled);
+  if (b.sums) {
+    Sums s{};
+    s.dy = g->dy;
+    s.dy_stride = g->dy_stride;
+    s.z = g->z;
+    s.z_stride = g->z_stride;
+    s.gate = a->gate;
+    s.act = a->activation;
+    s.dz = b.copy_dy ? ws + b.dz : nullptr;
+    s.scaled = b.scale_dy ? scaled : nullptr;
+    s.dz_stride = b.pad;
+    s.bias_part = bias_part;
+    s.gate_part = b.act ? gate_part : nullptr;
+    s.rows = rows;
+    s.outer = outer;
+    s.per_block = b.per_block;
+    s.wide = outer % 8 == 0 && wide_rows(g->dy, g->dy_stride, a->stream_dtype) &&
+             (!b.act || wide_rows(g->z, g->z_stride, a->dtype)) && wide_rows(a->gate, 8, a->dtype);
+    const dim3 grid((unsigned)((outer + 255) / 256), (unsigned)b.row_blocks);
+    if (a->stream_dtype == VGGT_DTYPE_FP32)
+      sums_kernel<float, T><<<grid, 256, 0, stream>>>(s);
+    else
+      sums_kernel<T, T><<<grid, 256, 0, stream>>>(s);
+    if (cudaError_t e = cudaGetLastError()) return e;
+  }
+  const void* dz = b.copy_dy ? ws + b.dz : g->dy;
+  const int64_t dz_stride = b.copy_dy ? b.pad : g->dy_stride;
+  if (b.dx) {
+    const void* w = a->weight;
+    int64_t w_stride = a->weight_stride;
+    if (b.scale_w) {
+      T* to = reinterpret_cast<T*>(ws + b.weight);
+      const int64_t all = outer * (inner / 8);
+      scale_weight_kernel<T><<<(unsigned)std::min<int64_t>((all + 255) / 256, 148 * 16), 256, 0,
+                               stream>>>(static_cast<const T*>(w), w_stride,
+                                         static_cast<const T*>(a->gate), to, outer, inner);
+      if (cudaError_t e = cudaGetLastError()) return e;
+      w = to;
+      w_stride = inner;
+    }
+    Epilogue e;
+    e.y = g->dx;
+    e.y_stride = g->dx_stride;
+    e.y_head_stride = g->dx_head_stride;
+    e.y_heads = a->heads > 1 ? a->heads : 1;
+    e.y_dim = inner / e.y_heads;
+    e.y_type = a->dtype;
+    const Operand d = b.scale_dy ? matrix(scaled, outer, b.pad, false)
+                                 : matrix(dz, outer, dz_stride, false);
+    if (cudaError_t rc = launch_product(b.px, a->dtype, rows, inner, outer, d,
+                                        matrix(w, inner, w_stride, true), e, slots, status, stream))
+      return rc;
+    if (b.px.split)
+      if (cudaError_t rc = finish_product(b.px, a->dtype, rows, inner, e, slots, stream)) return rc;
+  }
+  if (b.product)
+    if (cudaError_t rc = launch_product(b.pw, a->dtype, outer, inner, rows,
+                                        matrix(dz, outer, dz_stride, true), x_operand(a, true),
+                                        Epilogue{}, slots, status, stream))
+      return rc;
+  Weights f{};
+  f.weight = a->weight;
+  f.weight_stride = a->weight_stride;
+  f.bias = a->bias;
+  f.gate = a->gate;
+  f.act = b.act;
+  f.dweight = g->dweight;
+  f.dweight_stride = g->dweight_stride;
+  f.dbias = a->bias ? g->dbias : nullptr;
+  f.dgate = a->gate ? g->dgate : nullptr;
+  if (!b.product && !f.dbias && !f.dgate) return cudaSuccess;
+  f.bias_part = b.sums ? bias_part : nullptr;
+  f.gate_part = gate_part;
+  f.row_blocks = b.row_blocks;
+  f.outer = outer;
+  f.inner = inner;
+  f.product = b.product;
+  f.wide = wide_rows(g->dweight, g->dweight_stride, a->dtype);
+  const Slots s = b.product ? slots_of(b.pw, slots) : Slots{};
+  finish_weight_kernel<T><<<(unsigned)outer, 128, 0, stream>>>(s, f);
+  return cudaGetLastError();
+}
+
+}  // namespace lin
+}  // namespace vggt
+
+extern "C" size_t vggt_linear_grad_workspace_size(const vggt_linear_args* a,
+                                                  const vggt_linear_grads* g) {
+  if (!a || !g || a->rows <= 0 || a->inner < 1 || a->outer < 1) return 0;
+  return vggt::lin::plan_back(a, g).bytes;
+}
+
+extern "C" int vggt_linear_grad(const vggt_linear_args* a, const vggt_linear_grads* g,
+                                int32_t* status, void* workspace, size_t workspace_bytes,
+                                void* stream) {
+  using namespace vggt;
+  using namespace vggt::lin;
+  if (int rc = check(a)) return rc;
+  if (!g) return api_fail("grads must be non-NULL");
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (g->dweight && a->outer > 1 && g->dweight_stride < a->inner)
+    return api_fail("dweight's stride is below inner");
+  if (a->rows == 0) {  // the sums of no rows
+    if (g->dweight)
+      if (int rc = api_cuda(cudaMemset2DAsync(g->dweight, (size_t)g->dweight_stride * 2, 0,
+                                              (size_t)a->inner * 2, (size_t)a->outer, st)))
+        return rc;
+    for (void* p : {a->bias ? g->dbias : nullptr, a->gate ? g->dgate : nullptr})
+      if (p)
+        if (int rc = api_cuda(cudaMemsetAsync(p, 0, (size_t)a->outer * 2, st))) return rc;
+    return api_fail(nullptr);
+  }
+  if (!g->dy) return api_fail("dy must be non-NULL");
+  if (a->activation != VGGT_ACT_NONE && !g->z)
+    return api_fail("with an activation the gradient needs z");
+  if (a->rows > 1 && (g->dy_stride < 0 || (g->z && g->z_stride < 0)))
+    return api_fail("negative stride");
+  const int64_t dim = a->heads > 1 ? a->inner / a->heads : a->inner;
+  if (g->dx && ((a->rows > 1 && g->dx_stride < dim) || (a->heads > 1 && g->dx_head_stride < dim)))
+    return api_fail("a stride of dx is below the row's width");
+  const Back b = plan_back(a, g);
+  if (b.bytes > 0 && (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 255u) ||
+                      workspace_bytes < b.bytes))
+    return api_fail("the workspace is too small or not 256-byte aligned");
+  unsigned char* ws = static_cast<unsigned char*>(workspace);
+  return api_cuda(a->dtype == VGGT_DTYPE_BF16
+                      ? run_back<__nv_bfloat16>(a, g, b, status, ws, st)
+                      : run_back<__half>(a, g, b, status, ws, st));
+}

@@ -269,7 +269,7 @@ __device__ __forceinline__ void tmem_wait_st() {
 // Host: 3-D tensor map [d2][d1][d0] of 2-byte elements (VGGT_DTYPE_*), box
 // (box0, box1, 1), 128-byte swizzle, zero fill out of bounds.  False when the
 // driver entry point is unavailable or the driver rejects the arguments.
-// Tiled map of 2-byte elements of any rank (strides in bytes, of dimensions 1
+// Tiled map of elements of VGGT_DTYPE_* of any rank (strides in bytes, of dimensions 1
 // and up), 128-byte swizzle, zero fill out of bounds.
 bool encode_tmap_sw128(CUtensorMap* map, const void* ptr, int dtype, int rank,
                        const uint64_t* dims, const uint64_t* strides, const uint32_t* box);

@@ -1,5 +1,5 @@
-"""ctypes binding of the C ABI declared in include/vggt_sparse.h and
-include/vggt_cache.h.
+"""ctypes binding of the C ABI declared in include/vggt_sparse.h,
+include/vggt_cache.h and include/vggt_block.h.
 
 The shared library is built in-tree (``vggt_sparse.build``).  There is no
 CPU or Python fallback: if the library is missing every operator raises
@@ -72,6 +72,14 @@ SIGNATURES = {
     "vggt_paged_evict_workspace_size": (ctypes.c_size_t, [_I64, _I, _I64, _I64]),
     "vggt_paged_evict": (_I, [_P, _P, _I, _P, _P, *_POOL, _P, _I64, _P, _I64, _P, _P, _P, _P, _P,
                               ctypes.c_size_t, _P]),
+    # structures by address: vggt_linear_args and the like (include/vggt_block.h)
+    "vggt_linear_workspace_size": (ctypes.c_size_t, [_P]),
+    "vggt_linear": (_I, [_P, _P, _I64, _P, _I64, _P, _P, ctypes.c_size_t, _P]),
+    "vggt_linear_grad_workspace_size": (ctypes.c_size_t, [_P, _P]),
+    "vggt_linear_grad": (_I, [_P, _P, _P, _P, ctypes.c_size_t, _P]),
+    "vggt_residual_norm": (_I, [_P, _P, _I64, _P, _I64, _P]),
+    "vggt_residual_norm_grad_workspace_size": (ctypes.c_size_t, [_I64, _I64, _I64]),
+    "vggt_residual_norm_grad": (_I, [_P, _P, _P, ctypes.c_size_t, _P]),
 }
 
 

@@ -18,7 +18,8 @@ CSRC = os.path.join(ROOT, "csrc")
 INCLUDE = os.path.join(REPO, "include")
 BUILD_DIR = os.path.join(ROOT, "_build")
 LIB_PATH = os.path.join(PKG_DIR, "libvggt_sparse.so")
-BINDING_PATH = os.path.join(PKG_DIR, "_cache_binding.so")  # Python module over the library
+BINDING_PATH = os.path.join(PKG_DIR, "_cache_binding.so")  # Python modules over the library
+BLOCK_BINDING_PATH = os.path.join(PKG_DIR, "_block_binding.so")
 
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = ["-std=c++17", "-O3", "-lineinfo", "-Xcompiler", "-fPIC", "--expt-relaxed-constexpr",
@@ -57,29 +58,30 @@ def _compile(nvcc, src, obj, extra):
     return res.stderr
 
 
-def _build_binding(force):
-    """The Python module of csrc/cache_binding.cpp, linked against the library next to it.
+def _build_binding(force, name="cache_binding"):
+    """The Python module of csrc/<name>.cpp, linked against the library next to it.
 
     It uses torch's C++ interface, which holds for one version: a stamp beside
     the objects says which torch and which Python it was built for."""
     import sysconfig
 
     import torch
-    src = os.path.join(CSRC, "cache_binding.cpp")
-    stamp = os.path.join(BUILD_DIR, "_cache_binding.stamp")
+    path = BINDING_PATH if name == "cache_binding" else BLOCK_BINDING_PATH
+    src = os.path.join(CSRC, name + ".cpp")
+    stamp = os.path.join(BUILD_DIR, "_%s.stamp" % name)
     made_for = "torch %s, %s\n" % (torch.__version__, sys.implementation.cache_tag)
-    if not force and not _stale(BINDING_PATH, [src, *_headers()]) and os.path.exists(stamp):
+    if not force and not _stale(path, [src, *_headers()]) and os.path.exists(stamp):
         with open(stamp) as f:
             if f.read() == made_for:
                 return
     root = os.path.dirname(torch.__file__)
     cuda = os.path.dirname(os.path.dirname(os.path.realpath(_nvcc())))
-    include = [INCLUDE, os.path.join(root, "include"),
+    include = [INCLUDE, CSRC, os.path.join(root, "include"),
                os.path.join(root, "include", "torch", "csrc", "api", "include"),
                sysconfig.get_paths()["include"], os.path.join(cuda, "include")]
     cmd = [os.environ.get("CXX") or "g++", "-std=c++17", "-O2", "-fPIC", "-shared", "-w",
            "-D_GLIBCXX_USE_CXX11_ABI=%d" % torch._C._GLIBCXX_USE_CXX11_ABI,
-           *["-I" + d for d in include], src, "-o", BINDING_PATH, "-L" + PKG_DIR,
+           *["-I" + d for d in include], src, "-o", path, "-L" + PKG_DIR,
            "-l:libvggt_sparse.so", "-Wl,-rpath,$ORIGIN", "-L" + os.path.join(root, "lib"), "-lc10",
            "-lc10_cuda", "-ltorch_cpu", "-ltorch_python"]
     res = subprocess.run(cmd, capture_output=True, text=True)
@@ -113,7 +115,8 @@ def build(force=False, verbose=False, ptxas_info=False):
         res = subprocess.run(cmd, capture_output=True, text=True)
         if res.returncode != 0:
             raise RuntimeError("link failed:\n%s\n%s" % (res.stdout, res.stderr))
-    _build_binding(force)
+    with cf.ThreadPoolExecutor() as ex:
+        list(ex.map(lambda name: _build_binding(force, name), ("cache_binding", "block_binding")))
     if verbose:
         for log in logs:
             sys.stderr.write(log)
