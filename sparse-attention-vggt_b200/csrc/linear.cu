@@ -100,6 +100,26 @@ struct Walk {
   }
 };
 
+// tc05.cuh's bounded wait with the clock read late and seldom: the waits here are mostly shorter
+// than reading the clock takes, and the time from a block's release to its refill counts.
+__device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity, volatile int* abort_flag,
+                                     uint64_t limit_ns) {
+  uint64_t t0 = 0;
+  for (uint32_t spin = 1;; ++spin) {
+    if (tc::mbar_try_wait(bar, parity)) return true;
+    if ((spin & 63u) == 0u) {
+      if (*abort_flag) return false;
+      const uint64_t now = tc::globaltimer_ns();
+      if (t0 == 0) {
+        t0 = now;
+      } else if (now - t0 > limit_ns) {
+        *abort_flag = 1;
+        return false;
+      }
+    }
+  }
+}
+
 // ---- what pairs of CTAs need beside tc05.cuh -------------------------------------------------
 __device__ __forceinline__ uint32_t cluster_rank() {
   uint32_t r;
@@ -254,6 +274,34 @@ __device__ __forceinline__ void copy_rows(uint32_t buf, int row0, E* g, int64_t 
   }
 }
 
+// The stage that comes next and the parity of its round.
+struct Ring {
+  uint32_t at = 0, turn = 0;
+  __device__ __forceinline__ void step() {
+    if (++at == STAGES) {
+      at = 0;
+      turn ^= 1;
+    }
+  }
+};
+
+// The c-th 64 elements of a row whose heads hold `per` of them.
+struct Place {
+  int x = 0, head = 0;
+  Place() = default;
+  __device__ __forceinline__ Place(int c, int per) {
+    head = c / per;
+    x = (c - head * per) * 64;
+  }
+  __device__ __forceinline__ void step(int per) {
+    x += 64;
+    if (per != INT_MAX && x == per * 64) {
+      x = 0;
+      ++head;
+    }
+  }
+};
+
 // What one use of an epilogue buffer holds.
 enum { kUseZ, kUseY, kUseSlot };
 
@@ -301,54 +349,63 @@ __global__ void __launch_bounds__(THREADS, 1)
   if (warp == 0) {
     // ================= TMA producer =================
     if (lane == 0) {
+      const uint32_t full0 = CTA == 2 ? map_rank(bar(B_FULL), 0) : bar(B_FULL);
       tc::prefetch_tmap(&tm_a);
       tc::prefetch_tmap(&tm_b);
       Walk w(p, worker);
-      uint32_t it = 0;
+      Ring ring;
+      uint32_t issued = 0;
       bool ok = true;
       while (ok && w.next()) {
         const int m0 = (int)(w.tile / p.tiles_n) * BN + rank * BM;
         const int n0 = (int)(w.tile % p.tiles_n) * BN + rank * BM;
-        for (int k = w.k0; k < w.k1; ++k, ++it) {
-          const uint32_t s = it % STAGES;
-          if (it >= STAGES && !tc::mbar_wait(bar(B_EMPTY + s), (it / STAGES - 1) & 1, abort_flag,
-                                             p.wait_ns)) {
+        // where the operands' first blocks lie: one thread feeds the tensor core here, so that
+        // no division is left in the loop
+        Place a0, a1, b0, b1;
+        if (AMN) {
+          a0 = Place(m0 / 64, p.a_heads64);
+          a1 = Place(m0 / 64 + 1, p.a_heads64);
+        } else {
+          a0 = Place(w.k0, p.a_heads64);
+        }
+        if (BMN) {
+          b0 = Place(n0 / 64, p.b_heads64);
+          b1 = Place(n0 / 64 + 1, p.b_heads64);
+        } else {
+          b0 = Place(w.k0, p.b_heads64);
+        }
+        for (int k = w.k0; k < w.k1; ++k) {
+          if (issued >= STAGES &&
+              !wait(bar(B_EMPTY) + 8 * ring.at, ring.turn ^ 1, abort_flag, p.wait_ns)) {
             ok = false;
             break;
           }
           // the barrier is the first CTA's: it counts both CTAs' bytes
-          uint32_t full = bar(B_FULL + s);
-          if (CTA == 2) full = map_rank(full, 0);
-          if (rank == 0) tc::mbar_expect_tx(bar(B_FULL + s), CTA * STAGE_BYTES);
-          const uint32_t a = base + s * STAGE_BYTES, b = a + HALF_BYTES;
+          const uint32_t full = full0 + 8 * ring.at;
+          if (rank == 0) tc::mbar_expect_tx(bar(B_FULL) + 8 * ring.at, CTA * STAGE_BYTES);
+          const uint32_t a = base + ring.at * STAGE_BYTES, b = a + HALF_BYTES;
           if (AMN) {
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-              const int c = m0 / 64 + j, head = c / p.a_heads64;
-              Pair<CTA>::load(a + j * (HALF_BYTES / 2), &tm_a, full, (c - head * p.a_heads64) * 64,
-                              k * BK, head);
-            }
+            Pair<CTA>::load(a, &tm_a, full, a0.x, k * BK, a0.head);
+            Pair<CTA>::load(a + HALF_BYTES / 2, &tm_a, full, a1.x, k * BK, a1.head);
           } else {
-            const int head = k / p.a_heads64;
-            Pair<CTA>::load(a, &tm_a, full, (k - head * p.a_heads64) * BK, m0, head);
+            Pair<CTA>::load(a, &tm_a, full, a0.x, m0, a0.head);
+            a0.step(p.a_heads64);
           }
           if (BMN) {
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-              const int c = n0 / 64 + j, head = c / p.b_heads64;
-              Pair<CTA>::load(b + j * (HALF_BYTES / 2), &tm_b, full, (c - head * p.b_heads64) * 64,
-                              k * BK, head);
-            }
+            Pair<CTA>::load(b, &tm_b, full, b0.x, k * BK, b0.head);
+            Pair<CTA>::load(b + HALF_BYTES / 2, &tm_b, full, b1.x, k * BK, b1.head);
           } else {
-            const int head = k / p.b_heads64;
-            Pair<CTA>::load(b, &tm_b, full, (k - head * p.b_heads64) * BK, n0, head);
+            Pair<CTA>::load(b, &tm_b, full, b0.x, n0, b0.head);
+            b0.step(p.b_heads64);
           }
+          ring.step();
+          ++issued;
         }
       }
       // the last copies have landed before the memory goes (the MMAs that read them are awaited
       // by their issuer)
       if (rank == 0)
-        for (uint32_t t = it > STAGES ? it - STAGES : 0; t < it; ++t)
+        for (uint32_t t = issued > STAGES ? issued - STAGES : 0; t < issued; ++t)
           tc::mbar_wait_drain(bar(B_FULL + t % STAGES), (t / STAGES) & 1, p.wait_ns);
     }
   } else if (warp == 1) {
@@ -358,34 +415,34 @@ __global__ void __launch_bounds__(THREADS, 1)
       const uint32_t idesc = tc::idesc_f16(fmt, BMN ? 1u : 0u, BN, BN) | (AMN ? 1u << 15 : 0u);
       // a step of 16 reduced elements: 32 bytes along a K-major row, 16 MN-major rows
       constexpr uint64_t kStepA = AMN ? 16 * 128 / 16 : 2, kStepB = BMN ? 16 * 128 / 16 : 2;
+      const uint64_t desc0 = tc::sw128_desc(base, HALF_BYTES / 2);
       bool ok = true;
-      if (p.wait_selftest) ok = tc::mbar_wait(bar(B_DRAIN), 0, abort_flag, p.wait_ns);
+      if (p.wait_selftest) ok = wait(bar(B_DRAIN), 0, abort_flag, p.wait_ns);
       Walk w(p, worker);
-      uint32_t it = 0, i = 0;
+      Ring ring;
+      uint32_t i = 0;
       while (ok && w.next()) {
         const uint32_t b = i & 1;
         if (i >= 2 &&
-            !tc::mbar_wait(bar(B_ACCEMPTY + b), ((i >> 1) + 1) & 1, abort_flag, p.wait_ns)) {
+            !wait(bar(B_ACCEMPTY + b), ((i >> 1) + 1) & 1, abort_flag, p.wait_ns)) {
           ok = false;
           break;
         }
         tc::tc_fence_after();
         const uint32_t acc = tmem + b * BN;
-        for (int k = w.k0; k < w.k1; ++k, ++it) {
-          const uint32_t s = it % STAGES;
-          if (!tc::mbar_wait(bar(B_FULL + s), (it / STAGES) & 1, abort_flag, p.wait_ns)) {
+        for (int k = w.k0; k < w.k1; ++k) {
+          if (!wait(bar(B_FULL) + 8 * ring.at, ring.turn, abort_flag, p.wait_ns)) {
             ok = false;
             break;
           }
           tc::tc_fence_after();
-          const uint32_t a = base + s * STAGE_BYTES;
-          const uint64_t ad = tc::sw128_desc(a, HALF_BYTES / 2),
-                         bd = tc::sw128_desc(a + HALF_BYTES, HALF_BYTES / 2);
+          const uint64_t ad = desc0 + ring.at * (STAGE_BYTES / 16), bd = ad + HALF_BYTES / 16;
 #pragma unroll
           for (int kk = 0; kk < BK / 16; ++kk)
             Pair<CTA>::mma(acc, ad + kk * kStepA, bd + kk * kStepB, idesc,
                            (k > w.k0 || kk > 0) ? 1u : 0u);
-          Pair<CTA>::commit(bar(B_EMPTY + s));
+          Pair<CTA>::commit(bar(B_EMPTY) + 8 * ring.at);
+          ring.step();
         }
         if (ok) Pair<CTA>::commit(bar(B_ACCFULL + b));
         ++i;
@@ -420,7 +477,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     while (ok && w.next()) {
       const uint32_t b = i & 1;
       const int64_t m0 = w.tile / p.tiles_n * BN + rank * BM, n0 = w.tile % p.tiles_n * BN;
-      const bool got = tc::warp_wait(bar(B_ACCFULL + b), (i >> 1) & 1, abort_flag, p.wait_ns);
+      const bool got = wait(bar(B_ACCFULL + b), (i >> 1) & 1, abort_flag, p.wait_ns);
       if (!agree(const_cast<int*>(votes) + 4 * b, got)) {
         ok = false;
         break;
@@ -457,7 +514,7 @@ __global__ void __launch_bounds__(THREADS, 1)
                 tc::tma_load_3d(buf, &tm_res, bar(B_RES + 2 * g + u), (int)c0, (int)m0, 0);
               }
               __syncwarp();
-              fine = tc::warp_wait(bar(B_RES + 2 * g + u), res_uses[u] & 1, abort_flag, p.wait_ns);
+              fine = wait(bar(B_RES + 2 * g + u), res_uses[u] & 1, abort_flag, p.wait_ns);
               ++res_uses[u];
             }
             if (!agree(const_cast<int*>(votes) + 8 + 4 * u, fine)) {
@@ -667,18 +724,35 @@ static int sm_count() {
   return device_sms(&sms) == cudaSuccess && sms > 0 ? sms : 148;
 }
 
+// The way a product is cut is the one of the least estimated time, in SM cycles: a reduction block
+// takes a pair of CTAs 512 cycles (the MMAs' time) and a single CTA 256, or up to twice that when
+// all SMs read their operands from L2 at once.  Splitting evens the load out where tiles are few
+// or the last round is short, at the price of partial sums through memory and another launch.
 Plan plan_product(int64_t m, int64_t n, int64_t red, bool must_split) {
   const int sms = sm_count();
-  Plan p;
-  p.cta = 1;
-  p.split = must_split ? 1 : 0;
-  p.workers = sms / p.cta;
-  p.tiles_m = (m + 128 * p.cta - 1) / (128 * p.cta);
-  p.tiles_n = (n + 128 * p.cta - 1) / (128 * p.cta);
-  p.blocks = (red + BK - 1) / BK;
-  const int64_t work = p.tiles_m * p.tiles_n * (p.split ? p.blocks : 1);
-  if (p.workers > work) p.workers = (int)work;
-  return p;
+  Plan best;
+  double least = 0;
+  for (int cta = 1; cta <= 2; ++cta)
+    for (int split = must_split ? 1 : 0; split < 2; ++split) {
+      Plan p;
+      p.cta = cta;
+      p.split = split;
+      p.tiles_m = (m + 128 * cta - 1) / (128 * cta);
+      p.tiles_n = (n + 128 * cta - 1) / (128 * cta);
+      p.blocks = (red + BK - 1) / BK;
+      const int64_t tiles = p.tiles_m * p.tiles_n, units = split ? tiles * p.blocks : tiles;
+      p.workers = (int)std::min<int64_t>(sms / cta, units);
+      const double busy = (double)p.workers * cta / sms;
+      const double block = cta == 2 ? 512 : 256 * std::max(1.0, 2 * busy);
+      const int64_t rounds = (units + p.workers - 1) / p.workers;
+      double t = (double)rounds * (split ? 1 : p.blocks) * block;
+      if (split) t += 5000 + (double)p.slot_bytes() * 2 / 2500;
+      if (least == 0 || t < least) {
+        least = t;
+        best = p;
+      }
+    }
+  return best;
 }
 
 static bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
@@ -783,9 +857,12 @@ cudaError_t launch_product(const Plan& plan, int dtype, int64_t m, int64_t n, in
   p.status = status;
   p.wait_ns = api_wait_ns();
   p.wait_selftest = api_wait_selftest();
+  const bool am = a.mn_major, bm = b.mn_major;
   if (dtype == VGGT_DTYPE_BF16)
-    return launch_majors<__nv_bfloat16, 1>(a.mn_major, b.mn_major, plan.split, maps, p, stream);
-  return launch_majors<__half, 1>(a.mn_major, b.mn_major, plan.split, maps, p, stream);
+    return plan.cta == 2 ? launch_majors<__nv_bfloat16, 2>(am, bm, plan.split, maps, p, stream)
+                         : launch_majors<__nv_bfloat16, 1>(am, bm, plan.split, maps, p, stream);
+  return plan.cta == 2 ? launch_majors<__half, 2>(am, bm, plan.split, maps, p, stream)
+                       : launch_majors<__half, 1>(am, bm, plan.split, maps, p, stream);
 }
 
 Slots slots_of(const Plan& plan, const float* p) {
