@@ -17,104 +17,130 @@ struct Fwd {
   int64_t h_stride, y_stride;
 };
 
-template <typename S, typename T, int WPR, int J>
-__global__ void __launch_bounds__(WPR > 8 ? WPR * 32 : 256) forward_kernel(const Fwd f) {
+template <typename S, typename T, int WPR, int J, bool ONE>
+__global__ void __launch_bounds__(kMaxThreads, 1) forward_kernel(const Fwd f) {
+  constexpr int kX = sizeof(S) / 2, kF = sizeof(T) / 2;  // 16-byte units of 8 elements
+  constexpr int kUnits = J * (kX + kF);
+  typedef Shared<WPR, J, kUnits, ONE> SH;
+  extern __shared__ __align__(16) unsigned char smem[];
   __shared__ float scratch[2 * 2 * 32];
   const Args& a = f.a;
   RowSum<WPR> sum(scratch);
+  const Pipe<kUnits> pipe(smem);
   const int lane = threadIdx.x & 31, slots = (blockDim.x >> 5) / WPR;
   const float inv_width = 1.f / (float)a.width;
-  const bool vec = a.vec;
+  const bool vec = a.vec, branch = a.branch != nullptr;
   int n[J];
 #pragma unroll
   for (int j = 0; j < J; ++j)
     n[j] = max(0, min(8, (int)a.width - 8 * ((j * WPR + sum.warp) * 32 + lane)));
   const int first = 8 * (sum.warp * 32 + lane);
   constexpr int step = 8 * WPR * 32;
-  for (int64_t row = (int64_t)blockIdx.x * slots + sum.slot; row < a.rows;
-       row += (int64_t)gridDim.x * slots) {
-    float v[J][8];
-    const S* x = static_cast<const S*>(a.x) + row * a.x_stride + first;
+  // a run of rows to a slot: gates change seldom
+  const int64_t slot = (int64_t)blockIdx.x * slots + sum.slot, all = (int64_t)gridDim.x * slots;
+  int64_t row = ONE ? slot : slot * a.rows / all;
+  const int64_t end = ONE ? min(slot + 1, a.rows) : (slot + 1) * a.rows / all;
+  const S* const x0 = static_cast<const S*>(a.x) + first;
+  const T* const b0 = static_cast<const T*>(a.branch) + first;
+  auto fetch = [&](int64_t r, int stage) {
+    if (vec && r < end) {
 #pragma unroll
-    for (int j = 0; j < J; ++j) get8(x + j * step, n[j], vec, v[j]);
-    if (a.branch != nullptr) {
-      float p[J][8];
-      const T* b = static_cast<const T*>(a.branch) + row * a.branch_stride + first;
+      for (int j = 0; j < J; ++j)
+        if (n[j] > 0) {
+          pipe.fetch(stage, j * (kX + kF), x0 + r * a.x_stride + j * step);
+          if (branch) pipe.fetch(stage, j * (kX + kF) + kX, b0 + r * a.branch_stride + j * step);
+        }
+    }
+    cp_async_commit();
+  };
+  if (SH::kRows) fetch(row, 0);
+  const bool gates = a.gate.p != nullptr && a.rows_per_gate > 0;
+  int64_t gate_row = gates ? min(row, a.rows - 1) / a.rows_per_gate : 0;
+  int64_t gate_end = gates ? (gate_row + 1) * a.rows_per_gate : a.rows;
+  Params<WPR, J, SH, ONE> params(a, smem + SH::kAfterRows, first, n, gate_row);
+  if (SH::kParams) __syncthreads();
+  for (int stage = 0; row < end; ++row, stage ^= 1) {
+    if (SH::kRows) {
+      fetch(row + 1, stage ^ 1);
+      cp_async_wait<1>();
+    }
+    float_pair v[J][4], p[J][4];
 #pragma unroll
-      for (int j = 0; j < J; ++j) get8(b + j * step, n[j], vec, p[j]);
+    for (int j = 0; j < J; ++j) {
+      if (!SH::kRows || !vec) {
+        get_pairs(x0 + row * a.x_stride + j * step, n[j], vec, v[j]);
+        if (branch) get_pairs(b0 + row * a.branch_stride + j * step, n[j], vec, p[j]);
+      } else if (n[j] > 0) {
+        pipe.template read<S>(stage, j * (kX + kF), v[j]);
+        if (branch) pipe.template read<T>(stage, j * (kX + kF) + kX, p[j]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[j][i] = p[j][i] = both(0.f);
+      }
+    }
+    if (branch) {
       if (a.post != 0) {
         norm_row<WPR, J>(p, n, a.post, inv_width, a.eps, sum);
-        if (a.post_weight.p != nullptr)
 #pragma unroll
-          for (int j = 0; j < J; ++j) {
-            float w[8];
-            get_param8(a.post_weight, first + j * step, n[j], vec, w);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) p[j][i] *= w[i];
-          }
-        if (a.post_bias.p != nullptr)
-#pragma unroll
-          for (int j = 0; j < J; ++j) {
-            float w[8];
-            get_param8(a.post_bias, first + j * step, n[j], vec, w);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) p[j][i] += w[i];
-          }
+        for (int j = 0; j < J; ++j) {
+          params.scale(kPostWeight, j, p[j]);
+          params.shift(kPostBias, j, p[j]);
+        }
       }
-      const int64_t at = a.rows_per_gate > 0 ? row / a.rows_per_gate * a.width : 0;
+      if (gates && row == gate_end) {
+        gate_end += a.rows_per_gate;
+        params.turn_to(++gate_row);
+      }
       S* h = static_cast<S*>(f.h) + row * f.h_stride + first;
 #pragma unroll
       for (int j = 0; j < J; ++j) {
-        if (a.gate.p != nullptr) {
-          float g[8];
-          get_param8(a.gate, at + first + j * step, n[j], vec, g);
-#pragma unroll
-          for (int i = 0; i < 8; ++i) v[j][i] = fmaf(g[i], p[j][i], v[j][i]);
-        } else {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) v[j][i] += p[j][i];
-        }
-        put8(h + j * step, n[j], vec, v[j]);
+        params.gated(j, p[j], v[j]);
+        put_pairs(h + j * step, n[j], vec, v[j]);
       }
     }
     norm_row<WPR, J>(v, n, a.norm, inv_width, a.eps, sum);
     T* y = static_cast<T*>(f.y) + row * f.y_stride + first;
 #pragma unroll
     for (int j = 0; j < J; ++j) {
-      if (a.weight.p != nullptr) {
-        float w[8];
-        get_param8(a.weight, first + j * step, n[j], vec, w);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[j][i] *= w[i];
-      }
-      if (a.bias.p != nullptr) {
-        float w[8];
-        get_param8(a.bias, first + j * step, n[j], vec, w);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[j][i] += w[i];
-      }
-      put8(y + j * step, n[j], vec, v[j]);
+      params.scale(kWeight, j, v[j]);
+      params.shift(kBias, j, v[j]);
+      put_pairs(y + j * step, n[j], vec, v[j]);
     }
   }
 }
 
-template <typename S, typename T, int WPR, int J>
-cudaError_t launch_shape(const Fwd& f, int sms, cudaStream_t stream) {
-  const int threads = WPR > 8 ? WPR * 32 : 256, slots = threads / 32 / WPR;
-  const int64_t blocks = std::min<int64_t>((f.a.rows + slots - 1) / slots, (int64_t)sms * 32);
-  forward_kernel<S, T, WPR, J><<<(unsigned)blocks, threads, 0, stream>>>(f);
+template <typename S, typename T, int WPR, int J, bool ONE>
+cudaError_t launch_shape(const Fwd& f, int64_t blocks, int slots, cudaStream_t stream) {
+  constexpr uint32_t bytes =
+      Shared<WPR, J, J*(sizeof(S) / 2 + sizeof(T) / 2), ONE>::kBytes;
+  auto k = forward_kernel<S, T, WPR, J, ONE>;
+  if (cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes))
+    return e;
+  k<<<(unsigned)blocks, slots * WPR * 32, bytes, stream>>>(f);
   return cudaGetLastError();
+}
+
+template <typename S, typename T, int WPR, int J>
+cudaError_t launch_rows(const Fwd& f, int sms, cudaStream_t stream) {
+  constexpr int most = kMaxThreads / 32 / WPR;
+  // few rows: spread over the SMs, each with a slot of its own
+  if (f.a.rows <= (int64_t)sms * most) {
+    const int slots = (int)((f.a.rows + sms - 1) / sms);
+    return launch_shape<S, T, WPR, J, true>(f, (f.a.rows + slots - 1) / slots, slots, stream);
+  }
+  return launch_shape<S, T, WPR, J, false>(f, sms, most, stream);
 }
 
 template <typename S, typename T>
 cudaError_t launch_types(const Fwd& f, int sms, cudaStream_t stream) {
   const int64_t w = f.a.width;
-  if (w <= 256) return launch_shape<S, T, 1, 1>(f, sms, stream);
-  if (w <= 1024) return launch_shape<S, T, 1, 4>(f, sms, stream);
-  if (w <= 2048) return launch_shape<S, T, 2, 4>(f, sms, stream);
-  if (w <= 4096) return launch_shape<S, T, 4, 4>(f, sms, stream);
-  if (w <= 8192) return launch_shape<S, T, 8, 4>(f, sms, stream);
-  return launch_shape<S, T, 16, 4>(f, sms, stream);
+  if (w <= 256) return launch_rows<S, T, 1, 1>(f, sms, stream);
+  if (w <= 512) return launch_rows<S, T, 1, 2>(f, sms, stream);
+  if (w <= 1024) return launch_rows<S, T, 2, 2>(f, sms, stream);
+  if (w <= 2048) return launch_rows<S, T, 4, 2>(f, sms, stream);
+  if (w <= 4096) return launch_rows<S, T, 8, 2>(f, sms, stream);
+  if (w <= 8192) return launch_rows<S, T, 16, 2>(f, sms, stream);
+  return launch_rows<S, T, 16, 4>(f, sms, stream);
 }
 
 }  // namespace rnorm

@@ -4,12 +4,20 @@
 //   h = x + gate * p             gate: per channel, or per channel and run of rows
 //   y = norm(h) * weight + bias  norm: (h - mean) / sqrt(var + eps), or h / sqrt(mean h^2 + eps)
 //
-// A row is held in registers by WPR warps, 8 * J elements a lane, in chunks of 8 that are 16-byte
-// loads where the layout allows (`vec`): chunk j of lane l of the row's warp w starts at column
-// 8 * ((j * WPR + w) * 32 + l).  All arithmetic is in fp32; means are formed first and variances
-// from what is left after them, so that a row far from zero loses nothing.
+// A row is held in registers by WPR warps, 8 * J elements a lane, in chunks of 8: chunk j of lane
+// l of the row's warp w starts at column 8 * ((j * WPR + w) * 32 + l).  A block has up to 16 warps,
+// one block to an SM, and each of its groups of WPR warps (a slot) works through rows of its own.
+// While it works on one row, its threads copy their chunks of the next one into shared memory
+// (cp.async, where the layout allows 16-byte accesses: `vec`), and the parameters lie there too, in
+// fp32, read once per block: what a thread needs of either is its own, so that no barrier is
+// needed.  (Read from global memory where they are used, the parameters' latencies took half the
+// time: 32 frames of width 1024, fp32 stream, 159 us.)  With few rows, one to a slot (ONE),
+// everything is read into registers at once.  All arithmetic is in fp32, in packed pairs; means
+// are formed first and variances from what is left after them, so that a row far from zero loses
+// nothing.
 #pragma once
 
+#include "exp2.cuh"
 #include "vec8.cuh"
 
 namespace vggt {
@@ -23,14 +31,209 @@ struct Param {
   int type = VGGT_DTYPE_FP32;
 };
 
-__device__ __forceinline__ void get_param8(const Param& q, int64_t at, int n, bool vec,
-                                           float* v) {
+__device__ __forceinline__ float_pair both(float a) { return pack_pair(a, a); }
+__device__ __forceinline__ float sum_pair(float_pair v) {
+  float a, b;
+  unpack_pair(a, b, v);
+  return a + b;
+}
+
+// Eight elements as pairs, of which the first `n` exist (the rest are zero).
+template <typename E>
+__device__ __forceinline__ void get_pairs(const E* p, int n, bool vec, float_pair* v) {
+  float f[8];
+  get8(p, n, vec, f);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = pack_pair(f[2 * i], f[2 * i + 1]);
+}
+template <typename E>
+__device__ __forceinline__ void put_pairs(E* p, int n, bool vec, const float_pair* v) {
+  float f[8];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) unpack_pair(f[2 * i], f[2 * i + 1], v[i]);
+  put8(p, n, vec, f);
+}
+__device__ __forceinline__ void get_param(const Param& q, int64_t at, int n, bool vec,
+                                          float_pair* v) {
   if (q.type == VGGT_DTYPE_FP32)
-    get8(static_cast<const float*>(q.p) + at, n, vec, v);
+    get_pairs(static_cast<const float*>(q.p) + at, n, vec, v);
   else if (q.type == VGGT_DTYPE_BF16)
-    get8(static_cast<const __nv_bfloat16*>(q.p) + at, n, vec, v);
+    get_pairs(static_cast<const __nv_bfloat16*>(q.p) + at, n, vec, v);
   else
-    get8(static_cast<const __half*>(q.p) + at, n, vec, v);
+    get_pairs(static_cast<const __half*>(q.p) + at, n, vec, v);
+}
+
+// A call's tensors (vggt_block.h).
+struct Args {
+  const void* x;
+  const void* branch;
+  Param gate, weight, bias, post_weight, post_bias;
+  int64_t rows, width, x_stride, branch_stride, rows_per_gate;
+  int stream_type, type;  // of x and h, and of branch and y
+  int norm, post;         // VGGT_NORM_*
+  float eps;
+  bool vec;
+};
+
+constexpr int kMaxThreads = 512, kStages = 2;
+constexpr uint32_t kSharedBytes = 208 * 1024;
+
+enum { kWeight, kBias, kGate, kPostWeight, kPostBias, kArrays };
+
+// Shared memory of a block: rows to come (UNITS 16-byte units a thread and stage), parameters
+// (all slots' the same), and the slot's gate where it is one of several.  What does not fit is read
+// where it is used.
+template <int WPR, int J, int UNITS, bool ONE>
+struct Shared {
+  static constexpr uint32_t kRowBytes = kMaxThreads * kStages * UNITS * 16;
+  static constexpr uint32_t kParamBytes = WPR * 32 * J * 32, kGateBytes = kMaxThreads * J * 32;
+  static constexpr bool kRows = !ONE && kRowBytes <= kSharedBytes;
+  static constexpr uint32_t kAfterRows = kRows ? kRowBytes : 0;
+  // four parameters and the gate
+  static constexpr bool kParams =
+      !ONE && kAfterRows + 4 * kParamBytes + kGateBytes <= kSharedBytes;
+  static constexpr uint32_t kBytes = kAfterRows + (kParams ? 4 * kParamBytes + kGateBytes : 0);
+};
+
+// The parameters as one thread sees them.
+template <int WPR, int J, typename SH, bool ONE>
+struct Params {
+  const Args& a;
+  unsigned char* at;  // this thread's place among the parameters
+  int first;
+  const int* n;
+  int64_t gate_row = 0;
+  float_pair reg[ONE ? kArrays : 1][ONE ? J : 1][4];
+
+  static constexpr int kStep = 8 * WPR * 32;
+  __device__ __forceinline__ const Param& param(int k) const {
+    return k == kWeight  ? a.weight
+           : k == kBias  ? a.bias
+           : k == kGate  ? a.gate
+           : k == kPostWeight ? a.post_weight : a.post_bias;
+  }
+  // place of chunk j's half u of parameter k: the gate has a place per thread
+  __device__ __forceinline__ unsigned char* place(int k, int j, int u) const {
+    if (k == kGate)
+      return at + 4 * SH::kParamBytes + ((j * 2 + u) * kMaxThreads + threadIdx.x) * 16;
+    const int slot = k < kGate ? k : k - 1;
+    return at + slot * SH::kParamBytes +
+           ((j * 2 + u) * (WPR * 32) + (int)threadIdx.x % (WPR * 32)) * 16;
+  }
+  __device__ __forceinline__ void fill(int k) {
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+      float_pair v[4];
+      get_param(param(k), (k == kGate ? gate_row * a.width : 0) + first + j * kStep, n[j], a.vec, v);
+      *reinterpret_cast<ulonglong2*>(place(k, j, 0)) = make_ulonglong2(v[0], v[1]);
+      *reinterpret_cast<ulonglong2*>(place(k, j, 1)) = make_ulonglong2(v[2], v[3]);
+    }
+  }
+  // ONE: reads all that the call uses; else fills the shared places (a barrier has to follow)
+  __device__ __forceinline__ Params(const Args& args, unsigned char* smem, int first_, const int* n_,
+                                    int64_t gate_row_)
+      : a(args), at(smem), first(first_), n(n_), gate_row(gate_row_) {
+    if (ONE) {
+#pragma unroll
+      for (int k = 0; k < kArrays; ++k)
+        if (param(k).p != nullptr)
+#pragma unroll
+          for (int j = 0; j < J; ++j)
+            get_param(param(k), (k == kGate ? gate_row * a.width : 0) + first + j * kStep, n[j],
+                      a.vec, reg[ONE ? k : 0][ONE ? j : 0]);
+    } else if (SH::kParams) {
+#pragma unroll
+      for (int k = 0; k < kArrays; ++k)
+        if (param(k).p != nullptr && (k == kGate || threadIdx.x < WPR * 32)) fill(k);
+    }
+  }
+  // the gate of another run of rows
+  __device__ __forceinline__ void turn_to(int64_t row) {
+    if (row == gate_row) return;
+    gate_row = row;
+    if (!ONE && SH::kParams) fill(kGate);
+  }
+  __device__ __forceinline__ void get(int k, int j, float_pair* v) const {
+    if (ONE) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = reg[ONE ? k : 0][ONE ? j : 0][i];
+    } else if (SH::kParams) {
+      const ulonglong2 lo = *reinterpret_cast<const ulonglong2*>(place(k, j, 0));
+      const ulonglong2 hi = *reinterpret_cast<const ulonglong2*>(place(k, j, 1));
+      v[0] = lo.x, v[1] = lo.y, v[2] = hi.x, v[3] = hi.y;
+    } else {
+      get_param(param(k), (k == kGate ? gate_row * a.width : 0) + first + j * kStep, n[j], a.vec, v);
+    }
+  }
+  __device__ __forceinline__ void scale(int k, int j, float_pair* v) const {
+    if (param(k).p == nullptr) return;
+    float_pair w[4];
+    get(k, j, w);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = mul_pair(v[i], w[i]);
+  }
+  __device__ __forceinline__ void shift(int k, int j, float_pair* v) const {
+    if (param(k).p == nullptr) return;
+    float_pair w[4];
+    get(k, j, w);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = add_pair(v[i], w[i]);
+  }
+  // h += gate * p
+  __device__ __forceinline__ void gated(int j, const float_pair* p, float_pair* h) const {
+    if (a.gate.p != nullptr) {
+      float_pair w[4];
+      get(kGate, j, w);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) h[i] = fma_pair(w[i], p[i], h[i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) h[i] = add_pair(h[i], p[i]);
+    }
+  }
+};
+
+// A thread's chunks of the rows to come: stage, then 16-byte unit, then thread, so that a warp's
+// accesses lie side by side.
+template <int UNITS>
+struct Pipe {
+  unsigned char* mine;
+  uint32_t mine_u32;
+  __device__ __forceinline__ explicit Pipe(unsigned char* smem) : mine(smem + threadIdx.x * 16) {
+    mine_u32 = smem_u32(mine);
+  }
+  // chunk `unit0` on of an 8-element group of E
+  template <typename E>
+  __device__ __forceinline__ void fetch(int stage, int unit0, const E* p) const {
+#pragma unroll
+    for (int u = 0; u < (int)sizeof(E) / 2; ++u)
+      cp_async_16(mine_u32 + (stage * UNITS + unit0 + u) * (kMaxThreads * 16),
+                  reinterpret_cast<const unsigned char*>(p) + 16 * u, 16);
+  }
+  template <typename E>
+  __device__ __forceinline__ void read(int stage, int unit0, float_pair* v) const {
+    const unsigned char* p = mine + (stage * UNITS + unit0) * (kMaxThreads * 16);
+    if (sizeof(E) == 4) {
+      const ulonglong2 lo = *reinterpret_cast<const ulonglong2*>(p);
+      const ulonglong2 hi = *reinterpret_cast<const ulonglong2*>(p + kMaxThreads * 16);
+      v[0] = lo.x, v[1] = lo.y, v[2] = hi.x, v[3] = hi.y;
+    } else {
+      get_pairs(reinterpret_cast<const E*>(p), 8, true, v);
+    }
+  }
+};
+
+// v - c in the first n of 8 elements, the others (zeros) left as they are.
+__device__ __forceinline__ void subtract(float_pair* v, int n, float c) {
+  if (n == 8) {
+    const float_pair m = both(-c);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = add_pair(v[i], m);
+  } else if (n > 0) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      v[i] = add_pair(v[i], pack_pair(2 * i < n ? -c : 0.f, 2 * i + 1 < n ? -c : 0.f));
+  }
 }
 
 // Sums over the row's WPR warps; every thread gets them, added in the same order.  `scratch`
@@ -73,47 +276,43 @@ struct RowSum {
 
 // v normed in place (elements past the row's end stay zero); returns 1 / deviation.
 template <int WPR, int J>
-__device__ __forceinline__ float norm_row(float (*v)[8], const int* n, int kind, float inv_width,
-                                          float eps, RowSum<WPR>& sum) {
+__device__ __forceinline__ float norm_row(float_pair (*v)[4], const int* n, int kind,
+                                          float inv_width, float eps, RowSum<WPR>& sum) {
   if (kind == kNormLayer) {
-    float s = 0.f;
+    float_pair s = both(0.f);
 #pragma unroll
     for (int j = 0; j < J; ++j)
 #pragma unroll
-      for (int i = 0; i < 8; ++i) s += v[j][i];
-    const float mean = sum.one(s) * inv_width;
+      for (int i = 0; i < 4; ++i) s = add_pair(s, v[j][i]);
+    const float mean = sum.one(sum_pair(s)) * inv_width;
 #pragma unroll
-    for (int j = 0; j < J; ++j)
-#pragma unroll
-      for (int i = 0; i < 8; ++i) v[j][i] = i < n[j] ? v[j][i] - mean : 0.f;
+    for (int j = 0; j < J; ++j) subtract(v[j], n[j], mean);
   }
-  float q = 0.f;
+  float_pair q = both(0.f);
 #pragma unroll
   for (int j = 0; j < J; ++j)
 #pragma unroll
-    for (int i = 0; i < 8; ++i) q = fmaf(v[j][i], v[j][i], q);
-  const float r = 1.f / sqrtf(sum.one(q) * inv_width + eps);
+    for (int i = 0; i < 4; ++i) q = fma_pair(v[j][i], v[j][i], q);
+  const float r = 1.f / sqrtf(sum.one(sum_pair(q)) * inv_width + eps);
+  const float_pair rr = both(r);
 #pragma unroll
   for (int j = 0; j < J; ++j)
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[j][i] *= r;
+    for (int i = 0; i < 4; ++i) v[j][i] = mul_pair(v[j][i], rr);
   return r;
 }
 
-// A call's tensors (vggt_block.h).
-struct Args {
-  const void* x;
-  const void* branch;
-  Param gate, weight, bias, post_weight, post_bias;
-  int64_t rows, width, x_stride, branch_stride, rows_per_gate;
-  int stream_type, type;  // of x and h, and of branch and y
-  int norm, post;         // VGGT_NORM_*
-  float eps;
-  bool vec;
-};
-
 // residual_norm.cu: checks a call's arguments and fills `a`; 0, or the error
 int check(const vggt_residual_norm_args* c, Args* a);
+
+// Warps to a row: 16 elements a lane, or 8 where a backward pass also has the sums of the branch's
+// norm, whose registers take the room; the widest rows have 32 (and spill).
+inline int row_warps(int64_t width, bool half) {
+  const int64_t per_warp = half || width <= 256 ? 256 : 512;
+  int w = 1;
+  while (w < 16 && w * per_warp < width) w *= 2;
+  return w;
+}
 
 }  // namespace rnorm
 }  // namespace vggt

@@ -8,19 +8,18 @@
 // parameters' gradients carry no rounding of a 16-bit h.
 //
 // Bound by memory (x, branch, dy, dh read, dx, dbranch written, once each).  A row lies in the
-// registers of WPR warps (16 elements a lane: the row's values and the parameters' sums, three
-// to five fp32 numbers an element, fit together).  Each group of warps takes a run of rows; its
+// registers of WPR warps, 8 or 16 elements a lane: the row's values and the parameters' sums, three
+// to five fp32 numbers an element, fit together.  Each group of warps takes a run of rows; its
 // parameters' sums are added over the block's groups in shared memory and written as one partial
 // per block, which a second kernel adds in order.  No atomics: equal calls give equal bits.
 #include <algorithm>
+#include <type_traits>
 
 #include "kernels.h"
 #include "residual_norm.cuh"
 
 namespace vggt {
 namespace rnorm {
-
-enum { kWeight, kBias, kGate, kPostWeight, kPostBias, kArrays };
 
 struct Bwd {
   Args a;
@@ -33,7 +32,7 @@ struct Bwd {
   int out_type[kArrays];
   float* part[kArrays];    // [blocks][width] partial sums; of a gate per run of rows
                            // [slots + gates][width]
-  int64_t slots;           // groups of warps that have rows (one at least): group s takes
+  int64_t slots;           // slots that have rows (one at least): slot s takes the rows
                            // [s rows / slots, (s + 1) rows / slots)
 };
 
@@ -47,216 +46,228 @@ __device__ __forceinline__ void put_param8(void* p, int type, int64_t at, int n,
     put8(static_cast<__half*>(p) + at, n, vec, v);
 }
 
-template <int WPR>
-constexpr int bwd_threads() {
-  return WPR > 8 ? WPR * 32 : 256;
-}
-
 // The gradient of what was normed to hat, from that of hat (d, in place).
 template <int WPR, int J>
-__device__ __forceinline__ void norm_back(float (*d)[8], const float (*hat)[8], const int* n,
-                                          int kind, float r, float inv_width, RowSum<WPR>& sum) {
-  float s = 0.f, t = 0.f;
+__device__ __forceinline__ void norm_back(float_pair (*d)[4], const float_pair (*hat)[4],
+                                          const int* n, int kind, float r, float inv_width,
+                                          RowSum<WPR>& sum) {
+  float_pair s2 = both(0.f), t2 = both(0.f);
 #pragma unroll
   for (int j = 0; j < J; ++j)
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      s = fmaf(d[j][i], hat[j][i], s);
-      t += d[j][i];
+    for (int i = 0; i < 4; ++i) {
+      s2 = fma_pair(d[j][i], hat[j][i], s2);
+      t2 = add_pair(t2, d[j][i]);
     }
+  float s = sum_pair(s2), t = sum_pair(t2);
   sum.two(s, t);
-  s *= inv_width;
-  t = kind == kNormLayer ? t * inv_width : 0.f;
+  const float_pair m = both(-s * inv_width), rr = both(r);
+  t *= inv_width;
 #pragma unroll
-  for (int j = 0; j < J; ++j)
+  for (int j = 0; j < J; ++j) {
+    if (kind == kNormLayer) subtract(d[j], n[j], t);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) d[j][i] = i < n[j] ? r * (d[j][i] - t - hat[j][i] * s) : 0.f;
+    for (int i = 0; i < 4; ++i) d[j][i] = mul_pair(rr, fma_pair(hat[j][i], m, d[j][i]));
+  }
 }
 
-template <typename S, typename T, int WPR, int J, bool POST>
-__global__ void __launch_bounds__(bwd_threads<WPR>()) backward_kernel(const Bwd f) {
-  constexpr int kThreads = bwd_threads<WPR>(), kSlots = kThreads / 32 / WPR;
+template <typename S, typename T, int WPR, int J, bool POST, bool ONE>
+__global__ void __launch_bounds__(kMaxThreads, 1) backward_kernel(const Bwd f) {
   constexpr int kAccs = POST ? 5 : 3;
-  constexpr int kRow = WPR * 32 * 8 * J;  // columns that a group of warps holds
+  constexpr int kRow = WPR * 32 * 8 * J;  // columns that a slot holds
+  constexpr int kX = sizeof(S) / 2, kF = sizeof(T) / 2, kUnits = 2 * (kX + kF);
+  typedef Shared<WPR, J, J * kUnits, ONE> SH;
+  extern __shared__ __align__(16) unsigned char smem[];
   __shared__ float scratch[2 * 2 * 32];
-  __shared__ float fold[kSlots > 1 ? kSlots * kRow : 1];
+  float* fold = reinterpret_cast<float*>(smem);  // after the rows
   const Args& a = f.a;
   RowSum<WPR> sum(scratch);
+  const Pipe<J * kUnits> pipe(smem);
+  const int slots = (blockDim.x >> 5) / WPR;
   const int lane = threadIdx.x & 31;
   const float inv_width = 1.f / (float)a.width;
-  const bool vec = a.vec;
+  const bool vec = a.vec, branch = a.branch != nullptr, has_dy = f.dy != nullptr,
+             has_dh = f.dh != nullptr;
   int n[J];
 #pragma unroll
   for (int j = 0; j < J; ++j)
     n[j] = max(0, min(8, (int)a.width - 8 * ((j * WPR + sum.warp) * 32 + lane)));
   const int first = 8 * (sum.warp * 32 + lane);
   constexpr int step = 8 * WPR * 32;
-  const int64_t slot = (int64_t)blockIdx.x * kSlots + sum.slot;
+  const int64_t slot = (int64_t)blockIdx.x * slots + sum.slot;
   const int64_t row0 = slot < f.slots ? slot * a.rows / f.slots : 0;
   const int64_t row1 = slot < f.slots ? (slot + 1) * a.rows / f.slots : 0;
 
-  float acc[kAccs][J][8];
+  float_pair acc[kAccs][J][4];
 #pragma unroll
   for (int k = 0; k < kAccs; ++k)
 #pragma unroll
     for (int j = 0; j < J; ++j)
 #pragma unroll
-      for (int i = 0; i < 8; ++i) acc[k][j][i] = 0.f;
+      for (int i = 0; i < 4; ++i) acc[k][j][i] = both(0.f);
+
+  const S* const x0 = static_cast<const S*>(a.x) + first;
+  const T* const b0 = static_cast<const T*>(a.branch) + first;
+  const T* const dy0 = static_cast<const T*>(f.dy) + first;
+  const S* const dh0 = static_cast<const S*>(f.dh) + first;
+  auto fetch = [&](int64_t row, int stage) {
+    if (vec && row < row1) {
+#pragma unroll
+      for (int j = 0; j < J; ++j)
+        if (n[j] > 0) {
+          pipe.fetch(stage, j * kUnits, x0 + row * a.x_stride + j * step);
+          if (branch) pipe.fetch(stage, j * kUnits + kX, b0 + row * a.branch_stride + j * step);
+          if (has_dy) pipe.fetch(stage, j * kUnits + kX + kF, dy0 + row * f.dy_stride + j * step);
+          if (has_dh)
+            pipe.fetch(stage, j * kUnits + kX + 2 * kF, dh0 + row * f.dh_stride + j * step);
+        }
+    }
+    cp_async_commit();
+  };
+  // chunk j of one of the row's four tensors
+  auto take = [&](auto* p, int stage, int unit, int j, float_pair* v) {
+    typedef std::remove_cv_t<std::remove_pointer_t<decltype(p)>> E;
+    if (!SH::kRows || !vec) {
+      get_pairs(p + j * step, n[j], vec, v);
+    } else if (n[j] > 0) {
+      pipe.template read<E>(stage, j * kUnits + unit, v);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = both(0.f);
+    }
+  };
 
   const bool gates = a.gate.p != nullptr && a.rows_per_gate > 0;  // a gate per run of rows
-  for (int64_t row = row0; row < row1; ++row) {
-    float h[J][8], p[J][8], hat[J][8], d[J][8], gv[J][8];
-    const S* x = static_cast<const S*>(a.x) + row * a.x_stride + first;
+  int64_t gate_row = gates ? row0 / a.rows_per_gate : 0;
+  int64_t gate_end = gates ? (gate_row + 1) * a.rows_per_gate : row1;  // the run's end
+  if (SH::kRows) fetch(row0, 0);
+  Params<WPR, J, SH, ONE> params(a, smem + SH::kAfterRows, first, n, gate_row);
+  if (SH::kParams) __syncthreads();
+  int stage = 0;
+  for (int64_t row = row0; row < row1; ++row, stage ^= 1) {
+    if (SH::kRows) {
+      fetch(row + 1, stage ^ 1);
+      cp_async_wait<1>();
+    }
+    float_pair h[J][4], p[J][4], hat[POST ? J : 1][4], d[J][4];
 #pragma unroll
-    for (int j = 0; j < J; ++j) get8(x + j * step, n[j], vec, h[j]);
+    for (int j = 0; j < J; ++j) take(x0 + row * a.x_stride, stage, 0, j, h[j]);
     float pr = 0.f;
-    const int64_t gate_row = gates ? row / a.rows_per_gate : 0;
-    if (a.branch != nullptr) {
-      const T* b = static_cast<const T*>(a.branch) + row * a.branch_stride + first;
+    if (branch) {
 #pragma unroll
-      for (int j = 0; j < J; ++j) get8(b + j * step, n[j], vec, p[j]);
+      for (int j = 0; j < J; ++j) take(b0 + row * a.branch_stride, stage, kX, j, p[j]);
       if (POST) {
         pr = norm_row<WPR, J>(p, n, a.post, inv_width, a.eps, sum);
 #pragma unroll
-        for (int j = 0; j < J; ++j)
+        for (int j = 0; j < J; ++j) {
 #pragma unroll
-          for (int i = 0; i < 8; ++i) hat[j][i] = p[j][i];
-        if (a.post_weight.p != nullptr)
-#pragma unroll
-          for (int j = 0; j < J; ++j) {
-            float w[8];
-            get_param8(a.post_weight, first + j * step, n[j], vec, w);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) p[j][i] *= w[i];
-          }
-        if (a.post_bias.p != nullptr)
-#pragma unroll
-          for (int j = 0; j < J; ++j) {
-            float w[8];
-            get_param8(a.post_bias, first + j * step, n[j], vec, w);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) p[j][i] += w[i];
-          }
-      }
-      const int64_t at = gate_row * a.width;
-#pragma unroll
-      for (int j = 0; j < J; ++j) {
-        if (a.gate.p != nullptr) {
-          get_param8(a.gate, at + first + j * step, n[j], vec, gv[j]);
-        } else {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) gv[j][i] = 1.f;
+          for (int i = 0; i < 4; ++i) hat[POST ? j : 0][i] = p[j][i];
+          params.scale(kPostWeight, j, p[j]);
+          params.shift(kPostBias, j, p[j]);
         }
-#pragma unroll
-        for (int i = 0; i < 8; ++i) h[j][i] = fmaf(gv[j][i], p[j][i], h[j][i]);
       }
+#pragma unroll
+      for (int j = 0; j < J; ++j) params.gated(j, p[j], h[j]);
     }
     const float r = norm_row<WPR, J>(h, n, a.norm, inv_width, a.eps, sum);  // h is normed now
-    if (f.dy != nullptr) {
-      const T* dy = static_cast<const T*>(f.dy) + row * f.dy_stride + first;
+    if (has_dy) {
 #pragma unroll
       for (int j = 0; j < J; ++j) {
-        get8(dy + j * step, n[j], vec, d[j]);
+        take(dy0 + row * f.dy_stride, stage, kX + kF, j, d[j]);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          acc[kWeight][j][i] = fmaf(d[j][i], h[j][i], acc[kWeight][j][i]);
-          acc[kBias][j][i] += d[j][i];
+        for (int i = 0; i < 4; ++i) {
+          acc[kWeight][j][i] = fma_pair(d[j][i], h[j][i], acc[kWeight][j][i]);
+          acc[kBias][j][i] = add_pair(acc[kBias][j][i], d[j][i]);
         }
-        if (a.weight.p != nullptr) {
-          float w[8];
-          get_param8(a.weight, first + j * step, n[j], vec, w);
-#pragma unroll
-          for (int i = 0; i < 8; ++i) d[j][i] *= w[i];
-        }
+        params.scale(kWeight, j, d[j]);
       }
       norm_back<WPR, J>(d, h, n, a.norm, r, inv_width, sum);
     } else {
 #pragma unroll
       for (int j = 0; j < J; ++j)
 #pragma unroll
-        for (int i = 0; i < 8; ++i) d[j][i] = 0.f;
+        for (int i = 0; i < 4; ++i) d[j][i] = both(0.f);
     }
-    if (f.dh != nullptr) {
-      const S* dh = static_cast<const S*>(f.dh) + row * f.dh_stride + first;
+    if (has_dh) {
 #pragma unroll
       for (int j = 0; j < J; ++j) {
-        float t[8];
-        get8(dh + j * step, n[j], vec, t);
+        float_pair t[4];
+        take(dh0 + row * f.dh_stride, stage, kX + 2 * kF, j, t);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) d[j][i] += t[i];
+        for (int i = 0; i < 4; ++i) d[j][i] = add_pair(d[j][i], t[i]);
       }
     }
     if (f.dx != nullptr) {
       S* dx = static_cast<S*>(f.dx) + row * f.dx_stride + first;
 #pragma unroll
-      for (int j = 0; j < J; ++j) put8(dx + j * step, n[j], vec, d[j]);
+      for (int j = 0; j < J; ++j) put_pairs(dx + j * step, n[j], vec, d[j]);
     }
-    if (a.branch != nullptr) {
+    if (!branch) continue;
 #pragma unroll
-      for (int j = 0; j < J; ++j)
+    for (int j = 0; j < J; ++j) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          acc[kGate][j][i] = fmaf(d[j][i], p[j][i], acc[kGate][j][i]);
-          d[j][i] *= gv[j][i];
+      for (int i = 0; i < 4; ++i) acc[kGate][j][i] = fma_pair(d[j][i], p[j][i], acc[kGate][j][i]);
+      params.scale(kGate, j, d[j]);
+    }
+    if (POST) {
+#pragma unroll
+      for (int j = 0; j < J; ++j) {
+        float_pair(&aw)[4] = acc[kPostWeight % kAccs][j], (&ab)[4] = acc[kPostBias % kAccs][j];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          aw[i] = fma_pair(d[j][i], hat[POST ? j : 0][i], aw[i]);
+          ab[i] = add_pair(ab[i], d[j][i]);
         }
-      if (POST) {
-#pragma unroll
-        for (int j = 0; j < J; ++j)
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            acc[kPostWeight % kAccs][j][i] = fmaf(d[j][i], hat[j][i], acc[kPostWeight % kAccs][j][i]);
-            acc[kPostBias % kAccs][j][i] += d[j][i];
-          }
-        if (a.post_weight.p != nullptr)
-#pragma unroll
-          for (int j = 0; j < J; ++j) {
-            float w[8];
-            get_param8(a.post_weight, first + j * step, n[j], vec, w);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) d[j][i] *= w[i];
-          }
-        norm_back<WPR, J>(d, hat, n, a.post, pr, inv_width, sum);
+        params.scale(kPostWeight, j, d[j]);
       }
-      if (f.dbranch != nullptr) {
-        T* db = static_cast<T*>(f.dbranch) + row * f.dbranch_stride + first;
+      norm_back<WPR, J>(d, hat, n, a.post, pr, inv_width, sum);
+    }
+    if (f.dbranch != nullptr) {
+      T* db = static_cast<T*>(f.dbranch) + row * f.dbranch_stride + first;
 #pragma unroll
-        for (int j = 0; j < J; ++j) put8(db + j * step, n[j], vec, d[j]);
-      }
+      for (int j = 0; j < J; ++j) put_pairs(db + j * step, n[j], vec, d[j]);
+    }
+    if (gates && (row + 1 == row1 || row + 1 == gate_end)) {
       // the last row here of a run of rows with one gate: its sum goes out
-      if (gates && f.out[kGate] != nullptr &&
-          (row + 1 == row1 || (row + 1) % a.rows_per_gate == 0)) {
+      if (f.out[kGate] != nullptr) {
 #pragma unroll
         for (int j = 0; j < J; ++j) {
-          if (a.rows_per_gate == 1)
-            put_param8(f.out[kGate], f.out_type[kGate], gate_row * a.width + first + j * step, n[j],
-                       vec, acc[kGate][j]);
-          else
-            put8(f.part[kGate] + (slot + gate_row) * a.width + first + j * step, n[j], vec,
-                 acc[kGate][j]);
+          const int64_t c = first + j * step;
+          if (a.rows_per_gate == 1) {
+            float v[8];
 #pragma unroll
-          for (int i = 0; i < 8; ++i) acc[kGate][j][i] = 0.f;
+            for (int i = 0; i < 4; ++i) unpack_pair(v[2 * i], v[2 * i + 1], acc[kGate][j][i]);
+            put_param8(f.out[kGate], f.out_type[kGate], gate_row * a.width + c, n[j], vec, v);
+          } else {
+            put_pairs(f.part[kGate] + (slot + gate_row) * a.width + c, n[j], vec, acc[kGate][j]);
+          }
+#pragma unroll
+          for (int i = 0; i < 4; ++i) acc[kGate][j][i] = both(0.f);
         }
       }
+      ++gate_row;
+      gate_end += a.rows_per_gate;
+      if (row + 1 < row1) params.turn_to(gate_row);
     }
   }
+  cp_async_wait<0>();
 
 #pragma unroll
   for (int k = 0; k < kAccs; ++k) {
     if (f.out[k] == nullptr || (k == kGate && gates)) continue;  // the same for all threads
     float* to = f.part[k] + (int64_t)blockIdx.x * a.width;
-    if (kSlots == 1) {
+    if (slots == 1) {
 #pragma unroll
-      for (int j = 0; j < J; ++j) put8(to + first + j * step, n[j], vec, acc[k][j]);
+      for (int j = 0; j < J; ++j) put_pairs(to + first + j * step, n[j], vec, acc[k][j]);
     } else {
       __syncthreads();
 #pragma unroll
       for (int j = 0; j < J; ++j)
-        Elem<float>::store8(fold + sum.slot * kRow + first + j * step, acc[k][j]);
+        put_pairs(fold + sum.slot * kRow + first + j * step, 8, true, acc[k][j]);
       __syncthreads();
-      for (int c = threadIdx.x; c < (int)a.width; c += kThreads) {
+      for (int c = threadIdx.x; c < (int)a.width; c += blockDim.x) {
         float s = 0.f;
-#pragma unroll
-        for (int q = 0; q < kSlots; ++q) s += fold[q * kRow + c];
+        for (int q = 0; q < slots; ++q) s += fold[q * kRow + c];
         to[c] = s;
       }
     }
@@ -295,53 +306,74 @@ __global__ void __launch_bounds__(256) finish_kernel(const Bwd f, int64_t blocks
   }
 }
 
-// Warps to a row.
-int row_warps(int64_t width) {
-  return width <= 512 ? 1 : width <= 1024 ? 2 : width <= 2048 ? 4 : width <= 4096 ? 8 : 16;
+// Blocks of a call and slots of a block: one full block to an SM; with few rows a slot has one, and
+// they are spread over the SMs.
+struct Grid {
+  int64_t blocks;
+  int slots;
+  bool one;
+};
+Grid grid_of(int64_t rows, int64_t width, bool post) {
+  constexpr int sms = 148;
+  const int most = kMaxThreads / 32 / row_warps(width, post);
+  if (rows > (int64_t)sms * most) return {sms, most, false};
+  const int slots = (int)((rows + sms - 1) / sms);
+  return {(rows + slots - 1) / slots, slots, true};
 }
 
-// Blocks of a call: two of 256 threads to an SM are resident; with few rows a group of warps
-// takes one row each.
-int64_t bwd_blocks(int64_t rows, int64_t width) {
-  const int wpr = row_warps(width), slots = wpr > 8 ? 1 : 8 / wpr;
-  return std::min<int64_t>((rows + slots - 1) / slots, 2 * 148);
-}
-
-template <typename S, typename T, int WPR, int J>
-cudaError_t launch_back(const Bwd& f, int64_t blocks, cudaStream_t stream) {
-  if (f.a.post != 0)
-    backward_kernel<S, T, WPR, J, true><<<(unsigned)blocks, bwd_threads<WPR>(), 0, stream>>>(f);
-  else
-    backward_kernel<S, T, WPR, J, false><<<(unsigned)blocks, bwd_threads<WPR>(), 0, stream>>>(f);
+template <typename S, typename T, int WPR, int J, bool POST, bool ONE>
+cudaError_t launch_grid(const Bwd& f, const Grid& g, cudaStream_t stream) {
+  constexpr uint32_t rows = Shared<WPR, J, J*(sizeof(S) + sizeof(T)), ONE>::kBytes;
+  constexpr uint32_t fold = kMaxThreads * 8 * J * 4;
+  constexpr uint32_t bytes = rows > fold ? rows : fold;
+  auto k = backward_kernel<S, T, WPR, J, POST, ONE>;
+  if (cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes))
+    return e;
+  k<<<(unsigned)g.blocks, g.slots * WPR * 32, bytes, stream>>>(f);
   return cudaGetLastError();
 }
 
-template <typename S, typename T>
-cudaError_t launch_back_types(const Bwd& f, int64_t blocks, cudaStream_t stream) {
-  const int64_t w = f.a.width;
-  if (w <= 256) return launch_back<S, T, 1, 1>(f, blocks, stream);
-  if (w <= 512) return launch_back<S, T, 1, 2>(f, blocks, stream);
-  if (w <= 1024) return launch_back<S, T, 2, 2>(f, blocks, stream);
-  if (w <= 2048) return launch_back<S, T, 4, 2>(f, blocks, stream);
-  if (w <= 4096) return launch_back<S, T, 8, 2>(f, blocks, stream);
-  if (w <= 8192) return launch_back<S, T, 16, 2>(f, blocks, stream);
-  return launch_back<S, T, 16, 4>(f, blocks, stream);
+template <typename S, typename T, int WPR, int J, bool POST>
+cudaError_t launch_back(const Bwd& f, const Grid& g, cudaStream_t stream) {
+  return g.one ? launch_grid<S, T, WPR, J, POST, true>(f, g, stream)
+               : launch_grid<S, T, WPR, J, POST, false>(f, g, stream);
 }
 
-cudaError_t launch_residual_norm_grad(const Bwd& f, int64_t blocks, int64_t gates,
+template <typename S, typename T>
+cudaError_t launch_back_types(const Bwd& f, const Grid& g, cudaStream_t stream) {
+  const int64_t w = f.a.width;
+  if (f.a.post != 0) {
+    if (w <= 256) return launch_back<S, T, 1, 1, true>(f, g, stream);
+    if (w <= 512) return launch_back<S, T, 2, 1, true>(f, g, stream);
+    if (w <= 1024) return launch_back<S, T, 4, 1, true>(f, g, stream);
+    if (w <= 2048) return launch_back<S, T, 8, 1, true>(f, g, stream);
+    if (w <= 4096) return launch_back<S, T, 16, 1, true>(f, g, stream);
+    if (w <= 8192) return launch_back<S, T, 16, 2, true>(f, g, stream);
+    return launch_back<S, T, 16, 4, true>(f, g, stream);
+  }
+  if (w <= 256) return launch_back<S, T, 1, 1, false>(f, g, stream);
+  if (w <= 512) return launch_back<S, T, 1, 2, false>(f, g, stream);
+  if (w <= 1024) return launch_back<S, T, 2, 2, false>(f, g, stream);
+  if (w <= 2048) return launch_back<S, T, 4, 2, false>(f, g, stream);
+  if (w <= 4096) return launch_back<S, T, 8, 2, false>(f, g, stream);
+  if (w <= 8192) return launch_back<S, T, 16, 2, false>(f, g, stream);
+  return launch_back<S, T, 16, 4, false>(f, g, stream);
+}
+
+cudaError_t launch_residual_norm_grad(const Bwd& f, const Grid& g, int64_t gates,
                                       cudaStream_t stream) {
   const int s = f.a.stream_type, t = f.a.type;
   cudaError_t e;
   if (s == VGGT_DTYPE_FP32 && t == VGGT_DTYPE_FP32)
-    e = launch_back_types<float, float>(f, blocks, stream);
+    e = launch_back_types<float, float>(f, g, stream);
   else if (s == VGGT_DTYPE_FP32 && t == VGGT_DTYPE_BF16)
-    e = launch_back_types<float, __nv_bfloat16>(f, blocks, stream);
+    e = launch_back_types<float, __nv_bfloat16>(f, g, stream);
   else if (s == VGGT_DTYPE_FP32)
-    e = launch_back_types<float, __half>(f, blocks, stream);
+    e = launch_back_types<float, __half>(f, g, stream);
   else if (t == VGGT_DTYPE_BF16)
-    e = launch_back_types<__nv_bfloat16, __nv_bfloat16>(f, blocks, stream);
+    e = launch_back_types<__nv_bfloat16, __nv_bfloat16>(f, g, stream);
   else
-    e = launch_back_types<__half, __half>(f, blocks, stream);
+    e = launch_back_types<__half, __half>(f, g, stream);
   if (e != cudaSuccess) return e;
   bool any = false;
   for (int k = 0; k < kArrays; ++k) any = any || f.out[k] != nullptr;
@@ -350,7 +382,7 @@ cudaError_t launch_residual_norm_grad(const Bwd& f, int64_t blocks, int64_t gate
   const int64_t runs = f.a.rows_per_gate > 1 && f.out[kGate] ? gates : 0;
   const dim3 grid((unsigned)((f.a.width + 31) / 32),
                   (unsigned)(kArrays + std::min<int64_t>(runs, 4096)));
-  finish_kernel<<<grid, 256, 0, stream>>>(f, blocks, gates);
+  finish_kernel<<<grid, 256, 0, stream>>>(f, g.blocks, gates);
   return cudaGetLastError();
 }
 
@@ -361,11 +393,15 @@ extern "C" size_t vggt_residual_norm_grad_workspace_size(int64_t rows, int64_t w
                                                          int64_t rows_per_gate) {
   using namespace vggt::rnorm;
   if (rows <= 0 || width <= 0 || width > VGGT_NORM_MAX_WIDTH || rows_per_gate < 0) return 0;
-  const int64_t blocks = bwd_blocks(rows, width), wpr = row_warps(width);
-  const int64_t slots = blocks * (wpr > 8 ? 1 : 8 / wpr);
-  int64_t lines = kArrays * blocks;
-  if (rows_per_gate > 1) lines += slots + rows / rows_per_gate;
-  return (size_t)(lines * ((width + 3) / 4 * 4) * 4);
+  // with and without a norm of the branch, whichever takes more
+  size_t most = 0;
+  for (int post = 0; post < 2; ++post) {
+    const Grid g = grid_of(rows, width, post);
+    int64_t lines = kArrays * g.blocks;
+    if (rows_per_gate > 1) lines += g.blocks * g.slots + rows / rows_per_gate;
+    most = std::max(most, (size_t)(lines * ((width + 3) / 4 * 4) * 4));
+  }
+  return most;
 }
 
 extern "C" int vggt_residual_norm_grad(const vggt_residual_norm_args* args,
@@ -413,16 +449,16 @@ extern "C" int vggt_residual_norm_grad(const vggt_residual_norm_args* args,
     return api_fail("the workspace is too small or not 16-byte aligned");
   f.a.vec = f.a.vec && wide_rows(f.dy, f.dy_stride, f.a.type) && wide_rows(f.dh, f.dh_stride, f.a.stream_type) &&
             wide_rows(f.dx, f.dx_stride, f.a.stream_type) && wide_rows(f.dbranch, f.dbranch_stride, f.a.type);
-  const int64_t blocks = bwd_blocks(rows, width), wpr = row_warps(width);
-  f.slots = std::min(rows, blocks * (wpr > 8 ? 1 : 8 / wpr));
+  const Grid grid = grid_of(rows, width, f.a.post != 0);
+  f.slots = std::min(rows, grid.blocks * grid.slots);
   float* at = static_cast<float*>(workspace);
   for (int k = 0; k < kArrays; ++k) {
     f.out[k] = outs[k];
     f.out_type[k] = params[k]->dtype;
     f.a.vec = f.a.vec && wide_rows(outs[k], 8, f.out_type[k]);
     f.part[k] = at;
-    at += (k == kGate && f.a.rows_per_gate > 1 ? f.slots + gates : blocks) * width;
+    at += (k == kGate && f.a.rows_per_gate > 1 ? f.slots + gates : grid.blocks) * width;
     at += (4 - (at - static_cast<float*>(workspace)) % 4) % 4;
   }
-  return api_cuda(launch_residual_norm_grad(f, blocks, gates, static_cast<cudaStream_t>(stream)));
+  return api_cuda(launch_residual_norm_grad(f, grid, gates, static_cast<cudaStream_t>(stream)));
 }
