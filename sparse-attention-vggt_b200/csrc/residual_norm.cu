@@ -17,11 +17,11 @@ struct Fwd {
   int64_t h_stride, y_stride;
 };
 
-template <typename S, typename T, int WPR, int J, bool ONE>
+template <typename S, typename T, int WPR, int J, bool DIRECT>
 __global__ void __launch_bounds__(kMaxThreads, 1) forward_kernel(const Fwd f) {
   constexpr int kX = sizeof(S) / 2, kF = sizeof(T) / 2;  // 16-byte units of 8 elements
   constexpr int kUnits = J * (kX + kF);
-  typedef Shared<WPR, J, kUnits, ONE> SH;
+  typedef Shared<WPR, J, kUnits, DIRECT> SH;
   extern __shared__ __align__(16) unsigned char smem[];
   __shared__ float scratch[2 * 2 * 32];
   const Args& a = f.a;
@@ -29,7 +29,7 @@ __global__ void __launch_bounds__(kMaxThreads, 1) forward_kernel(const Fwd f) {
   const Pipe<kUnits> pipe(smem);
   const int lane = threadIdx.x & 31, slots = (blockDim.x >> 5) / WPR;
   const float inv_width = 1.f / (float)a.width;
-  const bool vec = a.vec, branch = a.branch != nullptr;
+  const bool vec = !DIRECT || a.vec, branch = a.branch != nullptr;
   int n[J];
 #pragma unroll
   for (int j = 0; j < J; ++j)
@@ -38,44 +38,52 @@ __global__ void __launch_bounds__(kMaxThreads, 1) forward_kernel(const Fwd f) {
   constexpr int step = 8 * WPR * 32;
   // a run of rows to a slot: gates change seldom
   const int64_t slot = (int64_t)blockIdx.x * slots + sum.slot, all = (int64_t)gridDim.x * slots;
-  int64_t row = ONE ? slot : slot * a.rows / all;
-  const int64_t end = ONE ? min(slot + 1, a.rows) : (slot + 1) * a.rows / all;
-  const S* const x0 = static_cast<const S*>(a.x) + first;
-  const T* const b0 = static_cast<const T*>(a.branch) + first;
-  auto fetch = [&](int64_t r, int stage) {
-    if (vec && r < end) {
+  int64_t row = slot * a.rows / all;
+  const int64_t end = (slot + 1) * a.rows / all;
+  const S* x = static_cast<const S*>(a.x) + row * a.x_stride + first;
+  const T* b = static_cast<const T*>(a.branch) + (branch ? row * a.branch_stride + first : 0);
+  S* h = static_cast<S*>(f.h) + (branch ? row * f.h_stride + first : 0);
+  T* y = static_cast<T*>(f.y) + row * f.y_stride + first;
+  // x and b are a row ahead where rows are copied ahead
+  auto fetch = [&](bool there, int stage) {
+    if (there) {
 #pragma unroll
       for (int j = 0; j < J; ++j)
         if (n[j] > 0) {
-          pipe.fetch(stage, j * (kX + kF), x0 + r * a.x_stride + j * step);
-          if (branch) pipe.fetch(stage, j * (kX + kF) + kX, b0 + r * a.branch_stride + j * step);
+          pipe.fetch(stage, j * (kX + kF), x + j * step);
+          if (branch) pipe.fetch(stage, j * (kX + kF) + kX, b + j * step);
         }
+      x += a.x_stride;
+      if (branch) b += a.branch_stride;
     }
     cp_async_commit();
   };
-  if (SH::kRows) fetch(row, 0);
+  if (!DIRECT) {
+    pipe.clear();
+    fetch(row < end, 0);
+  }
   const bool gates = a.gate.p != nullptr && a.rows_per_gate > 0;
   int64_t gate_row = gates ? min(row, a.rows - 1) / a.rows_per_gate : 0;
   int64_t gate_end = gates ? (gate_row + 1) * a.rows_per_gate : a.rows;
-  Params<WPR, J, SH, ONE> params(a, smem + SH::kAfterRows, first, n, gate_row);
+  Params<WPR, J, SH, DIRECT> params(a, smem + SH::kAfterRows, first, n, gate_row);
   if (SH::kParams) __syncthreads();
   for (int stage = 0; row < end; ++row, stage ^= 1) {
-    if (SH::kRows) {
-      fetch(row + 1, stage ^ 1);
-      cp_async_wait<1>();
-    }
     float_pair v[J][4], p[J][4];
+    if (DIRECT) {
 #pragma unroll
-    for (int j = 0; j < J; ++j) {
-      if (!SH::kRows || !vec) {
-        get_pairs(x0 + row * a.x_stride + j * step, n[j], vec, v[j]);
-        if (branch) get_pairs(b0 + row * a.branch_stride + j * step, n[j], vec, p[j]);
-      } else if (n[j] > 0) {
+      for (int j = 0; j < J; ++j) {
+        get_pairs(x + j * step, n[j], vec, v[j]);
+        if (branch) get_pairs(b + j * step, n[j], vec, p[j]);
+      }
+      x += a.x_stride;
+      if (branch) b += a.branch_stride;
+    } else {
+      fetch(row + 1 < end, stage ^ 1);
+      cp_async_wait<1>();
+#pragma unroll
+      for (int j = 0; j < J; ++j) {
         pipe.template read<S>(stage, j * (kX + kF), v[j]);
-        if (branch) pipe.template read<T>(stage, j * (kX + kF) + kX, p[j]);
-      } else {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) v[j][i] = p[j][i] = both(0.f);
+        pipe.template read<T>(stage, j * (kX + kF) + kX, p[j]);
       }
     }
     if (branch) {
@@ -91,29 +99,29 @@ __global__ void __launch_bounds__(kMaxThreads, 1) forward_kernel(const Fwd f) {
         gate_end += a.rows_per_gate;
         params.turn_to(++gate_row);
       }
-      S* h = static_cast<S*>(f.h) + row * f.h_stride + first;
 #pragma unroll
       for (int j = 0; j < J; ++j) {
         params.gated(j, p[j], v[j]);
         put_pairs(h + j * step, n[j], vec, v[j]);
       }
+      h += f.h_stride;
     }
     norm_row<WPR, J>(v, n, a.norm, inv_width, a.eps, sum);
-    T* y = static_cast<T*>(f.y) + row * f.y_stride + first;
 #pragma unroll
     for (int j = 0; j < J; ++j) {
       params.scale(kWeight, j, v[j]);
       params.shift(kBias, j, v[j]);
       put_pairs(y + j * step, n[j], vec, v[j]);
     }
+    y += f.y_stride;
   }
 }
 
-template <typename S, typename T, int WPR, int J, bool ONE>
+template <typename S, typename T, int WPR, int J, bool DIRECT>
 cudaError_t launch_shape(const Fwd& f, int64_t blocks, int slots, cudaStream_t stream) {
   constexpr uint32_t bytes =
-      Shared<WPR, J, J*(sizeof(S) / 2 + sizeof(T) / 2), ONE>::kBytes;
-  auto k = forward_kernel<S, T, WPR, J, ONE>;
+      Shared<WPR, J, J*(sizeof(S) / 2 + sizeof(T) / 2), DIRECT>::kBytes;
+  auto k = forward_kernel<S, T, WPR, J, DIRECT>;
   if (cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes))
     return e;
   k<<<(unsigned)blocks, slots * WPR * 32, bytes, stream>>>(f);
@@ -123,12 +131,14 @@ cudaError_t launch_shape(const Fwd& f, int64_t blocks, int slots, cudaStream_t s
 template <typename S, typename T, int WPR, int J>
 cudaError_t launch_rows(const Fwd& f, int sms, cudaStream_t stream) {
   constexpr int most = kMaxThreads / 32 / WPR;
+  constexpr bool fits = Shared<WPR, J, J*(sizeof(S) / 2 + sizeof(T) / 2), false>::kFits;
   // few rows: spread over the SMs, each with a slot of its own
-  if (f.a.rows <= (int64_t)sms * most) {
-    const int slots = (int)((f.a.rows + sms - 1) / sms);
-    return launch_shape<S, T, WPR, J, true>(f, (f.a.rows + slots - 1) / slots, slots, stream);
-  }
-  return launch_shape<S, T, WPR, J, false>(f, sms, most, stream);
+  const int slots = (int)std::min<int64_t>(most, (f.a.rows + sms - 1) / sms);
+  const int64_t blocks = std::min<int64_t>(sms, (f.a.rows + slots - 1) / slots);
+  if constexpr (fits)
+    if (f.a.vec && f.a.rows > blocks * slots)
+      return launch_shape<S, T, WPR, J, false>(f, blocks, slots, stream);
+  return launch_shape<S, T, WPR, J, true>(f, blocks, slots, stream);
 }
 
 template <typename S, typename T>

@@ -11,8 +11,8 @@
 // (cp.async, where the layout allows 16-byte accesses: `vec`), and the parameters lie there too, in
 // fp32, read once per block: what a thread needs of either is its own, so that no barrier is
 // needed.  (Read from global memory where they are used, the parameters' latencies took half the
-// time: 32 frames of width 1024, fp32 stream, 159 us.)  With few rows, one to a slot (ONE),
-// everything is read into registers at once.  All arithmetic is in fp32, in packed pairs; means
+// time: 32 frames of width 1024, fp32 stream, 159 us.)  Few rows, unaligned ones and the widest are
+// read straight into registers, the parameters once for all rows (DIRECT).  All arithmetic is in fp32, in packed pairs; means
 // are formed first and variances from what is left after them, so that a row far from zero loses
 // nothing.
 #pragma once
@@ -23,6 +23,7 @@
 namespace vggt {
 namespace rnorm {
 
+constexpr int kMaxThreads = 512;  // of a block
 constexpr int kNormLayer = VGGT_NORM_LAYER, kNormRms = VGGT_NORM_RMS;
 
 // A vector of parameters in any of the three element types, or none.
@@ -75,35 +76,35 @@ struct Args {
   bool vec;
 };
 
-constexpr int kMaxThreads = 512, kStages = 2;
+constexpr int kStages = 2;
 constexpr uint32_t kSharedBytes = 208 * 1024;
 
 enum { kWeight, kBias, kGate, kPostWeight, kPostBias, kArrays };
 
 // Shared memory of a block: rows to come (UNITS 16-byte units a thread and stage), parameters
-// (all slots' the same), and the slot's gate where it is one of several.  What does not fit is read
-// where it is used.
-template <int WPR, int J, int UNITS, bool ONE>
+// (all slots' the same), and the slot's gate, which may be one of several.  Parameters that do not
+// fit are read where they are used; rows that do not are DIRECT.
+template <int WPR, int J, int UNITS, bool DIRECT>
 struct Shared {
   static constexpr uint32_t kRowBytes = kMaxThreads * kStages * UNITS * 16;
   static constexpr uint32_t kParamBytes = WPR * 32 * J * 32, kGateBytes = kMaxThreads * J * 32;
-  static constexpr bool kRows = !ONE && kRowBytes <= kSharedBytes;
-  static constexpr uint32_t kAfterRows = kRows ? kRowBytes : 0;
+  static constexpr bool kFits = kRowBytes <= kSharedBytes;
   // four parameters and the gate
   static constexpr bool kParams =
-      !ONE && kAfterRows + 4 * kParamBytes + kGateBytes <= kSharedBytes;
+      !DIRECT && kRowBytes + 4 * kParamBytes + kGateBytes <= kSharedBytes;
+  static constexpr uint32_t kAfterRows = DIRECT ? 0 : kRowBytes;
   static constexpr uint32_t kBytes = kAfterRows + (kParams ? 4 * kParamBytes + kGateBytes : 0);
 };
 
 // The parameters as one thread sees them.
-template <int WPR, int J, typename SH, bool ONE>
+template <int WPR, int J, typename SH, bool DIRECT>
 struct Params {
   const Args& a;
   unsigned char* at;  // this thread's place among the parameters
   int first;
   const int* n;
   int64_t gate_row = 0;
-  float_pair reg[ONE ? kArrays : 1][ONE ? J : 1][4];
+  float_pair reg[DIRECT ? kArrays : 1][DIRECT ? J : 1][4];
 
   static constexpr int kStep = 8 * WPR * 32;
   __device__ __forceinline__ const Param& param(int k) const {
@@ -129,18 +130,18 @@ struct Params {
       *reinterpret_cast<ulonglong2*>(place(k, j, 1)) = make_ulonglong2(v[2], v[3]);
     }
   }
-  // ONE: reads all that the call uses; else fills the shared places (a barrier has to follow)
+  // DIRECT: reads all that the call uses; else fills the shared places (a barrier has to follow)
   __device__ __forceinline__ Params(const Args& args, unsigned char* smem, int first_, const int* n_,
                                     int64_t gate_row_)
       : a(args), at(smem), first(first_), n(n_), gate_row(gate_row_) {
-    if (ONE) {
+    if (DIRECT) {
 #pragma unroll
       for (int k = 0; k < kArrays; ++k)
         if (param(k).p != nullptr)
 #pragma unroll
           for (int j = 0; j < J; ++j)
             get_param(param(k), (k == kGate ? gate_row * a.width : 0) + first + j * kStep, n[j],
-                      a.vec, reg[ONE ? k : 0][ONE ? j : 0]);
+                      a.vec, reg[DIRECT ? k : 0][DIRECT ? j : 0]);
     } else if (SH::kParams) {
 #pragma unroll
       for (int k = 0; k < kArrays; ++k)
@@ -151,12 +152,19 @@ struct Params {
   __device__ __forceinline__ void turn_to(int64_t row) {
     if (row == gate_row) return;
     gate_row = row;
-    if (!ONE && SH::kParams) fill(kGate);
+    if (DIRECT) {
+#pragma unroll
+      for (int j = 0; j < J; ++j)
+        get_param(a.gate, row * a.width + first + j * kStep, n[j], a.vec,
+                  reg[DIRECT ? kGate : 0][DIRECT ? j : 0]);
+    } else if (SH::kParams) {
+      fill(kGate);
+    }
   }
   __device__ __forceinline__ void get(int k, int j, float_pair* v) const {
-    if (ONE) {
+    if (DIRECT) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) v[i] = reg[ONE ? k : 0][ONE ? j : 0][i];
+      for (int i = 0; i < 4; ++i) v[i] = reg[DIRECT ? k : 0][DIRECT ? j : 0][i];
     } else if (SH::kParams) {
       const ulonglong2 lo = *reinterpret_cast<const ulonglong2*>(place(k, j, 0));
       const ulonglong2 hi = *reinterpret_cast<const ulonglong2*>(place(k, j, 1));
@@ -202,6 +210,12 @@ struct Pipe {
   __device__ __forceinline__ explicit Pipe(unsigned char* smem) : mine(smem + threadIdx.x * 16) {
     mine_u32 = smem_u32(mine);
   }
+  // what is never fetched (past the row's end, tensors that are not there) reads as zeros
+  __device__ __forceinline__ void clear() const {
+#pragma unroll
+    for (int u = 0; u < kStages * UNITS; ++u)
+      *reinterpret_cast<uint4*>(mine + u * (kMaxThreads * 16)) = make_uint4(0, 0, 0, 0);
+  }
   // chunk `unit0` on of an 8-element group of E
   template <typename E>
   __device__ __forceinline__ void fetch(int stage, int unit0, const E* p) const {
@@ -242,34 +256,63 @@ __device__ __forceinline__ void subtract(float_pair* v, int n, float c) {
 template <int WPR>
 struct RowSum {
   float* scratch;
-  int slot, warp, turn = 0;
+  int slot, warp, lane, turn = 0;
   __device__ __forceinline__ RowSum(float* s) : scratch(s) {
     slot = (threadIdx.x >> 5) / WPR;
     warp = (threadIdx.x >> 5) % WPR;
+    lane = threadIdx.x & 31;
   }
+  __device__ __forceinline__ float* row() {
+    float* s = scratch + (turn * (kMaxThreads / 32) + slot * WPR) * 2;
+    turn ^= 1;
+    return s;
+  }
+  __device__ __forceinline__ void meet() const {
+    asm volatile("bar.sync %0, %1;" ::"r"(1 + slot), "n"(WPR * 32) : "memory");
+  }
+  // lanes below 16 go on with a, the others with b
   __device__ __forceinline__ void two(float& a, float& b) {
+    const bool high = lane >= 16;
+    float v = (high ? b : a) + __shfl_xor_sync(0xffffffffu, high ? a : b, 16);
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      a += __shfl_xor_sync(0xffffffffu, a, o);
-      b += __shfl_xor_sync(0xffffffffu, b, o);
-    }
+    for (int o = 8; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
     if (WPR > 1) {
-      float2* s = reinterpret_cast<float2*>(scratch) + (turn * (blockDim.x >> 5)) + slot * WPR;
-      turn ^= 1;
-      if ((threadIdx.x & 31) == 0) s[warp] = make_float2(a, b);
-      asm volatile("bar.sync %0, %1;" ::"r"(1 + slot), "n"(WPR * 32) : "memory");
-      a = b = 0.f;
+      float* s = row();
+      if ((lane & 15) == 0) s[(lane >> 4) * WPR + warp] = v;
+      meet();
+      if (WPR <= 4) {
+        a = b = 0.f;
 #pragma unroll
-      for (int i = 0; i < WPR; ++i) {
-        const float2 t = s[i];
-        a += t.x;
-        b += t.y;
+        for (int i = 0; i < WPR; ++i) {
+          a += s[i];
+          b += s[WPR + i];
+        }
+        return;
       }
+      v = s[(lane >> 4) * WPR + (lane & (WPR - 1))];
+#pragma unroll
+      for (int o = WPR / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
     }
+    a = __shfl_sync(0xffffffffu, v, 0);
+    b = __shfl_sync(0xffffffffu, v, 16);
   }
   __device__ __forceinline__ float one(float a) {
-    float b = 0.f;
-    two(a, b);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) a += __shfl_xor_sync(0xffffffffu, a, o);
+    if (WPR > 1) {
+      float* s = row();
+      if (lane == 0) s[warp] = a;
+      meet();
+      if (WPR <= 4) {
+        a = 0.f;
+#pragma unroll
+        for (int i = 0; i < WPR; ++i) a += s[i];
+        return a;
+      }
+      a = s[lane & (WPR - 1)];
+#pragma unroll
+      for (int o = WPR / 2; o > 0; o >>= 1) a += __shfl_xor_sync(0xffffffffu, a, o);
+    }
     return a;
   }
 };

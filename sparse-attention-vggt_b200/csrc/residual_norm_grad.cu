@@ -71,12 +71,12 @@ __device__ __forceinline__ void norm_back(float_pair (*d)[4], const float_pair (
   }
 }
 
-template <typename S, typename T, int WPR, int J, bool POST, bool ONE>
+template <typename S, typename T, int WPR, int J, bool POST, bool DIRECT>
 __global__ void __launch_bounds__(kMaxThreads, 1) backward_kernel(const Bwd f) {
   constexpr int kAccs = POST ? 5 : 3;
   constexpr int kRow = WPR * 32 * 8 * J;  // columns that a slot holds
   constexpr int kX = sizeof(S) / 2, kF = sizeof(T) / 2, kUnits = 2 * (kX + kF);
-  typedef Shared<WPR, J, J * kUnits, ONE> SH;
+  typedef Shared<WPR, J, J * kUnits, DIRECT> SH;
   extern __shared__ __align__(16) unsigned char smem[];
   __shared__ float scratch[2 * 2 * 32];
   float* fold = reinterpret_cast<float*>(smem);  // after the rows
@@ -86,7 +86,7 @@ __global__ void __launch_bounds__(kMaxThreads, 1) backward_kernel(const Bwd f) {
   const int slots = (blockDim.x >> 5) / WPR;
   const int lane = threadIdx.x & 31;
   const float inv_width = 1.f / (float)a.width;
-  const bool vec = a.vec, branch = a.branch != nullptr, has_dy = f.dy != nullptr,
+  const bool vec = !DIRECT || a.vec, branch = a.branch != nullptr, has_dy = f.dy != nullptr,
              has_dh = f.dh != nullptr;
   int n[J];
 #pragma unroll
@@ -106,56 +106,65 @@ __global__ void __launch_bounds__(kMaxThreads, 1) backward_kernel(const Bwd f) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) acc[k][j][i] = both(0.f);
 
-  const S* const x0 = static_cast<const S*>(a.x) + first;
-  const T* const b0 = static_cast<const T*>(a.branch) + first;
-  const T* const dy0 = static_cast<const T*>(f.dy) + first;
-  const S* const dh0 = static_cast<const S*>(f.dh) + first;
-  auto fetch = [&](int64_t row, int stage) {
-    if (vec && row < row1) {
+  // a tensor that is not there is not read
+  const S* x = static_cast<const S*>(a.x) + row0 * a.x_stride + first;
+  const T* b = static_cast<const T*>(a.branch) + (branch ? row0 * a.branch_stride + first : 0);
+  const T* dy = static_cast<const T*>(f.dy) + (has_dy ? row0 * f.dy_stride + first : 0);
+  const S* dh = static_cast<const S*>(f.dh) + (has_dh ? row0 * f.dh_stride + first : 0);
+  S* dx = static_cast<S*>(f.dx) + (f.dx != nullptr ? row0 * f.dx_stride + first : 0);
+  T* db = static_cast<T*>(f.dbranch) + (f.dbranch != nullptr ? row0 * f.dbranch_stride + first : 0);
+  auto ahead = [&] {
+    x += a.x_stride;
+    if (branch) b += a.branch_stride;
+    if (has_dy) dy += f.dy_stride;
+    if (has_dh) dh += f.dh_stride;
+  };
+  // the pointers are a row ahead where rows are copied ahead
+  auto fetch = [&](bool there, int stage) {
+    if (there) {
 #pragma unroll
       for (int j = 0; j < J; ++j)
         if (n[j] > 0) {
-          pipe.fetch(stage, j * kUnits, x0 + row * a.x_stride + j * step);
-          if (branch) pipe.fetch(stage, j * kUnits + kX, b0 + row * a.branch_stride + j * step);
-          if (has_dy) pipe.fetch(stage, j * kUnits + kX + kF, dy0 + row * f.dy_stride + j * step);
-          if (has_dh)
-            pipe.fetch(stage, j * kUnits + kX + 2 * kF, dh0 + row * f.dh_stride + j * step);
+          pipe.fetch(stage, j * kUnits, x + j * step);
+          if (branch) pipe.fetch(stage, j * kUnits + kX, b + j * step);
+          if (has_dy) pipe.fetch(stage, j * kUnits + kX + kF, dy + j * step);
+          if (has_dh) pipe.fetch(stage, j * kUnits + kX + 2 * kF, dh + j * step);
         }
+      ahead();
     }
     cp_async_commit();
   };
   // chunk j of one of the row's four tensors
   auto take = [&](auto* p, int stage, int unit, int j, float_pair* v) {
     typedef std::remove_cv_t<std::remove_pointer_t<decltype(p)>> E;
-    if (!SH::kRows || !vec) {
+    if (DIRECT)
       get_pairs(p + j * step, n[j], vec, v);
-    } else if (n[j] > 0) {
+    else
       pipe.template read<E>(stage, j * kUnits + unit, v);
-    } else {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) v[i] = both(0.f);
-    }
   };
 
   const bool gates = a.gate.p != nullptr && a.rows_per_gate > 0;  // a gate per run of rows
   int64_t gate_row = gates ? row0 / a.rows_per_gate : 0;
   int64_t gate_end = gates ? (gate_row + 1) * a.rows_per_gate : row1;  // the run's end
-  if (SH::kRows) fetch(row0, 0);
-  Params<WPR, J, SH, ONE> params(a, smem + SH::kAfterRows, first, n, gate_row);
+  if (!DIRECT) {
+    pipe.clear();
+    fetch(row0 < row1, 0);
+  }
+  Params<WPR, J, SH, DIRECT> params(a, smem + SH::kAfterRows, first, n, gate_row);
   if (SH::kParams) __syncthreads();
   int stage = 0;
   for (int64_t row = row0; row < row1; ++row, stage ^= 1) {
-    if (SH::kRows) {
-      fetch(row + 1, stage ^ 1);
+    if (!DIRECT) {
+      fetch(row + 1 < row1, stage ^ 1);
       cp_async_wait<1>();
     }
     float_pair h[J][4], p[J][4], hat[POST ? J : 1][4], d[J][4];
 #pragma unroll
-    for (int j = 0; j < J; ++j) take(x0 + row * a.x_stride, stage, 0, j, h[j]);
+    for (int j = 0; j < J; ++j) take(x, stage, 0, j, h[j]);
     float pr = 0.f;
     if (branch) {
 #pragma unroll
-      for (int j = 0; j < J; ++j) take(b0 + row * a.branch_stride, stage, kX, j, p[j]);
+      for (int j = 0; j < J; ++j) take(b, stage, kX, j, p[j]);
       if (POST) {
         pr = norm_row<WPR, J>(p, n, a.post, inv_width, a.eps, sum);
 #pragma unroll
@@ -173,7 +182,7 @@ __global__ void __launch_bounds__(kMaxThreads, 1) backward_kernel(const Bwd f) {
     if (has_dy) {
 #pragma unroll
       for (int j = 0; j < J; ++j) {
-        take(dy0 + row * f.dy_stride, stage, kX + kF, j, d[j]);
+        take(dy, stage, kX + kF, j, d[j]);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           acc[kWeight][j][i] = fma_pair(d[j][i], h[j][i], acc[kWeight][j][i]);
@@ -192,15 +201,16 @@ __global__ void __launch_bounds__(kMaxThreads, 1) backward_kernel(const Bwd f) {
 #pragma unroll
       for (int j = 0; j < J; ++j) {
         float_pair t[4];
-        take(dh0 + row * f.dh_stride, stage, kX + 2 * kF, j, t);
+        take(dh, stage, kX + 2 * kF, j, t);
 #pragma unroll
         for (int i = 0; i < 4; ++i) d[j][i] = add_pair(d[j][i], t[i]);
       }
     }
+    if (DIRECT) ahead();
     if (f.dx != nullptr) {
-      S* dx = static_cast<S*>(f.dx) + row * f.dx_stride + first;
 #pragma unroll
       for (int j = 0; j < J; ++j) put_pairs(dx + j * step, n[j], vec, d[j]);
+      dx += f.dx_stride;
     }
     if (!branch) continue;
 #pragma unroll
@@ -223,9 +233,9 @@ __global__ void __launch_bounds__(kMaxThreads, 1) backward_kernel(const Bwd f) {
       norm_back<WPR, J>(d, hat, n, a.post, pr, inv_width, sum);
     }
     if (f.dbranch != nullptr) {
-      T* db = static_cast<T*>(f.dbranch) + row * f.dbranch_stride + first;
 #pragma unroll
       for (int j = 0; j < J; ++j) put_pairs(db + j * step, n[j], vec, d[j]);
+      db += f.dbranch_stride;
     }
     if (gates && (row + 1 == row1 || row + 1 == gate_end)) {
       // the last row here of a run of rows with one gate: its sum goes out
@@ -306,27 +316,24 @@ __global__ void __launch_bounds__(256) finish_kernel(const Bwd f, int64_t blocks
   }
 }
 
-// Blocks of a call and slots of a block: one full block to an SM; with few rows a slot has one, and
-// they are spread over the SMs.
+// Blocks of a call and slots of a block: one full block to an SM; few rows are spread over the SMs.
 struct Grid {
   int64_t blocks;
   int slots;
-  bool one;
 };
 Grid grid_of(int64_t rows, int64_t width, bool post) {
   constexpr int sms = 148;
   const int most = kMaxThreads / 32 / row_warps(width, post);
-  if (rows > (int64_t)sms * most) return {sms, most, false};
-  const int slots = (int)((rows + sms - 1) / sms);
-  return {(rows + slots - 1) / slots, slots, true};
+  const int slots = (int)std::min<int64_t>(most, (rows + sms - 1) / sms);
+  return {std::min<int64_t>(sms, (rows + slots - 1) / slots), slots};
 }
 
-template <typename S, typename T, int WPR, int J, bool POST, bool ONE>
+template <typename S, typename T, int WPR, int J, bool POST, bool DIRECT>
 cudaError_t launch_grid(const Bwd& f, const Grid& g, cudaStream_t stream) {
-  constexpr uint32_t rows = Shared<WPR, J, J*(sizeof(S) + sizeof(T)), ONE>::kBytes;
+  constexpr uint32_t rows = Shared<WPR, J, J*(sizeof(S) + sizeof(T)), DIRECT>::kBytes;
   constexpr uint32_t fold = kMaxThreads * 8 * J * 4;
   constexpr uint32_t bytes = rows > fold ? rows : fold;
-  auto k = backward_kernel<S, T, WPR, J, POST, ONE>;
+  auto k = backward_kernel<S, T, WPR, J, POST, DIRECT>;
   if (cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes))
     return e;
   k<<<(unsigned)g.blocks, g.slots * WPR * 32, bytes, stream>>>(f);
@@ -335,8 +342,11 @@ cudaError_t launch_grid(const Bwd& f, const Grid& g, cudaStream_t stream) {
 
 template <typename S, typename T, int WPR, int J, bool POST>
 cudaError_t launch_back(const Bwd& f, const Grid& g, cudaStream_t stream) {
-  return g.one ? launch_grid<S, T, WPR, J, POST, true>(f, g, stream)
-               : launch_grid<S, T, WPR, J, POST, false>(f, g, stream);
+  constexpr bool fits = Shared<WPR, J, J*(sizeof(S) + sizeof(T)), false>::kFits;
+  if constexpr (fits)
+    if (f.a.vec && f.a.rows > g.blocks * g.slots)
+      return launch_grid<S, T, WPR, J, POST, false>(f, g, stream);
+  return launch_grid<S, T, WPR, J, POST, true>(f, g, stream);
 }
 
 template <typename S, typename T>
