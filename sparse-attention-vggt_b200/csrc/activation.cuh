@@ -3,7 +3,7 @@
 
 #include <type_traits>
 
-#include "common.cuh"
+#include "exp2.cuh"
 #include "vggt_block.h"
 
 namespace vggt {
@@ -17,11 +17,6 @@ __device__ __forceinline__ float rcp(float x) {
 __device__ __forceinline__ float min_nan(float a, float b) {
   float y;
   asm("min.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
-  return y;
-}
-__device__ __forceinline__ float max_nan(float a, float b) {
-  float y;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
   return y;
 }
 
@@ -93,6 +88,33 @@ __device__ __forceinline__ float value_slope(float z, float& slope) {
   }
   slope = 1.f;
   return z;
+}
+
+// a(z) of a pair, in packed instructions where there are some: half of what the epilogue of a
+// product issues (32 frames widened with gelu took 392 us with value(), 246 without an activation).
+template <int KIND>
+__device__ __forceinline__ float_pair value_pair(float_pair z) {
+  float a, b;
+  unpack_pair(a, b, z);
+  if (KIND == VGGT_ACT_GELU) {
+    const float ua = min_nan(fabsf(a), 64.f), ub = min_nan(fabsf(b), 64.f);
+    const float_pair u = pack_pair(ua, ub);
+    float da, db, ea, eb;
+    unpack_pair(da, db, fma_pair(u, pack_pair(0.3f, 0.3f), pack_pair(1.f, 1.f)));
+    const float_pair t = pack_pair(rcp(da), rcp(db));
+    unpack_pair(ea, eb, mul_pair(mul_pair(u, u), pack_pair(-0.5f * kLog2e, -0.5f * kLog2e)));
+    const float_pair e = pack_pair(fast_exp2(ea), fast_exp2(eb));
+    // the polynomial with its sign turned: -q
+    float_pair r = fma_pair(pack_pair(0.0818372592f, 0.0818372592f), t,
+                            pack_pair(-0.230586097f, -0.230586097f));
+    r = fma_pair(r, t, pack_pair(0.0340376124f, 0.0340376124f));
+    r = fma_pair(r, t, pack_pair(-0.153751031f, -0.153751031f));
+    r = fma_pair(r, t, pack_pair(-0.111210488f, -0.111210488f));
+    r = fma_pair(r, t, pack_pair(-0.120327726f, -0.120327726f));
+    const float_pair q = mul_pair(mul_pair(r, t), e);
+    return fma_pair(q, u, pack_pair(max_nan(a, 0.f), max_nan(b, 0.f)));
+  }
+  return pack_pair(value<KIND>(a), value<KIND>(b));
 }
 
 // f with the activation as a compile-time constant: f(std::integral_constant<int, KIND>)

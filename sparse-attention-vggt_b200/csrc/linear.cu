@@ -3,11 +3,12 @@
 // A tile of C is 128 CTA x 128 CTA elements, CTA = 1 or 2 CTAs (a pair works on one tile: each
 // holds half of A's rows and half of B's, the MMA of the pair reads both halves of B).  Warp 0
 // streams the operands by TMA through a ring of 64-element reduction blocks, warp 1 issues the
-// MMAs into one of two accumulators in TMEM, and warps 4-11, two warpgroups that take alternate
-// 64-column pieces, run the epilogue of the tile before: TMEM -> registers -> bias, activation,
-// gate, residual -> a swizzled 16 KB buffer -> TMA store.  The residual comes by TMA into the same
-// buffer before.  What TMA cannot address (odd widths, other strides) is copied between buffer
-// and memory by the warps that own the rows.
+// MMAs into one of two accumulators in TMEM, and warps 4-19, four warpgroups of which each takes 64
+// columns, run the epilogue of the tile before: TMEM -> registers -> bias, activation, gate,
+// residual -> the group's swizzled 16 KB buffer -> TMA store.  The residual comes by TMA into the
+// same buffer before.  What TMA cannot address (odd widths, other strides) is copied between
+// buffer and memory by the warps that own the rows.  (With two warpgroups an activation's latencies
+// bounded the kernel.)
 //
 // Bound by the tensor cores and by the operands' way from L2 (a pair's 256 x 256 tile needs
 // 64 B a cycle and SM at the full rate, a single CTA's 128 x 128 twice that).
@@ -28,18 +29,19 @@ namespace lin {
 
 constexpr int BM = 128, BK = 64;
 constexpr int STAGES = 5;
-constexpr int THREADS = 384;
+constexpr int GROUPS = 4;                     // warpgroups of the epilogue
+constexpr int THREADS = 128 + GROUPS * 128;
 constexpr uint32_t HALF_BYTES = BM * BK * 2;         // one operand's block: 16 KB
 constexpr uint32_t STAGE_BYTES = 2 * HALF_BYTES;
 constexpr uint32_t BUF_BYTES = BM * 128;             // epilogue buffer: 128 rows of 128 bytes
-constexpr uint32_t OFF_BUF = STAGES * STAGE_BYTES;   // [2 groups][2]
-constexpr uint32_t OFF_VEC = OFF_BUF + 4 * BUF_BYTES;  // float[2 groups][bias 64, gate 64]
-constexpr uint32_t OFF_BAR = OFF_VEC + 2 * 128 * 4;
+constexpr uint32_t OFF_BUF = STAGES * STAGE_BYTES;           // [GROUPS]
+constexpr uint32_t OFF_VEC = OFF_BUF + GROUPS * BUF_BYTES;   // float[GROUPS][bias 64, gate 64]
+constexpr uint32_t OFF_BAR = OFF_VEC + GROUPS * 128 * 4;
 constexpr int B_FULL = 0, B_EMPTY = B_FULL + STAGES, B_ACCFULL = B_EMPTY + STAGES,
-              B_ACCEMPTY = B_ACCFULL + 2, B_RES = B_ACCEMPTY + 2 /* [2 groups][2] */,
-              B_DRAIN = B_RES + 4, NBAR = B_DRAIN + 1;
-constexpr uint32_t OFF_MISC = OFF_BAR + NBAR * 8;  // tmem base, abort flag, votes[2 groups][2][2][4]
-constexpr uint32_t SMEM_BYTES = OFF_MISC + 8 + 32 * 4 + 1024;  // and the way to a 1024-byte border
+              B_ACCEMPTY = B_ACCFULL + 2, B_RES = B_ACCEMPTY + 2 /* [GROUPS] */,
+              B_DRAIN = B_RES + GROUPS, NBAR = B_DRAIN + 1;
+constexpr uint32_t OFF_MISC = OFF_BAR + NBAR * 8;  // tmem base, abort flag, votes[GROUPS][2][2][4]
+constexpr uint32_t SMEM_BYTES = OFF_MISC + 8 + GROUPS * 16 * 4;
 static_assert(SMEM_BYTES <= 232448, "shared memory");
 
 struct Params {
@@ -312,9 +314,15 @@ __global__ void __launch_bounds__(THREADS, 1)
                    const __grid_constant__ CUtensorMap tm_res,
                    const __grid_constant__ CUtensorMap tm_z, const Params p) {
   constexpr int BN = 128 * CTA;  // columns of a tile; 128 of B's rows lie in each CTA
-  extern __shared__ unsigned char smem_raw[];
-  const uint32_t raw = smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
-  unsigned char* sbase = smem_raw + (base - raw);
+  extern __shared__ __align__(1024) unsigned char smem_raw[];
+  // the swizzle wants 1024-byte borders, where dynamic shared memory begins as long as there is no
+  // static one; there is no room to move up
+  const uint32_t base = smem_u32(smem_raw);
+  if (base & 1023u) {
+    if (threadIdx.x == 0 && p.status != nullptr) atomicOr(p.status, VGGT_STATUS_TIMEOUT);
+    return;
+  }
+  unsigned char* sbase = smem_raw;
   auto bar = [&](int i) { return base + OFF_BAR + 8u * (uint32_t)i; };
   uint32_t* misc = reinterpret_cast<uint32_t*>(sbase + OFF_MISC);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(misc + 1);
@@ -329,9 +337,9 @@ __global__ void __launch_bounds__(THREADS, 1)
     }
     for (int b = 0; b < 2; ++b) {
       tc::mbar_init(bar(B_ACCFULL + b), 1);
-      tc::mbar_init(bar(B_ACCEMPTY + b), 8 * CTA);
+      tc::mbar_init(bar(B_ACCEMPTY + b), 4 * GROUPS * CTA);
     }
-    for (int b = 0; b < 4; ++b) tc::mbar_init(bar(B_RES + b), 1);
+    for (int b = 0; b < GROUPS; ++b) tc::mbar_init(bar(B_RES + b), 1);
     tc::mbar_init(bar(B_DRAIN), 1);
     misc[1] = 0u;
     tc::mbar_fence_init();
@@ -453,195 +461,199 @@ __global__ void __launch_bounds__(THREADS, 1)
       }
     }
   } else if (warp >= 4) {
-    // ================= epilogue: groups of warps 4-7 and 8-11 =================
+    // ================= epilogue: group g takes columns 64 g .. 64 g + 63 of a tile =================
     const int g = (warp - 4) >> 2, sub = warp & 3, row = sub * 32 + lane, t = tid & 127;
     const uint32_t lanes = (uint32_t)(sub * 32) << 16;
     float* vec = reinterpret_cast<float*>(sbase + OFF_VEC) + g * 128;  // bias | gate
-    volatile int* votes = reinterpret_cast<volatile int*>(misc + 2) + g * 16;
-    const T* bias = static_cast<const T*>(p.bias);
-    const T* gate = static_cast<const T*>(p.gate);
+    int* votes = reinterpret_cast<int*>(misc + 2) + g * 16;
+    const uint32_t buf = base + OFF_BUF + (uint32_t)g * BUF_BYTES, res_bar = bar(B_RES + g);
     auto group_sync = [&] { asm volatile("bar.sync %0, 128;" ::"r"(1 + g) : "memory"); };
     // true in all four warps or in none: the barriers of a group are not bounded, so that its
     // warps have to leave together
-    auto agree = [&](int* slots4, bool ok) {
+    auto agree = [&](int at, bool ok) {
       const bool all = __all_sync(0xffffffffu, ok);
-      volatile int* v = slots4;
+      volatile int* v = votes + at;
       if (lane == 0) v[sub] = all ? 1 : 0;
       group_sync();
       return v[0] && v[1] && v[2] && v[3];
     };
     const bool has_res = !SPLIT && p.residual != nullptr, has_z = !SPLIT && p.z != nullptr;
+    auto fetch_residual = [&](int64_t c0, int64_t m0) {  // by one thread
+      store_wait_read<0>();  // the buffer's last store has read it
+      tc::mbar_expect_tx(res_bar, BUF_BYTES);
+      tc::tma_load_3d(buf, &tm_res, res_bar, (int)c0, (int)m0, 0);
+    };
     Walk w(p, worker);
-    uint32_t i = 0, uses = 0, res_uses[2] = {0, 0};
+    uint32_t i = 0, uses = 0, res_uses = 0;
     bool ok = true;
     while (ok && w.next()) {
       const uint32_t b = i & 1;
-      const int64_t m0 = w.tile / p.tiles_n * BN + rank * BM, n0 = w.tile % p.tiles_n * BN;
+      const int64_t m0 = w.tile / p.tiles_n * BN + rank * BM;
+      const int64_t col = w.tile % p.tiles_n * BN + g * 64;
+      const bool active = g < BN / 64 && col < p.n;
+      bool fetched = false;
+      if (!SPLIT && active) {
+        // seen by the group after the next barrier; the last readers are before the last one
+        const int64_t c = col + (t & 63);
+        float v = t < 64 ? 0.f : 1.f;
+        const T* src = static_cast<const T*>(t < 64 ? p.bias : p.gate);
+        if (src != nullptr && c < p.n) v = to_float(src[c]);
+        vec[t] = v;
+        fetched = has_res && p.res_tma && !has_z;
+        if (fetched && t == 0) fetch_residual(col, m0);
+        __syncwarp();
+      }
       const bool got = wait(bar(B_ACCFULL + b), (i >> 1) & 1, abort_flag, p.wait_ns);
-      if (!agree(const_cast<int*>(votes) + 4 * b, got)) {
+      if (!agree(4 * b, got)) {
         ok = false;
         break;
       }
       tc::tc_fence_after();
-      const uint32_t acc = tmem + b * BN + lanes;
-      for (int sc = g; ok && sc < BN / 64; sc += 2) {
-        const int64_t col = n0 + sc * 64;
-        if (col >= p.n) continue;
-        if (!SPLIT) {
-          // seen by the group after the next barrier; the last readers are before the last one
-          const int64_t c = col + (t & 63);
-          float v = t < 64 ? 0.f : 1.f;
-          const T* src = t < 64 ? bias : gate;
-          if (src != nullptr && c < p.n) v = to_float(src[c]);
-          vec[t] = v;
-        }
-        const int first = has_z ? kUseZ : SPLIT ? kUseSlot : kUseY;
-        for (int kind = first; ok && kind <= (SPLIT ? kUseSlot : kUseY); ++kind) {
-          // a buffer row is 64 elements of T or 32 of fp32
-          const bool wide = SPLIT || (kind == kUseY && p.y_fp32);
-          for (int part = 0; ok && part < (wide ? 2 : 1); ++part, ++uses) {
-            const int64_t c0 = col + part * 32;  // first column of the use
-            if (!SPLIT && c0 >= p.n) break;
-            const uint32_t u = uses & 1, buf = base + OFF_BUF + (uint32_t)(2 * g + u) * BUF_BYTES;
-            const bool res = kind == kUseY && has_res;
-            const int head = (int)(c0 / 64) / p.y_heads64;
-            const int in_head = (int)(c0 - (int64_t)head * p.y_heads64 * 64);
-            bool fine = true;
-            if (t == 0) store_wait_read<1>();  // the store before last, from this buffer
-            if (res && p.res_tma) {
-              if (t == 0) {
-                tc::mbar_expect_tx(bar(B_RES + 2 * g + u), BUF_BYTES);
-                tc::tma_load_3d(buf, &tm_res, bar(B_RES + 2 * g + u), (int)c0, (int)m0, 0);
-              }
-              __syncwarp();
-              fine = wait(bar(B_RES + 2 * g + u), res_uses[u] & 1, abort_flag, p.wait_ns);
-              ++res_uses[u];
+      const uint32_t acc = tmem + b * BN + lanes + g * 64;
+      const int first = has_z ? kUseZ : SPLIT ? kUseSlot : kUseY;
+      for (int kind = first; active && ok && kind <= (SPLIT ? kUseSlot : kUseY); ++kind) {
+        // a buffer row is 64 elements of T or 32 of fp32
+        const bool wide = SPLIT || (kind == kUseY && p.y_fp32);
+        for (int part = 0; part < (wide ? 2 : 1); ++part, ++uses) {
+          const int64_t c0 = col + part * 32;  // first column of the use
+          if (!SPLIT && c0 >= p.n) break;
+          const bool res = kind == kUseY && has_res;
+          bool fine = true;
+          if (res && p.res_tma) {
+            if (t == 0 && !fetched) fetch_residual(c0, m0);
+            fetched = false;
+            __syncwarp();
+            fine = wait(res_bar, res_uses & 1, abort_flag, p.wait_ns);
+            ++res_uses;
+          } else if (t == 0) {
+            store_wait_read<0>();
+          }
+          if (!agree(8 + 4 * (uses & 1), fine)) {
+            ok = false;
+            break;
+          }
+          const int64_t r0 = m0 + sub * 32, rows = p.m - r0, left = p.n - c0;  // this warp's rows
+          if (res && !p.res_tma) {
+            const int64_t at = r0 * p.residual_stride + c0;
+            if (p.y_fp32)
+              copy_rows(buf, sub * 32, const_cast<float*>(static_cast<const float*>(p.residual)) + at,
+                        p.residual_stride, rows, left, true);
+            else
+              copy_rows(buf, sub * 32, const_cast<T*>(static_cast<const T*>(p.residual)) + at,
+                        p.residual_stride, rows, left, true);
+            __syncwarp();
+          }
+          // 32 columns at a time: TMEM -> registers -> buffer
+          for (int h = wide ? part : 0; h < (wide ? part + 1 : 2); ++h) {
+            uint32_t r[32];
+            tc::tmem_ld32(acc + h * 32, r);
+            tc::tmem_wait_ld();
+            if (SPLIT) {
+#pragma unroll
+              for (int j = 0; j < 8; ++j)
+                sts128(piece(buf, row, j), r[4 * j], r[4 * j + 1], r[4 * j + 2], r[4 * j + 3]);
+              continue;
             }
-            if (!agree(const_cast<int*>(votes) + 8 + 4 * u, fine)) {
-              ok = false;
-              break;
+            const ulonglong2* bv = reinterpret_cast<const ulonglong2*>(vec + h * 32);
+            float_pair v[16];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              const ulonglong2 q = bv[j];
+              v[2 * j] = add_pair(
+                  pack_pair(__uint_as_float(r[4 * j]), __uint_as_float(r[4 * j + 1])), q.x);
+              v[2 * j + 1] = add_pair(
+                  pack_pair(__uint_as_float(r[4 * j + 2]), __uint_as_float(r[4 * j + 3])), q.y);
             }
-            if (res && !p.res_tma) {
-              const int64_t r0 = m0 + sub * 32;
-              if (p.y_fp32)
-                copy_rows(buf, sub * 32,
-                          const_cast<float*>(static_cast<const float*>(p.residual)) +
-                              r0 * p.residual_stride + c0,
-                          p.residual_stride, p.m - r0, p.n - c0, true);
-              else
-                copy_rows(buf, sub * 32,
-                          const_cast<T*>(static_cast<const T*>(p.residual)) +
-                              r0 * p.residual_stride + c0,
-                          p.residual_stride, p.m - r0, p.n - c0, true);
-              __syncwarp();
-            }
-            // 32 columns at a time: TMEM -> registers -> buffer
-            for (int h = wide ? part : 0; h < (wide ? part + 1 : 2); ++h) {
-              uint32_t r[32];
-              tc::tmem_ld32(acc + sc * 64 + h * 32, r);
-              tc::tmem_wait_ld();
-              if (SPLIT) {
+            if (kind == kUseY) {
+              act::dispatch(p.act, [&](auto k) {
 #pragma unroll
-                for (int j = 0; j < 8; ++j)
-                  sts128(piece(buf, row, j), r[4 * j], r[4 * j + 1], r[4 * j + 2], r[4 * j + 3]);
-                continue;
-              }
-              const float* bv = vec + h * 32;
-              float v[32];
-#pragma unroll
-              for (int j = 0; j < 8; ++j) {
-                const float4 q = reinterpret_cast<const float4*>(bv)[j];
-                v[4 * j] = __uint_as_float(r[4 * j]) + q.x;
-                v[4 * j + 1] = __uint_as_float(r[4 * j + 1]) + q.y;
-                v[4 * j + 2] = __uint_as_float(r[4 * j + 2]) + q.z;
-                v[4 * j + 3] = __uint_as_float(r[4 * j + 3]) + q.w;
-              }
-              if (kind == kUseY) {
-                act::dispatch(p.act, [&](auto k) {
-#pragma unroll
-                  for (int j = 0; j < 32; ++j) v[j] = act::value<decltype(k)::value>(v[j]);
-                });
-                if (gate != nullptr) {
-#pragma unroll
-                  for (int j = 0; j < 8; ++j) {
-                    const float4 q = reinterpret_cast<const float4*>(bv + 64)[j];
-                    v[4 * j] *= q.x;
-                    v[4 * j + 1] *= q.y;
-                    v[4 * j + 2] *= q.z;
-                    v[4 * j + 3] *= q.w;
-                  }
-                }
-              }
-              if (wide) {
+                for (int j = 0; j < 16; ++j) v[j] = act::value_pair<decltype(k)::value>(v[j]);
+              });
+              if (p.gate != nullptr) {
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
-                  const uint32_t a = piece(buf, row, j);
-                  if (res) {
-                    uint32_t q[4];
-                    lds128(a, q);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) v[4 * j + e] += __uint_as_float(q[e]);
-                  }
-                  sts128(a, __float_as_uint(v[4 * j]), __float_as_uint(v[4 * j + 1]),
-                         __float_as_uint(v[4 * j + 2]), __float_as_uint(v[4 * j + 3]));
-                }
-              } else {
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                  const uint32_t a = piece(buf, row, h * 4 + j);
-                  if (res) {
-                    uint32_t q[4];
-                    lds128(a, q);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                      const float2 f = ElemOps<T>::to_float2(q[e]);
-                      v[8 * j + 2 * e] += f.x;
-                      v[8 * j + 2 * e + 1] += f.y;
-                    }
-                  }
-                  sts128(a, ElemOps<T>::pack2(v[8 * j], v[8 * j + 1]),
-                         ElemOps<T>::pack2(v[8 * j + 2], v[8 * j + 3]),
-                         ElemOps<T>::pack2(v[8 * j + 4], v[8 * j + 5]),
-                         ElemOps<T>::pack2(v[8 * j + 6], v[8 * j + 7]));
+                  const ulonglong2 q = bv[16 + j];
+                  v[2 * j] = mul_pair(v[2 * j], q.x);
+                  v[2 * j + 1] = mul_pair(v[2 * j + 1], q.y);
                 }
               }
             }
-            const bool by_tma = SPLIT || (kind == kUseZ ? p.z_tma : p.y_tma);
-            if (by_tma) {
-              asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-              group_sync();
-              if (t == 0) {
-                if (SPLIT) {
-                  const int64_t slot = worker + w.tile;
-                  store_bulk(reinterpret_cast<unsigned char*>(p.slots) +
-                                 ((slot * CTA + rank) * (BN / 32) + sc * 2 + part) * BUF_BYTES,
-                             buf, BUF_BYTES);
-                } else if (m0 < p.m) {
-                  if (kind == kUseZ)
-                    store_3d(&tm_z, buf, (int)c0, (int)m0, 0);
-                  else
-                    store_3d(&tm_y, buf, in_head, (int)m0, head);
+            if (wide) {
+#pragma unroll
+              for (int j = 0; j < 8; ++j) {
+                const uint32_t a = piece(buf, row, j);
+                uint32_t q[4];
+                if (res) {
+                  lds128(a, q);
+                  v[2 * j] =
+                      add_pair(v[2 * j], pack_pair(__uint_as_float(q[0]), __uint_as_float(q[1])));
+                  v[2 * j + 1] = add_pair(v[2 * j + 1],
+                                          pack_pair(__uint_as_float(q[2]), __uint_as_float(q[3])));
                 }
-                store_commit();
+                float o[4];
+                unpack_pair(o[0], o[1], v[2 * j]);
+                unpack_pair(o[2], o[3], v[2 * j + 1]);
+                sts128(a, __float_as_uint(o[0]), __float_as_uint(o[1]), __float_as_uint(o[2]),
+                       __float_as_uint(o[3]));
               }
             } else {
-              __syncwarp();
-              const int64_t r0 = m0 + sub * 32, rows = p.m - r0, left = p.n - c0;
-              if (kind == kUseZ)
-                copy_rows(buf, sub * 32, static_cast<T*>(p.z) + r0 * p.z_stride + c0, p.z_stride,
-                          rows, left, false);
-              else if (p.y_fp32)
-                copy_rows(buf, sub * 32, static_cast<float*>(p.y) + r0 * p.y_stride + c0,
-                          p.y_stride, rows, left, false);
-              else
-                copy_rows(buf, sub * 32,
-                          static_cast<T*>(p.y) + head * p.y_head_stride + r0 * p.y_stride + in_head,
-                          p.y_stride, rows, left, false);
-              // the buffer's next use may begin with a copy by TMA
-              asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-              group_sync();
-              if (t == 0) store_commit();  // a group per use, this one empty
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                const uint32_t a = piece(buf, row, h * 4 + j);
+                uint32_t q[4];
+                if (res) {
+                  lds128(a, q);
+#pragma unroll
+                  for (int e = 0; e < 4; ++e) {
+                    const float2 f = ElemOps<T>::to_float2(q[e]);
+                    v[4 * j + e] = add_pair(v[4 * j + e], pack_pair(f.x, f.y));
+                  }
+                }
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                  float x0, x1;
+                  unpack_pair(x0, x1, v[4 * j + e]);
+                  q[e] = ElemOps<T>::pack2(x0, x1);
+                }
+                sts128(a, q[0], q[1], q[2], q[3]);
+              }
             }
+          }
+          if (SPLIT || (kind == kUseZ ? p.z_tma : p.y_tma)) {
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            group_sync();
+            if (t == 0) {
+              if (SPLIT) {
+                const int64_t slot = worker + w.tile;
+                store_bulk(reinterpret_cast<unsigned char*>(p.slots) +
+                               ((slot * CTA + rank) * (BN / 32) + g * 2 + part) * BUF_BYTES,
+                           buf, BUF_BYTES);
+              } else if (m0 < p.m) {
+                const int head = (int)(c0 / 64) / p.y_heads64;
+                if (kind == kUseZ)
+                  store_3d(&tm_z, buf, (int)c0, (int)m0, 0);
+                else
+                  store_3d(&tm_y, buf, (int)(c0 - (int64_t)head * p.y_heads64 * 64), (int)m0, head);
+              }
+              store_commit();
+            }
+          } else {
+            __syncwarp();
+            if (kind == kUseZ) {
+              copy_rows(buf, sub * 32, static_cast<T*>(p.z) + r0 * p.z_stride + c0, p.z_stride, rows,
+                        left, false);
+            } else if (p.y_fp32) {
+              copy_rows(buf, sub * 32, static_cast<float*>(p.y) + r0 * p.y_stride + c0, p.y_stride,
+                        rows, left, false);
+            } else {
+              const int64_t head = c0 / 64 / p.y_heads64, in_head = c0 - head * p.y_heads64 * 64;
+              copy_rows(buf, sub * 32,
+                        static_cast<T*>(p.y) + head * p.y_head_stride + r0 * p.y_stride + in_head,
+                        p.y_stride, rows, left, false);
+            }
+            // the buffer's next use may begin with a copy by TMA
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            group_sync();
           }
         }
       }
