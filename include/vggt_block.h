@@ -54,12 +54,14 @@ typedef struct vggt_vector {
  * y = residual + gate * activation(z)
  *
  * x [rows][inner], or with heads > 1 head-major: [heads][rows][inner / heads]
- * with x_head_stride between heads, inner / heads a multiple of 64, read as
- * [rows][inner].  weight [outer][inner], bias and gate [outer], x and z of
- * dtype (BF16 or FP16); residual and y [rows][outer] of stream_dtype, which is
- * dtype or FP32.  x and weight start on 16 bytes, with strides and inner
- * multiples of 8.  z [rows][outer], where non-NULL, gets the activation's
- * argument for the backward pass.  residual and y may be the same.
+ * with x_head_stride between heads, read as [rows][inner].  weight
+ * [outer][inner], bias and gate [outer], x and z of dtype (BF16 or FP16);
+ * residual and y [rows][outer] of stream_dtype, which is dtype or FP32.  z
+ * [rows][outer], where non-NULL, gets the activation's argument for the
+ * backward pass.  residual and y may be the same.
+ *
+ * x and weight are read in place where their rows (and heads, then of a multiple
+ * of 64 elements) start on 16 bytes, else copied into the workspace first.
  *
  * The workspace needs vggt_linear_workspace_size bytes (none: it may be NULL),
  * 256-byte aligned, and no clearing.
@@ -85,8 +87,9 @@ int vggt_linear(const vggt_linear_args* args, void* y, int64_t y_stride, void* z
                 int32_t* status, void* workspace, size_t workspace_bytes, void* stream);
 
 /*
- * Gradients of the above from that of y (dy, of stream_dtype): dx, like x (its
- * strides too are the caller's), dweight [outer][inner], dbias and dgate
+ * Gradients of the above from that of y (dy, of stream_dtype): dx [rows][inner]
+ * or, with dx_head_stride > 0, head-major like x (heads of a multiple of 64
+ * elements), dweight [outer][inner], dbias and dgate
  * [outer], all of dtype; that of residual is dy.  z is what vggt_linear wrote;
  * without an activation it is not needed.  Sums are formed in a fixed order.
  */

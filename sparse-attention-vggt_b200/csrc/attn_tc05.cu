@@ -916,6 +916,11 @@ bool encode_tmap_3d_sw128(CUtensorMap* map, const void* ptr, int dtype, int64_t 
 
 bool encode_tmap_sw128(CUtensorMap* map, const void* ptr, int dtype, int rank,
                        const uint64_t* dims, const uint64_t* strides, const uint32_t* box) {
+  return encode_tmap(map, ptr, dtype, rank, dims, strides, box, 128);
+}
+
+bool encode_tmap(CUtensorMap* map, const void* ptr, int dtype, int rank, const uint64_t* dims,
+                 const uint64_t* strides, const uint32_t* box, int swizzle) {
   tcattn::EncodeTiledFn fn = tcattn::encode_fn();
   if (!fn || rank < 1 || rank > 5) return false;
   cuuint64_t d[5], s[5];
@@ -930,7 +935,8 @@ bool encode_tmap_sw128(CUtensorMap* map, const void* ptr, int dtype, int rank,
                                  : dtype == VGGT_DTYPE_FP16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
                                                             : CU_TENSOR_MAP_DATA_TYPE_FLOAT32;
   return fn(map, dt, (cuuint32_t)rank, const_cast<void*>(ptr), d, s, b, estr,
-            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+            CU_TENSOR_MAP_INTERLEAVE_NONE,
+            swizzle == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 

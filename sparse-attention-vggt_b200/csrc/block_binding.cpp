@@ -6,7 +6,6 @@
 
 #include "binding.h"
 
-#include <ATen/ops/constant_pad_nd.h>
 #include <torch/csrc/Dtype.h>
 
 #include <initializer_list>
@@ -255,29 +254,12 @@ PyObject* residual_norm_grad(PyObject*, PyObject* const* o, Py_ssize_t n) {
 }
 
 // ---- linear -----------------------------------------------------------------------------------
-// An operand of a product: 16-byte rows, whose width is a multiple of 8 (zeros behind it).
-at::Tensor fit(const at::Tensor& t, int64_t width8, int64_t* stride) {
-  const int64_t width = t.size(1);
-  if (width8 != width) {
-    *stride = width8;
-    return at::constant_pad_nd(t, {0, width8 - width}, 0);
-  }
-  const bool one = t.size(0) <= 1;
-  if ((t.stride(1) == 1 || width == 1) && (one || (t.stride(0) % 8 == 0 && t.stride(0) >= width)) &&
-      reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0) {
-    *stride = one ? width : t.stride(0);
-    return t;
-  }
-  *stride = width;
-  return t.clone(at::MemoryFormat::Contiguous);
-}
-
 struct LinearCall {
   vggt_linear_args a{};
   at::Tensor x, weight, held[2];
   Rows residual;
   const at::Tensor *xt, *wt, *params[2], *rt;
-  int64_t inner = 0;     // x's own width (a.inner may have zeros behind it)
+  int64_t inner = 0;
   bool head_major = false;
   at::ScalarType type, stream;
 
@@ -329,24 +311,20 @@ struct LinearCall {
 
   // The tensors as the kernels take them (on the device that the caller has made current).
   void lay_out() {
-    a.inner = (inner + 7) / 8 * 8;
-    weight = fit(*wt, a.inner, &a.weight_stride);
-    a.weight = weight.data_ptr();
-    const bool heads = head_major && xt->size(0) > 1;
-    if (heads && xt->size(2) % 64 == 0) {
-      const int64_t dim = xt->size(2);
-      a.heads = xt->size(0);
-      x = *xt;
-      if (x.stride(2) != 1 || x.stride(0) % 8 || x.stride(0) < dim ||
-          (a.rows > 1 && (x.stride(1) % 8 || x.stride(1) < dim)) ||
-          reinterpret_cast<uintptr_t>(x.data_ptr()) % 16)
-        x = x.clone(at::MemoryFormat::Contiguous);
+    a.inner = inner;
+    const Rows w(*wt);
+    weight = w.t;
+    a.weight = w.data();
+    a.weight_stride = w.stride;
+    if (head_major && xt->size(0) > 1) {
+      x = xt->size(2) > 1 && xt->stride(2) != 1 ? xt->contiguous() : *xt;
+      a.heads = x.size(0);
       a.x_head_stride = x.stride(0);
-      a.x_stride = a.rows > 1 ? x.stride(1) : dim;
-    } else if (head_major) {
-      x = fit(xt->transpose(0, 1).reshape({a.rows, inner}), a.inner, &a.x_stride);
+      a.x_stride = a.rows > 1 ? x.stride(1) : x.size(2);
     } else {
-      x = fit(xt->dim() == 2 ? *xt : xt->reshape({a.rows, inner}), a.inner, &a.x_stride);
+      const Rows rows(head_major ? xt->squeeze(0) : *xt);
+      x = rows.t;
+      a.x_stride = rows.stride;
     }
     a.x = x.data_ptr();
     const void** to[2] = {&a.bias, &a.gate};
@@ -417,23 +395,25 @@ PyObject* linear_grad(PyObject*, PyObject* const* o, Py_ssize_t n) {
       g.z = rz.data();
       g.z_stride = rz.stride;
     }
-    const int64_t wide = c.a.inner;  // with the zeros behind the rows
     at::Tensor dx, dw, db, dg;
+    // a head-major dx whose heads do not end on 64 elements is turned round afterwards
+    const bool turn = c.a.heads > 1 && c.xt->size(2) % 64 != 0;
     if (wanted & 1) {
-      if (c.a.heads > 1) {
+      if (turn)
+        dx = at::empty({c.a.rows, c.inner}, c.xt->options());
+      else
         dx = at::empty(c.xt->sizes(), c.xt->options());
-        g.dx_head_stride = dx.stride(0);
-        g.dx_stride = dx.stride(1);
-      } else {
-        dx = at::empty({c.a.rows, wide}, c.xt->options());
-        g.dx_stride = wide;
+      g.dx_stride = c.inner;
+      if (c.a.heads > 1 && !turn) {
+        g.dx_head_stride = c.a.rows * c.xt->size(2);
+        g.dx_stride = c.xt->size(2);
       }
       g.dx = dx.data_ptr();
     }
     if (wanted & 2) {
-      dw = at::empty({c.a.outer, wide}, c.wt->options());
+      dw = at::empty({c.a.outer, c.inner}, c.wt->options());
       g.dweight = dw.data_ptr();
-      g.dweight_stride = wide;
+      g.dweight_stride = c.inner;
     }
     if ((wanted & 4) && c.params[0]) {
       db = at::empty({c.a.outer}, c.xt->options());
@@ -448,14 +428,8 @@ PyObject* linear_grad(PyObject*, PyObject* const* o, Py_ssize_t n) {
     if (bytes) ws = workspace(bytes, device);
     check(vggt_linear_grad(&c.a, &g, word, bytes ? ws.data_ptr() : nullptr, bytes,
                            c10::cuda::getCurrentCUDAStream().stream()));
-    if (dx.defined() && c.a.heads <= 1) {
-      if (wide != c.inner) dx = dx.narrow(1, 0, c.inner).contiguous();
-      if (c.head_major)
-        dx = dx.view({c.a.rows, c.xt->size(0), c.xt->size(2)}).transpose(0, 1).contiguous();
-      else
-        dx = dx.view(c.xt->sizes());
-    }
-    if (dw.defined() && wide != c.inner) dw = dw.narrow(1, 0, c.inner).contiguous();
+    if (dx.defined() && turn)
+      dx = dx.view({c.a.rows, c.xt->size(0), c.xt->size(2)}).transpose(0, 1).contiguous();
     return tuple_of({&dx, &dw, &db, &dg});
   });
 }

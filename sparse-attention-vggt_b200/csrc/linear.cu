@@ -28,28 +28,37 @@ namespace vggt {
 namespace lin {
 
 constexpr int BM = 128, BK = 64;
-constexpr int STAGES = 5;
 constexpr int GROUPS = 4;                     // warpgroups of the epilogue
 constexpr int THREADS = 128 + GROUPS * 128;
-constexpr uint32_t HALF_BYTES = BM * BK * 2;         // one operand's block: 16 KB
-constexpr uint32_t STAGE_BYTES = 2 * HALF_BYTES;
-constexpr uint32_t BUF_BYTES = BM * 128;             // epilogue buffer: 128 rows of 128 bytes
-constexpr uint32_t OFF_BUF = STAGES * STAGE_BYTES;           // [GROUPS]
-constexpr uint32_t OFF_VEC = OFF_BUF + GROUPS * BUF_BYTES;   // float[GROUPS][bias 64, gate 64]
-constexpr uint32_t OFF_BAR = OFF_VEC + GROUPS * 128 * 4;
-constexpr int B_FULL = 0, B_EMPTY = B_FULL + STAGES, B_ACCFULL = B_EMPTY + STAGES,
-              B_ACCEMPTY = B_ACCFULL + 2, B_RES = B_ACCEMPTY + 2 /* [GROUPS] */,
-              B_DRAIN = B_RES + GROUPS, NBAR = B_DRAIN + 1;
-constexpr uint32_t OFF_MISC = OFF_BAR + NBAR * 8;  // tmem base, abort flag, votes[GROUPS][2][2][4]
-constexpr uint32_t SMEM_BYTES = OFF_MISC + 8 + GROUPS * 16 * 4;
-static_assert(SMEM_BYTES <= 232448, "shared memory");
+constexpr uint32_t A_BYTES = BM * BK * 2;     // A's block: 16 KB
+constexpr uint32_t BUF_BYTES = BM * 128;      // epilogue buffer: 128 rows of up to 128 bytes
+
+// BNC of B's rows (columns of C) lie in each CTA.
+template <int CTA, int BNC>
+struct Shape {
+  static constexpr int BN = BNC * CTA;
+  static constexpr int COLS = BN / GROUPS > 32 ? BN / GROUPS : 32;  // of one epilogue group
+  static constexpr uint32_t B_BYTES = BNC * BK * 2, STAGE_BYTES = A_BYTES + B_BYTES;
+  static constexpr int STAGES = BNC == 128 ? 5 : 6;
+  static constexpr uint32_t TMEM_COLS = 2 * BN;                       // two accumulators
+  static constexpr uint32_t OFF_BUF = STAGES * STAGE_BYTES;           // [GROUPS]
+  static constexpr uint32_t OFF_VEC = OFF_BUF + GROUPS * BUF_BYTES;   // float[GROUPS][bias 64, gate 64]
+  static constexpr uint32_t OFF_BAR = OFF_VEC + GROUPS * 128 * 4;
+  static constexpr int B_FULL = 0, B_EMPTY = B_FULL + STAGES, B_ACCFULL = B_EMPTY + STAGES,
+                       B_ACCEMPTY = B_ACCFULL + 2, B_RES = B_ACCEMPTY + 2 /* [GROUPS] */,
+                       B_DRAIN = B_RES + GROUPS, NBAR = B_DRAIN + 1;
+  // tmem base, abort flag, votes[GROUPS][2][4]
+  static constexpr uint32_t OFF_MISC = OFF_BAR + NBAR * 8;
+  static constexpr uint32_t SMEM_BYTES = OFF_MISC + 8 + GROUPS * 8 * 4;
+  static_assert(SMEM_BYTES <= 232448 && TMEM_COLS <= 512, "shared memory and TMEM");
+};
 
 struct Params {
   int64_t m, n;
-  int64_t tiles, tiles_n;
-  int blocks;   // reduction blocks of a tile
-  int workers;
-  int split;
+  uint32_t tiles, tiles_n;
+  uint32_t blocks;     // reduction blocks of a tile
+  uint32_t workers;
+  uint32_t per, rest;  // of a split product, see Slots
   int a_heads64, b_heads64, y_heads64;  // 64-element pieces of a row in one head
   const void* bias;
   const void* gate;
@@ -67,37 +76,32 @@ struct Params {
   int wait_selftest;
 };
 
-// A worker's next piece of work: reduction blocks [k0, k1) of a tile.
+// A worker's next piece of work: reduction blocks [k0, k1) of tile (tm, tn).
+template <bool SPLIT>
 struct Walk {
-  int64_t at, end, step;
-  int blocks;
-  bool split;
-  int64_t tile;
+  const Params& p;
+  uint32_t at, end;
+  uint32_t tile, tm, tn;
   int k0, k1;
-  __device__ __forceinline__ Walk(const Params& p, int worker) : blocks(p.blocks), split(p.split) {
-    if (split) {
-      const int64_t units = p.tiles * p.blocks;
-      at = worker * units / p.workers;
-      end = (worker + 1) * units / p.workers;
-    } else {
-      at = worker;
-      end = p.tiles;
-      step = p.workers;
-    }
+  __device__ __forceinline__ Walk(const Params& params, uint32_t worker) : p(params) {
+    at = SPLIT ? worker * p.per + min(worker, p.rest) : worker;
+    end = SPLIT ? at + p.per + (worker < p.rest ? 1 : 0) : p.tiles;
   }
   __device__ __forceinline__ bool next() {
     if (at >= end) return false;
-    if (split) {
-      tile = at / blocks;
-      k0 = (int)(at - tile * blocks);
-      k1 = (int)min((int64_t)blocks, k0 + (end - at));
+    if (SPLIT) {
+      tile = at / p.blocks;
+      k0 = (int)(at - tile * p.blocks);
+      k1 = (int)min(p.blocks, k0 + (end - at));
       at += k1 - k0;
     } else {
       tile = at;
       k0 = 0;
-      k1 = blocks;
-      at += step;
+      k1 = (int)p.blocks;
+      at += p.workers;
     }
+    tm = tile / p.tiles_n;
+    tn = tile - tm * p.tiles_n;
     return true;
   }
 };
@@ -138,17 +142,16 @@ __device__ __forceinline__ uint32_t map_rank(uint32_t addr, uint32_t rank) {
   return r;
 }
 __device__ __forceinline__ void arrive_cluster(uint32_t bar) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar)
-               : "memory");
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 
 template <int CTA>
 struct Pair;
 template <>
 struct Pair<1> {
-  static __device__ __forceinline__ void alloc(uint32_t dst) { tc::tmem_alloc(dst, 256); }
+  static __device__ __forceinline__ void alloc(uint32_t dst, uint32_t n) { tc::tmem_alloc(dst, n); }
   static __device__ __forceinline__ void relinquish() { tc::tmem_relinquish(); }
-  static __device__ __forceinline__ void dealloc(uint32_t t) { tc::tmem_dealloc(t, 256); }
+  static __device__ __forceinline__ void dealloc(uint32_t t, uint32_t n) { tc::tmem_dealloc(t, n); }
   static __device__ __forceinline__ void load(uint32_t dst, const CUtensorMap* map, uint32_t bar,
                                               int c0, int c1, int c2) {
     tc::tma_load_3d(dst, map, bar, c0, c1, c2);
@@ -161,15 +164,16 @@ struct Pair<1> {
 };
 template <>
 struct Pair<2> {
-  static __device__ __forceinline__ void alloc(uint32_t dst) {
-    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(dst)
+  static __device__ __forceinline__ void alloc(uint32_t dst, uint32_t n) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(dst),
+                 "r"(n)
                  : "memory");
   }
   static __device__ __forceinline__ void relinquish() {
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
   }
-  static __device__ __forceinline__ void dealloc(uint32_t t) {
-    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(t) : "memory");
+  static __device__ __forceinline__ void dealloc(uint32_t t, uint32_t n) {
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(t), "r"(n) : "memory");
   }
   // into this CTA's memory, completion on a barrier of either CTA of the pair
   static __device__ __forceinline__ void load(uint32_t dst, const CUtensorMap* map, uint32_t bar,
@@ -234,24 +238,27 @@ __device__ __forceinline__ float to_float(E v) {
   return (float)v;
 }
 
-// Address of 16-byte piece j of row r in an epilogue buffer (the 128-byte swizzle of TMA).
+// Address of 16-byte piece j of row r in an epilogue buffer with rows of 128 or 64 bytes (TMA's
+// swizzle of that many bytes).
+template <int ROW>
 __device__ __forceinline__ uint32_t piece(uint32_t buf, int r, int j) {
+  if (ROW == 64) return buf + (uint32_t)(r * 64 + ((j ^ ((r >> 1) & 3)) << 4));
   return buf + (uint32_t)(r * 128 + ((j ^ (r & 7)) << 4));
 }
 
-// Copies this warp's 32 rows between an epilogue buffer and memory, element by element: 128 bytes
+// Copies this warp's 32 rows between an epilogue buffer and memory, element by element: ROW bytes
 // of a row, `left` elements of which exist, in the first `rows` rows.
-template <typename E>
+template <int ROW, typename E>
 __device__ __forceinline__ void copy_rows(uint32_t buf, int row0, E* g, int64_t stride, int64_t rows,
                                           int64_t left, bool in) {
-  constexpr int kPer = 128 / (int)sizeof(E) / 32, kPiece = 16 / (int)sizeof(E);
+  constexpr int kAll = ROW / (int)sizeof(E), kPiece = 16 / (int)sizeof(E);
   const int lane = threadIdx.x & 31;
   for (int r = 0; r < 32 && r < rows; ++r) {
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-      const int c = lane * kPer + i;
+    for (int i = 0; i < kAll / 32; ++i) {
+      const int c = lane + i * 32;
       if (c >= left) continue;
-      const uint32_t a = piece(buf, row0 + r, c / kPiece) + (uint32_t)(c % kPiece) * sizeof(E);
+      const uint32_t a = piece<ROW>(buf, row0 + r, c / kPiece) + (uint32_t)(c % kPiece) * sizeof(E);
       E* p = g + (int64_t)r * stride + c;
       if (sizeof(E) == 2) {
         uint16_t v;
@@ -277,6 +284,7 @@ __device__ __forceinline__ void copy_rows(uint32_t buf, int row0, E* g, int64_t 
 }
 
 // The stage that comes next and the parity of its round.
+template <int STAGES>
 struct Ring {
   uint32_t at = 0, turn = 0;
   __device__ __forceinline__ void step() {
@@ -297,55 +305,56 @@ struct Place {
   }
   __device__ __forceinline__ void step(int per) {
     x += 64;
-    if (per != INT_MAX && x == per * 64) {
+    if (x == per * 64) {
       x = 0;
       ++head;
     }
   }
 };
 
-// What one use of an epilogue buffer holds.
-enum { kUseZ, kUseY, kUseSlot };
-
-template <typename T, int CTA, bool AMN, bool BMN, bool SPLIT>
+template <typename T, int CTA, int BNC, bool AMN, bool BMN, bool SPLIT>
 __global__ void __launch_bounds__(THREADS, 1)
     product_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b,
                    const __grid_constant__ CUtensorMap tm_y,
                    const __grid_constant__ CUtensorMap tm_res,
                    const __grid_constant__ CUtensorMap tm_z, const Params p) {
-  constexpr int BN = 128 * CTA;  // columns of a tile; 128 of B's rows lie in each CTA
-  extern __shared__ __align__(1024) unsigned char smem_raw[];
+  typedef Shape<CTA, BNC> SH;
+  constexpr int BN = SH::BN, STAGES = SH::STAGES, COLS = SH::COLS;
+  constexpr uint32_t STAGE_BYTES = SH::STAGE_BYTES;
+  extern __shared__ __align__(1024) unsigned char smem[];
   // the swizzle wants 1024-byte borders, where dynamic shared memory begins as long as there is no
   // static one; there is no room to move up
-  const uint32_t base = smem_u32(smem_raw);
+  const uint32_t base = smem_u32(smem);
   if (base & 1023u) {
     if (threadIdx.x == 0 && p.status != nullptr) atomicOr(p.status, VGGT_STATUS_TIMEOUT);
     return;
   }
-  unsigned char* sbase = smem_raw;
-  auto bar = [&](int i) { return base + OFF_BAR + 8u * (uint32_t)i; };
-  uint32_t* misc = reinterpret_cast<uint32_t*>(sbase + OFF_MISC);
+  auto bar = [&](int i) { return base + SH::OFF_BAR + 8u * (uint32_t)i; };
+  uint32_t* misc = reinterpret_cast<uint32_t*>(smem + SH::OFF_MISC);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(misc + 1);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int rank = CTA == 2 ? (int)cluster_rank() : 0;
-  const int worker = (int)blockIdx.x / CTA;
+  const uint32_t worker = blockIdx.x / CTA;
 
   if (tid == 0) {
+    tc::prefetch_tmap(&tm_a);
+    tc::prefetch_tmap(&tm_b);
+    if (!SPLIT) tc::prefetch_tmap(&tm_y);
     for (int s = 0; s < STAGES; ++s) {
-      tc::mbar_init(bar(B_FULL + s), 1);
-      tc::mbar_init(bar(B_EMPTY + s), 1);
+      tc::mbar_init(bar(SH::B_FULL + s), 1);
+      tc::mbar_init(bar(SH::B_EMPTY + s), 1);
     }
     for (int b = 0; b < 2; ++b) {
-      tc::mbar_init(bar(B_ACCFULL + b), 1);
-      tc::mbar_init(bar(B_ACCEMPTY + b), 4 * GROUPS * CTA);
+      tc::mbar_init(bar(SH::B_ACCFULL + b), 1);
+      tc::mbar_init(bar(SH::B_ACCEMPTY + b), 4 * GROUPS * CTA);
     }
-    for (int b = 0; b < GROUPS; ++b) tc::mbar_init(bar(B_RES + b), 1);
-    tc::mbar_init(bar(B_DRAIN), 1);
+    for (int b = 0; b < GROUPS; ++b) tc::mbar_init(bar(SH::B_RES + b), 1);
+    tc::mbar_init(bar(SH::B_DRAIN), 1);
     misc[1] = 0u;
     tc::mbar_fence_init();
   }
   if (warp == 2) {
-    Pair<CTA>::alloc(base + OFF_MISC);
+    Pair<CTA>::alloc(base + SH::OFF_MISC, SH::TMEM_COLS);
     Pair<CTA>::relinquish();
   }
   tc::tc_fence_before();
@@ -353,20 +362,22 @@ __global__ void __launch_bounds__(THREADS, 1)
   if (CTA == 2) cluster_sync();
   tc::tc_fence_after();
   const uint32_t tmem = misc[0];
+  // Up to here the kernel may run beside the end of the one before it in the stream, from here on
+  // it has that one's results; the next one may begin its own preparations.
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
   if (warp == 0) {
     // ================= TMA producer =================
     if (lane == 0) {
-      const uint32_t full0 = CTA == 2 ? map_rank(bar(B_FULL), 0) : bar(B_FULL);
-      tc::prefetch_tmap(&tm_a);
-      tc::prefetch_tmap(&tm_b);
-      Walk w(p, worker);
-      Ring ring;
+      const uint32_t full0 = CTA == 2 ? map_rank(bar(SH::B_FULL), 0) : bar(SH::B_FULL);
+      Walk<SPLIT> w(p, worker);
+      Ring<STAGES> ring;
       uint32_t issued = 0;
       bool ok = true;
       while (ok && w.next()) {
-        const int m0 = (int)(w.tile / p.tiles_n) * BN + rank * BM;
-        const int n0 = (int)(w.tile % p.tiles_n) * BN + rank * BM;
+        const int m0 = (int)w.tm * (BM * CTA) + rank * BM;
+        const int n0 = (int)w.tn * BN + rank * BNC;
         // where the operands' first blocks lie: one thread feeds the tensor core here, so that
         // no division is left in the loop
         Place a0, a1, b0, b1;
@@ -378,30 +389,30 @@ __global__ void __launch_bounds__(THREADS, 1)
         }
         if (BMN) {
           b0 = Place(n0 / 64, p.b_heads64);
-          b1 = Place(n0 / 64 + 1, p.b_heads64);
+          if (BNC == 128) b1 = Place(n0 / 64 + 1, p.b_heads64);
         } else {
           b0 = Place(w.k0, p.b_heads64);
         }
         for (int k = w.k0; k < w.k1; ++k) {
           if (issued >= STAGES &&
-              !wait(bar(B_EMPTY) + 8 * ring.at, ring.turn ^ 1, abort_flag, p.wait_ns)) {
+              !wait(bar(SH::B_EMPTY) + 8 * ring.at, ring.turn ^ 1, abort_flag, p.wait_ns)) {
             ok = false;
             break;
           }
           // the barrier is the first CTA's: it counts both CTAs' bytes
           const uint32_t full = full0 + 8 * ring.at;
-          if (rank == 0) tc::mbar_expect_tx(bar(B_FULL) + 8 * ring.at, CTA * STAGE_BYTES);
-          const uint32_t a = base + ring.at * STAGE_BYTES, b = a + HALF_BYTES;
+          if (rank == 0) tc::mbar_expect_tx(bar(SH::B_FULL) + 8 * ring.at, CTA * STAGE_BYTES);
+          const uint32_t a = base + ring.at * STAGE_BYTES, b = a + A_BYTES;
           if (AMN) {
             Pair<CTA>::load(a, &tm_a, full, a0.x, k * BK, a0.head);
-            Pair<CTA>::load(a + HALF_BYTES / 2, &tm_a, full, a1.x, k * BK, a1.head);
+            Pair<CTA>::load(a + A_BYTES / 2, &tm_a, full, a1.x, k * BK, a1.head);
           } else {
             Pair<CTA>::load(a, &tm_a, full, a0.x, m0, a0.head);
             a0.step(p.a_heads64);
           }
           if (BMN) {
             Pair<CTA>::load(b, &tm_b, full, b0.x, k * BK, b0.head);
-            Pair<CTA>::load(b + HALF_BYTES / 2, &tm_b, full, b1.x, k * BK, b1.head);
+            if (BNC == 128) Pair<CTA>::load(b + A_BYTES / 2, &tm_b, full, b1.x, k * BK, b1.head);
           } else {
             Pair<CTA>::load(b, &tm_b, full, b0.x, n0, b0.head);
             b0.step(p.b_heads64);
@@ -414,147 +425,152 @@ __global__ void __launch_bounds__(THREADS, 1)
       // by their issuer)
       if (rank == 0)
         for (uint32_t t = issued > STAGES ? issued - STAGES : 0; t < issued; ++t)
-          tc::mbar_wait_drain(bar(B_FULL + t % STAGES), (t / STAGES) & 1, p.wait_ns);
+          tc::mbar_wait_drain(bar(SH::B_FULL + t % STAGES), (t / STAGES) & 1, p.wait_ns);
     }
   } else if (warp == 1) {
     // ================= MMA issuer (of the pair's first CTA) =================
     if (lane == 0 && rank == 0) {
       const uint32_t fmt = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
-      const uint32_t idesc = tc::idesc_f16(fmt, BMN ? 1u : 0u, BN, BN) | (AMN ? 1u << 15 : 0u);
+      const uint32_t idesc =
+          tc::idesc_f16(fmt, BMN ? 1u : 0u, BM * CTA, BN) | (AMN ? 1u << 15 : 0u);
       // a step of 16 reduced elements: 32 bytes along a K-major row, 16 MN-major rows
       constexpr uint64_t kStepA = AMN ? 16 * 128 / 16 : 2, kStepB = BMN ? 16 * 128 / 16 : 2;
-      const uint64_t desc0 = tc::sw128_desc(base, HALF_BYTES / 2);
+      const uint64_t desc0 = tc::sw128_desc(base, A_BYTES / 2);
       bool ok = true;
-      if (p.wait_selftest) ok = wait(bar(B_DRAIN), 0, abort_flag, p.wait_ns);
-      Walk w(p, worker);
-      Ring ring;
+      if (p.wait_selftest) ok = wait(bar(SH::B_DRAIN), 0, abort_flag, p.wait_ns);
+      Walk<SPLIT> w(p, worker);
+      Ring<STAGES> ring;
       uint32_t i = 0;
       while (ok && w.next()) {
         const uint32_t b = i & 1;
         if (i >= 2 &&
-            !wait(bar(B_ACCEMPTY + b), ((i >> 1) + 1) & 1, abort_flag, p.wait_ns)) {
+            !wait(bar(SH::B_ACCEMPTY + b), ((i >> 1) + 1) & 1, abort_flag, p.wait_ns)) {
           ok = false;
           break;
         }
         tc::tc_fence_after();
         const uint32_t acc = tmem + b * BN;
         for (int k = w.k0; k < w.k1; ++k) {
-          if (!wait(bar(B_FULL) + 8 * ring.at, ring.turn, abort_flag, p.wait_ns)) {
+          if (!wait(bar(SH::B_FULL) + 8 * ring.at, ring.turn, abort_flag, p.wait_ns)) {
             ok = false;
             break;
           }
           tc::tc_fence_after();
-          const uint64_t ad = desc0 + ring.at * (STAGE_BYTES / 16), bd = ad + HALF_BYTES / 16;
+          const uint64_t ad = desc0 + ring.at * (STAGE_BYTES / 16), bd = ad + A_BYTES / 16;
 #pragma unroll
           for (int kk = 0; kk < BK / 16; ++kk)
             Pair<CTA>::mma(acc, ad + kk * kStepA, bd + kk * kStepB, idesc,
                            (k > w.k0 || kk > 0) ? 1u : 0u);
-          Pair<CTA>::commit(bar(B_EMPTY) + 8 * ring.at);
+          Pair<CTA>::commit(bar(SH::B_EMPTY) + 8 * ring.at);
           ring.step();
         }
-        if (ok) Pair<CTA>::commit(bar(B_ACCFULL + b));
+        if (ok) Pair<CTA>::commit(bar(SH::B_ACCFULL + b));
         ++i;
       }
       if (!p.wait_selftest) {
-        Pair<CTA>::commit(bar(B_DRAIN));
-        tc::mbar_wait_drain(bar(B_DRAIN), 0, p.wait_ns);
+        Pair<CTA>::commit(bar(SH::B_DRAIN));
+        tc::mbar_wait_drain(bar(SH::B_DRAIN), 0, p.wait_ns);
       }
     }
   } else if (warp >= 4) {
-    // ================= epilogue: group g takes columns 64 g .. 64 g + 63 of a tile =================
+    // ================= epilogue: group g takes COLS columns of a tile =================
     const int g = (warp - 4) >> 2, sub = warp & 3, row = sub * 32 + lane, t = tid & 127;
-    const uint32_t lanes = (uint32_t)(sub * 32) << 16;
-    float* vec = reinterpret_cast<float*>(sbase + OFF_VEC) + g * 128;  // bias | gate
-    int* votes = reinterpret_cast<int*>(misc + 2) + g * 16;
-    const uint32_t buf = base + OFF_BUF + (uint32_t)g * BUF_BYTES, res_bar = bar(B_RES + g);
+    float* vec = reinterpret_cast<float*>(smem + SH::OFF_VEC) + g * 128;  // bias | gate
+    int* votes = reinterpret_cast<int*>(misc + 2) + g * 8;
+    const uint32_t buf = base + SH::OFF_BUF + (uint32_t)g * BUF_BYTES, res_bar = bar(SH::B_RES + g);
     auto group_sync = [&] { asm volatile("bar.sync %0, 128;" ::"r"(1 + g) : "memory"); };
+    uint32_t turns = 0;
     // true in all four warps or in none: the barriers of a group are not bounded, so that its
     // warps have to leave together
-    auto agree = [&](int at, bool ok) {
+    auto agree = [&](bool ok) {
       const bool all = __all_sync(0xffffffffu, ok);
-      volatile int* v = votes + at;
+      volatile int* v = votes + 4 * (turns++ & 1);
       if (lane == 0) v[sub] = all ? 1 : 0;
       group_sync();
       return v[0] && v[1] && v[2] && v[3];
     };
     const bool has_res = !SPLIT && p.residual != nullptr, has_z = !SPLIT && p.z != nullptr;
-    auto fetch_residual = [&](int64_t c0, int64_t m0) {  // by one thread
-      store_wait_read<0>();  // the buffer's last store has read it
-      tc::mbar_expect_tx(res_bar, BUF_BYTES);
-      tc::tma_load_3d(buf, &tm_res, res_bar, (int)c0, (int)m0, 0);
-    };
-    Walk w(p, worker);
-    uint32_t i = 0, uses = 0, res_uses = 0;
+    // a use of the buffer: COLS elements of T or 32 of fp32 in a row
+    const bool y_wide = SPLIT || p.y_fp32;
+    uint32_t i = 0, res_uses = 0;
     bool ok = true;
+    Walk<SPLIT> w(p, worker);
     while (ok && w.next()) {
       const uint32_t b = i & 1;
-      const int64_t m0 = w.tile / p.tiles_n * BN + rank * BM;
-      const int64_t col = w.tile % p.tiles_n * BN + g * 64;
-      const bool active = g < BN / 64 && col < p.n;
-      bool fetched = false;
-      if (!SPLIT && active) {
-        // seen by the group after the next barrier; the last readers are before the last one
-        const int64_t c = col + (t & 63);
-        float v = t < 64 ? 0.f : 1.f;
-        const T* src = static_cast<const T*>(t < 64 ? p.bias : p.gate);
-        if (src != nullptr && c < p.n) v = to_float(src[c]);
-        vec[t] = v;
-        fetched = has_res && p.res_tma && !has_z;
-        if (fetched && t == 0) fetch_residual(col, m0);
+      const int m0 = (int)w.tm * (BM * CTA) + rank * BM, col = (int)w.tn * BN + g * COLS;
+      const bool active = g < BN / COLS && col < p.n;
+      const int r0 = m0 + sub * 32;  // this warp's first row
+      const int64_t rows = p.m - r0;
+      // the buffer is free once its last store has read it; the residual comes into it
+      auto open = [&](int c0, bool residual) {
+        if (t == 0) {
+          store_wait_read<0>();
+          if (residual && p.res_tma) {
+            constexpr uint32_t narrow = BM * COLS * 2;
+            tc::mbar_expect_tx(res_bar, y_wide ? BUF_BYTES : narrow);
+            tc::tma_load_3d(buf, &tm_res, res_bar, c0, m0, 0);
+          }
+        }
         __syncwarp();
+      };
+      if (active) {
+        if (!SPLIT) {
+          // seen by the group after the next barrier; the last readers are before the last one
+          const int c = col + (t & 63);
+          float v = t < 64 ? 0.f : 1.f;
+          const T* src = static_cast<const T*>(t < 64 ? p.bias : p.gate);
+          if (src != nullptr && (t & 63) < COLS && c < p.n) v = to_float(src[c]);
+          vec[t] = v;
+        }
+        open(col, has_res && !has_z);
       }
-      const bool got = wait(bar(B_ACCFULL + b), (i >> 1) & 1, abort_flag, p.wait_ns);
-      if (!agree(4 * b, got)) {
+      if (!agree(wait(bar(SH::B_ACCFULL + b), (i >> 1) & 1, abort_flag, p.wait_ns))) {
         ok = false;
         break;
       }
       tc::tc_fence_after();
-      const uint32_t acc = tmem + b * BN + lanes + g * 64;
-      const int first = has_z ? kUseZ : SPLIT ? kUseSlot : kUseY;
-      for (int kind = first; active && ok && kind <= (SPLIT ? kUseSlot : kUseY); ++kind) {
-        // a buffer row is 64 elements of T or 32 of fp32
-        const bool wide = SPLIT || (kind == kUseY && p.y_fp32);
-        for (int part = 0; part < (wide ? 2 : 1); ++part, ++uses) {
-          const int64_t c0 = col + part * 32;  // first column of the use
+      const uint32_t acc = tmem + b * BN + ((uint32_t)(sub * 32) << 16) + g * COLS;
+      bool opened = true;
+      for (int which = has_z ? 0 : 1; active && ok && which < 2; ++which) {  // z, then y
+        const bool wide = which == 1 && y_wide, res = which == 1 && has_res;
+        for (int c = 0; c < COLS; c += wide ? 32 : COLS) {
+          const int c0 = col + c;  // first column of the use
           if (!SPLIT && c0 >= p.n) break;
-          const bool res = kind == kUseY && has_res;
-          bool fine = true;
-          if (res && p.res_tma) {
-            if (t == 0 && !fetched) fetch_residual(c0, m0);
-            fetched = false;
-            __syncwarp();
-            fine = wait(res_bar, res_uses & 1, abort_flag, p.wait_ns);
-            ++res_uses;
-          } else if (t == 0) {
-            store_wait_read<0>();
+          if (!opened) open(c0, res);
+          const int64_t left = p.n - c0;
+          if (!opened || (res && p.res_tma)) {
+            const bool fine = !(res && p.res_tma) ||
+                              wait(res_bar, res_uses++ & 1, abort_flag, p.wait_ns);
+            if (!agree(fine)) {
+              ok = false;
+              break;
+            }
           }
-          if (!agree(8 + 4 * (uses & 1), fine)) {
-            ok = false;
-            break;
-          }
-          const int64_t r0 = m0 + sub * 32, rows = p.m - r0, left = p.n - c0;  // this warp's rows
+          opened = false;
           if (res && !p.res_tma) {
-            const int64_t at = r0 * p.residual_stride + c0;
-            if (p.y_fp32)
-              copy_rows(buf, sub * 32, const_cast<float*>(static_cast<const float*>(p.residual)) + at,
-                        p.residual_stride, rows, left, true);
+            const int64_t at = (int64_t)r0 * p.residual_stride + c0;
+            if (wide)
+              copy_rows<128>(buf, sub * 32,
+                             const_cast<float*>(static_cast<const float*>(p.residual)) + at,
+                             p.residual_stride, rows, left, true);
             else
-              copy_rows(buf, sub * 32, const_cast<T*>(static_cast<const T*>(p.residual)) + at,
-                        p.residual_stride, rows, left, true);
+              copy_rows<COLS * 2>(buf, sub * 32,
+                                  const_cast<T*>(static_cast<const T*>(p.residual)) + at,
+                                  p.residual_stride, rows, left, true);
             __syncwarp();
           }
           // 32 columns at a time: TMEM -> registers -> buffer
-          for (int h = wide ? part : 0; h < (wide ? part + 1 : 2); ++h) {
+          for (int h = c; h < (wide ? c + 32 : COLS); h += 32) {
             uint32_t r[32];
-            tc::tmem_ld32(acc + h * 32, r);
+            tc::tmem_ld32(acc + h, r);
             tc::tmem_wait_ld();
             if (SPLIT) {
 #pragma unroll
               for (int j = 0; j < 8; ++j)
-                sts128(piece(buf, row, j), r[4 * j], r[4 * j + 1], r[4 * j + 2], r[4 * j + 3]);
+                sts128(piece<128>(buf, row, j), r[4 * j], r[4 * j + 1], r[4 * j + 2], r[4 * j + 3]);
               continue;
             }
-            const ulonglong2* bv = reinterpret_cast<const ulonglong2*>(vec + h * 32);
+            const ulonglong2* bv = reinterpret_cast<const ulonglong2*>(vec + h);
             float_pair v[16];
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
@@ -564,11 +580,12 @@ __global__ void __launch_bounds__(THREADS, 1)
               v[2 * j + 1] = add_pair(
                   pack_pair(__uint_as_float(r[4 * j + 2]), __uint_as_float(r[4 * j + 3])), q.y);
             }
-            if (kind == kUseY) {
-              act::dispatch(p.act, [&](auto k) {
+            if (which == 1) {
+              if (p.act != VGGT_ACT_NONE)
+                act::dispatch(p.act, [&](auto k) {
 #pragma unroll
-                for (int j = 0; j < 16; ++j) v[j] = act::value_pair<decltype(k)::value>(v[j]);
-              });
+                  for (int j = 0; j < 16; ++j) v[j] = act::value_pair<decltype(k)::value>(v[j]);
+                });
               if (p.gate != nullptr) {
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
@@ -581,7 +598,7 @@ __global__ void __launch_bounds__(THREADS, 1)
             if (wide) {
 #pragma unroll
               for (int j = 0; j < 8; ++j) {
-                const uint32_t a = piece(buf, row, j);
+                const uint32_t a = piece<128>(buf, row, j);
                 uint32_t q[4];
                 if (res) {
                   lds128(a, q);
@@ -599,7 +616,7 @@ __global__ void __launch_bounds__(THREADS, 1)
             } else {
 #pragma unroll
               for (int j = 0; j < 4; ++j) {
-                const uint32_t a = piece(buf, row, h * 4 + j);
+                const uint32_t a = piece<COLS * 2>(buf, row, h / 8 + j);
                 uint32_t q[4];
                 if (res) {
                   lds128(a, q);
@@ -619,37 +636,41 @@ __global__ void __launch_bounds__(THREADS, 1)
               }
             }
           }
-          if (SPLIT || (kind == kUseZ ? p.z_tma : p.y_tma)) {
+          if (SPLIT || (which == 0 ? p.z_tma : p.y_tma)) {
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             group_sync();
             if (t == 0) {
               if (SPLIT) {
-                const int64_t slot = worker + w.tile;
+                const int64_t slot = (int64_t)worker + w.tile;
                 store_bulk(reinterpret_cast<unsigned char*>(p.slots) +
-                               ((slot * CTA + rank) * (BN / 32) + g * 2 + part) * BUF_BYTES,
+                               ((slot * CTA + rank) * (BN / 32) + (g * COLS + c) / 32) * BUF_BYTES,
                            buf, BUF_BYTES);
               } else if (m0 < p.m) {
-                const int head = (int)(c0 / 64) / p.y_heads64;
-                if (kind == kUseZ)
-                  store_3d(&tm_z, buf, (int)c0, (int)m0, 0);
-                else
-                  store_3d(&tm_y, buf, (int)(c0 - (int64_t)head * p.y_heads64 * 64), (int)m0, head);
+                if (which == 0) {
+                  store_3d(&tm_z, buf, c0, m0, 0);
+                } else {
+                  const int head = c0 / 64 / p.y_heads64;
+                  store_3d(&tm_y, buf, c0 - head * p.y_heads64 * 64, m0, head);
+                }
               }
               store_commit();
             }
           } else {
             __syncwarp();
-            if (kind == kUseZ) {
-              copy_rows(buf, sub * 32, static_cast<T*>(p.z) + r0 * p.z_stride + c0, p.z_stride, rows,
-                        left, false);
-            } else if (p.y_fp32) {
-              copy_rows(buf, sub * 32, static_cast<float*>(p.y) + r0 * p.y_stride + c0, p.y_stride,
-                        rows, left, false);
+            if (which == 0) {
+              copy_rows<COLS * 2>(buf, sub * 32,
+                                  static_cast<T*>(p.z) + (int64_t)r0 * p.z_stride + c0, p.z_stride,
+                                  rows, left, false);
+            } else if (wide) {
+              copy_rows<128>(buf, sub * 32,
+                             static_cast<float*>(p.y) + (int64_t)r0 * p.y_stride + c0, p.y_stride,
+                             rows, left, false);
             } else {
-              const int64_t head = c0 / 64 / p.y_heads64, in_head = c0 - head * p.y_heads64 * 64;
-              copy_rows(buf, sub * 32,
-                        static_cast<T*>(p.y) + head * p.y_head_stride + r0 * p.y_stride + in_head,
-                        p.y_stride, rows, left, false);
+              const int head = c0 / 64 / p.y_heads64;
+              copy_rows<COLS * 2>(buf, sub * 32,
+                                  static_cast<T*>(p.y) + head * p.y_head_stride +
+                                      (int64_t)r0 * p.y_stride + (c0 - head * p.y_heads64 * 64),
+                                  p.y_stride, rows, left, false);
             }
             // the buffer's next use may begin with a copy by TMA
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -662,13 +683,13 @@ __global__ void __launch_bounds__(THREADS, 1)
       __syncwarp();
       if (lane == 0) {
         if (CTA == 2)
-          arrive_cluster(map_rank(bar(B_ACCEMPTY + b), 0));
+          arrive_cluster(map_rank(bar(SH::B_ACCEMPTY + b), 0));
         else
-          tc::mbar_arrive(bar(B_ACCEMPTY + b));
+          tc::mbar_arrive(bar(SH::B_ACCEMPTY + b));
       }
       ++i;
     }
-    if (t == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+    if (t == 0) store_wait_read<0>();  // the memory outlives the stores' reads of it
   }
 
   tc::tc_fence_before();
@@ -677,7 +698,7 @@ __global__ void __launch_bounds__(THREADS, 1)
   if (CTA == 2) cluster_sync();
   tc::tc_fence_after();
   if (tid == 0 && *abort_flag && p.status != nullptr) atomicOr(p.status, VGGT_STATUS_TIMEOUT);
-  if (warp == 2) Pair<CTA>::dealloc(tmem);
+  if (warp == 2) Pair<CTA>::dealloc(tmem, SH::TMEM_COLS);
 }
 
 // Adds up a split product's partial sums and runs the epilogue: a thread takes 8 columns of a row.
@@ -728,7 +749,7 @@ __global__ void __launch_bounds__(256)
 
 // ---- host -------------------------------------------------------------------------------------
 size_t Plan::slot_bytes() const {
-  return split ? (size_t)(workers + tiles_m * tiles_n) * cta * cta * BM * 128 * 4 : 0;
+  return split ? (size_t)(workers + tiles_m * tiles_n) * cta * BM * (bnc * cta) * 4 : 0;
 }
 
 static int sm_count() {
@@ -736,28 +757,29 @@ static int sm_count() {
   return device_sms(&sms) == cudaSuccess && sms > 0 ? sms : 148;
 }
 
-// The way a product is cut is the one of the least estimated time, in SM cycles: a reduction block
-// takes a pair of CTAs 512 cycles (the MMAs' time) and a single CTA 256, or up to twice that when
-// all SMs read their operands from L2 at once.  Splitting evens the load out where tiles are few
-// or the last round is short, at the price of partial sums through memory and another launch.
+// The way a product is cut is the one of the least estimated time, in SM cycles.  A reduction block
+// takes as long as its bytes take through shared memory, written once and read once at 128 B a
+// cycle (measured 525 cycles for the 32 KB of a 128 x 128 or of half a 256 x 256 tile): the larger
+// tile does four times the work in that.  A launch and a tile's epilogue cost about 8,000 cycles.
+// Splitting evens the load out where tiles are few or the last round is short, at the price of
+// partial sums through memory and another launch.
 Plan plan_product(int64_t m, int64_t n, int64_t red, bool must_split) {
+  static const int kShapes[][2] = {{1, 64}, {1, 128}, {2, 64}, {2, 128}};  // cta, bnc
   const int sms = sm_count();
   Plan best;
   double least = 0;
-  for (int cta = 1; cta <= 2; ++cta)
+  for (const int* shape : kShapes)
     for (int split = must_split ? 1 : 0; split < 2; ++split) {
       Plan p;
-      p.cta = cta;
+      p.cta = shape[0];
+      p.bnc = shape[1];
       p.split = split;
-      p.tiles_m = (m + 128 * cta - 1) / (128 * cta);
-      p.tiles_n = (n + 128 * cta - 1) / (128 * cta);
+      p.tiles_m = (m + BM * p.cta - 1) / (BM * p.cta);
+      p.tiles_n = (n + p.bnc * p.cta - 1) / (p.bnc * p.cta);
       p.blocks = (red + BK - 1) / BK;
-      const int64_t tiles = p.tiles_m * p.tiles_n, units = split ? tiles * p.blocks : tiles;
-      p.workers = (int)std::min<int64_t>(sms / cta, units);
-      const double busy = (double)p.workers * cta / sms;
-      const double block = cta == 2 ? 512 : 256 * std::max(1.0, 2 * busy);
-      const int64_t rounds = (units + p.workers - 1) / p.workers;
-      double t = (double)rounds * (split ? 1 : p.blocks) * block;
+      p.workers = (int)std::min<int64_t>(sms / p.cta, p.units());
+      const int64_t rounds = (p.units() + p.workers - 1) / p.workers;
+      double t = (double)rounds * (split ? 1 : p.blocks) * (p.bnc + BM) * 2.05 + p.bnc * p.cta * 10;
       if (split) t += 5000 + (double)p.slot_bytes() * 2 / 2500;
       if (least == 0 || t < least) {
         least = t;
@@ -769,82 +791,97 @@ Plan plan_product(int64_t m, int64_t n, int64_t red, bool must_split) {
 
 static bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
-static bool operand_map(CUtensorMap* map, const Operand& o, int dtype, int64_t rows) {
+static bool operand_map(CUtensorMap* map, const Operand& o, int dtype, int64_t rows, int box_rows) {
   const uint64_t dims[3] = {(uint64_t)o.dim, (uint64_t)rows, (uint64_t)o.heads};
   // a stride that is never used may be anything: give a valid one
   const int64_t row = rows > 1 ? o.stride : (o.dim + 7) / 8 * 8;
   const uint64_t strides[2] = {(uint64_t)row * 2,
                                (uint64_t)(o.heads > 1 ? o.head_stride : row * rows) * 2};
-  const uint32_t box[3] = {64, o.mn_major ? (uint32_t)BK : (uint32_t)BM, 1};
+  const uint32_t box[3] = {64, o.mn_major ? (uint32_t)BK : (uint32_t)box_rows, 1};
   return encode_tmap_sw128(map, o.p, dtype, 3, dims, strides, box);
 }
 
-// Rows of an output or of the residual, for copies of 128 rows x 128 bytes; false where TMA
+// Rows of an output or of the residual, for copies of 128 rows of `cols` elements; false where TMA
 // cannot address them.
 static bool rows_map(CUtensorMap* map, const void* p, int type, int64_t stride, int64_t head_stride,
-                     int64_t heads, int64_t dim, int64_t rows) {
+                     int64_t heads, int64_t dim, int64_t rows, int cols) {
   const int per = type == VGGT_DTYPE_FP32 ? 4 : 8, size = 16 / per;
-  if (!aligned16(p) || dim % per || (rows > 1 && stride % per) || (heads > 1 && head_stride % per))
+  if (!aligned16(p) || dim % per || (rows > 1 && (stride % per || stride < dim)) ||
+      (heads > 1 && (head_stride % per || head_stride < dim)))
     return false;
   const int64_t row = rows > 1 ? stride : dim;
   const uint64_t dims[3] = {(uint64_t)dim, (uint64_t)rows, (uint64_t)heads};
   const uint64_t strides[2] = {(uint64_t)row * size,
                                (uint64_t)(heads > 1 ? head_stride : row * rows) * size};
-  const uint32_t box[3] = {(uint32_t)(128 / size), (uint32_t)BM, 1};
-  return encode_tmap_sw128(map, p, type, 3, dims, strides, box);
+  const uint32_t box[3] = {(uint32_t)cols, (uint32_t)BM, 1};
+  return encode_tmap(map, p, type, 3, dims, strides, box, cols * size);
 }
 
-template <typename T, int CTA, bool AMN, bool BMN, bool SPLIT>
+template <typename T, int CTA, int BNC, bool AMN, bool BMN, bool SPLIT>
 static cudaError_t launch_kernel(const CUtensorMap* maps, const Params& p, cudaStream_t stream) {
-  auto k = product_kernel<T, CTA, AMN, BMN, SPLIT>;
-  cudaError_t e =
-      cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SMEM_BYTES);
+  auto k = product_kernel<T, CTA, BNC, AMN, BMN, SPLIT>;
+  constexpr int smem = (int)Shape<CTA, BNC>::SMEM_BYTES;
+  cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)(p.workers * CTA));
   cfg.blockDim = dim3(THREADS);
-  cfg.dynamicSmemBytes = SMEM_BYTES;
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = CTA;
-  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = CTA;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = CTA == 2 ? 2 : 1;
   e = cudaLaunchKernelEx(&cfg, k, maps[0], maps[1], maps[2], maps[3], maps[4], p);
   return e != cudaSuccess ? e : cudaGetLastError();
 }
 
-template <typename T, int CTA>
+template <typename T, int CTA, int BNC>
 static cudaError_t launch_majors(bool amn, bool bmn, bool split, const CUtensorMap* maps,
                                  const Params& p, cudaStream_t stream) {
   if (!amn && !bmn)
-    return split ? launch_kernel<T, CTA, false, false, true>(maps, p, stream)
-                 : launch_kernel<T, CTA, false, false, false>(maps, p, stream);
+    return split ? launch_kernel<T, CTA, BNC, false, false, true>(maps, p, stream)
+                 : launch_kernel<T, CTA, BNC, false, false, false>(maps, p, stream);
   if (!amn)
-    return split ? launch_kernel<T, CTA, false, true, true>(maps, p, stream)
-                 : launch_kernel<T, CTA, false, true, false>(maps, p, stream);
+    return split ? launch_kernel<T, CTA, BNC, false, true, true>(maps, p, stream)
+                 : launch_kernel<T, CTA, BNC, false, true, false>(maps, p, stream);
   // the weight's gradient is always split
-  return split && bmn ? launch_kernel<T, CTA, true, true, true>(maps, p, stream)
+  return split && bmn ? launch_kernel<T, CTA, BNC, true, true, true>(maps, p, stream)
                       : cudaErrorInvalidValue;
+}
+
+template <typename T>
+static cudaError_t launch_shapes(const Plan& plan, bool amn, bool bmn, const CUtensorMap* maps,
+                                 const Params& p, cudaStream_t stream) {
+  const bool s = plan.split;
+  if (plan.cta == 2)
+    return plan.bnc == 128 ? launch_majors<T, 2, 128>(amn, bmn, s, maps, p, stream)
+                           : launch_majors<T, 2, 64>(amn, bmn, s, maps, p, stream);
+  return plan.bnc == 128 ? launch_majors<T, 1, 128>(amn, bmn, s, maps, p, stream)
+                         : launch_majors<T, 1, 64>(amn, bmn, s, maps, p, stream);
 }
 
 cudaError_t launch_product(const Plan& plan, int dtype, int64_t m, int64_t n, int64_t red,
                            const Operand& a, const Operand& b, const Epilogue& e, float* slots,
                            int32_t* status, cudaStream_t stream) {
   CUtensorMap maps[5] = {};
-  if (!operand_map(&maps[0], a, dtype, a.mn_major ? red : m) ||
-      !operand_map(&maps[1], b, dtype, b.mn_major ? red : n))
+  if (!operand_map(&maps[0], a, dtype, a.mn_major ? red : m, BM) ||
+      !operand_map(&maps[1], b, dtype, b.mn_major ? red : n, plan.bnc))
     return cudaErrorInvalidValue;
   Params p{};
   p.m = m;
   p.n = n;
-  p.tiles = plan.tiles_m * plan.tiles_n;
-  p.tiles_n = plan.tiles_n;
-  p.blocks = (int)plan.blocks;
-  p.workers = plan.workers;
-  p.split = plan.split;
-  auto heads64 = [](int64_t heads, int64_t dim) { return heads > 1 ? (int)(dim / 64) : INT_MAX; };
+  p.tiles = (uint32_t)(plan.tiles_m * plan.tiles_n);
+  p.tiles_n = (uint32_t)plan.tiles_n;
+  p.blocks = (uint32_t)plan.blocks;
+  p.workers = (uint32_t)plan.workers;
+  p.per = (uint32_t)(plan.units() / plan.workers);
+  p.rest = (uint32_t)(plan.units() % plan.workers);
+  auto heads64 = [](int64_t heads, int64_t dim) { return heads > 1 ? (int)(dim / 64) : INT_MAX / 64; };
   p.a_heads64 = heads64(a.heads, a.dim);
   p.b_heads64 = heads64(b.heads, b.dim);
   p.y_heads64 = heads64(e.y_heads, e.y_dim);
@@ -860,26 +897,26 @@ cudaError_t launch_product(const Plan& plan, int dtype, int64_t m, int64_t n, in
   p.z = e.z;
   p.z_stride = e.z_stride;
   if (!plan.split) {
-    p.y_tma = rows_map(&maps[2], e.y, e.y_type, e.y_stride, e.y_head_stride, e.y_heads, e.y_dim, m);
-    p.res_tma = e.residual &&
-                rows_map(&maps[3], e.residual, e.y_type, e.residual_stride, 0, 1, n, m);
-    p.z_tma = e.z && rows_map(&maps[4], e.z, dtype, e.z_stride, 0, 1, n, m);
+    // columns of a buffer's row, as the kernel's Shape has them
+    const int cols = std::max(plan.bnc * plan.cta / GROUPS, 32), y_cols = p.y_fp32 ? 32 : cols;
+    p.y_tma = rows_map(&maps[2], e.y, e.y_type, e.y_stride, e.y_head_stride, e.y_heads, e.y_dim, m,
+                       y_cols);
+    p.res_tma = e.residual && rows_map(&maps[3], e.residual, e.y_type, e.residual_stride, 0, 1, n, m,
+                                       y_cols);
+    p.z_tma = e.z && rows_map(&maps[4], e.z, dtype, e.z_stride, 0, 1, n, m, cols);
   }
   p.slots = slots;
   p.status = status;
   p.wait_ns = api_wait_ns();
   p.wait_selftest = api_wait_selftest();
-  const bool am = a.mn_major, bm = b.mn_major;
-  if (dtype == VGGT_DTYPE_BF16)
-    return plan.cta == 2 ? launch_majors<__nv_bfloat16, 2>(am, bm, plan.split, maps, p, stream)
-                         : launch_majors<__nv_bfloat16, 1>(am, bm, plan.split, maps, p, stream);
-  return plan.cta == 2 ? launch_majors<__half, 2>(am, bm, plan.split, maps, p, stream)
-                       : launch_majors<__half, 1>(am, bm, plan.split, maps, p, stream);
+  return dtype == VGGT_DTYPE_BF16
+             ? launch_shapes<__nv_bfloat16>(plan, a.mn_major, b.mn_major, maps, p, stream)
+             : launch_shapes<__half>(plan, a.mn_major, b.mn_major, maps, p, stream);
 }
 
 Slots slots_of(const Plan& plan, const float* p) {
-  return {p, plan.tiles_m * plan.tiles_n * plan.blocks, plan.tiles_n, plan.cta, (int)plan.blocks,
-          plan.workers};
+  return {p, (uint32_t)plan.tiles_n, (uint32_t)plan.blocks, (uint32_t)(plan.units() / plan.workers),
+          (uint32_t)(plan.units() % plan.workers), plan.cta, plan.bnc * plan.cta};
 }
 
 cudaError_t finish_product(const Plan& plan, int dtype, int64_t m, int64_t n, const Epilogue& e,
@@ -899,6 +936,91 @@ cudaError_t finish_product(const Plan& plan, int dtype, int64_t m, int64_t n, co
   return cudaGetLastError();
 }
 
+// ---- operands that TMA cannot address ----------------------------------------------------------
+struct Copy {
+  const uint16_t* from;
+  uint16_t* to;
+  int64_t rows, width, pad, stride, head_stride, dim;
+};
+
+__global__ void __launch_bounds__(256) copy_operand_kernel(const Copy c) {
+  const int64_t all = c.rows * c.pad;
+  for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < all;
+       i += (int64_t)gridDim.x * blockDim.x) {
+    const int64_t r = i / c.pad, k = i - r * c.pad, head = k / c.dim;
+    c.to[i] = k < c.width ? c.from[head * c.head_stride + r * c.stride + (k - head * c.dim)] : 0;
+  }
+}
+
+Laid plan_operands(const vggt_linear_args* a, bool need_x, bool need_w) {
+  Laid l{};
+  const int64_t heads = a->heads > 1 ? a->heads : 1, dim = a->inner / heads;
+  auto rows_fit = [](const void* p, int64_t rows, int64_t stride, int64_t width) {
+    return aligned16(p) && (rows <= 1 || (stride % 8 == 0 && stride >= width));
+  };
+  l.copy_x = need_x && !(rows_fit(a->x, a->rows, a->x_stride, dim) &&
+                         (heads == 1 || (dim % 64 == 0 && a->x_head_stride % 8 == 0 &&
+                                         a->x_head_stride >= dim)));
+  l.copy_w = need_w && !rows_fit(a->weight, a->outer, a->weight_stride, a->inner);
+  l.pad = (a->inner + 7) / 8 * 8;
+  auto take = [&](bool need, int64_t rows) {
+    const size_t at = l.bytes;
+    if (need) l.bytes += ((size_t)rows * l.pad * 2 + 255) / 256 * 256;
+    return at;
+  };
+  l.x_at = take(l.copy_x, a->rows);
+  l.w_at = take(l.copy_w, a->outer);
+  return l;
+}
+
+cudaError_t copy_operands(const vggt_linear_args* a, const Laid& l, unsigned char* ws,
+                          cudaStream_t stream) {
+  const int64_t heads = a->heads > 1 ? a->heads : 1;
+  for (int which = 0; which < 2; ++which) {
+    if (!(which == 0 ? l.copy_x : l.copy_w)) continue;
+    Copy c;
+    c.from = static_cast<const uint16_t*>(which == 0 ? a->x : a->weight);
+    c.to = reinterpret_cast<uint16_t*>(ws + (which == 0 ? l.x_at : l.w_at));
+    c.rows = which == 0 ? a->rows : a->outer;
+    c.width = a->inner;
+    c.pad = l.pad;
+    c.stride = which == 0 ? a->x_stride : a->weight_stride;
+    c.head_stride = a->x_head_stride;
+    c.dim = which == 0 ? a->inner / heads : l.pad;
+    if (c.dim == a->inner) c.dim = l.pad;  // one head
+    const int64_t all = c.rows * c.pad;
+    copy_operand_kernel<<<(unsigned)std::min<int64_t>((all + 255) / 256, 148 * 16), 256, 0,
+                          stream>>>(c);
+    if (cudaError_t e = cudaGetLastError()) return e;
+  }
+  return cudaSuccess;
+}
+
+Operand matrix(const void* p, int64_t width, int64_t stride, bool mn_major) {
+  Operand o;
+  o.p = p;
+  o.stride = stride;
+  o.dim = width;
+  o.mn_major = mn_major;
+  return o;
+}
+
+Operand x_operand(const vggt_linear_args* a, const Laid& l, const unsigned char* ws, bool mn_major) {
+  if (l.copy_x) return matrix(ws + l.x_at, a->inner, l.pad, mn_major);
+  Operand o = matrix(a->x, a->inner, a->x_stride, mn_major);
+  if (a->heads > 1) {
+    o.heads = a->heads;
+    o.head_stride = a->x_head_stride;
+    o.dim = a->inner / a->heads;
+  }
+  return o;
+}
+
+Operand w_operand(const vggt_linear_args* a, const Laid& l, const unsigned char* ws, bool mn_major) {
+  return l.copy_w ? matrix(ws + l.w_at, a->inner, l.pad, mn_major)
+                  : matrix(a->weight, a->inner, a->weight_stride, mn_major);
+}
+
 }  // namespace lin
 }  // namespace vggt
 
@@ -915,43 +1037,21 @@ int check(const vggt_linear_args* a) {
   if (a->rows < 0 || a->inner < 1 || a->outer < 1) return api_fail("bad size argument");
   if (a->rows > INT_MAX - 512 || a->inner > INT_MAX - 512 || a->outer > INT_MAX - 512)
     return api_fail("too many rows or too wide");
-  if (a->inner % 8) return api_fail("inner (%lld) must be a multiple of 8", (long long)a->inner);
-  if (a->heads > 1 && (a->inner % a->heads || a->inner / a->heads % 64))
-    return api_fail("a head-major x needs heads of a multiple of 64 elements");
+  if (a->heads > 1 && a->inner % a->heads)
+    return api_fail("inner (%lld) must be a multiple of heads (%lld)", (long long)a->inner,
+                    (long long)a->heads);
   if (a->activation < VGGT_ACT_NONE || a->activation > VGGT_ACT_RELU)
     return api_fail("unknown activation %d", a->activation);
   if (a->rows == 0) return 0;
   if (!a->x || !a->weight) return api_fail("x and weight must be non-NULL");
-  const int64_t dim = a->heads > 1 ? a->inner / a->heads : a->inner;
-  if (!aligned16(a->x) || !aligned16(a->weight) || (a->rows > 1 && a->x_stride % 8) ||
-      (a->heads > 1 && a->x_head_stride % 8) || (a->outer > 1 && a->weight_stride % 8))
-    return api_fail("x and weight must start on 16 bytes, with strides that are multiples of 8");
-  if ((a->rows > 1 && a->x_stride < dim) || (a->heads > 1 && a->x_head_stride < dim) ||
-      (a->outer > 1 && a->weight_stride < a->inner))
-    return api_fail("a stride of x or weight is below the row's width");
+  if ((a->rows > 1 && a->x_stride < 0) || (a->heads > 1 && a->x_head_stride < 0) ||
+      (a->outer > 1 && a->weight_stride < 0))
+    return api_fail("negative stride");
+  if ((a->rows + 127) / 128 * ((a->outer + 63) / 64) * ((a->inner + 63) / 64) > INT_MAX ||
+      (a->outer + 127) / 128 * ((a->inner + 63) / 64) * ((a->rows + 63) / 64) > INT_MAX)
+    return api_fail("the product is too large");
   if (a->residual && a->rows > 1 && a->residual_stride < 0) return api_fail("negative stride");
   return 0;
-}
-
-Operand x_operand(const vggt_linear_args* a, bool mn_major) {
-  const int64_t heads = a->heads > 1 ? a->heads : 1;
-  Operand o;
-  o.p = a->x;
-  o.stride = a->x_stride;
-  o.head_stride = a->x_head_stride;
-  o.heads = heads;
-  o.dim = a->inner / heads;
-  o.mn_major = mn_major;
-  return o;
-}
-
-Operand matrix(const void* p, int64_t width, int64_t stride, bool mn_major) {
-  Operand o;
-  o.p = p;
-  o.stride = stride;
-  o.dim = width;
-  o.mn_major = mn_major;
-  return o;
 }
 
 }  // namespace lin
@@ -960,7 +1060,8 @@ Operand matrix(const void* p, int64_t width, int64_t stride, bool mn_major) {
 extern "C" size_t vggt_linear_workspace_size(const vggt_linear_args* a) {
   using namespace vggt::lin;
   if (!a || a->rows <= 0 || a->inner < 1 || a->outer < 1) return 0;
-  return plan_product(a->rows, a->outer, a->inner, false).slot_bytes();
+  return plan_operands(a, true, true).bytes +
+         plan_product(a->rows, a->outer, a->inner, false).slot_bytes();
 }
 
 extern "C" int vggt_linear(const vggt_linear_args* a, void* y, int64_t y_stride, void* z,
@@ -973,10 +1074,12 @@ extern "C" int vggt_linear(const vggt_linear_args* a, void* y, int64_t y_stride,
   if (!y) return api_fail("y must be non-NULL");
   if (a->rows > 1 && (y_stride < a->outer || (z && z_stride < a->outer)))
     return api_fail("an output's rows overlap: its stride is below outer");
+  const Laid laid = plan_operands(a, true, true);
   const Plan plan = plan_product(a->rows, a->outer, a->inner, false);
-  if (plan.slot_bytes() > 0 &&
-      (!workspace || !aligned16(workspace) || workspace_bytes < plan.slot_bytes()))
-    return api_fail("the workspace is too small or not 16-byte aligned");
+  const size_t bytes = laid.bytes + plan.slot_bytes();
+  if (bytes > 0 && (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 255u) ||
+                    workspace_bytes < bytes))
+    return api_fail("the workspace is too small or not 256-byte aligned");
   Epilogue e;
   e.bias = a->bias;
   e.gate = a->gate;
@@ -990,10 +1093,12 @@ extern "C" int vggt_linear(const vggt_linear_args* a, void* y, int64_t y_stride,
   e.z = z;
   e.z_stride = z_stride;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
-  float* slots = static_cast<float*>(workspace);
-  cudaError_t rc = launch_product(plan, a->dtype, a->rows, a->outer, a->inner, x_operand(a, false),
-                                  matrix(a->weight, a->inner, a->weight_stride, false), e, slots,
-                                  status, st);
+  unsigned char* ws = static_cast<unsigned char*>(workspace);
+  float* slots = reinterpret_cast<float*>(ws + laid.bytes);
+  cudaError_t rc = copy_operands(a, laid, ws, st);
+  if (rc == cudaSuccess)
+    rc = launch_product(plan, a->dtype, a->rows, a->outer, a->inner, x_operand(a, laid, ws, false),
+                        w_operand(a, laid, ws, false), e, slots, status, st);
   if (rc == cudaSuccess && plan.split)
     rc = finish_product(plan, a->dtype, a->rows, a->outer, e, slots, st);
   return api_cuda(rc);

@@ -36,39 +36,38 @@ struct Epilogue {
   int64_t z_stride = 0;
 };
 
-// How a product is cut: tiles of 128 cta x 128 cta, worked on by `workers` groups of cta CTAs,
-// whole (split 0), or as equal runs of the tiles' reduction blocks (split 1).
+// How a product is cut: tiles of 128 cta x bnc cta (cta CTAs work on one), dealt out whole to
+// `workers` groups of CTAs (split 0), or as equal runs of the tiles' reduction blocks (split 1).
 struct Plan {
-  int cta = 1, split = 0, workers = 1;
+  int cta = 1, bnc = 128, split = 0, workers = 1;
   int64_t tiles_m = 0, tiles_n = 0, blocks = 0;  // blocks: of 64 reduced elements
+  int64_t units() const { return tiles_m * tiles_n * (split ? blocks : 1); }
   size_t slot_bytes() const;                     // partial sums of a split product
 };
 
 Plan plan_product(int64_t m, int64_t n, int64_t red, bool must_split);
 
-// A split product's partial sums.  Tile t's reduction blocks [t blocks, (t + 1) blocks) of all lie with the workers that begin at
-// or before them; worker w's part is slot w + t.
+// A split product's partial sums.  All tiles' reduction blocks, one tile after the other, are dealt
+// out in runs: the first `rest` workers take per + 1 of them, the others per.  Worker w's part of
+// tile t is slot w + t: per CTA 32-column pieces of 128 rows, in the epilogue buffers' layout.
 struct Slots {
   const float* p;
-  int64_t units;
-  int64_t tiles_n;
-  int cta, blocks, workers;
-  __device__ __forceinline__ int first(int64_t tile) const {
-    return (int)(((tile * blocks + 1) * workers - 1) / units);
-  }
-  __device__ __forceinline__ int last(int64_t tile) const {
-    return (int)(((tile + 1) * blocks * workers - 1) / units);
+  uint32_t tiles_n, blocks, per, rest;
+  int cta, bn;
+  __device__ __forceinline__ uint32_t worker_of(uint32_t unit) const {
+    const uint32_t border = rest * (per + 1);
+    return unit < border ? unit / (per + 1) : rest + (unit - border) / per;
   }
   // the sums at row r, columns c .. c + 8, c a multiple of 8
   __device__ __forceinline__ void get8(int64_t r, int64_t c, float* v) const {
-    const int bn = 128 * cta;
-    const int64_t tm = r / bn, tn = c / bn, tile = tm * tiles_n + tn;
-    const int rank = (int)(r - tm * bn) / 128, row = (int)(r & 127), in = (int)(c - tn * bn);
+    const uint32_t bm = 128 * cta;
+    const uint32_t tm = (uint32_t)r / bm, tn = (uint32_t)c / bn, tile = tm * tiles_n + tn;
+    const uint32_t rank = ((uint32_t)r - tm * bm) / 128, row = (uint32_t)r & 127, in = (uint32_t)c - tn * bn;
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = 0.f;
-    const int j = (in & 31) / 4;
-    for (int w = first(tile), e = last(tile); w <= e; ++w) {
-      const float* q = p + (((w + tile) * cta + rank) * (bn / 32) + in / 32) * (128 * 32) + row * 32;
+    const uint32_t j = (in & 31) / 4;
+    for (uint32_t w = worker_of(tile * blocks), e = worker_of((tile + 1) * blocks - 1); w <= e; ++w) {
+      const float* q = p + (((int64_t)(w + tile) * cta + rank) * (bn / 32) + in / 32) * (128 * 32) + row * 32;
       const float4 a = *reinterpret_cast<const float4*>(q + ((j ^ (row & 7)) << 2));
       const float4 b = *reinterpret_cast<const float4*>(q + (((j + 1) ^ (row & 7)) << 2));
       v[0] += a.x, v[1] += a.y, v[2] += a.z, v[3] += a.w;
@@ -76,7 +75,6 @@ struct Slots {
     }
   }
 };
-
 Slots slots_of(const Plan& plan, const float* p);
 
 // Launches the product; with plan.split the partial sums go to `slots` and finish_product or
@@ -89,8 +87,21 @@ cudaError_t finish_product(const Plan& plan, int dtype, int64_t m, int64_t n, co
 
 // Argument checks (0, or the error) and operands of a call.
 int check(const vggt_linear_args* a);
-Operand x_operand(const vggt_linear_args* a, bool mn_major);
 Operand matrix(const void* p, int64_t width, int64_t stride, bool mn_major);
+
+// x and weight as the kernels read them: in place, or copied into rows that start on 16 bytes.
+struct Laid {
+  bool copy_x, copy_w;
+  int64_t pad;  // row stride of the copies
+  size_t x_at, w_at, bytes;
+};
+Laid plan_operands(const vggt_linear_args* a, bool need_x, bool need_w);
+cudaError_t copy_operands(const vggt_linear_args* a, const Laid& l, unsigned char* workspace,
+                          cudaStream_t stream);
+Operand x_operand(const vggt_linear_args* a, const Laid& l, const unsigned char* workspace,
+                  bool mn_major);
+Operand w_operand(const vggt_linear_args* a, const Laid& l, const unsigned char* workspace,
+                  bool mn_major);
 
 }  // namespace lin
 }  // namespace vggt

@@ -95,18 +95,19 @@ __global__ void __launch_bounds__(256) sums_kernel(const Sums a) {
 // gate W, rounded once more to W's type: one rounding of dx's factors, as dy gate would be.
 template <typename T>
 __global__ void __launch_bounds__(256)
-    scale_weight_kernel(const T* w, int64_t stride, const T* gate, T* to, int64_t outer,
-                        int64_t inner) {
-  const int64_t groups = inner / 8, all = outer * groups;
+    scale_weight_kernel(const T* w, int64_t stride, const T* gate, T* to, int64_t pad,
+                        int64_t outer, int64_t inner) {
+  const int64_t groups = (inner + 7) / 8, all = outer * groups;
   for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < all;
        i += (int64_t)gridDim.x * blockDim.x) {
     const int64_t r = i / groups, c = (i - r * groups) * 8;
     float v[8];
-    Elem<T>::load8(w + r * stride + c, v);
+    const int n = (int)min((int64_t)8, inner - c);
+    get8(w + r * stride + c, n, true, v);
     const float g = (float)gate[r];
 #pragma unroll
     for (int j = 0; j < 8; ++j) v[j] *= g;
-    Elem<T>::store8(to + r * inner + c, v);
+    put8(to + r * pad + c, n, true, v);
   }
 }
 
@@ -146,18 +147,19 @@ __global__ void __launch_bounds__(128) finish_weight_kernel(const Slots s, const
   float dot = 0.f;
   if (a.product)
     for (int64_t c = threadIdx.x * 8; c < a.inner; c += 128 * 8) {
+      const int n = (int)min((int64_t)8, a.inner - c);
       float v[8];
       s.get8(r, c, v);
       if (want_dot) {
         float w[8];
-        Elem<T>::load8(static_cast<const T*>(a.weight) + r * a.weight_stride + c, w);
+        get8(static_cast<const T*>(a.weight) + r * a.weight_stride + c, n, true, w);
 #pragma unroll
         for (int i = 0; i < 8; ++i) dot = fmaf(v[i], w[i], dot);
       }
       if (a.dweight != nullptr) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) v[i] *= gate;
-        put8(static_cast<T*>(a.dweight) + r * a.dweight_stride + c, 8, a.wide, v);
+        put8(static_cast<T*>(a.dweight) + r * a.dweight_stride + c, n, a.wide, v);
       }
     }
   float sum = 0.f;
@@ -185,6 +187,7 @@ __global__ void __launch_bounds__(128) finish_weight_kernel(const Slots s, const
 struct Back {
   bool act, dx, product, sums, copy_dy, scale_dy, scale_w;
   int64_t row_blocks, per_block, pad;  // pad: row stride of dz
+  Laid laid;
   Plan px, pw;
   size_t dz, scaled, weight, bias_part, gate_part, slots, bytes;
 };
@@ -210,6 +213,8 @@ static Back plan_back(const vggt_linear_args* a, const vggt_linear_grads* g) {
     b.scale_w = !b.scale_dy;
   }
   b.sums = b.copy_dy || b.scale_dy || (g->dbias && a->bias) || dgate;
+  b.laid = plan_operands(a, b.product, b.dx || (dgate && !b.act));
+  b.bytes = b.laid.bytes;
   const int64_t cols = (a->outer + 255) / 256;
   b.row_blocks = std::max<int64_t>(1, std::min<int64_t>((a->rows + 31) / 32, 148 * 8 / cols));
   b.per_block = (a->rows + b.row_blocks - 1) / b.row_blocks;
@@ -222,7 +227,7 @@ static Back plan_back(const vggt_linear_args* a, const vggt_linear_grads* g) {
   };
   b.dz = take(b.copy_dy, (size_t)a->rows * b.pad * 2);
   b.scaled = take(b.scale_dy, (size_t)a->rows * b.pad * 2);
-  b.weight = take(b.scale_w, (size_t)a->outer * a->inner * 2);
+  b.weight = take(b.scale_w, (size_t)a->outer * b.laid.pad * 2);
   b.bias_part = take(b.sums, (size_t)b.row_blocks * a->outer * 4);
   b.gate_part = take(b.sums && b.act, (size_t)b.row_blocks * a->outer * 4);
   if (b.dx) b.px = plan_product(a->rows, a->inner, a->outer, false);
@@ -265,44 +270,46 @@ static cudaError_t run_back(const vggt_linear_args* a, const vggt_linear_grads* 
       sums_kernel<T, T><<<grid, 256, 0, stream>>>(s);
     if (cudaError_t e = cudaGetLastError()) return e;
   }
+  if (cudaError_t e = copy_operands(a, b.laid, ws, stream)) return e;
+  const Operand weight = w_operand(a, b.laid, ws, true);
   const void* dz = b.copy_dy ? ws + b.dz : g->dy;
   const int64_t dz_stride = b.copy_dy ? b.pad : g->dy_stride;
   if (b.dx) {
-    const void* w = a->weight;
-    int64_t w_stride = a->weight_stride;
+    Operand w = weight;
     if (b.scale_w) {
       T* to = reinterpret_cast<T*>(ws + b.weight);
-      const int64_t all = outer * (inner / 8);
+      const int64_t all = outer * ((inner + 7) / 8);
       scale_weight_kernel<T><<<(unsigned)std::min<int64_t>((all + 255) / 256, 148 * 16), 256, 0,
-                               stream>>>(static_cast<const T*>(w), w_stride,
-                                         static_cast<const T*>(a->gate), to, outer, inner);
+                               stream>>>(static_cast<const T*>(w.p), w.stride,
+                                         static_cast<const T*>(a->gate), to, b.laid.pad, outer, inner);
       if (cudaError_t e = cudaGetLastError()) return e;
-      w = to;
-      w_stride = inner;
+      w.p = to;
+      w.stride = b.laid.pad;
     }
     Epilogue e;
     e.y = g->dx;
     e.y_stride = g->dx_stride;
     e.y_head_stride = g->dx_head_stride;
-    e.y_heads = a->heads > 1 ? a->heads : 1;
+    e.y_heads = a->heads > 1 && g->dx_head_stride > 0 ? a->heads : 1;
     e.y_dim = inner / e.y_heads;
     e.y_type = a->dtype;
     const Operand d = b.scale_dy ? matrix(scaled, outer, b.pad, false)
                                  : matrix(dz, outer, dz_stride, false);
-    if (cudaError_t rc = launch_product(b.px, a->dtype, rows, inner, outer, d,
-                                        matrix(w, inner, w_stride, true), e, slots, status, stream))
+    if (cudaError_t rc =
+            launch_product(b.px, a->dtype, rows, inner, outer, d, w, e, slots, status, stream))
       return rc;
     if (b.px.split)
       if (cudaError_t rc = finish_product(b.px, a->dtype, rows, inner, e, slots, stream)) return rc;
   }
   if (b.product)
     if (cudaError_t rc = launch_product(b.pw, a->dtype, outer, inner, rows,
-                                        matrix(dz, outer, dz_stride, true), x_operand(a, true),
-                                        Epilogue{}, slots, status, stream))
+                                        matrix(dz, outer, dz_stride, true),
+                                        x_operand(a, b.laid, ws, true), Epilogue{}, slots, status,
+                                        stream))
       return rc;
   Weights f{};
-  f.weight = a->weight;
-  f.weight_stride = a->weight_stride;
+  f.weight = weight.p;
+  f.weight_stride = weight.stride;
   f.bias = a->bias;
   f.gate = a->gate;
   f.act = b.act;
@@ -357,8 +364,11 @@ extern "C" int vggt_linear_grad(const vggt_linear_args* a, const vggt_linear_gra
     return api_fail("with an activation the gradient needs z");
   if (a->rows > 1 && (g->dy_stride < 0 || (g->z && g->z_stride < 0)))
     return api_fail("negative stride");
-  const int64_t dim = a->heads > 1 ? a->inner / a->heads : a->inner;
-  if (g->dx && ((a->rows > 1 && g->dx_stride < dim) || (a->heads > 1 && g->dx_head_stride < dim)))
+  const bool split_dx = a->heads > 1 && g->dx_head_stride > 0;
+  const int64_t dim = split_dx ? a->inner / a->heads : a->inner;
+  if (g->dx && split_dx && dim % 64)
+    return api_fail("a head-major dx needs heads of a multiple of 64 elements");
+  if (g->dx && ((a->rows > 1 && g->dx_stride < dim) || (split_dx && g->dx_head_stride < dim)))
     return api_fail("a stride of dx is below the row's width");
   const Back b = plan_back(a, g);
   if (b.bytes > 0 && (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 255u) ||

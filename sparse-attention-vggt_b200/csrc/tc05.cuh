@@ -273,6 +273,9 @@ __device__ __forceinline__ void tmem_wait_st() {
 // and up), 128-byte swizzle, zero fill out of bounds.
 bool encode_tmap_sw128(CUtensorMap* map, const void* ptr, int dtype, int rank,
                        const uint64_t* dims, const uint64_t* strides, const uint32_t* box);
+// the same with a 64- or 128-byte swizzle
+bool encode_tmap(CUtensorMap* map, const void* ptr, int dtype, int rank, const uint64_t* dims,
+                 const uint64_t* strides, const uint32_t* box, int swizzle);
 bool encode_tmap_3d_sw128(CUtensorMap* map, const void* ptr, int dtype, int64_t d0, int64_t d1,
                           int64_t d2, uint32_t box0, uint32_t box1);
 
