@@ -126,6 +126,25 @@ __device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity, volatile int
   }
 }
 
+// The wait of a full warp: true on all lanes or on none, and the branch on it is uniform.  (The roles
+// that feed the tensor core run as whole warps and elect a lane to issue: the instructions take
+// their descriptors from uniform registers then.  Issued under `lane == 0` an MMA took 63 cycles to
+// get out, and four of them as long as a 128 x 128 block's multiplication.)
+__device__ __forceinline__ bool wait_warp(uint32_t bar, uint32_t parity, volatile int* abort_flag,
+                                          uint64_t limit_ns) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "vote.sync.all.pred q, p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  if (ok) return true;
+  return __all_sync(0xffffffffu, wait(bar, parity, abort_flag, limit_ns));
+}
+
 // ---- what pairs of CTAs need beside tc05.cuh -------------------------------------------------
 __device__ __forceinline__ uint32_t cluster_rank() {
   uint32_t r;
@@ -369,67 +388,67 @@ __global__ void __launch_bounds__(THREADS, 1)
 
   if (warp == 0) {
     // ================= TMA producer =================
-    if (lane == 0) {
-      const uint32_t full0 = CTA == 2 ? map_rank(bar(SH::B_FULL), 0) : bar(SH::B_FULL);
-      Walk<SPLIT> w(p, worker);
-      Ring<STAGES> ring;
-      uint32_t issued = 0;
-      bool ok = true;
-      while (ok && w.next()) {
-        const int m0 = (int)w.tm * (BM * CTA) + rank * BM;
-        const int n0 = (int)w.tn * BN + rank * BNC;
-        // where the operands' first blocks lie: one thread feeds the tensor core here, so that
-        // no division is left in the loop
-        Place a0, a1, b0, b1;
-        if (AMN) {
-          a0 = Place(m0 / 64, p.a_heads64);
-          a1 = Place(m0 / 64 + 1, p.a_heads64);
-        } else {
-          a0 = Place(w.k0, p.a_heads64);
+    const uint32_t full0 = CTA == 2 ? map_rank(bar(SH::B_FULL), 0) : bar(SH::B_FULL);
+    Walk<SPLIT> w(p, worker);
+    Ring<STAGES> ring;
+    uint32_t issued = 0;
+    bool ok = true;
+    while (ok && w.next()) {
+      const int m0 = (int)w.tm * (BM * CTA) + rank * BM;
+      const int n0 = (int)w.tn * BN + rank * BNC;
+      // where the operands' first blocks lie: no division is left in the loop
+      Place a0, a1, b0, b1;
+      if (AMN) {
+        a0 = Place(m0 / 64, p.a_heads64);
+        a1 = Place(m0 / 64 + 1, p.a_heads64);
+      } else {
+        a0 = Place(w.k0, p.a_heads64);
+      }
+      if (BMN) {
+        b0 = Place(n0 / 64, p.b_heads64);
+        if (BNC == 128) b1 = Place(n0 / 64 + 1, p.b_heads64);
+      } else {
+        b0 = Place(w.k0, p.b_heads64);
+      }
+      for (int k = w.k0; k < w.k1; ++k) {
+        if (issued >= STAGES &&
+            !wait_warp(bar(SH::B_EMPTY) + 8 * ring.at, ring.turn ^ 1, abort_flag, p.wait_ns)) {
+          ok = false;
+          break;
         }
-        if (BMN) {
-          b0 = Place(n0 / 64, p.b_heads64);
-          if (BNC == 128) b1 = Place(n0 / 64 + 1, p.b_heads64);
-        } else {
-          b0 = Place(w.k0, p.b_heads64);
-        }
-        for (int k = w.k0; k < w.k1; ++k) {
-          if (issued >= STAGES &&
-              !wait(bar(SH::B_EMPTY) + 8 * ring.at, ring.turn ^ 1, abort_flag, p.wait_ns)) {
-            ok = false;
-            break;
-          }
-          // the barrier is the first CTA's: it counts both CTAs' bytes
-          const uint32_t full = full0 + 8 * ring.at;
+        // the barrier is the first CTA's: it counts both CTAs' bytes
+        const uint32_t full = full0 + 8 * ring.at;
+        const uint32_t a = base + ring.at * STAGE_BYTES, b = a + A_BYTES;
+        if (tc::elect_one()) {
           if (rank == 0) tc::mbar_expect_tx(bar(SH::B_FULL) + 8 * ring.at, CTA * STAGE_BYTES);
-          const uint32_t a = base + ring.at * STAGE_BYTES, b = a + A_BYTES;
           if (AMN) {
             Pair<CTA>::load(a, &tm_a, full, a0.x, k * BK, a0.head);
             Pair<CTA>::load(a + A_BYTES / 2, &tm_a, full, a1.x, k * BK, a1.head);
           } else {
             Pair<CTA>::load(a, &tm_a, full, a0.x, m0, a0.head);
-            a0.step(p.a_heads64);
           }
           if (BMN) {
             Pair<CTA>::load(b, &tm_b, full, b0.x, k * BK, b0.head);
             if (BNC == 128) Pair<CTA>::load(b + A_BYTES / 2, &tm_b, full, b1.x, k * BK, b1.head);
           } else {
             Pair<CTA>::load(b, &tm_b, full, b0.x, n0, b0.head);
-            b0.step(p.b_heads64);
           }
-          ring.step();
-          ++issued;
         }
+        __syncwarp();
+        if (!AMN) a0.step(p.a_heads64);
+        if (!BMN) b0.step(p.b_heads64);
+        ring.step();
+        ++issued;
       }
-      // the last copies have landed before the memory goes (the MMAs that read them are awaited
-      // by their issuer)
-      if (rank == 0)
-        for (uint32_t t = issued > STAGES ? issued - STAGES : 0; t < issued; ++t)
-          tc::mbar_wait_drain(bar(SH::B_FULL + t % STAGES), (t / STAGES) & 1, p.wait_ns);
     }
+    // the last copies have landed before the memory goes (the MMAs that read them are awaited
+    // by their issuer)
+    if (rank == 0 && lane == 0)
+      for (uint32_t t = issued > STAGES ? issued - STAGES : 0; t < issued; ++t)
+        tc::mbar_wait_drain(bar(SH::B_FULL + t % STAGES), (t / STAGES) & 1, p.wait_ns);
   } else if (warp == 1) {
     // ================= MMA issuer (of the pair's first CTA) =================
-    if (lane == 0 && rank == 0) {
+    if (rank == 0) {
       const uint32_t fmt = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
       const uint32_t idesc =
           tc::idesc_f16(fmt, BMN ? 1u : 0u, BM * CTA, BN) | (AMN ? 1u << 15 : 0u);
@@ -437,39 +456,43 @@ __global__ void __launch_bounds__(THREADS, 1)
       constexpr uint64_t kStepA = AMN ? 16 * 128 / 16 : 2, kStepB = BMN ? 16 * 128 / 16 : 2;
       const uint64_t desc0 = tc::sw128_desc(base, A_BYTES / 2);
       bool ok = true;
-      if (p.wait_selftest) ok = wait(bar(SH::B_DRAIN), 0, abort_flag, p.wait_ns);
+      if (p.wait_selftest) ok = wait_warp(bar(SH::B_DRAIN), 0, abort_flag, p.wait_ns);
       Walk<SPLIT> w(p, worker);
       Ring<STAGES> ring;
       uint32_t i = 0;
       while (ok && w.next()) {
         const uint32_t b = i & 1;
         if (i >= 2 &&
-            !wait(bar(SH::B_ACCEMPTY + b), ((i >> 1) + 1) & 1, abort_flag, p.wait_ns)) {
+            !wait_warp(bar(SH::B_ACCEMPTY + b), ((i >> 1) + 1) & 1, abort_flag, p.wait_ns)) {
           ok = false;
           break;
         }
         tc::tc_fence_after();
         const uint32_t acc = tmem + b * BN;
         for (int k = w.k0; k < w.k1; ++k) {
-          if (!wait(bar(SH::B_FULL) + 8 * ring.at, ring.turn, abort_flag, p.wait_ns)) {
+          if (!wait_warp(bar(SH::B_FULL) + 8 * ring.at, ring.turn, abort_flag, p.wait_ns)) {
             ok = false;
             break;
           }
           tc::tc_fence_after();
           const uint64_t ad = desc0 + ring.at * (STAGE_BYTES / 16), bd = ad + A_BYTES / 16;
+          if (tc::elect_one()) {
 #pragma unroll
-          for (int kk = 0; kk < BK / 16; ++kk)
-            Pair<CTA>::mma(acc, ad + kk * kStepA, bd + kk * kStepB, idesc,
-                           (k > w.k0 || kk > 0) ? 1u : 0u);
-          Pair<CTA>::commit(bar(SH::B_EMPTY) + 8 * ring.at);
+            for (int kk = 0; kk < BK / 16; ++kk)
+              Pair<CTA>::mma(acc, ad + kk * kStepA, bd + kk * kStepB, idesc,
+                             (k > w.k0 || kk > 0) ? 1u : 0u);
+            Pair<CTA>::commit(bar(SH::B_EMPTY) + 8 * ring.at);
+            if (k + 1 == w.k1) Pair<CTA>::commit(bar(SH::B_ACCFULL + b));
+          }
+          __syncwarp();
           ring.step();
         }
-        if (ok) Pair<CTA>::commit(bar(SH::B_ACCFULL + b));
         ++i;
       }
       if (!p.wait_selftest) {
-        Pair<CTA>::commit(bar(SH::B_DRAIN));
-        tc::mbar_wait_drain(bar(SH::B_DRAIN), 0, p.wait_ns);
+        if (tc::elect_one()) Pair<CTA>::commit(bar(SH::B_DRAIN));
+        __syncwarp();
+        if (lane == 0) tc::mbar_wait_drain(bar(SH::B_DRAIN), 0, p.wait_ns);
       }
     }
   } else if (warp >= 4) {
