@@ -780,14 +780,14 @@ static int sm_count() {
   return device_sms(&sms) == cudaSuccess && sms > 0 ? sms : 148;
 }
 
-// The way a product is cut is the one of the least estimated time, in SM cycles.  A reduction block
-// takes as long as its bytes take through shared memory, written once and read once at 128 B a
-// cycle (measured 525 cycles for the 32 KB of a 128 x 128 or of half a 256 x 256 tile): the larger
-// tile does four times the work in that.  A launch and a tile's epilogue cost about 8,000 cycles.
-// Splitting evens the load out where tiles are few or the last round is short, at the price of
-// partial sums through memory and another launch.
+// The way a product is cut is the one of the least estimated time, in SM cycles: what a launch and a
+// reduction block take, measured alone and (block: + busy) with all SMs at work, and for a split one
+// the partial sums' way through memory and another launch.  Splitting evens the load out where
+// tiles are few or the last round is short.
 Plan plan_product(int64_t m, int64_t n, int64_t red, bool must_split) {
-  static const int kShapes[][2] = {{1, 64}, {1, 128}, {2, 64}, {2, 128}};  // cta, bnc
+  // cta, bnc, a launch, a block, a block's share that grows with the load
+  static const int kShapes[][5] = {
+      {1, 64, 6500, 420, 40}, {1, 128, 7700, 450, 60}, {2, 64, 8200, 320, 60}, {2, 128, 10500, 530, 80}};
   const int sms = sm_count();
   Plan best;
   double least = 0;
@@ -802,8 +802,9 @@ Plan plan_product(int64_t m, int64_t n, int64_t red, bool must_split) {
       p.blocks = (red + BK - 1) / BK;
       p.workers = (int)std::min<int64_t>(sms / p.cta, p.units());
       const int64_t rounds = (p.units() + p.workers - 1) / p.workers;
-      double t = (double)rounds * (split ? 1 : p.blocks) * (p.bnc + BM) * 2.05 + p.bnc * p.cta * 10;
-      if (split) t += 5000 + (double)p.slot_bytes() * 2 / 2500;
+      const double busy = (double)p.workers * p.cta / sms;
+      double t = shape[2] + (double)rounds * (split ? 1 : p.blocks) * (shape[3] + shape[4] * busy);
+      if (split) t += 7000 + (double)p.slot_bytes() * 2 / 2500;
       if (least == 0 || t < least) {
         least = t;
         best = p;
@@ -1083,8 +1084,9 @@ int check(const vggt_linear_args* a) {
 extern "C" size_t vggt_linear_workspace_size(const vggt_linear_args* a) {
   using namespace vggt::lin;
   if (!a || a->rows <= 0 || a->inner < 1 || a->outer < 1) return 0;
-  return plan_operands(a, true, true).bytes +
-         plan_product(a->rows, a->outer, a->inner, false).slot_bytes();
+  const size_t copies = plan_operands(a, true, true).bytes;
+  if (few_rows(a->rows, a->outer, a->inner)) return copies;
+  return copies + plan_product(a->rows, a->outer, a->inner, false).slot_bytes();
 }
 
 extern "C" int vggt_linear(const vggt_linear_args* a, void* y, int64_t y_stride, void* z,
@@ -1098,7 +1100,8 @@ extern "C" int vggt_linear(const vggt_linear_args* a, void* y, int64_t y_stride,
   if (a->rows > 1 && (y_stride < a->outer || (z && z_stride < a->outer)))
     return api_fail("an output's rows overlap: its stride is below outer");
   const Laid laid = plan_operands(a, true, true);
-  const Plan plan = plan_product(a->rows, a->outer, a->inner, false);
+  const bool few = few_rows(a->rows, a->outer, a->inner);
+  const Plan plan = few ? Plan{} : plan_product(a->rows, a->outer, a->inner, false);
   const size_t bytes = laid.bytes + plan.slot_bytes();
   if (bytes > 0 && (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 255u) ||
                     workspace_bytes < bytes))
@@ -1119,6 +1122,9 @@ extern "C" int vggt_linear(const vggt_linear_args* a, void* y, int64_t y_stride,
   unsigned char* ws = static_cast<unsigned char*>(workspace);
   float* slots = reinterpret_cast<float*>(ws + laid.bytes);
   cudaError_t rc = copy_operands(a, laid, ws, st);
+  if (rc == cudaSuccess && few)
+    return api_cuda(launch_rows(a->dtype, a->rows, a->outer, a->inner, x_operand(a, laid, ws, false),
+                                w_operand(a, laid, ws, false), e, st));
   if (rc == cudaSuccess)
     rc = launch_product(plan, a->dtype, a->rows, a->outer, a->inner, x_operand(a, laid, ws, false),
                         w_operand(a, laid, ws, false), e, slots, status, st);

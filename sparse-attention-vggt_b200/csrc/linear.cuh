@@ -85,6 +85,11 @@ cudaError_t launch_product(const Plan& plan, int dtype, int64_t m, int64_t n, in
 cudaError_t finish_product(const Plan& plan, int dtype, int64_t m, int64_t n, const Epilogue& e,
                            const float* slots, cudaStream_t stream);
 
+// linear_rows.cu: the product for few rows of x, all epilogues, no workspace.
+bool few_rows(int64_t m, int64_t n, int64_t k);
+cudaError_t launch_rows(int dtype, int64_t m, int64_t n, int64_t k, const Operand& x,
+                        const Operand& w, const Epilogue& e, cudaStream_t stream);
+
 // Argument checks (0, or the error) and operands of a call.
 int check(const vggt_linear_args* a);
 Operand matrix(const void* p, int64_t width, int64_t stride, bool mn_major);
