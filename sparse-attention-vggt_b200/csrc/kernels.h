@@ -4,6 +4,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 namespace vggt {
 
 // capi.cu: an argument error (sets the message, returns -1); with a null
@@ -14,8 +16,25 @@ int api_cuda(cudaError_t e);
 uint64_t api_wait_ns();
 // vggt_sparse_set_wait_selftest
 int api_wait_selftest();
-// residual_norm.cu: multiprocessors of the current device
+// residual_norm.cu: multiprocessors of the current device (asked for once)
 cudaError_t device_sms(int* sms);
+// A kernel's dynamic shared memory allowed on the current device: once for each device, since
+// asking costs as much as a launch.  One OncePerDevice to a kernel.
+struct OncePerDevice {
+  std::atomic<uint64_t> devices{0};
+};
+template <typename K>
+cudaError_t allow_shared(K kernel, int bytes, OncePerDevice* once) {
+  int dev = 0;
+  if (cudaError_t e = cudaGetDevice(&dev)) return e;
+  const uint64_t bit = dev < 64 ? 1ull << dev : 0;
+  if (once->devices.load(std::memory_order_relaxed) & bit) return cudaSuccess;
+  if (cudaError_t e =
+          cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes))
+    return e;
+  once->devices.fetch_or(bit, std::memory_order_relaxed);
+  return cudaSuccess;
+}
 
 inline bool units_zero(int64_t a, int64_t b) { return a == 0 || b == 0; }
 

@@ -270,35 +270,46 @@ __device__ __forceinline__ uint32_t piece(uint32_t buf, int r, int j) {
 template <int ROW, typename E>
 __device__ __forceinline__ void copy_rows(uint32_t buf, int row0, E* g, int64_t stride, int64_t rows,
                                           int64_t left, bool in) {
-  constexpr int kAll = ROW / (int)sizeof(E), kPiece = 16 / (int)sizeof(E);
+  constexpr int kPer = ROW / (int)sizeof(E) / 32, kPiece = 16 / (int)sizeof(E), kAhead = 8;
+  typedef std::conditional_t<sizeof(E) == 2, uint16_t, uint32_t> Bits;
   const int lane = threadIdx.x & 31;
-  for (int r = 0; r < 32 && r < rows; ++r) {
-#pragma unroll
-    for (int i = 0; i < kAll / 32; ++i) {
+  for (int r0 = 0; r0 < 32 && r0 < rows; r0 += kAhead) {
+    Bits v[kAhead][kPer];  // loads of several rows in flight
+    auto at = [&](int q, int i) {
       const int c = lane + i * 32;
-      if (c >= left) continue;
-      const uint32_t a = piece<ROW>(buf, row0 + r, c / kPiece) + (uint32_t)(c % kPiece) * sizeof(E);
-      E* p = g + (int64_t)r * stride + c;
-      if (sizeof(E) == 2) {
-        uint16_t v;
+      return piece<ROW>(buf, row0 + r0 + q, c / kPiece) + (uint32_t)(c % kPiece * sizeof(E));
+    };
+#pragma unroll
+    for (int q = 0; q < kAhead; ++q)
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) {
         if (in) {
-          v = *reinterpret_cast<const uint16_t*>(p);
-          asm volatile("st.shared.u16 [%0], %1;" ::"r"(a), "h"(v) : "memory");
+          v[q][i] = 0;
+          if (r0 + q < rows && lane + i * 32 < left)
+            v[q][i] = *reinterpret_cast<const Bits*>(g + (r0 + q) * stride + lane + i * 32);
+        } else if constexpr (sizeof(E) == 2) {
+          uint16_t w;
+          asm volatile("ld.shared.u16 %0, [%1];" : "=h"(w) : "r"(at(q, i)) : "memory");
+          v[q][i] = (Bits)w;
         } else {
-          asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(a) : "memory");
-          *reinterpret_cast<uint16_t*>(p) = v;
-        }
-      } else {
-        uint32_t v;
-        if (in) {
-          v = *reinterpret_cast<const uint32_t*>(p);
-          asm volatile("st.shared.u32 [%0], %1;" ::"r"(a), "r"(v) : "memory");
-        } else {
-          asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
-          *reinterpret_cast<uint32_t*>(p) = v;
+          uint32_t w;
+          asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w) : "r"(at(q, i)) : "memory");
+          v[q][i] = (Bits)w;
         }
       }
-    }
+#pragma unroll
+    for (int q = 0; q < kAhead; ++q)
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) {
+        if (!in) {
+          if (r0 + q < rows && lane + i * 32 < left)
+            *reinterpret_cast<Bits*>(g + (r0 + q) * stride + lane + i * 32) = v[q][i];
+        } else if constexpr (sizeof(E) == 2) {
+          asm volatile("st.shared.u16 [%0], %1;" ::"r"(at(q, i)), "h"(v[q][i]) : "memory");
+        } else {
+          asm volatile("st.shared.u32 [%0], %1;" ::"r"(at(q, i)), "r"(v[q][i]) : "memory");
+        }
+      }
   }
 }
 
@@ -805,6 +816,10 @@ Plan plan_product(int64_t m, int64_t n, int64_t red, bool must_split) {
       const double busy = (double)p.workers * p.cta / sms;
       double t = shape[2] + (double)rounds * (split ? 1 : p.blocks) * (shape[3] + shape[4] * busy);
       if (split) t += 7000 + (double)p.slot_bytes() * 2 / 2500;
+      // workers that begin in different places of long operands do not meet in L2 (44,000 rows'
+      // weight gradient 254 us whole, 351 split)
+      if (split && (double)(m + n) * red * 2 > 60e6)
+        t = std::max(t, (double)p.tiles_m * p.tiles_n * red * 2 * (BM + p.bnc) * p.cta / 3500);
       if (least == 0 || t < least) {
         least = t;
         best = p;
@@ -845,7 +860,8 @@ template <typename T, int CTA, int BNC, bool AMN, bool BMN, bool SPLIT>
 static cudaError_t launch_kernel(const CUtensorMap* maps, const Params& p, cudaStream_t stream) {
   auto k = product_kernel<T, CTA, BNC, AMN, BMN, SPLIT>;
   constexpr int smem = (int)Shape<CTA, BNC>::SMEM_BYTES;
-  cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  static OncePerDevice allowed;
+  cudaError_t e = allow_shared(k, smem, &allowed);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)(p.workers * CTA));
@@ -873,9 +889,9 @@ static cudaError_t launch_majors(bool amn, bool bmn, bool split, const CUtensorM
   if (!amn)
     return split ? launch_kernel<T, CTA, BNC, false, true, true>(maps, p, stream)
                  : launch_kernel<T, CTA, BNC, false, true, false>(maps, p, stream);
-  // the weight's gradient is always split
-  return split && bmn ? launch_kernel<T, CTA, BNC, true, true, true>(maps, p, stream)
-                      : cudaErrorInvalidValue;
+  if (!bmn) return cudaErrorInvalidValue;  // no product has these
+  return split ? launch_kernel<T, CTA, BNC, true, true, true>(maps, p, stream)
+               : launch_kernel<T, CTA, BNC, true, true, false>(maps, p, stream);
 }
 
 template <typename T>
@@ -968,11 +984,11 @@ struct Copy {
 };
 
 __global__ void __launch_bounds__(256) copy_operand_kernel(const Copy c) {
-  const int64_t all = c.rows * c.pad;
-  for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < all;
-       i += (int64_t)gridDim.x * blockDim.x) {
-    const int64_t r = i / c.pad, k = i - r * c.pad, head = k / c.dim;
-    c.to[i] = k < c.width ? c.from[head * c.head_stride + r * c.stride + (k - head * c.dim)] : 0;
+  const int64_t r = blockIdx.x;
+  for (int k = threadIdx.x; k < (int)c.pad; k += 256) {
+    const int head = k / (int)c.dim;
+    c.to[r * c.pad + k] =
+        k < c.width ? c.from[head * c.head_stride + r * c.stride + (k - head * (int)c.dim)] : 0;
   }
 }
 
@@ -1012,9 +1028,7 @@ cudaError_t copy_operands(const vggt_linear_args* a, const Laid& l, unsigned cha
     c.head_stride = a->x_head_stride;
     c.dim = which == 0 ? a->inner / heads : l.pad;
     if (c.dim == a->inner) c.dim = l.pad;  // one head
-    const int64_t all = c.rows * c.pad;
-    copy_operand_kernel<<<(unsigned)std::min<int64_t>((all + 255) / 256, 148 * 16), 256, 0,
-                          stream>>>(c);
+    copy_operand_kernel<<<(unsigned)c.rows, 256, 0, stream>>>(c);
     if (cudaError_t e = cudaGetLastError()) return e;
   }
   return cudaSuccess;

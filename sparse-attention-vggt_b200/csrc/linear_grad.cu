@@ -6,10 +6,12 @@
 //   dW = gate G,  db = gate s,  dgate_n = <W_n, G_n> + b_n s_n,  dx = dy (gate W):
 // the only pass over [rows][outer] beside the two products is the one that forms s.
 //
-// dW is a product over the rows, cut evenly over the SMs (its tiles are few); the partial sums
-// lie in fp32 in the workspace until finish_weight adds them, scales them by the gate and forms
-// the row products of dgate.  Nothing is added with atomics: equal calls give equal bits.
+// dW is a product over the rows.  With a gate and no activation, or where its tiles are few, it is
+// cut evenly over the SMs; the partial sums lie in fp32 in the workspace until finish_weight adds
+// them, scales them by the gate and forms the row products of dgate.  Nothing is added with
+// atomics: equal calls give equal bits.
 #include <algorithm>
+#include <type_traits>
 
 #include "activation.cuh"
 #include "linear.cuh"
@@ -35,9 +37,12 @@ struct Sums {
   bool wide;
 };
 
-template <typename S, typename T>
-__global__ void __launch_bounds__(256) sums_kernel(const Sums a) {
+template <typename S, typename T, int ACT, bool WIDE>
+__global__ void __launch_bounds__(256, ACT == VGGT_ACT_NONE ? 4 : 2) sums_kernel(const Sums a) {
   __shared__ float fold[8][256];
+  // rows whose loads are in flight (with a branch for unaligned ones in the loop none were, and
+  // the sums of 22,000 x 1024 took 34 us)
+  constexpr int kAhead = 4;
   const int cx = threadIdx.x & 31, ry = threadIdx.x >> 5;
   const int64_t c = ((int64_t)blockIdx.x * 32 + cx) * 8;
   const int n = (int)max((int64_t)0, min((int64_t)8, a.outer - c));
@@ -45,35 +50,47 @@ __global__ void __launch_bounds__(256) sums_kernel(const Sums a) {
   float sb[8], sg[8], gate[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) sb[i] = sg[i] = 0.f, gate[i] = 1.f;
+  auto get = [&](const auto* p, float* v) {
+    typedef std::remove_cv_t<std::remove_pointer_t<decltype(p)>> E;
+    if (WIDE)
+      Elem<E>::load8(p, v);
+    else
+      get8(p, n, false, v);
+  };
   if (n > 0) {
-    if (a.gate != nullptr) get8(static_cast<const T*>(a.gate) + c, n, a.wide, gate);
-    act::dispatch(a.act, [&](auto k) {
-      constexpr int kind = decltype(k)::value;
-#pragma unroll 4
-      for (int64_t r = r0 + ry; r < r1; r += 8) {
-        float d[8];
-        get8(static_cast<const S*>(a.dy) + r * a.dy_stride + c, n, a.wide, d);
-        if (kind != VGGT_ACT_NONE) {
-          float z[8];
-          get8(static_cast<const T*>(a.z) + r * a.z_stride + c, n, a.wide, z);
+    if (a.gate != nullptr) get(static_cast<const T*>(a.gate) + c, gate);
+    for (int64_t rr = r0 + ry; rr < r1; rr += 8 * kAhead) {
+      float d[kAhead][8], z[ACT != VGGT_ACT_NONE ? kAhead : 1][8];
+#pragma unroll
+      for (int q = 0; q < kAhead; ++q) {
+        const int64_t r = min(rr + 8 * q, r1 - 1);  // past the end the last row, unused
+        get(static_cast<const S*>(a.dy) + r * a.dy_stride + c, d[q]);
+        if (ACT != VGGT_ACT_NONE) get(static_cast<const T*>(a.z) + r * a.z_stride + c, z[q]);
+      }
+#pragma unroll
+      for (int q = 0; q < kAhead; ++q) {
+        const int64_t r = rr + 8 * q;
+        if (r >= r1) break;
+        if (ACT != VGGT_ACT_NONE) {
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
             float slope;
-            const float v = act::value_slope<kind>(z[i], slope);
-            sg[i] = fmaf(d[i], v, sg[i]);
-            d[i] *= gate[i] * slope;
+            const float v = act::value_slope<ACT>(z[q][i], slope);
+            sg[i] = fmaf(d[q][i], v, sg[i]);
+            // rounded as it stands: whether dz goes out as well must not change the sums
+            d[q][i] = __fmul_rn(d[q][i], __fmul_rn(gate[i], slope));
           }
         }
 #pragma unroll
-        for (int i = 0; i < 8; ++i) sb[i] += d[i];
-        if (a.dz != nullptr) put8(static_cast<T*>(a.dz) + r * a.dz_stride + c, n, a.wide, d);
+        for (int i = 0; i < 8; ++i) sb[i] += d[q][i];
+        if (a.dz != nullptr) put8(static_cast<T*>(a.dz) + r * a.dz_stride + c, n, WIDE, d[q]);
         if (a.scaled != nullptr) {
 #pragma unroll
-          for (int i = 0; i < 8; ++i) d[i] *= gate[i];
-          put8(static_cast<T*>(a.scaled) + r * a.dz_stride + c, n, a.wide, d);
+          for (int i = 0; i < 8; ++i) d[q][i] *= gate[i];
+          put8(static_cast<T*>(a.scaled) + r * a.dz_stride + c, n, WIDE, d[q]);
         }
       }
-    });
+    }
   }
   for (int which = 0; which < 2; ++which) {
     float* out = which == 0 ? a.bias_part : a.gate_part;
@@ -89,6 +106,19 @@ __global__ void __launch_bounds__(256) sums_kernel(const Sums a) {
       for (int q = 0; q < 8; ++q) s += fold[q][threadIdx.x];
       out[blockIdx.y * a.outer + col] = s;
     }
+  }
+}
+
+template <typename S, typename T, bool WIDE>
+static void launch_sums(const Sums& a, dim3 grid, cudaStream_t stream) {
+  switch (a.act) {
+    case VGGT_ACT_GELU: sums_kernel<S, T, VGGT_ACT_GELU, WIDE><<<grid, 256, 0, stream>>>(a); break;
+    case VGGT_ACT_GELU_TANH:
+      sums_kernel<S, T, VGGT_ACT_GELU_TANH, WIDE><<<grid, 256, 0, stream>>>(a);
+      break;
+    case VGGT_ACT_SILU: sums_kernel<S, T, VGGT_ACT_SILU, WIDE><<<grid, 256, 0, stream>>>(a); break;
+    case VGGT_ACT_RELU: sums_kernel<S, T, VGGT_ACT_RELU, WIDE><<<grid, 256, 0, stream>>>(a); break;
+    default: sums_kernel<S, T, VGGT_ACT_NONE, WIDE><<<grid, 256, 0, stream>>>(a);
   }
 }
 
@@ -231,7 +261,7 @@ static Back plan_back(const vggt_linear_args* a, const vggt_linear_grads* g) {
   b.bias_part = take(b.sums, (size_t)b.row_blocks * a->outer * 4);
   b.gate_part = take(b.sums && b.act, (size_t)b.row_blocks * a->outer * 4);
   if (b.dx) b.px = plan_product(a->rows, a->inner, a->outer, false);
-  if (b.product) b.pw = plan_product(a->outer, a->inner, a->rows, true);
+  if (b.product) b.pw = plan_product(a->outer, a->inner, a->rows, a->gate && !b.act);
   // the products run one after the other
   b.slots = take(true, std::max(b.dx ? b.px.slot_bytes() : 0, b.product ? b.pw.slot_bytes() : 0));
   return b;
@@ -265,9 +295,10 @@ static cudaError_t run_back(const vggt_linear_args* a, const vggt_linear_grads* 
              (!b.act || wide_rows(g->z, g->z_stride, a->dtype)) && wide_rows(a->gate, 8, a->dtype);
     const dim3 grid((unsigned)((outer + 255) / 256), (unsigned)b.row_blocks);
     if (a->stream_dtype == VGGT_DTYPE_FP32)
-      sums_kernel<float, T><<<grid, 256, 0, stream>>>(s);
+      s.wide ? launch_sums<float, T, true>(s, grid, stream)
+             : launch_sums<float, T, false>(s, grid, stream);
     else
-      sums_kernel<T, T><<<grid, 256, 0, stream>>>(s);
+      s.wide ? launch_sums<T, T, true>(s, grid, stream) : launch_sums<T, T, false>(s, grid, stream);
     if (cudaError_t e = cudaGetLastError()) return e;
   }
   if (cudaError_t e = copy_operands(a, b.laid, ws, stream)) return e;
@@ -301,12 +332,17 @@ static cudaError_t run_back(const vggt_linear_args* a, const vggt_linear_grads* 
     if (b.px.split)
       if (cudaError_t rc = finish_product(b.px, a->dtype, rows, inner, e, slots, stream)) return rc;
   }
-  if (b.product)
+  if (b.product) {
+    Epilogue e;  // of a product that is not split
+    e.y = g->dweight;
+    e.y_stride = g->dweight_stride;
+    e.y_dim = inner;
+    e.y_type = a->dtype;
     if (cudaError_t rc = launch_product(b.pw, a->dtype, outer, inner, rows,
                                         matrix(dz, outer, dz_stride, true),
-                                        x_operand(a, b.laid, ws, true), Epilogue{}, slots, status,
-                                        stream))
+                                        x_operand(a, b.laid, ws, true), e, slots, status, stream))
       return rc;
+  }
   Weights f{};
   f.weight = weight.p;
   f.weight_stride = weight.stride;
@@ -317,15 +353,16 @@ static cudaError_t run_back(const vggt_linear_args* a, const vggt_linear_grads* 
   f.dweight_stride = g->dweight_stride;
   f.dbias = a->bias ? g->dbias : nullptr;
   f.dgate = a->gate ? g->dgate : nullptr;
-  if (!b.product && !f.dbias && !f.dgate) return cudaSuccess;
+  const bool partial = b.product && b.pw.split;
+  if (!partial && !f.dbias && !f.dgate) return cudaSuccess;
   f.bias_part = b.sums ? bias_part : nullptr;
   f.gate_part = gate_part;
   f.row_blocks = b.row_blocks;
   f.outer = outer;
   f.inner = inner;
-  f.product = b.product;
+  f.product = partial;
   f.wide = wide_rows(g->dweight, g->dweight_stride, a->dtype);
-  const Slots s = b.product ? slots_of(b.pw, slots) : Slots{};
+  const Slots s = partial ? slots_of(b.pw, slots) : Slots{};
   finish_weight_kernel<T><<<(unsigned)outer, 128, 0, stream>>>(s, f);
   return cudaGetLastError();
 }

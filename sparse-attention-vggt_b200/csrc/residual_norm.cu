@@ -122,8 +122,8 @@ cudaError_t launch_shape(const Fwd& f, int64_t blocks, int slots, cudaStream_t s
   constexpr uint32_t bytes =
       Shared<WPR, J, J*(sizeof(S) / 2 + sizeof(T) / 2), DIRECT>::kBytes;
   auto k = forward_kernel<S, T, WPR, J, DIRECT>;
-  if (cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes))
-    return e;
+  static OncePerDevice allowed;
+  if (cudaError_t e = allow_shared(k, (int)bytes, &allowed)) return e;
   k<<<(unsigned)blocks, slots * WPR * 32, bytes, stream>>>(f);
   return cudaGetLastError();
 }
@@ -156,10 +156,13 @@ cudaError_t launch_types(const Fwd& f, int sms, cudaStream_t stream) {
 }  // namespace rnorm
 
 cudaError_t device_sms(int* sms) {
+  static std::atomic<int> known[64];
   int dev = 0;
-  const cudaError_t e = cudaGetDevice(&dev);
-  return e != cudaSuccess ? e
-                          : cudaDeviceGetAttribute(sms, cudaDevAttrMultiProcessorCount, dev);
+  if (cudaError_t e = cudaGetDevice(&dev)) return e;
+  if (dev < 64 && (*sms = known[dev].load(std::memory_order_relaxed)) > 0) return cudaSuccess;
+  const cudaError_t e = cudaDeviceGetAttribute(sms, cudaDevAttrMultiProcessorCount, dev);
+  if (e == cudaSuccess && dev < 64) known[dev].store(*sms, std::memory_order_relaxed);
+  return e;
 }
 
 static cudaError_t launch_residual_norm(const rnorm::Fwd& f, int sms, cudaStream_t stream) {

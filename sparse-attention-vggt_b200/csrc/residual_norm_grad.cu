@@ -334,8 +334,8 @@ cudaError_t launch_grid(const Bwd& f, const Grid& g, cudaStream_t stream) {
   constexpr uint32_t fold = kMaxThreads * 8 * J * 4;
   constexpr uint32_t bytes = rows > fold ? rows : fold;
   auto k = backward_kernel<S, T, WPR, J, POST, DIRECT>;
-  if (cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes))
-    return e;
+  static OncePerDevice allowed;
+  if (cudaError_t e = allow_shared(k, (int)bytes, &allowed)) return e;
   k<<<(unsigned)g.blocks, g.slots * WPR * 32, bytes, stream>>>(f);
   return cudaGetLastError();
 }

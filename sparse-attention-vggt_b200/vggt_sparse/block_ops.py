@@ -19,9 +19,6 @@ tensors' device, and may be captured in CUDA graphs.
 """
 import os
 
-import torch
-from torch.autograd.function import once_differentiable
-
 from . import _lib
 from .build import BLOCK_BINDING_PATH
 
@@ -40,42 +37,6 @@ def _binding():
         from . import _block_binding
         _module = _block_binding
     return _module
-
-
-def _any_grad(*tensors):
-    if torch.is_grad_enabled():
-        for t in tensors:
-            if t is not None and getattr(t, "requires_grad", False):
-                return True
-    return False
-
-
-def _bits(needs):
-    return sum(1 << i for i, n in enumerate(needs) if n)
-
-
-class _Linear(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, weight, bias, gate, residual, activation, head_major, status):
-        keep = activation is not None
-        y = _binding().linear(x, weight, bias, activation, gate, residual, head_major, None, keep,
-                              status)
-        y, z = y if keep else (y, None)
-        ctx.save_for_backward(x, weight, bias, gate, z)
-        ctx.how = activation, head_major, status
-        return y
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dy):
-        x, weight, bias, gate, z = ctx.saved_tensors
-        activation, head_major, status = ctx.how
-        needs = ctx.needs_input_grad
-        grads = (None,) * 4
-        if any(needs[:4]):
-            grads = _binding().linear_grad(x, weight, bias, activation, gate, None, head_major, dy,
-                                           z, _bits(needs[:4]), status)
-        return (*grads, dy if needs[4] else None, None, None, None)
 
 
 def linear(x, weight, bias=None, *, activation=None, gate=None, residual=None, head_major=False,
@@ -99,33 +60,7 @@ def linear(x, weight, bias=None, *, activation=None, gate=None, residual=None, h
     needed.  ``status``, an int32 tensor, gets VGGT_STATUS_TIMEOUT if a wait of
     the kernel ran out.
     """
-    if _any_grad(x, weight, bias, gate, residual):
-        if out is not None:
-            raise ValueError("out is for calls without a gradient")
-        return _Linear.apply(x, weight, bias, gate, residual, activation, head_major, status)
-    return _binding().linear(x, weight, bias, activation, gate, residual, head_major, out, False,
-                             status)
-
-
-class _ResidualNorm(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, branch, weight, bias, gate, post_weight, post_bias, norm, post_norm, eps,
-                dtype):
-        ctx.set_materialize_grads(False)
-        ctx.save_for_backward(x, branch, weight, bias, gate, post_weight, post_bias)
-        y, h = _binding().residual_norm(x, branch, weight, bias, gate, post_weight, post_bias, norm,
-                                        post_norm, eps, dtype, None, None)
-        ctx.how = norm, post_norm, eps, dtype
-        return y if branch is None else (y, h)
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dy, dh=None):
-        needs = ctx.needs_input_grad[:7]
-        if dy is None and dh is None:
-            return (None,) * 11
-        grads = _binding().residual_norm_grad(*ctx.saved_tensors, *ctx.how, dy, dh, _bits(needs))
-        return (*grads, None, None, None, None)
+    return _binding().linear(x, weight, bias, activation, gate, residual, head_major, out, status)
 
 
 def residual_norm(x, branch=None, weight=None, bias=None, *, norm="layer", gate=None,
@@ -147,11 +82,5 @@ def residual_norm(x, branch=None, weight=None, bias=None, *, norm="layer", gate=
     ``out`` and ``stream_out`` (contiguous; stream_out may be x) take y and h
     where no gradient is needed.
     """
-    if _any_grad(x, branch, weight, bias, gate, post_weight, post_bias):
-        if out is not None or stream_out is not None:
-            raise ValueError("out and stream_out are for calls without a gradient")
-        both = _ResidualNorm.apply(x, branch, weight, bias, gate, post_weight, post_bias, norm,
-                                   post_norm, eps, dtype)
-        return (both, x) if branch is None else both
     return _binding().residual_norm(x, branch, weight, bias, gate, post_weight, post_bias, norm,
                                     post_norm, eps, dtype, out, stream_out)
