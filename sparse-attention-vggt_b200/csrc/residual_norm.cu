@@ -88,7 +88,7 @@ __global__ void __launch_bounds__(kMaxThreads, 1) forward_kernel(const Fwd f) {
     }
     if (branch) {
       if (a.post != 0) {
-        norm_row<WPR, J>(p, n, a.post, inv_width, a.eps, sum);
+        norm_row<!DIRECT, WPR, J>(p, n, a.post, inv_width, a.eps, sum);
 #pragma unroll
         for (int j = 0; j < J; ++j) {
           params.scale(kPostWeight, j, p[j]);
@@ -102,16 +102,16 @@ __global__ void __launch_bounds__(kMaxThreads, 1) forward_kernel(const Fwd f) {
 #pragma unroll
       for (int j = 0; j < J; ++j) {
         params.gated(j, p[j], v[j]);
-        put_pairs(h + j * step, n[j], vec, v[j]);
+        put_pairs<!DIRECT>(h + j * step, n[j], vec, v[j]);
       }
       h += f.h_stride;
     }
-    norm_row<WPR, J>(v, n, a.norm, inv_width, a.eps, sum);
+    norm_row<!DIRECT, WPR, J>(v, n, a.norm, inv_width, a.eps, sum);
 #pragma unroll
     for (int j = 0; j < J; ++j) {
       params.scale(kWeight, j, v[j]);
       params.shift(kBias, j, v[j]);
-      put_pairs(y + j * step, n[j], vec, v[j]);
+      put_pairs<!DIRECT>(y + j * step, n[j], vec, v[j]);
     }
     y += f.y_stride;
   }

@@ -47,12 +47,16 @@ __device__ __forceinline__ void get_pairs(const E* p, int n, bool vec, float_pai
 #pragma unroll
   for (int i = 0; i < 4; ++i) v[i] = pack_pair(f[2 * i], f[2 * i + 1]);
 }
-template <typename E>
+// VEC: 16-byte accesses, with n 0 or 8.
+template <bool VEC, typename E>
 __device__ __forceinline__ void put_pairs(E* p, int n, bool vec, const float_pair* v) {
   float f[8];
 #pragma unroll
   for (int i = 0; i < 4; ++i) unpack_pair(f[2 * i], f[2 * i + 1], v[i]);
-  put8(p, n, vec, f);
+  if (!VEC)
+    put8(p, n, vec, f);
+  else if (n > 0)
+    Elem<E>::store8(p, f);
 }
 __device__ __forceinline__ void get_param(const Param& q, int64_t at, int n, bool vec,
                                           float_pair* v) {
@@ -238,12 +242,13 @@ struct Pipe {
 };
 
 // v - c in the first n of 8 elements, the others (zeros) left as they are.
+template <bool VEC>
 __device__ __forceinline__ void subtract(float_pair* v, int n, float c) {
-  if (n == 8) {
-    const float_pair m = both(-c);
+  if (VEC || n == 8) {
+    const float_pair m = both(n > 0 ? -c : 0.f);
 #pragma unroll
     for (int i = 0; i < 4; ++i) v[i] = add_pair(v[i], m);
-  } else if (n > 0) {
+  } else {
 #pragma unroll
     for (int i = 0; i < 4; ++i)
       v[i] = add_pair(v[i], pack_pair(2 * i < n ? -c : 0.f, 2 * i + 1 < n ? -c : 0.f));
@@ -318,7 +323,7 @@ struct RowSum {
 };
 
 // v normed in place (elements past the row's end stay zero); returns 1 / deviation.
-template <int WPR, int J>
+template <bool VEC, int WPR, int J>
 __device__ __forceinline__ float norm_row(float_pair (*v)[4], const int* n, int kind,
                                           float inv_width, float eps, RowSum<WPR>& sum) {
   if (kind == kNormLayer) {
@@ -329,7 +334,7 @@ __device__ __forceinline__ float norm_row(float_pair (*v)[4], const int* n, int 
       for (int i = 0; i < 4; ++i) s = add_pair(s, v[j][i]);
     const float mean = sum.one(sum_pair(s)) * inv_width;
 #pragma unroll
-    for (int j = 0; j < J; ++j) subtract(v[j], n[j], mean);
+    for (int j = 0; j < J; ++j) subtract<VEC>(v[j], n[j], mean);
   }
   float_pair q = both(0.f);
 #pragma unroll

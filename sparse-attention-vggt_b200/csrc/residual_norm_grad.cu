@@ -47,7 +47,7 @@ __device__ __forceinline__ void put_param8(void* p, int type, int64_t at, int n,
 }
 
 // The gradient of what was normed to hat, from that of hat (d, in place).
-template <int WPR, int J>
+template <bool VEC, int WPR, int J>
 __device__ __forceinline__ void norm_back(float_pair (*d)[4], const float_pair (*hat)[4],
                                           const int* n, int kind, float r, float inv_width,
                                           RowSum<WPR>& sum) {
@@ -65,7 +65,7 @@ __device__ __forceinline__ void norm_back(float_pair (*d)[4], const float_pair (
   t *= inv_width;
 #pragma unroll
   for (int j = 0; j < J; ++j) {
-    if (kind == kNormLayer) subtract(d[j], n[j], t);
+    if (kind == kNormLayer) subtract<VEC>(d[j], n[j], t);
 #pragma unroll
     for (int i = 0; i < 4; ++i) d[j][i] = mul_pair(rr, fma_pair(hat[j][i], m, d[j][i]));
   }
@@ -106,31 +106,23 @@ __global__ void __launch_bounds__(kMaxThreads, 1) backward_kernel(const Bwd f) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) acc[k][j][i] = both(0.f);
 
-  // a tensor that is not there is not read
-  const S* x = static_cast<const S*>(a.x) + row0 * a.x_stride + first;
-  const T* b = static_cast<const T*>(a.branch) + (branch ? row0 * a.branch_stride + first : 0);
-  const T* dy = static_cast<const T*>(f.dy) + (has_dy ? row0 * f.dy_stride + first : 0);
-  const S* dh = static_cast<const S*>(f.dh) + (has_dh ? row0 * f.dh_stride + first : 0);
-  S* dx = static_cast<S*>(f.dx) + (f.dx != nullptr ? row0 * f.dx_stride + first : 0);
-  T* db = static_cast<T*>(f.dbranch) + (f.dbranch != nullptr ? row0 * f.dbranch_stride + first : 0);
-  auto ahead = [&] {
-    x += a.x_stride;
-    if (branch) b += a.branch_stride;
-    if (has_dy) dy += f.dy_stride;
-    if (has_dh) dh += f.dh_stride;
-  };
-  // the pointers are a row ahead where rows are copied ahead
-  auto fetch = [&](bool there, int stage) {
-    if (there) {
+  // a row of a tensor (one that is not there is not read); addresses are formed where they are
+  // used, which takes fewer registers than six running pointers
+  auto at = [&](auto* p, int64_t row, int64_t stride) { return p + (row * stride + first); };
+  auto x = [&](int64_t row) { return at(static_cast<const S*>(a.x), row, a.x_stride); };
+  auto b = [&](int64_t row) { return at(static_cast<const T*>(a.branch), row, a.branch_stride); };
+  auto dy = [&](int64_t row) { return at(static_cast<const T*>(f.dy), row, f.dy_stride); };
+  auto dh = [&](int64_t row) { return at(static_cast<const S*>(f.dh), row, f.dh_stride); };
+  auto fetch = [&](int64_t row, int stage) {
+    if (row < row1) {
 #pragma unroll
       for (int j = 0; j < J; ++j)
         if (n[j] > 0) {
-          pipe.fetch(stage, j * kUnits, x + j * step);
-          if (branch) pipe.fetch(stage, j * kUnits + kX, b + j * step);
-          if (has_dy) pipe.fetch(stage, j * kUnits + kX + kF, dy + j * step);
-          if (has_dh) pipe.fetch(stage, j * kUnits + kX + 2 * kF, dh + j * step);
+          pipe.fetch(stage, j * kUnits, x(row) + j * step);
+          if (branch) pipe.fetch(stage, j * kUnits + kX, b(row) + j * step);
+          if (has_dy) pipe.fetch(stage, j * kUnits + kX + kF, dy(row) + j * step);
+          if (has_dh) pipe.fetch(stage, j * kUnits + kX + 2 * kF, dh(row) + j * step);
         }
-      ahead();
     }
     cp_async_commit();
   };
@@ -148,25 +140,25 @@ __global__ void __launch_bounds__(kMaxThreads, 1) backward_kernel(const Bwd f) {
   int64_t gate_end = gates ? (gate_row + 1) * a.rows_per_gate : row1;  // the run's end
   if (!DIRECT) {
     pipe.clear();
-    fetch(row0 < row1, 0);
+    fetch(row0, 0);
   }
   Params<WPR, J, SH, DIRECT> params(a, smem + SH::kAfterRows, first, n, gate_row);
   if (SH::kParams) __syncthreads();
   int stage = 0;
   for (int64_t row = row0; row < row1; ++row, stage ^= 1) {
     if (!DIRECT) {
-      fetch(row + 1 < row1, stage ^ 1);
+      fetch(row + 1, stage ^ 1);
       cp_async_wait<1>();
     }
     float_pair h[J][4], p[J][4], hat[POST ? J : 1][4], d[J][4];
 #pragma unroll
-    for (int j = 0; j < J; ++j) take(x, stage, 0, j, h[j]);
+    for (int j = 0; j < J; ++j) take(x(row), stage, 0, j, h[j]);
     float pr = 0.f;
     if (branch) {
 #pragma unroll
-      for (int j = 0; j < J; ++j) take(b, stage, kX, j, p[j]);
+      for (int j = 0; j < J; ++j) take(b(row), stage, kX, j, p[j]);
       if (POST) {
-        pr = norm_row<WPR, J>(p, n, a.post, inv_width, a.eps, sum);
+        pr = norm_row<!DIRECT, WPR, J>(p, n, a.post, inv_width, a.eps, sum);
 #pragma unroll
         for (int j = 0; j < J; ++j) {
 #pragma unroll
@@ -178,11 +170,11 @@ __global__ void __launch_bounds__(kMaxThreads, 1) backward_kernel(const Bwd f) {
 #pragma unroll
       for (int j = 0; j < J; ++j) params.gated(j, p[j], h[j]);
     }
-    const float r = norm_row<WPR, J>(h, n, a.norm, inv_width, a.eps, sum);  // h is normed now
+    const float r = norm_row<!DIRECT, WPR, J>(h, n, a.norm, inv_width, a.eps, sum);  // h is normed now
     if (has_dy) {
 #pragma unroll
       for (int j = 0; j < J; ++j) {
-        take(dy, stage, kX + kF, j, d[j]);
+        take(dy(row), stage, kX + kF, j, d[j]);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           acc[kWeight][j][i] = fma_pair(d[j][i], h[j][i], acc[kWeight][j][i]);
@@ -190,7 +182,7 @@ __global__ void __launch_bounds__(kMaxThreads, 1) backward_kernel(const Bwd f) {
         }
         params.scale(kWeight, j, d[j]);
       }
-      norm_back<WPR, J>(d, h, n, a.norm, r, inv_width, sum);
+      norm_back<!DIRECT, WPR, J>(d, h, n, a.norm, r, inv_width, sum);
     } else {
 #pragma unroll
       for (int j = 0; j < J; ++j)
@@ -201,16 +193,15 @@ __global__ void __launch_bounds__(kMaxThreads, 1) backward_kernel(const Bwd f) {
 #pragma unroll
       for (int j = 0; j < J; ++j) {
         float_pair t[4];
-        take(dh, stage, kX + 2 * kF, j, t);
+        take(dh(row), stage, kX + 2 * kF, j, t);
 #pragma unroll
         for (int i = 0; i < 4; ++i) d[j][i] = add_pair(d[j][i], t[i]);
       }
     }
-    if (DIRECT) ahead();
     if (f.dx != nullptr) {
 #pragma unroll
-      for (int j = 0; j < J; ++j) put_pairs(dx + j * step, n[j], vec, d[j]);
-      dx += f.dx_stride;
+      for (int j = 0; j < J; ++j)
+        put_pairs<!DIRECT>(at(static_cast<S*>(f.dx), row, f.dx_stride) + j * step, n[j], vec, d[j]);
     }
     if (!branch) continue;
 #pragma unroll
@@ -230,12 +221,13 @@ __global__ void __launch_bounds__(kMaxThreads, 1) backward_kernel(const Bwd f) {
         }
         params.scale(kPostWeight, j, d[j]);
       }
-      norm_back<WPR, J>(d, hat, n, a.post, pr, inv_width, sum);
+      norm_back<!DIRECT, WPR, J>(d, hat, n, a.post, pr, inv_width, sum);
     }
     if (f.dbranch != nullptr) {
 #pragma unroll
-      for (int j = 0; j < J; ++j) put_pairs(db + j * step, n[j], vec, d[j]);
-      db += f.dbranch_stride;
+      for (int j = 0; j < J; ++j)
+        put_pairs<!DIRECT>(at(static_cast<T*>(f.dbranch), row, f.dbranch_stride) + j * step, n[j], vec,
+                           d[j]);
     }
     if (gates && (row + 1 == row1 || row + 1 == gate_end)) {
       // the last row here of a run of rows with one gate: its sum goes out
@@ -249,7 +241,7 @@ __global__ void __launch_bounds__(kMaxThreads, 1) backward_kernel(const Bwd f) {
             for (int i = 0; i < 4; ++i) unpack_pair(v[2 * i], v[2 * i + 1], acc[kGate][j][i]);
             put_param8(f.out[kGate], f.out_type[kGate], gate_row * a.width + c, n[j], vec, v);
           } else {
-            put_pairs(f.part[kGate] + (slot + gate_row) * a.width + c, n[j], vec, acc[kGate][j]);
+            put_pairs<!DIRECT>(f.part[kGate] + (slot + gate_row) * a.width + c, n[j], vec, acc[kGate][j]);
           }
 #pragma unroll
           for (int i = 0; i < 4; ++i) acc[kGate][j][i] = both(0.f);
@@ -268,12 +260,12 @@ __global__ void __launch_bounds__(kMaxThreads, 1) backward_kernel(const Bwd f) {
     float* to = f.part[k] + (int64_t)blockIdx.x * a.width;
     if (slots == 1) {
 #pragma unroll
-      for (int j = 0; j < J; ++j) put_pairs(to + first + j * step, n[j], vec, acc[k][j]);
+      for (int j = 0; j < J; ++j) put_pairs<!DIRECT>(to + first + j * step, n[j], vec, acc[k][j]);
     } else {
       __syncthreads();
 #pragma unroll
       for (int j = 0; j < J; ++j)
-        put_pairs(fold + sum.slot * kRow + first + j * step, 8, true, acc[k][j]);
+        put_pairs<true>(fold + sum.slot * kRow + first + j * step, 8, true, acc[k][j]);
       __syncthreads();
       for (int c = threadIdx.x; c < (int)a.width; c += blockDim.x) {
         float s = 0.f;
