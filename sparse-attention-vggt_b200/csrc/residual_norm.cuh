@@ -85,19 +85,21 @@ constexpr uint32_t kSharedBytes = 208 * 1024;
 
 enum { kWeight, kBias, kGate, kPostWeight, kPostBias, kArrays };
 
-// Shared memory of a block: rows to come (UNITS 16-byte units a thread and stage), parameters
-// (all slots' the same), and the slot's gate, which may be one of several.  Parameters that do not
-// fit are read where they are used; rows that do not are DIRECT.
+// Shared memory of a block: rows to come (UNITS 16-byte units a thread and stage) and parameters,
+// all slots' the same but for a gate of several, which each slot has for itself.  Parameters that do
+// not fit are read where they are used; rows that do not are DIRECT.
 template <int WPR, int J, int UNITS, bool DIRECT>
 struct Shared {
   static constexpr uint32_t kRowBytes = kMaxThreads * kStages * UNITS * 16;
-  static constexpr uint32_t kParamBytes = WPR * 32 * J * 32, kGateBytes = kMaxThreads * J * 32;
+  static constexpr uint32_t kParamBytes = WPR * 32 * J * 32, kOwnBytes = kMaxThreads * J * 32;
   static constexpr bool kFits = kRowBytes <= kSharedBytes;
-  // four parameters and the gate
-  static constexpr bool kParams =
-      !DIRECT && kRowBytes + 4 * kParamBytes + kGateBytes <= kSharedBytes;
+  static constexpr bool kParams = !DIRECT && kRowBytes + kArrays * kParamBytes <= kSharedBytes;
+  // room for a gate of each slot's own
+  static constexpr bool kOwnGate =
+      kParams && kRowBytes + 4 * kParamBytes + kOwnBytes <= kSharedBytes;
   static constexpr uint32_t kAfterRows = DIRECT ? 0 : kRowBytes;
-  static constexpr uint32_t kBytes = kAfterRows + (kParams ? 4 * kParamBytes + kGateBytes : 0);
+  static constexpr uint32_t kBytes =
+      kAfterRows + (kParams ? 4 * kParamBytes + (kOwnGate ? kOwnBytes : kParamBytes) : 0);
 };
 
 // The parameters as one thread sees them.
@@ -117,11 +119,15 @@ struct Params {
            : k == kGate  ? a.gate
            : k == kPostWeight ? a.post_weight : a.post_bias;
   }
-  // place of chunk j's half u of parameter k: the gate has a place per thread
+  // whether parameter k lies in shared memory
+  __device__ __forceinline__ bool held(int k) const {
+    return SH::kParams && (k != kGate || SH::kOwnGate || a.rows_per_gate == 0);
+  }
+  // place of chunk j's half u of parameter k
   __device__ __forceinline__ unsigned char* place(int k, int j, int u) const {
-    if (k == kGate)
+    if (k == kGate && SH::kOwnGate)
       return at + 4 * SH::kParamBytes + ((j * 2 + u) * kMaxThreads + threadIdx.x) * 16;
-    const int slot = k < kGate ? k : k - 1;
+    const int slot = k < kGate ? k : k == kGate ? 4 : k - 1;
     return at + slot * SH::kParamBytes +
            ((j * 2 + u) * (WPR * 32) + (int)threadIdx.x % (WPR * 32)) * 16;
   }
@@ -149,7 +155,9 @@ struct Params {
     } else if (SH::kParams) {
 #pragma unroll
       for (int k = 0; k < kArrays; ++k)
-        if (param(k).p != nullptr && (k == kGate || threadIdx.x < WPR * 32)) fill(k);
+        if (param(k).p != nullptr && held(k) &&
+            ((k == kGate && SH::kOwnGate) || threadIdx.x < WPR * 32))
+          fill(k);
     }
   }
   // the gate of another run of rows
@@ -161,7 +169,7 @@ struct Params {
       for (int j = 0; j < J; ++j)
         get_param(a.gate, row * a.width + first + j * kStep, n[j], a.vec,
                   reg[DIRECT ? kGate : 0][DIRECT ? j : 0]);
-    } else if (SH::kParams) {
+    } else if (SH::kOwnGate) {
       fill(kGate);
     }
   }
@@ -169,7 +177,7 @@ struct Params {
     if (DIRECT) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) v[i] = reg[DIRECT ? k : 0][DIRECT ? j : 0][i];
-    } else if (SH::kParams) {
+    } else if (held(k)) {
       const ulonglong2 lo = *reinterpret_cast<const ulonglong2*>(place(k, j, 0));
       const ulonglong2 hi = *reinterpret_cast<const ulonglong2*>(place(k, j, 1));
       v[0] = lo.x, v[1] = lo.y, v[2] = hi.x, v[3] = hi.y;

@@ -71,9 +71,17 @@ __device__ __forceinline__ void norm_back(float_pair (*d)[4], const float_pair (
   }
 }
 
-template <typename S, typename T, int WPR, int J, bool POST, bool DIRECT>
+// POST: a norm of the branch.  Its sums are three without biases' gradients (POST 1) or five (2);
+// without it they are three.
+template <int POST>
+constexpr int acc_of(int k) {
+  return POST != 1 ? k : k == kWeight ? 0 : k == kGate ? 1 : k == kPostWeight ? 2 : -1;
+}
+
+template <typename S, typename T, int WPR, int J, int POST, bool DIRECT>
 __global__ void __launch_bounds__(kMaxThreads, 1) backward_kernel(const Bwd f) {
-  constexpr int kAccs = POST ? 5 : 3;
+  constexpr int kAccs = POST == 2 ? 5 : 3;
+  constexpr int kGateAcc = acc_of<POST>(kGate), kPostAcc = POST ? acc_of<POST>(kPostWeight) : 0;
   constexpr int kRow = WPR * 32 * 8 * J;  // columns that a slot holds
   constexpr int kX = sizeof(S) / 2, kF = sizeof(T) / 2, kUnits = 2 * (kX + kF);
   typedef Shared<WPR, J, J * kUnits, DIRECT> SH;
@@ -150,25 +158,29 @@ __global__ void __launch_bounds__(kMaxThreads, 1) backward_kernel(const Bwd f) {
       fetch(row + 1, stage ^ 1);
       cp_async_wait<1>();
     }
-    float_pair h[J][4], p[J][4], hat[POST ? J : 1][4], d[J][4];
+    // the branch: as it is, or normed; what is added is formed from it again where it is needed
+    float_pair h[J][4], p[J][4], d[J][4];
+    auto added = [&](int j, float_pair* v) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = p[j][i];
+      if (POST) {
+        params.scale(kPostWeight, j, v);
+        params.shift(kPostBias, j, v);
+      }
+    };
 #pragma unroll
     for (int j = 0; j < J; ++j) take(x(row), stage, 0, j, h[j]);
     float pr = 0.f;
     if (branch) {
 #pragma unroll
       for (int j = 0; j < J; ++j) take(b(row), stage, kX, j, p[j]);
-      if (POST) {
-        pr = norm_row<!DIRECT, WPR, J>(p, n, a.post, inv_width, a.eps, sum);
+      if (POST) pr = norm_row<!DIRECT, WPR, J>(p, n, a.post, inv_width, a.eps, sum);
 #pragma unroll
-        for (int j = 0; j < J; ++j) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) hat[POST ? j : 0][i] = p[j][i];
-          params.scale(kPostWeight, j, p[j]);
-          params.shift(kPostBias, j, p[j]);
-        }
+      for (int j = 0; j < J; ++j) {
+        float_pair v[4];
+        added(j, v);
+        params.gated(j, v, h[j]);
       }
-#pragma unroll
-      for (int j = 0; j < J; ++j) params.gated(j, p[j], h[j]);
     }
     const float r = norm_row<!DIRECT, WPR, J>(h, n, a.norm, inv_width, a.eps, sum);  // h is normed now
     if (has_dy) {
@@ -177,8 +189,9 @@ __global__ void __launch_bounds__(kMaxThreads, 1) backward_kernel(const Bwd f) {
         take(dy(row), stage, kX + kF, j, d[j]);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          acc[kWeight][j][i] = fma_pair(d[j][i], h[j][i], acc[kWeight][j][i]);
-          acc[kBias][j][i] = add_pair(acc[kBias][j][i], d[j][i]);
+          float_pair& w = acc[acc_of<POST>(kWeight)][j][i];
+          w = fma_pair(d[j][i], h[j][i], w);
+          if (POST != 1) acc[kBias % kAccs][j][i] = add_pair(acc[kBias % kAccs][j][i], d[j][i]);
         }
         params.scale(kWeight, j, d[j]);
       }
@@ -206,22 +219,27 @@ __global__ void __launch_bounds__(kMaxThreads, 1) backward_kernel(const Bwd f) {
     if (!branch) continue;
 #pragma unroll
     for (int j = 0; j < J; ++j) {
+      float_pair v[4];
+      added(j, v);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) acc[kGate][j][i] = fma_pair(d[j][i], p[j][i], acc[kGate][j][i]);
+      for (int i = 0; i < 4; ++i) {
+        float_pair& g = acc[kGateAcc][j][i];
+        g = fma_pair(d[j][i], v[i], g);
+      }
       params.scale(kGate, j, d[j]);
     }
     if (POST) {
 #pragma unroll
       for (int j = 0; j < J; ++j) {
-        float_pair(&aw)[4] = acc[kPostWeight % kAccs][j], (&ab)[4] = acc[kPostBias % kAccs][j];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          aw[i] = fma_pair(d[j][i], hat[POST ? j : 0][i], aw[i]);
-          ab[i] = add_pair(ab[i], d[j][i]);
+          float_pair& w = acc[kPostAcc][j][i];
+          w = fma_pair(d[j][i], p[j][i], w);
+          if (POST == 2) acc[kPostBias % kAccs][j][i] = add_pair(acc[kPostBias % kAccs][j][i], d[j][i]);
         }
         params.scale(kPostWeight, j, d[j]);
       }
-      norm_back<!DIRECT, WPR, J>(d, hat, n, a.post, pr, inv_width, sum);
+      norm_back<!DIRECT, WPR, J>(d, p, n, a.post, pr, inv_width, sum);
     }
     if (f.dbranch != nullptr) {
 #pragma unroll
@@ -238,13 +256,13 @@ __global__ void __launch_bounds__(kMaxThreads, 1) backward_kernel(const Bwd f) {
           if (a.rows_per_gate == 1) {
             float v[8];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) unpack_pair(v[2 * i], v[2 * i + 1], acc[kGate][j][i]);
+            for (int i = 0; i < 4; ++i) unpack_pair(v[2 * i], v[2 * i + 1], acc[kGateAcc][j][i]);
             put_param8(f.out[kGate], f.out_type[kGate], gate_row * a.width + c, n[j], vec, v);
           } else {
-            put_pairs<!DIRECT>(f.part[kGate] + (slot + gate_row) * a.width + c, n[j], vec, acc[kGate][j]);
+            put_pairs<!DIRECT>(f.part[kGate] + (slot + gate_row) * a.width + c, n[j], vec, acc[kGateAcc][j]);
           }
 #pragma unroll
-          for (int i = 0; i < 4; ++i) acc[kGate][j][i] = both(0.f);
+          for (int i = 0; i < 4; ++i) acc[kGateAcc][j][i] = both(0.f);
         }
       }
       ++gate_row;
@@ -255,21 +273,24 @@ __global__ void __launch_bounds__(kMaxThreads, 1) backward_kernel(const Bwd f) {
   cp_async_wait<0>();
 
 #pragma unroll
-  for (int k = 0; k < kAccs; ++k) {
-    if (f.out[k] == nullptr || (k == kGate && gates)) continue;  // the same for all threads
+  for (int k = 0; k < (POST ? kArrays : 3); ++k) {
+    constexpr int kLast = kAccs - 1;
+    const int q = acc_of<POST>(k);  // known at compile time
+    if (q < 0 || f.out[k] == nullptr || (k == kGate && gates)) continue;  // the same for all threads
+    const float_pair(&sums)[J][4] = acc[q < 0 ? kLast : q];
     float* to = f.part[k] + (int64_t)blockIdx.x * a.width;
     if (slots == 1) {
 #pragma unroll
-      for (int j = 0; j < J; ++j) put_pairs<!DIRECT>(to + first + j * step, n[j], vec, acc[k][j]);
+      for (int j = 0; j < J; ++j) put_pairs<!DIRECT>(to + first + j * step, n[j], vec, sums[j]);
     } else {
       __syncthreads();
 #pragma unroll
       for (int j = 0; j < J; ++j)
-        put_pairs<true>(fold + sum.slot * kRow + first + j * step, 8, true, acc[k][j]);
+        put_pairs<true>(fold + sum.slot * kRow + first + j * step, 8, true, sums[j]);
       __syncthreads();
       for (int c = threadIdx.x; c < (int)a.width; c += blockDim.x) {
         float s = 0.f;
-        for (int q = 0; q < slots; ++q) s += fold[q * kRow + c];
+        for (int o = 0; o < slots; ++o) s += fold[o * kRow + c];
         to[c] = s;
       }
     }
@@ -313,14 +334,14 @@ struct Grid {
   int64_t blocks;
   int slots;
 };
-Grid grid_of(int64_t rows, int64_t width, bool post) {
+Grid grid_of(int64_t rows, int64_t width, int post) {
   constexpr int sms = 148;
-  const int most = kMaxThreads / 32 / row_warps(width, post);
+  const int most = kMaxThreads / 32 / row_warps(width, post == 2);
   const int slots = (int)std::min<int64_t>(most, (rows + sms - 1) / sms);
   return {std::min<int64_t>(sms, (rows + slots - 1) / slots), slots};
 }
 
-template <typename S, typename T, int WPR, int J, bool POST, bool DIRECT>
+template <typename S, typename T, int WPR, int J, int POST, bool DIRECT>
 cudaError_t launch_grid(const Bwd& f, const Grid& g, cudaStream_t stream) {
   constexpr uint32_t rows = Shared<WPR, J, J*(sizeof(S) + sizeof(T)), DIRECT>::kBytes;
   constexpr uint32_t fold = kMaxThreads * 8 * J * 4;
@@ -332,7 +353,7 @@ cudaError_t launch_grid(const Bwd& f, const Grid& g, cudaStream_t stream) {
   return cudaGetLastError();
 }
 
-template <typename S, typename T, int WPR, int J, bool POST>
+template <typename S, typename T, int WPR, int J, int POST>
 cudaError_t launch_back(const Bwd& f, const Grid& g, cudaStream_t stream) {
   constexpr bool fits = Shared<WPR, J, J*(sizeof(S) + sizeof(T)), false>::kFits;
   if constexpr (fits)
@@ -341,41 +362,46 @@ cudaError_t launch_back(const Bwd& f, const Grid& g, cudaStream_t stream) {
   return launch_grid<S, T, WPR, J, POST, true>(f, g, stream);
 }
 
-template <typename S, typename T>
-cudaError_t launch_back_types(const Bwd& f, const Grid& g, cudaStream_t stream) {
+template <typename S, typename T, int POST>
+cudaError_t launch_back_wide(const Bwd& f, const Grid& g, cudaStream_t stream) {
   const int64_t w = f.a.width;
-  if (f.a.post != 0) {
-    if (w <= 256) return launch_back<S, T, 1, 1, true>(f, g, stream);
-    if (w <= 512) return launch_back<S, T, 2, 1, true>(f, g, stream);
-    if (w <= 1024) return launch_back<S, T, 4, 1, true>(f, g, stream);
-    if (w <= 2048) return launch_back<S, T, 8, 1, true>(f, g, stream);
-    if (w <= 4096) return launch_back<S, T, 16, 1, true>(f, g, stream);
-    if (w <= 8192) return launch_back<S, T, 16, 2, true>(f, g, stream);
-    return launch_back<S, T, 16, 4, true>(f, g, stream);
-  }
-  if (w <= 256) return launch_back<S, T, 1, 1, false>(f, g, stream);
-  if (w <= 512) return launch_back<S, T, 1, 2, false>(f, g, stream);
-  if (w <= 1024) return launch_back<S, T, 2, 2, false>(f, g, stream);
-  if (w <= 2048) return launch_back<S, T, 4, 2, false>(f, g, stream);
-  if (w <= 4096) return launch_back<S, T, 8, 2, false>(f, g, stream);
-  if (w <= 8192) return launch_back<S, T, 16, 2, false>(f, g, stream);
-  return launch_back<S, T, 16, 4, false>(f, g, stream);
+  if (w <= 256) return launch_back<S, T, 1, 1, POST>(f, g, stream);
+  if (w <= 512) return launch_back<S, T, 1, 2, POST>(f, g, stream);
+  if (w <= 1024) return launch_back<S, T, 2, 2, POST>(f, g, stream);
+  if (w <= 2048) return launch_back<S, T, 4, 2, POST>(f, g, stream);
+  if (w <= 4096) return launch_back<S, T, 8, 2, POST>(f, g, stream);
+  if (w <= 8192) return launch_back<S, T, 16, 2, POST>(f, g, stream);
+  return launch_back<S, T, 16, 4, POST>(f, g, stream);
 }
 
-cudaError_t launch_residual_norm_grad(const Bwd& f, const Grid& g, int64_t gates,
+template <typename S, typename T>
+cudaError_t launch_back_types(const Bwd& f, const Grid& g, int post, cudaStream_t stream) {
+  const int64_t w = f.a.width;
+  if (post == 0) return launch_back_wide<S, T, 0>(f, g, stream);
+  if (post == 1) return launch_back_wide<S, T, 1>(f, g, stream);
+  if (w <= 256) return launch_back<S, T, 1, 1, 2>(f, g, stream);
+  if (w <= 512) return launch_back<S, T, 2, 1, 2>(f, g, stream);
+  if (w <= 1024) return launch_back<S, T, 4, 1, 2>(f, g, stream);
+  if (w <= 2048) return launch_back<S, T, 8, 1, 2>(f, g, stream);
+  if (w <= 4096) return launch_back<S, T, 16, 1, 2>(f, g, stream);
+  if (w <= 8192) return launch_back<S, T, 16, 2, 2>(f, g, stream);
+  return launch_back<S, T, 16, 4, 2>(f, g, stream);
+}
+
+cudaError_t launch_residual_norm_grad(const Bwd& f, const Grid& g, int post, int64_t gates,
                                       cudaStream_t stream) {
   const int s = f.a.stream_type, t = f.a.type;
   cudaError_t e;
   if (s == VGGT_DTYPE_FP32 && t == VGGT_DTYPE_FP32)
-    e = launch_back_types<float, float>(f, g, stream);
+    e = launch_back_types<float, float>(f, g, post, stream);
   else if (s == VGGT_DTYPE_FP32 && t == VGGT_DTYPE_BF16)
-    e = launch_back_types<float, __nv_bfloat16>(f, g, stream);
+    e = launch_back_types<float, __nv_bfloat16>(f, g, post, stream);
   else if (s == VGGT_DTYPE_FP32)
-    e = launch_back_types<float, __half>(f, g, stream);
+    e = launch_back_types<float, __half>(f, g, post, stream);
   else if (t == VGGT_DTYPE_BF16)
-    e = launch_back_types<__nv_bfloat16, __nv_bfloat16>(f, g, stream);
+    e = launch_back_types<__nv_bfloat16, __nv_bfloat16>(f, g, post, stream);
   else
-    e = launch_back_types<__half, __half>(f, g, stream);
+    e = launch_back_types<__half, __half>(f, g, post, stream);
   if (e != cudaSuccess) return e;
   bool any = false;
   for (int k = 0; k < kArrays; ++k) any = any || f.out[k] != nullptr;
@@ -395,9 +421,9 @@ extern "C" size_t vggt_residual_norm_grad_workspace_size(int64_t rows, int64_t w
                                                          int64_t rows_per_gate) {
   using namespace vggt::rnorm;
   if (rows <= 0 || width <= 0 || width > VGGT_NORM_MAX_WIDTH || rows_per_gate < 0) return 0;
-  // with and without a norm of the branch, whichever takes more
+  // the kernel that takes most
   size_t most = 0;
-  for (int post = 0; post < 2; ++post) {
+  for (int post = 0; post < 3; ++post) {
     const Grid g = grid_of(rows, width, post);
     int64_t lines = kArrays * g.blocks;
     if (rows_per_gate > 1) lines += g.blocks * g.slots + rows / rows_per_gate;
@@ -451,7 +477,9 @@ extern "C" int vggt_residual_norm_grad(const vggt_residual_norm_args* args,
     return api_fail("the workspace is too small or not 16-byte aligned");
   f.a.vec = f.a.vec && wide_rows(f.dy, f.dy_stride, f.a.type) && wide_rows(f.dh, f.dh_stride, f.a.stream_type) &&
             wide_rows(f.dx, f.dx_stride, f.a.stream_type) && wide_rows(f.dbranch, f.dbranch_stride, f.a.type);
-  const Grid grid = grid_of(rows, width, f.a.post != 0);
+  const bool biases = outs[kBias] != nullptr || outs[kPostBias] != nullptr;
+  const int post = f.a.post == 0 ? 0 : biases ? 2 : 1;
+  const Grid grid = grid_of(rows, width, post);
   f.slots = std::min(rows, grid.blocks * grid.slots);
   float* at = static_cast<float*>(workspace);
   for (int k = 0; k < kArrays; ++k) {
@@ -462,5 +490,5 @@ extern "C" int vggt_residual_norm_grad(const vggt_residual_norm_args* args,
     at += (k == kGate && f.a.rows_per_gate > 1 ? f.slots + gates : grid.blocks) * width;
     at += (4 - (at - static_cast<float*>(workspace)) % 4) % 4;
   }
-  return api_cuda(launch_residual_norm_grad(f, grid, gates, static_cast<cudaStream_t>(stream)));
+  return api_cuda(launch_residual_norm_grad(f, grid, post, gates, static_cast<cudaStream_t>(stream)));
 }
