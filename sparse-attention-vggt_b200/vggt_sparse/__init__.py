@@ -10,6 +10,7 @@ from . import ops  # noqa: F401  (registers torch.ops.vggt_sparse.*)
 from ._lib import ExtensionMissing, load as load_library  # noqa: F401
 from .assembly import assemble_masks, history_update, select_block_mask  # noqa: F401
 from .block_attention import block_attention, check_status  # noqa: F401
+from .block import GlobalBlock  # noqa: F401
 from .block_ops import linear, residual_norm  # noqa: F401
 from .configs import CONFIGS, LayerConfig  # noqa: F401
 from .estimator import BlockMasks, block_mask_estimate, block_select  # noqa: F401
