@@ -38,6 +38,25 @@ cudaError_t allow_shared(K kernel, int bytes, OncePerDevice* once) {
 
 inline bool units_zero(int64_t a, int64_t b) { return a == 0 || b == 0; }
 
+// Launches a kernel that may begin beside the end of the one before it in the stream: it has to
+// wait (grid_wait, common.cuh) before it reads or writes what others do, in every block.
+template <typename... A, typename... B>
+cudaError_t launch_early(void (*kernel)(A...), dim3 grid, dim3 block, size_t smem,
+                         cudaStream_t stream, B&&... args) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, A(args)...);
+  return e != cudaSuccess ? e : cudaGetLastError();
+}
+
 // estimator.cu
 cudaError_t launch_pool(const void* x, int dtype, int64_t len, int d, int block, int64_t nblocks,
                         const int32_t* head_ids, int64_t n_slots, int64_t heads, float* pooled,

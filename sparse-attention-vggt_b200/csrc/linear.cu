@@ -394,8 +394,7 @@ __global__ void __launch_bounds__(THREADS, 1)
   const uint32_t tmem = misc[0];
   // Up to here the kernel may run beside the end of the one before it in the stream, from here on
   // it has that one's results; the next one may begin its own preparations.
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  grid_wait();
 
   if (warp == 0) {
     // ================= TMA producer =================

@@ -57,8 +57,7 @@ __global__ void __launch_bounds__(most_warps<MT, COLS>() * 32) rows_kernel(const
   __shared__ float part[most_warps<MT, COLS>()][MT * 16 * COLS];  // of each warp
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
   const int g = lane >> 2, t = lane & 3, n0 = blockIdx.x * COLS;
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  grid_wait();
   float c[MT][NT][4];
 #pragma unroll
   for (int i = 0; i < MT; ++i)
@@ -151,17 +150,8 @@ template <typename T, int MT, int COLS>
 static cudaError_t launch(const RowsArgs& a, cudaStream_t stream) {
   // two pieces of 64 to a warp at least
   const int warps = std::max(1, std::min(most_warps<MT, COLS>(), a.k / 128));
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)((a.n + COLS - 1) / COLS));
-  cfg.blockDim = dim3(warps * 32);
-  cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, rows_kernel<T, MT, COLS>, a);
-  return e != cudaSuccess ? e : cudaGetLastError();
+  return launch_early(rows_kernel<T, MT, COLS>, dim3((unsigned)((a.n + COLS - 1) / COLS)),
+                      dim3(warps * 32), 0, stream, a);
 }
 
 template <typename T>

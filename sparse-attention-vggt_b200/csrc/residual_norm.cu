@@ -38,8 +38,12 @@ __global__ void __launch_bounds__(kMaxThreads, 1) forward_kernel(const Fwd f) {
   constexpr int step = 8 * WPR * 32;
   // a run of rows to a slot: gates change seldom
   const int64_t slot = (int64_t)blockIdx.x * slots + sum.slot, all = (int64_t)gridDim.x * slots;
-  int64_t row = slot * a.rows / all;
-  const int64_t end = (slot + 1) * a.rows / all;
+  int64_t row = slot, end = min(slot + 1, a.rows);
+  if (a.rows > all) {
+    row = slot * a.rows / all;
+    end = (slot + 1) * a.rows / all;
+  }
+  grid_wait();
   const S* x = static_cast<const S*>(a.x) + row * a.x_stride + first;
   const T* b = static_cast<const T*>(a.branch) + (branch ? row * a.branch_stride + first : 0);
   S* h = static_cast<S*>(f.h) + (branch ? row * f.h_stride + first : 0);
@@ -48,19 +52,29 @@ __global__ void __launch_bounds__(kMaxThreads, 1) forward_kernel(const Fwd f) {
   auto fetch = [&](bool there, int stage) {
     if (there) {
 #pragma unroll
-      for (int j = 0; j < J; ++j)
-        if (n[j] > 0) {
-          pipe.fetch(stage, j * (kX + kF), x + j * step);
-          if (branch) pipe.fetch(stage, j * (kX + kF) + kX, b + j * step);
-        }
+      for (int j = 0; j < J; ++j) {
+        pipe.fetch(stage, j * (kX + kF), x + j * step, n[j] > 0);
+        if (branch) pipe.fetch(stage, j * (kX + kF) + kX, b + j * step, n[j] > 0);
+      }
       x += a.x_stride;
       if (branch) b += a.branch_stride;
     }
     cp_async_commit();
   };
+  // what DIRECT has of the row to come: all of it at once
+  Raw8 xr[J], br[J];
+  auto ahead = [&] {
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+      xr[j].load(x, TypeOf<S>::value, j * step, n[j]);
+      if (branch) br[j].load(b, TypeOf<T>::value, j * step, n[j]);
+    }
+  };
   if (!DIRECT) {
     pipe.clear();
     fetch(row < end, 0);
+  } else if (vec && row < end) {
+    ahead();
   }
   const bool gates = a.gate.p != nullptr && a.rows_per_gate > 0;
   int64_t gate_row = gates ? min(row, a.rows - 1) / a.rows_per_gate : 0;
@@ -72,14 +86,22 @@ __global__ void __launch_bounds__(kMaxThreads, 1) forward_kernel(const Fwd f) {
     if (DIRECT) {
 #pragma unroll
       for (int j = 0; j < J; ++j) {
-        get_pairs(x + j * step, n[j], vec, v[j]);
-        if (branch) get_pairs(b + j * step, n[j], vec, p[j]);
+        if (vec) {
+          xr[j].convert(v[j]);
+          if (branch) br[j].convert(p[j]);
+        } else {
+          get_pairs(x + j * step, n[j], false, v[j]);
+          if (branch) get_pairs(b + j * step, n[j], false, p[j]);
+        }
       }
       x += a.x_stride;
       if (branch) b += a.branch_stride;
+      if (vec && row + 1 < end) ahead();
     } else {
+      __syncwarp();  // all lanes are done with the stage
       fetch(row + 1 < end, stage ^ 1);
       cp_async_wait<1>();
+      __syncwarp();
 #pragma unroll
       for (int j = 0; j < J; ++j) {
         pipe.template read<S>(stage, j * (kX + kF), v[j]);
@@ -102,7 +124,10 @@ __global__ void __launch_bounds__(kMaxThreads, 1) forward_kernel(const Fwd f) {
 #pragma unroll
       for (int j = 0; j < J; ++j) {
         params.gated(j, p[j], v[j]);
-        put_pairs<!DIRECT>(h + j * step, n[j], vec, v[j]);
+        if (DIRECT)
+          put_pairs<false>(h + j * step, n[j], vec, v[j]);
+        else
+          pipe.store(stage, j * (kX + kF), h + j * step, n[j] > 0, v[j]);
       }
       h += f.h_stride;
     }
@@ -111,7 +136,11 @@ __global__ void __launch_bounds__(kMaxThreads, 1) forward_kernel(const Fwd f) {
     for (int j = 0; j < J; ++j) {
       params.scale(kWeight, j, v[j]);
       params.shift(kBias, j, v[j]);
-      put_pairs<!DIRECT>(y + j * step, n[j], vec, v[j]);
+      if (DIRECT)
+        put_pairs<false>(y + j * step, n[j], vec, v[j]);
+      else
+        pipe.store(stage, j * (kX + kF) + (sizeof(S) == 4 && sizeof(T) == 4 ? kX : 0), y + j * step,
+                   n[j] > 0, v[j]);
     }
     y += f.y_stride;
   }
@@ -124,33 +153,49 @@ cudaError_t launch_shape(const Fwd& f, int64_t blocks, int slots, cudaStream_t s
   auto k = forward_kernel<S, T, WPR, J, DIRECT>;
   static OncePerDevice allowed;
   if (cudaError_t e = allow_shared(k, (int)bytes, &allowed)) return e;
-  k<<<(unsigned)blocks, slots * WPR * 32, bytes, stream>>>(f);
-  return cudaGetLastError();
+  return launch_early(k, dim3((unsigned)blocks), dim3(slots * WPR * 32), bytes, stream, f);
 }
 
+// Rows copied ahead where they are aligned, fit and are more than the slots; false where not.
 template <typename S, typename T, int WPR, int J>
-cudaError_t launch_rows(const Fwd& f, int sms, cudaStream_t stream) {
+bool launch_ahead(const Fwd& f, int sms, cudaStream_t stream, cudaError_t* e) {
+  constexpr int slots = kMaxThreads / 32 / WPR;
+  if constexpr (Shared<WPR, J, J*(sizeof(S) / 2 + sizeof(T) / 2), false>::kFits)
+    if (f.a.vec && f.a.rows > (int64_t)sms * slots) {
+      *e = launch_shape<S, T, WPR, J, false>(f, sms, slots, stream);
+      return true;
+    }
+  return false;
+}
+
+// Rows read straight into registers: few rows spread over the SMs, each with a slot of its own.
+template <typename S, typename T, int WPR, int J>
+cudaError_t launch_direct(const Fwd& f, int sms, cudaStream_t stream) {
   constexpr int most = kMaxThreads / 32 / WPR;
-  constexpr bool fits = Shared<WPR, J, J*(sizeof(S) / 2 + sizeof(T) / 2), false>::kFits;
-  // few rows: spread over the SMs, each with a slot of its own
   const int slots = (int)std::min<int64_t>(most, (f.a.rows + sms - 1) / sms);
   const int64_t blocks = std::min<int64_t>(sms, (f.a.rows + slots - 1) / slots);
-  if constexpr (fits)
-    if (f.a.vec && f.a.rows > blocks * slots)
-      return launch_shape<S, T, WPR, J, false>(f, blocks, slots, stream);
   return launch_shape<S, T, WPR, J, true>(f, blocks, slots, stream);
 }
 
 template <typename S, typename T>
 cudaError_t launch_types(const Fwd& f, int sms, cudaStream_t stream) {
   const int64_t w = f.a.width;
-  if (w <= 256) return launch_rows<S, T, 1, 1>(f, sms, stream);
-  if (w <= 512) return launch_rows<S, T, 1, 2>(f, sms, stream);
-  if (w <= 1024) return launch_rows<S, T, 2, 2>(f, sms, stream);
-  if (w <= 2048) return launch_rows<S, T, 4, 2>(f, sms, stream);
-  if (w <= 4096) return launch_rows<S, T, 8, 2>(f, sms, stream);
-  if (w <= 8192) return launch_rows<S, T, 16, 2>(f, sms, stream);
-  return launch_rows<S, T, 16, 4>(f, sms, stream);
+  cudaError_t e = cudaSuccess;
+  if (w <= 256    ? launch_ahead<S, T, 1, 1>(f, sms, stream, &e)
+      : w <= 512  ? launch_ahead<S, T, 1, 2>(f, sms, stream, &e)
+      : w <= 1024 ? launch_ahead<S, T, 2, 2>(f, sms, stream, &e)
+      : w <= 2048 ? launch_ahead<S, T, 4, 2>(f, sms, stream, &e)
+      : w <= 4096 ? launch_ahead<S, T, 8, 2>(f, sms, stream, &e)
+      : w <= 8192 ? launch_ahead<S, T, 16, 2>(f, sms, stream, &e)
+                  : launch_ahead<S, T, 16, 4>(f, sms, stream, &e))
+    return e;
+  if (w <= 256) return launch_direct<S, T, 1, 1>(f, sms, stream);
+  if (w <= 512) return launch_direct<S, T, 1, 2>(f, sms, stream);
+  if (w <= 1024) return launch_direct<S, T, 2, 2>(f, sms, stream);
+  if (w <= 2048) return launch_direct<S, T, 4, 2>(f, sms, stream);
+  if (w <= 4096) return launch_direct<S, T, 8, 2>(f, sms, stream);
+  if (w <= 8192) return launch_direct<S, T, 16, 2>(f, sms, stream);
+  return launch_direct<S, T, 16, 4>(f, sms, stream);
 }
 
 }  // namespace rnorm

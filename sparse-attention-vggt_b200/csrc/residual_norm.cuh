@@ -17,6 +17,8 @@
 // nothing.
 #pragma once
 
+#include <type_traits>
+
 #include "exp2.cuh"
 #include "vec8.cuh"
 
@@ -81,7 +83,7 @@ struct Args {
 };
 
 constexpr int kStages = 2;
-constexpr uint32_t kSharedBytes = 208 * 1024;
+constexpr uint32_t kSharedBytes = 224 * 1024;
 
 enum { kWeight, kBias, kGate, kPostWeight, kPostBias, kArrays };
 
@@ -100,6 +102,47 @@ struct Shared {
   static constexpr uint32_t kAfterRows = DIRECT ? 0 : kRowBytes;
   static constexpr uint32_t kBytes =
       kAfterRows + (kParams ? 4 * kParamBytes + (kOwnGate ? kOwnBytes : kParamBytes) : 0);
+};
+
+// Eight elements as they lie in memory, converted later: loads of several tensors are in flight at
+// once only if nothing is done with the first before the last is issued.
+struct Raw8 {
+  uint4 a, b;
+  bool fp32, bf16;
+  // of 16-byte aligned memory, n 0 or 8
+  __device__ __forceinline__ void load(const void* base, int type, int64_t at, int n) {
+    fp32 = type == VGGT_DTYPE_FP32;
+    bf16 = type == VGGT_DTYPE_BF16;
+    const unsigned char* p = static_cast<const unsigned char*>(base) + at * (fp32 ? 4 : 2);
+    a = b = make_uint4(0, 0, 0, 0);
+    if (n > 0) {
+      a = *reinterpret_cast<const uint4*>(p);
+      if (fp32) b = *reinterpret_cast<const uint4*>(p + 16);
+    }
+  }
+  __device__ __forceinline__ void convert(float_pair* v) const {
+    const uint32_t w[4] = {a.x, a.y, a.z, a.w}, u[4] = {b.x, b.y, b.z, b.w};
+    if (fp32) {
+      v[0] = pack_pair(__uint_as_float(w[0]), __uint_as_float(w[1]));
+      v[1] = pack_pair(__uint_as_float(w[2]), __uint_as_float(w[3]));
+      v[2] = pack_pair(__uint_as_float(u[0]), __uint_as_float(u[1]));
+      v[3] = pack_pair(__uint_as_float(u[2]), __uint_as_float(u[3]));
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float2 f =
+            bf16 ? ElemOps<__nv_bfloat16>::to_float2(w[i]) : ElemOps<__half>::to_float2(w[i]);
+        v[i] = pack_pair(f.x, f.y);
+      }
+    }
+  }
+};
+
+template <typename E>
+struct TypeOf {
+  static constexpr int value = std::is_same<E, float>::value           ? VGGT_DTYPE_FP32
+                               : std::is_same<E, __nv_bfloat16>::value ? VGGT_DTYPE_BF16
+                                                                       : VGGT_DTYPE_FP16;
 };
 
 // The parameters as one thread sees them.
@@ -144,14 +187,28 @@ struct Params {
   __device__ __forceinline__ Params(const Args& args, unsigned char* smem, int first_, const int* n_,
                                     int64_t gate_row_)
       : a(args), at(smem), first(first_), n(n_), gate_row(gate_row_) {
-    if (DIRECT) {
+    if (DIRECT && a.vec) {
+      Raw8 raw[kArrays][J];
+#pragma unroll
+      for (int k = 0; k < kArrays; ++k)
+        if (param(k).p != nullptr)
+#pragma unroll
+          for (int j = 0; j < J; ++j)
+            raw[k][j].load(param(k).p, param(k).type,
+                           (k == kGate ? gate_row * a.width : 0) + first + j * kStep, n[j]);
+#pragma unroll
+      for (int k = 0; k < kArrays; ++k)
+        if (param(k).p != nullptr)
+#pragma unroll
+          for (int j = 0; j < J; ++j) raw[k][j].convert(reg[DIRECT ? k : 0][DIRECT ? j : 0]);
+    } else if (DIRECT) {
 #pragma unroll
       for (int k = 0; k < kArrays; ++k)
         if (param(k).p != nullptr)
 #pragma unroll
           for (int j = 0; j < J; ++j)
             get_param(param(k), (k == kGate ? gate_row * a.width : 0) + first + j * kStep, n[j],
-                      a.vec, reg[DIRECT ? k : 0][DIRECT ? j : 0]);
+                      false, reg[DIRECT ? k : 0][DIRECT ? j : 0]);
     } else if (SH::kParams) {
 #pragma unroll
       for (int k = 0; k < kArrays; ++k)
@@ -214,37 +271,77 @@ struct Params {
 };
 
 // A thread's chunks of the rows to come: stage, then 16-byte unit, then thread, so that a warp's
-// accesses lie side by side.
+// accesses lie side by side.  A chunk of 8 fp32 elements is two units, and lanes that copied their
+// own would touch every 32-byte sector twice: the warp copies its 64 units in order instead, each to
+// its owner's place, and stores go the same way round (__syncwarp on both sides).  (32 frames, fp32
+// stream: 116 us without.)
 template <int UNITS>
 struct Pipe {
   unsigned char* mine;
-  uint32_t mine_u32;
-  __device__ __forceinline__ explicit Pipe(unsigned char* smem) : mine(smem + threadIdx.x * 16) {
-    mine_u32 = smem_u32(mine);
-  }
+  int lane;
+  __device__ __forceinline__ explicit Pipe(unsigned char* smem)
+      : mine(smem + threadIdx.x * 16), lane(threadIdx.x & 31) {}
   // what is never fetched (past the row's end, tensors that are not there) reads as zeros
   __device__ __forceinline__ void clear() const {
 #pragma unroll
     for (int u = 0; u < kStages * UNITS; ++u)
       *reinterpret_cast<uint4*>(mine + u * (kMaxThreads * 16)) = make_uint4(0, 0, 0, 0);
+    __syncwarp();
   }
-  // chunk `unit0` on of an 8-element group of E
+  __device__ __forceinline__ unsigned char* place(int stage, int unit, int owner) const {
+    return mine + (stage * UNITS + unit) * (kMaxThreads * 16) + (owner - lane) * 16;
+  }
+  // a chunk of the row that `p` (this lane's elements) lies in, `there` for this lane's elements
   template <typename E>
-  __device__ __forceinline__ void fetch(int stage, int unit0, const E* p) const {
+  __device__ __forceinline__ void fetch(int stage, int unit0, const E* p, bool there) const {
+    if (sizeof(E) == 2) {
+      if (there) cp_async_16(smem_u32(place(stage, unit0, lane)), p, 16);
+      return;
+    }
+    const unsigned lanes = __ballot_sync(0xffffffffu, there);
+    const E* base = p - 8 * lane;
 #pragma unroll
-    for (int u = 0; u < (int)sizeof(E) / 2; ++u)
-      cp_async_16(mine_u32 + (stage * UNITS + unit0 + u) * (kMaxThreads * 16),
-                  reinterpret_cast<const unsigned char*>(p) + 16 * u, 16);
+    for (int k = 0; k < 2; ++k) {
+      const int q = k * 32 + lane, owner = q >> 1;
+      if (lanes >> owner & 1)
+        cp_async_16(smem_u32(place(stage, unit0 + (q & 1), owner)), base + 4 * q, 16);
+    }
   }
   template <typename E>
   __device__ __forceinline__ void read(int stage, int unit0, float_pair* v) const {
-    const unsigned char* p = mine + (stage * UNITS + unit0) * (kMaxThreads * 16);
+    const unsigned char* p = place(stage, unit0, lane);
     if (sizeof(E) == 4) {
       const ulonglong2 lo = *reinterpret_cast<const ulonglong2*>(p);
       const ulonglong2 hi = *reinterpret_cast<const ulonglong2*>(p + kMaxThreads * 16);
       v[0] = lo.x, v[1] = lo.y, v[2] = hi.x, v[3] = hi.y;
     } else {
       get_pairs(reinterpret_cast<const E*>(p), 8, true, v);
+    }
+  }
+  // stores a chunk, by way of the places of one that has been read
+  template <typename E>
+  __device__ __forceinline__ void store(int stage, int unit0, E* p, bool there,
+                                        const float_pair* v) const {
+    if (sizeof(E) == 2) {
+      put_pairs<true>(p, there ? 8 : 0, true, v);
+      return;
+    }
+    const unsigned lanes = __ballot_sync(0xffffffffu, there);
+    *reinterpret_cast<ulonglong2*>(place(stage, unit0, lane)) = make_ulonglong2(v[0], v[1]);
+    *reinterpret_cast<ulonglong2*>(place(stage, unit0 + 1, lane)) = make_ulonglong2(v[2], v[3]);
+    __syncwarp();
+    E* base = p - 8 * lane;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const int q = k * 32 + lane, owner = q >> 1;
+      if (lanes >> owner & 1)
+        *reinterpret_cast<uint4*>(base + 4 * q) =
+            *reinterpret_cast<const uint4*>(place(stage, unit0 + (q & 1), owner));
+    }
+    // places past the row's end keep their zeros
+    if (!there) {
+      *reinterpret_cast<uint4*>(place(stage, unit0, lane)) = make_uint4(0, 0, 0, 0);
+      *reinterpret_cast<uint4*>(place(stage, unit0 + 1, lane)) = make_uint4(0, 0, 0, 0);
     }
   }
 };

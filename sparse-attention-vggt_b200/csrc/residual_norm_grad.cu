@@ -103,9 +103,13 @@ __global__ void __launch_bounds__(kMaxThreads, 1) backward_kernel(const Bwd f) {
   const int first = 8 * (sum.warp * 32 + lane);
   constexpr int step = 8 * WPR * 32;
   const int64_t slot = (int64_t)blockIdx.x * slots + sum.slot;
-  const int64_t row0 = slot < f.slots ? slot * a.rows / f.slots : 0;
-  const int64_t row1 = slot < f.slots ? (slot + 1) * a.rows / f.slots : 0;
+  int64_t row0 = 0, row1 = 0;
+  if (slot < f.slots) {
+    row0 = f.slots == a.rows ? slot : slot * a.rows / f.slots;
+    row1 = f.slots == a.rows ? slot + 1 : (slot + 1) * a.rows / f.slots;
+  }
 
+  grid_wait();
   float_pair acc[kAccs][J][4];
 #pragma unroll
   for (int k = 0; k < kAccs; ++k)
@@ -124,23 +128,36 @@ __global__ void __launch_bounds__(kMaxThreads, 1) backward_kernel(const Bwd f) {
   auto fetch = [&](int64_t row, int stage) {
     if (row < row1) {
 #pragma unroll
-      for (int j = 0; j < J; ++j)
-        if (n[j] > 0) {
-          pipe.fetch(stage, j * kUnits, x(row) + j * step);
-          if (branch) pipe.fetch(stage, j * kUnits + kX, b(row) + j * step);
-          if (has_dy) pipe.fetch(stage, j * kUnits + kX + kF, dy(row) + j * step);
-          if (has_dh) pipe.fetch(stage, j * kUnits + kX + 2 * kF, dh(row) + j * step);
-        }
+      for (int j = 0; j < J; ++j) {
+        const bool in = n[j] > 0;
+        pipe.fetch(stage, j * kUnits, x(row) + j * step, in);
+        if (branch) pipe.fetch(stage, j * kUnits + kX, b(row) + j * step, in);
+        if (has_dy) pipe.fetch(stage, j * kUnits + kX + kF, dy(row) + j * step, in);
+        if (has_dh) pipe.fetch(stage, j * kUnits + kX + 2 * kF, dh(row) + j * step, in);
+      }
     }
     cp_async_commit();
   };
-  // chunk j of one of the row's four tensors
-  auto take = [&](auto* p, int stage, int unit, int j, float_pair* v) {
+  // chunk j of one of the row's four tensors; DIRECT has asked for the row's before
+  Raw8 raw[DIRECT ? 4 : 1][DIRECT ? J : 1];
+  auto ask = [&](int64_t row) {
+#pragma unroll
+    for (int j = 0; j < (DIRECT ? J : 0); ++j) {
+      raw[0][j].load(x(row), TypeOf<S>::value, j * step, n[j]);
+      if (branch) raw[DIRECT ? 1 : 0][j].load(b(row), TypeOf<T>::value, j * step, n[j]);
+      if (has_dy) raw[DIRECT ? 2 : 0][j].load(dy(row), TypeOf<T>::value, j * step, n[j]);
+      if (has_dh) raw[DIRECT ? 3 : 0][j].load(dh(row), TypeOf<S>::value, j * step, n[j]);
+    }
+  };
+  auto take = [&](auto* p, int stage, int which, int j, float_pair* v) {
     typedef std::remove_cv_t<std::remove_pointer_t<decltype(p)>> E;
-    if (DIRECT)
-      get_pairs(p + j * step, n[j], vec, v);
+    constexpr int unit[4] = {0, kX, kX + kF, kX + 2 * kF};
+    if (!DIRECT)
+      pipe.template read<E>(stage, j * kUnits + unit[which], v);
+    else if (vec)
+      raw[DIRECT ? which : 0][DIRECT ? j : 0].convert(v);
     else
-      pipe.template read<E>(stage, j * kUnits + unit, v);
+      get_pairs(p + j * step, n[j], false, v);
   };
 
   const bool gates = a.gate.p != nullptr && a.rows_per_gate > 0;  // a gate per run of rows
@@ -149,14 +166,20 @@ __global__ void __launch_bounds__(kMaxThreads, 1) backward_kernel(const Bwd f) {
   if (!DIRECT) {
     pipe.clear();
     fetch(row0, 0);
+  } else if (vec && row0 < row1) {
+    ask(row0);
   }
   Params<WPR, J, SH, DIRECT> params(a, smem + SH::kAfterRows, first, n, gate_row);
   if (SH::kParams) __syncthreads();
   int stage = 0;
   for (int64_t row = row0; row < row1; ++row, stage ^= 1) {
     if (!DIRECT) {
+      __syncwarp();  // all lanes are done with the stage
       fetch(row + 1, stage ^ 1);
       cp_async_wait<1>();
+      __syncwarp();
+    } else if (vec && row > row0) {
+      ask(row);
     }
     // the branch: as it is, or normed; what is added is formed from it again where it is needed
     float_pair h[J][4], p[J][4], d[J][4];
@@ -173,7 +196,7 @@ __global__ void __launch_bounds__(kMaxThreads, 1) backward_kernel(const Bwd f) {
     float pr = 0.f;
     if (branch) {
 #pragma unroll
-      for (int j = 0; j < J; ++j) take(b(row), stage, kX, j, p[j]);
+      for (int j = 0; j < J; ++j) take(b(row), stage, 1, j, p[j]);
       if (POST) pr = norm_row<!DIRECT, WPR, J>(p, n, a.post, inv_width, a.eps, sum);
 #pragma unroll
       for (int j = 0; j < J; ++j) {
@@ -186,7 +209,7 @@ __global__ void __launch_bounds__(kMaxThreads, 1) backward_kernel(const Bwd f) {
     if (has_dy) {
 #pragma unroll
       for (int j = 0; j < J; ++j) {
-        take(dy(row), stage, kX + kF, j, d[j]);
+        take(dy(row), stage, 2, j, d[j]);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           float_pair& w = acc[acc_of<POST>(kWeight)][j][i];
@@ -206,7 +229,7 @@ __global__ void __launch_bounds__(kMaxThreads, 1) backward_kernel(const Bwd f) {
 #pragma unroll
       for (int j = 0; j < J; ++j) {
         float_pair t[4];
-        take(dh(row), stage, kX + 2 * kF, j, t);
+        take(dh(row), stage, 3, j, t);
 #pragma unroll
         for (int i = 0; i < 4; ++i) d[j][i] = add_pair(d[j][i], t[i]);
       }
@@ -214,7 +237,11 @@ __global__ void __launch_bounds__(kMaxThreads, 1) backward_kernel(const Bwd f) {
     if (f.dx != nullptr) {
 #pragma unroll
       for (int j = 0; j < J; ++j)
-        put_pairs<!DIRECT>(at(static_cast<S*>(f.dx), row, f.dx_stride) + j * step, n[j], vec, d[j]);
+        if (DIRECT)
+          put_pairs<false>(at(static_cast<S*>(f.dx), row, f.dx_stride) + j * step, n[j], vec, d[j]);
+        else
+          pipe.store(stage, j * kUnits, at(static_cast<S*>(f.dx), row, f.dx_stride) + j * step,
+                     n[j] > 0, d[j]);
     }
     if (!branch) continue;
 #pragma unroll
@@ -244,8 +271,12 @@ __global__ void __launch_bounds__(kMaxThreads, 1) backward_kernel(const Bwd f) {
     if (f.dbranch != nullptr) {
 #pragma unroll
       for (int j = 0; j < J; ++j)
-        put_pairs<!DIRECT>(at(static_cast<T*>(f.dbranch), row, f.dbranch_stride) + j * step, n[j], vec,
+        if (DIRECT)
+          put_pairs<false>(at(static_cast<T*>(f.dbranch), row, f.dbranch_stride) + j * step, n[j], vec,
                            d[j]);
+        else
+          pipe.store(stage, j * kUnits + kX,
+                     at(static_cast<T*>(f.dbranch), row, f.dbranch_stride) + j * step, n[j] > 0, d[j]);
     }
     if (gates && (row + 1 == row1 || row + 1 == gate_end)) {
       // the last row here of a run of rows with one gate: its sum goes out
@@ -301,6 +332,7 @@ __global__ void __launch_bounds__(kMaxThreads, 1) backward_kernel(const Bwd f) {
 // gates of runs of rows.  32 columns x 8 lanes over the partials.
 __global__ void __launch_bounds__(256) finish_kernel(const Bwd f, int64_t blocks, int64_t gates) {
   __shared__ float fold[8][32];
+  grid_wait();
   const int cx = threadIdx.x & 31, ry = threadIdx.x >> 5;
   const int64_t width = f.a.width, c = (int64_t)blockIdx.x * 32 + cx;
   const bool runs = blockIdx.y >= kArrays;
@@ -349,8 +381,7 @@ cudaError_t launch_grid(const Bwd& f, const Grid& g, cudaStream_t stream) {
   auto k = backward_kernel<S, T, WPR, J, POST, DIRECT>;
   static OncePerDevice allowed;
   if (cudaError_t e = allow_shared(k, (int)bytes, &allowed)) return e;
-  k<<<(unsigned)g.blocks, g.slots * WPR * 32, bytes, stream>>>(f);
-  return cudaGetLastError();
+  return launch_early(k, dim3((unsigned)g.blocks), dim3(g.slots * WPR * 32), bytes, stream, f);
 }
 
 template <typename S, typename T, int WPR, int J, int POST>
@@ -410,8 +441,7 @@ cudaError_t launch_residual_norm_grad(const Bwd& f, const Grid& g, int post, int
   const int64_t runs = f.a.rows_per_gate > 1 && f.out[kGate] ? gates : 0;
   const dim3 grid((unsigned)((f.a.width + 31) / 32),
                   (unsigned)(kArrays + std::min<int64_t>(runs, 4096)));
-  finish_kernel<<<grid, 256, 0, stream>>>(f, g.blocks, gates);
-  return cudaGetLastError();
+  return launch_early(finish_kernel, grid, dim3(256), 0, stream, f, g.blocks, gates);
 }
 
 }  // namespace rnorm
