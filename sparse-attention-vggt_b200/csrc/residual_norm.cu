@@ -21,12 +21,12 @@ template <typename S, typename T, int WPR, int J, bool DIRECT>
 __global__ void __launch_bounds__(kMaxThreads, 1) forward_kernel(const Fwd f) {
   constexpr int kX = sizeof(S) / 2, kF = sizeof(T) / 2;  // 16-byte units of 8 elements
   constexpr int kUnits = J * (kX + kF);
-  typedef Shared<WPR, J, kUnits, DIRECT> SH;
+  typedef Shared<kMaxThreads, WPR, J, kUnits, DIRECT> SH;
   extern __shared__ __align__(16) unsigned char smem[];
   __shared__ float scratch[2 * 2 * 32];
   const Args& a = f.a;
   RowSum<WPR> sum(scratch);
-  const Pipe<kUnits> pipe(smem);
+  const Pipe<kMaxThreads, kUnits> pipe(smem);
   const int lane = threadIdx.x & 31, slots = (blockDim.x >> 5) / WPR;
   const float inv_width = 1.f / (float)a.width;
   const bool vec = !DIRECT || a.vec, branch = a.branch != nullptr;
@@ -36,10 +36,14 @@ __global__ void __launch_bounds__(kMaxThreads, 1) forward_kernel(const Fwd f) {
     n[j] = max(0, min(8, (int)a.width - 8 * ((j * WPR + sum.warp) * 32 + lane)));
   const int first = 8 * (sum.warp * 32 + lane);
   constexpr int step = 8 * WPR * 32;
-  // a run of rows to a slot: gates change seldom
+  // The slots go over the rows side by side, which keeps what they read and write near each other
+  // in memory; with a gate for each run of rows every slot takes a run of its own instead, so that
+  // gates change seldom.
+  const bool gates = a.gate.p != nullptr && a.rows_per_gate > 0;
   const int64_t slot = (int64_t)blockIdx.x * slots + sum.slot, all = (int64_t)gridDim.x * slots;
-  int64_t row = slot, end = min(slot + 1, a.rows);
-  if (a.rows > all) {
+  int64_t row = slot, end = a.rows;
+  const int64_t step_rows = gates ? 1 : all;
+  if (gates) {
     row = slot * a.rows / all;
     end = (slot + 1) * a.rows / all;
   }
@@ -56,8 +60,8 @@ __global__ void __launch_bounds__(kMaxThreads, 1) forward_kernel(const Fwd f) {
         pipe.fetch(stage, j * (kX + kF), x + j * step, n[j] > 0);
         if (branch) pipe.fetch(stage, j * (kX + kF) + kX, b + j * step, n[j] > 0);
       }
-      x += a.x_stride;
-      if (branch) b += a.branch_stride;
+      x += step_rows * a.x_stride;
+      if (branch) b += step_rows * a.branch_stride;
     }
     cp_async_commit();
   };
@@ -76,12 +80,11 @@ __global__ void __launch_bounds__(kMaxThreads, 1) forward_kernel(const Fwd f) {
   } else if (vec && row < end) {
     ahead();
   }
-  const bool gates = a.gate.p != nullptr && a.rows_per_gate > 0;
   int64_t gate_row = gates ? min(row, a.rows - 1) / a.rows_per_gate : 0;
   int64_t gate_end = gates ? (gate_row + 1) * a.rows_per_gate : a.rows;
   Params<WPR, J, SH, DIRECT> params(a, smem + SH::kAfterRows, first, n, gate_row);
   if (SH::kParams) __syncthreads();
-  for (int stage = 0; row < end; ++row, stage ^= 1) {
+  for (int stage = 0; row < end; row += step_rows, stage ^= 1) {
     float_pair v[J][4], p[J][4];
     if (DIRECT) {
 #pragma unroll
@@ -94,12 +97,12 @@ __global__ void __launch_bounds__(kMaxThreads, 1) forward_kernel(const Fwd f) {
           if (branch) get_pairs(b + j * step, n[j], false, p[j]);
         }
       }
-      x += a.x_stride;
-      if (branch) b += a.branch_stride;
-      if (vec && row + 1 < end) ahead();
+      x += step_rows * a.x_stride;
+      if (branch) b += step_rows * a.branch_stride;
+      if (vec && row + step_rows < end) ahead();
     } else {
       __syncwarp();  // all lanes are done with the stage
-      fetch(row + 1 < end, stage ^ 1);
+      fetch(row + step_rows < end, stage ^ 1);
       cp_async_wait<1>();
       __syncwarp();
 #pragma unroll
@@ -129,7 +132,7 @@ __global__ void __launch_bounds__(kMaxThreads, 1) forward_kernel(const Fwd f) {
         else
           pipe.store(stage, j * (kX + kF), h + j * step, n[j] > 0, v[j]);
       }
-      h += f.h_stride;
+      h += step_rows * f.h_stride;
     }
     norm_row<!DIRECT, WPR, J>(v, n, a.norm, inv_width, a.eps, sum);
 #pragma unroll
@@ -142,14 +145,14 @@ __global__ void __launch_bounds__(kMaxThreads, 1) forward_kernel(const Fwd f) {
         pipe.store(stage, j * (kX + kF) + (sizeof(S) == 4 && sizeof(T) == 4 ? kX : 0), y + j * step,
                    n[j] > 0, v[j]);
     }
-    y += f.y_stride;
+    y += step_rows * f.y_stride;
   }
 }
 
 template <typename S, typename T, int WPR, int J, bool DIRECT>
 cudaError_t launch_shape(const Fwd& f, int64_t blocks, int slots, cudaStream_t stream) {
   constexpr uint32_t bytes =
-      Shared<WPR, J, J*(sizeof(S) / 2 + sizeof(T) / 2), DIRECT>::kBytes;
+      Shared<kMaxThreads, WPR, J, J*(sizeof(S) / 2 + sizeof(T) / 2), DIRECT>::kBytes;
   auto k = forward_kernel<S, T, WPR, J, DIRECT>;
   static OncePerDevice allowed;
   if (cudaError_t e = allow_shared(k, (int)bytes, &allowed)) return e;
@@ -160,7 +163,7 @@ cudaError_t launch_shape(const Fwd& f, int64_t blocks, int slots, cudaStream_t s
 template <typename S, typename T, int WPR, int J>
 bool launch_ahead(const Fwd& f, int sms, cudaStream_t stream, cudaError_t* e) {
   constexpr int slots = kMaxThreads / 32 / WPR;
-  if constexpr (Shared<WPR, J, J*(sizeof(S) / 2 + sizeof(T) / 2), false>::kFits)
+  if constexpr (Shared<kMaxThreads, WPR, J, J*(sizeof(S) / 2 + sizeof(T) / 2), false>::kFits)
     if (f.a.vec && f.a.rows > (int64_t)sms * slots) {
       *e = launch_shape<S, T, WPR, J, false>(f, sms, slots, stream);
       return true;

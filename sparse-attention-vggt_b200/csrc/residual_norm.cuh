@@ -9,12 +9,12 @@
 // one block to an SM, and each of its groups of WPR warps (a slot) works through rows of its own.
 // While it works on one row, its threads copy their chunks of the next one into shared memory
 // (cp.async, where the layout allows 16-byte accesses: `vec`), and the parameters lie there too, in
-// fp32, read once per block: what a thread needs of either is its own, so that no barrier is
-// needed.  (Read from global memory where they are used, the parameters' latencies took half the
-// time: 32 frames of width 1024, fp32 stream, 159 us.)  Few rows, unaligned ones and the widest are
-// read straight into registers, the parameters once for all rows (DIRECT).  All arithmetic is in fp32, in packed pairs; means
-// are formed first and variances from what is left after them, so that a row far from zero loses
-// nothing.
+// fp32, read once per block: what a thread needs of either is its own or its warp's, so that no
+// barrier is needed.  (Read from global memory where they are used, the parameters' latencies took
+// a third of the time: 32 frames of width 1024, fp32 stream, 159 us.)  Few rows, unaligned ones and
+// the widest are read straight into registers, the parameters once for all rows (DIRECT).  All
+// arithmetic is in fp32, in packed pairs; means are formed first and variances from what is left
+// after them, so that a row far from zero loses nothing.
 #pragma once
 
 #include <type_traits>
@@ -90,10 +90,11 @@ enum { kWeight, kBias, kGate, kPostWeight, kPostBias, kArrays };
 // Shared memory of a block: rows to come (UNITS 16-byte units a thread and stage) and parameters,
 // all slots' the same but for a gate of several, which each slot has for itself.  Parameters that do
 // not fit are read where they are used; rows that do not are DIRECT.
-template <int WPR, int J, int UNITS, bool DIRECT>
+template <int TH, int WPR, int J, int UNITS, bool DIRECT>
 struct Shared {
-  static constexpr uint32_t kRowBytes = kMaxThreads * kStages * UNITS * 16;
-  static constexpr uint32_t kParamBytes = WPR * 32 * J * 32, kOwnBytes = kMaxThreads * J * 32;
+  static constexpr int kThreads = TH;
+  static constexpr uint32_t kRowBytes = TH * kStages * UNITS * 16;
+  static constexpr uint32_t kParamBytes = WPR * 32 * J * 32, kOwnBytes = TH * J * 32;
   static constexpr bool kFits = kRowBytes <= kSharedBytes;
   static constexpr bool kParams = !DIRECT && kRowBytes + kArrays * kParamBytes <= kSharedBytes;
   // room for a gate of each slot's own
@@ -169,7 +170,7 @@ struct Params {
   // place of chunk j's half u of parameter k
   __device__ __forceinline__ unsigned char* place(int k, int j, int u) const {
     if (k == kGate && SH::kOwnGate)
-      return at + 4 * SH::kParamBytes + ((j * 2 + u) * kMaxThreads + threadIdx.x) * 16;
+      return at + 4 * SH::kParamBytes + ((j * 2 + u) * SH::kThreads + threadIdx.x) * 16;
     const int slot = k < kGate ? k : k == kGate ? 4 : k - 1;
     return at + slot * SH::kParamBytes +
            ((j * 2 + u) * (WPR * 32) + (int)threadIdx.x % (WPR * 32)) * 16;
@@ -275,7 +276,7 @@ struct Params {
 // own would touch every 32-byte sector twice: the warp copies its 64 units in order instead, each to
 // its owner's place, and stores go the same way round (__syncwarp on both sides).  (32 frames, fp32
 // stream: 116 us without.)
-template <int UNITS>
+template <int TH, int UNITS>
 struct Pipe {
   unsigned char* mine;
   int lane;
@@ -285,11 +286,11 @@ struct Pipe {
   __device__ __forceinline__ void clear() const {
 #pragma unroll
     for (int u = 0; u < kStages * UNITS; ++u)
-      *reinterpret_cast<uint4*>(mine + u * (kMaxThreads * 16)) = make_uint4(0, 0, 0, 0);
+      *reinterpret_cast<uint4*>(mine + u * (TH * 16)) = make_uint4(0, 0, 0, 0);
     __syncwarp();
   }
   __device__ __forceinline__ unsigned char* place(int stage, int unit, int owner) const {
-    return mine + (stage * UNITS + unit) * (kMaxThreads * 16) + (owner - lane) * 16;
+    return mine + (stage * UNITS + unit) * (TH * 16) + (owner - lane) * 16;
   }
   // a chunk of the row that `p` (this lane's elements) lies in, `there` for this lane's elements
   template <typename E>
@@ -312,7 +313,7 @@ struct Pipe {
     const unsigned char* p = place(stage, unit0, lane);
     if (sizeof(E) == 4) {
       const ulonglong2 lo = *reinterpret_cast<const ulonglong2*>(p);
-      const ulonglong2 hi = *reinterpret_cast<const ulonglong2*>(p + kMaxThreads * 16);
+      const ulonglong2 hi = *reinterpret_cast<const ulonglong2*>(p + TH * 16);
       v[0] = lo.x, v[1] = lo.y, v[2] = hi.x, v[3] = hi.y;
     } else {
       get_pairs(reinterpret_cast<const E*>(p), 8, true, v);
@@ -373,7 +374,7 @@ struct RowSum {
     lane = threadIdx.x & 31;
   }
   __device__ __forceinline__ float* row() {
-    float* s = scratch + (turn * (kMaxThreads / 32) + slot * WPR) * 2;
+    float* s = scratch + (turn * 32 + slot * WPR) * 2;
     turn ^= 1;
     return s;
   }

@@ -9,7 +9,7 @@
 //
 // Bound by memory (x, branch, dy, dh read, dx, dbranch written, once each).  A row lies in the
 // registers of WPR warps, 8 or 16 elements a lane: the row's values and the parameters' sums, three
-// to five fp32 numbers an element, fit together.  Each group of warps takes a run of rows; its
+// to five fp32 numbers an element, fit together.  Each group of warps takes rows of its own; its
 // parameters' sums are added over the block's groups in shared memory and written as one partial
 // per block, which a second kernel adds in order.  No atomics: equal calls give equal bits.
 #include <algorithm>
@@ -32,8 +32,8 @@ struct Bwd {
   int out_type[kArrays];
   float* part[kArrays];    // [blocks][width] partial sums; of a gate per run of rows
                            // [slots + gates][width]
-  int64_t slots;           // slots that have rows (one at least): slot s takes the rows
-                           // [s rows / slots, (s + 1) rows / slots)
+  int64_t slots;           // slots that have rows; with gates of runs of rows slot s takes the rows
+                           // [s rows / slots, (s + 1) rows / slots), else every slots-th row
 };
 
 __device__ __forceinline__ void put_param8(void* p, int type, int64_t at, int n, bool vec,
@@ -84,13 +84,13 @@ __global__ void __launch_bounds__(kMaxThreads, 1) backward_kernel(const Bwd f) {
   constexpr int kGateAcc = acc_of<POST>(kGate), kPostAcc = POST ? acc_of<POST>(kPostWeight) : 0;
   constexpr int kRow = WPR * 32 * 8 * J;  // columns that a slot holds
   constexpr int kX = sizeof(S) / 2, kF = sizeof(T) / 2, kUnits = 2 * (kX + kF);
-  typedef Shared<WPR, J, J * kUnits, DIRECT> SH;
+  typedef Shared<kMaxThreads, WPR, J, J * kUnits, DIRECT> SH;
   extern __shared__ __align__(16) unsigned char smem[];
   __shared__ float scratch[2 * 2 * 32];
   float* fold = reinterpret_cast<float*>(smem);  // after the rows
   const Args& a = f.a;
   RowSum<WPR> sum(scratch);
-  const Pipe<J * kUnits> pipe(smem);
+  const Pipe<kMaxThreads, J * kUnits> pipe(smem);
   const int slots = (blockDim.x >> 5) / WPR;
   const int lane = threadIdx.x & 31;
   const float inv_width = 1.f / (float)a.width;
@@ -103,10 +103,13 @@ __global__ void __launch_bounds__(kMaxThreads, 1) backward_kernel(const Bwd f) {
   const int first = 8 * (sum.warp * 32 + lane);
   constexpr int step = 8 * WPR * 32;
   const int64_t slot = (int64_t)blockIdx.x * slots + sum.slot;
+  // side by side over the rows, or with a gate for each run of rows a run to a slot, as forward
+  const bool gates = a.gate.p != nullptr && a.rows_per_gate > 0;
   int64_t row0 = 0, row1 = 0;
+  const int64_t step_rows = gates ? 1 : f.slots;
   if (slot < f.slots) {
-    row0 = f.slots == a.rows ? slot : slot * a.rows / f.slots;
-    row1 = f.slots == a.rows ? slot + 1 : (slot + 1) * a.rows / f.slots;
+    row0 = gates ? slot * a.rows / f.slots : slot;
+    row1 = gates ? (slot + 1) * a.rows / f.slots : a.rows;
   }
 
   grid_wait();
@@ -160,7 +163,6 @@ __global__ void __launch_bounds__(kMaxThreads, 1) backward_kernel(const Bwd f) {
       get_pairs(p + j * step, n[j], false, v);
   };
 
-  const bool gates = a.gate.p != nullptr && a.rows_per_gate > 0;  // a gate per run of rows
   int64_t gate_row = gates ? row0 / a.rows_per_gate : 0;
   int64_t gate_end = gates ? (gate_row + 1) * a.rows_per_gate : row1;  // the run's end
   if (!DIRECT) {
@@ -172,10 +174,10 @@ __global__ void __launch_bounds__(kMaxThreads, 1) backward_kernel(const Bwd f) {
   Params<WPR, J, SH, DIRECT> params(a, smem + SH::kAfterRows, first, n, gate_row);
   if (SH::kParams) __syncthreads();
   int stage = 0;
-  for (int64_t row = row0; row < row1; ++row, stage ^= 1) {
+  for (int64_t row = row0; row < row1; row += step_rows, stage ^= 1) {
     if (!DIRECT) {
       __syncwarp();  // all lanes are done with the stage
-      fetch(row + 1, stage ^ 1);
+      fetch(row + step_rows, stage ^ 1);
       cp_async_wait<1>();
       __syncwarp();
     } else if (vec && row > row0) {
@@ -375,7 +377,7 @@ Grid grid_of(int64_t rows, int64_t width, int post) {
 
 template <typename S, typename T, int WPR, int J, int POST, bool DIRECT>
 cudaError_t launch_grid(const Bwd& f, const Grid& g, cudaStream_t stream) {
-  constexpr uint32_t rows = Shared<WPR, J, J*(sizeof(S) + sizeof(T)), DIRECT>::kBytes;
+  constexpr uint32_t rows = Shared<kMaxThreads, WPR, J, J*(sizeof(S) + sizeof(T)), DIRECT>::kBytes;
   constexpr uint32_t fold = kMaxThreads * 8 * J * 4;
   constexpr uint32_t bytes = rows > fold ? rows : fold;
   auto k = backward_kernel<S, T, WPR, J, POST, DIRECT>;
@@ -386,7 +388,7 @@ cudaError_t launch_grid(const Bwd& f, const Grid& g, cudaStream_t stream) {
 
 template <typename S, typename T, int WPR, int J, int POST>
 cudaError_t launch_back(const Bwd& f, const Grid& g, cudaStream_t stream) {
-  constexpr bool fits = Shared<WPR, J, J*(sizeof(S) + sizeof(T)), false>::kFits;
+  constexpr bool fits = Shared<kMaxThreads, WPR, J, J*(sizeof(S) + sizeof(T)), false>::kFits;
   if constexpr (fits)
     if (f.a.vec && f.a.rows > g.blocks * g.slots)
       return launch_grid<S, T, WPR, J, POST, false>(f, g, stream);
