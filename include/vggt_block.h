@@ -55,10 +55,10 @@ typedef struct vggt_vector {
  *
  * x [rows][inner], or with heads > 1 head-major: [heads][rows][inner / heads]
  * with x_head_stride between heads, read as [rows][inner].  weight
- * [outer][inner], bias and gate [outer], x and z of dtype (BF16 or FP16);
+ * [outer][inner], bias and gate [outer], x of dtype (BF16 or FP16);
  * residual and y [rows][outer] of stream_dtype, which is dtype or FP32.  z
- * [rows][outer], where non-NULL, gets the activation's argument for the
- * backward pass.  residual and y may be the same.
+ * [rows][outer] of z_dtype (dtype or FP32), where non-NULL, gets the
+ * activation's argument for the backward pass.  residual and y may be the same.
  *
  * x and weight are read in place where their rows (and heads, then of a multiple
  * of 64 elements) start on 16 bytes, else copied into the workspace first.
@@ -80,6 +80,7 @@ typedef struct vggt_linear_args {
   const void* residual; /* or NULL */
   int64_t residual_stride;
   int activation;
+  int z_dtype;          /* of z, here and in the backward pass */
 } vggt_linear_args;
 
 size_t vggt_linear_workspace_size(const vggt_linear_args* args);

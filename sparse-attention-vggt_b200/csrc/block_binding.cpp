@@ -366,7 +366,7 @@ struct LinearCall {
   const LinearIn& in;
   at::Tensor x, weight, held[2];
   Rows residual;
-  at::ScalarType type, stream;
+  at::ScalarType type, stream, z_type;
 
   // Checks; nothing is copied before lay_out.
   explicit LinearCall(const LinearIn& call) : in(call) {
@@ -398,6 +398,9 @@ struct LinearCall {
         refuse("residual must have the result's shape");
     }
     a.stream_dtype = dtype_of("residual", stream, true);
+    // the gate's gradient is a sum of what is formed from z: in fp32, so that it rounds but once
+    z_type = in.gate.defined() ? at::kFloat : type;
+    a.z_dtype = dtype_of("z", z_type, true);
   }
 
   std::vector<int64_t> y_shape() const {
@@ -451,7 +454,7 @@ std::pair<at::Tensor, at::Tensor> linear_forward(const LinearIn& in, const at::T
     c.a.residual_stride = c.residual.stride;
   }
   at::Tensor y = out.defined() ? out : at::empty(shape, in.x.options().dtype(c.stream)), z;
-  if (keep) z = at::empty(shape, in.x.options());
+  if (keep) z = at::empty(shape, in.x.options().dtype(c.z_type));
   const size_t bytes = vggt_linear_workspace_size(&c.a);
   at::Tensor ws;
   if (bytes) ws = workspace(bytes, device);

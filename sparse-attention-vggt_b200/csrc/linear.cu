@@ -63,7 +63,7 @@ struct Params {
   const void* bias;
   const void* gate;
   int act;
-  int y_fp32, y_tma, res_tma, z_tma;
+  int y_fp32, z_fp32, y_tma, res_tma, z_tma;
   const void* residual;
   int64_t residual_stride;
   void* y;
@@ -565,7 +565,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       const uint32_t acc = tmem + b * BN + ((uint32_t)(sub * 32) << 16) + g * COLS;
       bool opened = true;
       for (int which = has_z ? 0 : 1; active && ok && which < 2; ++which) {  // z, then y
-        const bool wide = which == 1 && y_wide, res = which == 1 && has_res;
+        const bool wide = which == 1 ? y_wide : p.z_fp32, res = which == 1 && has_res;
         for (int c = 0; c < COLS; c += wide ? 32 : COLS) {
           const int c0 = col + c;  // first column of the use
           if (!SPLIT && c0 >= p.n) break;
@@ -690,14 +690,14 @@ __global__ void __launch_bounds__(THREADS, 1)
             }
           } else {
             __syncwarp();
-            if (which == 0) {
-              copy_rows<COLS * 2>(buf, sub * 32,
-                                  static_cast<T*>(p.z) + (int64_t)r0 * p.z_stride + c0, p.z_stride,
-                                  rows, left, false);
-            } else if (wide) {
-              copy_rows<128>(buf, sub * 32,
-                             static_cast<float*>(p.y) + (int64_t)r0 * p.y_stride + c0, p.y_stride,
-                             rows, left, false);
+            void* const to = which == 0 ? p.z : p.y;
+            const int64_t stride = which == 0 ? p.z_stride : p.y_stride;
+            if (wide) {
+              copy_rows<128>(buf, sub * 32, static_cast<float*>(to) + (int64_t)r0 * stride + c0,
+                             stride, rows, left, false);
+            } else if (which == 0) {
+              copy_rows<COLS * 2>(buf, sub * 32, static_cast<T*>(to) + (int64_t)r0 * stride + c0,
+                                  stride, rows, left, false);
             } else {
               const int head = c0 / 64 / p.y_heads64;
               copy_rows<COLS * 2>(buf, sub * 32,
@@ -751,7 +751,10 @@ __global__ void __launch_bounds__(256)
 #pragma unroll
       for (int j = 0; j < 8; ++j) v[j] += t[j];
     }
-    if (e.z != nullptr) put8(static_cast<T*>(e.z) + r * e.z_stride + c, k, wide, v);
+    if (e.z != nullptr && e.z_type == VGGT_DTYPE_FP32)
+      put8(static_cast<float*>(e.z) + r * e.z_stride + c, k, wide, v);
+    else if (e.z != nullptr)
+      put8(static_cast<T*>(e.z) + r * e.z_stride + c, k, wide, v);
     act::dispatch(e.act, [&](auto kind) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) v[j] = act::value<decltype(kind)::value>(v[j]);
@@ -935,6 +938,7 @@ cudaError_t launch_product(const Plan& plan, int dtype, int64_t m, int64_t n, in
   p.y_head_stride = e.y_head_stride;
   p.z = e.z;
   p.z_stride = e.z_stride;
+  p.z_fp32 = e.z_type == VGGT_DTYPE_FP32;
   if (!plan.split) {
     // columns of a buffer's row, as the kernel's Shape has them
     const int cols = std::max(plan.bnc * plan.cta / GROUPS, 32), y_cols = p.y_fp32 ? 32 : cols;
@@ -942,7 +946,8 @@ cudaError_t launch_product(const Plan& plan, int dtype, int64_t m, int64_t n, in
                        y_cols);
     p.res_tma = e.residual && rows_map(&maps[3], e.residual, e.y_type, e.residual_stride, 0, 1, n, m,
                                        y_cols);
-    p.z_tma = e.z && rows_map(&maps[4], e.z, dtype, e.z_stride, 0, 1, n, m, cols);
+    p.z_tma = e.z && rows_map(&maps[4], e.z, e.z_type, e.z_stride, 0, 1, n, m,
+                              p.z_fp32 ? 32 : cols);
   }
   p.slots = slots;
   p.status = status;
@@ -964,7 +969,7 @@ cudaError_t finish_product(const Plan& plan, int dtype, int64_t m, int64_t n, co
   const unsigned grid = (unsigned)std::min<int64_t>((all + 255) / 256, 148 * 16);
   const bool wide = wide_rows(e.y, e.y_stride, e.y_type) && e.y_dim % 8 == 0 &&
                     (e.y_heads <= 1 || e.y_head_stride % 8 == 0) &&
-                    wide_rows(e.z, e.z_stride, dtype) && wide_rows(e.bias, 8, dtype) &&
+                    wide_rows(e.z, e.z_stride, e.z_type) && wide_rows(e.bias, 8, dtype) &&
                     wide_rows(e.gate, 8, dtype) &&
                     wide_rows(e.residual, e.residual_stride, e.y_type);
   const Slots s = slots_of(plan, slots);
@@ -1071,6 +1076,8 @@ int check(const vggt_linear_args* a) {
     return api_fail("linear requires BF16 or FP16");
   if (a->stream_dtype != a->dtype && a->stream_dtype != VGGT_DTYPE_FP32)
     return api_fail("the residual and y are of x's type or FP32");
+  if (a->activation != VGGT_ACT_NONE && a->z_dtype != a->dtype && a->z_dtype != VGGT_DTYPE_FP32)
+    return api_fail("z is of x's type or FP32");
   if (a->rows < 0 || a->inner < 1 || a->outer < 1) return api_fail("bad size argument");
   if (a->rows > INT_MAX - 512 || a->inner > INT_MAX - 512 || a->outer > INT_MAX - 512)
     return api_fail("too many rows or too wide");
@@ -1131,6 +1138,7 @@ extern "C" int vggt_linear(const vggt_linear_args* a, void* y, int64_t y_stride,
   e.y_type = a->stream_dtype;
   e.z = z;
   e.z_stride = z_stride;
+  e.z_type = a->z_dtype;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   unsigned char* ws = static_cast<unsigned char*>(workspace);
   float* slots = reinterpret_cast<float*>(ws + laid.bytes);

@@ -34,6 +34,7 @@ struct Epilogue {
   int y_type = 0;  // of y and the residual
   void* z = nullptr;
   int64_t z_stride = 0;
+  int z_type = 0;
 };
 
 // How a product is cut: tiles of 128 cta x bnc cta (cta CTAs work on one), dealt out whole to

@@ -37,7 +37,7 @@ struct Sums {
   bool wide;
 };
 
-template <typename S, typename T, int ACT, bool WIDE>
+template <typename S, typename Z, typename T, int ACT, bool WIDE>
 __global__ void __launch_bounds__(256, ACT == VGGT_ACT_NONE ? 4 : 2) sums_kernel(const Sums a) {
   __shared__ float fold[8][256];
   // rows whose loads are in flight (with a branch for unaligned ones in the loop none were, and
@@ -65,7 +65,7 @@ __global__ void __launch_bounds__(256, ACT == VGGT_ACT_NONE ? 4 : 2) sums_kernel
       for (int q = 0; q < kAhead; ++q) {
         const int64_t r = min(rr + 8 * q, r1 - 1);  // past the end the last row, unused
         get(static_cast<const S*>(a.dy) + r * a.dy_stride + c, d[q]);
-        if (ACT != VGGT_ACT_NONE) get(static_cast<const T*>(a.z) + r * a.z_stride + c, z[q]);
+        if (ACT != VGGT_ACT_NONE) get(static_cast<const Z*>(a.z) + r * a.z_stride + c, z[q]);
       }
 #pragma unroll
       for (int q = 0; q < kAhead; ++q) {
@@ -109,17 +109,27 @@ __global__ void __launch_bounds__(256, ACT == VGGT_ACT_NONE ? 4 : 2) sums_kernel
   }
 }
 
-template <typename S, typename T, bool WIDE>
+template <typename S, typename Z, typename T, bool WIDE>
 static void launch_sums(const Sums& a, dim3 grid, cudaStream_t stream) {
   switch (a.act) {
-    case VGGT_ACT_GELU: sums_kernel<S, T, VGGT_ACT_GELU, WIDE><<<grid, 256, 0, stream>>>(a); break;
+    case VGGT_ACT_GELU: sums_kernel<S, Z, T, VGGT_ACT_GELU, WIDE><<<grid, 256, 0, stream>>>(a); break;
     case VGGT_ACT_GELU_TANH:
-      sums_kernel<S, T, VGGT_ACT_GELU_TANH, WIDE><<<grid, 256, 0, stream>>>(a);
+      sums_kernel<S, Z, T, VGGT_ACT_GELU_TANH, WIDE><<<grid, 256, 0, stream>>>(a);
       break;
-    case VGGT_ACT_SILU: sums_kernel<S, T, VGGT_ACT_SILU, WIDE><<<grid, 256, 0, stream>>>(a); break;
-    case VGGT_ACT_RELU: sums_kernel<S, T, VGGT_ACT_RELU, WIDE><<<grid, 256, 0, stream>>>(a); break;
-    default: sums_kernel<S, T, VGGT_ACT_NONE, WIDE><<<grid, 256, 0, stream>>>(a);
+    case VGGT_ACT_SILU: sums_kernel<S, Z, T, VGGT_ACT_SILU, WIDE><<<grid, 256, 0, stream>>>(a); break;
+    case VGGT_ACT_RELU: sums_kernel<S, Z, T, VGGT_ACT_RELU, WIDE><<<grid, 256, 0, stream>>>(a); break;
+    default: sums_kernel<S, T, T, VGGT_ACT_NONE, WIDE><<<grid, 256, 0, stream>>>(a);
   }
+}
+
+template <typename S, typename T>
+static void launch_sums(const Sums& a, bool z_fp32, dim3 grid, cudaStream_t stream) {
+  if (z_fp32)
+    a.wide ? launch_sums<S, float, T, true>(a, grid, stream)
+           : launch_sums<S, float, T, false>(a, grid, stream);
+  else
+    a.wide ? launch_sums<S, T, T, true>(a, grid, stream)
+           : launch_sums<S, T, T, false>(a, grid, stream);
 }
 
 // gate W, rounded once more to W's type: one rounding of dx's factors, as dy gate would be.
@@ -238,8 +248,9 @@ static Back plan_back(const vggt_linear_args* a, const vggt_linear_grads* g) {
               (b.act || a->stream_dtype == VGGT_DTYPE_FP32 ||
                !tma_rows(g->dy, g->dy_stride, a->outer, a->rows));
   if (b.dx && a->gate && !b.act) {
-    // the gate goes to the smaller factor of dx
-    b.scale_dy = a->rows < a->inner;
+    // the gate goes to the smaller factor of dx, or to dy where that is rounded anyway: one
+    // rounding of a factor in either case
+    b.scale_dy = b.copy_dy || a->rows < a->inner;
     b.scale_w = !b.scale_dy;
   }
   b.sums = b.copy_dy || b.scale_dy || (g->dbias && a->bias) || dgate;
@@ -292,13 +303,13 @@ static cudaError_t run_back(const vggt_linear_args* a, const vggt_linear_grads* 
     s.outer = outer;
     s.per_block = b.per_block;
     s.wide = outer % 8 == 0 && wide_rows(g->dy, g->dy_stride, a->stream_dtype) &&
-             (!b.act || wide_rows(g->z, g->z_stride, a->dtype)) && wide_rows(a->gate, 8, a->dtype);
+             (!b.act || wide_rows(g->z, g->z_stride, a->z_dtype)) && wide_rows(a->gate, 8, a->dtype);
     const dim3 grid((unsigned)((outer + 255) / 256), (unsigned)b.row_blocks);
+    const bool z_fp32 = a->z_dtype == VGGT_DTYPE_FP32;
     if (a->stream_dtype == VGGT_DTYPE_FP32)
-      s.wide ? launch_sums<float, T, true>(s, grid, stream)
-             : launch_sums<float, T, false>(s, grid, stream);
+      launch_sums<float, T>(s, z_fp32, grid, stream);
     else
-      s.wide ? launch_sums<T, T, true>(s, grid, stream) : launch_sums<T, T, false>(s, grid, stream);
+      launch_sums<T, T>(s, z_fp32, grid, stream);
     if (cudaError_t e = cudaGetLastError()) return e;
   }
   if (cudaError_t e = copy_operands(a, b.laid, ws, stream)) return e;

@@ -123,7 +123,9 @@ __global__ void __launch_bounds__(most_warps<MT, COLS>() * 32) rows_kernel(const
     float v = 0.f;
     for (int q = 0; q < warps; ++q) v += part[q][i];
     if (e.bias != nullptr) v += (float)static_cast<const T*>(e.bias)[n];
-    if (e.z != nullptr)
+    if (e.z != nullptr && e.z_type == VGGT_DTYPE_FP32)
+      static_cast<float*>(e.z)[r * e.z_stride + n] = v;
+    else if (e.z != nullptr)
       static_cast<T*>(e.z)[r * e.z_stride + n] = ElemOps<T>::from_float(v);
     act::dispatch(e.act, [&](auto k) { v = act::value<decltype(k)::value>(v); });
     if (e.gate != nullptr) v *= (float)static_cast<const T*>(e.gate)[n];

@@ -51,10 +51,11 @@ def linear(x, weight, bias=None, *, activation=None, gate=None, residual=None, h
     distribution), "gelu_tanh", "silu" or "relu"; ``gate`` scales per channel
     (LayerScale).
 
-    x and weight are copied where their rows do not start on 16 bytes or have an
-    inner size that is not a multiple of 8.  For a backward pass the activation's
-    argument is kept, rounded to x's dtype; without an activation x, weight, bias
-    and gate alone are.
+    x and weight are copied where their rows do not start on 16 bytes.  For a
+    backward pass the activation's argument is kept, rounded to x's dtype (with a
+    gate in fp32); without an activation x, weight, bias and gate alone are.
+    Gradients of the products are rounded to x's dtype: with fp16 scale the loss,
+    as ever, where they may fall below its range.
 
     ``out`` (contiguous; may be residual) takes the result where no gradient is
     needed.  ``status``, an int32 tensor, gets VGGT_STATUS_TIMEOUT if a wait of
