@@ -70,6 +70,8 @@ struct Params {
   int64_t y_stride, y_head_stride;
   void* z;
   int64_t z_stride;
+  const void* row_gate;  // see Epilogue
+  float* row_dot;
   float* slots;
   int32_t* status;
   uint64_t wait_ns;
@@ -563,6 +565,12 @@ __global__ void __launch_bounds__(THREADS, 1)
       }
       tc::tc_fence_after();
       const uint32_t acc = tmem + b * BN + ((uint32_t)(sub * 32) << 16) + g * COLS;
+      // of a weight's gradient: this row's gate, and its product with the weight's row
+      float_pair row_gate = pack_pair(1.f, 1.f), dot = pack_pair(0.f, 0.f);
+      if (AMN && !SPLIT && p.row_gate != nullptr && m0 + row < p.m) {
+        const float v = to_float(static_cast<const T*>(p.row_gate)[m0 + row]);
+        row_gate = pack_pair(v, v);
+      }
       bool opened = true;
       for (int which = has_z ? 0 : 1; active && ok && which < 2; ++which) {  // z, then y
         const bool wide = which == 1 ? y_wide : p.z_fp32, res = which == 1 && has_res;
@@ -656,9 +664,15 @@ __global__ void __launch_bounds__(THREADS, 1)
 #pragma unroll
                   for (int e = 0; e < 4; ++e) {
                     const float2 f = ElemOps<T>::to_float2(q[e]);
-                    v[4 * j + e] = add_pair(v[4 * j + e], pack_pair(f.x, f.y));
+                    if (AMN && p.row_dot != nullptr)
+                      dot = fma_pair(v[4 * j + e], pack_pair(f.x, f.y), dot);
+                    else
+                      v[4 * j + e] = add_pair(v[4 * j + e], pack_pair(f.x, f.y));
                   }
                 }
+                if (AMN)
+#pragma unroll
+                  for (int e = 0; e < 4; ++e) v[4 * j + e] = mul_pair(v[4 * j + e], row_gate);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                   float x0, x1;
@@ -669,7 +683,14 @@ __global__ void __launch_bounds__(THREADS, 1)
               }
             }
           }
-          if (SPLIT || (which == 0 ? p.z_tma : p.y_tma)) {
+          if (AMN && !SPLIT && p.row_dot != nullptr && m0 + row < p.m) {
+            float d0, d1;
+            unpack_pair(d0, d1, dot);
+            p.row_dot[(int64_t)(col / COLS) * p.m + m0 + row] = d0 + d1;
+          }
+          if (AMN && !SPLIT && p.y == nullptr) {  // the rows' products alone are wanted
+            group_sync();
+          } else if (SPLIT || (which == 0 ? p.z_tma : p.y_tma)) {
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             group_sync();
             if (t == 0) {
@@ -797,7 +818,7 @@ static int sm_count() {
 // reduction block take, measured alone and (block: + busy) with all SMs at work, and for a split one
 // the partial sums' way through memory and another launch.  Splitting evens the load out where
 // tiles are few or the last round is short.
-Plan plan_product(int64_t m, int64_t n, int64_t red, bool must_split) {
+Plan plan_product(int64_t m, int64_t n, int64_t red) {
   // cta, bnc, a launch, a block, a block's share that grows with the load
   static const int kShapes[][5] = {
       {1, 64, 6500, 420, 40}, {1, 128, 7700, 450, 60}, {2, 64, 8200, 320, 60}, {2, 128, 10500, 530, 80}};
@@ -805,7 +826,7 @@ Plan plan_product(int64_t m, int64_t n, int64_t red, bool must_split) {
   Plan best;
   double least = 0;
   for (const int* shape : kShapes)
-    for (int split = must_split ? 1 : 0; split < 2; ++split) {
+    for (int split = 0; split < 2; ++split) {
       Plan p;
       p.cta = shape[0];
       p.bnc = shape[1];
@@ -828,6 +849,11 @@ Plan plan_product(int64_t m, int64_t n, int64_t red, bool must_split) {
       }
     }
   return best;
+}
+
+int64_t dot_groups(const Plan& plan, int64_t n) {
+  const int cols = std::max(plan.bnc * plan.cta / GROUPS, 32);
+  return (n + cols - 1) / cols;
 }
 
 static bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
@@ -942,13 +968,15 @@ cudaError_t launch_product(const Plan& plan, int dtype, int64_t m, int64_t n, in
   if (!plan.split) {
     // columns of a buffer's row, as the kernel's Shape has them
     const int cols = std::max(plan.bnc * plan.cta / GROUPS, 32), y_cols = p.y_fp32 ? 32 : cols;
-    p.y_tma = rows_map(&maps[2], e.y, e.y_type, e.y_stride, e.y_head_stride, e.y_heads, e.y_dim, m,
+    p.y_tma = e.y && rows_map(&maps[2], e.y, e.y_type, e.y_stride, e.y_head_stride, e.y_heads, e.y_dim, m,
                        y_cols);
     p.res_tma = e.residual && rows_map(&maps[3], e.residual, e.y_type, e.residual_stride, 0, 1, n, m,
                                        y_cols);
     p.z_tma = e.z && rows_map(&maps[4], e.z, e.z_type, e.z_stride, 0, 1, n, m,
                               p.z_fp32 ? 32 : cols);
   }
+  p.row_gate = e.row_gate;
+  p.row_dot = e.row_dot;
   p.slots = slots;
   p.status = status;
   p.wait_ns = api_wait_ns();
@@ -1106,7 +1134,7 @@ extern "C" size_t vggt_linear_workspace_size(const vggt_linear_args* a) {
   if (!a || a->rows <= 0 || a->inner < 1 || a->outer < 1) return 0;
   const size_t copies = plan_operands(a, true, true).bytes;
   if (few_rows(a->rows, a->outer, a->inner)) return copies;
-  return copies + plan_product(a->rows, a->outer, a->inner, false).slot_bytes();
+  return copies + plan_product(a->rows, a->outer, a->inner).slot_bytes();
 }
 
 extern "C" int vggt_linear(const vggt_linear_args* a, void* y, int64_t y_stride, void* z,
@@ -1121,7 +1149,7 @@ extern "C" int vggt_linear(const vggt_linear_args* a, void* y, int64_t y_stride,
     return api_fail("an output's rows overlap: its stride is below outer");
   const Laid laid = plan_operands(a, true, true);
   const bool few = few_rows(a->rows, a->outer, a->inner);
-  const Plan plan = few ? Plan{} : plan_product(a->rows, a->outer, a->inner, false);
+  const Plan plan = few ? Plan{} : plan_product(a->rows, a->outer, a->inner);
   const size_t bytes = laid.bytes + plan.slot_bytes();
   if (bytes > 0 && (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 255u) ||
                     workspace_bytes < bytes))

@@ -35,6 +35,12 @@ struct Epilogue {
   void* z = nullptr;
   int64_t z_stride = 0;
   int z_type = 0;
+  // of a weight's gradient C [outer][inner] that is not split: rows scaled by row_gate, and where
+  // row_dot is given their products (unscaled) with the rows of `residual`, which is then not
+  // added: one sum for each row and each of dot_groups pieces of columns, [dot_groups][m].  y may
+  // be null then.
+  const void* row_gate = nullptr;
+  float* row_dot = nullptr;
 };
 
 // How a product is cut: tiles of 128 cta x bnc cta (cta CTAs work on one), dealt out whole to
@@ -46,7 +52,9 @@ struct Plan {
   size_t slot_bytes() const;                     // partial sums of a split product
 };
 
-Plan plan_product(int64_t m, int64_t n, int64_t red, bool must_split);
+Plan plan_product(int64_t m, int64_t n, int64_t red);
+// pieces of columns in which a row's product with another is summed (Epilogue::row_dot)
+int64_t dot_groups(const Plan& plan, int64_t n);
 
 // A split product's partial sums.  All tiles' reduction blocks, one tile after the other, are dealt
 // out in runs: the first `rest` workers take per + 1 of them, the others per.  Worker w's part of

@@ -6,10 +6,10 @@
 //   dW = gate G,  db = gate s,  dgate_n = <W_n, G_n> + b_n s_n,  dx = dy (gate W):
 // the only pass over [rows][outer] beside the two products is the one that forms s.
 //
-// dW is a product over the rows.  With a gate and no activation, or where its tiles are few, it is
-// cut evenly over the SMs; the partial sums lie in fp32 in the workspace until finish_weight adds
-// them, scales them by the gate and forms the row products of dgate.  Nothing is added with
-// atomics: equal calls give equal bits.
+// dW is a product over the rows.  Its epilogue scales the rows by the gate and sums their products
+// with W's rows for dgate.  Where its tiles are few it is cut evenly over the SMs, and the partial
+// sums lie in fp32 in the workspace until finish_weight adds them and does the same.  Nothing is
+// added with atomics: equal calls give equal bits.
 #include <algorithm>
 #include <type_traits>
 
@@ -166,6 +166,8 @@ struct Weights {
   const float* gate_part;
   int64_t row_blocks, outer, inner;
   bool product;  // whether there are partial sums of a product
+  const float* dots;  // or its rows' products with W's, [dot_groups][outer]
+  int64_t dot_groups;
   bool wide;
 };
 
@@ -213,6 +215,8 @@ __global__ void __launch_bounds__(128) finish_weight_kernel(const Slots s, const
   float g = 0.f;
   if (a.act) {
     for (int64_t i = threadIdx.x; i < a.row_blocks; i += 128) g += a.gate_part[i * a.outer + r];
+  } else if (a.dots != nullptr) {
+    for (int64_t i = threadIdx.x; i < a.dot_groups; i += 128) g += a.dots[i * a.outer + r];
   } else {
     g = dot;
   }
@@ -225,11 +229,11 @@ __global__ void __launch_bounds__(128) finish_weight_kernel(const Slots s, const
 
 // What a backward call does, and where its workspace lies (offsets in bytes).
 struct Back {
-  bool act, dx, product, sums, copy_dy, scale_dy, scale_w;
+  bool act, dx, product, dot, sums, copy_dy, scale_dy, scale_w;
   int64_t row_blocks, per_block, pad;  // pad: row stride of dz
   Laid laid;
   Plan px, pw;
-  size_t dz, scaled, weight, bias_part, gate_part, slots, bytes;
+  size_t dz, scaled, weight, bias_part, gate_part, dots, slots, bytes;
 };
 
 static bool tma_rows(const void* p, int64_t stride, int64_t width, int64_t rows) {
@@ -271,8 +275,10 @@ static Back plan_back(const vggt_linear_args* a, const vggt_linear_grads* g) {
   b.weight = take(b.scale_w, (size_t)a->outer * b.laid.pad * 2);
   b.bias_part = take(b.sums, (size_t)b.row_blocks * a->outer * 4);
   b.gate_part = take(b.sums && b.act, (size_t)b.row_blocks * a->outer * 4);
-  if (b.dx) b.px = plan_product(a->rows, a->inner, a->outer, false);
-  if (b.product) b.pw = plan_product(a->outer, a->inner, a->rows, a->gate && !b.act);
+  if (b.dx) b.px = plan_product(a->rows, a->inner, a->outer);
+  if (b.product) b.pw = plan_product(a->outer, a->inner, a->rows);
+  b.dot = b.product && !b.pw.split && dgate && !b.act;
+  b.dots = take(b.dot, b.dot ? (size_t)dot_groups(b.pw, a->inner) * a->outer * 4 : 0);
   // the products run one after the other
   b.slots = take(true, std::max(b.dx ? b.px.slot_bytes() : 0, b.product ? b.pw.slot_bytes() : 0));
   return b;
@@ -349,6 +355,12 @@ static cudaError_t run_back(const vggt_linear_args* a, const vggt_linear_grads* 
     e.y_stride = g->dweight_stride;
     e.y_dim = inner;
     e.y_type = a->dtype;
+    if (a->gate && !b.act) e.row_gate = a->gate;
+    if (b.dot) {
+      e.residual = weight.p;
+      e.residual_stride = weight.stride;
+      e.row_dot = reinterpret_cast<float*>(ws + b.dots);
+    }
     if (cudaError_t rc = launch_product(b.pw, a->dtype, outer, inner, rows,
                                         matrix(dz, outer, dz_stride, true),
                                         x_operand(a, b.laid, ws, true), e, slots, status, stream))
@@ -372,6 +384,8 @@ static cudaError_t run_back(const vggt_linear_args* a, const vggt_linear_grads* 
   f.outer = outer;
   f.inner = inner;
   f.product = partial;
+  f.dots = b.dot ? reinterpret_cast<float*>(ws + b.dots) : nullptr;
+  f.dot_groups = b.dot ? dot_groups(b.pw, inner) : 0;
   f.wide = wide_rows(g->dweight, g->dweight_stride, a->dtype);
   const Slots s = partial ? slots_of(b.pw, slots) : Slots{};
   finish_weight_kernel<T><<<(unsigned)outer, 128, 0, stream>>>(s, f);

@@ -679,3 +679,23 @@ def test_operators_on_a_device_that_is_not_current(cuda):
     n.check_all()
     with pytest.raises(ValueError, match="one device"):
         vggt_sparse.linear(c.x, c.w.to(cuda))
+
+
+@pytest.mark.parametrize("rows,inner,outer", [(1, 64, 64), (90, 520, 1040), (700, 1001, 130),
+                                              (5000, 1032, 2000)])
+@pytest.mark.parametrize("bias", [False, True])
+def test_gate_gradients_by_themselves(cuda, rows, inner, outer, bias):
+    """Every subset of weight, bias and gate: dgate with dW from the tiles, and without it from
+    partial sums, is the same to its bounds."""
+    c = Linear(cuda, rows, inner, outer, FP, gate=True, bias=bias, seed=rows)
+    x = c.x
+    for mask in range(1, 8):
+        leaves = [t for i, t in enumerate((c.w, c.b, c.g)) if mask >> i & 1 and t is not None]
+        for t in (c.w, c.b, c.g):
+            if t is not None:
+                t.requires_grad_(any(t is u for u in leaves))
+        if not leaves:
+            continue
+        grads = dict(zip(map(id, leaves), torch.autograd.grad(c.call(), leaves, c.dy)))
+        c.check_grads(None, *(grads.get(id(t)) for t in (c.w, c.b, c.g)))
+    assert not x.requires_grad
