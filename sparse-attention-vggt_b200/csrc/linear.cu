@@ -689,6 +689,7 @@ __global__ void __launch_bounds__(THREADS, 1)
             p.row_dot[(int64_t)(col / COLS) * p.m + m0 + row] = d0 + d1;
           }
           if (AMN && !SPLIT && p.y == nullptr) {  // the rows' products alone are wanted
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             group_sync();
           } else if (SPLIT || (which == 0 ? p.z_tma : p.y_tma)) {
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");

@@ -8,7 +8,7 @@ a truncation of at most 2^-23 of the running magnitude each: ez = 2^-23 (inner /
 8) (|x| |W| + |b|).  An activation is good to 1e-5 |a| and has a slope of at most
 1.13 (gelu; the others 1.1), so y: u |y| + |g| (1.13 ez + 1e-5 |a|) + 2^-22 (|r| +
 |g a|) + 2^-25 (half a step of fp16's subnormal numbers).
-Gradients.  z is kept in v: dz is off by d = |dy g| (v |z| + ez + 1e-5) (the second
+Gradients.  z is kept in v (with a gate better, in fp32): dz is off by d = |dy g| (v |z| + ez + 1e-5) (the second
 derivatives stay below 1), for relu by |dy g| where |z| <= ez; then rounded: v |dz|.
 A product of dz adds 2^-23 (n / 16 + 8) of its magnitudes.  Without an activation the
 gate goes to dy or to W: one rounding v of a factor, and dy in fp32 is rounded too.
