@@ -17,16 +17,25 @@ struct Fwd {
   int64_t h_stride, y_stride;
 };
 
+// Threads of a block.  Rows over four or eight warps wait for one another's sums, and a third slot
+// fills the gaps (8,000 rows of 4096 with two norms: 51 us with 512, 45 with 768); shorter rows are
+// slower for it (44,000 of 1024: 59 and 65 us).
+template <int WPR, bool DIRECT>
+constexpr int block_threads() {
+  return !DIRECT && (WPR == 4 || WPR == 8) ? 768 : kMaxThreads;
+}
+
 template <typename S, typename T, int WPR, int J, bool DIRECT>
-__global__ void __launch_bounds__(kMaxThreads, 1) forward_kernel(const Fwd f) {
+__global__ void __launch_bounds__(block_threads<WPR, DIRECT>(), 1) forward_kernel(const Fwd f) {
+  constexpr int kThreads = block_threads<WPR, DIRECT>();
   constexpr int kX = sizeof(S) / 2, kF = sizeof(T) / 2;  // 16-byte units of 8 elements
   constexpr int kUnits = J * (kX + kF);
-  typedef Shared<kMaxThreads, WPR, J, kUnits, DIRECT> SH;
+  typedef Shared<kThreads, WPR, J, kUnits, DIRECT> SH;
   extern __shared__ __align__(16) unsigned char smem[];
   __shared__ float scratch[2 * 2 * 32];
   const Args& a = f.a;
   RowSum<WPR> sum(scratch);
-  const Pipe<kMaxThreads, kUnits> pipe(smem);
+  const Pipe<kThreads, kUnits> pipe(smem);
   const int lane = threadIdx.x & 31, slots = (blockDim.x >> 5) / WPR;
   const float inv_width = 1.f / (float)a.width;
   const bool vec = !DIRECT || a.vec, branch = a.branch != nullptr;
@@ -152,7 +161,8 @@ __global__ void __launch_bounds__(kMaxThreads, 1) forward_kernel(const Fwd f) {
 template <typename S, typename T, int WPR, int J, bool DIRECT>
 cudaError_t launch_shape(const Fwd& f, int64_t blocks, int slots, cudaStream_t stream) {
   constexpr uint32_t bytes =
-      Shared<kMaxThreads, WPR, J, J*(sizeof(S) / 2 + sizeof(T) / 2), DIRECT>::kBytes;
+      Shared<block_threads<WPR, DIRECT>(), WPR, J, J*(sizeof(S) / 2 + sizeof(T) / 2),
+             DIRECT>::kBytes;
   auto k = forward_kernel<S, T, WPR, J, DIRECT>;
   static OncePerDevice allowed;
   if (cudaError_t e = allow_shared(k, (int)bytes, &allowed)) return e;
@@ -162,8 +172,8 @@ cudaError_t launch_shape(const Fwd& f, int64_t blocks, int slots, cudaStream_t s
 // Rows copied ahead where they are aligned, fit and are more than the slots; false where not.
 template <typename S, typename T, int WPR, int J>
 bool launch_ahead(const Fwd& f, int sms, cudaStream_t stream, cudaError_t* e) {
-  constexpr int slots = kMaxThreads / 32 / WPR;
-  if constexpr (Shared<kMaxThreads, WPR, J, J*(sizeof(S) / 2 + sizeof(T) / 2), false>::kFits)
+  constexpr int threads = block_threads<WPR, false>(), slots = threads / 32 / WPR;
+  if constexpr (Shared<threads, WPR, J, J*(sizeof(S) / 2 + sizeof(T) / 2), false>::kFits)
     if (f.a.vec && f.a.rows > (int64_t)sms * slots) {
       *e = launch_shape<S, T, WPR, J, false>(f, sms, slots, stream);
       return true;

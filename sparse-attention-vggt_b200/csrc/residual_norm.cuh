@@ -5,8 +5,8 @@
 //   y = norm(h) * weight + bias  norm: (h - mean) / sqrt(var + eps), or h / sqrt(mean h^2 + eps)
 //
 // A row is held in registers by WPR warps, 8 * J elements a lane, in chunks of 8: chunk j of lane
-// l of the row's warp w starts at column 8 * ((j * WPR + w) * 32 + l).  A block has up to 16 warps,
-// one block to an SM, and each of its groups of WPR warps (a slot) works through rows of its own.
+// l of the row's warp w starts at column 8 * ((j * WPR + w) * 32 + l).  A block has 16 warps or a
+// few more, one block to an SM, and each of its groups of WPR warps (a slot) works through rows of its own.
 // While it works on one row, its threads copy their chunks of the next one into shared memory
 // (cp.async, where the layout allows 16-byte accesses: `vec`), and the parameters lie there too, in
 // fp32, read once per block: what a thread needs of either is its own or its warp's, so that no
