@@ -559,7 +559,12 @@ __global__ void __launch_bounds__(THREADS, 1)
         }
         open(col, has_res && !has_z);
       }
-      if (!agree(wait(bar(SH::B_ACCFULL + b), (i >> 1) & 1, abort_flag, p.wait_ns))) {
+      // the first use's residual is there before the accumulator as a rule: one vote on both
+      bool got = true;
+      if (active && has_res && !has_z && p.res_tma)
+        got = wait(res_bar, res_uses++ & 1, abort_flag, p.wait_ns);
+      got = got && wait(bar(SH::B_ACCFULL + b), (i >> 1) & 1, abort_flag, p.wait_ns);
+      if (!agree(got)) {
         ok = false;
         break;
       }
@@ -577,9 +582,9 @@ __global__ void __launch_bounds__(THREADS, 1)
         for (int c = 0; c < COLS; c += wide ? 32 : COLS) {
           const int c0 = col + c;  // first column of the use
           if (!SPLIT && c0 >= p.n) break;
-          if (!opened) open(c0, res);
           const int64_t left = p.n - c0;
-          if (!opened || (res && p.res_tma)) {
+          if (!opened) {
+            open(c0, res);
             const bool fine = !(res && p.res_tma) ||
                               wait(res_bar, res_uses++ & 1, abort_flag, p.wait_ns);
             if (!agree(fine)) {
