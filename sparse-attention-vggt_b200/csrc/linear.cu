@@ -749,6 +749,8 @@ __global__ void __launch_bounds__(THREADS, 1)
       }
       ++i;
     }
+    // after a wait that gave up: a residual on its way lands before the block ends
+    if (!ok && res_uses > 0) tc::mbar_wait_drain(res_bar, (res_uses - 1) & 1, p.wait_ns);
     if (t == 0) store_wait_read<0>();  // the memory outlives the stores' reads of it
   }
 
