@@ -95,6 +95,11 @@ class GlobalBlock:
     @torch.no_grad()
     def __call__(self, x, pos=None, pos_count=None):
         """x [N, C] (or [1, N, C]); pos as in ``project_qkv``."""
+        # the tokens of one sample attend to one another: flattened, a batch would be one
+        if x.dim() == 3 and x.shape[0] != 1:
+            raise ValueError("batch one only")
+        if x.dim() not in (2, 3):
+            raise ValueError("x must be [N, C]")
         flat = x.reshape(-1, x.shape[-1])
         a = self.attention(flat, pos, pos_count)
         return self.mlp(flat, linear(a, *self.proj, head_major=True)).view(x.shape)
