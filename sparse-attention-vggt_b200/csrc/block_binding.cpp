@@ -106,6 +106,14 @@ bool needs_graph(const Ts&... t) {
   return c10::GradMode::is_enabled() && ((t.defined() && t.requires_grad()) || ...);
 }
 
+// Tensors with a tangent (dual tensors need no backward graph) are refused: the kernels form none,
+// and a result without one reads as zero.
+template <typename... Ts>
+void no_tangents(const Ts&... t) {
+  if (((t.defined() && t._fw_grad(0).defined()) || ...))
+    refuse("there is no forward-mode derivative of this operator");
+}
+
 // Gradients that a second differentiation must not go through raise there.
 variable_list once(variable_list grads) {
   if (!c10::GradMode::is_enabled()) return grads;
@@ -328,6 +336,7 @@ PyObject* residual_norm(PyObject*, PyObject* const* o, Py_ssize_t n) {
     const NormIn in(o);
     const at::Tensor out = given_or_none(o[11], "out"), hout = given_or_none(o[12], "stream_out");
     const at::Tensor* t = in.t;
+    no_tangents(t[0], t[1], t[2], t[3], t[4], t[5], t[6], out, hout);
     at::Tensor y, h;
     if (needs_graph(t[0], t[1], t[2], t[3], t[4], t[5], t[6])) {
       if (out.defined() || hout.defined())
@@ -576,6 +585,7 @@ PyObject* linear(PyObject*, PyObject* const* o, Py_ssize_t n) {
     in.head_major = truth(o[6]);
     in.status = given_or_none(o[8], "status");
     const at::Tensor out = given_or_none(o[7], "out");
+    no_tangents(in.x, in.weight, in.bias, in.gate, in.residual, out);
     if (needs_graph(in.x, in.weight, in.bias, in.gate, in.residual)) {
       if (out.defined()) refuse("out is for calls without a gradient");
       return THPVariable_Wrap(LinearFunction::apply(

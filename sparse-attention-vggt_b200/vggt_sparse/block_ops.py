@@ -10,7 +10,8 @@ With ``project_qkv`` and the attention they make up the reference's block
 projection, LayerScale, residual, LayerNorm, MLP, LayerScale, residual);
 ``GlobalBlock`` (block.py) is that block.
 
-Both are differentiable, once, in all their tensors.  Sums, statistics and
+Both are differentiable, once, in all their tensors, by a backward pass (tensors
+with a forward-mode tangent are refused).  Sums, statistics and
 activations are formed in fp32 and rounded once, to the result's type; a
 backward pass adds in a fixed order, so that equal calls give equal results.
 

@@ -4,7 +4,9 @@ import os
 
 import pytest
 import torch
+import torch.autograd.forward_ad as fwAD
 
+import vggt_sparse
 from vggt_sparse import GlobalBlock
 
 BF, FP, F32 = torch.bfloat16, torch.float16, torch.float32
@@ -43,3 +45,32 @@ def test_block_takes_one_sample(shape, text):
     pos = torch.zeros(*shape[:-1], 2, dtype=torch.long)
     with pytest.raises(ValueError, match=text):
         block(x, pos, 7)
+
+
+@pytest.mark.parametrize("graph", [False, True])
+@pytest.mark.parametrize("which", ["x", "weight", "bias", "gate", "residual"])
+def test_linear_refuses_forward_mode(which, graph):
+    """A dual tensor needs no backward graph: without a look at its tangent the result would have
+    none, which reads as zero."""
+    t = dict(x=torch.zeros(4, 64, dtype=BF), weight=torch.zeros(16, 64, dtype=BF),
+             bias=torch.zeros(16, dtype=BF), gate=torch.zeros(16, dtype=BF),
+             residual=torch.zeros(4, 16, dtype=F32))
+    if graph:
+        t["x"].requires_grad_()
+    with fwAD.dual_level():
+        t[which] = fwAD.make_dual(t[which], torch.ones_like(t[which]))
+        with pytest.raises(ValueError, match="forward-mode"):
+            vggt_sparse.linear(t.pop("x"), t.pop("weight"), **t)
+
+
+@pytest.mark.parametrize("which", ["x", "branch", "weight", "bias", "gate", "post_weight", "post_bias"])
+def test_residual_norm_refuses_forward_mode(which):
+    t = {n: torch.zeros(64) for n in ("weight", "bias", "gate", "post_weight", "post_bias")}
+    t.update(x=torch.zeros(4, 64), branch=torch.zeros(4, 64))
+    with fwAD.dual_level():
+        t[which] = fwAD.make_dual(t[which], torch.ones_like(t[which]))
+        with pytest.raises(ValueError, match="forward-mode"), torch.no_grad():
+            vggt_sparse.residual_norm(t.pop("x"), post_norm="layer", **t)
+        with pytest.raises(ValueError, match="forward-mode"):
+            vggt_sparse.residual_norm(torch.zeros(4, 64), out=fwAD.make_dual(
+                torch.zeros(4, 64), torch.ones(4, 64)))
