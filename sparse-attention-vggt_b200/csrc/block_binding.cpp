@@ -12,6 +12,7 @@
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 
+#include <algorithm>
 #include <optional>
 #include <tuple>
 #include <utility>
@@ -81,6 +82,42 @@ void written(const at::Tensor& t) {
 void check_given(const char* name, const at::Tensor& t, at::IntArrayRef sizes, at::ScalarType type) {
   if (t.sizes() != sizes || t.scalar_type() != type || !t.is_contiguous())
     refuse("%s must be contiguous, of the result's shape and dtype", name);
+}
+
+// Whether an element of a strided tensor at byte `at` lies in [lo, hi).  The dimension of the largest
+// stride is taken first: of its steps only those whose elements can lie there are looked into, and
+// all but the outer two of those lie there whole.
+bool meets(at::IntArrayRef sizes, at::IntArrayRef strides, int64_t item, uint32_t taken, int64_t at,
+           int64_t lo, int64_t hi) {
+  int64_t span = item;
+  int most = -1;
+  for (int k = 0; k < (int)sizes.size(); ++k) {
+    if ((taken >> k & 1) || sizes[k] == 1 || strides[k] == 0) continue;
+    span += (sizes[k] - 1) * strides[k] * item;
+    if (most < 0 || strides[k] > strides[most]) most = k;
+  }
+  if (at >= hi || at + span <= lo) return false;
+  if (most < 0 || at >= lo) return true;
+  const int64_t step = strides[most] * item, inner = span - (sizes[most] - 1) * step;
+  int64_t i = std::max<int64_t>(0, (lo - at - inner) / step);
+  for (; i < sizes[most] && at + i * step < hi; ++i)
+    if (meets(sizes, strides, item, taken | 1u << most, at + i * step, lo, hi)) return true;
+  return false;
+}
+
+// An output that the caller gives lies apart from an input, or, where `same` allows that, in its
+// very elements.
+void check_apart(const char* name, const at::Tensor& out, const char* input, const at::Tensor& t,
+                 bool same) {
+  if (!out.defined() || !t.defined() || out.numel() == 0 || t.numel() == 0) return;
+  if (same && t.data_ptr() == out.data_ptr() && t.is_contiguous() &&
+      t.scalar_type() == out.scalar_type())
+    return;
+  const int64_t lo = (int64_t)out.data_ptr();
+  if (t.dim() <= 32 && !meets(t.sizes(), t.strides(), t.element_size(), 0, (int64_t)t.data_ptr(), lo,
+                              lo + (int64_t)out.nbytes()))
+    return;
+  refuse("%s must not lie in %s%s", name, input, same ? " (unless it is that very tensor)" : "");
 }
 
 at::Tensor workspace(size_t bytes, c10::Device device) {
@@ -238,6 +275,14 @@ std::pair<at::Tensor, at::Tensor> norm_forward(const NormIn& in, const at::Tenso
     if (!both) refuse("stream_out needs a branch: without one the stream is x");
     check_given("stream_out", hout, xt.sizes(), c.stream);
   }
+  static const char* inputs[kNormTensors] = {"x",    "branch",      "weight",   "bias",
+                                             "gate", "post_weight", "post_bias"};
+  // a row is read whole before it is written
+  for (int k = 0; k < kNormTensors; ++k) {
+    check_apart("out", out, inputs[k], in.t[k], k <= kBranch);
+    check_apart("stream_out", hout, inputs[k], in.t[k], k <= kBranch);
+  }
+  check_apart("out", out, "stream_out", hout, false);
   const c10::cuda::CUDAGuard guard(device_of(in, out, hout));
   at::Tensor y = out.defined() ? out : at::empty(xt.sizes(), xt.options().dtype(in.type));
   at::Tensor h = !both ? at::Tensor() : hout.defined() ? hout : at::empty(xt.sizes(), xt.options());
@@ -338,7 +383,7 @@ PyObject* residual_norm(PyObject*, PyObject* const* o, Py_ssize_t n) {
     const at::Tensor* t = in.t;
     no_tangents(t[0], t[1], t[2], t[3], t[4], t[5], t[6], out, hout);
     at::Tensor y, h;
-    if (needs_graph(t[0], t[1], t[2], t[3], t[4], t[5], t[6])) {
+    if (needs_graph(t[0], t[1], t[2], t[3], t[4], t[5], t[6], out, hout)) {
       if (out.defined() || hout.defined())
         refuse("out and stream_out are for calls without a gradient");
       variable_list both = NormFunction::apply(
@@ -453,6 +498,13 @@ std::pair<at::Tensor, at::Tensor> linear_forward(const LinearIn& in, const at::T
   const std::vector<int64_t> shape = c.y_shape();
   if (out.defined()) check_given("out", out, shape, c.stream);
   int32_t* word = status_of(there(in.status));
+  // tiles are read while others are written
+  check_apart("out", out, "x", in.x, false);
+  check_apart("out", out, "weight", in.weight, false);
+  check_apart("out", out, "bias", in.bias, false);
+  check_apart("out", out, "gate", in.gate, false);
+  check_apart("out", out, "residual", in.residual, true);
+  check_apart("out", out, "status", in.status, false);
   const c10::Device device = one_device(in.x, there(in.weight), there(in.bias), there(in.gate),
                                         there(in.residual), there(out), there(in.status));
   const c10::cuda::CUDAGuard guard(device);
@@ -586,7 +638,7 @@ PyObject* linear(PyObject*, PyObject* const* o, Py_ssize_t n) {
     in.status = given_or_none(o[8], "status");
     const at::Tensor out = given_or_none(o[7], "out");
     no_tangents(in.x, in.weight, in.bias, in.gate, in.residual, out);
-    if (needs_graph(in.x, in.weight, in.bias, in.gate, in.residual)) {
+    if (needs_graph(in.x, in.weight, in.bias, in.gate, in.residual, out)) {
       if (out.defined()) refuse("out is for calls without a gradient");
       return THPVariable_Wrap(LinearFunction::apply(
           in.x, in.weight, maybe(in.bias), maybe(in.gate), maybe(in.residual), (int64_t)in.activation,

@@ -58,8 +58,8 @@ def linear(x, weight, bias=None, *, activation=None, gate=None, residual=None, h
     Gradients of the products are rounded to x's dtype: with fp16 scale the loss,
     as ever, where they may fall below its range.
 
-    ``out`` (contiguous; may be residual) takes the result where no gradient is
-    needed.  ``status``, an int32 tensor, gets VGGT_STATUS_TIMEOUT if a wait of
+    ``out`` (contiguous; residual itself, or apart from every input) takes the
+    result where no gradient is needed.  ``status``, an int32 tensor, gets VGGT_STATUS_TIMEOUT if a wait of
     the kernel ran out.
     """
     return _binding().linear(x, weight, bias, activation, gate, residual, head_major, out, status)
@@ -81,8 +81,8 @@ def residual_norm(x, branch=None, weight=None, bias=None, *, norm="layer", gate=
     rows each (a gate per sample of a batch, or per row), in any of the three
     dtypes.
 
-    ``out`` and ``stream_out`` (contiguous; stream_out may be x) take y and h
-    where no gradient is needed.
+    ``out`` and ``stream_out`` (contiguous; each x or branch itself, or apart from
+    every input and from the other) take y and h where no gradient is needed.
     """
     return _binding().residual_norm(x, branch, weight, bias, gate, post_weight, post_bias, norm,
                                     post_norm, eps, dtype, out, stream_out)

@@ -74,3 +74,112 @@ def test_residual_norm_refuses_forward_mode(which):
         with pytest.raises(ValueError, match="forward-mode"):
             vggt_sparse.residual_norm(torch.zeros(4, 64), out=fwAD.make_dual(
                 torch.zeros(4, 64), torch.ones(4, 64)))
+
+
+def linear_args(outer=64, stream=BF):
+    t = dict(x=torch.zeros(4, 64, dtype=BF), weight=torch.zeros(outer, 64, dtype=BF),
+             bias=torch.zeros(outer, dtype=BF), gate=torch.zeros(outer, dtype=BF),
+             residual=torch.zeros(4, outer, dtype=stream))
+    return t
+
+
+def call_linear(t, **kw):
+    t = dict(t)
+    return vggt_sparse.linear(t.pop("x"), t.pop("weight"), **t, **kw)
+
+
+@pytest.mark.parametrize("which", ["x", "weight", "bias", "gate", "residual", "status"])
+def test_linear_out_does_not_lie_in_an_input(which):
+    """Tiles that are done write their part of out while others still read: only the residual's own
+    elements may be there."""
+    t = linear_args()
+    room = torch.zeros(16384, dtype=BF)
+    t["status"] = torch.zeros(1, dtype=torch.int32)
+    n = t[which].numel() * t[which].element_size() // 2
+    place = lambda at: room[at:at + n].view(t[which].dtype).view(t[which].shape)  # noqa: E731
+    out = room[4096:4352].view(4, 64)
+    for at in (4096 - n + 2, 4096, 4350):  # its last elements in out, both from one place on, its first
+        if which == "residual" and at == 4096:
+            continue
+        t[which] = place(at)
+        with pytest.raises(ValueError, match="out must not"):
+            call_linear(t, out=out)
+    # beside it is fine: what is refused then is that there is no GPU
+    for at in (4096 - n, 4352):
+        t[which] = place(at)
+        with pytest.raises(ValueError, match="CUDA tensors"):
+            call_linear(t, out=out)
+
+
+def test_linear_out_may_be_the_residual_or_lie_between_rows():
+    t = linear_args()
+    with pytest.raises(ValueError, match="CUDA tensors"):
+        call_linear(t, out=t["residual"])
+    # the same memory by other rows, or in another type
+    room = torch.zeros(1024, dtype=BF)
+    t["residual"] = room.as_strided((4, 64), (128, 1))
+    with pytest.raises(ValueError, match="out must not"):
+        call_linear(t, out=room[:256].view(4, 64))
+    t["residual"] = room[:64].expand(4, 64)
+    with pytest.raises(ValueError, match="out must not"):
+        call_linear(t, out=room[:256].view(4, 64))
+    # between the rows of x, and of head-major ones
+    t = linear_args()
+    t["x"] = room.as_strided((4, 64), (320, 1))
+    with pytest.raises(ValueError, match="CUDA tensors"):
+        call_linear(t, out=room[64:320].view(4, 64))
+    with pytest.raises(ValueError, match="out must not"):
+        call_linear(t, out=room[65:321].view(4, 64))
+    t["x"] = room.as_strided((2, 4, 32), (512, 32, 1))
+    with pytest.raises(ValueError, match="CUDA tensors"):
+        call_linear(t, out=room[128:384].view(4, 64), head_major=True)
+    with pytest.raises(ValueError, match="out must not"):
+        call_linear(t, out=room[264:520].view(4, 64), head_major=True)
+
+
+@pytest.mark.parametrize("which", ["weight", "bias", "gate", "post_weight", "post_bias"])
+def test_residual_norm_outputs_do_not_lie_in_parameters(which):
+    room = torch.zeros(1024)
+    t = {n: torch.zeros(64) for n in ("weight", "bias", "gate", "post_weight", "post_bias")}
+    t[which] = room[300:364]
+    x, f = torch.zeros(4, 64), torch.zeros(4, 64)
+    with pytest.raises(ValueError, match="stream_out must not"):
+        vggt_sparse.residual_norm(x, f, post_norm="layer", stream_out=room[256:512].view(4, 64), **t)
+    with pytest.raises(ValueError, match="^out must not"):
+        vggt_sparse.residual_norm(x, f, post_norm="layer", out=room[256:512].view(4, 64), **t)
+
+
+def test_residual_norm_outputs_are_rows_of_an_input_or_apart():
+    room = torch.zeros(2048)
+    x, f = room[:256].view(4, 64), room[1024:1280].view(4, 64)
+    call = lambda **kw: vggt_sparse.residual_norm(x, f, **kw)  # noqa: E731
+    # a row is read whole before it is written: either output may be either input
+    for kw in (dict(out=x), dict(out=f), dict(stream_out=x), dict(stream_out=f),
+               dict(out=f, stream_out=x), dict(out=room[256:512].view(4, 64))):
+        with pytest.raises(ValueError, match="CUDA tensors"):
+            call(**kw)
+    for kw in (dict(out=x, stream_out=x), dict(out=room[64:320].view(4, 64)),
+               dict(stream_out=room[1000:1256].view(4, 64)),
+               dict(out=room[400:656].view(4, 64), stream_out=room[500:756].view(4, 64))):
+        with pytest.raises(ValueError, match="out must not"):
+            call(**kw)
+    # other rows of the same memory, another type
+    for x in (room.as_strided((4, 64), (128, 1)), room[:64].expand(4, 64)):
+        with pytest.raises(ValueError, match="out must not"):
+            call(out=room[:256].view(4, 64))
+    with pytest.raises(ValueError, match="out must not"):
+        vggt_sparse.residual_norm(room[:256].view(4, 64), dtype=BF,
+                                  out=room.view(BF)[:256].view(4, 64))
+
+
+def test_outputs_that_need_a_gradient_are_refused():
+    """Written in place they would keep a gradient that knows nothing of it."""
+    out = torch.zeros(4, 64, dtype=BF, requires_grad=True)
+    t = linear_args()
+    x = torch.zeros(4, 64, dtype=BF)
+    for call in (lambda: call_linear(t, out=out), lambda: vggt_sparse.residual_norm(x, x, out=out),
+                 lambda: vggt_sparse.residual_norm(x, x, stream_out=out)):
+        with pytest.raises(ValueError, match="without a gradient"):
+            call()
+        with pytest.raises(ValueError, match="CUDA tensors"), torch.no_grad():
+            call()
