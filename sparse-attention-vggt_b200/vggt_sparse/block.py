@@ -14,6 +14,7 @@ another layout or an elementwise pass.
 """
 import torch
 
+from .block_attention import deferred_status
 from .block_ops import linear, residual_norm
 from .layer import SparseGlobalLayer
 from .qkv import project_qkv
@@ -41,7 +42,9 @@ class GlobalBlock:
 
     Weights are converted to ``dtype`` (bf16 or fp16) once, here; the norms'
     stay in fp32.  x [N, C] may be of ``dtype`` or fp32 (a residual stream held
-    in 32 bits), and so is the result.  There is no gradient through the
+    in 32 bits), and so is the result.  A wait that runs out on the device is
+    raised as a ValueError by a later call or by ``check_status``, without the
+    host's waiting for it; what that call returned is not valid.  There is no gradient through the
     attention: a call runs without one.  ``mlp`` alone is differentiable in x.
     """
 
@@ -62,6 +65,8 @@ class GlobalBlock:
         self.qkv, self.proj, self.fc1, self.fc2 = (tuple(cast(t) for t in pair(m))
                                                   for m in (qkv, proj, fc1, fc2))
         self.ls1, self.ls2 = cast(ls1), cast(ls2)
+        with deferred_status(self.qkv[0].device):
+            pass  # a graph's capture finds the status word in place
 
     @classmethod
     def from_module(cls, block, *, tokens_per_frame, **options):
@@ -76,21 +81,29 @@ class GlobalBlock:
 
     def attention(self, x, pos=None, pos_count=None):
         """The attention of the normed tokens, head-major [heads, N, 64]."""
+        with deferred_status(x.device) as status:
+            return self._attention(x, pos, pos_count, status)
+
+    def _attention(self, x, pos, pos_count, status):
         weight, bias, eps = self.norm1
         y, _ = residual_norm(x, None, weight, bias, eps=eps, dtype=self.dtype)
         qkv = project_qkv(y, *self.qkv, heads=self.heads, tokens_per_frame=self.tokens_per_frame,
                           special_per_frame=self.special_per_frame, q_norm=self.q_norm,
                           k_norm=self.k_norm, pos=pos, rope_base=self.rope_base,
-                          pos_count=pos_count)
-        return self.layer.forward_projected(qkv)
+                          pos_count=pos_count, status=status)
+        return self.layer.forward_projected(qkv, status=status)
 
     def mlp(self, x, branch=None):
         """h + ls2 * fc2(gelu(fc1(norm2(h)))) with h = x, or x + ls1 * branch."""
+        with deferred_status(x.device) as status:
+            return self._mlp(x, branch, status)
+
+    def _mlp(self, x, branch, status):
         weight, bias, eps = self.norm2
         y, h = residual_norm(x, branch, weight, bias, eps=eps, dtype=self.dtype,
                              gate=self.ls1 if branch is not None else None)
-        wide = linear(y, *self.fc1, activation="gelu")
-        return linear(wide, *self.fc2, gate=self.ls2, residual=h)
+        wide = linear(y, *self.fc1, activation="gelu", status=status)
+        return linear(wide, *self.fc2, gate=self.ls2, residual=h, status=status)
 
     @torch.no_grad()
     def __call__(self, x, pos=None, pos_count=None):
@@ -101,5 +114,7 @@ class GlobalBlock:
         if x.dim() not in (2, 3):
             raise ValueError("x must be [N, C]")
         flat = x.reshape(-1, x.shape[-1])
-        a = self.attention(flat, pos, pos_count)
-        return self.mlp(flat, linear(a, *self.proj, head_major=True)).view(x.shape)
+        with deferred_status(x.device) as status:
+            a = self._attention(flat, pos, pos_count, status)
+            p = linear(a, *self.proj, head_major=True, status=status)
+            return self._mlp(flat, p, status).view(x.shape)

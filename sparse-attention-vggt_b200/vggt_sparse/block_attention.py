@@ -19,6 +19,7 @@ default path never blocks the host.  ``validate=True`` keeps the old
 synchronous check (one host sync per call, the error raised by the faulty
 call itself); ``validate=False`` skips status reporting entirely.
 """
+import contextlib
 import math
 import threading
 
@@ -56,7 +57,7 @@ class _StatusMonitor:
         # the error is reported once: reset the word and forget copies in flight
         self.events = [None] * _RING
         self.word.zero_()
-        raise ValueError("block_attention (an earlier call on %s): %s"
+        raise ValueError("block_attention or GlobalBlock (an earlier call on %s): %s"
                          % (self.word.device, _status_message(bits)))
 
     def poll(self, wait=False):
@@ -76,7 +77,7 @@ class _StatusMonitor:
                 self._raise(bits)
         self.host[j:j + 1].copy_(self.word, non_blocking=True)
         ev = torch.cuda.Event()
-        ev.record()
+        ev.record(torch.cuda.current_stream(self.word.device))
         self.events[j] = ev
 
 
@@ -95,11 +96,35 @@ def _monitor(device):
 
 def check_status(device=None, wait=True):
     """Raise ValueError if any earlier deferred-validation call on ``device``
-    (default: the current device) found bad ids, counts or head ids.  With
-    ``wait`` (default) it first waits for every pending status copy."""
+    (default: the current device) found bad ids, counts or head ids, or gave up
+    a wait.  With ``wait`` (default) it first waits for every pending status copy,
+    and for what is enqueued on the current stream (replayed graphs and backward
+    passes, which no copy follows)."""
     dev = torch.device("cuda", torch.cuda.current_device()) if device is None \
         else torch.device(device)
-    _monitor(dev).poll(wait=wait)
+    monitor = _monitor(dev)
+    if wait:
+        monitor.enqueue_copy()
+    monitor.poll(wait=wait)
+
+
+@contextlib.contextmanager
+def deferred_status(device):
+    """The status word of ``device`` (None where that is no GPU) for the calls of a
+    ``with`` block: errors of earlier ones are raised first, and what these find is
+    raised by a later one or by ``check_status``.  Nothing waits, and a graph capture
+    takes only the word."""
+    if device.type != "cuda":
+        yield None
+        return
+    monitor = _monitor(device)
+    with torch.cuda.device(device):
+        live = not torch.cuda.is_current_stream_capturing()
+    if live:
+        monitor.poll()
+    yield monitor.word
+    if live:
+        monitor.enqueue_copy()
 
 
 def _status_message(bits):

@@ -120,15 +120,16 @@ class SparseGlobalLayer:
         self.last_masks = (buf["indices"], buf["counts"])
         return buf
 
-    def forward_projected(self, qkv, out=None):
+    def forward_projected(self, qkv, out=None, status=None):
         """The layer on the outputs of ``vggt_sparse.project_qkv`` (q, split
-        K/V and block means): selection from the means, then attention."""
+        K/V and block means): selection from the means, then attention (which
+        reports to ``status``, an int32 tensor, where given)."""
         n, npatch, nspecial = qkv.q.shape[1], qkv.patch_k.shape[1], qkv.special_k.shape[1]
         self.estimate_pooled(qkv.pooled_q, qkv.pooled_k, n, npatch, nspecial)
         return self.attend(qkv.q, qkv.patch_k, qkv.patch_v, qkv.special_k, qkv.special_v,
-                           out=out)
+                           out=out, status=status)
 
-    def attend(self, q, kp, vp, ks, vs, out=None):
+    def attend(self, q, kp, vp, ks, vs, out=None, status=None):
         """Block-sparse attention with the masks of the last ``estimate``."""
         h, n, d = q.shape
         buf = self._buffers(q.device, n, kp.shape[1], ks.shape[1])
@@ -141,7 +142,7 @@ class SparseGlobalLayer:
         ops.launch_block_attention(q, kp, vp, ks, vs, buf["indices"], buf["counts"],
                                    buf["slot_ids"], head_dense=buf["dense_flags"],
                                    query_block=self.block, key_block=self.block, out=out,
-                                   evidence=evidence, kernel=self.kernel,
+                                   evidence=evidence, status=status, kernel=self.kernel,
                                    pair_qblocks=self.pair_qblocks and bool(self.sparse_heads),
                                    workspace=buf["attn_ws"])
         self.last_masks = (buf["indices"], buf["counts"])
