@@ -29,6 +29,30 @@ def _norm(norm):
     return keep(weight), keep(bias), float(eps)
 
 
+def _activation(act):
+    """The name, as ``linear`` takes it, of an activation's module."""
+    if act is None:  # the MLP's default
+        return "gelu"
+    name = {torch.nn.GELU: "gelu_tanh" if getattr(act, "approximate", "none") == "tanh" else "gelu",
+            torch.nn.SiLU: "silu", torch.nn.ReLU: "relu"}.get(type(act))
+    if name is None:
+        raise ValueError("the module's activation %s is not one of linear's: give activation"
+                         % type(act).__name__)
+    return name
+
+
+def _rope_base(attn):
+    """The rotary embedding's base of an attention module; None where it has none."""
+    if not hasattr(attn, "rope"):
+        return 100.0
+    if attn.rope is None:
+        return None
+    for name in ("base_frequency", "frequency"):
+        if hasattr(attn.rope, name):
+            return float(getattr(attn.rope, name))
+    raise ValueError("the module's rope has no base_frequency: give rope_base")
+
+
 class GlobalBlock:
     """``block(x, pos)`` for the tokens of a fixed set of frames.
 
@@ -37,6 +61,8 @@ class GlobalBlock:
                      Linear modules or (weight, bias)
     ls1, ls2         the scales per channel, or None
     q_norm, k_norm   as ``project_qkv`` takes them
+    rope_base        likewise; None: positions are not looked at
+    activation       the MLP's, as ``linear`` takes it
     layer            the ``SparseGlobalLayer`` (by default one with
                      ``layer_options``)
 
@@ -44,13 +70,15 @@ class GlobalBlock:
     stay in fp32.  x [N, C] may be of ``dtype`` or fp32 (a residual stream held
     in 32 bits), and so is the result.  A wait that runs out on the device is
     raised as a ValueError by a later call or by ``check_status``, without the
-    host's waiting for it; what that call returned is not valid.  There is no gradient through the
-    attention: a call runs without one.  ``mlp`` alone is differentiable in x.
+    host's waiting for it; what the call at fault returned is not valid.  Calls
+    share the layer's buffers: they belong on one stream, or behind one another.
+    There is no gradient through the attention: a call runs without one.  ``mlp``
+    alone is differentiable in x.
     """
 
     def __init__(self, heads, *, tokens_per_frame, norm1, qkv, proj, norm2, fc1, fc2, ls1=None,
                  ls2=None, q_norm=None, k_norm=None, special_per_frame=5, rope_base=100.0,
-                 layer=None, dtype=torch.bfloat16, **layer_options):
+                 activation="gelu", layer=None, dtype=torch.bfloat16, **layer_options):
         if layer is not None and layer_options:
             raise ValueError("give either layer or its options")
         self.layer = layer or SparseGlobalLayer(heads, **layer_options)
@@ -59,6 +87,7 @@ class GlobalBlock:
         self.heads, self.dtype = heads, dtype
         self.tokens_per_frame, self.special_per_frame = tokens_per_frame, special_per_frame
         self.rope_base, self.q_norm, self.k_norm = rope_base, q_norm, k_norm
+        self.activation = activation
         cast = lambda t: None if t is None else t.detach().to(dtype).contiguous()  # noqa: E731
         pair = lambda m: (m.weight, m.bias) if isinstance(m, torch.nn.Linear) else m  # noqa: E731
         self.norm1, self.norm2 = _norm(norm1), _norm(norm2)
@@ -70,10 +99,16 @@ class GlobalBlock:
 
     @classmethod
     def from_module(cls, block, *, tokens_per_frame, **options):
-        """From the reference's Block (its attention's qkv, q_norm, k_norm and
-        proj, the LayerScales' gamma where there are any)."""
+        """From the reference's Block (its attention's qkv, q_norm, k_norm, proj
+        and rope, its MLP's layers and activation, the LayerScales' gamma where there
+        are any); an activation or a rope that is not known is refused, unless the
+        option is given."""
         gamma = lambda m: getattr(m, "gamma", None)  # noqa: E731
         attn = block.attn
+        if "activation" not in options:
+            options["activation"] = _activation(getattr(block.mlp, "act", None))
+        if "rope_base" not in options:
+            options["rope_base"] = _rope_base(attn)
         return cls(attn.num_heads, tokens_per_frame=tokens_per_frame, norm1=block.norm1,
                    qkv=attn.qkv, proj=attn.proj, norm2=block.norm2, fc1=block.mlp.fc1,
                    fc2=block.mlp.fc2, ls1=gamma(block.ls1), ls2=gamma(block.ls2),
@@ -87,6 +122,8 @@ class GlobalBlock:
     def _attention(self, x, pos, pos_count, status):
         weight, bias, eps = self.norm1
         y, _ = residual_norm(x, None, weight, bias, eps=eps, dtype=self.dtype)
+        if self.rope_base is None:
+            pos = None
         qkv = project_qkv(y, *self.qkv, heads=self.heads, tokens_per_frame=self.tokens_per_frame,
                           special_per_frame=self.special_per_frame, q_norm=self.q_norm,
                           k_norm=self.k_norm, pos=pos, rope_base=self.rope_base,
@@ -102,7 +139,7 @@ class GlobalBlock:
         weight, bias, eps = self.norm2
         y, h = residual_norm(x, branch, weight, bias, eps=eps, dtype=self.dtype,
                              gate=self.ls1 if branch is not None else None)
-        wide = linear(y, *self.fc1, activation="gelu", status=status)
+        wide = linear(y, *self.fc1, activation=self.activation, status=status)
         return linear(wide, *self.fc2, gate=self.ls2, residual=h, status=status)
 
     @torch.no_grad()

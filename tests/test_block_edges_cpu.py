@@ -183,3 +183,60 @@ def test_outputs_that_need_a_gradient_are_refused():
             call()
         with pytest.raises(ValueError, match="CUDA tensors"), torch.no_grad():
             call()
+
+
+class Rope(torch.nn.Module):
+    def __init__(self, base):
+        super().__init__()
+        self.base_frequency = base
+
+
+def test_from_module_takes_the_module_s_activation():
+    block = parts()
+    build = lambda **kw: GlobalBlock.from_module(block, tokens_per_frame=TPF, **kw)  # noqa: E731
+    assert build().activation == "gelu"
+    for act, name in ((torch.nn.GELU(), "gelu"), (torch.nn.GELU(approximate="tanh"), "gelu_tanh"),
+                      (torch.nn.SiLU(), "silu"), (torch.nn.ReLU(), "relu")):
+        block.mlp.act = act
+        assert build().activation == name
+    for act in (torch.nn.Tanh(), torch.nn.LeakyReLU(), torch.nn.Identity()):
+        block.mlp.act = act
+        with pytest.raises(ValueError, match="activation"):
+            build()
+        assert build(activation="silu").activation == "silu"
+
+
+def test_from_module_takes_the_module_s_rope():
+    block = parts()
+    build = lambda **kw: GlobalBlock.from_module(block, tokens_per_frame=TPF, **kw)  # noqa: E731
+    assert build().rope_base == 100.0
+    block.attn.rope = Rope(10000.0)
+    assert build().rope_base == 10000.0
+    assert build(rope_base=50.0).rope_base == 50.0
+    block.attn.rope = torch.nn.Identity()
+    with pytest.raises(ValueError, match="rope"):
+        build()
+    assert build(rope_base=50.0).rope_base == 50.0
+    block.attn.rope = None  # positions are then not looked at
+    assert build().rope_base is None
+
+
+def test_from_module_without_rope_ignores_positions(monkeypatch):
+    from vggt_sparse import block as module
+    seen = []
+
+    class Stop(Exception):
+        pass
+
+    def project(*args, **kw):
+        seen.append(kw["pos"])
+        raise Stop
+    monkeypatch.setattr(module, "project_qkv", project)
+    monkeypatch.setattr(module, "residual_norm", lambda x, *a, **kw: (x, x))
+    block = parts()
+    x, pos = torch.zeros(TPF, 128), torch.zeros(TPF, 2)
+    for rope, given in ((Rope(100.0), True), (None, False)):
+        block.attn.rope = rope
+        with pytest.raises(Stop):
+            GlobalBlock.from_module(block, tokens_per_frame=TPF)(x, pos, 7)
+        assert (seen.pop() is not None) == given
