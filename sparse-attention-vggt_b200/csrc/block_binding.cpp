@@ -441,9 +441,16 @@ struct LinearCall {
         refuse("x must be [..., inner] with the weight's inner size");
       a.rows = xt.numel() / a.inner;
     }
-    for (const at::Tensor* t : {&in.bias, &in.gate})
-      if (t->defined() && (t->dim() != 1 || t->size(0) != a.outer || t->scalar_type() != type))
-        refuse("%s must be [outer], of x's dtype", t == &in.bias ? "bias" : "gate");
+    const at::Tensor &bt = in.bias, &gt = in.gate;
+    if (bt.defined() && (bt.dim() != 1 || bt.size(0) != a.outer || bt.scalar_type() != type))
+      refuse("bias must be [outer], of x's dtype");
+    a.gate_dtype = a.dtype;
+    if (gt.defined()) {
+      if (gt.dim() != 1 || gt.size(0) != a.outer ||
+          (gt.scalar_type() != type && gt.scalar_type() != at::kFloat))
+        refuse("gate must be [outer], of x's dtype or FP32");
+      a.gate_dtype = dtype_of("gate", gt.scalar_type(), true);
+    }
     stream = type;
     if (in.residual.defined()) {
       stream = in.residual.scalar_type();
@@ -567,7 +574,7 @@ variable_list linear_backward(const LinearIn& in, const at::Tensor& dy, const at
     g.dbias = d[2].data_ptr();
   }
   if (wanted[3] && in.gate.defined()) {
-    d[3] = at::empty({c.a.outer}, in.x.options());
+    d[3] = at::empty({c.a.outer}, in.gate.options());
     g.dgate = d[3].data_ptr();
   }
   const size_t bytes = vggt_linear_grad_workspace_size(&c.a, &g);

@@ -63,7 +63,7 @@ struct Params {
   const void* bias;
   const void* gate;
   int act;
-  int y_fp32, z_fp32, y_tma, res_tma, z_tma;
+  int y_fp32, z_fp32, gate_fp32, y_tma, res_tma, z_tma;
   const void* residual;
   int64_t residual_stride;
   void* y;
@@ -252,11 +252,6 @@ __device__ __forceinline__ void lds128(uint32_t a, uint32_t* r) {
 __device__ __forceinline__ void sts128(uint32_t a, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
   asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(x), "r"(y), "r"(z), "r"(w)
                : "memory");
-}
-
-template <typename E>
-__device__ __forceinline__ float to_float(E v) {
-  return (float)v;
 }
 
 // Address of 16-byte piece j of row r in an epilogue buffer with rows of 128 or 64 bytes (TMA's
@@ -553,8 +548,9 @@ __global__ void __launch_bounds__(THREADS, 1)
           // seen by the group after the next barrier; the last readers are before the last one
           const int c = col + (t & 63);
           float v = t < 64 ? 0.f : 1.f;
-          const T* src = static_cast<const T*>(t < 64 ? p.bias : p.gate);
-          if (src != nullptr && (t & 63) < COLS && c < p.n) v = to_float(src[c]);
+          const void* src = t < 64 ? p.bias : p.gate;
+          if (src != nullptr && (t & 63) < COLS && c < p.n)
+            v = vector_at<T>(src, t >= 64 && p.gate_fp32, c);
           vec[t] = v;
         }
         open(col, has_res && !has_z);
@@ -573,7 +569,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       // of a weight's gradient: this row's gate, and its product with the weight's row
       float_pair row_gate = pack_pair(1.f, 1.f), dot = pack_pair(0.f, 0.f);
       if (AMN && !SPLIT && p.row_gate != nullptr && m0 + row < p.m) {
-        const float v = to_float(static_cast<const T*>(p.row_gate)[m0 + row]);
+        const float v = vector_at<T>(p.row_gate, p.gate_fp32, m0 + row);
         row_gate = pack_pair(v, v);
       }
       bool opened = true;
@@ -789,7 +785,7 @@ __global__ void __launch_bounds__(256)
       for (int j = 0; j < 8; ++j) v[j] = act::value<decltype(kind)::value>(v[j]);
     });
     if (e.gate != nullptr) {
-      get8(static_cast<const T*>(e.gate) + c, k, wide, t);
+      vector_get8<T>(e.gate, e.gate_fp32, c, k, wide, t);
 #pragma unroll
       for (int j = 0; j < 8; ++j) v[j] *= t[j];
     }
@@ -963,6 +959,7 @@ cudaError_t launch_product(const Plan& plan, int dtype, int64_t m, int64_t n, in
   p.y_heads64 = heads64(e.y_heads, e.y_dim);
   p.bias = e.bias;
   p.gate = e.gate;
+  p.gate_fp32 = e.gate_fp32;
   p.act = e.act;
   p.y_fp32 = e.y_type == VGGT_DTYPE_FP32;
   p.residual = e.residual;
@@ -1114,6 +1111,8 @@ int check(const vggt_linear_args* a) {
     return api_fail("the residual and y are of x's type or FP32");
   if (a->activation != VGGT_ACT_NONE && a->z_dtype != a->dtype && a->z_dtype != VGGT_DTYPE_FP32)
     return api_fail("z is of x's type or FP32");
+  if (a->gate && a->gate_dtype != a->dtype && a->gate_dtype != VGGT_DTYPE_FP32)
+    return api_fail("gate is of x's type or FP32");
   if (a->rows < 0 || a->inner < 1 || a->outer < 1) return api_fail("bad size argument");
   if (a->rows > INT_MAX - 512 || a->inner > INT_MAX - 512 || a->outer > INT_MAX - 512)
     return api_fail("too many rows or too wide");
@@ -1165,6 +1164,7 @@ extern "C" int vggt_linear(const vggt_linear_args* a, void* y, int64_t y_stride,
   Epilogue e;
   e.bias = a->bias;
   e.gate = a->gate;
+  e.gate_fp32 = a->gate_dtype == VGGT_DTYPE_FP32;
   e.act = a->activation;
   e.residual = a->residual;
   e.residual_stride = a->residual_stride;

@@ -26,6 +26,7 @@ struct Operand {
 struct Epilogue {
   const void* bias = nullptr;  // [n]
   const void* gate = nullptr;  // [n]
+  bool gate_fp32 = false;      // of gate and row_gate: fp32, or the operands' type
   int act = VGGT_ACT_NONE;
   const void* residual = nullptr;
   int64_t residual_stride = 0;

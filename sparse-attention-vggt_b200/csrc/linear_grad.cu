@@ -27,6 +27,7 @@ struct Sums {
   const void* z;
   int64_t z_stride;
   const void* gate;
+  bool gate_fp32;
   int act;
   void* dz;      // [rows][dz_stride], or null
   void* scaled;  // gate dy (no activation), or null
@@ -58,7 +59,7 @@ __global__ void __launch_bounds__(256, ACT == VGGT_ACT_NONE ? 4 : 2) sums_kernel
       get8(p, n, false, v);
   };
   if (n > 0) {
-    if (a.gate != nullptr) get(static_cast<const T*>(a.gate) + c, gate);
+    if (a.gate != nullptr) vector_get8<T>(a.gate, a.gate_fp32, c, n, WIDE, gate);
     for (int64_t rr = r0 + ry; rr < r1; rr += 8 * kAhead) {
       float d[kAhead][8], z[ACT != VGGT_ACT_NONE ? kAhead : 1][8];
 #pragma unroll
@@ -134,7 +135,7 @@ static void launch_sums(const Sums& a, bool z_fp32, dim3 grid, cudaStream_t stre
 
 // gate W, rounded once more to W's type (bf16): one rounding of dx's factors, as dy gate would be.
 __global__ void __launch_bounds__(256)
-    scale_weight_kernel(const __nv_bfloat16* w, int64_t stride, const __nv_bfloat16* gate,
+    scale_weight_kernel(const __nv_bfloat16* w, int64_t stride, const void* gate, bool gate_fp32,
                         __nv_bfloat16* to, int64_t pad, int64_t outer, int64_t inner) {
   const int64_t groups = (inner + 7) / 8, all = outer * groups;
   for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < all;
@@ -143,7 +144,7 @@ __global__ void __launch_bounds__(256)
     float v[8];
     const int n = (int)min((int64_t)8, inner - c);
     get8(w + r * stride + c, n, true, v);
-    const float g = (float)gate[r];
+    const float g = vector_at<__nv_bfloat16>(gate, gate_fp32, r);
 #pragma unroll
     for (int j = 0; j < 8; ++j) v[j] *= g;
     put8(to + r * pad + c, n, true, v);
@@ -156,6 +157,7 @@ struct Weights {
   int64_t weight_stride;
   const void* bias;
   const void* gate;
+  bool gate_fp32;
   bool act;       // with an activation dz has the gate already, and gate_part the gate's sums
   void* dweight;  // or null
   int64_t dweight_stride;
@@ -183,7 +185,7 @@ template <typename T>
 __global__ void __launch_bounds__(128) finish_weight_kernel(const Slots s, const Weights a) {
   __shared__ float fold[4];
   const int64_t r = blockIdx.x;
-  const float gate = a.gate != nullptr && !a.act ? (float)static_cast<const T*>(a.gate)[r] : 1.f;
+  const float gate = a.gate != nullptr && !a.act ? vector_at<T>(a.gate, a.gate_fp32, r) : 1.f;
   const bool want_dot = a.dgate != nullptr && !a.act;
   float dot = 0.f;
   if (a.product)
@@ -222,7 +224,10 @@ __global__ void __launch_bounds__(128) finish_weight_kernel(const Slots s, const
   g = block_sum(g, fold);
   if (threadIdx.x == 0) {
     if (!a.act && a.bias != nullptr) g = fmaf((float)static_cast<const T*>(a.bias)[r], sum, g);
-    static_cast<T*>(a.dgate)[r] = ElemOps<T>::from_float(g);
+    if (a.gate_fp32)
+      static_cast<float*>(a.dgate)[r] = g;
+    else
+      static_cast<T*>(a.dgate)[r] = ElemOps<T>::from_float(g);
   }
 }
 
@@ -294,6 +299,7 @@ static cudaError_t run_back(const vggt_linear_args* a, const vggt_linear_grads* 
   float* gate_part = reinterpret_cast<float*>(ws + b.gate_part);
   float* slots = reinterpret_cast<float*>(ws + b.slots);
   T* scaled = reinterpret_cast<T*>(ws + b.scaled);
+  const bool gate_fp32 = a->gate_dtype == VGGT_DTYPE_FP32;
   if (b.sums) {
     Sums s{};
     s.dy = g->dy;
@@ -301,6 +307,7 @@ static cudaError_t run_back(const vggt_linear_args* a, const vggt_linear_grads* 
     s.z = g->z;
     s.z_stride = g->z_stride;
     s.gate = a->gate;
+    s.gate_fp32 = gate_fp32;
     s.act = a->activation;
     s.dz = b.copy_dy ? ws + b.dz : nullptr;
     s.scaled = b.scale_dy ? scaled : nullptr;
@@ -311,7 +318,7 @@ static cudaError_t run_back(const vggt_linear_args* a, const vggt_linear_grads* 
     s.outer = outer;
     s.per_block = b.per_block;
     s.wide = outer % 8 == 0 && wide_rows(g->dy, g->dy_stride, a->stream_dtype) &&
-             (!b.act || wide_rows(g->z, g->z_stride, a->z_dtype)) && wide_rows(a->gate, 8, a->dtype);
+             (!b.act || wide_rows(g->z, g->z_stride, a->z_dtype)) && wide_rows(a->gate, 8, a->gate_dtype);
     const dim3 grid((unsigned)((outer + 255) / 256), (unsigned)b.row_blocks);
     const bool z_fp32 = a->z_dtype == VGGT_DTYPE_FP32;
     if (a->stream_dtype == VGGT_DTYPE_FP32)
@@ -331,8 +338,8 @@ static cudaError_t run_back(const vggt_linear_args* a, const vggt_linear_grads* 
       B* to = reinterpret_cast<B*>(ws + b.weight);
       const int64_t all = outer * ((inner + 7) / 8);
       scale_weight_kernel<<<(unsigned)std::min<int64_t>((all + 255) / 256, 148 * 16), 256, 0,
-                            stream>>>(static_cast<const B*>(w.p), w.stride,
-                                      static_cast<const B*>(a->gate), to, b.laid.pad, outer, inner);
+                            stream>>>(static_cast<const B*>(w.p), w.stride, a->gate, gate_fp32, to,
+                                      b.laid.pad, outer, inner);
       if (cudaError_t e = cudaGetLastError()) return e;
       w.p = to;
       w.stride = b.laid.pad;
@@ -359,6 +366,7 @@ static cudaError_t run_back(const vggt_linear_args* a, const vggt_linear_grads* 
     e.y_dim = inner;
     e.y_type = a->dtype;
     if (a->gate && !b.act) e.row_gate = a->gate;
+    e.gate_fp32 = gate_fp32;
     if (b.dot) {
       e.residual = weight.p;
       e.residual_stride = weight.stride;
@@ -374,6 +382,7 @@ static cudaError_t run_back(const vggt_linear_args* a, const vggt_linear_grads* 
   f.weight_stride = weight.stride;
   f.bias = a->bias;
   f.gate = a->gate;
+  f.gate_fp32 = gate_fp32;
   f.act = b.act;
   f.dweight = g->dweight;
   f.dweight_stride = g->dweight_stride;
@@ -419,9 +428,12 @@ extern "C" int vggt_linear_grad(const vggt_linear_args* a, const vggt_linear_gra
       if (int rc = api_cuda(cudaMemset2DAsync(g->dweight, (size_t)g->dweight_stride * 2, 0,
                                               (size_t)a->inner * 2, (size_t)a->outer, st)))
         return rc;
-    for (void* p : {a->bias ? g->dbias : nullptr, a->gate ? g->dgate : nullptr})
-      if (p)
-        if (int rc = api_cuda(cudaMemsetAsync(p, 0, (size_t)a->outer * 2, st))) return rc;
+    void* const sums[2] = {a->bias ? g->dbias : nullptr, a->gate ? g->dgate : nullptr};
+    for (int k = 0; k < 2; ++k) {
+      const size_t size = k == 1 && a->gate_dtype == VGGT_DTYPE_FP32 ? 4 : 2;
+      if (sums[k])
+        if (int rc = api_cuda(cudaMemsetAsync(sums[k], 0, (size_t)a->outer * size, st))) return rc;
+    }
     return api_fail(nullptr);
   }
   if (!g->dy) return api_fail("dy must be non-NULL");

@@ -128,7 +128,7 @@ __global__ void __launch_bounds__(most_warps<MT, COLS>() * 32) rows_kernel(const
     else if (e.z != nullptr)
       static_cast<T*>(e.z)[r * e.z_stride + n] = ElemOps<T>::from_float(v);
     act::dispatch(e.act, [&](auto k) { v = act::value<decltype(k)::value>(v); });
-    if (e.gate != nullptr) v *= (float)static_cast<const T*>(e.gate)[n];
+    if (e.gate != nullptr) v *= vector_at<T>(e.gate, e.gate_fp32, n);
     if (e.y_type == VGGT_DTYPE_FP32) {
       if (e.residual != nullptr)
         v += static_cast<const float*>(e.residual)[r * e.residual_stride + n];

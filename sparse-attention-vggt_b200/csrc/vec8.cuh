@@ -64,6 +64,19 @@ __device__ __forceinline__ void put8(E* p, int n, bool vec, const float* v) {
       if (i < n) Elem<E>::store(p + i, v[i]);
   }
 }
+// An element, or eight, of a vector that is of T or fp32.
+template <typename T>
+__device__ __forceinline__ float vector_at(const void* p, bool fp32, int64_t i) {
+  return fp32 ? static_cast<const float*>(p)[i] : (float)static_cast<const T*>(p)[i];
+}
+template <typename T>
+__device__ __forceinline__ void vector_get8(const void* p, bool fp32, int64_t at, int n, bool vec,
+                                            float* v) {
+  if (fp32)
+    get8(static_cast<const float*>(p) + at, n, vec, v);
+  else
+    get8(static_cast<const T*>(p) + at, n, vec, v);
+}
 // Whether rows at `p` with this stride (in elements of VGGT_DTYPE_*) allow the wide accesses.
 inline bool wide_rows(const void* p, int64_t stride, int type) {
   return p == nullptr || ((reinterpret_cast<uintptr_t>(p) & 15u) == 0 &&

@@ -20,13 +20,16 @@ from .layer import SparseGlobalLayer
 from .qkv import project_qkv
 
 
+def _fp32(t):
+    return None if t is None else t.detach().float().contiguous()
+
+
 def _norm(norm):
     """(weight, bias, eps) of a LayerNorm module or triple, in fp32."""
     if isinstance(norm, torch.nn.LayerNorm):
         norm = norm.weight, norm.bias, norm.eps
     weight, bias, eps = norm
-    keep = lambda t: None if t is None else t.detach().float().contiguous()  # noqa: E731
-    return keep(weight), keep(bias), float(eps)
+    return _fp32(weight), _fp32(bias), float(eps)
 
 
 def _activation(act):
@@ -67,7 +70,7 @@ class GlobalBlock:
                      ``layer_options``)
 
     Weights are converted to ``dtype`` (bf16 or fp16) once, here; the norms'
-    stay in fp32.  x [N, C] may be of ``dtype`` or fp32 (a residual stream held
+    and the scales per channel, which may be far below fp16's range, stay in fp32.  x [N, C] may be of ``dtype`` or fp32 (a residual stream held
     in 32 bits), and so is the result.  A wait that runs out on the device is
     raised as a ValueError by a later call or by ``check_status``, without the
     host's waiting for it; what the call at fault returned is not valid.  Calls
@@ -93,7 +96,7 @@ class GlobalBlock:
         self.norm1, self.norm2 = _norm(norm1), _norm(norm2)
         self.qkv, self.proj, self.fc1, self.fc2 = (tuple(cast(t) for t in pair(m))
                                                   for m in (qkv, proj, fc1, fc2))
-        self.ls1, self.ls2 = cast(ls1), cast(ls2)
+        self.ls1, self.ls2 = _fp32(ls1), _fp32(ls2)
         with deferred_status(self.qkv[0].device):
             pass  # a graph's capture finds the status word in place
 

@@ -44,8 +44,8 @@ def linear(x, weight, bias=None, *, activation=None, gate=None, residual=None, h
            out=None, status=None):
     """residual + gate * activation(x @ weight.T + bias), in one kernel.
 
-    x [..., inner] bf16 or fp16, weight [outer, inner], bias and gate [outer],
-    all of x's dtype; residual [..., outer] of x's dtype or fp32, which is then
+    x [..., inner] bf16 or fp16, weight [outer, inner] and bias [outer] of x's
+    dtype, gate [outer] of x's dtype or fp32; residual [..., outer] of x's dtype or fp32, which is then
     the result's.  ``head_major``: x is [heads, rows, dim], as the attention
     operators return it, and is read in place as [rows, heads * dim] (the result
     is [rows, outer]).  ``activation`` is None, "gelu" (with the normal

@@ -240,3 +240,23 @@ def test_from_module_without_rope_ignores_positions(monkeypatch):
         with pytest.raises(Stop):
             GlobalBlock.from_module(block, tokens_per_frame=TPF)(x, pos, 7)
         assert (seen.pop() is not None) == given
+
+
+def test_linear_takes_a_gate_of_its_type_or_fp32():
+    t = linear_args()
+    t["gate"] = torch.zeros(64)
+    with pytest.raises(ValueError, match="CUDA tensors"):
+        call_linear(t)
+    for gate in (torch.zeros(64, dtype=FP), torch.zeros(64, dtype=torch.float64), torch.zeros(63)):
+        t["gate"] = gate
+        with pytest.raises(ValueError, match="gate must be"):
+            call_linear(t)
+
+
+def test_block_keeps_its_scales_in_fp32():
+    block = parts()
+    block.ls1, block.ls2 = torch.nn.Module(), torch.nn.Module()
+    block.ls1.gamma = torch.nn.Parameter(torch.full((128,), 1e-8))
+    block.ls2.gamma = torch.nn.Parameter(torch.full((128,), 1e-5))
+    half = GlobalBlock.from_module(block, tokens_per_frame=TPF, dtype=FP)
+    assert torch.equal(half.ls1, block.ls1.gamma) and torch.equal(half.ls2, block.ls2.gamma)

@@ -8,10 +8,58 @@ import pytest
 import torch
 
 import vggt_sparse
-from test_gpu_block_ops import BF, F32, FP, U, Linear, make, near
+from test_gpu_block_ops import BF, F32, FP, SMALL, U, Linear, activation, make, near
 from vggt_sparse import _lib
 
 pytestmark = pytest.mark.gpu
+
+
+class Call(Linear):
+    """A call with the bounds of its gradients, in fp16 with those of its factors' subnormal numbers:
+    dz is rounded before the products (and so is gate * dy or gate * W), to v of itself or to half a
+    subnormal step, 2^-25, for each of the products that are added; a gate of 5e-6 is enough.
+    """
+
+    def check_grads(self, dx, dw, db, dg):
+        self.define()
+        v, step = U[self.dtype], 2.0 ** -25 if self.dtype == FP else 0.0
+        dy = self.dy.detach().double().flatten(0, -2)
+        one = torch.ones(1, device=dy.device, dtype=dy.dtype)
+        g = one if self.g is None else self.g.detach().double()
+        z, a, ez = self.z.detach(), self.a.detach(), self.ez.detach()
+        zl = z.clone().requires_grad_()
+        slope, = torch.autograd.grad(activation(zl, self.act).sum(), zl)
+        dz, xd, wd = dy * g * slope, self.xd.detach(), self.wd.detach()
+        if self.act is None:
+            off = off_w = v * dz.abs()
+            off_b = 2.0 ** -22 * dz.abs()
+            off_g = v * dy.abs() * (xd.abs() @ wd.abs().t()) + 2.0 ** -20 * dy.abs() * a.abs()
+        else:
+            off_b = (dy * g).abs() * ((z.abs() <= ez).double() if self.act == "relu"
+                                      else v * z.abs() + ez + 1e-5)
+            off = off_w = off_b + v * dz.abs()
+            off_g = dy.abs() * (1.13 * (v * z.abs() + ez) + 1e-5 * a.abs())
+        add = lambda n: 2.0 ** -23 * (n / 16 + 8)  # noqa: E731
+        n_rows = dy.shape[0]
+        if dx is not None:
+            want = dz @ wd
+            dx = dx.transpose(0, 1).flatten(1) if self.heads else dx.flatten(0, -2)
+            near(dx, want, v * want.abs() + 1.01 * ((off + step) @ wd.abs())
+                 + add(self.outer) * (dz.abs() @ wd.abs()) + SMALL, "dx")
+        if dw is not None:
+            # without an activation the gate scales dW after the product of dy
+            want = dz.t() @ xd
+            near(dw, want, v * want.abs() + 1.01 * ((off_w + step).t() @ xd.abs())
+                 + add(n_rows) * (dz.abs().t() @ xd.abs()) + SMALL, "dw")
+        if db is not None:
+            want = dz.sum(0)
+            near(db, want, v * want.abs() + 1.01 * off_b.sum(0) + 2.0 ** -20 * dz.abs().sum(0) + SMALL,
+                 "db")
+        if dg is not None:
+            want = (dy * a).sum(0)
+            mag = (dy.abs() * (xd.abs() @ wd.abs().t())).sum(0)
+            near(dg, want, v * want.abs() + 1.01 * off_g.sum(0) + (add(n_rows) + add(self.inner)) * mag
+                 + SMALL, "dgate")
 
 
 @pytest.mark.parametrize("scale", [1e-3, 1e-4, 1e-5, 1e-6])
@@ -157,3 +205,70 @@ def test_block_does_not_wait_for_the_gpu(cuda):
     finally:
         torch.cuda.set_sync_debug_mode("default")
     vggt_sparse.check_status()
+
+
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("scale", [0.3, 1e-5, 1e-7])
+def test_block_keeps_its_scales_per_channel(cuda, dtype, scale):
+    """A scale per channel as small as it is initialised, fp16's subnormal numbers and below: on an
+    fp32 stream what the block adds is off by the branches' own roundings, not by the scale's.
+
+    The branch p = proj(attention) is rounded once (u) and scaled in fp32; the MLP half rounds y and
+    the widened tokens once each and ends in fp32, with three roundings' room for each as in
+    test_gpu_block.py: 2 u and 6 u of their norms.  The stream adds 2^-24 of itself, twice.
+    """
+    torch.manual_seed(3)
+    part = Part(2, scale).to(cuda)
+    block = vggt_sparse.GlobalBlock.from_module(part, tokens_per_frame=TPF, dtype=dtype, topk=2)
+    # a stream of the size of what is added to it, so that it hides nothing
+    x, pos = scale * torch.randn(3 * TPF, 128, device=cuda), positions(3, cuda)
+    block.norm1 = block.norm1[:2] + (1e-20,)
+    block.norm2 = block.norm2[:2] + (1e-20,)
+    out = block(x, pos, 7)
+    a = block.attention(x, pos, 7)
+    d = lambda t: t.double()  # noqa: E731
+    p = d(a).transpose(0, 1).flatten(1) @ d(block.proj[0]).t() + d(block.proj[1])
+    p = p * d(part.ls1.gamma.detach())
+    h = d(x) + p
+    y = torch.nn.functional.layer_norm(h, (128,), d(block.norm2[0]), d(block.norm2[1]), 1e-20)
+    z = y @ d(block.fc1[0]).t() + d(block.fc1[1])
+    m = (z * torch.special.ndtr(z)) @ d(block.fc2[0]).t() + d(block.fc2[1])
+    m = m * d(part.ls2.gamma.detach())
+    u = U[dtype]
+    room = 2 * u * p.norm() + 6 * u * m.norm() + 2 * U[F32] * (h + m).norm()
+    assert float((d(out) - h - m).norm()) <= float(room)
+
+
+SIZES = [(1, 64, 64), (20, 512, 4104), (43, 1001, 517), (129, 72, 257), (300, 136, 1024),
+         (1374, 1024, 1024), (2000, 264, 136)]
+
+
+@pytest.mark.parametrize("rows,inner,outer", SIZES)
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("act,residual", [(None, None), ("gelu", F32)])
+@pytest.mark.parametrize("misaligned", [False, True])
+def test_linear_with_a_gate_in_fp32(cuda, rows, inner, outer, dtype, act, residual, misaligned):
+    c = Call(cuda, rows, inner, outer, dtype, act=act, gate=True, residual=residual, seed=outer)
+    g = torch.Generator().manual_seed(1)
+    c.g = make(g, cuda, outer + 1, dtype=F32, scale=0.5)
+    c.g = c.g[1:] if misaligned else c.g[:outer].contiguous()
+    with torch.no_grad():
+        c.check(c.call())
+    leaves = [t.requires_grad_() for t in c.leaves()]
+    y = c.call()
+    grads = torch.autograd.grad(y, leaves, c.dy, retain_graph=True)
+    assert [d.dtype for d in grads] == [t.dtype for t in leaves]
+    c.check_grads(*grads[:4])
+    one, = torch.autograd.grad(y, c.g, c.dy)
+    assert torch.equal(one, grads[3])
+
+
+def test_linear_without_rows_and_a_gate_in_fp32(cuda):
+    x = torch.zeros(0, 64, dtype=BF, device=cuda)
+    w = torch.ones(16, 64, dtype=BF, device=cuda)
+    g = torch.ones(16, device=cuda, requires_grad=True)
+    room = torch.ones(64, device=cuda)  # the allocator's next block, so that zeros are not by chance
+    del room
+    y = vggt_sparse.linear(x, w, gate=g)
+    d, = torch.autograd.grad(y, g, torch.zeros_like(y))
+    assert d.dtype == F32 and bool((d == 0).all())
