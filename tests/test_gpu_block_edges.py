@@ -272,3 +272,29 @@ def test_linear_without_rows_and_a_gate_in_fp32(cuda):
     y = vggt_sparse.linear(x, w, gate=g)
     d, = torch.autograd.grad(y, g, torch.zeros_like(y))
     assert d.dtype == F32 and bool((d == 0).all())
+
+
+@pytest.mark.parametrize("rows,inner,outer", [(300, 136, 200), (1374, 1024, 1024), (2049, 2056, 2040),
+                                              (4000, 1024, 1024), (129, 4096, 128)])
+def test_every_product_gives_up_its_waits(cuda, short_waits, rows, inner, outer):
+    """One CTA to a tile and pairs, whole and split: each reports and leaves, and what comes after it
+    on the SMs is right."""
+    short_waits()
+    c = Linear(cuda, rows, inner, outer, gate=True, residual=BF)
+    want = c.call()
+    leaves = [t.requires_grad_() for t in c.leaves()]
+    y = c.call()
+    status = torch.zeros(1, dtype=torch.int32, device=cuda)
+    with torch.no_grad():
+        _lib.set_wait_limit_ns(2_000_000), _lib.set_wait_selftest(True)
+        c.call(status=status)
+        short_waits()
+        assert int(status) == _lib.STATUS_TIMEOUT
+        status.zero_()
+        assert torch.equal(c.call(status=status), want) and int(status) == 0
+    grads = torch.autograd.grad(y, leaves, c.dy, retain_graph=True)
+    _lib.set_wait_limit_ns(2_000_000), _lib.set_wait_selftest(True)
+    torch.autograd.grad(y, leaves, c.dy, retain_graph=True)
+    short_waits()
+    for a, b in zip(grads, torch.autograd.grad(y, leaves, c.dy)):
+        assert torch.equal(a, b)
