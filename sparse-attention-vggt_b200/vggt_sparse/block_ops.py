@@ -13,7 +13,8 @@ projection, LayerScale, residual, LayerNorm, MLP, LayerScale, residual);
 Both are differentiable, once, in all their tensors, by a backward pass (tensors
 with a forward-mode tangent are refused).  Sums, statistics and
 activations are formed in fp32 and rounded once, to the result's type; a
-backward pass adds in a fixed order, so that equal calls give equal results.
+backward pass adds in a fixed order, so that equal calls give equal results, and
+a gradient is the same alone and among others.
 
 Like the other operators these only enqueue work on the current stream of their
 tensors' device, and may be captured in CUDA graphs.

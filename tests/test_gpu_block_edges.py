@@ -8,7 +8,7 @@ import pytest
 import torch
 
 import vggt_sparse
-from test_gpu_block_ops import BF, F32, FP, SMALL, U, Linear, activation, make, near
+from test_gpu_block_ops import BF, F32, FP, SMALL, U, Linear, Norm, activation, make, near
 from vggt_sparse import _lib
 
 pytestmark = pytest.mark.gpu
@@ -298,3 +298,25 @@ def test_every_product_gives_up_its_waits(cuda, short_waits, rows, inner, outer)
     short_waits()
     for a, b in zip(grads, torch.autograd.grad(y, leaves, c.dy)):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dtype,stream", [(BF, BF), (FP, F32)])
+@pytest.mark.parametrize("rows,width,norm,post,groups", [(200, 1024, "layer", "layer", 1),
+                                                         (900, 264, "rms", "layer", 1),
+                                                         (40, 4096, "layer", "rms", 4),
+                                                         (300, 520, "layer", None, 3),
+                                                         (33, 2100, "layer", "layer", 0)])
+def test_norm_gradients_by_themselves(cuda, dtype, stream, rows, width, norm, post, groups):
+    """Each gradient alone, and all but one, have the bits that they have among all."""
+    c = Norm(cuda, rows, width, dtype, stream, norm, post, groups=groups)
+    leaves = {n: t.requires_grad_() for n, t in c.leaves().items()}
+    y, h = c.call()
+    take = lambda names: torch.autograd.grad(  # noqa: E731
+        (y, h), [leaves[n] for n in names], (c.dy, c.dh), retain_graph=True)
+    all_of = dict(zip(leaves, take(list(leaves))))
+    c.check(y.detach(), h.detach(), all_of, c.dy, c.dh)
+    for n in leaves:
+        others = [m for m in leaves if m != n]
+        for names in ([n], others):
+            for m, d in zip(names, take(names)):
+                assert torch.equal(d, all_of[m]), (m, names)
