@@ -58,7 +58,14 @@ int64_t integer(PyObject* o, const char* name) {
   }
   return v;
 }
-bool truth(PyObject* o) { return PyObject_IsTrue(o) == 1; }
+bool truth(PyObject* o, const char* name) {
+  const int v = PyObject_IsTrue(o);
+  if (v < 0) {
+    PyErr_Clear();
+    refuse("%s must be a truth value", name);
+  }
+  return v == 1;
+}
 
 void* ptr(const at::Tensor* t) { return t ? t->data_ptr() : nullptr; }
 

@@ -641,7 +641,7 @@ PyObject* linear(PyObject*, PyObject* const* o, Py_ssize_t n) {
     in.activation = activation_of(o[3]);
     in.gate = given_or_none(o[4], "gate");
     in.residual = given_or_none(o[5], "residual");
-    in.head_major = truth(o[6]);
+    in.head_major = truth(o[6], "head_major");
     in.status = given_or_none(o[8], "status");
     const at::Tensor out = given_or_none(o[7], "out");
     no_tangents(in.x, in.weight, in.bias, in.gate, in.residual, out);

@@ -173,7 +173,7 @@ PyObject* rotary(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const at::Tensor out = given ? *given : at::empty(x.sizes(), x.options());
     check(vggt_rotary(x.data_ptr(), dtype, x.size(0), (int)x.size(1), (int)x.size(2), x.stride(0),
                       x.stride(1), t.positions, t.axes, t.freq, t.pairs, t.layout,
-                      (float)number(a[4], "lengthen"), truth(a[5]), out.data_ptr(), out.stride(0),
+                      (float)number(a[4], "lengthen"), truth(a[5], "inverse"), out.data_ptr(), out.stride(0),
                       out.stride(1), c10::cuda::getCurrentCUDAStream().stream()));
     return returned(a[6], out);
   });
@@ -289,7 +289,7 @@ PyObject* attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
         q.data_ptr(), p.dtype, total, qr.token, qr.head, kp.data_ptr(), vp.data_ptr(),
         p.pages, (int)p.heads, (int)p.page, (int)p.dim, p.page_stride, p.head_stride, p.row_stride,
         p.table, p.width, p.seqs, static_cast<const int32_t*>(lengths.data_ptr()),
-        static_cast<const int32_t*>(starts.data_ptr()), (int)group, truth(a[8]), scale, max_new,
+        static_cast<const int32_t*>(starts.data_ptr()), (int)group, truth(a[8], "causal"), scale, max_new,
         max_len, out.data_ptr(), to.token, to.head, static_cast<float*>(lse.data_ptr()),
         word, ws.data_ptr(), ws.numel() * ws.element_size(), stream));
     PyObject *o = returned(a[10], out), *l = returned(a[11], lse);
@@ -327,7 +327,7 @@ PyObject* weigh(PyObject*, PyObject* const* a, Py_ssize_t n) {
         static_cast<const float*>(lse.data_ptr()), kp.data_ptr(), p.pages, (int)p.heads,
         (int)p.page, (int)p.dim, p.page_stride, p.head_stride, p.row_stride, p.table, p.width,
         p.seqs, static_cast<const int32_t*>(lengths.data_ptr()),
-        static_cast<const int32_t*>(starts.data_ptr()), (int)group, truth(a[9]), scale,
+        static_cast<const int32_t*>(starts.data_ptr()), (int)group, truth(a[9], "causal"), scale,
         (float)number(a[11], "decay"), integer(a[7], "max_new"), max_len,
         static_cast<float*>(weights.data_ptr()), word,
         c10::cuda::getCurrentCUDAStream().stream()));

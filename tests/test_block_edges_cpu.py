@@ -260,3 +260,12 @@ def test_block_keeps_its_scales_in_fp32():
     block.ls2.gamma = torch.nn.Parameter(torch.full((128,), 1e-5))
     half = GlobalBlock.from_module(block, tokens_per_frame=TPF, dtype=FP)
     assert torch.equal(half.ls1, block.ls1.gamma) and torch.equal(half.ls2, block.ls2.gamma)
+
+
+def test_a_flag_that_is_no_truth_value_is_refused():
+    """Its exception must not stay behind a result."""
+    t = linear_args()
+    with pytest.raises(ValueError, match="head_major must be a truth value"):
+        call_linear(t, head_major=torch.zeros(2))
+    with pytest.raises(ValueError, match="CUDA tensors"):
+        call_linear(t, head_major=0)
