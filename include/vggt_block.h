@@ -56,9 +56,10 @@ typedef struct vggt_vector {
  * x [rows][inner], or with heads > 1 head-major: [heads][rows][inner / heads]
  * with x_head_stride between heads, read as [rows][inner].  weight
  * [outer][inner], bias [outer], x of dtype (BF16 or FP16); gate [outer] of
- * gate_dtype (dtype or FP32); residual and y [rows][outer] of stream_dtype, which is dtype or FP32.  z
- * [rows][outer] of z_dtype (dtype or FP32), where non-NULL, gets the
- * activation's argument for the backward pass.  residual and y may be the same.
+ * dtype, or with gate_fp32 FP32; residual and y [rows][outer] of stream_dtype,
+ * which is dtype or FP32.  z [rows][outer] of z_dtype (dtype or FP32), where
+ * non-NULL, gets the activation's argument for the backward pass.  residual and
+ * y may be the same; otherwise the outputs lie apart from the inputs.
  *
  * x and weight are read in place where their rows (and heads, then of a multiple
  * of 64 elements) start on 16 bytes, else copied into the workspace first.
@@ -81,7 +82,7 @@ typedef struct vggt_linear_args {
   int64_t residual_stride;
   int activation;
   int z_dtype;          /* of z, here and in the backward pass */
-  int gate_dtype;       /* of gate and its gradient */
+  int gate_fp32;        /* nonzero: gate and its gradient are FP32, not of dtype */
 } vggt_linear_args;
 
 size_t vggt_linear_workspace_size(const vggt_linear_args* args);
@@ -92,7 +93,7 @@ int vggt_linear(const vggt_linear_args* args, void* y, int64_t y_stride, void* z
  * Gradients of the above from that of y (dy, of stream_dtype): dx [rows][inner]
  * or, with dx_head_stride > 0, head-major like x (heads of a multiple of 64
  * elements), dweight [outer][inner], dbias [outer], all of dtype, and dgate
- * [outer] of gate_dtype; that of residual is dy.  z is what vggt_linear wrote;
+ * [outer] of the gate's type; that of residual is dy.  z is what vggt_linear wrote;
  * without an activation it is not needed.  Sums are formed in a fixed order.
  */
 typedef struct vggt_linear_grads {

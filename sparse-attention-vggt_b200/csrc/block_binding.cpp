@@ -444,12 +444,11 @@ struct LinearCall {
     const at::Tensor &bt = in.bias, &gt = in.gate;
     if (bt.defined() && (bt.dim() != 1 || bt.size(0) != a.outer || bt.scalar_type() != type))
       refuse("bias must be [outer], of x's dtype");
-    a.gate_dtype = a.dtype;
     if (gt.defined()) {
       if (gt.dim() != 1 || gt.size(0) != a.outer ||
           (gt.scalar_type() != type && gt.scalar_type() != at::kFloat))
         refuse("gate must be [outer], of x's dtype or FP32");
-      a.gate_dtype = dtype_of("gate", gt.scalar_type(), true);
+      a.gate_fp32 = gt.scalar_type() != type;
     }
     stream = type;
     if (in.residual.defined()) {

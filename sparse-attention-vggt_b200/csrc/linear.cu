@@ -1123,8 +1123,6 @@ int check(const vggt_linear_args* a) {
     return api_fail("the residual and y are of x's type or FP32");
   if (a->activation != VGGT_ACT_NONE && a->z_dtype != a->dtype && a->z_dtype != VGGT_DTYPE_FP32)
     return api_fail("z is of x's type or FP32");
-  if (a->gate && a->gate_dtype != a->dtype && a->gate_dtype != VGGT_DTYPE_FP32)
-    return api_fail("gate is of x's type or FP32");
   if (a->rows < 0 || a->inner < 1 || a->outer < 1) return api_fail("bad size argument");
   if (a->rows > INT_MAX - 512 || a->inner > INT_MAX - 512 || a->outer > INT_MAX - 512)
     return api_fail("too many rows or too wide");
@@ -1176,7 +1174,7 @@ extern "C" int vggt_linear(const vggt_linear_args* a, void* y, int64_t y_stride,
   Epilogue e;
   e.bias = a->bias;
   e.gate = a->gate;
-  e.gate_fp32 = a->gate_dtype == VGGT_DTYPE_FP32;
+  e.gate_fp32 = a->gate_fp32 != 0;
   e.act = a->activation;
   e.residual = a->residual;
   e.residual_stride = a->residual_stride;

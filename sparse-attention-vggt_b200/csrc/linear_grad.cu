@@ -299,7 +299,7 @@ static cudaError_t run_back(const vggt_linear_args* a, const vggt_linear_grads* 
   float* gate_part = reinterpret_cast<float*>(ws + b.gate_part);
   float* slots = reinterpret_cast<float*>(ws + b.slots);
   T* scaled = reinterpret_cast<T*>(ws + b.scaled);
-  const bool gate_fp32 = a->gate_dtype == VGGT_DTYPE_FP32;
+  const bool gate_fp32 = a->gate_fp32 != 0;
   if (b.sums) {
     Sums s{};
     s.dy = g->dy;
@@ -318,7 +318,8 @@ static cudaError_t run_back(const vggt_linear_args* a, const vggt_linear_grads* 
     s.outer = outer;
     s.per_block = b.per_block;
     s.wide = outer % 8 == 0 && wide_rows(g->dy, g->dy_stride, a->stream_dtype) &&
-             (!b.act || wide_rows(g->z, g->z_stride, a->z_dtype)) && wide_rows(a->gate, 8, a->gate_dtype);
+             (!b.act || wide_rows(g->z, g->z_stride, a->z_dtype)) &&
+             wide_rows(a->gate, 8, gate_fp32 ? VGGT_DTYPE_FP32 : a->dtype);
     const dim3 grid((unsigned)((outer + 255) / 256), (unsigned)b.row_blocks);
     const bool z_fp32 = a->z_dtype == VGGT_DTYPE_FP32;
     if (a->stream_dtype == VGGT_DTYPE_FP32)
@@ -430,7 +431,7 @@ extern "C" int vggt_linear_grad(const vggt_linear_args* a, const vggt_linear_gra
         return rc;
     void* const sums[2] = {a->bias ? g->dbias : nullptr, a->gate ? g->dgate : nullptr};
     for (int k = 0; k < 2; ++k) {
-      const size_t size = k == 1 && a->gate_dtype == VGGT_DTYPE_FP32 ? 4 : 2;
+      const size_t size = k == 1 && a->gate_fp32 ? 4 : 2;
       if (sums[k])
         if (int rc = api_cuda(cudaMemsetAsync(sums[k], 0, (size_t)a->outer * size, st))) return rc;
     }

@@ -1,5 +1,6 @@
 """Calls of the block's operators that are refused before anything is launched: a batch
 of samples, derivatives that are not there, outputs that lie in inputs."""
+import ctypes
 import os
 
 import pytest
@@ -269,3 +270,23 @@ def test_a_flag_that_is_no_truth_value_is_refused():
         call_linear(t, head_major=torch.zeros(2))
     with pytest.raises(ValueError, match="CUDA tensors"):
         call_linear(t, head_major=0)
+
+
+class LinearArgs(ctypes.Structure):
+    """vggt_linear_args (include/vggt_block.h)."""
+    _fields_ = ([(n, ctypes.c_int64) for n in ("rows", "inner", "outer")]
+                + [("dtype", ctypes.c_int), ("stream_dtype", ctypes.c_int), ("x", ctypes.c_void_p)]
+                + [(n, ctypes.c_int64) for n in ("x_stride", "x_head_stride", "heads")]
+                + [("weight", ctypes.c_void_p), ("weight_stride", ctypes.c_int64)]
+                + [(n, ctypes.c_void_p) for n in ("bias", "gate", "residual")]
+                + [("residual_stride", ctypes.c_int64)]
+                + [(n, ctypes.c_int) for n in ("activation", "z_dtype", "gate_fp32")])
+
+
+@pytest.mark.parametrize("dtype", [0, 1])  # VGGT_DTYPE_BF16, VGGT_DTYPE_FP16
+def test_a_gate_is_of_the_products_type_where_nothing_is_said(lib, dtype):
+    """A caller that zeroes the arguments and sets what it has had to set so far."""
+    a = LinearArgs(rows=0, inner=8, outer=8, dtype=dtype, stream_dtype=dtype, gate=256)
+    assert lib.vggt_linear(ctypes.byref(a), None, 8, None, 0, None, None, 0, None) == 0
+    a.dtype = 5
+    assert lib.vggt_linear(ctypes.byref(a), None, 8, None, 0, None, None, 0, None) < 0
