@@ -1,11 +1,12 @@
 // Matrix product on the tensor cores with bias, activation, gate and residual in its epilogue.
 //
-// A tile of C is 128 CTA x 128 CTA elements, CTA = 1 or 2 CTAs (a pair works on one tile: each
-// holds half of A's rows and half of B's, the MMA of the pair reads both halves of B).  Warp 0
-// streams the operands by TMA through a ring of 64-element reduction blocks, warp 1 issues the
-// MMAs into one of two accumulators in TMEM, and warps 4-19, four warpgroups of which each takes 64
-// columns, run the epilogue of the tile before: TMEM -> registers -> bias, activation, gate,
-// residual -> the group's swizzled 16 KB buffer -> TMA store.  The residual comes by TMA into the
+// A tile of C is worked on by one CTA (128 x 64 or 128 x 128 elements) or by a pair (256 x 128 or
+// 256 x 256: each holds half of A's rows and half of B's, the MMA of the pair reads both halves of
+// B).  Warp 0 streams the operands by TMA through a ring of 64-element reduction blocks, warp 1
+// issues the MMAs into one of two accumulators in TMEM, and warps 4-19, four warpgroups of which
+// each takes a quarter of the columns, 32 at least (of 64 columns two take all), run the epilogue of
+// the tile before: TMEM -> registers -> bias, activation, gate, residual -> the group's swizzled
+// 16 KB buffer -> TMA store.  The residual comes by TMA into the
 // same buffer before.  What TMA cannot address (odd widths, other strides) is copied between
 // buffer and memory by the warps that own the rows.  (With two warpgroups an activation's latencies
 // bounded the kernel.)

@@ -259,8 +259,8 @@ static Back plan_back(const vggt_linear_args* a, const vggt_linear_grads* g) {
     // the gate goes to the smaller factor of dx, or to dy where that is rounded anyway: one
     // rounding of a factor in either case.  In fp16 always to dy: gate W would fall among the
     // subnormal numbers for a gate of 1e-4 (dx off by 1 %; by 10 % for 1e-5) and, unlike gate dy,
-    // not come out of them with a scaled loss (22,000 rows of 4096 -> 1024,
-    // forward and gradient: 444 to 464 us with the gate on W, 439 to 494 on dy)
+    // not come out of them with a scaled loss (22,000 rows of 4096 -> 1024, forward and gradient:
+    // 444 to 464 us with the gate on W, 439 to 494 on dy)
     b.scale_dy = b.copy_dy || a->dtype == VGGT_DTYPE_FP16 || a->rows < a->inner;
     b.scale_w = !b.scale_dy;
   }

@@ -510,10 +510,9 @@ extern "C" int vggt_residual_norm_grad(const vggt_residual_norm_args* args,
   f.a.vec = f.a.vec && wide_rows(f.dy, f.dy_stride, f.a.type) && wide_rows(f.dh, f.dh_stride, f.a.stream_type) &&
             wide_rows(f.dx, f.dx_stride, f.a.stream_type) && wide_rows(f.dbranch, f.dbranch_stride, f.a.type);
   // by what the call has, not by what is wanted of it: the kernels add in different orders, and a
-  // gradient is the same alone and among others (where a
-  // post norm's biases are there and their gradients are not wanted, the kernel without their sums
-  // would be faster: 7,996 x 4096 with the forward pass 241 us against 206, 30,000 x 1024 195
-  // against 174)
+  // gradient is the same alone and among others (where biases are there and their gradients are not
+  // wanted, the kernel without their sums would be faster: 7,996 x 4096 with the forward pass 206 us
+  // against 241, 30,000 x 1024 174 against 195)
   const bool biases = args->bias.data != nullptr || args->post_bias.data != nullptr;
   const int post = f.a.post == 0 ? 0 : biases ? 2 : 1;
   const Grid grid = grid_of(rows, width, post);

@@ -70,10 +70,11 @@ class GlobalBlock:
                      ``layer_options``)
 
     Weights are converted to ``dtype`` (bf16 or fp16) once, here; the norms'
-    and the scales per channel, which may be far below fp16's range, stay in fp32.  x [N, C] may be of ``dtype`` or fp32 (a residual stream held
-    in 32 bits), and so is the result.  A wait that runs out on the device is
-    raised as a ValueError by a later call or by ``check_status``, without the
-    host's waiting for it; what the call at fault returned is not valid.  Calls
+    and the scales per channel, which may be far below fp16's range, stay in fp32.
+    x [N, C] may be of ``dtype`` or fp32 (a residual stream held in 32 bits), and so
+    is the result.  A wait that runs out on the device is raised as a ValueError by
+    a later call or by ``check_status``, without the host's waiting for it; what the
+    call at fault returned is not valid.  Calls
     share the layer's buffers: they belong on one stream, or behind one another.
     There is no gradient through the attention: a call runs without one.  ``mlp``
     alone is differentiable in x.

@@ -112,8 +112,9 @@ def check_status(device=None, wait=True):
 def deferred_status(device):
     """The status word of ``device`` (None where that is no GPU) for the calls of a
     ``with`` block: errors of earlier ones are raised first, and what these find is
-    raised by a later one or by ``check_status``.  Nothing waits, and a graph capture
-    takes only the word."""
+    raised by a later one or by ``check_status``.  Nothing waits but a host that is
+    as many calls ahead as there are status copies, for the oldest of them; a graph
+    capture takes only the word."""
     if device.type != "cuda":
         yield None
         return

@@ -46,10 +46,10 @@ def linear(x, weight, bias=None, *, activation=None, gate=None, residual=None, h
     """residual + gate * activation(x @ weight.T + bias), in one kernel.
 
     x [..., inner] bf16 or fp16, weight [outer, inner] and bias [outer] of x's
-    dtype, gate [outer] of x's dtype or fp32; residual [..., outer] of x's dtype or fp32, which is then
-    the result's.  ``head_major``: x is [heads, rows, dim], as the attention
-    operators return it, and is read in place as [rows, heads * dim] (the result
-    is [rows, outer]).  ``activation`` is None, "gelu" (with the normal
+    dtype, gate [outer] of x's dtype or fp32; residual [..., outer] of x's dtype
+    or fp32, which is then the result's.  ``head_major``: x is [heads, rows, dim],
+    as the attention operators return it, and is read in place as
+    [rows, heads * dim] (the result is [rows, outer]).  ``activation`` is None, "gelu" (with the normal
     distribution), "gelu_tanh", "silu" or "relu"; ``gate`` scales per channel
     (LayerScale).
 
@@ -60,8 +60,8 @@ def linear(x, weight, bias=None, *, activation=None, gate=None, residual=None, h
     as ever, where they may fall below its range.
 
     ``out`` (contiguous; residual itself, or apart from every input) takes the
-    result where no gradient is needed.  ``status``, an int32 tensor, gets VGGT_STATUS_TIMEOUT if a wait of
-    the kernel ran out.
+    result where no gradient is needed.  ``status``, an int32 tensor, gets
+    VGGT_STATUS_TIMEOUT if a wait of the kernel, or of its backward pass, ran out.
     """
     return _binding().linear(x, weight, bias, activation, gate, residual, head_major, out, status)
 
