@@ -35,8 +35,10 @@ class _StatusMonitor:
     calls enqueue; completed copies are inspected without blocking."""
 
     def __init__(self, device):
-        self.word = torch.zeros(1, device=device, dtype=torch.int32)
-        self.host = torch.zeros(_RING, dtype=torch.int32).pin_memory()
+        # the first call may run in inference mode, whose tensors could not be written outside it
+        with torch.inference_mode(False):
+            self.word = torch.zeros(1, device=device, dtype=torch.int32)
+            self.host = torch.zeros(_RING, dtype=torch.int32).pin_memory()
         self.events = [None] * _RING
         self.next = 0
 

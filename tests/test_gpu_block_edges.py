@@ -2,6 +2,7 @@
 
 Bounds as in test_gpu_block_ops.py (u: unit roundoff of an output's type, v: of the products').
 """
+import importlib
 import math
 
 import pytest
@@ -320,3 +321,19 @@ def test_norm_gradients_by_themselves(cuda, dtype, stream, rows, width, norm, po
         for names in ([n], others):
             for m, d in zip(names, take(names)):
                 assert torch.equal(d, all_of[m]), (m, names)
+
+
+def test_block_first_run_in_inference_mode(cuda, monkeypatch):
+    """What the first call sets up must serve calls in every mode."""
+    module = importlib.import_module("vggt_sparse.block_attention")
+    monkeypatch.setattr(module, "_monitors", {})
+    x, pos = torch.randn(3 * TPF, 128, device=cuda), positions(3, cuda)
+    with torch.inference_mode():
+        block = vggt_sparse.GlobalBlock.from_module(Part(2).to(cuda), tokens_per_frame=TPF, topk=2)
+        want = block(x, pos, 7).clone()
+    assert torch.equal(block(x, pos, 7), want)
+    with torch.no_grad():
+        assert torch.equal(block(x, pos, 7), want)
+    with torch.inference_mode():
+        assert torch.equal(block(x, pos, 7), want)
+    vggt_sparse.check_status()
