@@ -101,9 +101,13 @@ def check_status(device=None, wait=True):
     (default: the current device) found bad ids, counts or head ids, or gave up
     a wait.  With ``wait`` (default) it first waits for every pending status copy,
     and for what is enqueued on the current stream (replayed graphs and backward
-    passes, which no copy follows)."""
+    passes, which no copy follows).  Within the capture of a graph it does nothing:
+    call it behind the replay."""
     dev = torch.device("cuda", torch.cuda.current_device()) if device is None \
         else torch.device(device)
+    with torch.cuda.device(dev):
+        if torch.cuda.is_current_stream_capturing():
+            return  # what is captured has not run, and a wait would end the capture
     monitor = _monitor(dev)
     if wait:
         monitor.enqueue_copy()

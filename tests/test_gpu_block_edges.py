@@ -337,3 +337,18 @@ def test_block_first_run_in_inference_mode(cuda, monkeypatch):
     with torch.inference_mode():
         assert torch.equal(block(x, pos, 7), want)
     vggt_sparse.check_status()
+
+
+def test_check_status_within_a_capture(cuda):
+    """It takes nothing into the graph, and the capture goes on."""
+    block = vggt_sparse.GlobalBlock.from_module(Part(2).to(cuda), tokens_per_frame=TPF, topk=2)
+    x = torch.randn(3 * TPF, 128, device=cuda)
+    want = block.mlp(x)
+    vggt_sparse.check_status()
+    graph = torch.cuda.CUDAGraph()
+    with torch.no_grad(), torch.cuda.graph(graph):
+        out = block.mlp(x)
+        vggt_sparse.check_status()
+    graph.replay()
+    vggt_sparse.check_status()
+    assert torch.equal(out, want)
