@@ -6,10 +6,9 @@
 // issues the MMAs into one of two accumulators in TMEM, and warps 4-19, four warpgroups of which
 // each takes a quarter of the columns, 32 at least (of 64 columns two take all), run the epilogue of
 // the tile before: TMEM -> registers -> bias, activation, gate, residual -> the group's swizzled
-// 16 KB buffer -> TMA store.  The residual comes by TMA into the
-// same buffer before.  What TMA cannot address (odd widths, other strides) is copied between
-// buffer and memory by the warps that own the rows.  (With two warpgroups an activation's latencies
-// bounded the kernel.)
+// 16 KB buffer -> TMA store.  The residual comes by TMA into the same buffer before.  What TMA
+// cannot address (odd widths, other strides) is copied between buffer and memory by the warps that
+// own the rows.  (With two warpgroups an activation's latencies bounded the kernel.)
 //
 // Bound by the tensor cores and by the operands' way from L2 (a pair's 256 x 256 tile needs
 // 64 B a cycle and SM at the full rate, a single CTA's 128 x 128 twice that).

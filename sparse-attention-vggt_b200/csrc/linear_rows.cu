@@ -1,6 +1,6 @@
 // The matrix product of `linear` for few rows (single tokens, a decode batch).
 //
-// Bound by reading the weight once.  A block takes COLS = 8 or 16 columns of y, i.e. as many rows
+// Bound by reading the weight once.  A block takes COLS = 8, 16 or 32 columns of y, i.e. as many rows
 // of the weight; its warps deal out the reduced length in pieces of 64 elements.  A lane reads 16
 // bytes of a weight row and of x's rows straight into the registers of mma.sync m16n8k16 (x the
 // 16 rows, the weight the 8 columns): the instruction sums over the reduced index, so that which
