@@ -880,38 +880,46 @@ static EncodeTiledFn encode_fn() {
   return fn;
 }
 
+// Encodes a tiled map.  A thread that has called nothing of the runtime's yet (autograd's on a
+// process's first gradient, a new one of the caller's) has no context to encode in: cudaSetDevice
+// gives it its device's, also within a stream's capture.
+static bool encode(CUtensorMap* map, CUtensorMapDataType type, cuuint32_t rank, const void* ptr,
+                   const cuuint64_t* dims, const cuuint64_t* strides, const cuuint32_t* box,
+                   CUtensorMapSwizzle swizzle) {
+  const EncodeTiledFn fn = encode_fn();
+  if (!fn) return false;
+  const cuuint32_t step[5] = {1, 1, 1, 1, 1};
+  auto run = [&] {
+    return fn(map, type, rank, const_cast<void*>(ptr), dims, strides, box, step,
+              CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+  };
+  if (run()) return true;
+  int dev = 0;
+  return cudaGetDevice(&dev) == cudaSuccess && cudaSetDevice(dev) == cudaSuccess && run();
+}
+
 // [heads, rows, 64] tensor of 2-byte elements, box (64, box_rows, 1), 128-B swizzle.
 static bool make_map(CUtensorMap* map, const void* ptr, int dtype, int64_t heads, int64_t rows,
                      uint32_t box_rows) {
-  EncodeTiledFn fn = encode_fn();
-  if (!fn) return false;
   const cuuint64_t dims[3] = {(cuuint64_t)HD, (cuuint64_t)rows, (cuuint64_t)heads};
   const cuuint64_t strides[2] = {(cuuint64_t)HD * 2, (cuuint64_t)rows * HD * 2};
   const cuuint32_t box[3] = {(cuuint32_t)HD, box_rows, 1};
-  const cuuint32_t estr[3] = {1, 1, 1};
   const CUtensorMapDataType dt =
       dtype == VGGT_DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
-  CUresult r = fn(map, dt, 3, const_cast<void*>(ptr), dims, strides, box, estr,
-                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  return r == CUDA_SUCCESS;
+  return encode(map, dt, 3, ptr, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
 }  // namespace tcattn
 
 bool encode_tmap_3d_sw128(CUtensorMap* map, const void* ptr, int dtype, int64_t d0, int64_t d1,
                           int64_t d2, uint32_t box0, uint32_t box1) {
-  tcattn::EncodeTiledFn fn = tcattn::encode_fn();
-  if (!fn) return false;
   const cuuint64_t dims[3] = {(cuuint64_t)d0, (cuuint64_t)d1, (cuuint64_t)d2};
   const cuuint64_t strides[2] = {(cuuint64_t)d0 * 2, (cuuint64_t)(d0 * d1) * 2};
   const cuuint32_t box[3] = {box0, box1, 1};
-  const cuuint32_t estr[3] = {1, 1, 1};
   const CUtensorMapDataType dt =
       dtype == VGGT_DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
-  return fn(map, dt, 3, const_cast<void*>(ptr), dims, strides, box, estr,
-            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+  return tcattn::encode(map, dt, 3, ptr, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
 bool encode_tmap_sw128(CUtensorMap* map, const void* ptr, int dtype, int rank,
@@ -921,23 +929,19 @@ bool encode_tmap_sw128(CUtensorMap* map, const void* ptr, int dtype, int rank,
 
 bool encode_tmap(CUtensorMap* map, const void* ptr, int dtype, int rank, const uint64_t* dims,
                  const uint64_t* strides, const uint32_t* box, int swizzle) {
-  tcattn::EncodeTiledFn fn = tcattn::encode_fn();
-  if (!fn || rank < 1 || rank > 5) return false;
+  if (rank < 1 || rank > 5) return false;
   cuuint64_t d[5], s[5];
-  cuuint32_t b[5], estr[5];
+  cuuint32_t b[5];
   for (int i = 0; i < rank; ++i) {
     d[i] = dims[i];
     s[i] = i + 1 < rank ? strides[i] : 0;
     b[i] = box[i];
-    estr[i] = 1;
   }
   const CUtensorMapDataType dt = dtype == VGGT_DTYPE_BF16   ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
                                  : dtype == VGGT_DTYPE_FP16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
                                                             : CU_TENSOR_MAP_DATA_TYPE_FLOAT32;
-  return fn(map, dt, (cuuint32_t)rank, const_cast<void*>(ptr), d, s, b, estr,
-            CU_TENSOR_MAP_INTERLEAVE_NONE,
-            swizzle == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
-            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+  return tcattn::encode(map, dt, (cuuint32_t)rank, ptr, d, s, b,
+                        swizzle == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
 bool attn_tc05_supported(const AttnArgs& a) {

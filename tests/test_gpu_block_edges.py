@@ -4,6 +4,10 @@ Bounds as in test_gpu_block_ops.py (u: unit roundoff of an output's type, v: of 
 """
 import importlib
 import math
+import os
+import subprocess
+import sys
+import threading
 
 import pytest
 import torch
@@ -352,3 +356,39 @@ def test_check_status_within_a_capture(cuda):
     graph.replay()
     vggt_sparse.check_status()
     assert torch.equal(out, want)
+
+
+FIRST = """
+import sys
+import torch
+import vggt_sparse
+x, w = (torch.ones(n, 64, dtype=torch.bfloat16, device="cuda", requires_grad=True) for n in (200, 64))
+y = vggt_sparse.linear(x, w)
+dy = torch.ones_like(y)
+torch.cuda.synchronize()
+dx, dw = torch.autograd.grad(y, (x, w), dy)
+assert bool((dx == 64).all()) and bool((dw == 200).all())
+"""
+
+
+def test_first_gradient_of_a_process(cuda):
+    """Autograd's thread has no CUDA context of its own before it has called the runtime."""
+    path = os.pathsep.join(p for p in sys.path if p)
+    subprocess.run([sys.executable, "-c", FIRST], check=True, env=dict(os.environ, PYTHONPATH=path))
+
+
+def test_first_call_of_a_thread(cuda):
+    """Nor has a thread of the caller's."""
+    c, out = Linear(cuda, 200, 64, 64), torch.empty(200, 64, dtype=BF, device=cuda)
+    want = c.call()
+    a = torch.randn(3 * TPF, 128, device=cuda).to(BF)
+    w = torch.randn(384, 128, device=cuda).to(BF)
+    project = lambda: vggt_sparse.project_qkv(a, w, heads=2, tokens_per_frame=TPF)  # noqa: E731
+    q = project().q
+    torch.cuda.synchronize()
+    got = []
+    for run in (lambda: c.call(out=out), lambda: project().q):
+        thread = threading.Thread(target=lambda: got.append(run()))
+        thread.start()
+        thread.join()
+    assert len(got) == 2 and torch.equal(got[0], want) and torch.equal(got[1], q)
